@@ -270,7 +270,7 @@ def run(state):
         if own:
             from slayerpytorch_b200.loss import policyLoss
             loss = policyLoss(state["logits"], state["action"], state["old"], state["advantage"], refLogProb=state["ref"], mask=state["mask"],
-                              clip=CLIP, klCoef=KL, scale=case["scale"], reduction=case["reduction"])
+                              clip=CLIP, klCoef=KL if case["kl"] else 0.0, scale=case["scale"], reduction=case["reduction"])
         else:
             loss = _plain_policy(state)
     elif own:
