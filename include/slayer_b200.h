@@ -2,8 +2,8 @@
  * slayer_b200 — C ABI of the Blackwell (sm_100a) SLAYER spiking-neuron operators.
  *
  * Every entry point takes plain device pointers and sizes; no framework types cross this
- * boundary.  All tensors are float32, row-major [rows, T] with time last and contiguous,
- * resident on the CUDA device that is current on the calling thread.  `stream` is a
+ * boundary.  Unless an entry says otherwise, tensors are float32, row-major [rows, T] with time last
+ * and contiguous, resident on the CUDA device that is current on the calling thread.  `stream` is a
  * cudaStream_t passed as void* (NULL = the legacy default stream).  Calls are asynchronous
  * with respect to the host: they enqueue work on `stream` and return.
  *
@@ -28,6 +28,16 @@ extern "C" {
 #define SLAYER_B200_ECUDA      -2   /* a CUDA runtime call or kernel launch failed          */
 #define SLAYER_B200_EUNSUPPORTED -3 /* argument outside what the kernels implement          */
 #define SLAYER_B200_EDEVICE    -4   /* a kernel reported a device-side error status         */
+
+/* Element types of the entries that take more than float32. */
+#define SLAYER_B200_F32         0
+#define SLAYER_B200_BF16        1
+#define SLAYER_B200_F16         2
+
+/* How a loss adds up its rows or pairs. */
+#define SLAYER_B200_SUM         0
+#define SLAYER_B200_MEAN        1   /* over the rows that are not masked (pairs: over all)  */
+#define SLAYER_B200_SEQUENCE    2   /* mean over sequences of the mean in each of them      */
 
 /* ABI version of this header (bumped when a signature changes). */
 int slayer_b200_abi_version(void);
@@ -262,6 +272,67 @@ int slayer_b200_bin_events_packed(uint32_t *bits, const int32_t *n, const int32_
 int slayer_b200_num_spikes_loss(float *grad, double *row_sq, const float *s, const float *desired_count,
                                 const float *filter, int64_t rows, int64_t T, int64_t K,
                                 int64_t start, int64_t stop, float Ts, float scale, void *stream);
+
+/*
+ * Log-probability of one chosen entry per row of logits:
+ *   z = scale * logits[r, :],  logp[r] = z[action[r]] - log sum_j exp(z[j])          (r < rows, j < V)
+ * logits: [rows, V] of type `dtype` (SLAYER_B200_F32 ...), `stride` elements from row to row, the
+ * entries of a row next to each other; any alignment of a multiple of the element.  mask: one byte
+ * per row or NULL; a row whose byte is 0 is not read, its logp is 0.  stats: 2 * rows floats for
+ * slayer_b200_logit_grad, or NULL.  An action outside [0, V) gives NaN.  scale > 0 (spike counts
+ * are logits with a gain).  It has no counterpart in the reference, whose classifier takes the
+ * largest spike count (src/spikeClassifier.py:9-20).
+ */
+int slayer_b200_log_prob(float *logp, float *stats, const void *logits, int dtype, const int64_t *action, const uint8_t *mask,
+                         int64_t rows, int64_t V, int64_t stride, float scale, void *stream);
+
+/*
+ * Gradient of rows' log-probabilities with respect to the logits:
+ *   grad[r, j] = upstream * coef[r / coef_len] * scale * ((j == action[r]) - softmax(z)[j]),
+ * 0 in masked rows (which are not read).  grad: [rows, V] of type `dtype`, contiguous.  stats: as
+ * slayer_b200_log_prob or slayer_b200_policy_loss left them.  coef: rows / coef_len floats, or
+ * NULL for 1.  upstream: a float on the device, or one per row if upstream_rows is not 0.  With
+ * only_if_not_one (and one upstream) nothing is done if that upstream is 1.  It has no counterpart
+ * in the reference.
+ */
+int slayer_b200_logit_grad(void *grad, const void *logits, int dtype, const int64_t *action, const uint8_t *mask, const float *stats,
+                           const float *coef, int64_t coef_len, const float *upstream, int upstream_rows, int only_if_not_one,
+                           int64_t rows, int64_t V, int64_t stride, float scale, void *stream);
+
+/*
+ * Clipped policy loss with a KL term, value and gradient in one pass.  Per row, with logp as above:
+ *   ratio = exp(logp - old_logp[r]),  A = advantage[r / adv_len],  d = ref_logp[r] - logp
+ *   per   = -min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A) + kl (exp(d) - d - 1)
+ * loss = sum of per over the rows (SLAYER_B200_SUM), its mean over the rows that are not masked
+ * (SLAYER_B200_MEAN), or the mean over the rows / seq_len sequences of the mean over each one's rows
+ * that are not masked (SLAYER_B200_SEQUENCE); a mean over no rows is 0.  ref_logp may be NULL (no KL
+ * term).  old_logp, ref_logp and advantage are constants.  grad ([rows, V], contiguous, or NULL) is
+ * d loss / d logits; with logp, stats (either may be NULL) and coef (rows floats) a later
+ * slayer_b200_logit_grad gives it for another upstream gradient.  workspace:
+ * slayer_b200_policy_loss_workspace(rows, seq_len) bytes of device memory, aligned to 8.  It has no
+ * counterpart in the reference, whose losses need the desired answer (src/spikeLoss.py:39-104).
+ */
+int slayer_b200_policy_loss(float *loss, void *grad, float *logp, float *stats, float *coef, void *workspace, const void *logits,
+                            int dtype, const int64_t *action, const float *old_logp, const float *advantage, int64_t adv_len,
+                            const float *ref_logp, const uint8_t *mask, int64_t rows, int64_t seq_len, int64_t V, int64_t stride,
+                            float scale, float clip_low, float clip_high, float kl, int reduction, void *stream);
+int64_t slayer_b200_policy_loss_workspace(int64_t rows, int64_t seq_len);
+
+/*
+ * Loss of paired sequences.  logp: [sequences, seq_len] from slayer_b200_log_prob (0 where masked);
+ * ref_logp: one sum per sequence; pairs: n_pairs x 2 sequence indices, the preferred one first (a
+ * sequence may be in several pairs):
+ *   margin[s] = sum_l logp[s, l] - ref_logp[s],   h = beta (margin[first] - margin[second])
+ *   loss = sum or mean over the pairs of (1 - smoothing) log(1 + exp(-h)) + smoothing log(1 + exp(h))
+ * coef[s] = d loss / d (sum of logp of s), for slayer_b200_logit_grad with coef_len = seq_len.  A
+ * pair with an index outside makes the loss NaN.  workspace:
+ * slayer_b200_preference_loss_workspace(sequences) bytes of device memory, aligned to 8.  It has
+ * no counterpart in the reference.
+ */
+int slayer_b200_preference_loss(float *loss, float *coef, void *workspace, const float *logp, const float *ref_logp, const int64_t *pairs,
+                                int64_t sequences, int64_t seq_len, int64_t n_pairs, float beta, float smoothing, int reduction,
+                                void *stream);
+int64_t slayer_b200_preference_loss_workspace(int64_t sequences);
 
 /*
  * slayer_b200_srm_get_spikes without any memory allocation, for callers that cannot allocate

@@ -40,11 +40,12 @@ CUDA_SOURCES = {
     "packed.cu": [],
     "events.cu": [],
     "loss.cu": ["-ftz=true"],
+    "policy.cu": ["-ftz=true"],      # exponentials below 1.2e-38 are nothing beside a row's sum of at least 1
     "tma.cu": [],
 }
 HEADERS = ["common.cuh", "tile.cuh", "tma.cuh", "fir_sparse.cuh", os.path.join(INCLUDE, "slayer_b200.h")]
 
-MODULES = {"slayerCuda": "bindings_slayer.cpp", "slayerLoihiCuda": "bindings_loihi.cpp"}
+MODULES = {"slayerCuda": ["bindings_slayer.cpp", "bindings_learning.cpp"], "slayerLoihiCuda": ["bindings_loihi.cpp"]}
 
 
 def _newer(target, deps):
@@ -105,21 +106,29 @@ def build_modules(force=False, verbose=False):
         inc += ["-isystem" if "torch" in p or "python" in p else "-I", p]
     tlib = os.path.join(os.path.dirname(torch.__file__), "lib")
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    built = []
-    for name, src in MODULES.items():
-        s = os.path.join(CSRC, src)
+    common = (["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-DTORCH_API_INCLUDE_EXTENSION_H",
+               "-D_GLIBCXX_USE_CXX11_ABI=%d" % abi])
+    headers = [os.path.join(CSRC, "bindings_common.h"), os.path.join(INCLUDE, "slayer_b200.h")]
+    compile_cmds, link_cmds, built = [], [], []
+    for name, sources in MODULES.items():
         target = os.path.join(LIBDIR, name + ext)
-        deps = [s, os.path.join(CSRC, "bindings_common.h"), os.path.join(INCLUDE, "slayer_b200.h")]
-        if force or _newer(target, deps):
-            cmd = (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-                    "-DTORCH_EXTENSION_NAME=" + name, "-DTORCH_API_INCLUDE_EXTENSION_H",
-                    "-D_GLIBCXX_USE_CXX11_ABI=%d" % abi]
-                   + inc + [s, "-o", target,
-                            "-L", LIBDIR, "-lslayer_b200", "-Wl,-rpath,$ORIGIN",
-                            "-L", tlib, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch",
-                            "-ltorch_python", "-Wl,-rpath," + tlib])
-            _run(cmd, verbose)
+        objs, changed = [], force or not os.path.isfile(target)
+        for src in sources:
+            s = os.path.join(CSRC, src)
+            o = os.path.join(OBJDIR, src.replace(".cpp", ".o"))
+            if force or _newer(o, [s] + headers + [os.path.abspath(__file__)]):
+                compile_cmds.append(common + ["-DTORCH_EXTENSION_NAME=" + name] + inc + ["-c", s, "-o", o])
+                changed = True
+            objs.append(o)
+        if changed or _newer(target, objs):
+            link_cmds.append(["g++", "-shared"] + objs + ["-o", target, "-L", LIBDIR, "-lslayer_b200", "-Wl,-rpath,$ORIGIN",
+                              "-L", tlib, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch",
+                              "-ltorch_python", "-Wl,-rpath," + tlib])
         built.append(target)
+    with concurrent.futures.ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
+        list(pool.map(lambda cmd: _run(cmd, verbose), compile_cmds))
+    for cmd in link_cmds:
+        _run(cmd, verbose)
     return built
 
 

@@ -38,6 +38,13 @@ SYMBOLS = {
     "slayer_b200_bin_events_packed": (_int, [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64,
                                              ctypes.c_double, _i64, _p]),
     "slayer_b200_num_spikes_loss": (_int, [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _f, _f, _p]),
+    "slayer_b200_log_prob": (_int, [_p, _p, _p, _int, _p, _p, _i64, _i64, _i64, _f, _p]),
+    "slayer_b200_logit_grad": (_int, [_p, _p, _int, _p, _p, _p, _p, _i64, _p, _int, _int, _i64, _i64, _i64, _f, _p]),
+    "slayer_b200_policy_loss": (_int, [_p, _p, _p, _p, _p, _p, _p, _int, _p, _p, _p, _i64, _p, _p, _i64, _i64, _i64, _i64,
+                                       _f, _f, _f, _f, _int, _p]),
+    "slayer_b200_policy_loss_workspace": (_i64, [_i64, _i64]),
+    "slayer_b200_preference_loss": (_int, [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _f, _f, _int, _p]),
+    "slayer_b200_preference_loss_workspace": (_i64, [_i64]),
     "slayer_b200_loihi_get_spikes": (_int, [_p, _p, _p, _p, _i64, _i64, _u32, _u32, _u32, _u32, _u32, _p]),
     "slayer_b200_loihi_spikes_only": (_int, [_p, _p, _i64, _i64, _u32, _u32, _u32, _u32, _u32, _i64, _p]),
     "slayer_b200_loihi_get_spikes_delayed": (_int, [_p, _p, _p, _p, _i64, _i64, _u32, _u32, _u32, _u32, _u32, _i64, _p]),

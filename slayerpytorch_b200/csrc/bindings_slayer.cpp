@@ -431,6 +431,8 @@ static torch::Tensor binEventsPackedCuda(std::vector<int64_t> shape, torch::Tens
     return bits;
 }
 
+void bind_learning(pybind11::module_ &m);        // bindings_learning.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
 {
     m.def("getSpikes", &getSpikesCuda, "Get spikes (CUDA)");
@@ -454,5 +456,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
     m.def("numSpikesLoss", &numSpikesLossCuda, "Spike-count loss: sum of squared errors and gradient in one pass (CUDA)");
     m.def("binEvents", &binEventsCuda, "Address events -> spike tensor (CUDA)");
     m.def("binEventsPacked", &binEventsPackedCuda, "Address events -> bit-packed spike tensor (CUDA)");
+    bind_learning(m);
     m.attr("backend") = "slayer_b200";
 }
