@@ -335,6 +335,47 @@ int slayer_b200_preference_loss(float *loss, float *coef, void *workspace, const
 int64_t slayer_b200_preference_loss_workspace(int64_t sequences);
 
 /*
+ * A stack of matrices made near orthogonal by Newton-Schulz products: each [rows, cols] matrix u of
+ * in (type `dtype`, contiguous, `batch` of them) becomes X after
+ *   X = u / (|u|_F + eps),   `steps` times  X <- a X + (b A + c A A) X,  A = X X^T
+ * (of a matrix with more rows than columns, the transpose's).  out may be in.  Float32 and float16
+ * matrices are worked on with products of 22 bits, bfloat16 ones with 11.  Coefficients whose steps
+ * take singular values from [0, 1] past 3.5 are refused.  At most 32768 on the shorter side and
+ * 2^31 elements per matrix, else SLAYER_B200_EUNSUPPORTED.  workspace:
+ * slayer_b200_orthogonalize_workspace(...) bytes of device memory, aligned to 256.  It has
+ * no counterpart in the reference.
+ */
+int slayer_b200_orthogonalize(void *out, const void *in, int dtype, int64_t batch, int64_t rows, int64_t cols, int steps, float a, float b,
+                              float c, float eps, void *workspace, void *stream);
+int64_t slayer_b200_orthogonalize_workspace(int64_t batch, int64_t rows, int64_t cols, int dtype);
+
+/* One weight of slayer_b200_muon_step: weight and grad [rows, cols] of the call's type, momentum float32. */
+typedef struct {
+    void *weight;
+    const void *grad;
+    float *momentum;
+    int64_t rows, cols;
+} slayer_b200_muon_matrix;
+
+/* What the learning rate of slayer_b200_muon_step is multiplied by. */
+#define SLAYER_B200_MUON_NONE   0
+#define SLAYER_B200_MUON_SHAPE  1   /* sqrt(max(1, rows / cols))                            */
+#define SLAYER_B200_MUON_RMS    2   /* 0.2 sqrt(max(rows, cols)): updates as large as Adam's */
+
+/*
+ * One step of the Muon optimiser on `count` weights (list: host memory, read before the call
+ * returns), in a fixed number of launches:
+ *   momentum <- mu momentum + grad,   u = grad + mu momentum if nesterov else momentum,
+ *   weight   <- weight (1 - lr weight_decay) - lr factor X,   X = u made orthogonal as above.
+ * The weights must not overlap.  workspace: slayer_b200_muon_step_workspace(...) bytes of device
+ * memory, aligned to 256.  It has no counterpart in the reference, whose optimizer is Nadam
+ * (src/optimizer.py:6-113).
+ */
+int slayer_b200_muon_step(const slayer_b200_muon_matrix *list, int64_t count, int dtype, float lr, float mu, int nesterov,
+                          float weight_decay, int adjust, int steps, float a, float b, float c, float eps, void *workspace, void *stream);
+int64_t slayer_b200_muon_step_workspace(const slayer_b200_muon_matrix *list, int64_t count, int dtype);
+
+/*
  * slayer_b200_srm_get_spikes without any memory allocation, for callers that cannot allocate
  * device memory: an application that has already given all device memory to its own pool, or
  * code that runs where entering the CUDA allocator is not allowed (another library's callback,

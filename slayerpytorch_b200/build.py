@@ -41,6 +41,7 @@ CUDA_SOURCES = {
     "events.cu": [],
     "loss.cu": ["-ftz=true"],
     "policy.cu": ["-ftz=true"],      # exponentials below 1.2e-38 are nothing beside a row's sum of at least 1
+    "newton_schulz.cu": [],
     "tma.cu": [],
 }
 HEADERS = ["common.cuh", "tile.cuh", "tma.cuh", "fir_sparse.cuh", os.path.join(INCLUDE, "slayer_b200.h")]

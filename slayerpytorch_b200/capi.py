@@ -45,6 +45,10 @@ SYMBOLS = {
     "slayer_b200_policy_loss_workspace": (_i64, [_i64, _i64]),
     "slayer_b200_preference_loss": (_int, [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _f, _f, _int, _p]),
     "slayer_b200_preference_loss_workspace": (_i64, [_i64]),
+    "slayer_b200_orthogonalize": (_int, [_p, _p, _int, _i64, _i64, _i64, _int, _f, _f, _f, _f, _p, _p]),
+    "slayer_b200_orthogonalize_workspace": (_i64, [_i64, _i64, _i64, _int]),
+    "slayer_b200_muon_step": (_int, [_p, _i64, _int, _f, _f, _int, _f, _int, _int, _f, _f, _f, _f, _p, _p]),
+    "slayer_b200_muon_step_workspace": (_i64, [_p, _i64, _int]),
     "slayer_b200_loihi_get_spikes": (_int, [_p, _p, _p, _p, _i64, _i64, _u32, _u32, _u32, _u32, _u32, _p]),
     "slayer_b200_loihi_spikes_only": (_int, [_p, _p, _i64, _i64, _u32, _u32, _u32, _u32, _u32, _i64, _p]),
     "slayer_b200_loihi_get_spikes_delayed": (_int, [_p, _p, _p, _p, _i64, _i64, _u32, _u32, _u32, _u32, _u32, _i64, _p]),
@@ -59,6 +63,11 @@ SYMBOLS = {
     "slayer_b200_set_fir_flow": (_int, [_int]),
     "slayer_b200_set_srm_stages": (_int, [_int]),
 }
+
+class MuonMatrix(ctypes.Structure):
+    """One entry of the list that slayer_b200_muon_step takes: device pointers and the matrix's size."""
+    _fields_ = [("weight", _p), ("grad", _p), ("momentum", _p), ("rows", _i64), ("cols", _i64)]
+
 
 _lib = None
 

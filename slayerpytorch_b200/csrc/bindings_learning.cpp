@@ -1,5 +1,6 @@
 // Python module `slayerCuda`, second part: the operators behind the losses on logits (logProb, policyLoss, preferenceLoss,
-// logitGrad).  They take float32, bfloat16 and float16 logits; everything that belongs to a row is float32.
+// logitGrad), and the orthogonalised updates (orthogonalize, muonStep).  They take float32, bfloat16 and float16 logits, matrices
+// and weights; everything that belongs to a row, and the momenta, are float32.
 #include "bindings_common.h"
 
 #include <cuda_runtime_api.h>
@@ -156,6 +157,63 @@ std::vector<torch::Tensor> preferenceLossCuda(torch::Tensor logp, torch::Tensor 
     return {loss, coef};
 }
 
+void check_matrix(const torch::Tensor &x, const char *name)
+{
+    TORCH_CHECK(x.is_cuda(), name, " must be a CUDA tensor");
+    TORCH_CHECK(x.is_contiguous(), name, " must be contiguous");
+    TORCH_CHECK(x.dim() >= 2, name, " must have at least two dimensions, it has ", x.dim());
+}
+
+// A matrix, or a stack of them, made near orthogonal.
+torch::Tensor orthogonalizeCuda(torch::Tensor x, int64_t steps, double a, double b, double c, double eps)
+{
+    check_matrix(x, "matrix");
+    const int dtype = dtype_code(x, "matrix");
+    c10::cuda::CUDAGuard guard(x.device());
+    auto out = torch::empty_like(x);
+    const int64_t rows = x.size(-2), cols = x.size(-1), batch = x.numel() ? x.numel() / (rows * cols) : 0;
+    auto workspace = torch::empty({slayer_b200_orthogonalize_workspace(batch, rows, cols, dtype)}, x.options().dtype(torch::kUInt8));
+    check_rc(slayer_b200_orthogonalize(out.data_ptr(), x.data_ptr(), dtype, batch, rows, cols, (int)std::min<int64_t>(steps, 1 << 20),
+                                       (float)a, (float)b, (float)c, (float)eps, workspace.data_ptr(), current_stream()),
+             "orthogonalize");
+    return out;
+}
+
+// One optimiser step, in place, of weights of one type on one device: [d0, d1, ...] is a matrix of d0 rows.
+void muonStepCuda(std::vector<torch::Tensor> weights, const std::vector<torch::Tensor> &grads, std::vector<torch::Tensor> momenta, double lr,
+                  double momentum, bool nesterov, double weightDecay, int64_t adjust, int64_t steps, double a, double b, double c, double eps)
+{
+    TORCH_CHECK(weights.size() == grads.size() && weights.size() == momenta.size(), "as many gradients and momenta as weights");
+    if (weights.empty()) return;
+    const int dtype = dtype_code(weights[0], "weight");
+    std::vector<slayer_b200_muon_matrix> list;
+    list.reserve(weights.size());
+    for (size_t i = 0; i < weights.size(); ++i) {
+        const torch::Tensor &w = weights[i], &g = grads[i], &m = momenta[i];
+        check_matrix(w, "weight");
+        check_matrix(g, "grad");
+        check_matrix(m, "momentum");
+        TORCH_CHECK(w.scalar_type() == weights[0].scalar_type(), "the weights of one call must have one dtype");
+        TORCH_CHECK(g.scalar_type() == w.scalar_type(), "grad must have the dtype of its weight");
+        TORCH_CHECK(m.scalar_type() == torch::kFloat32, "momentum must be a float32 tensor");
+        TORCH_CHECK(g.sizes() == w.sizes() && m.sizes() == w.sizes(), "grad and momentum must have the shape of their weight");
+        check_device(w, weights[0], "weight", "the first weight");
+        check_device(g, w, "grad", "weight");
+        check_device(m, w, "momentum", "weight");
+        const int64_t rows = w.size(0);
+        list.push_back({w.data_ptr(), g.data_ptr(), m.data_ptr<float>(), rows, w.numel() ? w.numel() / rows : 0});
+    }
+    c10::cuda::CUDAGuard guard(weights[0].device());
+    auto workspace = torch::empty({slayer_b200_muon_step_workspace(list.data(), (int64_t)list.size(), dtype)},
+                                  weights[0].options().dtype(torch::kUInt8));
+    check_rc(slayer_b200_muon_step(list.data(), (int64_t)list.size(), dtype, (float)lr, (float)momentum, nesterov, (float)weightDecay,
+                                   (int)adjust, (int)std::min<int64_t>(steps, 1 << 20), (float)a, (float)b, (float)c, (float)eps,
+                                   workspace.data_ptr(), current_stream()),
+             "muonStep");
+    for (auto &w : weights) w.unsafeGetTensorImpl()->bump_version();      // autograd sees that they changed
+    for (auto &m : momenta) m.unsafeGetTensorImpl()->bump_version();
+}
+
 }  // namespace
 
 void bind_learning(pybind11::module_ &m)
@@ -164,5 +222,7 @@ void bind_learning(pybind11::module_ &m)
     m.def("logitGrad", &logitGradCuda, "Gradient of rows' log-probabilities with respect to the logits (CUDA)");
     m.def("policyLoss", &policyLossCuda, "Clipped policy loss with a KL term: value and gradient in one pass (CUDA)");
     m.def("preferenceLoss", &preferenceLossCuda, "Loss of paired sequences and its derivative by each sequence's log-probability (CUDA)");
+    m.def("orthogonalize", &orthogonalizeCuda, "Matrices made near orthogonal by Newton-Schulz products (CUDA)");
+    m.def("muonStep", &muonStepCuda, "Momentum, orthogonalised update and decay of a list of weights, in place (CUDA)");
     m.def("captureId", &capture_id, "Which stream capture the current stream of a tensor's device is in (0: none)");
 }
