@@ -44,7 +44,7 @@ CUDA_SOURCES = {
     "newton_schulz.cu": [],
     "tma.cu": [],
 }
-HEADERS = ["common.cuh", "tile.cuh", "tma.cuh", "fir_sparse.cuh", os.path.join(INCLUDE, "slayer_b200.h")]
+HEADERS = ["common.cuh", "tile.cuh", "tma.cuh", "tensor.cuh", "fir_sparse.cuh", os.path.join(INCLUDE, "slayer_b200.h")]
 
 MODULES = {"slayerCuda": ["bindings_slayer.cpp", "bindings_learning.cpp"], "slayerLoihiCuda": ["bindings_loihi.cpp"]}
 

@@ -4,17 +4,33 @@
 // Every step takes each singular value s to a s + b s^3 + c s^5, so they all end near one while the singular vectors stay.
 // An optimiser step takes u from a gradient and its momentum and applies the result to the weight:
 //   mom <- mu mom + g,   u = g + mu mom (or mom),   w <- w (1 - lr decay) - lr scale X
+//
+// The work is matrix products, m m n + m m m + 2 m m n multiply-adds a step for m <= n with the symmetric halves left out, so
+// they run on the tensor cores, on 16-bit parts of the 32-bit values.  Everything has a known size - |X|_F <= 1 at the start, no
+// singular value ever above 3.5 - so fp16 with a fixed power-of-two scale holds it, and holds 11 bits where bf16 holds 8.
+//   PARTS = 2 (float32, float16 weights): v = hi + lo, two fp16 values, 22 bits and a sign;  v w ~ hi hi + hi lo + lo hi, the
+//     left out lo lo being 2^-24 of it.  Three products instead of one, and results as good as fp32 arithmetic's.
+//   PARTS = 1 (bfloat16 weights, whose update is rounded to 8 bits in the end): v = hi.
+// Sums are fp32 in tensor memory.
+//
+// X, A and B = b A + c A A live in the workspace as blocks of 128 x 64 elements, padded with zeros, each block laid out as the
+// tensor core reads it from shared memory (tensor.cuh), hi before lo: every load is a contiguous copy of 8 to 32 KB, whatever
+// the matrix's sizes, and one form of X serves both as rows (X X^T) and as columns (B X).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
-
 #include <math.h>
 
 #include "common.cuh"
+#include "tensor.cuh"
 
 namespace sb200 {
 
 constexpr int kMaxJobs = 48;         // matrices per launch
-constexpr int kNormParts = 64;       // partial sums of squares per matrix
+constexpr int kNormParts = 256;      // partial sums of squares per matrix
+constexpr int kStatusNsTimeout = 0x5103;
+constexpr int kWaitLimit = 1 << 22;
+constexpr int kBlock = 128 * 64 * 2; // bytes of a block
+constexpr float kScaleX = 8192.0f, kScaleA = 4096.0f;      // of X; of A and B
 
 struct NsJob {
     const void *src;                 // gradient, or the matrix itself
@@ -23,7 +39,9 @@ struct NsJob {
     int rows, cols, m, n;            // as stored; m <= n: as worked on
     float keep, step;                // w <- keep w - step X
     double *parts;
-    float *x[2], *a, *b;
+    int norm_parts;
+    unsigned char *x[2], *a, *b;     // blocks: row blocks of 128, in each of them column blocks of 64
+    int first[3];                    // this launch's first block of the passes over elements; first tile of the products (A, X)
 };
 
 struct NsArgs {
@@ -32,6 +50,9 @@ struct NsArgs {
     float mu, ca, cb, cc, eps;
     bool nesterov;
 };
+
+static __host__ __device__ __forceinline__ int ns_rb(int v) { return (v + 127) / 128; }            // row blocks
+static __host__ __device__ __forceinline__ int ns_cb(int v) { return (v + 127) / 128 * 2; }        // column blocks
 
 template <typename T> __device__ __forceinline__ float ns_in(T v);
 template <> __device__ __forceinline__ float ns_in(float v) { return v; }
@@ -57,16 +78,27 @@ __device__ __forceinline__ S ns_block_sum(S v, S *part)
     return v;
 }
 
+// the job that a block or tile belongs to: the last one that does not begin behind it
+template <int WHICH>
+__device__ __forceinline__ int ns_find(const NsArgs &A, int at)
+{
+    int j = 0;
+    while (j + 1 < A.jobs && A.job[j + 1].first[WHICH] <= at) ++j;
+    return j;
+}
+
 // momentum, and the squares' partial sums (double: a sum over up to 2^31 squares, of values of any size)
 template <typename T>
 __global__ void __launch_bounds__(256) ns_momentum_kernel(const __grid_constant__ NsArgs A)
 {
     __shared__ double part[32];
-    const NsJob &J = A.job[blockIdx.y];
-    const int64_t count = (int64_t)J.rows * J.cols;
+    const NsJob &J = A.job[ns_find<0>(A, blockIdx.x)];
+    const int me = blockIdx.x - J.first[0];
+    const int64_t count = (int64_t)J.rows * J.cols, step = J.norm_parts * 256ll;
     const T *g = (const T *)J.src;
     double sq = 0.0;
-    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < count; i += gridDim.x * 256ll) {
+#pragma unroll 4
+    for (int64_t i = me * 256ll + threadIdx.x; i < count; i += step) {
         float u = ns_in(g[i]);
         if (J.mom) {
             const float m = fmaf(A.mu, J.mom[i], u);
@@ -76,106 +108,383 @@ __global__ void __launch_bounds__(256) ns_momentum_kernel(const __grid_constant_
         sq += (double)u * (double)u;
     }
     sq = ns_block_sum(sq, part);
-    if (threadIdx.x == 0) J.parts[blockIdx.x] = sq;
+    if (threadIdx.x == 0) J.parts[me] = sq;
 }
 
-template <typename T>
+// two values next to each other as their fp16 parts
+template <int PARTS>
+__device__ __forceinline__ void ns_split(float v0, float v1, uint32_t &hi, uint32_t &lo)
+{
+    const __half2 h = __floats2half2_rn(v0, v1);
+    hi = *reinterpret_cast<const uint32_t *>(&h);
+    if (PARTS == 2) {
+        const float2 f = __half22float2(h);
+        const __half2 l = __floats2half2_rn(v0 - f.x, v1 - f.y);
+        lo = *reinterpret_cast<const uint32_t *>(&l);
+    }
+}
+
+// where the 16-byte chunk (8 columns from c on) of element (r, c) begins, in blocks of cbs column blocks per row block
+template <int PARTS>
+__device__ __forceinline__ unsigned char *ns_chunk(unsigned char *x, int cbs, int r, int c)
+{
+    return x + ((int64_t)(r >> 7) * cbs + (c >> 6)) * (PARTS * kBlock) + (r & 127) * 128 + (((c >> 3) & 7) ^ (r & 7)) * 16;
+}
+
+// X0, as blocks: a thread makes a chunk of eight columns
+template <typename T, int PARTS>
 __global__ void __launch_bounds__(256) ns_normalise_kernel(const __grid_constant__ NsArgs A)
 {
-    const NsJob &J = A.job[blockIdx.y];
-    double sq = 0.0;
-    for (int i = 0; i < kNormParts; ++i) sq += J.parts[i];
-    const float inv = (float)(1.0 / (sqrt(sq) + (double)A.eps));
-    const int64_t count = (int64_t)J.rows * J.cols;
+    __shared__ double part[32];
+    const NsJob &J = A.job[ns_find<0>(A, blockIdx.x)];
+    const int me = blockIdx.x - J.first[0];
+    const double sq = ns_block_sum((int)threadIdx.x < J.norm_parts ? J.parts[threadIdx.x] : 0.0, part);
+    const float inv = (float)((double)kScaleX / (sqrt(sq) + (double)A.eps));
     const T *g = (const T *)J.src;
     const bool tall = J.rows > J.cols;
-    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < count; i += gridDim.x * 256ll) {
-        float u = ns_in(g[i]);
-        if (J.mom) u = A.nesterov ? fmaf(A.mu, J.mom[i], u) : J.mom[i];
-        const int64_t r = i / J.cols, c = i - r * J.cols;
-        J.x[0][tall ? c * J.n + r : i] = u * inv;
-    }
-}
-
-// PHASE 0: a = x x^T;  1: b = cb a + cc a a;  2: x' = ca x + b x.  One thread per element of a 16 x 16 tile.
-template <int PHASE>
-__global__ void __launch_bounds__(256) ns_product_kernel(const __grid_constant__ NsArgs A, int from)
-{
-    __shared__ float p[16][17], q[16][17];
-    const NsJob &J = A.job[blockIdx.z];
-    const int cols = PHASE == 2 ? J.n : J.m, K = PHASE == 0 ? J.n : J.m;
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const int i0 = blockIdx.y * 16, j0 = blockIdx.x * 16;
-    if (i0 >= J.m || j0 >= cols) return;
-    const float *x = J.x[from], *left = PHASE == 0 ? x : PHASE == 1 ? J.a : J.b;
-    float s = 0.0f;
-    for (int k0 = 0; k0 < K; k0 += 16) {
-        p[ty][tx] = i0 + ty < J.m && k0 + tx < K ? left[(int64_t)(i0 + ty) * K + k0 + tx] : 0.0f;
-        if (PHASE == 0) q[tx][ty] = j0 + ty < J.m && k0 + tx < K ? x[(int64_t)(j0 + ty) * K + k0 + tx] : 0.0f;
-        else q[ty][tx] = k0 + ty < K && j0 + tx < cols ? (PHASE == 1 ? J.a : x)[(int64_t)(k0 + ty) * cols + j0 + tx] : 0.0f;
-        __syncthreads();
+    const int rows = ns_rb(J.m) * 128, cbs = ns_cb(J.n), chunks = cbs * 8;
+    const unsigned total = (unsigned)rows * chunks;           // at most 2^28
+    for (unsigned i = me * 256 + threadIdx.x; i < total; i += J.norm_parts * 256) {
+        // neighbours in a warp read neighbours in memory: chunks of a row, or (tall) rows of a chunk
+        const int r = tall ? (int)(i % (unsigned)rows) : (int)(i / (unsigned)chunks);
+        const int c = (int)(tall ? i / (unsigned)rows : i % (unsigned)chunks) * 8;
+        float v[8];
 #pragma unroll
-        for (int k = 0; k < 16; ++k) s = fmaf(p[ty][k], q[k][tx], s);
-        __syncthreads();
-    }
-    if (i0 + ty >= J.m || j0 + tx >= cols) return;
-    const int64_t at = (int64_t)(i0 + ty) * cols + j0 + tx;
-    if (PHASE == 0) J.a[at] = s;
-    if (PHASE == 1) J.b[at] = A.cb * J.a[at] + A.cc * s;
-    if (PHASE == 2) J.x[from ^ 1][at] = fmaf(A.ca, x[at], s);
-}
-
-template <typename T>
-__global__ void __launch_bounds__(256) ns_apply_kernel(const __grid_constant__ NsArgs A, int from)
-{
-    const NsJob &J = A.job[blockIdx.y];
-    const int64_t count = (int64_t)J.rows * J.cols;
-    T *w = (T *)J.dst;
-    const bool tall = J.rows > J.cols;
-    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < count; i += gridDim.x * 256ll) {
-        const int64_t r = i / J.cols, c = i - r * J.cols;
-        const float o = J.x[from][tall ? c * J.n + r : i];
-        w[i] = ns_out<T>(J.mom ? fmaf(J.keep, ns_in(w[i]), -J.step * o) : o);
+        for (int k = 0; k < 8; ++k) {
+            v[k] = 0.0f;
+            if (r < J.m && c + k < J.n) {
+                const int64_t at = tall ? (int64_t)(c + k) * J.cols + r : (int64_t)r * J.cols + c + k;
+                float u = ns_in(g[at]);
+                if (J.mom) u = A.nesterov ? fmaf(A.mu, J.mom[at], u) : J.mom[at];
+                v[k] = u * inv;
+            }
+        }
+        uint4 hi, lo;
+        ns_split<PARTS>(v[0], v[1], hi.x, lo.x);
+        ns_split<PARTS>(v[2], v[3], hi.y, lo.y);
+        ns_split<PARTS>(v[4], v[5], hi.z, lo.z);
+        ns_split<PARTS>(v[6], v[7], hi.w, lo.w);
+        unsigned char *at = ns_chunk<PARTS>(J.x[0], cbs, r, c);
+        *(uint4 *)at = hi;
+        if (PARTS == 2) *(uint4 *)(at + kBlock) = lo;
     }
 }
 
-static size_t ns_job_bytes(int64_t m, int64_t n)
+// ------------------------------------------------------------------------------------------------ products
+enum NsPhase { kGram, kPolynomial, kUpdate, kLast };
+
+constexpr int kNsThreads = 320;      // a warp that loads, one that issues products, eight that take the results
+
+template <int PARTS, int TN>
+struct NsTile {
+    static constexpr int kA = PARTS * kBlock, kB = PARTS * kBlock * (TN / 128), kStage = kA + kB;
+    static constexpr int kRows = 8 * 32 * 33 * 4;            // one 32 x 32 piece for each of the eight warps
+    static constexpr int kStages = (227 * 1024 - 1024 - 512 - kRows) / kStage > 6 ? 6 : (227 * 1024 - 1024 - 512 - kRows) / kStage;
+    static constexpr size_t kSmem = 1024 + 512 + kRows + (size_t)kStages * kStage;
+};
+
+// Persistent: a CTA takes tiles of 128 x TN of the result.  PHASE
+//   kGram        a = x x^T                  kPolynomial  b = cb a + cc a a   (both symmetric: tiles that lie below the diagonal
+//   kUpdate      x' = ca x + b x                          are not computed, blocks above it are written twice)
+//   kLast        the same, and the result goes to the weight
+template <int PHASE, int PARTS, int TN, typename T>
+__global__ void __launch_bounds__(kNsThreads, 1) ns_product_kernel(const __grid_constant__ NsArgs A, int from, int tiles, int *status)
 {
-    const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
-    return up(kNormParts * 8) + 2 * up(4 * (size_t)(m * n)) + 2 * up(4 * (size_t)(m * m));
+    using Tile = NsTile<PARTS, TN>;
+    constexpr int S = Tile::kStages;
+    constexpr bool kSymmetric = PHASE == kGram || PHASE == kPolynomial;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char *smem = (unsigned char *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint64_t *full = (uint64_t *)(smem + S * Tile::kStage), *empty = full + S, *done = empty + S, *taken = done + 2;
+    uint32_t *base_at = (uint32_t *)(taken + 2);
+    float *pieces = (float *)(smem + S * Tile::kStage + 512);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (warp == 1) tensor_alloc(base_at, 2 * TN);
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S; ++i) {
+            mbar_init(full + i, 1);
+            mbar_init(empty + i, 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(done + i, 1);
+            mbar_init(taken + i, 8);
+        }
+        mbar_init_fence();
+    }
+    tensor_fence_before();
+    __syncthreads();
+    tensor_fence_after();
+    const uint32_t acc = *base_at;
+    bool fine = true;
+
+    // tile -> its job, the row block and the first column block of 128, and how many of those there are
+    auto locate = [&](int tile, const NsJob *&J, int &i, int &j, int &nb) {
+        const int k = ns_find<kSymmetric ? 1 : 2>(A, tile);
+        J = &A.job[k];
+        int at = tile - J->first[kSymmetric ? 1 : 2];
+        const int rb = ns_rb(J->m), W = TN / 128;
+        if (kSymmetric) {
+            // row block i has the column tiles from i / W on
+            const int ct = (rb + W - 1) / W;
+            for (i = 0; at >= ct - i / W; ++i) at -= ct - i / W;
+            j = (i / W + at) * W;
+            nb = min(W, rb - j);
+        } else {
+            // tiles that run side by side share columns of x
+            i = at % rb;
+            j = at / rb * W;
+            nb = min(W, ns_rb(J->n) - j);
+        }
+    };
+
+    if (warp == 0 && lane == 0) {
+        int s = 0, phase = 0;
+        for (int tile = blockIdx.x; fine && tile < tiles; tile += gridDim.x) {
+            const NsJob *J;
+            int i, j, nb;
+            locate(tile, J, i, j, nb);
+            const int cbm = ns_cb(J->m), cbn = ns_cb(J->n);
+            const int steps = PHASE == kGram ? cbn : cbm;
+            const unsigned char *left = PHASE == kGram ? J->x[from] : PHASE == kPolynomial ? J->a : J->b;
+            const unsigned char *right = PHASE == kPolynomial ? J->a : J->x[from];
+            const unsigned bytes = PARTS * kBlock * (1 + nb);
+            for (int k = 0; k < steps; ++k) {
+                if (!mbar_wait_bounded(empty + s, phase ^ 1, kWaitLimit)) { fine = false; break; }
+                unsigned char *to = smem + s * Tile::kStage;
+                mbar_expect_tx(full + s, bytes);
+                bulk_load(to, left + ((int64_t)i * steps + k) * (PARTS * kBlock), PARTS * kBlock, full + s);
+                to += Tile::kA;
+                if (kSymmetric) {
+                    // [part][block]: rows of the operand follow one another
+                    for (int b = 0; b < nb; ++b)
+                        for (int p = 0; p < PARTS; ++p)
+                            bulk_load(to + (p * (TN / 128) + b) * kBlock, right + (((int64_t)(j + b) * steps + k) * PARTS + p) * kBlock, kBlock, full + s);
+                } else {
+                    // 64 rows of each block of 64 columns: [part][column block]
+                    const unsigned char *row = right + ((int64_t)(k >> 1) * cbn + 2 * j) * (PARTS * kBlock) + (k & 1) * (kBlock / 2);
+                    for (int b = 0; b < 2 * nb; ++b)
+                        for (int p = 0; p < PARTS; ++p)
+                            bulk_load(to + (p * (TN / 64) + b) * (kBlock / 2), row + (b * PARTS + p) * kBlock, kBlock / 2, full + s);
+                }
+                if (++s == S) { s = 0; phase ^= 1; }
+            }
+        }
+        // every stage's last copy has been read before the CTA leaves
+        for (int k = 0; k < S; ++k) {
+            if (!mbar_wait_bounded(empty + s, phase ^ 1, kWaitLimit)) fine = false;
+            if (++s == S) { s = 0; phase ^= 1; }
+        }
+    } else if (warp == 1 && lane == 0) {
+        int s = 0, phase = 0, slot = 0, turn = 0;
+        for (int tile = blockIdx.x; fine && tile < tiles; tile += gridDim.x) {
+            const NsJob *J;
+            int i, j, nb;
+            locate(tile, J, i, j, nb);
+            const int steps = PHASE == kGram ? ns_cb(J->n) : ns_cb(J->m);
+            const uint32_t shape = product_shape(128, nb * 128, !kSymmetric), d = acc + slot * TN;
+            if (!mbar_wait_bounded(taken + slot, turn ^ 1, kWaitLimit)) { fine = false; break; }
+            tensor_fence_after();
+            for (int k = 0; k < steps; ++k) {
+                if (!mbar_wait_bounded(full + s, phase, kWaitLimit)) { fine = false; break; }
+                tensor_fence_after();
+                const unsigned a0 = smem_u32(smem + s * Tile::kStage), b0 = a0 + Tile::kA;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    uint64_t l[PARTS], r[PARTS];
+#pragma unroll
+                    for (int p = 0; p < PARTS; ++p) {
+                        l[p] = desc_rows(a0 + p * kBlock + q * 32);
+                        r[p] = kSymmetric ? desc_rows(b0 + p * (TN / 128) * kBlock + q * 32)
+                                          : desc_columns(b0 + p * (TN / 128) * kBlock + q * 2048, kBlock / 2);
+                    }
+                    product(d, l[0], r[0], shape, k + q > 0);
+                    if (PARTS == 2) {
+                        product(d, l[0], r[PARTS - 1], shape, true);
+                        product(d, l[PARTS - 1], r[0], shape, true);
+                    }
+                }
+                product_commit(empty + s);
+                if (++s == S) { s = 0; phase ^= 1; }
+            }
+            if (!fine) break;
+            product_commit(done + slot);
+            if ((slot ^= 1) == 0) turn ^= 1;
+        }
+        // the results have been taken before the CTA leaves
+        for (int k = 0; fine && k < 2; ++k) {
+            if (!mbar_wait_bounded(taken + slot, turn ^ 1, kWaitLimit)) fine = false;
+            if ((slot ^= 1) == 0) turn ^= 1;
+        }
+    } else if (warp >= 2) {
+        int slot = 0, turn = 0;
+        const int w = warp - 2, quarter = warp & 3, half = w >> 2;
+        float *piece = pieces + w * 32 * 33;
+        for (int tile = blockIdx.x; fine && tile < tiles; tile += gridDim.x) {
+            const NsJob *J;
+            int i, j, nb;
+            locate(tile, J, i, j, nb);
+            const int cbm = ns_cb(J->m), cbn = ns_cb(J->n);
+            if (!__all_sync(0xffffffffu, mbar_wait_bounded(done + slot, turn, kWaitLimit))) { fine = false; break; }
+            tensor_fence_after();
+            const int r = i * 128 + quarter * 32 + lane;
+            for (int c0 = half * (TN / 2); c0 < (half + 1) * (TN / 2) && c0 < nb * 128; c0 += 32) {
+                const int block = j + (c0 >> 7);          // column block of 128
+                if (kSymmetric && block < i) continue;
+                float v[32];
+                tensor_read(v, acc + slot * TN + ((uint32_t)(quarter * 32) << 16) + c0);
+                const int c = j * 128 + c0;
+                const int cbs = kSymmetric ? cbm : cbn;
+                if (PHASE != kGram) {
+                    // b = cb a + ..., x' = ca x + ...
+                    unsigned char *old = PHASE == kPolynomial ? J->a : J->x[from];
+                    const float f = PHASE == kPolynomial ? A.cb : A.ca;
+                    const float by = PHASE == kPolynomial ? A.cc / kScaleA : 1.0f / kScaleA;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const unsigned char *at = ns_chunk<PARTS>(old, cbs, r, c + 8 * k);
+                        const uint4 hi = *(const uint4 *)at;
+                        uint4 lo = make_uint4(0, 0, 0, 0);
+                        if (PARTS == 2) lo = *(const uint4 *)(at + kBlock);
+                        const uint32_t hs[4] = {hi.x, hi.y, hi.z, hi.w}, ls[4] = {lo.x, lo.y, lo.z, lo.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float2 o = __half22float2(*reinterpret_cast<const __half2 *>(&hs[e]));
+                            if (PARTS == 2) {
+                                const float2 l = __half22float2(*reinterpret_cast<const __half2 *>(&ls[e]));
+                                o.x += l.x;
+                                o.y += l.y;
+                            }
+                            v[8 * k + 2 * e] = fmaf(f, o.x, by * v[8 * k + 2 * e]);
+                            v[8 * k + 2 * e + 1] = fmaf(f, o.y, by * v[8 * k + 2 * e + 1]);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) v[k] *= kScaleA / (kScaleX * kScaleX);
+                }
+                if (PHASE == kLast) {
+                    // to the weight, 32 elements next to each other at a time: of a tall matrix, what the lanes hold of a column
+                    T *dst = (T *)J->dst;
+                    const auto put = [&](int row, int col, int64_t at, float o) {
+                        o *= 1.0f / kScaleX;
+                        if (row < J->m && col < J->n) dst[at] = ns_out<T>(J->mom ? fmaf(J->keep, ns_in(dst[at]), -J->step * o) : o);
+                    };
+                    if (J->rows > J->cols) {
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) put(r, c + k, (int64_t)(c + k) * J->cols + r, v[k]);
+                    } else {
+                        const int r0 = i * 128 + quarter * 32;
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) piece[lane * 33 + k] = v[k];
+                        __syncwarp();
+#pragma unroll 8
+                        for (int k = 0; k < 32; ++k) put(r0 + k, c + lane, (int64_t)(r0 + k) * J->cols + c + lane, piece[k * 33 + lane]);
+                    }
+                    __syncwarp();
+                    continue;
+                }
+                unsigned char *to = PHASE == kGram ? J->a : PHASE == kPolynomial ? J->b : J->x[from ^ 1];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    uint4 hi, lo;
+                    ns_split<PARTS>(v[8 * k], v[8 * k + 1], hi.x, lo.x);
+                    ns_split<PARTS>(v[8 * k + 2], v[8 * k + 3], hi.y, lo.y);
+                    ns_split<PARTS>(v[8 * k + 4], v[8 * k + 5], hi.z, lo.z);
+                    ns_split<PARTS>(v[8 * k + 6], v[8 * k + 7], hi.w, lo.w);
+                    unsigned char *at = ns_chunk<PARTS>(to, cbs, r, c + 8 * k);
+                    *(uint4 *)at = hi;
+                    if (PARTS == 2) *(uint4 *)(at + kBlock) = lo;
+                    if (kSymmetric && block > i) {
+                        // (c, r) too: 32 lanes write 64 bytes of a row
+                        const uint32_t hs[4] = {hi.x, hi.y, hi.z, hi.w}, ls[4] = {lo.x, lo.y, lo.z, lo.w};
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            unsigned char *mirror = ns_chunk<PARTS>(to, cbs, c + 8 * k + e, r) + (r & 7) * 2;
+                            *(uint16_t *)mirror = (uint16_t)(hs[e >> 1] >> (e & 1) * 16);
+                            if (PARTS == 2) *(uint16_t *)(mirror + kBlock) = (uint16_t)(ls[e >> 1] >> (e & 1) * 16);
+                        }
+                    }
+                }
+            }
+            tensor_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(taken + slot);
+            if ((slot ^= 1) == 0) turn ^= 1;
+        }
+    }
+    if (!fine) atomicExch(status, kStatusNsTimeout);
+    __syncwarp();
+    tensor_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tensor_fence_after();
+        tensor_free(acc, 2 * TN);
+    }
 }
 
-static int64_t ns_take(NsJob &J, unsigned char *at)
+static size_t ns_job_bytes(int64_t m, int64_t n, int dtype)
 {
-    unsigned char *const start = at;
-    const auto take = [&](size_t bytes) { unsigned char *p = at; at += (bytes + 255) / 256 * 256; return p; };
-    J.parts = (double *)take(kNormParts * 8);
-    for (int i = 0; i < 2; ++i) J.x[i] = (float *)take(4 * (size_t)J.m * J.n);
-    J.a = (float *)take(4 * (size_t)J.m * J.m);
-    J.b = (float *)take(4 * (size_t)J.m * J.m);
-    return at - start;
+    const int64_t parts = dtype == SLAYER_B200_BF16 ? 1 : 2, rb = ns_rb((int)m), cbn = ns_cb((int)n);
+    return kNormParts * 8 + (size_t)(2 * rb * cbn + 4 * rb * rb) * (size_t)(parts * kBlock);
 }
 
-template <typename T>
-static int ns_run(const NsArgs &A, int steps, cudaStream_t st)
+static void ns_take(NsJob &J, int parts, unsigned char *&at)
 {
-    int m = 1, n = 1;
+    const int64_t rb = ns_rb(J.m), x = rb * ns_cb(J.n) * parts * kBlock, a = 2 * rb * rb * parts * kBlock;
+    J.parts = (double *)at;
+    at += kNormParts * 8;
+    J.x[0] = at;
+    J.x[1] = J.x[0] + x;
+    J.a = J.x[1] + x;
+    J.b = J.a + a;
+    at = J.b + a;
+}
+
+template <int PHASE, int PARTS, int TN, typename T>
+static int ns_product(const NsArgs &A, int from, int tiles, int *status, cudaStream_t st)
+{
+    auto kern = ns_product_kernel<PHASE, PARTS, TN, T>;
+    constexpr size_t smem = NsTile<PARTS, TN>::kSmem;
+    int rc = reserve_dynamic_smem((const void *)kern, smem);
+    if (rc) return rc;
+    kern<<<tiles < sm_count() ? tiles : sm_count(), kNsThreads, smem, st>>>(A, from, tiles, status);
+    return check_launch("Newton-Schulz product launch");
+}
+
+template <typename T, int PARTS, int TN>
+static int ns_run(NsArgs &A, int steps, cudaStream_t st)
+{
+    int *status = device_status_word();
+    if (!status) {
+        set_error("Newton-Schulz products: no status word on this device");
+        return SLAYER_B200_ECUDA;
+    }
+    int blocks = 0, small = 0, large = 0;
     for (int j = 0; j < A.jobs; ++j) {
-        m = A.job[j].m > m ? A.job[j].m : m;
-        n = A.job[j].n > n ? A.job[j].n : n;
+        NsJob &J = A.job[j];
+        const int64_t want = ceil_div((int64_t)ns_rb(J.m) * ns_cb(J.n) * 128 * 64, 4096);
+        J.norm_parts = (int)(want < kNormParts ? want : kNormParts);
+        J.first[0] = blocks;
+        J.first[1] = small;
+        J.first[2] = large;
+        blocks += J.norm_parts;
+        const int rb = ns_rb(J.m), W = TN / 128, ct = (rb + W - 1) / W;
+        for (int i = 0; i < rb; ++i) small += ct - i / W;
+        large += rb * ((ns_rb(J.n) + W - 1) / W);
     }
-    const dim3 each(kNormParts, A.jobs);
-    ns_momentum_kernel<T><<<each, 256, 0, st>>>(A);
-    ns_normalise_kernel<T><<<each, 256, 0, st>>>(A);
-    const unsigned mt = (m + 15) / 16, nt = (n + 15) / 16;
+    ns_momentum_kernel<T><<<blocks, 256, 0, st>>>(A);
+    int rc = check_launch("momentum launch");
+    if (rc) return rc;
     int from = 0;
-    for (int s = 0; s < steps; ++s, from ^= 1) {
-        ns_product_kernel<0><<<dim3(mt, mt, A.jobs), 256, 0, st>>>(A, from);
-        ns_product_kernel<1><<<dim3(mt, mt, A.jobs), 256, 0, st>>>(A, from);
-        ns_product_kernel<2><<<dim3(nt, mt, A.jobs), 256, 0, st>>>(A, from);
+    ns_normalise_kernel<T, PARTS><<<blocks, 256, 0, st>>>(A);
+    rc = check_launch("Newton-Schulz normalisation launch");
+    for (int s = 0; s < steps && !rc; ++s, from ^= 1) {
+        rc = ns_product<kGram, PARTS, TN, float>(A, from, small, status, st);
+        if (!rc) rc = ns_product<kPolynomial, PARTS, TN, float>(A, from, small, status, st);
+        if (!rc) rc = s + 1 < steps ? ns_product<kUpdate, PARTS, TN, float>(A, from, large, status, st)
+                                    : ns_product<kLast, PARTS, TN, T>(A, from, large, status, st);
     }
-    ns_apply_kernel<T><<<each, 256, 0, st>>>(A, from);
-    return check_launch("Newton-Schulz kernel launch");
+    return rc;
 }
 
 // Whether the steps keep singular values from [0, 1] and the polynomial's factors in the range that the products can hold: the
@@ -217,12 +526,21 @@ static int ns_shape(const char *what, int64_t rows, int64_t cols)
     return SLAYER_B200_OK;
 }
 
-static int ns_dispatch(const NsArgs &A, int dtype, int steps, cudaStream_t st)
+template <typename T, int PARTS>
+static int ns_tiled(NsArgs &A, int steps, cudaStream_t st)
+{
+    // wide tiles where there are enough of them
+    int64_t tiles = 0;
+    for (int j = 0; j < A.jobs; ++j) tiles += (int64_t)ns_rb(A.job[j].m) * ns_rb(A.job[j].m) / 4;
+    return tiles >= sm_count() ? ns_run<T, PARTS, 256>(A, steps, st) : ns_run<T, PARTS, 128>(A, steps, st);
+}
+
+static int ns_dispatch(NsArgs &A, int dtype, int steps, cudaStream_t st)
 {
     switch (dtype) {
-    case SLAYER_B200_F32: return ns_run<float>(A, steps, st);
-    case SLAYER_B200_BF16: return ns_run<__nv_bfloat16>(A, steps, st);
-    default: return ns_run<__half>(A, steps, st);
+    case SLAYER_B200_F32: return ns_tiled<float, 2>(A, steps, st);
+    case SLAYER_B200_BF16: return ns_tiled<__nv_bfloat16, 1>(A, steps, st);
+    default: return ns_tiled<__half, 2>(A, steps, st);
     }
 }
 
@@ -232,9 +550,8 @@ using namespace sb200;
 
 extern "C" int64_t slayer_b200_orthogonalize_workspace(int64_t batch, int64_t rows, int64_t cols, int dtype)
 {
-    (void)dtype;
     if (batch <= 0 || rows <= 0 || cols <= 0) return 0;
-    return (int64_t)ns_job_bytes(rows < cols ? rows : cols, rows < cols ? cols : rows) * (batch < kMaxJobs ? batch : kMaxJobs);
+    return (int64_t)ns_job_bytes(rows < cols ? rows : cols, rows < cols ? cols : rows, dtype) * (batch < kMaxJobs ? batch : kMaxJobs);
 }
 
 extern "C" int slayer_b200_orthogonalize(void *out, const void *in, int dtype, int64_t batch, int64_t rows, int64_t cols, int steps,
@@ -266,7 +583,7 @@ extern "C" int slayer_b200_orthogonalize(void *out, const void *in, int dtype, i
             J.cols = (int)cols;
             J.m = (int)(rows < cols ? rows : cols);
             J.n = (int)(rows < cols ? cols : rows);
-            at += ns_take(J, at);
+            ns_take(J, dtype == SLAYER_B200_BF16 ? 1 : 2, at);
         }
         rc = ns_dispatch(A, dtype, steps, (cudaStream_t)stream);
         if (rc) return rc;
@@ -276,7 +593,6 @@ extern "C" int slayer_b200_orthogonalize(void *out, const void *in, int dtype, i
 
 extern "C" int64_t slayer_b200_muon_step_workspace(const slayer_b200_muon_matrix *list, int64_t count, int dtype)
 {
-    (void)dtype;
     size_t most = 0, now = 0;
     int in = 0;
     for (int64_t i = 0; list && i < count; ++i) {
@@ -286,7 +602,7 @@ extern "C" int64_t slayer_b200_muon_step_workspace(const slayer_b200_muon_matrix
             in = 1;
             now = 0;
         }
-        now += ns_job_bytes(rows < cols ? rows : cols, rows < cols ? cols : rows);
+        now += ns_job_bytes(rows < cols ? rows : cols, rows < cols ? cols : rows, dtype);
         most = now > most ? now : most;
     }
     return (int64_t)most;
@@ -335,7 +651,7 @@ extern "C" int slayer_b200_muon_step(const slayer_b200_muon_matrix *list, int64_
                                 : adjust == SLAYER_B200_MUON_RMS   ? 0.2 * sqrt((double)J.n) : 1.0;
             J.keep = (float)(1.0 - (double)lr * (double)weight_decay);
             J.step = (float)((double)lr * factor);
-            at += ns_take(J, at);
+            ns_take(J, dtype == SLAYER_B200_BF16 ? 1 : 2, at);
         }
         if (A.jobs == 0) break;
         rc = ns_dispatch(A, dtype, steps, (cudaStream_t)stream);

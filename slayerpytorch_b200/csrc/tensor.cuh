@@ -1,0 +1,93 @@
+// Fifth-generation tensor core helpers (PTX wrappers): products of 16-bit tiles in shared memory, accumulated in tensor memory.
+// The tiles are the blocks of newton_schulz.cu: 64 elements (128 bytes) per row, the 16-byte chunk c of row r at position
+// c ^ (r & 7), eight rows after one another (the 128-byte swizzle of the matrix descriptors).
+#pragma once
+
+#include "tma.cuh"
+
+namespace sb200 {
+
+#ifdef __CUDACC__
+// rows of the tile are rows of the operand, its columns the summation index: groups of eight rows lie 1024 bytes apart
+__device__ __forceinline__ uint64_t desc_rows(unsigned addr)
+{
+    return (uint64_t)((addr & 0x3ffff) >> 4) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+
+// rows of the tile are the summation index, its columns rows of the operand: eight summation steps lie 1024 bytes apart,
+// the next 64 columns `far` bytes
+__device__ __forceinline__ uint64_t desc_columns(unsigned addr, unsigned far)
+{
+    return (uint64_t)((addr & 0x3ffff) >> 4) | (uint64_t)(far >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+
+// fp16 x fp16 -> fp32, M x N; by_columns: the second operand is given by desc_columns
+__device__ __forceinline__ uint32_t product_shape(int m, int n, bool by_columns)
+{
+    return 1u << 4 | (by_columns ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24;
+}
+
+// one thread: d (+)= a b, 16 steps of the summation index
+__device__ __forceinline__ void product(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool add)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(shape), "r"((uint32_t)add)
+        : "memory");
+}
+
+// the barrier is told when all products that this thread has issued are done
+__device__ __forceinline__ void product_commit(uint64_t *bar)
+{
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// one warp; `columns` a power of two from 32 to 512
+__device__ __forceinline__ void tensor_alloc(uint32_t *where, uint32_t columns)
+{
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(where)), "r"(columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+
+__device__ __forceinline__ void tensor_free(uint32_t base, uint32_t columns)
+{
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(columns));
+}
+
+__device__ __forceinline__ void tensor_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tensor_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// one warp reads 32 columns of its 32 lanes (those of quarter warp % 4): lane = row
+__device__ __forceinline__ void tensor_read(float (&v)[32], uint32_t addr)
+{
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// contiguous copy of global memory into shared memory; both 16-byte aligned, bytes a multiple of 16
+__device__ __forceinline__ void bulk_load(void *dst, const void *src, unsigned bytes, uint64_t *bar)
+{
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+
+__device__ __forceinline__ void mbar_arrive(uint64_t *bar)
+{
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+#endif
+
+}  // namespace sb200
