@@ -87,6 +87,27 @@ __device__ __forceinline__ int ns_find(const NsArgs &A, int at)
     return j;
 }
 
+__device__ __forceinline__ bool ns_wide(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+// eight elements that follow one another, as 32-bit values
+template <typename T>
+__device__ __forceinline__ void ns_load8(float (&v)[8], const T *p)
+{
+    if constexpr (sizeof(T) == 4) {
+        const float4 a = *(const float4 *)p, b = *(const float4 *)(p + 4);
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+        const uint4 a = *(const uint4 *)p;
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint16_t h = (uint16_t)(w[i >> 1] >> (i & 1) * 16);
+            v[i] = ns_in(*reinterpret_cast<const T *>(&h));
+        }
+    }
+}
+
 // momentum, and the squares' partial sums (double: a sum over up to 2^31 squares, of values of any size)
 template <typename T>
 __global__ void __launch_bounds__(256) ns_momentum_kernel(const __grid_constant__ NsArgs A)
@@ -94,15 +115,49 @@ __global__ void __launch_bounds__(256) ns_momentum_kernel(const __grid_constant_
     __shared__ double part[32];
     const NsJob &J = A.job[ns_find<0>(A, blockIdx.x)];
     const int me = blockIdx.x - J.first[0];
-    const int64_t count = (int64_t)J.rows * J.cols, step = J.norm_parts * 256ll;
+    const int64_t count = (int64_t)J.rows * J.cols, step = J.norm_parts * 256ll, start = me * 256ll + threadIdx.x;
     const T *g = (const T *)J.src;
+    float *mom = J.mom;
     double sq = 0.0;
-#pragma unroll 4
-    for (int64_t i = me * 256ll + threadIdx.x; i < count; i += step) {
+    int64_t done = 0;
+    if (ns_wide(g) && ns_wide(mom)) {
+        const int64_t eights = count / 8;
+        done = eights * 8;
+        constexpr int U = 2;                       // pieces requested before the first is used
+        for (int64_t i0 = start; i0 < eights; i0 += U * step) {
+            float u[U][8], m[U][8];
+#pragma unroll
+            for (int k = 0; k < U; ++k) {
+                const int64_t i = i0 + k * step;
+                if (i < eights) {
+                    ns_load8(u[k], g + i * 8);
+                    if (mom) ns_load8(m[k], mom + i * 8);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < U; ++k) {
+                const int64_t i = i0 + k * step;
+                if (i < eights) {
+                    if (mom) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            m[k][e] = fmaf(A.mu, m[k][e], u[k][e]);
+                            u[k][e] = A.nesterov ? fmaf(A.mu, m[k][e], u[k][e]) : m[k][e];
+                        }
+                        *(float4 *)(mom + i * 8) = make_float4(m[k][0], m[k][1], m[k][2], m[k][3]);
+                        *(float4 *)(mom + i * 8 + 4) = make_float4(m[k][4], m[k][5], m[k][6], m[k][7]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) sq += (double)u[k][e] * (double)u[k][e];
+                }
+            }
+        }
+    }
+    for (int64_t i = done + start; i < count; i += step) {
         float u = ns_in(g[i]);
-        if (J.mom) {
-            const float m = fmaf(A.mu, J.mom[i], u);
-            J.mom[i] = m;
+        if (mom) {
+            const float m = fmaf(A.mu, mom[i], u);
+            mom[i] = m;
             u = A.nesterov ? fmaf(A.mu, m, u) : m;
         }
         sq += (double)u * (double)u;
@@ -141,7 +196,7 @@ __global__ void __launch_bounds__(256) ns_normalise_kernel(const __grid_constant
     const double sq = ns_block_sum((int)threadIdx.x < J.norm_parts ? J.parts[threadIdx.x] : 0.0, part);
     const float inv = (float)((double)kScaleX / (sqrt(sq) + (double)A.eps));
     const T *g = (const T *)J.src;
-    const bool tall = J.rows > J.cols;
+    const bool tall = J.rows > J.cols, wide = !tall && J.cols % 8 == 0 && ns_wide(g) && ns_wide(J.mom);
     const int rows = ns_rb(J.m) * 128, cbs = ns_cb(J.n), chunks = cbs * 8;
     const unsigned total = (unsigned)rows * chunks;           // at most 2^28
     for (unsigned i = me * 256 + threadIdx.x; i < total; i += J.norm_parts * 256) {
@@ -149,6 +204,20 @@ __global__ void __launch_bounds__(256) ns_normalise_kernel(const __grid_constant
         const int r = tall ? (int)(i % (unsigned)rows) : (int)(i / (unsigned)chunks);
         const int c = (int)(tall ? i / (unsigned)rows : i % (unsigned)chunks) * 8;
         float v[8];
+        if (wide && c < J.n) {
+            if (r < J.m) {
+                const int64_t at = (int64_t)r * J.cols + c;
+                ns_load8(v, g + at);
+                if (J.mom) {
+                    float m[8];
+                    ns_load8(m, J.mom + at);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) v[k] = A.nesterov ? fmaf(A.mu, m[k], v[k]) : m[k];
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = r < J.m ? v[k] * inv : 0.0f;
+        } else
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             v[k] = 0.0f;
@@ -173,252 +242,405 @@ __global__ void __launch_bounds__(256) ns_normalise_kernel(const __grid_constant
 // ------------------------------------------------------------------------------------------------ products
 enum NsPhase { kGram, kPolynomial, kUpdate, kLast };
 
-constexpr int kNsThreads = 320;      // a warp that loads, one that issues products, eight that take the results
+constexpr int kNsThreads = 384;      // a warp that loads, one that issues products, two to fill up; eight that take the results
 
-template <int PARTS, int TN>
+// CG = 1: a CTA makes tiles of 128 x 128.  CG = 2: two CTAs make tiles of 256 x 256 together, each with half of either operand, so
+// that a CTA loads as much per step for four times the products of a pair.
+template <int PARTS, int CG>
 struct NsTile {
-    static constexpr int kA = PARTS * kBlock, kB = PARTS * kBlock * (TN / 128), kStage = kA + kB;
-    static constexpr int kRows = 8 * 32 * 33 * 4;            // one 32 x 32 piece for each of the eight warps
-    static constexpr int kStages = (227 * 1024 - 1024 - 512 - kRows) / kStage > 6 ? 6 : (227 * 1024 - 1024 - 512 - kRows) / kStage;
-    static constexpr size_t kSmem = 1024 + 512 + kRows + (size_t)kStages * kStage;
+    static constexpr int TN = 128 * CG;                      // columns of the result, of which each CTA has 128 rows
+    static constexpr int kA = PARTS * kBlock, kB = PARTS * kBlock, kStage = kA + kB;
+    static constexpr int kPiece = 32 * 33 * 4;               // a 32 x 32 piece of each of the eight warps
+    static constexpr int kFixed = 1024 + 512 + 8 * kPiece;
+    static constexpr int kStages = (227 * 1024 - kFixed) / kStage > 6 ? 6 : (227 * 1024 - kFixed) / kStage;
+    static constexpr size_t kSmem = kFixed + (size_t)kStages * kStage;
+    // Steps of 64 whose sum stays in tensor memory.  The tensor core cuts what it adds to a sum instead of rounding it: over the
+    // 375 additions of a sum of 2000 products in two parts that is a bias of 1e-5, ten times the rounding of fp32 sums.  So
+    // with two parts the sums of 128 products are added up in registers, rounded, while the next ones are made.
+    static constexpr int kGroup = PARTS == 2 ? 2 : 1 << 20;
 };
 
-// Persistent: a CTA takes tiles of 128 x TN of the result.  PHASE
-//   kGram        a = x x^T                  kPolynomial  b = cb a + cc a a   (both symmetric: tiles that lie below the diagonal
-//   kUpdate      x' = ca x + b x                          are not computed, blocks above it are written twice)
-//   kLast        the same, and the result goes to the weight
-template <int PHASE, int PARTS, int TN, typename T>
+// 32 rows x 32 columns of a block in global memory and a warp's piece of shared memory: row by row 64 bytes, of which a lane
+// moves 16, four lanes side by side; in the piece the 16-byte chunks are turned so that a lane can take its own row
+// without two lanes meeting in a bank.
+__device__ __forceinline__ int ns_piece_at(int row, int chunk) { return row * 64 + ((chunk ^ (row >> 1)) & 3) * 16; }
+
+template <bool STORE>
+__device__ __forceinline__ void ns_move_piece(unsigned char *block, unsigned char *piece, int r0, int c0, int lane)
+{
+    uint4 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = i * 8 + (lane >> 2), chunk = lane & 3, r = r0 + row;
+        uint4 *far = (uint4 *)(block + (r & 127) * 128 + ((((c0 >> 3) & 7) + chunk) ^ (r & 7)) * 16);
+        uint4 *near = (uint4 *)(piece + ns_piece_at(row, chunk));
+        if (STORE) *far = *near;
+        else v[i] = *far;
+    }
+    if (!STORE) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *(uint4 *)(piece + ns_piece_at(i * 8 + (lane >> 2), lane & 3)) = v[i];
+    }
+}
+
+// What a warp does with 32 rows (from r0, lane = row) x 32 columns (from c) of a result.
+template <int PHASE, int PARTS, typename T>
+__device__ __forceinline__ void ns_take_piece(const NsArgs &A, const NsJob &J, int from, int r0, int c, float (&v)[32], unsigned char *piece, int lane)
+{
+    constexpr bool kSymmetric = PHASE == kGram || PHASE == kPolynomial;
+    const int cbs = kSymmetric ? ns_cb(J.m) : ns_cb(J.n);
+    const int64_t block = ((int64_t)(r0 >> 7) * cbs + (c >> 6)) * (PARTS * kBlock);
+    if (PHASE == kGram) {
+#pragma unroll
+        for (int k = 0; k < 32; ++k) v[k] *= kScaleA / (kScaleX * kScaleX);
+    } else {
+        // b = cb a + ..., x' = ca x + ...
+        unsigned char *old = (PHASE == kPolynomial ? J.a : J.x[from]) + block;
+        const float f = PHASE == kPolynomial ? A.cb : A.ca, by = PHASE == kPolynomial ? A.cc / kScaleA : 1.0f / kScaleA;
+        __syncwarp();
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) ns_move_piece<false>(old + p * kBlock, piece + p * 2048, r0, c, lane);
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const uint4 hi = *(const uint4 *)(piece + ns_piece_at(lane, k));
+            uint4 lo = make_uint4(0, 0, 0, 0);
+            if (PARTS == 2) lo = *(const uint4 *)(piece + 2048 + ns_piece_at(lane, k));
+            const uint32_t hs[4] = {hi.x, hi.y, hi.z, hi.w}, ls[4] = {lo.x, lo.y, lo.z, lo.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float2 o = __half22float2(*reinterpret_cast<const __half2 *>(&hs[e]));
+                if (PARTS == 2) {
+                    const float2 l = __half22float2(*reinterpret_cast<const __half2 *>(&ls[e]));
+                    o.x += l.x;
+                    o.y += l.y;
+                }
+                v[8 * k + 2 * e] = fmaf(f, o.x, by * v[8 * k + 2 * e]);
+                v[8 * k + 2 * e + 1] = fmaf(f, o.y, by * v[8 * k + 2 * e + 1]);
+            }
+        }
+    }
+    __syncwarp();
+    if (PHASE == kLast) {
+        // to the weight, 32 elements next to each other at a time: of a tall matrix, what the lanes hold of a column
+        T *dst = (T *)J.dst;
+        const bool tall = J.rows > J.cols;
+        float *turned = (float *)piece;
+        if (!tall) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) turned[lane * 33 + k] = v[k];
+            __syncwarp();
+        }
+        const int64_t step = J.cols, first = tall ? (int64_t)c * step + r0 + lane : (int64_t)r0 * step + c + lane;
+        const int many = min(32, tall ? J.n - c : J.m - r0);          // rows of the weight
+        const bool mine = tall ? r0 + lane < J.m : c + lane < J.n;
+#pragma unroll
+        for (int k0 = 0; k0 < 32; k0 += 8) {
+            float w[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) w[k] = J.mom && mine && k0 + k < many ? ns_in(dst[first + (k0 + k) * step]) : 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float o = (tall ? v[k0 + k] : turned[(k0 + k) * 33 + lane]) * (1.0f / kScaleX);
+                if (mine && k0 + k < many) dst[first + (k0 + k) * step] = ns_out<T>(J.mom ? fmaf(J.keep, w[k], -J.step * o) : o);
+            }
+        }
+        __syncwarp();
+    } else {
+        unsigned char *to = (PHASE == kGram ? J.a : PHASE == kPolynomial ? J.b : J.x[from ^ 1]) + block;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            uint4 hi, lo;
+            ns_split<PARTS>(v[8 * k], v[8 * k + 1], hi.x, lo.x);
+            ns_split<PARTS>(v[8 * k + 2], v[8 * k + 3], hi.y, lo.y);
+            ns_split<PARTS>(v[8 * k + 4], v[8 * k + 5], hi.z, lo.z);
+            ns_split<PARTS>(v[8 * k + 6], v[8 * k + 7], hi.w, lo.w);
+            *(uint4 *)(piece + ns_piece_at(lane, k)) = hi;
+            if (PARTS == 2) *(uint4 *)(piece + 2048 + ns_piece_at(lane, k)) = lo;
+        }
+        __syncwarp();
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) ns_move_piece<true>(to + p * kBlock, piece + p * 2048, r0, c, lane);
+    }
+}
+
+// Persistent: a CTA (a pair of them) takes tiles of the result.  PHASE
+//   kGram        a = x x^T                  kPolynomial  b = cb a + cc a a
+//   kUpdate      x' = ca x + b x            kLast        the same, and the result goes to the weight
+// a and b are symmetric: their blocks below the diagonal are neither computed nor stored.  Where a product wants one as
+// rows, it takes the block across the diagonal as columns.
+//
+// With CG = 1 and a cluster of several CTAs, these share one tile: each sums over its part of the steps, they exchange the sums
+// through shared memory, and each takes some 32 x 32 pieces of the total, added up in the order of the ranks.
+template <int PHASE, int PARTS, int CG, typename T>
 __global__ void __launch_bounds__(kNsThreads, 1) ns_product_kernel(const __grid_constant__ NsArgs A, int from, int tiles, int *status)
 {
-    using Tile = NsTile<PARTS, TN>;
-    constexpr int S = Tile::kStages;
+    using Tile = NsTile<PARTS, CG>;
+    constexpr int S = Tile::kStages, TN = Tile::TN;
     constexpr bool kSymmetric = PHASE == kGram || PHASE == kPolynomial;
     extern __shared__ unsigned char smem_raw[];
     unsigned char *smem = (unsigned char *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    uint64_t *full = (uint64_t *)(smem + S * Tile::kStage), *empty = full + S, *done = empty + S, *taken = done + 2;
+    // full: this CTA's loads are there; ready: the second CTA's are (at the first); empty: a stage has been read; done: a sum is
+    // complete; taken: it has been taken out
+    uint64_t *full = (uint64_t *)(smem + S * Tile::kStage), *ready = full + S, *empty = ready + S, *done = empty + S, *taken = done + 2;
     uint32_t *base_at = (uint32_t *)(taken + 2);
-    float *pieces = (float *)(smem + S * Tile::kStage + 512);
+    unsigned char *pieces = smem + S * Tile::kStage + 512;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (warp == 1) tensor_alloc(base_at, 2 * TN);
+    const int rank = (int)cluster_rank(), ranks = (int)cluster_size();
+    const int split = CG == 1 ? ranks : 1, pair = CG == 2 ? rank : 0;
+    if (warp == 1) tensor_alloc<CG>(base_at, 2 * TN);
     if (threadIdx.x == 0) {
         for (int i = 0; i < S; ++i) {
             mbar_init(full + i, 1);
+            mbar_init(ready + i, 1);
             mbar_init(empty + i, 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(done + i, 1);
-            mbar_init(taken + i, 8);
+            mbar_init(taken + i, 8 * CG);
         }
         mbar_init_fence();
     }
     tensor_fence_before();
     __syncthreads();
+    if (ranks > 1) cluster_wait_all();
     tensor_fence_after();
     const uint32_t acc = *base_at;
     bool fine = true;
+    const int tile0 = blockIdx.x / ranks, tile_step = gridDim.x / ranks;
 
-    // tile -> its job, the row block and the first column block of 128, and how many of those there are
-    auto locate = [&](int tile, const NsJob *&J, int &i, int &j, int &nb) {
+    // tile -> its job, its first row block and its first column block
+    auto locate = [&](int tile, const NsJob *&J, int &i, int &j) {
         const int k = ns_find<kSymmetric ? 1 : 2>(A, tile);
         J = &A.job[k];
         int at = tile - J->first[kSymmetric ? 1 : 2];
-        const int rb = ns_rb(J->m), W = TN / 128;
+        const int rt = (ns_rb(J->m) + CG - 1) / CG;
         if (kSymmetric) {
-            // row block i has the column tiles from i / W on
-            const int ct = (rb + W - 1) / W;
-            for (i = 0; at >= ct - i / W; ++i) at -= ct - i / W;
-            j = (i / W + at) * W;
-            nb = min(W, rb - j);
+            // a row of tiles begins at the diagonal
+            for (i = 0; at >= rt - i; ++i) at -= rt - i;
+            j = i + at;
         } else {
             // tiles that run side by side share columns of x
-            i = at % rb;
-            j = at / rb * W;
-            nb = min(W, ns_rb(J->n) - j);
+            i = at % rt;
+            j = at / rt;
         }
+        i *= CG;
+        j *= CG;
+    };
+    // whether step k takes an operand from across the diagonal (of the two row blocks of a pair, which take it alike, one may be the
+    // diagonal's own, which is the same either way)
+    auto left_turned = [&](int i, int k) { return PHASE != kGram && (k >> 1) < i + CG - 1; };
+    auto right_turned = [&](int j, int k) { return PHASE == kPolynomial ? (k >> 1) < j + CG - 1 : !kSymmetric; };
+    // this CTA's part of the steps
+    auto part = [&](const NsJob &J, int &k0, int &k1) {
+        const int steps = PHASE == kGram ? ns_cb(J.n) : ns_cb(J.m);
+        k0 = steps * rank / split * (CG == 1);
+        k1 = CG == 1 ? steps * (rank + 1) / split : steps;
     };
 
-    if (warp == 0 && lane == 0) {
-        int s = 0, phase = 0;
-        for (int tile = blockIdx.x; fine && tile < tiles; tile += gridDim.x) {
-            const NsJob *J;
-            int i, j, nb;
-            locate(tile, J, i, j, nb);
-            const int cbm = ns_cb(J->m), cbn = ns_cb(J->n);
-            const int steps = PHASE == kGram ? cbn : cbm;
-            const unsigned char *left = PHASE == kGram ? J->x[from] : PHASE == kPolynomial ? J->a : J->b;
-            const unsigned char *right = PHASE == kPolynomial ? J->a : J->x[from];
-            const unsigned bytes = PARTS * kBlock * (1 + nb);
-            for (int k = 0; k < steps; ++k) {
-                if (!mbar_wait_bounded(empty + s, phase ^ 1, kWaitLimit)) { fine = false; break; }
-                unsigned char *to = smem + s * Tile::kStage;
-                mbar_expect_tx(full + s, bytes);
-                bulk_load(to, left + ((int64_t)i * steps + k) * (PARTS * kBlock), PARTS * kBlock, full + s);
-                to += Tile::kA;
-                if (kSymmetric) {
-                    // [part][block]: rows of the operand follow one another
-                    for (int b = 0; b < nb; ++b)
+    if (warp < 4) {
+        // 128 threads give registers to the 256 that hold sums: 128 * 56 + 256 * 216 <= 384 * 168
+        if constexpr (CG == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 0 && lane == 0) {
+            int s = 0, phase = 0;
+            for (int tile = tile0; fine && tile < tiles; tile += tile_step) {
+                const NsJob *J;
+                int i, j, k0, k1;
+                locate(tile, J, i, j);
+                part(*J, k0, k1);
+                const int cbm = ns_cb(J->m), cbn = ns_cb(J->n);
+                const int cbl = PHASE == kGram ? cbn : cbm, cbr = PHASE == kPolynomial ? cbm : cbn;
+                const unsigned char *left = PHASE == kGram ? J->x[from] : PHASE == kPolynomial ? J->a : J->b;
+                const unsigned char *right = PHASE == kPolynomial ? J->a : J->x[from];
+                const int il = i + pair, jr = j + pair;        // this CTA's row block and column block; behind the last one, nothing
+                const bool has_left = il < ns_rb(J->m), has_right = jr < (kSymmetric ? ns_rb(J->m) : ns_rb(J->n));
+                const unsigned bytes = PARTS * kBlock * (has_left + has_right);
+                // 64 rows of two blocks of 64 columns: [part][column block]
+                auto columns = [&](unsigned char *to, const unsigned char *x, int cbs, int k, int block) {
+                    const unsigned char *row = x + ((int64_t)(k >> 1) * cbs + 2 * block) * (PARTS * kBlock) + (k & 1) * (kBlock / 2);
+                    for (int b = 0; b < 2; ++b)
                         for (int p = 0; p < PARTS; ++p)
-                            bulk_load(to + (p * (TN / 128) + b) * kBlock, right + (((int64_t)(j + b) * steps + k) * PARTS + p) * kBlock, kBlock, full + s);
-                } else {
-                    // 64 rows of each block of 64 columns: [part][column block]
-                    const unsigned char *row = right + ((int64_t)(k >> 1) * cbn + 2 * j) * (PARTS * kBlock) + (k & 1) * (kBlock / 2);
-                    for (int b = 0; b < 2 * nb; ++b)
-                        for (int p = 0; p < PARTS; ++p)
-                            bulk_load(to + (p * (TN / 64) + b) * (kBlock / 2), row + (b * PARTS + p) * kBlock, kBlock / 2, full + s);
+                            bulk_load(to + p * kBlock + b * (kBlock / 2), row + (b * PARTS + p) * kBlock, kBlock / 2, full + s);
+                };
+                for (int k = k0; k < k1; ++k) {
+                    if (!mbar_wait_bounded(empty + s, phase ^ 1, kWaitLimit)) { fine = false; break; }
+                    unsigned char *to = smem + s * Tile::kStage;
+                    mbar_expect_tx(full + s, bytes);
+                    if (has_left) {
+                        if (left_turned(i, k)) columns(to, left, cbl, k, il);
+                        else bulk_load(to, left + ((int64_t)il * cbl + k) * (PARTS * kBlock), PARTS * kBlock, full + s);
+                    }
+                    to += Tile::kA;
+                    if (has_right) {
+                        if (right_turned(j, k)) columns(to, right, cbr, k, jr);
+                        else bulk_load(to, right + ((int64_t)jr * cbr + k) * (PARTS * kBlock), PARTS * kBlock, full + s);
+                    }
+                    if (++s == S) { s = 0; phase ^= 1; }
                 }
+            }
+            // every stage's last copy has been read before the CTA leaves
+            for (int k = 0; k < S; ++k) {
+                if (!mbar_wait_bounded(empty + s, phase ^ 1, kWaitLimit)) fine = false;
                 if (++s == S) { s = 0; phase ^= 1; }
             }
-        }
-        // every stage's last copy has been read before the CTA leaves
-        for (int k = 0; k < S; ++k) {
-            if (!mbar_wait_bounded(empty + s, phase ^ 1, kWaitLimit)) fine = false;
-            if (++s == S) { s = 0; phase ^= 1; }
-        }
-    } else if (warp == 1 && lane == 0) {
-        int s = 0, phase = 0, slot = 0, turn = 0;
-        for (int tile = blockIdx.x; fine && tile < tiles; tile += gridDim.x) {
-            const NsJob *J;
-            int i, j, nb;
-            locate(tile, J, i, j, nb);
-            const int steps = PHASE == kGram ? ns_cb(J->n) : ns_cb(J->m);
-            const uint32_t shape = product_shape(128, nb * 128, !kSymmetric), d = acc + slot * TN;
-            if (!mbar_wait_bounded(taken + slot, turn ^ 1, kWaitLimit)) { fine = false; break; }
-            tensor_fence_after();
-            for (int k = 0; k < steps; ++k) {
-                if (!mbar_wait_bounded(full + s, phase, kWaitLimit)) { fine = false; break; }
-                tensor_fence_after();
-                const unsigned a0 = smem_u32(smem + s * Tile::kStage), b0 = a0 + Tile::kA;
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    uint64_t l[PARTS], r[PARTS];
-#pragma unroll
-                    for (int p = 0; p < PARTS; ++p) {
-                        l[p] = desc_rows(a0 + p * kBlock + q * 32);
-                        r[p] = kSymmetric ? desc_rows(b0 + p * (TN / 128) * kBlock + q * 32)
-                                          : desc_columns(b0 + p * (TN / 128) * kBlock + q * 2048, kBlock / 2);
-                    }
-                    product(d, l[0], r[0], shape, k + q > 0);
-                    if (PARTS == 2) {
-                        product(d, l[0], r[PARTS - 1], shape, true);
-                        product(d, l[PARTS - 1], r[0], shape, true);
-                    }
-                }
-                product_commit(empty + s);
-                if (++s == S) { s = 0; phase ^= 1; }
-            }
-            if (!fine) break;
-            product_commit(done + slot);
-            if ((slot ^= 1) == 0) turn ^= 1;
-        }
-        // the results have been taken before the CTA leaves
-        for (int k = 0; fine && k < 2; ++k) {
-            if (!mbar_wait_bounded(taken + slot, turn ^ 1, kWaitLimit)) fine = false;
-            if ((slot ^= 1) == 0) turn ^= 1;
-        }
-    } else if (warp >= 2) {
-        int slot = 0, turn = 0;
-        const int w = warp - 2, quarter = warp & 3, half = w >> 2;
-        float *piece = pieces + w * 32 * 33;
-        for (int tile = blockIdx.x; fine && tile < tiles; tile += gridDim.x) {
-            const NsJob *J;
-            int i, j, nb;
-            locate(tile, J, i, j, nb);
-            const int cbm = ns_cb(J->m), cbn = ns_cb(J->n);
-            if (!__all_sync(0xffffffffu, mbar_wait_bounded(done + slot, turn, kWaitLimit))) { fine = false; break; }
-            tensor_fence_after();
-            const int r = i * 128 + quarter * 32 + lane;
-            for (int c0 = half * (TN / 2); c0 < (half + 1) * (TN / 2) && c0 < nb * 128; c0 += 32) {
-                const int block = j + (c0 >> 7);          // column block of 128
-                if (kSymmetric && block < i) continue;
-                float v[32];
-                tensor_read(v, acc + slot * TN + ((uint32_t)(quarter * 32) << 16) + c0);
-                const int c = j * 128 + c0;
-                const int cbs = kSymmetric ? cbm : cbn;
-                if (PHASE != kGram) {
-                    // b = cb a + ..., x' = ca x + ...
-                    unsigned char *old = PHASE == kPolynomial ? J->a : J->x[from];
-                    const float f = PHASE == kPolynomial ? A.cb : A.ca;
-                    const float by = PHASE == kPolynomial ? A.cc / kScaleA : 1.0f / kScaleA;
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const unsigned char *at = ns_chunk<PARTS>(old, cbs, r, c + 8 * k);
-                        const uint4 hi = *(const uint4 *)at;
-                        uint4 lo = make_uint4(0, 0, 0, 0);
-                        if (PARTS == 2) lo = *(const uint4 *)(at + kBlock);
-                        const uint32_t hs[4] = {hi.x, hi.y, hi.z, hi.w}, ls[4] = {lo.x, lo.y, lo.z, lo.w};
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            float2 o = __half22float2(*reinterpret_cast<const __half2 *>(&hs[e]));
-                            if (PARTS == 2) {
-                                const float2 l = __half22float2(*reinterpret_cast<const __half2 *>(&ls[e]));
-                                o.x += l.x;
-                                o.y += l.y;
-                            }
-                            v[8 * k + 2 * e] = fmaf(f, o.x, by * v[8 * k + 2 * e]);
-                            v[8 * k + 2 * e + 1] = fmaf(f, o.y, by * v[8 * k + 2 * e + 1]);
-                        }
-                    }
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 32; ++k) v[k] *= kScaleA / (kScaleX * kScaleX);
-                }
-                if (PHASE == kLast) {
-                    // to the weight, 32 elements next to each other at a time: of a tall matrix, what the lanes hold of a column
-                    T *dst = (T *)J->dst;
-                    const auto put = [&](int row, int col, int64_t at, float o) {
-                        o *= 1.0f / kScaleX;
-                        if (row < J->m && col < J->n) dst[at] = ns_out<T>(J->mom ? fmaf(J->keep, ns_in(dst[at]), -J->step * o) : o);
+        } else if (warp == 1 && lane == 0 && pair == 0) {
+            int s = 0, phase = 0, slot = 0, turn = 0;
+            for (int tile = tile0; fine && tile < tiles; tile += tile_step) {
+                const NsJob *J;
+                int i, j, k0, k1;
+                locate(tile, J, i, j);
+                part(*J, k0, k1);
+                for (int k = k0; k < k1; ++k) {
+                    const bool first = (k - k0) % Tile::kGroup == 0;
+                    if (first && !mbar_wait_cluster(taken + slot, turn ^ 1, kWaitLimit)) { fine = false; break; }
+                    if (!mbar_wait_bounded(full + s, phase, kWaitLimit)) { fine = false; break; }
+                    if (CG == 2 && !mbar_wait_cluster(ready + s, phase, kWaitLimit)) { fine = false; break; }
+                    tensor_fence_after();
+                    const unsigned a0 = smem_u32(smem + s * Tile::kStage), b0 = a0 + Tile::kA;
+                    const bool lt = left_turned(i, k), rt = right_turned(j, k);
+                    const uint32_t shape = product_shape(128 * CG, TN, lt, rt), d = acc + slot * TN;
+                    const auto operand = [&](unsigned base, bool turned, int p, int q) {
+                        return turned ? desc_columns(base + p * kBlock + q * 2048, kBlock / 2) : desc_rows(base + p * kBlock + q * 32);
                     };
-                    if (J->rows > J->cols) {
+                    // the small products first: what they lose to the sum's size is less while it is small
+                    if (PARTS == 2) {
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) put(r, c + k, (int64_t)(c + k) * J->cols + r, v[k]);
-                    } else {
-                        const int r0 = i * 128 + quarter * 32;
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) piece[lane * 33 + k] = v[k];
-                        __syncwarp();
-#pragma unroll 8
-                        for (int k = 0; k < 32; ++k) put(r0 + k, c + lane, (int64_t)(r0 + k) * J->cols + c + lane, piece[k * 33 + lane]);
-                    }
-                    __syncwarp();
-                    continue;
-                }
-                unsigned char *to = PHASE == kGram ? J->a : PHASE == kPolynomial ? J->b : J->x[from ^ 1];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    uint4 hi, lo;
-                    ns_split<PARTS>(v[8 * k], v[8 * k + 1], hi.x, lo.x);
-                    ns_split<PARTS>(v[8 * k + 2], v[8 * k + 3], hi.y, lo.y);
-                    ns_split<PARTS>(v[8 * k + 4], v[8 * k + 5], hi.z, lo.z);
-                    ns_split<PARTS>(v[8 * k + 6], v[8 * k + 7], hi.w, lo.w);
-                    unsigned char *at = ns_chunk<PARTS>(to, cbs, r, c + 8 * k);
-                    *(uint4 *)at = hi;
-                    if (PARTS == 2) *(uint4 *)(at + kBlock) = lo;
-                    if (kSymmetric && block > i) {
-                        // (c, r) too: 32 lanes write 64 bytes of a row
-                        const uint32_t hs[4] = {hi.x, hi.y, hi.z, hi.w}, ls[4] = {lo.x, lo.y, lo.z, lo.w};
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            unsigned char *mirror = ns_chunk<PARTS>(to, cbs, c + 8 * k + e, r) + (r & 7) * 2;
-                            *(uint16_t *)mirror = (uint16_t)(hs[e >> 1] >> (e & 1) * 16);
-                            if (PARTS == 2) *(uint16_t *)(mirror + kBlock) = (uint16_t)(ls[e >> 1] >> (e & 1) * 16);
+                        for (int q = 0; q < 4; ++q) {
+                            product<CG>(d, operand(a0, lt, 0, q), operand(b0, rt, 1, q), shape, !first || q > 0);
+                            product<CG>(d, operand(a0, lt, 1, q), operand(b0, rt, 0, q), shape, true);
                         }
+                    }
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        product<CG>(d, operand(a0, lt, 0, q), operand(b0, rt, 0, q), shape, PARTS == 2 || !first || q > 0);
+                    product_commit<CG>(empty + s);
+                    if (++s == S) { s = 0; phase ^= 1; }
+                    if ((k + 1 - k0) % Tile::kGroup == 0 || k + 1 == k1) {
+                        product_commit<CG>(done + slot);
+                        if ((slot ^= 1) == 0) turn ^= 1;
                     }
                 }
             }
-            tensor_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(taken + slot);
-            if ((slot ^= 1) == 0) turn ^= 1;
+        } else if (CG == 2 && warp == 1 && lane == 0) {
+            // the second CTA tells the first what it has loaded
+            int s = 0, phase = 0;
+            for (int tile = tile0; fine && tile < tiles; tile += tile_step) {
+                const NsJob *J;
+                int i, j, k0, k1;
+                locate(tile, J, i, j);
+                part(*J, k0, k1);
+                for (int k = k0; k < k1; ++k) {
+                    if (!mbar_wait_bounded(full + s, phase, kWaitLimit)) { fine = false; break; }
+                    mbar_arrive_at(ready + s, 0);
+                    if (++s == S) { s = 0; phase ^= 1; }
+                }
+            }
         }
+        __syncwarp();
+        if (CG == 1 && split > 1) cluster_wait_all();
+    } else {
+        if constexpr (CG == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        int slot = 0, turn = 0;
+        const int w = warp - 4, quarter = warp & 3, half = w >> 2;
+        unsigned char *piece = pieces + w * Tile::kPiece;
+        for (int tile = tile0; fine && tile < tiles; tile += tile_step) {
+            const NsJob *J;
+            int i, j, k0, k1;
+            locate(tile, J, i, j);
+            part(*J, k0, k1);
+            const int r0 = (i + pair) * 128 + quarter * 32;
+            const int groups = (k1 - k0 + Tile::kGroup - 1) / Tile::kGroup;
+            const int il = i + pair, c0 = half * (TN / 2), jl = j + (c0 >> 7);      // this warp's columns of the tile; its blocks
+            const bool mine = il < ns_rb(J->m) && jl < (kSymmetric ? ns_rb(J->m) : ns_rb(J->n)) && !(kSymmetric && jl < il);
+            const uint32_t at = acc + ((uint32_t)(quarter * 32) << 16) + c0;
+            float sum[PARTS == 2 ? TN / 64 : 1][32];
+            // the exchange of a shared tile: four columns of all rows after one another
+            auto give = [&](const float (&v)[32], int u) {
+                float4 *to = (float4 *)smem + ((c0 + u * 32) / 4) * 128 + quarter * 32 + lane;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) to[k * 128] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+            };
+            if constexpr (PARTS == 2) {
+#pragma unroll
+                for (int u = 0; u < TN / 64; ++u)
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) sum[u][k] = 0.0f;
+            }
+            for (int g = 0; g < groups; ++g) {
+                if (!__all_sync(0xffffffffu, mbar_wait_cluster(done + slot, turn, kWaitLimit))) { fine = false; break; }
+                tensor_fence_after();
+                if (mine) {
+#pragma unroll
+                    for (int u = 0; u < TN / 64; ++u) {
+                        float v[32];
+                        tensor_read(v, at + slot * TN + u * 32);
+                        if constexpr (PARTS == 2) {
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) sum[u][k] += v[k];
+                        } else if (split > 1) {
+                            give(v, u);
+                        } else {
+                            ns_take_piece<PHASE, PARTS, T>(A, *J, from, il * 128 + quarter * 32, j * 128 + c0 + u * 32, v, piece, lane);
+                        }
+                    }
+                }
+                tensor_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if (CG == 2) mbar_arrive_at(taken + slot, 0);
+                    else mbar_arrive(taken + slot);
+                }
+                if ((slot ^= 1) == 0) turn ^= 1;
+            }
+            if (PARTS == 1 && groups == 0) {              // more CTAs than steps
+                const float v[32] = {};
+#pragma unroll
+                for (int u = 0; u < TN / 64; ++u) give(v, u);
+            }
+            if constexpr (PARTS == 2) {
+                if (fine && mine) {
+#pragma unroll
+                    for (int u = 0; u < TN / 64; ++u) {
+                        if (split > 1) give(sum[u], u);
+                        else ns_take_piece<PHASE, PARTS, T>(A, *J, from, r0, j * 128 + c0 + u * 32, sum[u], piece, lane);
+                    }
+                }
+            }
+        }
+        if (CG == 1 && split > 1) {
+            __syncwarp();
+            cluster_wait_all();
+            if (tile0 < tiles) {
+                const NsJob *J;
+                int i, j;
+                locate(tile0, J, i, j);
+                for (int u = w * split + rank; u < 16; u += 8 * split) {
+                    const int quarter = u & 3, c = u >> 2;
+                    const float4 *at = (const float4 *)smem + c * 8 * 128 + quarter * 32 + lane;
+                    float v[32] = {};
+                    for (int r = 0; r < split; ++r) {
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const float4 x = read_at(at + k * 128, r);
+                            v[4 * k] += x.x;
+                            v[4 * k + 1] += x.y;
+                            v[4 * k + 2] += x.z;
+                            v[4 * k + 3] += x.w;
+                        }
+                    }
+                    ns_take_piece<PHASE, PARTS, T>(A, *J, from, i * 128 + quarter * 32, j * 128 + c * 32, v, piece, lane);
+                }
+            }
+        }
+        __syncwarp();
     }
     if (!fine) atomicExch(status, kStatusNsTimeout);
-    __syncwarp();
     tensor_fence_before();
     __syncthreads();
+    if (ranks > 1) cluster_wait_all();               // no CTA leaves while another reads its memory or arrives at its barriers
     if (warp == 1) {
         tensor_fence_after();
-        tensor_free(acc, 2 * TN);
+        tensor_free<CG>(acc, 2 * TN);
     }
 }
 
@@ -440,18 +662,38 @@ static void ns_take(NsJob &J, int parts, unsigned char *&at)
     at = J.b + a;
 }
 
-template <int PHASE, int PARTS, int TN, typename T>
-static int ns_product(const NsArgs &A, int from, int tiles, int *status, cudaStream_t st)
+// CTAs that share a tile where there are too few tiles for the SMs, each with two steps at least
+static int ns_split(int tiles, int steps)
 {
-    auto kern = ns_product_kernel<PHASE, PARTS, TN, T>;
-    constexpr size_t smem = NsTile<PARTS, TN>::kSmem;
+    int split = 1;
+    while (split < 8 && tiles * split * 2 <= sm_count() && steps >= split * 4) split *= 2;
+    return split;
+}
+
+template <int PHASE, int PARTS, int CG, typename T>
+static int ns_product(const NsArgs &A, int from, int tiles, int split, int *status, cudaStream_t st)
+{
+    auto kern = ns_product_kernel<PHASE, PARTS, CG, T>;
+    constexpr size_t smem = NsTile<PARTS, CG>::kSmem;
     int rc = reserve_dynamic_smem((const void *)kern, smem);
     if (rc) return rc;
-    kern<<<tiles < sm_count() ? tiles : sm_count(), kNsThreads, smem, st>>>(A, from, tiles, status);
+    const int ranks = CG == 2 ? 2 : split, most = sm_count() / ranks;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((tiles < most ? tiles : most) * ranks);
+    cfg.blockDim = dim3(kNsThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ranks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, kern, A, from, tiles, status);
     return check_launch("Newton-Schulz product launch");
 }
 
-template <typename T, int PARTS, int TN>
+template <typename T, int PARTS, int CG>
 static int ns_run(NsArgs &A, int steps, cudaStream_t st)
 {
     int *status = device_status_word();
@@ -459,7 +701,7 @@ static int ns_run(NsArgs &A, int steps, cudaStream_t st)
         set_error("Newton-Schulz products: no status word on this device");
         return SLAYER_B200_ECUDA;
     }
-    int blocks = 0, small = 0, large = 0;
+    int blocks = 0, small = 0, large = 0, m = 0, n = 0;
     for (int j = 0; j < A.jobs; ++j) {
         NsJob &J = A.job[j];
         const int64_t want = ceil_div((int64_t)ns_rb(J.m) * ns_cb(J.n) * 128 * 64, 4096);
@@ -468,21 +710,21 @@ static int ns_run(NsArgs &A, int steps, cudaStream_t st)
         J.first[1] = small;
         J.first[2] = large;
         blocks += J.norm_parts;
-        const int rb = ns_rb(J.m), W = TN / 128, ct = (rb + W - 1) / W;
-        for (int i = 0; i < rb; ++i) small += ct - i / W;
-        large += rb * ((ns_rb(J.n) + W - 1) / W);
+        const int rt = (ns_rb(J.m) + CG - 1) / CG;
+        small += rt * (rt + 1) / 2;
+        large += rt * ((ns_rb(J.n) + CG - 1) / CG);
+        m = J.m > m ? J.m : m;
+        n = J.n > n ? J.n : n;
     }
     ns_momentum_kernel<T><<<blocks, 256, 0, st>>>(A);
-    int rc = check_launch("momentum launch");
-    if (rc) return rc;
-    int from = 0;
     ns_normalise_kernel<T, PARTS><<<blocks, 256, 0, st>>>(A);
-    rc = check_launch("Newton-Schulz normalisation launch");
+    int rc = check_launch("Newton-Schulz normalisation launch"), from = 0;
+    const int split_n = ns_split(small, ns_cb(n)), split_m = ns_split(small, ns_cb(m)), split_x = ns_split(large, ns_cb(m));
     for (int s = 0; s < steps && !rc; ++s, from ^= 1) {
-        rc = ns_product<kGram, PARTS, TN, float>(A, from, small, status, st);
-        if (!rc) rc = ns_product<kPolynomial, PARTS, TN, float>(A, from, small, status, st);
-        if (!rc) rc = s + 1 < steps ? ns_product<kUpdate, PARTS, TN, float>(A, from, large, status, st)
-                                    : ns_product<kLast, PARTS, TN, T>(A, from, large, status, st);
+        rc = ns_product<kGram, PARTS, CG, float>(A, from, small, split_n, status, st);
+        if (!rc) rc = ns_product<kPolynomial, PARTS, CG, float>(A, from, small, split_m, status, st);
+        if (!rc) rc = s + 1 < steps ? ns_product<kUpdate, PARTS, CG, float>(A, from, large, split_x, status, st)
+                                    : ns_product<kLast, PARTS, CG, T>(A, from, large, split_x, status, st);
     }
     return rc;
 }
@@ -529,10 +771,10 @@ static int ns_shape(const char *what, int64_t rows, int64_t cols)
 template <typename T, int PARTS>
 static int ns_tiled(NsArgs &A, int steps, cudaStream_t st)
 {
-    // wide tiles where there are enough of them
+    // tiles of two CTAs where there are enough of them
     int64_t tiles = 0;
-    for (int j = 0; j < A.jobs; ++j) tiles += (int64_t)ns_rb(A.job[j].m) * ns_rb(A.job[j].m) / 4;
-    return tiles >= sm_count() ? ns_run<T, PARTS, 256>(A, steps, st) : ns_run<T, PARTS, 128>(A, steps, st);
+    for (int j = 0; j < A.jobs; ++j) tiles += (int64_t)((ns_rb(A.job[j].m) + 1) / 2) * ((ns_rb(A.job[j].n) + 1) / 2);
+    return tiles >= sm_count() / 2 ? ns_run<T, PARTS, 2>(A, steps, st) : ns_run<T, PARTS, 1>(A, steps, st);
 }
 
 static int ns_dispatch(NsArgs &A, int dtype, int steps, cudaStream_t st)

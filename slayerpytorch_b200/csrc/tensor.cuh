@@ -21,39 +21,65 @@ __device__ __forceinline__ uint64_t desc_columns(unsigned addr, unsigned far)
     return (uint64_t)((addr & 0x3ffff) >> 4) | (uint64_t)(far >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
 
-// fp16 x fp16 -> fp32, M x N; by_columns: the second operand is given by desc_columns
-__device__ __forceinline__ uint32_t product_shape(int m, int n, bool by_columns)
+// fp16 x fp16 -> fp32, M x N; which operands are given by desc_columns
+__device__ __forceinline__ uint32_t product_shape(int m, int n, bool a_columns, bool b_columns)
 {
-    return 1u << 4 | (by_columns ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24;
+    return 1u << 4 | (a_columns ? 1u << 15 : 0u) | (b_columns ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24;
 }
+
+// The operations come for one CTA (CG = 1), or for a cluster of two (CG = 2) whose tensor cores make one product of twice the rows:
+// each CTA has half of the first operand's rows and half of the second's, at the same places of its shared memory, and gets
+// its own rows of the result.  The first CTA issues it.
 
 // one thread: d (+)= a b, 16 steps of the summation index
+template <int CG>
 __device__ __forceinline__ void product(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool add)
 {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(d), "l"(a), "l"(b), "r"(shape), "r"((uint32_t)add)
-        : "memory");
+    if constexpr (CG == 1)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+            ::"r"(d), "l"(a), "l"(b), "r"(shape), "r"((uint32_t)add)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+            ::"r"(d), "l"(a), "l"(b), "r"(shape), "r"((uint32_t)add)
+            : "memory");
 }
 
-// the barrier is told when all products that this thread has issued are done
+// the barrier (of both CTAs) is told when all products that this thread has issued are done
+template <int CG>
 __device__ __forceinline__ void product_commit(uint64_t *bar)
 {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+    if constexpr (CG == 1)
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                     ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
 }
 
-// one warp; `columns` a power of two from 32 to 512
+// one warp (of each CTA); `columns` a power of two from 32 to 512
+template <int CG>
 __device__ __forceinline__ void tensor_alloc(uint32_t *where, uint32_t columns)
 {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(where)), "r"(columns) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    if constexpr (CG == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(where)), "r"(columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(where)), "r"(columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    }
 }
 
+template <int CG>
 __device__ __forceinline__ void tensor_free(uint32_t base, uint32_t columns)
 {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(columns));
+    if constexpr (CG == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(columns));
+    else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(columns));
 }
 
 __device__ __forceinline__ void tensor_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -82,6 +108,64 @@ __device__ __forceinline__ void bulk_load(void *dst, const void *src, unsigned b
 {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+
+// the barrier at the same place of another CTA of the cluster
+__device__ __forceinline__ void mbar_arrive_at(uint64_t *bar, unsigned rank)
+{
+    asm volatile(
+        "{\n\t.reg .b32 far;\n\t"
+        "mapa.shared::cluster.u32 far, %0, %1;\n\t"
+        "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [far];\n\t}"
+        ::"r"(smem_u32(bar)), "r"(rank) : "memory");
+}
+
+// mbar_wait_bounded on a barrier that other CTAs of the cluster arrive at
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t *bar, unsigned parity, int limit)
+{
+    for (int i = 0; i < limit; ++i) {
+        unsigned ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+        if (ok) return true;
+    }
+    return false;
+}
+
+__device__ __forceinline__ unsigned cluster_rank()
+{
+    unsigned r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+
+__device__ __forceinline__ unsigned cluster_size()
+{
+    unsigned r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+
+// all threads of all CTAs of the cluster
+__device__ __forceinline__ void cluster_wait_all()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// 16 bytes at the same place of another CTA's shared memory
+__device__ __forceinline__ float4 read_at(const void *p, unsigned rank)
+{
+    float4 v;
+    asm volatile(
+        "{\n\t.reg .b32 far;\n\t"
+        "mapa.shared::cluster.u32 far, %4, %5;\n\t"
+        "ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [far];\n\t}"
+        : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(smem_u32(p)), "r"(rank) : "memory");
+    return v;
 }
 
 __device__ __forceinline__ void mbar_arrive(uint64_t *bar)

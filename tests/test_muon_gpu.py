@@ -69,6 +69,14 @@ def test_orthogonalize(shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(1500, 3300), (2310, 2050), (10, 400, 900), (9, 1, 640, 513), (40, 300, 150)])
+def test_orthogonalize_many_tiles(shape, dtype):
+    """Enough tiles for pairs of CTAs, row and column blocks that have no partner, more tiles than CTAs."""
+    x = gradient(shape, sum(shape), dtype)
+    near(optim.orthogonalize(x.cuda()), want_orthogonal(x.cuda()).cpu(), dtype, min(shape[-2:]) * math.prod(shape[:-2]))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_orthogonalize_stacks_orders_and_scales(dtype):
     x = gradient((2, 3, 40, 70), 5, dtype)
     want = want_orthogonal(x)
