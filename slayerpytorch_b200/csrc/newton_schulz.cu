@@ -492,9 +492,9 @@ __global__ void __launch_bounds__(kNsThreads, 1) ns_product_kernel(const __grid_
                 part(*J, k0, k1);
                 for (int k = k0; k < k1; ++k) {
                     const bool first = (k - k0) % Tile::kGroup == 0;
-                    if (first && !mbar_wait_cluster(taken + slot, turn ^ 1, kWaitLimit)) { fine = false; break; }
+                    if (first && !mbar_wait_bounded(taken + slot, turn ^ 1, kWaitLimit)) { fine = false; break; }
                     if (!mbar_wait_bounded(full + s, phase, kWaitLimit)) { fine = false; break; }
-                    if (CG == 2 && !mbar_wait_cluster(ready + s, phase, kWaitLimit)) { fine = false; break; }
+                    if (CG == 2 && !mbar_wait_bounded(ready + s, phase, kWaitLimit)) { fine = false; break; }
                     tensor_fence_after();
                     const unsigned a0 = smem_u32(smem + s * Tile::kStage), b0 = a0 + Tile::kA;
                     const bool lt = left_turned(i, k), rt = right_turned(j, k);
@@ -567,7 +567,7 @@ __global__ void __launch_bounds__(kNsThreads, 1) ns_product_kernel(const __grid_
                     for (int k = 0; k < 32; ++k) sum[u][k] = 0.0f;
             }
             for (int g = 0; g < groups; ++g) {
-                if (!__all_sync(0xffffffffu, mbar_wait_cluster(done + slot, turn, kWaitLimit))) { fine = false; break; }
+                if (!__all_sync(0xffffffffu, mbar_wait_bounded(done + slot, turn, kWaitLimit))) { fine = false; break; }
                 tensor_fence_after();
                 if (mine) {
 #pragma unroll

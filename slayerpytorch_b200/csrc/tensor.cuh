@@ -110,29 +110,16 @@ __device__ __forceinline__ void bulk_load(void *dst, const void *src, unsigned b
                  ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
 
-// the barrier at the same place of another CTA of the cluster
+// The barrier at the same place of another CTA of the cluster.  What these arrivals stand for lies in shared or tensor memory, where
+// it is by then, so they need none of the ordering of global memory that a release of cluster scope waits for (it and
+// the acquire on the other side took 2000 cycles a step where the products take 512).
 __device__ __forceinline__ void mbar_arrive_at(uint64_t *bar, unsigned rank)
 {
     asm volatile(
         "{\n\t.reg .b32 far;\n\t"
         "mapa.shared::cluster.u32 far, %0, %1;\n\t"
-        "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [far];\n\t}"
+        "mbarrier.arrive.shared::cluster.b64 _, [far];\n\t}"
         ::"r"(smem_u32(bar)), "r"(rank) : "memory");
-}
-
-// mbar_wait_bounded on a barrier that other CTAs of the cluster arrive at
-__device__ __forceinline__ bool mbar_wait_cluster(uint64_t *bar, unsigned parity, int limit)
-{
-    for (int i = 0; i < limit; ++i) {
-        unsigned ok;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
-        if (ok) return true;
-    }
-    return false;
 }
 
 __device__ __forceinline__ unsigned cluster_rank()
