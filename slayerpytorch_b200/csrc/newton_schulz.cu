@@ -20,6 +20,10 @@
 #include <cuda_fp16.h>
 #include <math.h>
 
+#include <map>
+#include <mutex>
+#include <tuple>
+
 #include "common.cuh"
 #include "tensor.cuh"
 
@@ -110,8 +114,9 @@ __device__ __forceinline__ void ns_load8(float (&v)[8], const T *p)
 
 // momentum, and the squares' partial sums (double: a sum over up to 2^31 squares, of values of any size)
 template <typename T>
-__global__ void __launch_bounds__(256) ns_momentum_kernel(const __grid_constant__ NsArgs A)
+__global__ void __launch_bounds__(256) ns_momentum_kernel(const __grid_constant__ NsArgs A, unsigned *arrived)
 {
+    if (blockIdx.x == 0 && threadIdx.x == 0) *arrived = 0;
     __shared__ double part[32];
     const NsJob &J = A.job[ns_find<0>(A, blockIdx.x)];
     const int me = blockIdx.x - J.first[0];
@@ -153,14 +158,24 @@ __global__ void __launch_bounds__(256) ns_momentum_kernel(const __grid_constant_
             }
         }
     }
-    for (int64_t i = done + start; i < count; i += step) {
-        float u = ns_in(g[i]);
-        if (mom) {
-            const float m = fmaf(A.mu, mom[i], u);
-            mom[i] = m;
-            u = A.nesterov ? fmaf(A.mu, m, u) : m;
+    for (int64_t i0 = done + start; i0 < count; i0 += 8 * step) {
+        float u[8], m[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int64_t i = i0 + k * step;
+            u[k] = i < count ? ns_in(g[i]) : 0.0f;
+            m[k] = mom && i < count ? mom[i] : 0.0f;
         }
-        sq += (double)u * (double)u;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int64_t i = i0 + k * step;
+            if (mom && i < count) {
+                m[k] = fmaf(A.mu, m[k], u[k]);
+                mom[i] = m[k];
+                u[k] = A.nesterov ? fmaf(A.mu, m[k], u[k]) : m[k];
+            }
+            sq += (double)u[k] * (double)u[k];
+        }
     }
     sq = ns_block_sum(sq, part);
     if (threadIdx.x == 0) J.parts[me] = sq;
@@ -240,7 +255,7 @@ __global__ void __launch_bounds__(256) ns_normalise_kernel(const __grid_constant
 }
 
 // ------------------------------------------------------------------------------------------------ products
-enum NsPhase { kGram, kPolynomial, kUpdate, kLast };
+enum NsPhase { kGram, kPolynomial, kUpdate };
 
 constexpr int kNsThreads = 384;      // a warp that loads, one that issues products, two to fill up; eight that take the results
 
@@ -275,7 +290,7 @@ __device__ __forceinline__ void ns_move_piece(unsigned char *block, unsigned cha
         uint4 *far = (uint4 *)(block + (r & 127) * 128 + ((((c0 >> 3) & 7) + chunk) ^ (r & 7)) * 16);
         uint4 *near = (uint4 *)(piece + ns_piece_at(row, chunk));
         if (STORE) *far = *near;
-        else v[i] = *far;
+        else v[i] = __ldcg(far);
     }
     if (!STORE) {
 #pragma unroll
@@ -284,19 +299,19 @@ __device__ __forceinline__ void ns_move_piece(unsigned char *block, unsigned cha
 }
 
 // What a warp does with 32 rows (from r0, lane = row) x 32 columns (from c) of a result.
-template <int PHASE, int PARTS, typename T>
-__device__ __forceinline__ void ns_take_piece(const NsArgs &A, const NsJob &J, int from, int r0, int c, float (&v)[32], unsigned char *piece, int lane)
+template <int PARTS, typename T>
+__device__ __forceinline__ void ns_take_piece(const NsArgs &A, const NsJob &J, int kind, bool last, int from, int r0, int c, float (&v)[32],
+                                              unsigned char *piece, int lane)
 {
-    constexpr bool kSymmetric = PHASE == kGram || PHASE == kPolynomial;
-    const int cbs = kSymmetric ? ns_cb(J.m) : ns_cb(J.n);
+    const int cbs = kind == kUpdate ? ns_cb(J.n) : ns_cb(J.m);
     const int64_t block = ((int64_t)(r0 >> 7) * cbs + (c >> 6)) * (PARTS * kBlock);
-    if (PHASE == kGram) {
+    if (kind == kGram) {
 #pragma unroll
         for (int k = 0; k < 32; ++k) v[k] *= kScaleA / (kScaleX * kScaleX);
     } else {
         // b = cb a + ..., x' = ca x + ...
-        unsigned char *old = (PHASE == kPolynomial ? J.a : J.x[from]) + block;
-        const float f = PHASE == kPolynomial ? A.cb : A.ca, by = PHASE == kPolynomial ? A.cc / kScaleA : 1.0f / kScaleA;
+        unsigned char *old = (kind == kPolynomial ? J.a : J.x[from]) + block;
+        const float f = kind == kPolynomial ? A.cb : A.ca, by = kind == kPolynomial ? A.cc / kScaleA : 1.0f / kScaleA;
         __syncwarp();
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) ns_move_piece<false>(old + p * kBlock, piece + p * 2048, r0, c, lane);
@@ -321,7 +336,7 @@ __device__ __forceinline__ void ns_take_piece(const NsArgs &A, const NsJob &J, i
         }
     }
     __syncwarp();
-    if (PHASE == kLast) {
+    if (last) {
         // to the weight, 32 elements next to each other at a time: of a tall matrix, what the lanes hold of a column
         T *dst = (T *)J.dst;
         const bool tall = J.rows > J.cols;
@@ -331,23 +346,25 @@ __device__ __forceinline__ void ns_take_piece(const NsArgs &A, const NsJob &J, i
             for (int k = 0; k < 32; ++k) turned[lane * 33 + k] = v[k];
             __syncwarp();
         }
-        const int64_t step = J.cols, first = tall ? (int64_t)c * step + r0 + lane : (int64_t)r0 * step + c + lane;
+        const int64_t step = J.cols;
         const int many = min(32, tall ? J.n - c : J.m - r0);          // rows of the weight
         const bool mine = tall ? r0 + lane < J.m : c + lane < J.n;
+        T *at = dst + (tall ? (int64_t)c * step + r0 + lane : (int64_t)r0 * step + c + lane);
 #pragma unroll
         for (int k0 = 0; k0 < 32; k0 += 8) {
             float w[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) w[k] = J.mom && mine && k0 + k < many ? ns_in(dst[first + (k0 + k) * step]) : 0.0f;
+            for (int k = 0; k < 8; ++k) w[k] = J.mom && mine && k0 + k < many ? ns_in(at[k * step]) : 0.0f;
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 const float o = (tall ? v[k0 + k] : turned[(k0 + k) * 33 + lane]) * (1.0f / kScaleX);
-                if (mine && k0 + k < many) dst[first + (k0 + k) * step] = ns_out<T>(J.mom ? fmaf(J.keep, w[k], -J.step * o) : o);
+                if (mine && k0 + k < many) at[k * step] = ns_out<T>(J.mom ? fmaf(J.keep, w[k], -J.step * o) : o);
             }
+            at += 8 * step;
         }
         __syncwarp();
     } else {
-        unsigned char *to = (PHASE == kGram ? J.a : PHASE == kPolynomial ? J.b : J.x[from ^ 1]) + block;
+        unsigned char *to = (kind == kGram ? J.a : kind == kPolynomial ? J.b : J.x[from ^ 1]) + block;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             uint4 hi, lo;
@@ -364,30 +381,41 @@ __device__ __forceinline__ void ns_take_piece(const NsArgs &A, const NsJob &J, i
     }
 }
 
-// Persistent: a CTA (a pair of them) takes tiles of the result.  PHASE
-//   kGram        a = x x^T                  kPolynomial  b = cb a + cc a a
-//   kUpdate      x' = ca x + b x            kLast        the same, and the result goes to the weight
+// All steps in one launch: three phases each,
+//   kGram        a = x x^T
+//   kPolynomial  b = cb a + cc a a
+//   kUpdate      x' = ca x + b x; in the last step the result goes to the weight
+// with all CTAs resident (a cooperative launch) and waiting for one another between phases: the small matrices' products take a
+// few microseconds, as long as a launch and the way of its first loads.  In a phase a CTA (a pair of them) takes tiles of the result.
 // a and b are symmetric: their blocks below the diagonal are neither computed nor stored.  Where a product wants one as
 // rows, it takes the block across the diagonal as columns.
 //
-// With CG = 1 and a cluster of several CTAs, these share one tile: each sums over its part of the steps, they exchange the sums
-// through shared memory, and each takes some 32 x 32 pieces of the total, added up in the order of the ranks.
-template <int PHASE, int PARTS, int CG, typename T>
-__global__ void __launch_bounds__(kNsThreads, 1) ns_product_kernel(const __grid_constant__ NsArgs A, int from, int tiles, int *status)
+// With CG = 1 and few tiles, split[phase] CTAs of a cluster share a tile: each sums over its part of the steps of the summation
+// index, they exchange the sums through shared memory, and each takes some 32 x 32 pieces of the total, added up in the order
+// of the ranks.
+struct NsPlan {
+    int steps;
+    int tiles[3], split[3];          // by phase
+    unsigned *arrived;               // zero before the launch
+    int *status;
+};
+
+template <int PARTS, int CG, typename T>
+__global__ void __launch_bounds__(kNsThreads, 1) ns_steps_kernel(const __grid_constant__ NsArgs A, const __grid_constant__ NsPlan P)
 {
     using Tile = NsTile<PARTS, CG>;
     constexpr int S = Tile::kStages, TN = Tile::TN;
-    constexpr bool kSymmetric = PHASE == kGram || PHASE == kPolynomial;
     extern __shared__ unsigned char smem_raw[];
     unsigned char *smem = (unsigned char *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     // full: this CTA's loads are there; ready: the second CTA's are (at the first); empty: a stage has been read; done: a sum is
-    // complete; taken: it has been taken out
+    // complete; taken: it has been taken out; given: the sums of all that share a tile are there
     uint64_t *full = (uint64_t *)(smem + S * Tile::kStage), *ready = full + S, *empty = ready + S, *done = empty + S, *taken = done + 2;
-    uint32_t *base_at = (uint32_t *)(taken + 2);
+    uint64_t *given = taken + 2;
+    uint32_t *base_at = (uint32_t *)(given + 3);
     unsigned char *pieces = smem + S * Tile::kStage + 512;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rank = (int)cluster_rank(), ranks = (int)cluster_size();
-    const int split = CG == 1 ? ranks : 1, pair = CG == 2 ? rank : 0;
+    const int rank = (int)cluster_rank(), pair = CG == 2 ? rank : 0;
+    const bool clustered = cluster_size() > 1;
     if (warp == 1) tensor_alloc<CG>(base_at, 2 * TN);
     if (threadIdx.x == 0) {
         for (int i = 0; i < S; ++i) {
@@ -399,245 +427,292 @@ __global__ void __launch_bounds__(kNsThreads, 1) ns_product_kernel(const __grid_
             mbar_init(done + i, 1);
             mbar_init(taken + i, 8 * CG);
         }
+        for (int i = 0; i < 3; ++i) mbar_init(given + i, 8 * P.split[i]);
         mbar_init_fence();
     }
     tensor_fence_before();
     __syncthreads();
-    if (ranks > 1) cluster_wait_all();
+    if (clustered) cluster_wait_all();
     tensor_fence_after();
     const uint32_t acc = *base_at;
     bool fine = true;
-    const int tile0 = blockIdx.x / ranks, tile_step = gridDim.x / ranks;
 
-    // tile -> its job, its first row block and its first column block
-    auto locate = [&](int tile, const NsJob *&J, int &i, int &j) {
-        const int k = ns_find<kSymmetric ? 1 : 2>(A, tile);
-        J = &A.job[k];
-        int at = tile - J->first[kSymmetric ? 1 : 2];
-        const int rt = (ns_rb(J->m) + CG - 1) / CG;
-        if (kSymmetric) {
+    // a phase: which tiles this CTA takes, and its part of the summation index
+    struct Phase {
+        int kind, from, tile, step, tiles, split, rank;
+        bool last;
+    };
+    auto phase_of = [&](int ph) {
+        Phase p;
+        p.kind = ph % 3;
+        p.from = ph / 3 & 1;
+        p.last = ph + 1 == 3 * P.steps;
+        p.tiles = P.tiles[p.kind];
+        p.split = P.split[p.kind];
+        const int width = CG == 2 ? 2 : p.split;
+        p.tile = blockIdx.x / width;
+        p.step = gridDim.x / width;
+        p.rank = rank % p.split;
+        return p;
+    };
+    // tile -> its job, its first row block and its first column block, and this CTA's part of the summation index
+    struct Spot {
+        const NsJob *J;
+        int i, j, k0, k1;
+    };
+    auto locate = [&](const Phase &p, int tile) {
+        Spot o;
+        const bool symmetric = p.kind != kUpdate;
+        int n = 0;
+        while (n + 1 < A.jobs && A.job[n + 1].first[symmetric ? 1 : 2] <= tile) ++n;
+        o.J = &A.job[n];
+        int at = tile - o.J->first[symmetric ? 1 : 2];
+        const int rt = (ns_rb(o.J->m) + CG - 1) / CG;
+        if (symmetric) {
             // a row of tiles begins at the diagonal
-            for (i = 0; at >= rt - i; ++i) at -= rt - i;
-            j = i + at;
+            for (o.i = 0; at >= rt - o.i; ++o.i) at -= rt - o.i;
+            o.j = o.i + at;
         } else {
             // tiles that run side by side share columns of x
-            i = at % rt;
-            j = at / rt;
+            o.i = at % rt;
+            o.j = at / rt;
         }
-        i *= CG;
-        j *= CG;
+        o.i *= CG;
+        o.j *= CG;
+        const int steps = p.kind == kGram ? ns_cb(o.J->n) : ns_cb(o.J->m);
+        o.k0 = steps * p.rank / p.split;
+        o.k1 = steps * (p.rank + 1) / p.split;
+        return o;
     };
     // whether step k takes an operand from across the diagonal (of the two row blocks of a pair, which take it alike, one may be the
     // diagonal's own, which is the same either way)
-    auto left_turned = [&](int i, int k) { return PHASE != kGram && (k >> 1) < i + CG - 1; };
-    auto right_turned = [&](int j, int k) { return PHASE == kPolynomial ? (k >> 1) < j + CG - 1 : !kSymmetric; };
-    // this CTA's part of the steps
-    auto part = [&](const NsJob &J, int &k0, int &k1) {
-        const int steps = PHASE == kGram ? ns_cb(J.n) : ns_cb(J.m);
-        k0 = steps * rank / split * (CG == 1);
-        k1 = CG == 1 ? steps * (rank + 1) / split : steps;
-    };
+    auto left_turned = [&](int kind, int i, int k) { return kind != kGram && (k >> 1) < i + CG - 1; };
+    auto right_turned = [&](int kind, int j, int k) { return kind == kPolynomial ? (k >> 1) < j + CG - 1 : kind == kUpdate; };
 
     if (warp < 4) {
         // 128 threads give registers to the 256 that hold sums: 128 * 56 + 256 * 216 <= 384 * 168
         if constexpr (CG == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == 0 && lane == 0) {
-            int s = 0, phase = 0;
-            for (int tile = tile0; fine && tile < tiles; tile += tile_step) {
-                const NsJob *J;
-                int i, j, k0, k1;
-                locate(tile, J, i, j);
-                part(*J, k0, k1);
-                const int cbm = ns_cb(J->m), cbn = ns_cb(J->n);
-                const int cbl = PHASE == kGram ? cbn : cbm, cbr = PHASE == kPolynomial ? cbm : cbn;
-                const unsigned char *left = PHASE == kGram ? J->x[from] : PHASE == kPolynomial ? J->a : J->b;
-                const unsigned char *right = PHASE == kPolynomial ? J->a : J->x[from];
-                const int il = i + pair, jr = j + pair;        // this CTA's row block and column block; behind the last one, nothing
-                const bool has_left = il < ns_rb(J->m), has_right = jr < (kSymmetric ? ns_rb(J->m) : ns_rb(J->n));
-                const unsigned bytes = PARTS * kBlock * (has_left + has_right);
-                // 64 rows of two blocks of 64 columns: [part][column block]
-                auto columns = [&](unsigned char *to, const unsigned char *x, int cbs, int k, int block) {
-                    const unsigned char *row = x + ((int64_t)(k >> 1) * cbs + 2 * block) * (PARTS * kBlock) + (k & 1) * (kBlock / 2);
-                    for (int b = 0; b < 2; ++b)
-                        for (int p = 0; p < PARTS; ++p)
-                            bulk_load(to + p * kBlock + b * (kBlock / 2), row + (b * PARTS + p) * kBlock, kBlock / 2, full + s);
-                };
-                for (int k = k0; k < k1; ++k) {
-                    if (!mbar_wait_bounded(empty + s, phase ^ 1, kWaitLimit)) { fine = false; break; }
-                    unsigned char *to = smem + s * Tile::kStage;
-                    mbar_expect_tx(full + s, bytes);
-                    if (has_left) {
-                        if (left_turned(i, k)) columns(to, left, cbl, k, il);
-                        else bulk_load(to, left + ((int64_t)il * cbl + k) * (PARTS * kBlock), PARTS * kBlock, full + s);
+            int s = 0, turn = 0;
+            for (int ph = 0; fine && ph < 3 * P.steps; ++ph) {
+                if (ph > 0) {
+                    if (!grid_wait_bounded(P.arrived, ph * gridDim.x, kWaitLimit)) { fine = false; break; }
+                    fence_async_all();
+                }
+                const Phase p = phase_of(ph);
+                for (int tile = p.tile; fine && tile < p.tiles; tile += p.step) {
+                    const Spot o = locate(p, tile);
+                    const NsJob &J = *o.J;
+                    const int cbm = ns_cb(J.m), cbn = ns_cb(J.n), rb = ns_rb(J.m);
+                    const int cbl = p.kind == kGram ? cbn : cbm, cbr = p.kind == kPolynomial ? cbm : cbn;
+                    const unsigned char *left = p.kind == kGram ? J.x[p.from] : p.kind == kPolynomial ? J.a : J.b;
+                    const unsigned char *right = p.kind == kPolynomial ? J.a : J.x[p.from];
+                    const int il = o.i + pair, jr = o.j + pair;        // this CTA's row block and column block; behind the last one, nothing
+                    const bool has_left = il < rb, has_right = jr < (p.kind != kUpdate ? rb : ns_rb(J.n));
+                    const unsigned bytes = PARTS * kBlock * (has_left + has_right);
+                    // 64 rows of two blocks of 64 columns: [part][column block]
+                    auto columns = [&](unsigned char *to, const unsigned char *x, int cbs, int k, int block) {
+                        const unsigned char *row = x + ((int64_t)(k >> 1) * cbs + 2 * block) * (PARTS * kBlock) + (k & 1) * (kBlock / 2);
+                        for (int b = 0; b < 2; ++b)
+                            for (int q = 0; q < PARTS; ++q)
+                                bulk_load(to + q * kBlock + b * (kBlock / 2), row + (b * PARTS + q) * kBlock, kBlock / 2, full + s);
+                    };
+                    for (int k = o.k0; k < o.k1; ++k) {
+                        if (!mbar_wait_bounded(empty + s, turn ^ 1, kWaitLimit)) { fine = false; break; }
+                        unsigned char *to = smem + s * Tile::kStage;
+                        mbar_expect_tx(full + s, bytes);
+                        if (has_left) {
+                            if (left_turned(p.kind, o.i, k)) columns(to, left, cbl, k, il);
+                            else bulk_load(to, left + ((int64_t)il * cbl + k) * (PARTS * kBlock), PARTS * kBlock, full + s);
+                        }
+                        to += Tile::kA;
+                        if (has_right) {
+                            if (right_turned(p.kind, o.j, k)) columns(to, right, cbr, k, jr);
+                            else bulk_load(to, right + ((int64_t)jr * cbr + k) * (PARTS * kBlock), PARTS * kBlock, full + s);
+                        }
+                        if (++s == S) { s = 0; turn ^= 1; }
                     }
-                    to += Tile::kA;
-                    if (has_right) {
-                        if (right_turned(j, k)) columns(to, right, cbr, k, jr);
-                        else bulk_load(to, right + ((int64_t)jr * cbr + k) * (PARTS * kBlock), PARTS * kBlock, full + s);
-                    }
-                    if (++s == S) { s = 0; phase ^= 1; }
                 }
             }
             // every stage's last copy has been read before the CTA leaves
             for (int k = 0; k < S; ++k) {
-                if (!mbar_wait_bounded(empty + s, phase ^ 1, kWaitLimit)) fine = false;
-                if (++s == S) { s = 0; phase ^= 1; }
+                if (!mbar_wait_bounded(empty + s, turn ^ 1, kWaitLimit)) fine = false;
+                if (++s == S) { s = 0; turn ^= 1; }
             }
         } else if (warp == 1 && lane == 0 && pair == 0) {
-            int s = 0, phase = 0, slot = 0, turn = 0;
-            for (int tile = tile0; fine && tile < tiles; tile += tile_step) {
-                const NsJob *J;
-                int i, j, k0, k1;
-                locate(tile, J, i, j);
-                part(*J, k0, k1);
-                for (int k = k0; k < k1; ++k) {
-                    const bool first = (k - k0) % Tile::kGroup == 0;
-                    if (first && !mbar_wait_bounded(taken + slot, turn ^ 1, kWaitLimit)) { fine = false; break; }
-                    if (!mbar_wait_bounded(full + s, phase, kWaitLimit)) { fine = false; break; }
-                    if (CG == 2 && !mbar_wait_bounded(ready + s, phase, kWaitLimit)) { fine = false; break; }
-                    tensor_fence_after();
-                    const unsigned a0 = smem_u32(smem + s * Tile::kStage), b0 = a0 + Tile::kA;
-                    const bool lt = left_turned(i, k), rt = right_turned(j, k);
-                    const uint32_t shape = product_shape(128 * CG, TN, lt, rt), d = acc + slot * TN;
-                    const auto operand = [&](unsigned base, bool turned, int p, int q) {
-                        return turned ? desc_columns(base + p * kBlock + q * 2048, kBlock / 2) : desc_rows(base + p * kBlock + q * 32);
-                    };
-                    // the small products first: what they lose to the sum's size is less while it is small
-                    if (PARTS == 2) {
+            int s = 0, turn = 0, slot = 0, again = 0;
+            for (int ph = 0; fine && ph < 3 * P.steps; ++ph) {
+                const Phase p = phase_of(ph);
+                for (int tile = p.tile; fine && tile < p.tiles; tile += p.step) {
+                    const Spot o = locate(p, tile);
+                    for (int k = o.k0; k < o.k1; ++k) {
+                        const bool first = (k - o.k0) % Tile::kGroup == 0;
+                        if (first && !mbar_wait_bounded(taken + slot, again ^ 1, kWaitLimit)) { fine = false; break; }
+                        if (!mbar_wait_bounded(full + s, turn, kWaitLimit)) { fine = false; break; }
+                        if (CG == 2 && !mbar_wait_bounded(ready + s, turn, kWaitLimit)) { fine = false; break; }
+                        tensor_fence_after();
+                        const unsigned a0 = smem_u32(smem + s * Tile::kStage), b0 = a0 + Tile::kA;
+                        const bool lt = left_turned(p.kind, o.i, k), rt = right_turned(p.kind, o.j, k);
+                        const uint32_t shape = product_shape(128 * CG, TN, lt, rt), d = acc + slot * TN;
+                        const auto operand = [&](unsigned base, bool turned, int q, int step) {
+                            return turned ? desc_columns(base + q * kBlock + step * 2048, kBlock / 2) : desc_rows(base + q * kBlock + step * 32);
+                        };
+                        // the small products first: what they lose to the sum's size is less while it is small
+                        if (PARTS == 2) {
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            product<CG>(d, operand(a0, lt, 0, q), operand(b0, rt, 1, q), shape, !first || q > 0);
-                            product<CG>(d, operand(a0, lt, 1, q), operand(b0, rt, 0, q), shape, true);
+                            for (int q = 0; q < 4; ++q) {
+                                product<CG>(d, operand(a0, lt, 0, q), operand(b0, rt, 1, q), shape, !first || q > 0);
+                                product<CG>(d, operand(a0, lt, 1, q), operand(b0, rt, 0, q), shape, true);
+                            }
                         }
-                    }
 #pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        product<CG>(d, operand(a0, lt, 0, q), operand(b0, rt, 0, q), shape, PARTS == 2 || !first || q > 0);
-                    product_commit<CG>(empty + s);
-                    if (++s == S) { s = 0; phase ^= 1; }
-                    if ((k + 1 - k0) % Tile::kGroup == 0 || k + 1 == k1) {
-                        product_commit<CG>(done + slot);
-                        if ((slot ^= 1) == 0) turn ^= 1;
+                        for (int q = 0; q < 4; ++q)
+                            product<CG>(d, operand(a0, lt, 0, q), operand(b0, rt, 0, q), shape, PARTS == 2 || !first || q > 0);
+                        product_commit<CG>(empty + s);
+                        if (++s == S) { s = 0; turn ^= 1; }
+                        if ((k + 1 - o.k0) % Tile::kGroup == 0 || k + 1 == o.k1) {
+                            product_commit<CG>(done + slot);
+                            if ((slot ^= 1) == 0) again ^= 1;
+                        }
                     }
                 }
             }
         } else if (CG == 2 && warp == 1 && lane == 0) {
             // the second CTA tells the first what it has loaded
-            int s = 0, phase = 0;
-            for (int tile = tile0; fine && tile < tiles; tile += tile_step) {
-                const NsJob *J;
-                int i, j, k0, k1;
-                locate(tile, J, i, j);
-                part(*J, k0, k1);
-                for (int k = k0; k < k1; ++k) {
-                    if (!mbar_wait_bounded(full + s, phase, kWaitLimit)) { fine = false; break; }
-                    mbar_arrive_at(ready + s, 0);
-                    if (++s == S) { s = 0; phase ^= 1; }
+            int s = 0, turn = 0;
+            for (int ph = 0; fine && ph < 3 * P.steps; ++ph) {
+                const Phase p = phase_of(ph);
+                for (int tile = p.tile; fine && tile < p.tiles; tile += p.step) {
+                    const Spot o = locate(p, tile);
+                    for (int k = o.k0; k < o.k1; ++k) {
+                        if (!mbar_wait_bounded(full + s, turn, kWaitLimit)) { fine = false; break; }
+                        mbar_arrive_at(ready + s, 0);
+                        if (++s == S) { s = 0; turn ^= 1; }
+                    }
                 }
             }
         }
         __syncwarp();
-        if (CG == 1 && split > 1) cluster_wait_all();
     } else {
         if constexpr (CG == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-        int slot = 0, turn = 0;
+        int slot = 0, again = 0;
         const int w = warp - 4, quarter = warp & 3, half = w >> 2;
         unsigned char *piece = pieces + w * Tile::kPiece;
-        for (int tile = tile0; fine && tile < tiles; tile += tile_step) {
-            const NsJob *J;
-            int i, j, k0, k1;
-            locate(tile, J, i, j);
-            part(*J, k0, k1);
-            const int r0 = (i + pair) * 128 + quarter * 32;
-            const int groups = (k1 - k0 + Tile::kGroup - 1) / Tile::kGroup;
-            const int il = i + pair, c0 = half * (TN / 2), jl = j + (c0 >> 7);      // this warp's columns of the tile; its blocks
-            const bool mine = il < ns_rb(J->m) && jl < (kSymmetric ? ns_rb(J->m) : ns_rb(J->n)) && !(kSymmetric && jl < il);
-            const uint32_t at = acc + ((uint32_t)(quarter * 32) << 16) + c0;
-            float sum[PARTS == 2 ? TN / 64 : 1][32];
-            // the exchange of a shared tile: four columns of all rows after one another
-            auto give = [&](const float (&v)[32], int u) {
-                float4 *to = (float4 *)smem + ((c0 + u * 32) / 4) * 128 + quarter * 32 + lane;
+        for (int ph = 0; fine && ph < 3 * P.steps; ++ph) {
+            const Phase p = phase_of(ph);
+            for (int tile = p.tile; fine && tile < p.tiles; tile += p.step) {
+                const Spot o = locate(p, tile);
+                const NsJob &J = *o.J;
+                const int groups = (o.k1 - o.k0 + Tile::kGroup - 1) / Tile::kGroup, rb = ns_rb(J.m);
+                const int il = o.i + pair, c0 = half * (TN / 2), jl = o.j + (c0 >> 7);      // this warp's columns of the tile; its blocks
+                const bool mine = il < rb && jl < (p.kind != kUpdate ? rb : ns_rb(J.n)) && !(p.kind != kUpdate && jl < il);
+                const int r0 = il * 128 + quarter * 32, c = o.j * 128 + c0;
+                const uint32_t at = acc + ((uint32_t)(quarter * 32) << 16) + c0;
+                float sum[PARTS == 2 ? TN / 64 : 1][32];
+                if constexpr (PARTS == 2) {
 #pragma unroll
-                for (int k = 0; k < 8; ++k) to[k * 128] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
-            };
-            if constexpr (PARTS == 2) {
+                    for (int u = 0; u < TN / 64; ++u)
 #pragma unroll
-                for (int u = 0; u < TN / 64; ++u)
+                        for (int k = 0; k < 32; ++k) sum[u][k] = 0.0f;
+                }
+                // a whole piece: to the others that share the tile (four columns of all rows after one another), or to its end
+                auto pass_on = [&](float (&v)[32], int u) {
+                    if (CG == 1 && p.split > 1) {
+                        float4 *to = (float4 *)smem + ((c0 + u * 32) / 4) * 128 + quarter * 32 + lane;
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) sum[u][k] = 0.0f;
-            }
-            for (int g = 0; g < groups; ++g) {
-                if (!__all_sync(0xffffffffu, mbar_wait_bounded(done + slot, turn, kWaitLimit))) { fine = false; break; }
-                tensor_fence_after();
-                if (mine) {
-#pragma unroll
-                    for (int u = 0; u < TN / 64; ++u) {
-                        float v[32];
-                        tensor_read(v, at + slot * TN + u * 32);
+                        for (int k = 0; k < 8; ++k) to[k * 128] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+                    } else {
+                        ns_take_piece<PARTS, T>(A, J, p.kind, p.last, p.from, r0, c + u * 32, v, piece, lane);
+                    }
+                };
+                for (int g = 0; g < groups; ++g) {
+                    if (!__all_sync(0xffffffffu, mbar_wait_bounded(done + slot, again, kWaitLimit))) { fine = false; break; }
+                    tensor_fence_after();
+                    if (mine) {
                         if constexpr (PARTS == 2) {
 #pragma unroll
-                            for (int k = 0; k < 32; ++k) sum[u][k] += v[k];
-                        } else if (split > 1) {
-                            give(v, u);
+                            for (int u = 0; u < TN / 64; ++u) {
+                                float v[32];
+                                tensor_read(v, at + slot * TN + u * 32);
+#pragma unroll
+                                for (int k = 0; k < 32; ++k) sum[u][k] += v[k];
+                            }
                         } else {
-                            ns_take_piece<PHASE, PARTS, T>(A, *J, from, il * 128 + quarter * 32, j * 128 + c0 + u * 32, v, piece, lane);
+#pragma unroll 1
+                            for (int u = 0; u < TN / 64; ++u) {
+                                float v[32];
+                                tensor_read(v, at + slot * TN + u * 32);
+                                pass_on(v, u);
+                            }
                         }
                     }
+                    tensor_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (CG == 2) mbar_arrive_at(taken + slot, 0);
+                        else mbar_arrive(taken + slot);
+                    }
+                    if ((slot ^= 1) == 0) again ^= 1;
                 }
-                tensor_fence_before();
-                __syncwarp();
-                if (lane == 0) {
-                    if (CG == 2) mbar_arrive_at(taken + slot, 0);
-                    else mbar_arrive(taken + slot);
-                }
-                if ((slot ^= 1) == 0) turn ^= 1;
-            }
-            if (PARTS == 1 && groups == 0) {              // more CTAs than steps
-                const float v[32] = {};
-#pragma unroll
-                for (int u = 0; u < TN / 64; ++u) give(v, u);
-            }
-            if constexpr (PARTS == 2) {
-                if (fine && mine) {
-#pragma unroll
+                if (fine && mine && (PARTS == 2 || groups == 0)) {        // no groups: more CTAs than steps
+#pragma unroll 1
                     for (int u = 0; u < TN / 64; ++u) {
-                        if (split > 1) give(sum[u], u);
-                        else ns_take_piece<PHASE, PARTS, T>(A, *J, from, r0, j * 128 + c0 + u * 32, sum[u], piece, lane);
+                        float v[32];
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) {
+                            v[k] = 0.0f;
+                            if constexpr (PARTS == 2) {
+#pragma unroll
+                                for (int e = 0; e < TN / 64; ++e) v[k] = u == e ? sum[e][k] : v[k];
+                            }
+                        }
+                        pass_on(v, u);
                     }
                 }
             }
-        }
-        if (CG == 1 && split > 1) {
-            __syncwarp();
-            cluster_wait_all();
-            if (tile0 < tiles) {
-                const NsJob *J;
-                int i, j;
-                locate(tile0, J, i, j);
-                for (int u = w * split + rank; u < 16; u += 8 * split) {
-                    const int quarter = u & 3, c = u >> 2;
-                    const float4 *at = (const float4 *)smem + c * 8 * 128 + quarter * 32 + lane;
-                    float v[32] = {};
-                    for (int r = 0; r < split; ++r) {
+            if (CG == 1 && p.split > 1 && fine) {
+                __syncwarp();
+                if (lane < p.split) mbar_release_at(given + p.kind, rank - p.rank + lane);
+                if (p.tile < p.tiles) {
+                    fine = __all_sync(0xffffffffu, mbar_acquire_bounded(given + p.kind, ph / 3 & 1, kWaitLimit));
+                    const Spot o = locate(p, p.tile);
+#pragma unroll 1
+                    for (int u = w * p.split + p.rank; u < 16; u += 8 * p.split) {
+                        const int part = u & 3, c = u >> 2;
+                        const float4 *at = (const float4 *)smem + c * 8 * 128 + part * 32 + lane;
+                        float v[32] = {};
+                        for (int r = 0; r < p.split; ++r) {
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            const float4 x = read_at(at + k * 128, r);
-                            v[4 * k] += x.x;
-                            v[4 * k + 1] += x.y;
-                            v[4 * k + 2] += x.z;
-                            v[4 * k + 3] += x.w;
+                            for (int k = 0; k < 8; ++k) {
+                                const float4 x = read_at(at + k * 128, rank - p.rank + r);
+                                v[4 * k] += x.x;
+                                v[4 * k + 1] += x.y;
+                                v[4 * k + 2] += x.z;
+                                v[4 * k + 3] += x.w;
+                            }
                         }
+                        ns_take_piece<PARTS, T>(A, *o.J, p.kind, p.last, p.from, o.i * 128 + part * 32, o.j * 128 + c * 32, v, piece, lane);
                     }
-                    ns_take_piece<PHASE, PARTS, T>(A, *J, from, i * 128 + quarter * 32, j * 128 + c * 32, v, piece, lane);
+                }
+            }
+            if (!p.last) {
+                // what this CTA has written is there for the others' loads
+                fence_async_all();
+                __threadfence();
+                fine = all_agree(1, 256, fine);            // a warp that gave up takes the others along
+                if (threadIdx.x == 128) {
+                    // a CTA without a tile in this phase has waited for nothing yet: its arrival must not count for the phase before
+                    if (!grid_wait_bounded(P.arrived, ph * gridDim.x, kWaitLimit)) fine = false;
+                    grid_arrive(P.arrived);
                 }
             }
         }
         __syncwarp();
     }
-    if (!fine) atomicExch(status, kStatusNsTimeout);
+    if (!fine) atomicExch(P.status, kStatusNsTimeout);
     tensor_fence_before();
     __syncthreads();
-    if (ranks > 1) cluster_wait_all();               // no CTA leaves while another reads its memory or arrives at its barriers
+    if (clustered) cluster_wait_all();               // no CTA leaves while another reads its memory or arrives at its barriers
     if (warp == 1) {
         tensor_fence_after();
         tensor_free<CG>(acc, 2 * TN);
@@ -647,14 +722,14 @@ __global__ void __launch_bounds__(kNsThreads, 1) ns_product_kernel(const __grid_
 static size_t ns_job_bytes(int64_t m, int64_t n, int dtype)
 {
     const int64_t parts = dtype == SLAYER_B200_BF16 ? 1 : 2, rb = ns_rb((int)m), cbn = ns_cb((int)n);
-    return kNormParts * 8 + (size_t)(2 * rb * cbn + 4 * rb * rb) * (size_t)(parts * kBlock);
+    return kNormParts * 8 + 256 + (size_t)(2 * rb * cbn + 4 * rb * rb) * (size_t)(parts * kBlock);
 }
 
 static void ns_take(NsJob &J, int parts, unsigned char *&at)
 {
     const int64_t rb = ns_rb(J.m), x = rb * ns_cb(J.n) * parts * kBlock, a = 2 * rb * rb * parts * kBlock;
     J.parts = (double *)at;
-    at += kNormParts * 8;
+    at += kNormParts * 8 + 256;                  // and a count
     J.x[0] = at;
     J.x[1] = J.x[0] + x;
     J.a = J.x[1] + x;
@@ -662,71 +737,110 @@ static void ns_take(NsJob &J, int parts, unsigned char *&at)
     at = J.b + a;
 }
 
-// CTAs that share a tile where there are too few tiles for the SMs, each with two steps at least
-static int ns_split(int tiles, int steps)
+// How many clusters of `ranks` CTAs of a kernel the device holds at once (remembered).
+static int ns_resident(const void *kern, int ranks, size_t smem)
 {
-    int split = 1;
-    while (split < 8 && tiles * split * 2 <= sm_count() && steps >= split * 4) split *= 2;
-    return split;
-}
-
-template <int PHASE, int PARTS, int CG, typename T>
-static int ns_product(const NsArgs &A, int from, int tiles, int split, int *status, cudaStream_t st)
-{
-    auto kern = ns_product_kernel<PHASE, PARTS, CG, T>;
-    constexpr size_t smem = NsTile<PARTS, CG>::kSmem;
-    int rc = reserve_dynamic_smem((const void *)kern, smem);
-    if (rc) return rc;
-    const int ranks = CG == 2 ? 2 : split, most = sm_count() / ranks;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((tiles < most ? tiles : most) * ranks);
-    cfg.blockDim = dim3(kNsThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = ranks;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, kern, A, from, tiles, status);
-    return check_launch("Newton-Schulz product launch");
+    static std::mutex mu;
+    static std::map<std::tuple<const void *, int, int>, int> known;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) dev = 0;
+    std::lock_guard<std::mutex> lock(mu);
+    int &n = known[std::make_tuple(kern, ranks, dev)];
+    if (n == 0) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(ranks);
+        cfg.blockDim = dim3(kNsThreads);
+        cfg.dynamicSmemBytes = smem;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = ranks;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) n = 0;
+    }
+    return n;
 }
 
 template <typename T, int PARTS, int CG>
 static int ns_run(NsArgs &A, int steps, cudaStream_t st)
 {
-    int *status = device_status_word();
-    if (!status) {
+    NsPlan P = {};
+    P.steps = steps;
+    P.status = device_status_word();
+    if (!P.status) {
         set_error("Newton-Schulz products: no status word on this device");
         return SLAYER_B200_ECUDA;
     }
-    int blocks = 0, small = 0, large = 0, m = 0, n = 0;
+    P.arrived = (unsigned *)(A.job[0].parts + kNormParts);
+    int blocks = 0, m = 0, n = 0;
     for (int j = 0; j < A.jobs; ++j) {
         NsJob &J = A.job[j];
         const int64_t want = ceil_div((int64_t)ns_rb(J.m) * ns_cb(J.n) * 128 * 64, 4096);
         J.norm_parts = (int)(want < kNormParts ? want : kNormParts);
         J.first[0] = blocks;
-        J.first[1] = small;
-        J.first[2] = large;
+        J.first[1] = P.tiles[kGram];
+        J.first[2] = P.tiles[kUpdate];
         blocks += J.norm_parts;
         const int rt = (ns_rb(J.m) + CG - 1) / CG;
-        small += rt * (rt + 1) / 2;
-        large += rt * ((ns_rb(J.n) + CG - 1) / CG);
+        P.tiles[kGram] += rt * (rt + 1) / 2;
+        P.tiles[kUpdate] += rt * ((ns_rb(J.n) + CG - 1) / CG);
         m = J.m > m ? J.m : m;
         n = J.n > n ? J.n : n;
     }
-    ns_momentum_kernel<T><<<blocks, 256, 0, st>>>(A);
-    ns_normalise_kernel<T, PARTS><<<blocks, 256, 0, st>>>(A);
-    int rc = check_launch("Newton-Schulz normalisation launch"), from = 0;
-    const int split_n = ns_split(small, ns_cb(n)), split_m = ns_split(small, ns_cb(m)), split_x = ns_split(large, ns_cb(m));
-    for (int s = 0; s < steps && !rc; ++s, from ^= 1) {
-        rc = ns_product<kGram, PARTS, CG, float>(A, from, small, split_n, status, st);
-        if (!rc) rc = ns_product<kPolynomial, PARTS, CG, float>(A, from, small, split_m, status, st);
-        if (!rc) rc = s + 1 < steps ? ns_product<kUpdate, PARTS, CG, float>(A, from, large, split_x, status, st)
-                                    : ns_product<kLast, PARTS, CG, T>(A, from, large, split_x, status, st);
+    P.tiles[kPolynomial] = P.tiles[kGram];
+
+    auto kern = ns_steps_kernel<PARTS, CG, T>;
+    constexpr size_t smem = NsTile<PARTS, CG>::kSmem;
+    int rc = reserve_dynamic_smem((const void *)kern, smem);
+    if (rc) return rc;
+    // CTAs that share a tile where there are too few tiles for the SMs, each with two steps of 64 at least
+    const int index[3] = {ns_cb(n), ns_cb(m), ns_cb(m)};
+    int ranks = CG, resident = 0;
+    for (int most = CG == 1 ? 8 : 1;; most = ranks) {
+        ranks = CG;
+        const int sms = resident ? resident : sm_count();
+        for (int k = 0; k < 3; ++k) {
+            P.split[k] = 1;
+            while (P.split[k] < most && P.tiles[k] * P.split[k] * 2 <= sms && index[k] >= P.split[k] * 4) P.split[k] *= 2;
+            if (CG == 1) ranks = P.split[k] > ranks ? P.split[k] : ranks;
+        }
+        const int held = ns_resident((const void *)kern, ranks, smem) * ranks;
+        if (held <= 0) {
+            set_error("Newton-Schulz products: the device holds no cluster of %d CTAs", ranks);
+            return SLAYER_B200_EUNSUPPORTED;
+        }
+        const bool settled = resident == held;
+        resident = held;
+        if (settled || CG == 2) break;
     }
-    return rc;
+    int grid = 0;
+    for (int k = 0; k < 3; ++k) {
+        const int64_t want = (int64_t)P.tiles[k] * (CG == 2 ? 2 : P.split[k]);
+        grid = want < resident ? ((int)want > grid ? (int)want : grid) : resident;
+        if (grid == resident) break;
+    }
+    grid = (int)ceil_div(grid, ranks) * ranks;
+
+    ns_momentum_kernel<T><<<blocks, 256, 0, st>>>(A, P.arrived);
+    ns_normalise_kernel<T, PARTS><<<blocks, 256, 0, st>>>(A);
+    rc = check_launch("Newton-Schulz normalisation launch");
+    if (rc) return rc;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(kNsThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ranks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeCooperative;
+    attr[1].val.cooperative = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    cudaLaunchKernelEx(&cfg, kern, A, P);
+    return check_launch("Newton-Schulz steps launch");
 }
 
 // Whether the steps keep singular values from [0, 1] and the polynomial's factors in the range that the products can hold: the

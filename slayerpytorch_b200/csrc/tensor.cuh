@@ -122,6 +122,59 @@ __device__ __forceinline__ void mbar_arrive_at(uint64_t *bar, unsigned rank)
         ::"r"(smem_u32(bar)), "r"(rank) : "memory");
 }
 
+// the same, and what other threads of the cluster have done before they arrived is seen
+__device__ __forceinline__ void mbar_release_at(uint64_t *bar, unsigned rank)
+{
+    asm volatile(
+        "{\n\t.reg .b32 far;\n\t"
+        "mapa.shared::cluster.u32 far, %0, %1;\n\t"
+        "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [far];\n\t}"
+        ::"r"(smem_u32(bar)), "r"(rank) : "memory");
+}
+
+__device__ __forceinline__ bool mbar_acquire_bounded(uint64_t *bar, unsigned parity, int limit)
+{
+    for (int i = 0; i < limit; ++i) {
+        unsigned ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+        if (ok) return true;
+    }
+    return false;
+}
+
+// Between plain accesses and asynchronous copies of the same global or shared memory, in either order.
+__device__ __forceinline__ void fence_async_all() { asm volatile("fence.proxy.async;" ::: "memory"); }
+
+// a barrier of `threads` threads of the CTA, which says whether all of them came with `value`
+__device__ __forceinline__ bool all_agree(int barrier, int threads, bool value)
+{
+    unsigned all;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 q, %3, 0;\n\t"
+        "barrier.cta.red.and.pred p, %1, %2, q;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(all) : "r"(barrier), "r"(threads), "r"((unsigned)value) : "memory");
+    return all != 0;
+}
+
+// A count that the CTAs of a grid which is resident as a whole arrive at.
+__device__ __forceinline__ void grid_arrive(unsigned *count) { asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(count) : "memory"); }
+
+__device__ __forceinline__ bool grid_wait_bounded(const unsigned *count, unsigned target, int limit)
+{
+    for (int i = 0; i < limit; ++i) {
+        unsigned now;
+        asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(now) : "l"(count) : "memory");
+        if (now >= target) return true;
+    }
+    return false;
+}
+
 __device__ __forceinline__ unsigned cluster_rank()
 {
     unsigned r;
