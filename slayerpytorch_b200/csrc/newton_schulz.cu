@@ -719,6 +719,364 @@ __global__ void __launch_bounds__(kNsThreads, 1) ns_steps_kernel(const __grid_co
     }
 }
 
+// ------------------------------------------------------------------------------------------- small matrices
+// Up to 128 rows: a matrix stays in the shared memory of a cluster from its gradient to its weight's update, in one launch.  Each
+// CTA has some column blocks of 64 of X and all of A.  A step: every CTA's part of X X^T, added up across the cluster (each CTA
+// adds up its share and gives it to all); A A by every CTA for itself; B X of its own columns, in place.  What bounds it is latency:
+// a step is three products of a microsecond and the way through tensor memory, registers and shared memory between them.
+// A block here has only as many rows as the matrix (a multiple of 16); the tensor core reads 128, and what lies behind gives
+// rows of the result that nobody looks at.
+constexpr int kSmallThreads = 512;
+constexpr int kSmallScratch = 16 * 32 * 17 * 4;          // a 32 x 16 piece of each warp
+
+struct NsSmall {
+    int rows, per, block, x, ab, scratch, total;         // rows and bytes
+    bool fits;
+};
+
+// where things lie in the shared memory of a CTA with `per` column blocks of a matrix of m rows
+static __host__ __device__ __forceinline__ NsSmall ns_small(int m, int per, int parts)
+{
+    NsSmall s;
+    s.rows = (m + 15) / 16 * 16;
+    s.per = per;
+    s.block = parts * s.rows * 128;
+    s.x = per * s.block;
+    // A, later B: as blocks; before that, fp32 sums for the exchange.  The last operand's 128 rows reach 16 KB behind its start.
+    const int abs = (s.rows + 63) / 64 * s.block, sums = s.rows * s.rows * 4, reach = abs - s.rows * 128 + kBlock;
+    s.ab = abs > sums ? abs : sums;
+    s.ab = s.ab > reach ? s.ab : reach;
+    // results on their way to the weight: over B where all columns fit tensor memory at once, so that B is not needed any more
+    s.scratch = s.rows > 64 ? s.x : s.x + s.ab;
+    s.total = s.rows > 64 ? s.x + (s.ab > kSmallScratch ? s.ab : kSmallScratch) : s.scratch + kSmallScratch;
+    s.fits = s.total <= 226 * 1024 - 1024 && (s.rows <= 64 || per <= 8);
+    return s;
+}
+
+// u of eight columns from c on of row r (0 outside the matrix); first: the momentum is brought up to date on the way
+template <typename T>
+__device__ __forceinline__ void ns_load_u(const NsArgs &A, const NsJob &J, int r, int c, bool first, float (&v)[8])
+{
+    const T *g = (const T *)J.src;
+    const bool tall = J.rows > J.cols, wide = !tall && J.cols % 8 == 0 && ns_wide(g) && ns_wide(J.mom);
+    const int64_t at0 = tall ? (int64_t)c * J.cols + r : (int64_t)r * J.cols + c, step = tall ? J.cols : 1;
+    float m[8];
+    if (wide) {
+        if (c < J.n) {
+            ns_load8(v, g + at0);
+            if (J.mom) ns_load8(m, J.mom + at0);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = m[k] = 0.0f;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            v[k] = c + k < J.n ? ns_in(g[at0 + k * step]) : 0.0f;
+            m[k] = J.mom && c + k < J.n ? J.mom[at0 + k * step] : 0.0f;
+        }
+    }
+    if (J.mom) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (first) {
+                m[k] = fmaf(A.mu, m[k], v[k]);
+                if (c + k < J.n) J.mom[at0 + k * step] = m[k];
+            }
+            v[k] = A.nesterov ? fmaf(A.mu, m[k], v[k]) : m[k];
+        }
+    }
+}
+
+// sixteen columns of a row, as two chunks of a block
+template <int PARTS>
+__device__ __forceinline__ void ns_put16(unsigned char *row, int part_bytes, int chunk, int r, const float (&v)[16])
+{
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        uint4 hi, lo;
+        ns_split<PARTS>(v[8 * k], v[8 * k + 1], hi.x, lo.x);
+        ns_split<PARTS>(v[8 * k + 2], v[8 * k + 3], hi.y, lo.y);
+        ns_split<PARTS>(v[8 * k + 4], v[8 * k + 5], hi.z, lo.z);
+        ns_split<PARTS>(v[8 * k + 6], v[8 * k + 7], hi.w, lo.w);
+        unsigned char *at = row + (((chunk + k) ^ r) & 7) * 16;
+        *(uint4 *)at = hi;
+        if (PARTS == 2) *(uint4 *)(at + part_bytes) = lo;
+    }
+}
+
+// v <- f old + by v for the same
+template <int PARTS>
+__device__ __forceinline__ void ns_add16(const unsigned char *row, int part_bytes, int chunk, int r, float f, float by, float (&v)[16])
+{
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const unsigned char *at = row + (((chunk + k) ^ r) & 7) * 16;
+        const uint4 hi = *(const uint4 *)at;
+        uint4 lo = make_uint4(0, 0, 0, 0);
+        if (PARTS == 2) lo = *(const uint4 *)(at + part_bytes);
+        const uint32_t hs[4] = {hi.x, hi.y, hi.z, hi.w}, ls[4] = {lo.x, lo.y, lo.z, lo.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float2 o = __half22float2(*reinterpret_cast<const __half2 *>(&hs[e]));
+            if (PARTS == 2) {
+                const float2 l = __half22float2(*reinterpret_cast<const __half2 *>(&ls[e]));
+                o.x += l.x;
+                o.y += l.y;
+            }
+            v[8 * k + 2 * e] = fmaf(f, o.x, by * v[8 * k + 2 * e]);
+            v[8 * k + 2 * e + 1] = fmaf(f, o.y, by * v[8 * k + 2 * e + 1]);
+        }
+    }
+}
+
+template <typename T, int PARTS>
+__global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid_constant__ NsArgs A, int steps, int *status)
+{
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char *smem = (unsigned char *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    __shared__ uint64_t bar;
+    __shared__ uint32_t base_at;
+    __shared__ double part[32], square;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int C = (int)cluster_size(), rank = (int)cluster_rank();
+    const NsJob &J = A.job[blockIdx.x / C];
+    const int blocks = (J.n + 63) / 64;
+    const NsSmall L = ns_small(J.m, (blocks + C - 1) / C, PARTS);
+    const int b0 = min(rank * L.per, blocks), nb = min(L.per, blocks - b0), R = L.rows, side = R * 128;
+    unsigned char *x = smem, *ab = smem + L.x;
+    if (warp == 0) tensor_alloc<1>(&base_at, 512);
+    if (tid == 0) {
+        mbar_init(&bar, 1);
+        mbar_init_fence();
+    }
+
+    // momentum and norm
+    const int chunks = nb * 8;
+    const bool tall = J.rows > J.cols;
+    double sq = 0.0;
+    for (int i = tid; i < J.m * chunks; i += kSmallThreads) {
+        float v[8];
+        ns_load_u<T>(A, J, tall ? i % J.m : i / chunks, b0 * 64 + (tall ? i / J.m : i % chunks) * 8, true, v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sq += (double)v[k] * (double)v[k];
+    }
+    sq = ns_block_sum(sq, part);
+    if (tid == 0) square = sq;
+    tensor_fence_before();
+    __syncthreads();
+    tensor_fence_after();
+    const uint32_t acc = base_at;
+    if (C > 1) {
+        cluster_wait_all();
+        sq = 0.0;
+        for (int r = 0; r < C; ++r) sq += read_double_at(&square, r);
+    }
+    const float inv = (float)((double)kScaleX / (sqrt(sq) + (double)A.eps));
+    for (int i = tid; i < R * chunks; i += kSmallThreads) {
+        const int r = tall ? i % R : i / chunks, ch = tall ? i / R : i % chunks;
+        float v[8] = {};
+        if (r < J.m) ns_load_u<T>(A, J, r, b0 * 64 + ch * 8, false, v);
+        uint4 hi, lo;
+        ns_split<PARTS>(v[0] * inv, v[1] * inv, hi.x, lo.x);
+        ns_split<PARTS>(v[2] * inv, v[3] * inv, hi.y, lo.y);
+        ns_split<PARTS>(v[4] * inv, v[5] * inv, hi.z, lo.z);
+        ns_split<PARTS>(v[6] * inv, v[7] * inv, hi.w, lo.w);
+        unsigned char *at = x + (ch >> 3) * L.block + r * 128 + ((ch ^ r) & 7) * 16;
+        *(uint4 *)at = hi;
+        if (PARTS == 2) *(uint4 *)(at + side) = lo;
+    }
+
+    // this warp's rows of a result, and its first sixteen columns of each 64
+    const int r = (warp & 3) * 32 + lane, first = (warp >> 2) * 16;
+    const bool mine = (warp & 3) * 32 < R, row_there = r < R;
+    const uint32_t at = acc + ((uint32_t)((warp & 3) * 32) << 16);
+    bool fine = true;
+    int turn = 0;
+    // what has been written to shared memory is there for the products; what is in tensor memory has been read
+    const auto ready = [&] {
+        fence_async_all();
+        tensor_fence_before();
+        __syncthreads();
+        tensor_fence_after();
+    };
+    const auto made = [&] {
+        if (!mbar_wait_bounded(&bar, turn, kWaitLimit)) fine = false;
+        turn ^= 1;
+        __syncwarp();
+        tensor_fence_after();
+    };
+    const unsigned xs = smem_u32(x), abs = smem_u32(ab);
+    // the products of one step of 16: the small ones first, what they lose to the sum's size is less while it is small
+    const auto multiply = [&](uint32_t d, auto left, auto right, uint32_t shape, int count, bool add) {
+        if (PARTS == 2)
+            for (int q = 0; q < count; ++q) {
+                product<1>(d, left(0, q), right(1, q), shape, add || q > 0);
+                product<1>(d, left(1, q), right(0, q), shape, true);
+            }
+        for (int q = 0; q < count; ++q) product<1>(d, left(0, q), right(0, q), shape, PARTS == 2 || add || q > 0);
+    };
+    // sums of at most a few blocks each, added up in registers (see kGroup)
+    const int sums = PARTS == 2 ? max(1, min(512 / R, (nb + 1) / 2)) : 1;
+
+    for (int s = 0; s < steps; ++s) {
+        const bool last = s + 1 == steps;
+        ready();
+        if (tid == 0) {
+            for (int g = 0; g < sums; ++g)
+                for (int b = nb * g / sums; b < nb * (g + 1) / sums; ++b) {
+                    const auto rows = [&](int p, int q) { return desc_rows(xs + b * L.block + p * side + q * 32); };
+                    multiply(acc + g * R, rows, rows, product_shape(128, R, false, false), 4, b > nb * g / sums);
+                }
+            product_commit<1>(&bar);
+        }
+        made();
+        if (mine)
+            for (int c = first; c < R; c += 64) {
+                float v[16], t[16];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) v[k] = 0.0f;
+                __syncwarp();
+                if (nb > 0)
+                    for (int g = 0; g < sums; ++g) {
+                        tensor_read(t, at + g * R + c);
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) v[k] += t[k];
+                    }
+                if (row_there && C == 1) {
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) v[k] *= kScaleA / (kScaleX * kScaleX);
+                    ns_put16<PARTS>(ab + (c >> 6) * L.block + r * 128, side, (c >> 3) & 7, r, v);
+                } else if (row_there) {
+                    // four columns of all rows after one another
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) ((float4 *)ab)[(c / 4 + k) * R + r] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+                }
+            }
+        if (C > 1) {
+            __syncwarp();
+            cluster_wait_all();
+            const int all = R * R / 4, e0 = all * rank / C, e1 = all * (rank + 1) / C;
+            float4 total[4];                             // 128 * 128 / 4 / 2 / 512
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int e = e0 + tid + k * kSmallThreads;
+                total[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (e < e1)
+                    for (int o = 0; o < C; ++o) {
+                        const float4 y = read_at((const float4 *)ab + e, o);
+                        total[k].x += y.x;
+                        total[k].y += y.y;
+                        total[k].z += y.z;
+                        total[k].w += y.w;
+                    }
+            }
+            __syncwarp();
+            cluster_wait_all();                          // all sums have been read: A takes their place
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int e = e0 + tid + k * kSmallThreads, row = e % R, c = e / R * 4;
+                if (e < e1) {
+                    const float f = kScaleA / (kScaleX * kScaleX);
+                    uint32_t h0, h1, l0, l1;
+                    ns_split<PARTS>(total[k].x * f, total[k].y * f, h0, l0);
+                    ns_split<PARTS>(total[k].z * f, total[k].w * f, h1, l1);
+                    unsigned char *to = ab + (c >> 6) * L.block + row * 128 + ((((c >> 3) ^ row) & 7) * 16) + (c & 4) * 2;
+                    for (int o = 0; o < C; ++o) {
+                        write_at(to, o, h0, h1);
+                        if (PARTS == 2) write_at(to + side, o, l0, l1);
+                    }
+                }
+            }
+            fence_async_all();
+            __syncwarp();
+            cluster_wait_all();
+        }
+        ready();
+        if (tid == 0) {
+            const auto rows = [&](int p, int q) { return desc_rows(abs + (q >> 2) * L.block + p * side + (q & 3) * 32); };
+            multiply(acc, rows, rows, product_shape(128, R, false, false), R / 16, false);
+            product_commit<1>(&bar);
+        }
+        made();
+        if (mine)
+            for (int c = first; c < R; c += 64) {
+                float v[16];
+                __syncwarp();
+                tensor_read(v, at + c);
+                if (row_there) {
+                    unsigned char *row = ab + (c >> 6) * L.block + r * 128;
+                    ns_add16<PARTS>(row, side, (c >> 3) & 7, r, A.cb, A.cc / kScaleA, v);
+                    ns_put16<PARTS>(row, side, (c >> 3) & 7, r, v);
+                }
+            }
+        // up to 512 columns of x at a time
+        for (int n0 = 0; n0 < nb; n0 += 8) {
+            const int n1 = min(n0 + 8, nb);
+            ready();
+            if (tid == 0) {
+                for (int b = n0; b < n1; b += 4) {
+                    const auto rows = [&](int p, int q) { return desc_rows(abs + (q >> 2) * L.block + p * side + (q & 3) * 32); };
+                    const auto columns = [&](int p, int q) { return desc_columns(xs + b * L.block + p * side + q * 2048, L.block); };
+                    multiply(acc + (b - n0) * 64, rows, columns, product_shape(128, min(4, n1 - b) * 64, false, true), R / 16, false);
+                }
+                product_commit<1>(&bar);
+            }
+            made();
+            if (last) __syncthreads();                   // B may be written over
+            if (mine)
+                for (int c = first; c < (n1 - n0) * 64; c += 64) {
+                    float v[16];
+                    __syncwarp();
+                    tensor_read(v, at + c);
+                    const int column = n0 * 64 + c;
+                    unsigned char *row = x + (column >> 6) * L.block + r * 128;
+                    if (row_there) ns_add16<PARTS>(row, side, (c >> 3) & 7, r, A.ca, 1.0f / kScaleA, v);
+                    if (!last) {
+                        if (row_there) ns_put16<PARTS>(row, side, (c >> 3) & 7, r, v);
+                        continue;
+                    }
+                    // to the weight: of a tall matrix what the lanes hold of a column, else sixteen elements of two rows at a time
+                    T *dst = (T *)J.dst;
+                    const int c0 = b0 * 64 + column;
+                    float *turned = (float *)(smem + L.scratch) + warp * (32 * 17);
+                    if (!tall) {
+                        __syncwarp();
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) turned[lane * 17 + k] = v[k];
+                        __syncwarp();
+                    }
+                    const int row0 = (warp & 3) * 32;
+                    const auto place = [&](int k, int64_t &to) {
+                        const int rr = tall ? r : row0 + 2 * k + (lane >> 4), cc = tall ? c0 + k : c0 + (lane & 15);
+                        to = tall ? (int64_t)cc * J.cols + rr : (int64_t)rr * J.cols + cc;
+                        return rr < J.m && cc < J.n;
+                    };
+                    float w[16];
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        int64_t to;
+                        w[k] = place(k, to) && J.mom ? ns_in(dst[to]) : 0.0f;
+                    }
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        int64_t to;
+                        const float o = (tall ? v[k] : turned[(2 * k + (lane >> 4)) * 17 + (lane & 15)]) * (1.0f / kScaleX);
+                        if (place(k, to)) dst[to] = ns_out<T>(J.mom ? fmaf(J.keep, w[k], -J.step * o) : o);
+                    }
+                }
+        }
+    }
+    if (!fine) atomicExch(status, kStatusNsTimeout);
+    tensor_fence_before();
+    __syncthreads();
+    if (C > 1) cluster_wait_all();
+    if (warp == 0) {
+        tensor_fence_after();
+        tensor_free<1>(acc, 512);
+    }
+}
+
 static size_t ns_job_bytes(int64_t m, int64_t n, int dtype)
 {
     const int64_t parts = dtype == SLAYER_B200_BF16 ? 1 : 2, rb = ns_rb((int)m), cbn = ns_cb((int)n);
@@ -882,9 +1240,61 @@ static int ns_shape(const char *what, int64_t rows, int64_t cols)
     return SLAYER_B200_OK;
 }
 
+// CTAs for each of the small matrices of a launch: about four column blocks each, fewer where there are many matrices; 0: a
+// matrix does not fit
+static int ns_small_cluster(const NsArgs &A, int parts)
+{
+    int C = 1;
+    for (; C <= 8; C *= 2) {
+        bool fits = true, roomy = true;
+        for (int j = 0; j < A.jobs && fits; ++j) {
+            const int per = ((A.job[j].n + 63) / 64 + C - 1) / C;
+            fits = A.job[j].m <= 128 && ns_small(A.job[j].m, per, parts).fits;
+            roomy = roomy && per <= 4;
+        }
+        if (fits && (roomy || C == 8 || A.jobs * C * 2 > sm_count())) return C;
+    }
+    return 0;
+}
+
+template <typename T, int PARTS>
+static int ns_run_small(const NsArgs &A, int C, int steps, cudaStream_t st)
+{
+    int *status = device_status_word();
+    if (!status) {
+        set_error("Newton-Schulz products: no status word on this device");
+        return SLAYER_B200_ECUDA;
+    }
+    // one CTA per SM, since each takes all of its tensor memory
+    size_t smem = 120 * 1024;
+    for (int j = 0; j < A.jobs; ++j) {
+        const size_t want = 1024 + ns_small(A.job[j].m, ((A.job[j].n + 63) / 64 + C - 1) / C, PARTS).total;
+        smem = want > smem ? want : smem;
+    }
+    auto kern = ns_small_kernel<T, PARTS>;
+    int rc = reserve_dynamic_smem((const void *)kern, smem);
+    if (rc) return rc;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(A.jobs * C);
+    cfg.blockDim = dim3(kSmallThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = C;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, kern, A, steps, status);
+    return check_launch("Newton-Schulz launch for small matrices");
+}
+
 template <typename T, int PARTS>
 static int ns_tiled(NsArgs &A, int steps, cudaStream_t st)
 {
+    const int C = ns_small_cluster(A, PARTS);
+    if (C) return ns_run_small<T, PARTS>(A, C, steps, st);
+
     // tiles of two CTAs where there are enough of them
     int64_t tiles = 0;
     for (int j = 0; j < A.jobs; ++j) tiles += (int64_t)((ns_rb(A.job[j].m) + 1) / 2) * ((ns_rb(A.job[j].n) + 1) / 2);

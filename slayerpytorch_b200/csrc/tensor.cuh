@@ -103,6 +103,21 @@ __device__ __forceinline__ void tensor_read(float (&v)[32], uint32_t addr)
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+// the same, 16 columns
+__device__ __forceinline__ void tensor_read(float (&v)[16], uint32_t addr)
+{
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
 // contiguous copy of global memory into shared memory; both 16-byte aligned, bytes a multiple of 16
 __device__ __forceinline__ void bulk_load(void *dst, const void *src, unsigned bytes, uint64_t *bar)
 {
@@ -205,6 +220,26 @@ __device__ __forceinline__ float4 read_at(const void *p, unsigned rank)
         "mapa.shared::cluster.u32 far, %4, %5;\n\t"
         "ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [far];\n\t}"
         : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(smem_u32(p)), "r"(rank) : "memory");
+    return v;
+}
+
+__device__ __forceinline__ void write_at(void *p, unsigned rank, uint32_t a, uint32_t b)
+{
+    asm volatile(
+        "{\n\t.reg .b32 far;\n\t"
+        "mapa.shared::cluster.u32 far, %0, %1;\n\t"
+        "st.shared::cluster.v2.b32 [far], {%2, %3};\n\t}"
+        ::"r"(smem_u32(p)), "r"(rank), "r"(a), "r"(b) : "memory");
+}
+
+__device__ __forceinline__ double read_double_at(const void *p, unsigned rank)
+{
+    double v;
+    asm volatile(
+        "{\n\t.reg .b32 far;\n\t"
+        "mapa.shared::cluster.u32 far, %1, %2;\n\t"
+        "ld.shared::cluster.f64 %0, [far];\n\t}"
+        : "=d"(v) : "r"(smem_u32(p)), "r"(rank) : "memory");
     return v;
 }
 

@@ -56,7 +56,7 @@ def gradient(shape, seed, dtype=torch.float32):
 
 
 SIZES = [(1, 1), (1, 7), (5, 1), (2, 3), (16, 50), (32, 144), (64, 288), (10, 4096), (127, 129), (128, 128), (129, 127), (200, 256), (257, 300),
-         (130, 1000), (700, 65), (512, 600), (300, 2100), (1030, 520)]
+         (130, 1000), (700, 65), (128, 2500), (128, 2600), (100, 5000), (64, 6200), (8100, 24), (17, 8192), (33, 65), (113, 300), (512, 600), (300, 2100), (1030, 520)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
