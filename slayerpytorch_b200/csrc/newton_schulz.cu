@@ -280,41 +280,49 @@ struct NsTile {
 // without two lanes meeting in a bank.
 __device__ __forceinline__ int ns_piece_at(int row, int chunk) { return row * 64 + ((chunk ^ (row >> 1)) & 3) * 16; }
 
-template <bool STORE>
-__device__ __forceinline__ void ns_move_piece(unsigned char *block, unsigned char *piece, int r0, int c0, int lane)
+__device__ __forceinline__ uint4 *ns_piece_line(unsigned char *block, int r0, int c0, int lane, int i)
 {
-    uint4 v[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int row = i * 8 + (lane >> 2), chunk = lane & 3, r = r0 + row;
-        uint4 *far = (uint4 *)(block + (r & 127) * 128 + ((((c0 >> 3) & 7) + chunk) ^ (r & 7)) * 16);
-        uint4 *near = (uint4 *)(piece + ns_piece_at(row, chunk));
-        if (STORE) *far = *near;
-        else v[i] = __ldcg(far);
-    }
-    if (!STORE) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) *(uint4 *)(piece + ns_piece_at(i * 8 + (lane >> 2), lane & 3)) = v[i];
-    }
+    const int r = r0 + i * 8 + (lane >> 2);
+    return (uint4 *)(block + (r & 127) * 128 + ((((c0 >> 3) & 7) + (lane & 3)) ^ (r & 7)) * 16);
 }
+
+// What the result is made of besides the product: of b, a; of x', x.
+template <int PARTS>
+struct NsOld {
+    uint4 v[PARTS][4];
+    // requested early, put into the piece when it is wanted
+    __device__ __forceinline__ void request(const NsJob &J, int kind, int from, int r0, int c, int lane)
+    {
+        if (kind == kGram) return;
+        const int cbs = kind == kUpdate ? ns_cb(J.n) : ns_cb(J.m);
+        unsigned char *block = (kind == kPolynomial ? J.a : J.x[from]) + ((int64_t)(r0 >> 7) * cbs + (c >> 6)) * (PARTS * kBlock);
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[p][i] = __ldcg(ns_piece_line(block + p * kBlock, r0, c, lane, i));
+    }
+    __device__ __forceinline__ void put(unsigned char *piece, int lane) const
+    {
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) *(uint4 *)(piece + p * 2048 + ns_piece_at(i * 8 + (lane >> 2), lane & 3)) = v[p][i];
+    }
+};
 
 // What a warp does with 32 rows (from r0, lane = row) x 32 columns (from c) of a result.
 template <int PARTS, typename T>
 __device__ __forceinline__ void ns_take_piece(const NsArgs &A, const NsJob &J, int kind, bool last, int from, int r0, int c, float (&v)[32],
-                                              unsigned char *piece, int lane)
+                                              unsigned char *piece, int lane, const NsOld<PARTS> &old)
 {
-    const int cbs = kind == kUpdate ? ns_cb(J.n) : ns_cb(J.m);
-    const int64_t block = ((int64_t)(r0 >> 7) * cbs + (c >> 6)) * (PARTS * kBlock);
     if (kind == kGram) {
 #pragma unroll
         for (int k = 0; k < 32; ++k) v[k] *= kScaleA / (kScaleX * kScaleX);
     } else {
         // b = cb a + ..., x' = ca x + ...
-        unsigned char *old = (kind == kPolynomial ? J.a : J.x[from]) + block;
         const float f = kind == kPolynomial ? A.cb : A.ca, by = kind == kPolynomial ? A.cc / kScaleA : 1.0f / kScaleA;
         __syncwarp();
-#pragma unroll
-        for (int p = 0; p < PARTS; ++p) ns_move_piece<false>(old + p * kBlock, piece + p * 2048, r0, c, lane);
+        old.put(piece, lane);
         __syncwarp();
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -364,7 +372,8 @@ __device__ __forceinline__ void ns_take_piece(const NsArgs &A, const NsJob &J, i
         }
         __syncwarp();
     } else {
-        unsigned char *to = (kind == kGram ? J.a : kind == kPolynomial ? J.b : J.x[from ^ 1]) + block;
+        const int cbs = kind == kUpdate ? ns_cb(J.n) : ns_cb(J.m);
+        unsigned char *to = (kind == kGram ? J.a : kind == kPolynomial ? J.b : J.x[from ^ 1]) + ((int64_t)(r0 >> 7) * cbs + (c >> 6)) * (PARTS * kBlock);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             uint4 hi, lo;
@@ -377,7 +386,10 @@ __device__ __forceinline__ void ns_take_piece(const NsArgs &A, const NsJob &J, i
         }
         __syncwarp();
 #pragma unroll
-        for (int p = 0; p < PARTS; ++p) ns_move_piece<true>(to + p * kBlock, piece + p * 2048, r0, c, lane);
+        for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *ns_piece_line(to + p * kBlock, r0, c, lane, i) = *(const uint4 *)(piece + p * 2048 + ns_piece_at(i * 8 + (lane >> 2), lane & 3));
     }
 }
 
@@ -491,7 +503,7 @@ __global__ void __launch_bounds__(kNsThreads, 1) ns_steps_kernel(const __grid_co
 
     if (warp < 4) {
         // 128 threads give registers to the 256 that hold sums: 128 * 56 + 256 * 216 <= 384 * 168
-        if constexpr (CG == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == 0 && lane == 0) {
             int s = 0, turn = 0;
             for (int ph = 0; fine && ph < 3 * P.steps; ++ph) {
@@ -554,20 +566,19 @@ __global__ void __launch_bounds__(kNsThreads, 1) ns_steps_kernel(const __grid_co
                         const unsigned a0 = smem_u32(smem + s * Tile::kStage), b0 = a0 + Tile::kA;
                         const bool lt = left_turned(p.kind, o.i, k), rt = right_turned(p.kind, o.j, k);
                         const uint32_t shape = product_shape(128 * CG, TN, lt, rt), d = acc + slot * TN;
-                        const auto operand = [&](unsigned base, bool turned, int q, int step) {
-                            return turned ? desc_columns(base + q * kBlock + step * 2048, kBlock / 2) : desc_rows(base + q * kBlock + step * 32);
-                        };
+                        // descriptors count 16 bytes: 16 columns are 2 further, 16 rows 128, the other part a block
+                        const uint64_t l = lt ? desc_columns(a0, kBlock / 2) : desc_rows(a0), r = rt ? desc_columns(b0, kBlock / 2) : desc_rows(b0);
+                        const unsigned dl = lt ? 128 : 2, dr = rt ? 128 : 2, other = kBlock / 16;
                         // the small products first: what they lose to the sum's size is less while it is small
                         if (PARTS == 2) {
 #pragma unroll
                             for (int q = 0; q < 4; ++q) {
-                                product<CG>(d, operand(a0, lt, 0, q), operand(b0, rt, 1, q), shape, !first || q > 0);
-                                product<CG>(d, operand(a0, lt, 1, q), operand(b0, rt, 0, q), shape, true);
+                                product<CG>(d, l + q * dl, r + q * dr + other, shape, !first || q > 0);
+                                product<CG>(d, l + q * dl + other, r + q * dr, shape, true);
                             }
                         }
 #pragma unroll
-                        for (int q = 0; q < 4; ++q)
-                            product<CG>(d, operand(a0, lt, 0, q), operand(b0, rt, 0, q), shape, PARTS == 2 || !first || q > 0);
+                        for (int q = 0; q < 4; ++q) product<CG>(d, l + q * dl, r + q * dr, shape, PARTS == 2 || !first || q > 0);
                         product_commit<CG>(empty + s);
                         if (++s == S) { s = 0; turn ^= 1; }
                         if ((k + 1 - o.k0) % Tile::kGroup == 0 || k + 1 == o.k1) {
@@ -594,12 +605,17 @@ __global__ void __launch_bounds__(kNsThreads, 1) ns_steps_kernel(const __grid_co
         }
         __syncwarp();
     } else {
-        if constexpr (CG == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         int slot = 0, again = 0;
         const int w = warp - 4, quarter = warp & 3, half = w >> 2;
         unsigned char *piece = pieces + w * Tile::kPiece;
         for (int ph = 0; fine && ph < 3 * P.steps; ++ph) {
             const Phase p = phase_of(ph);
+            if (ph > 0) {
+                // what the phase before has left; and a CTA without a tile must not arrive before its time
+                if (lane == 0) fine = grid_wait_bounded(P.arrived, ph * gridDim.x, kWaitLimit);
+                fine = __all_sync(0xffffffffu, fine);
+            }
             for (int tile = p.tile; fine && tile < p.tiles; tile += p.step) {
                 const Spot o = locate(p, tile);
                 const NsJob &J = *o.J;
@@ -615,6 +631,8 @@ __global__ void __launch_bounds__(kNsThreads, 1) ns_steps_kernel(const __grid_co
 #pragma unroll
                         for (int k = 0; k < 32; ++k) sum[u][k] = 0.0f;
                 }
+                NsOld<PARTS> old;
+                if (mine && !(CG == 1 && p.split > 1)) old.request(J, p.kind, p.from, r0, c, lane);
                 // a whole piece: to the others that share the tile (four columns of all rows after one another), or to its end
                 auto pass_on = [&](float (&v)[32], int u) {
                     if (CG == 1 && p.split > 1) {
@@ -622,7 +640,8 @@ __global__ void __launch_bounds__(kNsThreads, 1) ns_steps_kernel(const __grid_co
 #pragma unroll
                         for (int k = 0; k < 8; ++k) to[k * 128] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
                     } else {
-                        ns_take_piece<PARTS, T>(A, J, p.kind, p.last, p.from, r0, c + u * 32, v, piece, lane);
+                        if (u > 0) old.request(J, p.kind, p.from, r0, c + u * 32, lane);
+                        ns_take_piece<PARTS, T>(A, J, p.kind, p.last, p.from, r0, c + u * 32, v, piece, lane, old);
                     }
                 };
                 for (int g = 0; g < groups; ++g) {
@@ -670,41 +689,57 @@ __global__ void __launch_bounds__(kNsThreads, 1) ns_steps_kernel(const __grid_co
                     }
                 }
             }
-            if (CG == 1 && p.split > 1 && fine) {
+            if (CG == 1 && p.split > 1) {
                 __syncwarp();
                 if (lane < p.split) mbar_release_at(given + p.kind, rank - p.rank + lane);
                 if (p.tile < p.tiles) {
-                    fine = __all_sync(0xffffffffu, mbar_acquire_bounded(given + p.kind, ph / 3 & 1, kWaitLimit));
                     const Spot o = locate(p, p.tile);
-#pragma unroll 1
-                    for (int u = w * p.split + p.rank; u < 16; u += 8 * p.split) {
-                        const int part = u & 3, c = u >> 2;
-                        const float4 *at = (const float4 *)smem + c * 8 * 128 + part * 32 + lane;
-                        float v[32] = {};
-                        for (int r = 0; r < p.split; ++r) {
+                    // this CTA's pieces of 32 x 32: rank, rank + split, ...; warp w takes the w-th of them
+                    const int piece_of = w * p.split + p.rank, part = piece_of & 3, c = piece_of >> 2;
+                    NsOld<PARTS> old;
+                    if (piece_of < 16) old.request(*o.J, p.kind, p.from, o.i * 128 + part * 32, o.j * 128 + c * 32, lane);
+                    fine = __all_sync(0xffffffffu, mbar_acquire_bounded(given + p.kind, ph / 3 & 1, kWaitLimit)) && fine;
+                    // all threads add up the ranks' sums: 16 columns of four of a row, over 16 / split pieces
+                    float4 *const own = (float4 *)(smem + 128 * 128 * 4);      // behind what the others read
+                    const int many = 16 / p.split * 256;                       // float4 of this CTA's pieces
+                    for (int e0 = 0; e0 < many; e0 += 256) {
+                        const int e = e0 + threadIdx.x - 128, q = (e >> 8) * p.split + p.rank;
+                        const float4 *at = (const float4 *)smem + ((q >> 2) * 8 + ((e >> 5) & 7)) * 128 + (q & 3) * 32 + (e & 31);
+                        float4 x[8];
 #pragma unroll
-                            for (int k = 0; k < 8; ++k) {
-                                const float4 x = read_at(at + k * 128, rank - p.rank + r);
-                                v[4 * k] += x.x;
-                                v[4 * k + 1] += x.y;
-                                v[4 * k + 2] += x.z;
-                                v[4 * k + 3] += x.w;
+                        for (int r = 0; r < 8; ++r)
+                            if (r < p.split) x[r] = read_at(at, rank - p.rank + r);
+                        float4 total = x[0];
+#pragma unroll
+                        for (int r = 1; r < 8; ++r)
+                            if (r < p.split) {
+                                total.x += x[r].x;
+                                total.y += x[r].y;
+                                total.z += x[r].z;
+                                total.w += x[r].w;
                             }
+                        own[e] = total;
+                    }
+                    fine = all_agree(2, 256, fine);
+                    if (piece_of < 16) {
+                        float v[32];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const float4 x = own[w * 256 + k * 32 + lane];
+                            v[4 * k] = x.x;
+                            v[4 * k + 1] = x.y;
+                            v[4 * k + 2] = x.z;
+                            v[4 * k + 3] = x.w;
                         }
-                        ns_take_piece<PARTS, T>(A, *o.J, p.kind, p.last, p.from, o.i * 128 + part * 32, o.j * 128 + c * 32, v, piece, lane);
+                        ns_take_piece<PARTS, T>(A, *o.J, p.kind, p.last, p.from, o.i * 128 + part * 32, o.j * 128 + c * 32, v, piece, lane, old);
                     }
                 }
             }
             if (!p.last) {
                 // what this CTA has written is there for the others' loads
                 fence_async_all();
-                __threadfence();
                 fine = all_agree(1, 256, fine);            // a warp that gave up takes the others along
-                if (threadIdx.x == 128) {
-                    // a CTA without a tile in this phase has waited for nothing yet: its arrival must not count for the phase before
-                    if (!grid_wait_bounded(P.arrived, ph * gridDim.x, kWaitLimit)) fine = false;
-                    grid_arrive(P.arrived);
-                }
+                if (threadIdx.x == 128) grid_arrive(P.arrived);
             }
         }
         __syncwarp();
@@ -895,7 +930,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
     int turn = 0;
     // what has been written to shared memory is there for the products; what is in tensor memory has been read
     const auto ready = [&] {
-        fence_async_all();
+        fence_proxy_async();
         tensor_fence_before();
         __syncthreads();
         tensor_fence_after();
@@ -907,14 +942,21 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
         tensor_fence_after();
     };
     const unsigned xs = smem_u32(x), abs = smem_u32(ab);
-    // the products of one step of 16: the small ones first, what they lose to the sum's size is less while it is small
-    const auto multiply = [&](uint32_t d, auto left, auto right, uint32_t shape, int count, bool add) {
-        if (PARTS == 2)
-            for (int q = 0; q < count; ++q) {
-                product<1>(d, left(0, q), right(1, q), shape, add || q > 0);
-                product<1>(d, left(1, q), right(0, q), shape, true);
-            }
-        for (int q = 0; q < count; ++q) product<1>(d, left(0, q), right(0, q), shape, PARTS == 2 || add || q > 0);
+    // up to four steps of 16 of the summation index, descriptors dl and dr apart: the small products first, what they lose to the
+    // sum's size is less while it is small
+    const unsigned other = side / 16;
+    const auto multiply = [&](uint32_t d, uint64_t left, unsigned dl, uint64_t right, unsigned dr, uint32_t shape, int count, bool add) {
+        if (PARTS == 2) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (q < count) {
+                    product<1>(d, left + q * dl, right + q * dr + other, shape, add || q > 0);
+                    product<1>(d, left + q * dl + other, right + q * dr, shape, true);
+                }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            if (q < count) product<1>(d, left + q * dl, right + q * dr, shape, PARTS == 2 || add || q > 0);
     };
     // sums of at most a few blocks each, added up in registers (see kGroup)
     const int sums = PARTS == 2 ? max(1, min(512 / R, (nb + 1) / 2)) : 1;
@@ -925,8 +967,8 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
         if (tid == 0) {
             for (int g = 0; g < sums; ++g)
                 for (int b = nb * g / sums; b < nb * (g + 1) / sums; ++b) {
-                    const auto rows = [&](int p, int q) { return desc_rows(xs + b * L.block + p * side + q * 32); };
-                    multiply(acc + g * R, rows, rows, product_shape(128, R, false, false), 4, b > nb * g / sums);
+                    const uint64_t rows = desc_rows(xs + b * L.block);
+                    multiply(acc + g * R, rows, 2, rows, 2, product_shape(128, R, false, false), 4, b > nb * g / sums);
                 }
             product_commit<1>(&bar);
         }
@@ -962,14 +1004,20 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
             for (int k = 0; k < 4; ++k) {
                 const int e = e0 + tid + k * kSmallThreads;
                 total[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (e < e1)
-                    for (int o = 0; o < C; ++o) {
-                        const float4 y = read_at((const float4 *)ab + e, o);
-                        total[k].x += y.x;
-                        total[k].y += y.y;
-                        total[k].z += y.z;
-                        total[k].w += y.w;
-                    }
+                if (e < e1) {
+                    float4 y[8];
+#pragma unroll
+                    for (int o = 0; o < 8; ++o)
+                        if (o < C) y[o] = read_at((const float4 *)ab + e, o);
+#pragma unroll
+                    for (int o = 0; o < 8; ++o)
+                        if (o < C) {
+                            total[k].x += y[o].x;
+                            total[k].y += y[o].y;
+                            total[k].z += y[o].z;
+                            total[k].w += y[o].w;
+                        }
+                }
             }
             __syncwarp();
             cluster_wait_all();                          // all sums have been read: A takes their place
@@ -994,8 +1042,10 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
         }
         ready();
         if (tid == 0) {
-            const auto rows = [&](int p, int q) { return desc_rows(abs + (q >> 2) * L.block + p * side + (q & 3) * 32); };
-            multiply(acc, rows, rows, product_shape(128, R, false, false), R / 16, false);
+            for (int k = 0; k < R; k += 64) {
+                const uint64_t rows = desc_rows(abs + (k >> 6) * L.block);
+                multiply(acc, rows, 2, rows, 2, product_shape(128, R, false, false), (R - k) / 16, k > 0);
+            }
             product_commit<1>(&bar);
         }
         made();
@@ -1015,11 +1065,10 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
             const int n1 = min(n0 + 8, nb);
             ready();
             if (tid == 0) {
-                for (int b = n0; b < n1; b += 4) {
-                    const auto rows = [&](int p, int q) { return desc_rows(abs + (q >> 2) * L.block + p * side + (q & 3) * 32); };
-                    const auto columns = [&](int p, int q) { return desc_columns(xs + b * L.block + p * side + q * 2048, L.block); };
-                    multiply(acc + (b - n0) * 64, rows, columns, product_shape(128, min(4, n1 - b) * 64, false, true), R / 16, false);
-                }
+                for (int b = n0; b < n1; b += 4)
+                    for (int k = 0; k < R; k += 64)
+                        multiply(acc + (b - n0) * 64, desc_rows(abs + (k >> 6) * L.block), 2, desc_columns(xs + b * L.block + k * 128, L.block), 128,
+                                 product_shape(128, min(4, n1 - b) * 64, false, true), (R - k) / 16, k > 0);
                 product_commit<1>(&bar);
             }
             made();
