@@ -1,9 +1,10 @@
-// Python module `slayerCuda`, second part: the operators behind the losses on logits (logProb, policyLoss, preferenceLoss,
-// logitGrad), and the orthogonalised updates (orthogonalize, muonStep).  They take float32, bfloat16 and float16 logits, matrices
+// Python module `slayerCuda`, second part: the losses of rows of logits (actionLogProb, policyLoss, preferenceLoss) as autograd
+// functions - a step of a small network is bound by the host, and these are half as long there as their Python form - and the orthogonalised updates (orthogonalize, muonStep).  They take float32, bfloat16 and float16 logits, matrices
 // and weights; everything that belongs to a row, and the momenta, are float32.
 #include "bindings_common.h"
 
 #include <cuda_runtime_api.h>
+#include <math.h>
 
 using namespace sb200py;
 
@@ -59,102 +60,261 @@ int64_t capture_id(torch::Tensor like)
     return status == cudaStreamCaptureStatusActive ? (int64_t)id : 0;
 }
 
-// (logp [rows], stats [rows, 2])
-std::vector<torch::Tensor> logProbCuda(torch::Tensor logits, torch::Tensor action, c10::optional<torch::Tensor> mask, float scale)
+using torch::autograd::AutogradContext;
+using torch::autograd::Variable;
+using torch::autograd::variable_list;
+
+// ---- arguments: logits [..., V], what belongs to a row of the shape in front of V
+void check_logits_shape(const torch::Tensor &logits, const torch::Tensor &action, const c10::optional<torch::Tensor> &mask, double scale, const char *op)
 {
-    check_logits(logits);
-    const int64_t rows = logits.size(0);
-    check_rows(action, "action", torch::kInt64, rows, logits);
-    const uint8_t *m = mask_of(mask, rows, logits);
-    c10::cuda::CUDAGuard guard(logits.device());
-    auto logp = torch::empty({rows}, logits.options().dtype(torch::kFloat32));
-    auto stats = torch::empty({rows, 2}, logp.options());
-    check_rc(slayer_b200_log_prob(logp.data_ptr<float>(), stats.data_ptr<float>(), logits.data_ptr(), dtype_code(logits, "logits"),
-                                  action.data_ptr<int64_t>(), m, rows, logits.size(1), logits.stride(0), scale, current_stream()),
-             "logProb");
-    return {logp, stats};
+    TORCH_CHECK_VALUE(logits.dim() >= 1 && action.sizes() == logits.sizes().slice(0, logits.dim() - 1), op,
+                      ": action must have the shape of logits without its last dimension, got ", action.sizes(), " for ", logits.sizes());
+    TORCH_CHECK_TYPE(action.scalar_type() == torch::kInt64 || action.scalar_type() == torch::kInt32, op, ": action must be int64 or int32, got ",
+                     action.scalar_type());
+    TORCH_CHECK_VALUE(!mask.has_value() || mask->sizes() == action.sizes(), op, ": mask must have the shape of action");
+    TORCH_CHECK_VALUE(logits.size(-1) >= 1, op, ": logits must have at least one entry per row");
+    TORCH_CHECK_VALUE(scale > 0.0 && scale < INFINITY, op, ": scale must be positive and finite, got ", scale);
 }
 
-// d / d logits of sum_r upstream * coef[r / coefLen] * logp[r].  into: a buffer that holds the gradient for an upstream of one
-// already, which is kept if upstream is one.
-torch::Tensor logitGradCuda(torch::Tensor logits, torch::Tensor action, c10::optional<torch::Tensor> mask, torch::Tensor stats,
-                            c10::optional<torch::Tensor> coef, int64_t coefLen, torch::Tensor upstream, float scale,
-                            c10::optional<torch::Tensor> into)
+// constants: no gradient flows into them
+torch::Tensor flat(const torch::Tensor &x, torch::ScalarType dtype) { return x.detach().to(dtype).reshape({-1}).contiguous(); }
+
+torch::Tensor per_row(const torch::Tensor &x, at::IntArrayRef shape, const char *what)
 {
-    check_logits(logits);
-    const int64_t rows = logits.size(0), V = logits.size(1);
-    check_rows(action, "action", torch::kInt64, rows, logits);
-    const uint8_t *m = mask_of(mask, rows, logits);
-    check_rows(stats, "stats", torch::kFloat32, 2 * rows, logits);
-    TORCH_CHECK(coefLen >= 1 && rows % coefLen == 0, "coefLen must divide the rows");
-    if (coef.has_value() && rows > 0) check_rows(*coef, "coef", torch::kFloat32, rows / coefLen, logits);
-    const bool by_row = upstream.dim() > 0;
-    check_rows(upstream, "upstream", torch::kFloat32, by_row ? rows : 1, logits);
-    c10::cuda::CUDAGuard guard(logits.device());
-    if (rows == 0) return torch::empty({0, V}, logits.options());
-    torch::Tensor grad;
-    if (into.has_value()) {
-        grad = *into;
-        check_rows(grad, "into", logits.scalar_type(), rows * V, logits);
-        TORCH_CHECK(!by_row, "a gradient that is there already needs one upstream value");
-    } else {
-        grad = torch::empty({rows, V}, logits.options());
+    TORCH_CHECK_VALUE(x.sizes() == shape, what, " must have the shape ", shape, ", got ", x.sizes());
+    return flat(x, torch::kFloat32);
+}
+
+c10::optional<torch::Tensor> flat_mask(const c10::optional<torch::Tensor> &mask)
+{
+    if (!mask.has_value()) return c10::nullopt;
+    return (mask->scalar_type() == torch::kBool ? *mask : mask->ne(0)).reshape({-1}).contiguous();
+}
+
+// the rows of logits, a view where there is one
+torch::Tensor rows_of(const torch::Tensor &logits)
+{
+    const int64_t V = logits.size(-1);
+    auto rows = logits.reshape({logits.numel() / V, V});
+    if (V > 1 && rows.size(0) > 0 && rows.stride(1) != 1) rows = rows.contiguous();
+    check_logits(rows);
+    return rows;
+}
+
+// What the backward passes need of a row, in one buffer: stats (two floats a row), logp, coef, and a workspace.
+struct RowBuffer {
+    torch::Tensor all;
+    float *stats, *logp, *coef;
+    void *workspace;
+    RowBuffer(const torch::Tensor &like, int64_t rows, int64_t coefs, int64_t workspace_bytes)
+        : RowBuffer(torch::empty({4 + 2 * rows + rows + coefs + (workspace_bytes + 3) / 4}, like.options().dtype(torch::kFloat32)), rows, coefs)
+    {
     }
-    check_rc(slayer_b200_logit_grad(grad.data_ptr(), logits.data_ptr(), dtype_code(logits, "logits"), action.data_ptr<int64_t>(), m,
-                                    stats.data_ptr<float>(), or_null<float>(coef), coefLen, upstream.data_ptr<float>(), by_row,
-                                    into.has_value(), rows, V, logits.stride(0), scale, current_stream()),
-             "logitGrad");
-    return grad;
+    RowBuffer(torch::Tensor buffer, int64_t rows, int64_t coefs) : all(std::move(buffer))
+    {
+        const int64_t even = (3 * rows + coefs + 1) / 2 * 2;       // the workspace is aligned to 8 bytes
+        stats = all.data_ptr<float>();
+        logp = stats + 2 * rows;
+        coef = logp + rows;
+        workspace = stats + even;
+    }
+};
+
+torch::Tensor logit_grad(const torch::Tensor &logits, const torch::Tensor &action, const torch::Tensor &mask, const float *stats, const float *coef,
+                         int64_t coef_len, const torch::Tensor &up, double scale, const torch::Tensor *into, const char *op)
+{
+    const auto x = rows_of(logits);
+    const int64_t rows = x.size(0), V = x.size(1);
+    c10::cuda::CUDAGuard guard(x.device());
+    auto grad = into ? *into : torch::empty({rows, V}, x.options());
+    const bool by_row = up.dim() > 0;
+    const auto upstream = up.to(torch::kFloat32).contiguous();
+    if (rows > 0)
+        check_rc(slayer_b200_logit_grad(grad.data_ptr(), x.data_ptr(), dtype_code(x, "logits"), action.data_ptr<int64_t>(),
+                                        mask.defined() ? reinterpret_cast<const uint8_t *>(mask.data_ptr<bool>()) : nullptr, stats, coef, coef_len,
+                                        upstream.data_ptr<float>(), by_row, into != nullptr, rows, V, x.stride(0), (float)scale, current_stream()),
+                 op);
+    return grad.view(logits.sizes());
 }
 
-// (loss [], logp [rows], stats [rows, 2], coef [rows], gradient [rows, V] or an empty tensor)
-std::vector<torch::Tensor> policyLossCuda(torch::Tensor logits, torch::Tensor action, torch::Tensor oldLogProb, torch::Tensor advantage,
-                                          c10::optional<torch::Tensor> refLogProb, c10::optional<torch::Tensor> mask, int64_t seqLen,
-                                          float scale, float clipLow, float clipHigh, float klCoef, int64_t reduction, bool wantGrad)
+// Forward reads the logits once and keeps two floats per row; backward reads them again and writes their gradient.
+struct ActionLogProb : public torch::autograd::Function<ActionLogProb> {
+    static torch::Tensor forward(AutogradContext *ctx, const torch::Tensor &logits, const torch::Tensor &action,
+                                 const c10::optional<torch::Tensor> &mask, double scale)
+    {
+        const auto x = rows_of(logits);
+        const int64_t rows = x.size(0);
+        const auto act = flat(action, torch::kInt64);
+        const auto keep = flat_mask(mask);
+        check_rows(act, "action", torch::kInt64, rows, x);
+        const uint8_t *m = mask_of(keep, rows, x);
+        c10::cuda::CUDAGuard guard(x.device());
+        auto logp = torch::empty(action.sizes(), x.options().dtype(torch::kFloat32));
+        auto stats = torch::empty({2 * rows}, logp.options());
+        check_rc(slayer_b200_log_prob(logp.data_ptr<float>(), stats.data_ptr<float>(), x.data_ptr(), dtype_code(x, "logits"), act.data_ptr<int64_t>(), m,
+                                      rows, x.size(1), x.stride(0), (float)scale, current_stream()),
+                 "actionLogProb");
+        ctx->save_for_backward({logits, act, keep.value_or(torch::Tensor()), stats});
+        ctx->saved_data["scale"] = scale;
+        return logp;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list up)
+    {
+        const auto v = ctx->get_saved_variables();
+        const double scale = ctx->saved_data["scale"].toDouble();
+        torch::Tensor by_row = up[0];
+        if (by_row.dim() == 0) by_row = by_row.reshape({1});
+        return {logit_grad(v[0], v[1], v[2], v[3].data_ptr<float>(), nullptr, 1, by_row, scale, nullptr, "actionLogProb"), Variable(), Variable(),
+                Variable()};
+    }
+};
+
+// Value and gradient from one pass over the logits.  The gradient for an upstream gradient of one is written in the forward pass
+// and handed over by the first backward, which checks on the device whether the upstream gradient is one and forms the
+// gradient anew if not (rounding it once); later backward passes form it anew.  Half-precision logits get theirs in the
+// backward pass alone: their losses are scaled up before it, and unscaled gradients would be lost below 6e-8.
+struct PolicyLoss : public torch::autograd::Function<PolicyLoss> {
+    static variable_list forward(AutogradContext *ctx, const torch::Tensor &logits, const torch::Tensor &action, const torch::Tensor &old,
+                                 const torch::Tensor &advantage, const c10::optional<torch::Tensor> &ref, const c10::optional<torch::Tensor> &mask,
+                                 int64_t seqLen, double scale, double low, double high, double kl, int64_t reduction, bool want)
+    {
+        const auto x = rows_of(logits);
+        const int64_t rows = x.size(0), V = x.size(1);
+        const auto act = flat(action, torch::kInt64);
+        const auto keep = flat_mask(mask);
+        check_rows(act, "action", torch::kInt64, rows, x);
+        check_rows(old, "oldLogProb", torch::kFloat32, rows, x);
+        if (ref.has_value()) check_rows(*ref, "refLogProb", torch::kFloat32, rows, x);
+        const uint8_t *m = mask_of(keep, rows, x);
+        const int64_t advLen = advantage.numel() == rows ? 1 : seqLen;
+        check_rows(advantage, "advantage", torch::kFloat32, rows / advLen, x);
+        c10::cuda::CUDAGuard guard(x.device());
+        auto loss = torch::empty({}, x.options().dtype(torch::kFloat32));
+        RowBuffer buffer(x, rows, rows, slayer_b200_policy_loss_workspace(rows, seqLen));
+        const bool early = want && x.scalar_type() != torch::kFloat16;
+        torch::Tensor grad;
+        if (early) grad = torch::empty({rows, V}, x.options());
+        check_rc(slayer_b200_policy_loss(loss.data_ptr<float>(), early ? grad.data_ptr() : nullptr, buffer.logp, buffer.stats, buffer.coef,
+                                         buffer.workspace, x.data_ptr(), dtype_code(x, "logits"), act.data_ptr<int64_t>(), old.data_ptr<float>(),
+                                         advantage.data_ptr<float>(), advLen, or_null<float>(ref), m, rows, seqLen, V, x.stride(0), (float)scale,
+                                         (float)low, (float)high, (float)kl, (int)reduction, current_stream()),
+                 "policyLoss");
+        if (want) {
+            ctx->save_for_backward({logits, act, keep.value_or(torch::Tensor()), buffer.all});
+            ctx->saved_data["scale"] = scale;
+            if (early) {
+                ctx->saved_data["early"] = grad;
+                ctx->saved_data["capture"] = capture_id(x);
+            }
+        }
+        auto logp = buffer.all.narrow(0, 2 * rows, rows).view(action.sizes());
+        ctx->mark_non_differentiable({logp});
+        return {loss, logp};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list up)
+    {
+        const auto v = ctx->get_saved_variables();
+        const int64_t rows = v[1].numel();
+        const RowBuffer buffer(v[3], rows, rows);
+        torch::Tensor early;
+        const auto it = ctx->saved_data.find("early");
+        if (it != ctx->saved_data.end()) {
+            early = it->second.toTensor();
+            ctx->saved_data.erase(it);
+            // replayed without its forward pass, a captured backward pass would hand over a buffer that is the user's by then
+            if (capture_id(v[0]) != ctx->saved_data["capture"].toInt()) early = torch::Tensor();
+        }
+        variable_list out(13);
+        out[0] = logit_grad(v[0], v[1], v[2], buffer.stats, buffer.coef, 1, up[0], ctx->saved_data["scale"].toDouble(), early.defined() ? &early : nullptr,
+                            "policyLoss");
+        return out;
+    }
+};
+
+// The pairs' coefficients need every sequence's sum: the logits are read for those, and again where the gradient is written.
+struct PreferenceLoss : public torch::autograd::Function<PreferenceLoss> {
+    static torch::Tensor forward(AutogradContext *ctx, const torch::Tensor &logits, const torch::Tensor &action, const torch::Tensor &ref,
+                                 const torch::Tensor &pairs, const c10::optional<torch::Tensor> &mask, double beta, double smoothing, double scale,
+                                 int64_t reduction)
+    {
+        const auto x = rows_of(logits);
+        const int64_t rows = x.size(0), S = logits.size(0), L = logits.size(1);
+        const auto act = flat(action, torch::kInt64);
+        const auto keep = flat_mask(mask);
+        check_rows(act, "action", torch::kInt64, rows, x);
+        check_rows(ref, "refLogProb", torch::kFloat32, S, x);
+        check_rows(pairs, "pairs", torch::kInt64, pairs.numel(), x);
+        const uint8_t *m = mask_of(keep, rows, x);
+        c10::cuda::CUDAGuard guard(x.device());
+        auto loss = torch::empty({}, x.options().dtype(torch::kFloat32));
+        RowBuffer buffer(x, rows, S, slayer_b200_preference_loss_workspace(S));
+        check_rc(slayer_b200_log_prob(buffer.logp, buffer.stats, x.data_ptr(), dtype_code(x, "logits"), act.data_ptr<int64_t>(), m, rows, x.size(1),
+                                      x.stride(0), (float)scale, current_stream()),
+                 "preferenceLoss");
+        check_rc(slayer_b200_preference_loss(loss.data_ptr<float>(), buffer.coef, buffer.workspace, buffer.logp, ref.data_ptr<float>(),
+                                             pairs.data_ptr<int64_t>(), S, L, pairs.size(0), (float)beta, (float)smoothing, (int)reduction,
+                                             current_stream()),
+                 "preferenceLoss");
+        ctx->save_for_backward({logits, act, keep.value_or(torch::Tensor()), buffer.all});
+        ctx->saved_data["scale"] = scale;
+        return loss;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list up)
+    {
+        const auto v = ctx->get_saved_variables();
+        const int64_t rows = v[1].numel(), S = v[0].size(0), L = v[0].size(1);
+        const RowBuffer buffer(v[3], rows, S);
+        variable_list out(9);
+        out[0] = logit_grad(v[0], v[1], v[2], buffer.stats, buffer.coef, L > 0 ? L : 1, up[0], ctx->saved_data["scale"].toDouble(), nullptr,
+                            "preferenceLoss");
+        return out;
+    }
+};
+
+torch::Tensor actionLogProbCuda(const torch::Tensor &logits, const torch::Tensor &action, const c10::optional<torch::Tensor> &mask, double scale)
 {
-    check_logits(logits);
-    const int64_t rows = logits.size(0), V = logits.size(1);
-    check_rows(action, "action", torch::kInt64, rows, logits);
-    check_rows(oldLogProb, "oldLogProb", torch::kFloat32, rows, logits);
-    if (refLogProb.has_value()) check_rows(*refLogProb, "refLogProb", torch::kFloat32, rows, logits);
-    const uint8_t *m = mask_of(mask, rows, logits);
-    TORCH_CHECK(seqLen >= 1 && rows % seqLen == 0, "the rows must be whole sequences");
-    const int64_t advLen = advantage.numel() == rows ? 1 : seqLen;
-    check_rows(advantage, "advantage", torch::kFloat32, rows / advLen, logits);
-    c10::cuda::CUDAGuard guard(logits.device());
-    auto f32 = logits.options().dtype(torch::kFloat32);
-    auto loss = torch::empty({}, f32);
-    auto logp = torch::empty({rows}, f32), stats = torch::empty({rows, 2}, f32), coef = torch::empty({rows}, f32);
-    auto grad = wantGrad ? torch::empty({rows, V}, logits.options()) : torch::empty({0}, logits.options());
-    auto workspace = torch::empty({slayer_b200_policy_loss_workspace(rows, seqLen)}, logits.options().dtype(torch::kUInt8));
-    check_rc(slayer_b200_policy_loss(loss.data_ptr<float>(), wantGrad ? grad.data_ptr() : nullptr, logp.data_ptr<float>(),
-                                     stats.data_ptr<float>(), coef.data_ptr<float>(), workspace.data_ptr(), logits.data_ptr(),
-                                     dtype_code(logits, "logits"), action.data_ptr<int64_t>(), oldLogProb.data_ptr<float>(),
-                                     advantage.data_ptr<float>(), advLen, or_null<float>(refLogProb), m, rows, seqLen, V,
-                                     logits.stride(0), scale, clipLow, clipHigh, klCoef, (int)reduction, current_stream()),
-             "policyLoss");
-    return {loss, logp, stats, coef, grad};
+    check_logits_shape(logits, action, mask, scale, "actionLogProb");
+    return ActionLogProb::apply(logits, action, mask, scale);
 }
 
-// (loss [], coef [sequences])
-std::vector<torch::Tensor> preferenceLossCuda(torch::Tensor logp, torch::Tensor refLogProb, torch::Tensor pairs, int64_t sequences,
-                                              float beta, float smoothing, int64_t reduction)
+// (loss, the rows' log-probabilities)
+std::vector<torch::Tensor> policyLossCuda(const torch::Tensor &logits, const torch::Tensor &action, const torch::Tensor &oldLogProb,
+                                          const torch::Tensor &advantage, const c10::optional<torch::Tensor> &refLogProb,
+                                          const c10::optional<torch::Tensor> &mask, double clipLow, double clipHigh, double klCoef, double scale,
+                                          int64_t reduction)
 {
-    TORCH_CHECK(logp.is_cuda() && logp.is_contiguous() && logp.scalar_type() == torch::kFloat32, "logp must be a contiguous float32 CUDA tensor");
-    TORCH_CHECK(sequences >= 0 && (sequences ? logp.numel() % sequences == 0 : logp.numel() == 0), "logp must hold whole sequences");
-    check_rows(refLogProb, "refLogProb", torch::kFloat32, sequences, logp);
-    TORCH_CHECK(pairs.dim() == 2 && pairs.size(1) == 2, "pairs must be [pairs, 2]");
-    check_rows(pairs, "pairs", torch::kInt64, pairs.numel(), logp);
-    c10::cuda::CUDAGuard guard(logp.device());
-    auto loss = torch::empty({}, logp.options());
-    auto coef = torch::empty({sequences}, logp.options());
-    auto workspace = torch::empty({slayer_b200_preference_loss_workspace(sequences)}, logp.options().dtype(torch::kUInt8));
-    check_rc(slayer_b200_preference_loss(loss.data_ptr<float>(), coef.data_ptr<float>(), workspace.data_ptr(), logp.data_ptr<float>(),
-                                         refLogProb.data_ptr<float>(), pairs.data_ptr<int64_t>(), sequences,
-                                         sequences ? logp.numel() / sequences : 0, pairs.size(0), beta, smoothing, (int)reduction,
-                                         current_stream()),
-             "preferenceLoss");
-    return {loss, coef};
+    check_logits_shape(logits, action, mask, scale, "policyLoss");
+    const auto shape = action.sizes();
+    TORCH_CHECK_VALUE(reduction != SLAYER_B200_SEQUENCE || !shape.empty(), "policyLoss: reduction 'sequence' needs a dimension of choices");
+    const auto old = per_row(oldLogProb, shape, "policyLoss: oldLogProb");
+    c10::optional<torch::Tensor> ref;
+    if (refLogProb.has_value()) ref = per_row(*refLogProb, shape, "policyLoss: refLogProb");
+    const bool by_sequence = !shape.empty() && advantage.sizes() != shape && advantage.sizes() == shape.slice(0, shape.size() - 1);
+    const auto adv = per_row(advantage, by_sequence ? shape.slice(0, shape.size() - 1) : shape, "policyLoss: advantage");
+    const int64_t seqLen = shape.empty() ? 1 : std::max<int64_t>(1, shape.back());
+    const bool want = at::GradMode::is_enabled() && logits.requires_grad();
+    return PolicyLoss::apply(logits, action, old, adv, ref, mask, seqLen, scale, clipLow, clipHigh, klCoef, reduction, want);
+}
+
+torch::Tensor preferenceLossCuda(const torch::Tensor &logits, const torch::Tensor &action, const torch::Tensor &refLogProb,
+                                 const c10::optional<torch::Tensor> &pairs, const c10::optional<torch::Tensor> &mask, double beta, double smoothing,
+                                 double scale, int64_t reduction)
+{
+    TORCH_CHECK_VALUE(logits.dim() == 3, "preferenceLoss: logits must be [sequences, choices, entries], got ", logits.sizes());
+    check_logits_shape(logits, action, mask, scale, "preferenceLoss");
+    const int64_t S = logits.size(0);
+    const auto ref = per_row(refLogProb, {S}, "preferenceLoss: refLogProb");
+    torch::Tensor pair;
+    if (pairs.has_value()) {
+        TORCH_CHECK_VALUE(pairs->dim() == 2 && pairs->size(1) == 2 && (pairs->scalar_type() == torch::kInt64 || pairs->scalar_type() == torch::kInt32),
+                          "preferenceLoss: pairs must be [P, 2] integers, got ", pairs->sizes(), " ", pairs->scalar_type());
+        pair = pairs->to(torch::kInt64).contiguous();
+    } else {
+        TORCH_CHECK_VALUE(S % 2 == 0, "preferenceLoss: without pairs the number of sequences must be even, got ", S);
+        const auto first = torch::arange(S / 2, logits.options().dtype(torch::kInt64));
+        pair = torch::stack({first, first + S / 2}, 1);
+    }
+    return PreferenceLoss::apply(logits, action, ref, pair, mask, beta, smoothing, scale, reduction);
 }
 
 void check_matrix(const torch::Tensor &x, const char *name)
@@ -218,11 +378,9 @@ void muonStepCuda(std::vector<torch::Tensor> weights, const std::vector<torch::T
 
 void bind_learning(pybind11::module_ &m)
 {
-    m.def("logProb", &logProbCuda, "Log-probability of the chosen entry of each row of logits (CUDA)");
-    m.def("logitGrad", &logitGradCuda, "Gradient of rows' log-probabilities with respect to the logits (CUDA)");
-    m.def("policyLoss", &policyLossCuda, "Clipped policy loss with a KL term: value and gradient in one pass (CUDA)");
-    m.def("preferenceLoss", &preferenceLossCuda, "Loss of paired sequences and its derivative by each sequence's log-probability (CUDA)");
+    m.def("actionLogProb", &actionLogProbCuda, "Log-probability of the chosen entry of each row of logits, differentiable (CUDA)");
+    m.def("policyLoss", &policyLossCuda, "Clipped policy loss with a KL term, value and gradient in one pass, differentiable (CUDA)");
+    m.def("preferenceLoss", &preferenceLossCuda, "Loss of paired sequences of choices, differentiable (CUDA)");
     m.def("orthogonalize", &orthogonalizeCuda, "Matrices made near orthogonal by Newton-Schulz products (CUDA)");
     m.def("muonStep", &muonStepCuda, "Momentum, orthogonalised update and decay of a list of weights, in place (CUDA)");
-    m.def("captureId", &capture_id, "Which stream capture the current stream of a tensor's device is in (0: none)");
 }

@@ -19,7 +19,6 @@ the entry chosen in each (``actionLogProb`` gives the values of the policy that 
 """
 import numpy as np
 import torch
-from torch.autograd.function import once_differentiable
 
 from .layer import slayerCuda, spikeLayer
 
@@ -41,106 +40,6 @@ class _NumSpikesFunction(torch.autograd.Function):
 
 
 # ------------------------------------------------------------------- choices: rows of logits, one entry each
-def _rows(logits, action, mask, name):
-    """The rows of ``logits [..., V]`` as ``[rows, V]`` (a view where there is one), their actions and mask, contiguous."""
-    if logits.dim() < 1 or tuple(action.shape) != tuple(logits.shape[:-1]):
-        raise ValueError("%s: action must have the shape of logits without its last dimension, got %s for %s"
-                         % (name, tuple(action.shape), tuple(logits.shape)))
-    if action.dtype not in (torch.int64, torch.int32):
-        raise TypeError("%s: action must be int64 or int32, got %s" % (name, action.dtype))
-    if mask is not None:
-        if tuple(mask.shape) != tuple(action.shape):
-            raise ValueError("%s: mask must have the shape of action, got %s for %s" % (name, tuple(mask.shape), tuple(action.shape)))
-        mask = (mask if mask.dtype == torch.bool else mask != 0).reshape(-1).contiguous()
-    V = logits.shape[-1]
-    if V < 1:
-        raise ValueError("%s: logits must have at least one entry per row" % name)
-    rows = logits.reshape(-1, V)
-    if V > 1 and rows.stride(1) != 1:
-        rows = rows.contiguous()
-    return rows, action.reshape(-1).long().contiguous(), mask
-
-
-def _per_row(value, shape, name):
-    """A value per row (constant: no gradient flows into it) as a flat float32 tensor."""
-    if tuple(value.shape) != tuple(shape):
-        raise ValueError("%s must have the shape %s, got %s" % (name, tuple(shape), tuple(value.shape)))
-    return value.detach().reshape(-1).float().contiguous()
-
-
-def _scale_of(scale):
-    scale = float(scale)
-    if not 0.0 < scale < float("inf"):
-        raise ValueError("scale must be positive and finite, got %s" % scale)
-    return scale
-
-
-class _LogProbFunction(torch.autograd.Function):
-    """Forward reads the logits once and keeps two floats per row; backward reads them again and writes their gradient."""
-
-    @staticmethod
-    def forward(ctx, logits, action, mask, scale):
-        logp, stats = slayerCuda.logProb(logits, action, mask, scale)
-        ctx.save_for_backward(logits, action, mask, stats)
-        ctx.scale = scale
-        return logp
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, up):
-        logits, action, mask, stats = ctx.saved_tensors
-        return slayerCuda.logitGrad(logits, action, mask, stats, None, 1, up.contiguous(), ctx.scale, None), None, None, None
-
-
-class _PolicyLossFunction(torch.autograd.Function):
-    """Value and gradient from one pass over the logits.  The gradient for an upstream gradient of one is written in the
-    forward pass and handed over by the first backward, which checks on the device whether the upstream gradient is one and
-    forms the gradient anew if not (rounding it once); later backward passes form it anew.  Half-precision logits get theirs in
-    the backward pass alone: their losses are scaled up before it, and unscaled gradients would be lost below 6e-8."""
-
-    @staticmethod
-    def forward(ctx, logits, action, old, advantage, ref, mask, seqLen, scale, clip, klCoef, reduction, grad):
-        early = grad and logits.dtype != torch.float16
-        loss, logp, stats, coef, early_grad = slayerCuda.policyLoss(logits, action, old, advantage, ref, mask, seqLen, scale, clip[0],
-                                                                    clip[1], klCoef, reduction, early)
-        if grad:
-            ctx.save_for_backward(logits, action, mask, stats, coef)
-            ctx.scale = scale
-            ctx.early = early_grad if early else None
-            ctx.capture = slayerCuda.captureId(logits) if early else 0
-        ctx.mark_non_differentiable(logp)
-        return loss, logp
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, up, _up_logp):
-        logits, action, mask, stats, coef = ctx.saved_tensors
-        early, ctx.early = ctx.early, None
-        # replayed without its forward pass, a captured backward pass would hand over a buffer that is the user's by then
-        if early is not None and slayerCuda.captureId(logits) != ctx.capture:
-            early = None
-        return (slayerCuda.logitGrad(logits, action, mask, stats, coef, 1, up, ctx.scale, early),) + (None,) * 11
-
-
-class _PreferenceLossFunction(torch.autograd.Function):
-    """The pairs' coefficients need every sequence's sum: the logits are read for those, and again where the gradient is written."""
-
-    @staticmethod
-    def forward(ctx, logits, action, ref, pairs, mask, sequences, beta, smoothing, scale, reduction):
-        logp, stats = slayerCuda.logProb(logits, action, mask, scale)
-        loss, coef = slayerCuda.preferenceLoss(logp, ref, pairs, sequences, beta, smoothing, reduction)
-        ctx.save_for_backward(logits, action, mask, stats, coef)
-        ctx.scale = scale
-        ctx.seqLen = max(1, logits.shape[0] // max(1, sequences))
-        return loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, up):
-        logits, action, mask, stats, coef = ctx.saved_tensors
-        return (slayerCuda.logitGrad(logits, action, mask, stats, coef, ctx.seqLen, up, ctx.scale, None),) + (None,) * 9
-
-
 def actionLogProb(logits, action, mask=None, scale=1.0):
     """Log-probability of one chosen entry of each row: ``log softmax(scale * logits)[action]``, float32, of the shape of
     ``action``; 0 where ``mask`` is false (those rows are not read), NaN where the action lies outside.
@@ -148,8 +47,7 @@ def actionLogProb(logits, action, mask=None, scale=1.0):
     ``logits [..., V]``: float32, bfloat16 or float16, any strides (rows whose entries are apart are copied).  Differentiable in
     ``logits``.  It is what ``policyLoss`` and ``preferenceLoss`` take as old and reference values.  Not part of the
     reference's interface."""
-    rows, act, mask = _rows(logits, action, mask, "actionLogProb")
-    return _LogProbFunction.apply(rows, act, mask, _scale_of(scale)).reshape(action.shape)
+    return slayerCuda.actionLogProb(logits, action, mask, float(scale))
 
 
 def policyLoss(logits, action, oldLogProb, advantage, refLogProb=None, mask=None, clip=0.2, klCoef=0.0, scale=1.0, reduction='sum',
@@ -180,19 +78,9 @@ def policyLoss(logits, action, oldLogProb, advantage, refLogProb=None, mask=None
         raise ValueError("policyLoss: the clip range must not be negative, got %s" % (clip,))
     if (klCoef != 0.0) != (refLogProb is not None):
         raise ValueError("policyLoss: klCoef and refLogProb belong together")
-    shape = tuple(action.shape)
-    if reduction == 'sequence' and not shape:
-        raise ValueError("policyLoss: reduction 'sequence' needs a dimension of choices")
-    rows, act, mask = _rows(logits, action, mask, "policyLoss")
-    old = _per_row(oldLogProb, shape, "policyLoss: oldLogProb")
-    ref = None if refLogProb is None else _per_row(refLogProb, shape, "policyLoss: refLogProb")
-    by_sequence = len(shape) >= 1 and tuple(advantage.shape) == shape[:-1] and tuple(advantage.shape) != shape
-    adv = _per_row(advantage, shape[:-1] if by_sequence else shape, "policyLoss: advantage")
-    seqLen = max(1, shape[-1]) if shape else 1
-    grad = torch.is_grad_enabled() and rows.requires_grad
-    loss, logp = _PolicyLossFunction.apply(rows, act, old, adv, ref, mask, seqLen, _scale_of(scale), (low, high), float(klCoef),
-                                           kinds[reduction], grad)
-    return (loss, logp.reshape(shape)) if returnLogProb else loss
+    loss, logp = slayerCuda.policyLoss(logits, action, oldLogProb, advantage, refLogProb, mask, low, high, float(klCoef), float(scale),
+                                       kinds[reduction])
+    return (loss, logp) if returnLogProb else loss
 
 
 def preferenceLoss(logits, action, refLogProb, pairs=None, mask=None, beta=0.1, labelSmoothing=0.0, scale=1.0, reduction='sum'):
@@ -209,22 +97,9 @@ def preferenceLoss(logits, action, refLogProb, pairs=None, mask=None, beta=0.1, 
     kinds = {'sum': 0, 'mean': 1}
     if reduction not in kinds:
         raise ValueError("preferenceLoss: reduction must be one of %s, got %r" % (sorted(kinds), reduction))
-    if logits.dim() != 3:
-        raise ValueError("preferenceLoss: logits must be [sequences, choices, entries], got %s" % (tuple(logits.shape),))
     if not 0.0 <= labelSmoothing <= 1.0:
         raise ValueError("preferenceLoss: labelSmoothing must lie between 0 and 1, got %s" % labelSmoothing)
-    S = logits.shape[0]
-    rows, act, mask = _rows(logits, action, mask, "preferenceLoss")
-    ref = _per_row(refLogProb, (S,), "preferenceLoss: refLogProb")
-    if pairs is None:
-        if S % 2:
-            raise ValueError("preferenceLoss: without pairs the number of sequences must be even, got %d" % S)
-        first = torch.arange(S // 2, device=logits.device)
-        pairs = torch.stack([first, first + S // 2], 1)
-    if pairs.dim() != 2 or pairs.shape[1] != 2 or pairs.dtype not in (torch.int64, torch.int32):
-        raise ValueError("preferenceLoss: pairs must be [P, 2] integers, got %s %s" % (tuple(pairs.shape), pairs.dtype))
-    return _PreferenceLossFunction.apply(rows, act, ref, pairs.long().contiguous(), mask, S, float(beta), float(labelSmoothing),
-                                         _scale_of(scale), kinds[reduction])
+    return slayerCuda.preferenceLoss(logits, action, refLogProb, pairs, mask, float(beta), float(labelSmoothing), float(scale), kinds[reduction])
 
 
 class spikeLoss(torch.nn.Module):
