@@ -307,8 +307,8 @@ int slayer_b200_logit_grad(void *grad, const void *logits, int dtype, const int6
  * (SLAYER_B200_MEAN), or the mean over the rows / seq_len sequences of the mean over each one's rows
  * that are not masked (SLAYER_B200_SEQUENCE); a mean over no rows is 0.  ref_logp may be NULL (no KL
  * term).  old_logp, ref_logp and advantage are constants.  grad ([rows, V], contiguous, or NULL) is
- * d loss / d logits; with logp, stats (either may be NULL) and coef (rows floats) a later
- * slayer_b200_logit_grad gives it for another upstream gradient.  workspace:
+ * d loss / d logits; with stats (2 * rows floats) and coef (rows floats) a later
+ * slayer_b200_logit_grad gives it for another upstream gradient.  logp may be NULL.  workspace:
  * slayer_b200_policy_loss_workspace(rows, seq_len) bytes of device memory, aligned to 8.  It has no
  * counterpart in the reference, whose losses need the desired answer (src/spikeLoss.py:39-104).
  */

@@ -20,6 +20,9 @@ int sm_count();
 // device (raises the per-function limit above 48 KB when needed; remembered per device).
 int reserve_dynamic_smem(const void *func, size_t bytes);
 
+// How many clusters of `ranks` CTAs of a kernel the current device holds at once (remembered); 0: none.
+int resident_clusters(const void *func, int ranks, int threads, size_t smem);
+
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }

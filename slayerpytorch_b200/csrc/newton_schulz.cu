@@ -20,10 +20,6 @@
 #include <cuda_fp16.h>
 #include <math.h>
 
-#include <map>
-#include <mutex>
-#include <tuple>
-
 #include "common.cuh"
 #include "tensor.cuh"
 
@@ -1144,31 +1140,6 @@ static void ns_take(NsJob &J, int parts, unsigned char *&at)
     at = J.b + a;
 }
 
-// How many clusters of `ranks` CTAs of a kernel the device holds at once (remembered).
-static int ns_resident(const void *kern, int ranks, size_t smem)
-{
-    static std::mutex mu;
-    static std::map<std::tuple<const void *, int, int>, int> known;
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) dev = 0;
-    std::lock_guard<std::mutex> lock(mu);
-    int &n = known[std::make_tuple(kern, ranks, dev)];
-    if (n == 0) {
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(ranks);
-        cfg.blockDim = dim3(kNsThreads);
-        cfg.dynamicSmemBytes = smem;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = ranks;
-        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-        if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) n = 0;
-    }
-    return n;
-}
-
 template <typename T, int PARTS, int CG>
 static int ns_run(NsArgs &A, int steps, cudaStream_t st)
 {
@@ -1212,7 +1183,7 @@ static int ns_run(NsArgs &A, int steps, cudaStream_t st)
             while (P.split[k] < most && P.tiles[k] * P.split[k] * 2 <= sms && index[k] >= P.split[k] * 4) P.split[k] *= 2;
             if (CG == 1) ranks = P.split[k] > ranks ? P.split[k] : ranks;
         }
-        const int held = ns_resident((const void *)kern, ranks, smem) * ranks;
+        const int held = resident_clusters((const void *)kern, ranks, kNsThreads, smem) * ranks;
         if (held <= 0) {
             set_error("Newton-Schulz products: the device holds no cluster of %d CTAs", ranks);
             return SLAYER_B200_EUNSUPPORTED;

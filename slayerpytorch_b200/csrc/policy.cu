@@ -9,13 +9,18 @@
 // What bounds the kernels is one read of the logits and one write of their gradient (HBM).  A row is read once: its running
 // maximum and its sum of exponentials relative to that maximum are carried along (each thread's own, joined at the row's
 // end), and the row itself waits in shared memory until its coefficient is known; the gradient is then formed from there.
-// A thread keeps and takes back the 16-byte pieces that it loaded itself, so the copy needs no barrier.  Sums of
+// A thread keeps and takes back the 16-byte pieces that it loaded itself, so the copy needs no barrier.  A long row has a CTA of
+// its own, a few of them on an SM: while one waits for its row's coefficient the others load.  Sums of
 // exponentials are fp32 (each relative to the row's maximum, at most V terms of at most 1, added in a tree over the
 // threads); what is said of one row - lp, the ratio, the loss - is computed in double, because a ratio that lies next to a
-// border of the clip range decides whether the row has a gradient at all.
+// border of the clip range decides whether the row has a gradient at all.  A double exponential takes as long as a quarter of a
+// row's loads: the gradient waits for two of them, side by side in two lanes, and everything else that is said of
+// a row comes in the launch that adds up the loss.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -24,6 +29,8 @@ namespace cg = cooperative_groups;
 namespace sb200 {
 
 enum RowMode { kLogProb, kPolicy, kGrad };
+
+constexpr int kSums = 256;       // CTAs that add up a loss, at most
 
 struct RowArgs {
     const void *logits;
@@ -34,7 +41,7 @@ struct RowArgs {
     const int64_t *action;
     const uint8_t *mask;          // NULL: every row counts
     float *logp;                  // per row, may be NULL
-    float2 *stats;                // per row: maximum of x, 1 / sum of exponentials
+    float2 *stats;                // per row: maximum of x, sum of exponentials
     // policy
     const float *old_lp, *ref_lp, *advantage;
     int64_t adv_len;              // rows per advantage
@@ -42,12 +49,13 @@ struct RowArgs {
     const int *counts;            // unmasked rows of each group of seq_len rows; NULL: share is the row's share
     int64_t seq_len;
     double share;                 // of a row; with counts: divided by the group's count
-    double *row_loss;
+    double *gap;                  // kPolicy: (chosen - maximum) * scale, the part of lp that the sum does not give
     float *coef;                  // written by kPolicy; read by kGrad, where it may be NULL (1), one for each coef_len rows
     int64_t coef_len;
     const float *upstream;        // kGrad: one value, or one per row
     bool upstream_rows, only_if_not_one;
     void *grad;
+    unsigned *arrived;            // kPolicy: set to zero for the sum that follows
 };
 
 template <typename T> __device__ __forceinline__ float to_f(T v);
@@ -59,97 +67,248 @@ template <> __device__ __forceinline__ float from_f(float v) { return v; }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
 
+// 2^x to 2^-22 of itself, below 2^-126 zero: one instruction of the special function unit, where exp2f takes seven to
+// keep results that are nothing beside a row's sum (what bounds a long row are instructions: 13 an entry with exp2f, 9 so)
+__device__ __forceinline__ float two_to(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// sixteen bytes of a row
 template <typename T>
-struct alignas(16) Piece {
+struct Piece {
     static constexpr int N = 16 / sizeof(T);
-    T v[N];
+    static __device__ __forceinline__ void open(float (&f)[N], uint4 v)
+    {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 4) {
+                f[i] = __uint_as_float(w[i]);
+            } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                f[2 * i] = __uint_as_float(w[i] << 16);
+                f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            } else {
+                const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+                f[2 * i] = x.x;
+                f[2 * i + 1] = x.y;
+            }
+        }
+    }
+    // of 16-bit entries: two of them, and the larger ones of two pairs
+    static __device__ __forceinline__ void open2(float (&f)[2], uint32_t w)
+    {
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+            f[0] = __uint_as_float(w << 16);
+            f[1] = __uint_as_float(w & 0xffff0000u);
+        } else {
+            const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+            f[0] = x.x;
+            f[1] = x.y;
+        }
+    }
+    static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b)
+    {
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+            const __nv_bfloat162 x = __hmax2(*reinterpret_cast<const __nv_bfloat162 *>(&a), *reinterpret_cast<const __nv_bfloat162 *>(&b));
+            return *reinterpret_cast<const uint32_t *>(&x);
+        } else {
+            const __half2 x = __hmax2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b));
+            return *reinterpret_cast<const uint32_t *>(&x);
+        }
+    }
+    static __device__ __forceinline__ uint4 close(const float (&f)[N])
+    {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 4) {
+                w[i] = __float_as_uint(f[i]);
+            } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                const __nv_bfloat162 x = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t *>(&x);
+            } else {
+                const __half2 x = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t *>(&x);
+            }
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
 };
 
-// maximum and sum of exponentials of part of a row
+// Maximum m and sum of exponentials s of part of a row: s = sum of 2^(x k - c), c = m k rounded.  One multiply-add an entry; that c
+// is not m k exactly changes s and the gradient's exponentials alike, and log_sum takes it out again.  Only where m k
+// would overflow are the exponentials taken of (x - m) k.
 struct Soft {
     float m = -INFINITY, s = 0.0f;
-    // what the exponentials are taken relative to: of a part that holds only -inf, 0 (its exponentials are 0 then)
-    __device__ __forceinline__ static float base(float m) { return m == -INFINITY ? 0.0f : m; }
-    __device__ __forceinline__ void join(float om, float os, float k)
+    __device__ __forceinline__ static bool huge(float m) { return fabsf(m) > 1e37f; }
+    // (a part that holds only -inf has exponentials of 0, not of -inf + inf)
+    __device__ __forceinline__ static float shift(float m, float k) { return huge(m) ? 0.0f : __fmul_rn(m, k); }
+    __device__ __forceinline__ static float power(float x, float m, float c, float k) { return two_to(huge(m) && m > -INFINITY ? (x - m) * k : fmaf(x, k, -c)); }
+    // a sum relative to m as one relative to n >= m
+    __device__ __forceinline__ void raise(float n, float k)
     {
-        const float n = fmaxf(m, om), b = base(n);
-        s = s * exp2f((m - b) * k) + os * exp2f((om - b) * k);
+        if (n == m) return;
+        s *= m == -INFINITY ? 0.0f : two_to(huge(n) || huge(m) ? (m - n) * k : shift(m, k) - shift(n, k));
         m = n;
     }
-    template <typename T, int N>
-    __device__ __forceinline__ void add(const T (&v)[N], float k)
+    template <int N>
+    __device__ __forceinline__ void add(const float (&v)[N], float k)
     {
         float n = m;
 #pragma unroll
-        for (int i = 0; i < N; ++i) n = fmaxf(n, to_f(v[i]));
-        const float b = base(n);
-        if (n != m) s *= exp2f((m - b) * k);
-        m = n;
+        for (int i = 0; i < N; ++i) n = fmaxf(n, v[i]);
+        raise(n, k);
+        const float c = shift(m, k);
         float t = 0.0f;
 #pragma unroll
-        for (int i = 0; i < N; ++i) t += exp2f((to_f(v[i]) - b) * k);
+        for (int i = 0; i < N; ++i) t += power(v[i], m, c, k);
         s += t;
     }
+    // pieces of a row: their maximum first, of 16-bit entries two at a time
+    template <typename T, int NB>
+    __device__ __forceinline__ void add(const uint4 (&v)[NB], float k)
+    {
+        using P = Piece<T>;
+        float n = m;
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b) n = fmaxf(fmaxf(fmaxf(n, __uint_as_float(v[b].x)), fmaxf(__uint_as_float(v[b].y), __uint_as_float(v[b].z))), __uint_as_float(v[b].w));
+        } else {
+            uint32_t each[NB];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) each[b] = P::larger(P::larger(v[b].x, v[b].y), P::larger(v[b].z, v[b].w));
+            uint32_t top = each[0];
+#pragma unroll
+            for (int b = 1; b < NB; ++b) top = P::larger(top, each[b]);
+            float both[2];
+            P::open2(both, top);
+            n = fmaxf(n, fmaxf(both[0], both[1]));
+        }
+        raise(n, k);
+        const float c = shift(m, k);
+        float t[4] = {};
+        if (!huge(m)) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                float e[P::N];
+                P::open(e, v[b]);
+#pragma unroll
+                for (int i = 0; i < P::N; ++i) t[i & 3] += two_to(fmaf(e[i], k, -c));
+            }
+        } else {
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                float e[P::N];
+                P::open(e, v[b]);
+#pragma unroll
+                for (int i = 0; i < P::N; ++i) t[0] += power(e[i], m, c, k);
+            }
+        }
+        s += (t[0] + t[1]) + (t[2] + t[3]);
+    }
+    // all lanes of groups of G get the group's
+    template <int G>
+    __device__ __forceinline__ void meet(float k)
+    {
+        float n = m;
+#pragma unroll
+        for (int o = G / 2; o > 0; o >>= 1) n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, o));
+        raise(n, k);
+#pragma unroll
+        for (int o = G / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    }
+    // log of c's rounding: sum of exp((x - m) scale) = s (1 + that)
+    __device__ __forceinline__ static double rounding(float m, float k)
+    {
+        return huge(m) ? 0.0 : ((double)shift(m, k) - (double)m * (double)k) * 0.6931471805599453;
+    }
+    __device__ __forceinline__ static double log_sum(float m, float s, float k) { return log((double)s) + rounding(m, k); }
 };
 
-// What one row comes to: called by one thread with the row's maximum m and sum s.
-// Returns (c, c (1 / s)): the gradient is c * (j == a) - c (1 / s) * exp2((x[j] - m) k).
-// `write`: whether this thread is the one that stores the row's results.
-template <RowMode MODE>
-__device__ float2 row_result(const RowArgs &A, int64_t row, float m, float s, float xa, bool write)
-{
-    float c;
-    if constexpr (MODE == kGrad) {
-        c = (A.coef ? A.coef[row / A.coef_len] : 1.0f) * (A.upstream_rows ? A.upstream[row] : A.upstream[0]) * A.scale;
-        return make_float2(c, c * s);          // s is 1 / sum here
-    } else {
-        const double lp = (double)(xa - m) * (double)A.scale - log((double)s);
-        if (write) {
-            if (A.logp) A.logp[row] = (float)lp;
-            if (A.stats) A.stats[row] = make_float2(m, 1.0f / s);
-        }
-        if constexpr (MODE == kLogProb) return make_float2(0.0f, 0.0f);
-        const double gain = A.advantage[row / A.adv_len];
-        const double r = exp(lp - (double)A.old_lp[row]);
-        const double cut = (r < A.lo ? A.lo : r > A.hi ? A.hi : r) * gain, full = r * gain;
-        double per = -(full > cut ? cut : full), slope = full > cut ? 0.0 : -full;
-        if (A.ref_lp) {
-            const double d = (double)A.ref_lp[row] - lp, e = expm1(d);
-            per += A.kl * (e - d);
-            slope -= A.kl * e;
-        }
-        double share = A.share;
-        if (A.counts) {
-            const int n = A.counts[row / A.seq_len];
-            share /= (double)(n > 1 ? n : 1);
-        }
-        c = (float)(share * slope);
-        if (write) {
-            A.row_loss[row] = share * per;
-            A.coef[row] = c;
-        }
-        c = c * 1.0f * A.scale;          // in the order of kGrad with an upstream of one, and with its 1 / s: the same bits
-        return make_float2(c, c * (1.0f / s));
-    }
-}
-
-template <RowMode MODE>
-__device__ void masked_row(const RowArgs &A, int64_t row)
-{
-    if (A.logp) A.logp[row] = 0.0f;
-    if (MODE != kGrad && A.stats) A.stats[row] = make_float2(0.0f, 0.0f);
-    if constexpr (MODE == kPolicy) {
-        A.row_loss[row] = 0.0;
-        A.coef[row] = 0.0f;
-    }
-}
-
 template <typename T>
-__device__ __forceinline__ float chosen(const RowArgs &A, int64_t row, const T *x, int &a)
+__device__ __forceinline__ float chosen(const RowArgs &A, int64_t at, const T *x, int &a)
 {
-    const int64_t at = A.action[row];
     a = at >= 0 && at < A.V ? (int)at : -1;
     return a < 0 ? NAN : to_f(x[a]);            // an action outside the row makes the row's results NaN
+}
+
+// A row's share of the loss
+__device__ __forceinline__ double row_share(const RowArgs &A, int64_t row)
+{
+    if (!A.counts) return A.share;
+    const int n = A.counts[(unsigned)row / (unsigned)A.seq_len];
+    return A.share / (double)(n > 1 ? n : 1);
+}
+
+// The clipped term: its value at ratio r, and its derivative by lp
+__device__ __forceinline__ double2 clipped(const RowArgs &A, double r, double gain)
+{
+    const double cut = (r < A.lo ? A.lo : r > A.hi ? A.hi : r) * gain, full = r * gain;
+    return make_double2(-(full > cut ? cut : full), full > cut ? 0.0 : -full);
+}
+
+// What belongs to a row besides its logits: requested before they are read.
+struct RowFacts {
+    int a;                        // -1: outside the row
+    float xa, old_lp, ref_lp, gain;
+    double share;
+};
+
+template <RowMode MODE, typename T>
+__device__ __forceinline__ RowFacts row_facts(const RowArgs &A, int64_t row, const T *x, int64_t action)
+{
+    RowFacts f = {};
+    f.xa = chosen(A, action, x, f.a);
+    if (MODE == kPolicy) {
+        f.old_lp = A.old_lp[row];
+        f.ref_lp = A.ref_lp ? A.ref_lp[row] : 0.0f;
+        f.gain = A.advantage[(unsigned)row / (unsigned)A.adv_len];
+        f.share = row_share(A, row);
+    }
+    return f;
+}
+
+// What one row comes to, from its maximum m and sum s.  Called by `lanes` together (lane: which of its row's); `write`: the first of
+// these lanes stores the row's results.  Returns (c, c (1 / s)) to the first lane: the gradient is
+// c * (j == a) - c (1 / s) * 2^(x[j] k - m k).
+template <RowMode MODE>
+__device__ __forceinline__ float2 row_result(const RowArgs &A, int64_t row, const RowFacts &f, float m, float s, int lane, unsigned lanes, bool write)
+{
+    float c = 0.0f;
+    if constexpr (MODE == kGrad) {
+        c = (A.coef ? A.coef[(unsigned)row / (unsigned)A.coef_len] : 1.0f) * (A.upstream_rows ? A.upstream[row] : A.upstream[0]) * A.scale;
+    } else {
+        const double gap = (double)(f.xa - m) * (double)A.scale;
+        write = write && lane == 0;
+        if (write && A.stats) A.stats[row] = make_float2(m, s);
+        if constexpr (MODE == kLogProb) {
+            if (write) A.logp[row] = (float)(gap - Soft::log_sum(m, s, A.k));
+        } else {
+            // the first lane's is the ratio's exponential, the second's the KL term's
+            const double e = exp(lane == 0 ? gap - (double)f.old_lp : (double)f.ref_lp - gap);
+            const double off = Soft::rounding(m, A.k), sum = (double)s * (1.0 + off + 0.5 * off * off);      // off < 1e-5, or s is 0
+            const double kl = A.ref_lp ? A.kl * (__shfl_down_sync(lanes, e, 1) * sum - 1.0) : 0.0;
+            c = (float)(f.share * (clipped(A, e / sum, f.gain).y - kl));
+            if (write) {
+                A.gap[row] = gap;
+                A.coef[row] = c;
+            }
+            c = c * 1.0f * A.scale;          // in the order of kGrad with an upstream of one: the same bits
+        }
+    }
+    if (f.a < 0) c = NAN;
+    return make_float2(c, c * (1.0f / s));
+}
+
+template <RowMode MODE>
+__device__ __forceinline__ void masked_row(const RowArgs &A, int64_t row)
+{
+    if (MODE == kLogProb) A.logp[row] = 0.0f;
+    if (MODE != kGrad && A.stats) A.stats[row] = make_float2(0.0f, 0.0f);
+    if (MODE == kPolicy) A.coef[row] = 0.0f;
 }
 
 // ------------------------------------------------------------------------------------------- short rows
@@ -158,6 +317,7 @@ template <typename T, RowMode MODE, int G>
 __global__ void __launch_bounds__(256) rows_short_kernel(RowArgs A)
 {
     if (MODE == kGrad && A.only_if_not_one && A.upstream[0] == 1.0f) return;
+    if (MODE == kPolicy && blockIdx.x == 0 && threadIdx.x == 0) *A.arrived = 0;
     const int lane = threadIdx.x % G;
     const int64_t step = (int64_t)gridDim.x * (256 / G);
     for (int64_t row0 = (int64_t)blockIdx.x * (256 / G); row0 < A.rows; row0 += step) {
@@ -165,118 +325,122 @@ __global__ void __launch_bounds__(256) rows_short_kernel(RowArgs A)
         const bool there = row < A.rows, live = there && !(A.mask && !A.mask[row]);
         const T *x = (const T *)A.logits + (live ? row : 0) * A.stride;
         T *g = A.grad && there ? (T *)A.grad + row * (int64_t)A.V : nullptr;
+        RowFacts f = {};
+        f.a = -1;
+        if (live) f = row_facts<MODE>(A, row, x, A.action[row]);
         Soft soft;
         if (MODE != kGrad) {
             if (live)
                 for (int j = lane; j < A.V; j += G) {
-                    const T v[1] = {x[j]};
+                    const float v[1] = {to_f(x[j])};
                     soft.add(v, A.k);
                 }
-#pragma unroll
-            for (int o = G / 2; o > 0; o >>= 1) {
-                const float om = __shfl_xor_sync(0xffffffffu, soft.m, o), os = __shfl_xor_sync(0xffffffffu, soft.s, o);
-                soft.join(om, os, A.k);
-            }
+            __syncwarp();
+            soft.meet<G>(A.k);
         } else if (live) {
             const float2 st = A.stats[row];
             soft.m = st.x;
             soft.s = st.y;
         }
-        int a = -1;
-        float2 c = make_float2(0.0f, 0.0f);
-        if (live) {
-            const float xa = chosen(A, row, x, a);
-            if (lane == 0) {
-                c = row_result<MODE>(A, row, soft.m, soft.s, xa, true);
-                if (a < 0) c.x = c.y = NAN;
-            }
-        } else if (there && lane == 0) {
-            masked_row<MODE>(A, row);
-        }
+        __syncwarp();
+        float2 c = row_result<MODE>(A, live ? row : 0, f, soft.m, soft.s, lane, 0xffffffffu, live);
+        if (!live && there && lane == 0) masked_row<MODE>(A, row);
         c.x = __shfl_sync(0xffffffffu, c.x, 0, G);
         c.y = __shfl_sync(0xffffffffu, c.y, 0, G);
         if (g)
             for (int j = lane; j < A.V; j += G)
-                g[j] = from_f<T>(live ? (j == a ? c.x : 0.0f) - c.y * exp2f((to_f(x[j]) - soft.m) * A.k) : 0.0f);
+                g[j] = from_f<T>(live ? fmaf(-c.y, Soft::power(to_f(x[j]), soft.m, Soft::shift(soft.m, A.k), A.k), j == f.a ? c.x : 0.0f) : 0.0f);
     }
 }
 
 // -------------------------------------------------------------------------------------------- long rows
-// A cluster of CTAs per row (often of one); each has its own stretch of the row, cut at 16-byte boundaries.
+// A CTA per row, or a cluster of them; each has its own stretch of the row, cut at 16-byte boundaries.
 template <typename T, RowMode MODE, bool KEEP>
-__global__ void __launch_bounds__(512) rows_long_kernel(RowArgs A)
+__global__ void __launch_bounds__(512, 2) rows_long_kernel(RowArgs A)
 {
-    constexpr int N = Piece<T>::N;
+    using P = Piece<T>;
+    constexpr int N = P::N;
     extern __shared__ __align__(16) unsigned char kept_bytes[];
-    Piece<T> *kept = (Piece<T> *)kept_bytes;
-    __shared__ float2 part[32];
-    __shared__ float2 whole[2];          // this CTA's maximum and sum, by the row's parity
+    uint4 *kept = (uint4 *)kept_bytes;
+    __shared__ float2 part[16];          // the warps' maxima and sums
+    __shared__ float2 whole[2];          // this CTA's, by the row's parity: the others of a cluster may read the one before
     __shared__ float4 result;
     if (MODE == kGrad && A.only_if_not_one && A.upstream[0] == 1.0f) return;
+    if (MODE == kPolicy && blockIdx.x == 0 && threadIdx.x == 0) *A.arrived = 0;
     cg::cluster_group cluster = cg::this_cluster();
     const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, warp = tid >> 5;
+    // a row each; or, where that costs less than more CTAs (launch_rows), several
     int parity = 0;
-    for (int64_t row = blockIdx.x / C; row < A.rows; row += gridDim.x / C, parity ^= 1) {
+    for (int64_t row = blockIdx.x / C; row < A.rows; row += gridDim.x / C) {
         const T *x = (const T *)A.logits + row * A.stride;
         T *g = A.grad ? (T *)A.grad + row * (int64_t)A.V : nullptr;
-        const bool live = !(A.mask && !A.mask[row]);
         // the 16-byte pieces of the row, and the elements before and behind them
         const int head = min(A.V, (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T));
         const int pieces = (A.V - head) / N, per = (pieces + C - 1) / C;
         const int p0 = min(rank * per, pieces), p1 = min(p0 + per, pieces);
         const int tail0 = head + pieces * N;
-        const Piece<T> *xp = (const Piece<T> *)(x + head);
-        if (!live) {
+        const uint4 *xp = (const uint4 *)(x + head);
+        uint4 *gp = (uint4 *)(g + head);
+        const bool wide = ((uintptr_t)gp & 15) == 0;
+        const bool has_head = rank == 0 && tid < head, has_tail = rank == C - 1 && tail0 + tid < A.V;
+        // a piece of the gradient: as one if it lies like the logits, else element by element
+        const auto store = [&](int p, const float (&f)[N]) {
+            if (wide) {
+                gp[p] = P::close(f);
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; ++i) g[head + p * N + i] = from_f<T>(f[i]);
+            }
+        };
+        const int64_t action = A.action[row];           // on its way while the mask is
+        if (A.mask && !A.mask[row]) {
             if (rank == 0 && tid == 0) masked_row<MODE>(A, row);
             if (g) {
-                if (rank == 0 && tid < head) g[tid] = from_f<T>(0.0f);
-                if (rank == C - 1 && tail0 + tid < A.V) g[tail0 + tid] = from_f<T>(0.0f);
-                const bool wide = ((uintptr_t)(g + head) & 15) == 0;
-                Piece<T> zero;
-#pragma unroll
-                for (int i = 0; i < N; ++i) zero.v[i] = from_f<T>(0.0f);
-                for (int p = p0 + tid; p < p1; p += threads) {
-                    if (wide) ((Piece<T> *)(g + head))[p] = zero;
-                    else
-#pragma unroll
-                        for (int i = 0; i < N; ++i) g[head + p * N + i] = zero.v[i];
-                }
+                const float zero[N] = {};
+                for (int p = p0 + tid; p < p1; p += threads) store(p, zero);
+                if (has_head) g[tid] = from_f<T>(0.0f);
+                if (has_tail) g[tail0 + tid] = from_f<T>(0.0f);
             }
-            parity ^= 1;      // no exchange in this row
-            continue;
+            continue;                        // the whole cluster
         }
+        RowFacts f = {};
+        if (warp == 0) f = row_facts<MODE>(A, row, x, action);
         Soft soft;
         if (MODE != kGrad) {
             int p = p0 + tid;
-            for (; p + 3 * threads < p1; p += 4 * threads) {
-                Piece<T> v[4];
+            for (; p + 7 * threads < p1; p += 8 * threads) {
+                uint4 v[8];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = xp[p + i * threads];
+                for (int i = 0; i < 8; ++i) v[i] = xp[p + i * threads];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < 8; ++i)
                     if (KEEP) kept[p - p0 + i * threads] = v[i];
-                    soft.add(v[i].v, A.k);
+                soft.template add<T>(v, A.k);
+            }
+            for (; p + threads < p1; p += 2 * threads) {
+                const uint4 v[2] = {xp[p], xp[p + threads]};
+                if (KEEP) {
+                    kept[p - p0] = v[0];
+                    kept[p - p0 + threads] = v[1];
                 }
+                soft.template add<T>(v, A.k);
             }
-            for (; p < p1; p += threads) {
-                const Piece<T> v = xp[p];
-                if (KEEP) kept[p - p0] = v;
-                soft.add(v.v, A.k);
+            if (p < p1) {
+                const uint4 v[1] = {xp[p]};
+                if (KEEP) kept[p - p0] = v[0];
+                soft.template add<T>(v, A.k);
             }
-            if (rank == 0 && tid < head) {
-                const T v[1] = {x[tid]};
+            if (has_head) {
+                const float v[1] = {to_f(x[tid])};
                 soft.add(v, A.k);
             }
-            if (rank == C - 1 && tail0 + tid < A.V) {
-                const T v[1] = {x[tail0 + tid]};
+            if (has_tail) {
+                const float v[1] = {to_f(x[tail0 + tid])};
                 soft.add(v, A.k);
             }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                const float om = __shfl_xor_sync(0xffffffffu, soft.m, o), os = __shfl_xor_sync(0xffffffffu, soft.s, o);
-                soft.join(om, os, A.k);
-            }
+            __syncwarp();
+            soft.meet<32>(A.k);
             if (lane == 0) part[warp] = make_float2(soft.m, soft.s);
             __syncthreads();
             if (warp == 0) {
@@ -285,62 +449,55 @@ __global__ void __launch_bounds__(512) rows_long_kernel(RowArgs A)
                     soft.m = part[lane].x;
                     soft.s = part[lane].y;
                 }
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) {
-                    const float om = __shfl_xor_sync(0xffffffffu, soft.m, o), os = __shfl_xor_sync(0xffffffffu, soft.s, o);
-                    soft.join(om, os, A.k);
-                }
-                if (lane == 0) whole[parity] = make_float2(soft.m, soft.s);
+                soft.meet<16>(A.k);
             }
             if (C > 1) {
+                if (tid == 0) whole[parity] = make_float2(soft.m, soft.s);
                 cluster.sync();
                 if (warp == 0) {
                     soft = Soft();
-                    for (int r = 0; r < C; ++r) {
-                        const float2 o = *cluster.map_shared_rank(&whole[parity], r);
-                        soft.join(o.x, o.y, A.k);
+                    if (lane < C) {
+                        const float2 o = *cluster.map_shared_rank(&whole[parity], lane);
+                        soft.m = o.x;
+                        soft.s = o.y;
                     }
+                    soft.meet<8>(A.k);
                 }
+                parity ^= 1;
             }
+        } else if (warp == 0) {
+            const float2 st = A.stats[row];
+            soft.m = st.x;
+            soft.s = st.y;
         }
-        if (tid == 0) {
-            int a;
-            const float xa = chosen(A, row, x, a);
-            if (MODE == kGrad) {
-                const float2 st = A.stats[row];
-                soft.m = st.x;
-                soft.s = st.y;
-            }
-            float2 c = make_float2(0.0f, 0.0f);
-            if (rank == 0 || g) {
-                c = row_result<MODE>(A, row, soft.m, soft.s, xa, rank == 0);    // the other CTAs need the coefficients too
-                if (a < 0) c.x = c.y = NAN;
-            }
-            result = make_float4(c.x, c.y, soft.m, __int_as_float(a));
+        if (warp == 0 && lane < 2) {
+            const float2 c = row_result<MODE>(A, row, f, soft.m, soft.s, lane, 3u, rank == 0);
+            if (lane == 0) result = make_float4(c.x, c.y, soft.m, __int_as_float(f.a));
         }
         if (g) {
             __syncthreads();
-            const float cx = result.x, cs = result.y, m = result.z;
+            const float cx = result.x, cs = result.y, m = result.z, shift = Soft::shift(m, A.k);
             const int a = __float_as_int(result.w);
-            auto value = [&](T v, int j) { return from_f<T>((j == a ? cx : 0.0f) - cs * exp2f((to_f(v) - m) * A.k)); };
-            if (rank == 0 && tid < head) g[tid] = value(x[tid], tid);
-            if (rank == C - 1 && tail0 + tid < A.V) g[tail0 + tid] = value(x[tail0 + tid], tail0 + tid);
-            const bool wide = ((uintptr_t)(g + head) & 15) == 0;
+            const auto value = [&](float v, float chosen) { return fmaf(-cs, Soft::power(v, m, shift, A.k), chosen); };
             for (int p = p0 + tid; p < p1; p += threads) {
-                const Piece<T> v = KEEP ? kept[p - p0] : xp[p];
-                const int j = head + p * N;
-                if (wide) {
-                    Piece<T> o;
+                float e[N];
+                P::open(e, KEEP ? kept[p - p0] : xp[p]);
+                if (Soft::huge(m)) {
 #pragma unroll
-                    for (int i = 0; i < N; ++i) o.v[i] = value(v.v[i], j + i);
-                    ((Piece<T> *)(g + head))[p] = o;
+                    for (int i = 0; i < N; ++i) e[i] = value(e[i], 0.0f);
                 } else {
 #pragma unroll
-                    for (int i = 0; i < N; ++i) g[j + i] = value(v.v[i], j + i);
+                    for (int i = 0; i < N; ++i) e[i] = -cs * two_to(fmaf(e[i], A.k, -shift));
                 }
+                store(p, e);
             }
+            // the chosen entry, behind its piece's own store
+            const int pa = (a - head) / N;
+            if (a >= head && pa >= p0 && pa < p1 && (pa - p0) % threads == tid) g[a] = from_f<T>(value(to_f(x[a]), cx));
+            if (has_head) g[tid] = from_f<T>(value(to_f(x[tid]), tid == a ? cx : 0.0f));
+            if (has_tail) g[tail0 + tid] = from_f<T>(value(to_f(x[tail0 + tid]), tail0 + tid == a ? cx : 0.0f));
         }
-        __syncthreads();                 // part, result
+        if (gridDim.x < A.rows * C) __syncthreads();
     }
     if (C > 1) cluster.sync();           // no CTA leaves while another reads its sums
 }
@@ -357,21 +514,28 @@ int launch_rows(const RowArgs &A, cudaStream_t stream)
         else rows_short_kernel<T, MODE, 32><<<grid, 256, 0, stream>>>(A);
         return check_launch("rows kernel launch");
     }
-    const int threads = A.V <= 8192 ? 256 : 512;
-    // CTAs per row: until the row's stretch fits the shared memory kept for it, and while there are SMs without one
-    const size_t most = 100 * 1024;
-    const size_t bytes = ((size_t)A.V * sizeof(T) + 15) / 16 * 16;
+    const size_t bytes = ((size_t)A.V * sizeof(T) + 15) / 16 * 16, most = 100 * 1024;
+    // us with 128 / 256 / 512 threads (value and gradient): 4096 x 32768 bfloat16 160 / 123 / 127, 1505 x 50021 float32 182 / 149 / 142
+    const int threads = bytes <= 4096 ? 128 : bytes <= 80 * 1024 ? 256 : 512;
+    // CTAs per row: while there are SMs without one.  (A row that is too long for the shared memory kept for it is read again, out
+    // of the L2 cache: 1505 x 50021 float32 141 us, cut in two to be kept 158.)
     int C = 1;
-    while (C < 8 && (ceil_div(bytes, C) > (int64_t)most || (A.rows * C * 2 <= sms && (size_t)A.V / C > 8192))) C *= 2;
+    while (C < 8 && A.rows * C * 2 <= sms && (size_t)A.V / C > 8192) C *= 2;
+    if (A.rows * C > 0x7fffffff) {
+        set_error("%lld rows of %d entries", (long long)A.rows, A.V);
+        return SLAYER_B200_EUNSUPPORTED;
+    }
     const int64_t stretch = (ceil_div(bytes / 16, C) + 1) * 16;
     const bool keep = MODE == kPolicy && A.grad && stretch <= (int64_t)most;
     const size_t smem = keep ? (size_t)stretch : 0;
     auto kern = keep ? rows_long_kernel<T, MODE, MODE == kPolicy> : rows_long_kernel<T, MODE, false>;
     int rc = reserve_dynamic_smem((const void *)kern, smem);
     if (rc) return rc;
-    const int64_t cap = sms * (threads == 256 ? 8 : 4) / C;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((A.rows < cap ? A.rows : cap) * C));
+    // a row each: with rows dealt out to resident CTAs, masked rows make some end early (4096 x 32768 bfloat16, a third of the rows
+    // masked, 128 us, as it is 116).  A gradient that may be there already should be told so to few CTAs.
+    const int64_t cap = sms * 8 / C;
+    cfg.gridDim = dim3((unsigned)((MODE == kGrad && A.only_if_not_one && A.rows > cap ? cap : A.rows) * C));
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
@@ -422,13 +586,40 @@ __global__ void __launch_bounds__(256) count_kernel(int *counts, const uint8_t *
     if (threadIdx.x == 0) counts[blockIdx.x] = n;
 }
 
-__global__ void __launch_bounds__(1024) sum_kernel(float *out, const double *v, int64_t n)
+// The loss, and the rows' log-probabilities: a thread has a row, the last CTA to come adds up the CTAs' sums in their order.
+__global__ void __launch_bounds__(256) policy_sum_kernel(RowArgs A, float *loss, double *sums, unsigned *arrived)
 {
     __shared__ double part[32];
-    double s = 0.0;
-    for (int64_t i = threadIdx.x; i < n; i += blockDim.x) s += v[i];
-    s = block_sum(s, part);
-    if (threadIdx.x == 0) *out = (float)s;
+    __shared__ bool last;
+    double total = 0.0;
+    for (int64_t row = blockIdx.x * 256ll + threadIdx.x; row < A.rows; row += gridDim.x * 256ll) {
+        if (A.mask && !A.mask[row]) {
+            if (A.logp) A.logp[row] = 0.0f;
+            continue;
+        }
+        const float2 st = A.stats[row];
+        const double lp = A.gap[row] - Soft::log_sum(st.x, st.y, A.k);
+        if (A.logp) A.logp[row] = (float)lp;
+        double per = clipped(A, exp(lp - (double)A.old_lp[row]), A.advantage[(unsigned)row / (unsigned)A.adv_len]).x;
+        if (A.ref_lp) {
+            const double d = (double)A.ref_lp[row] - lp;
+            per += A.kl * (expm1(d) - d);
+        }
+        total += row_share(A, row) * per;
+    }
+    total = block_sum(total, part);
+    if (threadIdx.x == 0) {
+        sums[blockIdx.x] = total;
+        __threadfence();
+        last = atomicAdd(arrived, 1u) == gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    total = 0.0;
+    for (int i = threadIdx.x; i < (int)gridDim.x; i += 256) total += __ldcg(sums + i);
+    total = block_sum(total, part);
+    if (threadIdx.x == 0) *loss = (float)total;
 }
 
 // margin[s] = sum of a sequence's log-probabilities (masked ones are 0) - ref[s]
@@ -486,8 +677,8 @@ static int check_rows(const char *what, int dtype, int64_t rows, int64_t V, int6
     SB200_REQUIRE(dtype == SLAYER_B200_F32 || dtype == SLAYER_B200_BF16 || dtype == SLAYER_B200_F16, "%s: unknown type %d", what, dtype);
     SB200_REQUIRE(rows >= 0 && V >= 1 && stride >= 0, "%s: bad size", what);
     SB200_REQUIRE(scale > 0.0 && scale < INFINITY, "%s: scale must be positive and finite", what);
-    if (V > (1 << 30)) {
-        set_error("%s: rows of %lld entries", what, (long long)V);
+    if (V > (1 << 30) || rows > 0x7fffffff) {
+        set_error("%s: %lld rows of %lld entries", what, (long long)rows, (long long)V);
         return SLAYER_B200_EUNSUPPORTED;
     }
     return SLAYER_B200_OK;
@@ -550,7 +741,8 @@ extern "C" int slayer_b200_logit_grad(void *grad, const void *logits, int dtype,
 
 extern "C" int64_t slayer_b200_policy_loss_workspace(int64_t rows, int64_t seq_len)
 {
-    return rows < 0 ? 0 : 8 * rows + 4 * (seq_len > 0 ? ceil_div(rows, seq_len) : 0) + 16;
+    // what the sum does not give of each row, sums of the loss, a count, the sequences' counts
+    return rows < 0 ? 0 : 8 * rows + 8 * kSums + 8 + 4 * (seq_len > 0 ? ceil_div(rows, seq_len) : 0);
 }
 
 extern "C" int slayer_b200_policy_loss(float *loss, void *grad, float *logp, float *stats, float *coef, void *workspace,
@@ -571,7 +763,7 @@ extern "C" int slayer_b200_policy_loss(float *loss, void *grad, float *logp, flo
         if (cudaMemsetAsync(loss, 0, sizeof(float), (cudaStream_t)stream) != cudaSuccess) return check_launch("policy_loss");
         return SLAYER_B200_OK;
     }
-    SB200_REQUIRE(coef && workspace && logits && action && old_logp && advantage, "policy_loss: null pointer");
+    SB200_REQUIRE(coef && stats && workspace && logits && action && old_logp && advantage, "policy_loss: null pointer");
     SB200_REQUIRE(grad != logits, "policy_loss: grad must not alias logits");
     SB200_REQUIRE(((uintptr_t)workspace & 7) == 0, "policy_loss: the workspace must be aligned to 8 bytes");
     const cudaStream_t st = (cudaStream_t)stream;
@@ -587,12 +779,15 @@ extern "C" int slayer_b200_policy_loss(float *loss, void *grad, float *logp, flo
     A.kl = kl;
     A.coef = coef;
     A.coef_len = 1;
-    A.row_loss = (double *)workspace;
+    A.gap = (double *)workspace;
+    double *sums = A.gap + rows;
+    unsigned *arrived = (unsigned *)(sums + kSums);
+    A.arrived = arrived;
     A.grad = grad;
     const int64_t len = reduction == SLAYER_B200_MEAN ? rows : seq_len;
     A.share = reduction == SLAYER_B200_SUM ? 1.0 : 1.0 / (double)rows;     // without a mask all sequences are equally long
     if (reduction != SLAYER_B200_SUM && mask) {
-        int *counts = (int *)(A.row_loss + rows);
+        int *counts = (int *)(arrived + 2);
         SB200_REQUIRE(rows / len <= 0x7fffffff, "policy_loss: too many sequences");
         count_kernel<<<(unsigned)(rows / len), 256, 0, st>>>(counts, mask, len);
         rc = check_launch("count kernel launch");
@@ -603,8 +798,9 @@ extern "C" int slayer_b200_policy_loss(float *loss, void *grad, float *logp, flo
     }
     rc = launch_rows<kPolicy>(dtype, A, st);
     if (rc) return rc;
-    sum_kernel<<<1, 1024, 0, st>>>(loss, A.row_loss, rows);
-    return check_launch("sum kernel launch");
+    const int64_t blocks = ceil_div(rows, 256);
+    policy_sum_kernel<<<(unsigned)(blocks < kSums ? blocks : kSums), 256, 0, st>>>(A, loss, sums, arrived);
+    return check_launch("policy sum kernel launch");
 }
 
 extern "C" int64_t slayer_b200_preference_loss_workspace(int64_t sequences) { return sequences < 0 ? 0 : 8 * sequences + 8; }

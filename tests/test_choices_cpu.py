@@ -82,10 +82,10 @@ def test_c_entries_check_their_arguments():
     assert lp(V=1 << 31) == -3
     assert lp(rows=0, logits=null) == 0
     pl = lambda **k: lib.slayer_b200_policy_loss(*{**dict(  # noqa: E731
-        loss=p, grad=null, logp=null, stats=null, coef=p, workspace=p, logits=q, dtype=0, action=p, old=p, adv=p, adv_len=1, ref=null, mask=null,
+        loss=p, grad=null, logp=null, stats=p, coef=p, workspace=p, logits=q, dtype=0, action=p, old=p, adv=p, adv_len=1, ref=null, mask=null,
         rows=6, seq_len=3, V=5, stride=5, scale=1.0, lo=0.2, hi=0.2, kl=0.0, reduction=0, stream=null), **k}.values())
     for bad in (dict(loss=null), dict(lo=-0.1), dict(hi=float("nan")), dict(reduction=3), dict(adv_len=0), dict(seq_len=4), dict(seq_len=0),
-                dict(workspace=ctypes.c_void_p(12)), dict(grad=q), dict(coef=null), dict(old=null)):
+                dict(workspace=ctypes.c_void_p(12)), dict(grad=q), dict(coef=null), dict(old=null), dict(stats=null)):
         assert pl(**bad) == -1, bad
     lg = lambda **k: lib.slayer_b200_logit_grad(*{**dict(  # noqa: E731
         grad=p, logits=q, dtype=0, action=p, mask=null, stats=p, coef=null, coef_len=1, up=p, up_rows=0, only=0, rows=2, V=5, stride=5, scale=1.0,

@@ -193,6 +193,33 @@ def test_policy_loss_and_gradient(S, L, V, kl, masked, dtype, reduction):
     close(scaled, grad * 8.0, spare * 8.0)
 
 
+@pytest.mark.parametrize("dtype,V", [(torch.float32, 9001), (torch.float32, 70001), (torch.bfloat16, 20003), (torch.float16, 120001), (torch.bfloat16, 40000)])
+@pytest.mark.parametrize("masked", [True, False])
+def test_policy_many_long_rows(dtype, V, masked):
+    """Enough rows for the walk over them, in one CTA and in clusters, rows that start anywhere."""
+    S, L = 40, 9
+    x, action, old, adv, ref, mask = policy_case(S, L, V, dtype, V, True, masked)
+    x64 = x.cuda().double()
+    leaf = x.cuda().requires_grad_()
+    dev = [t if t is None else t.cuda() for t in (action, old, adv, ref, mask)]
+    for want in (True, False):
+        with torch.set_grad_enabled(want):
+            got, lp = loss.policyLoss(leaf, dev[0], dev[1], dev[2], refLogProb=dev[3], mask=dev[4], clip=CLIP, klCoef=0.3, scale=0.9, reduction="mean",
+                                      returnLogProb=True)
+        value, slack, coef, size = policy_want(x64, dev[0], dev[1], dev[2], dev[3], dev[4] if masked else torch.ones(S, L, device="cuda").bool(), 0.3, "mean")
+        assert abs(float(got.detach()) - float(value)) <= float(slack) + 2 ** -24 * abs(float(value)) + 1e-30
+        keep = torch.ones(S, L, dtype=torch.bool) if mask is None else mask
+        close(lp, torch.where(keep, want_logp(x64, dev[0], 0.9).cpu(), 0.0), SUM)
+    got = loss.policyLoss(leaf, dev[0], dev[1], dev[2], refLogProb=dev[3], mask=dev[4], clip=CLIP, klCoef=0.3, scale=0.9, reduction="mean")
+    (g,) = torch.autograd.grad(got, [leaf], retain_graph=True)
+    (again,) = torch.autograd.grad(got, [leaf])
+    assert torch.equal(g, again)
+    for s in range(0, S, 13):
+        grad, spare = want_grad(x64[s], dev[0][s], coef[s], 0.9)
+        spare = spare + 0.9 * (size[s] * SUM)[..., None] * (grad / torch.where(coef[s] == 0, 1.0, coef[s] * 0.9)[..., None]).abs()
+        close(g[s], grad.cpu(), spare.cpu())
+
+
 @pytest.mark.parametrize("V", [12, 3001])
 def test_policy_advantage_of_a_whole_sequence_and_first_backward_scaled(V):
     x, action, old, adv, ref, mask = policy_case(6, 5, V, torch.float32, 11)
