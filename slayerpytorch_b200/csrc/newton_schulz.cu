@@ -253,16 +253,22 @@ __global__ void __launch_bounds__(256) ns_normalise_kernel(const __grid_constant
 // ------------------------------------------------------------------------------------------------ products
 enum NsPhase { kGram, kPolynomial, kUpdate };
 
-constexpr int kNsThreads = 384;      // a warp that loads, one that issues products, two to fill up; eight that take the results
 
-// CG = 1: a CTA makes tiles of 128 x 128.  CG = 2: two CTAs make tiles of 256 x 256 together, each with half of either operand, so
+// MODE kAlone: a CTA makes tiles of 128 x 128.  kShared: so, and where there are few tiles several CTAs share one.  kPair: two CTAs make tiles of 256 x 256 together, each with half of either operand, so
 // that a CTA loads as much per step for four times the products of a pair.
-template <int PARTS, int CG>
+enum NsMode { kAlone, kShared, kPair };
+
+template <int PARTS, int MODE>
 struct NsTile {
+    static constexpr int CG = MODE == kPair ? 2 : 1;
     static constexpr int TN = 128 * CG;                      // columns of the result, of which each CTA has 128 rows
     static constexpr int kA = PARTS * kBlock, kB = PARTS * kBlock, kStage = kA + kB;
-    static constexpr int kPiece = 32 * 33 * 4;               // a 32 x 32 piece of each of the eight warps
-    static constexpr int kFixed = 1024 + 512 + 8 * kPiece;
+    // a warp that loads, one that issues products, two to fill up; and those that take the results
+    static constexpr int kTakers = 8, kThreads = 128 + 32 * kTakers;
+    static constexpr int kWide = TN / (kTakers / 4), kPieces = kWide / 32;       // columns of a warp's 32 rows, pieces
+    static constexpr int kPiece = 32 * 33 * 4;               // a 32 x 32 piece of each of these warps
+    static constexpr int kExchange = MODE == kShared ? 128 * 128 * 4 : 0;          // the sums of those that share a tile
+    static constexpr int kFixed = 1024 + 512 + kTakers * kPiece + kExchange;
     static constexpr int kStages = (227 * 1024 - kFixed) / kStage > 6 ? 6 : (227 * 1024 - kFixed) / kStage;
     static constexpr size_t kSmem = kFixed + (size_t)kStages * kStage;
     // Steps of 64 whose sum stays in tensor memory.  The tensor core cuts what it adds to a sum instead of rounding it: over the
@@ -276,10 +282,10 @@ struct NsTile {
 // without two lanes meeting in a bank.
 __device__ __forceinline__ int ns_piece_at(int row, int chunk) { return row * 64 + ((chunk ^ (row >> 1)) & 3) * 16; }
 
-__device__ __forceinline__ uint4 *ns_piece_line(unsigned char *block, int r0, int c0, int lane, int i)
+// (r0 is a multiple of 32: rows that lie eight apart have their chunks at the same places)
+__device__ __forceinline__ uint4 *ns_piece_line(unsigned char *block, int r0, int c0, int lane)
 {
-    const int r = r0 + i * 8 + (lane >> 2);
-    return (uint4 *)(block + (r & 127) * 128 + ((((c0 >> 3) & 7) + (lane & 3)) ^ (r & 7)) * 16);
+    return (uint4 *)(block + ((r0 & 96) + (lane >> 2)) * 128 + ((((c0 >> 3) & 4) + (lane & 3)) ^ (lane >> 2)) * 16);
 }
 
 // What the result is made of besides the product: of b, a; of x', x.
@@ -295,21 +301,22 @@ struct NsOld {
 #pragma unroll
         for (int p = 0; p < PARTS; ++p)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[p][i] = __ldcg(ns_piece_line(block + p * kBlock, r0, c, lane, i));
+            for (int i = 0; i < 4; ++i) v[p][i] = __ldcg(ns_piece_line(block, r0, c, lane) + (p * kBlock + i * 1024) / 16);
     }
     __device__ __forceinline__ void put(unsigned char *piece, int lane) const
     {
 #pragma unroll
         for (int p = 0; p < PARTS; ++p)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) *(uint4 *)(piece + p * 2048 + ns_piece_at(i * 8 + (lane >> 2), lane & 3)) = v[p][i];
+            for (int i = 0; i < 4; ++i) *(uint4 *)(piece + ns_piece_at(lane >> 2, lane & 3) + p * 2048 + i * 512) = v[p][i];
     }
 };
 
-// What a warp does with 32 rows (from r0, lane = row) x 32 columns (from c) of a result.
+// What a warp does with 32 rows (from r0, lane = row) x 32 columns (from c) of a result.  next: the columns of the piece that
+// follows, whose old values are requested meanwhile, or -1.
 template <int PARTS, typename T>
 __device__ __forceinline__ void ns_take_piece(const NsArgs &A, const NsJob &J, int kind, bool last, int from, int r0, int c, float (&v)[32],
-                                              unsigned char *piece, int lane, const NsOld<PARTS> &old)
+                                              unsigned char *piece, int lane, NsOld<PARTS> &old, int next)
 {
     if (kind == kGram) {
 #pragma unroll
@@ -320,6 +327,7 @@ __device__ __forceinline__ void ns_take_piece(const NsArgs &A, const NsJob &J, i
         __syncwarp();
         old.put(piece, lane);
         __syncwarp();
+        if (next >= 0) old.request(J, kind, from, r0, next, lane);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const uint4 hi = *(const uint4 *)(piece + ns_piece_at(lane, k));
@@ -385,7 +393,7 @@ __device__ __forceinline__ void ns_take_piece(const NsArgs &A, const NsJob &J, i
         for (int p = 0; p < PARTS; ++p)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                *ns_piece_line(to + p * kBlock, r0, c, lane, i) = *(const uint4 *)(piece + p * 2048 + ns_piece_at(i * 8 + (lane >> 2), lane & 3));
+                ns_piece_line(to, r0, c, lane)[(p * kBlock + i * 1024) / 16] = *(const uint4 *)(piece + ns_piece_at(lane >> 2, lane & 3) + p * 2048 + i * 512);
     }
 }
 
@@ -398,7 +406,7 @@ __device__ __forceinline__ void ns_take_piece(const NsArgs &A, const NsJob &J, i
 // a and b are symmetric: their blocks below the diagonal are neither computed nor stored.  Where a product wants one as
 // rows, it takes the block across the diagonal as columns.
 //
-// With CG = 1 and few tiles, split[phase] CTAs of a cluster share a tile: each sums over its part of the steps of the summation
+// In mode kShared split[phase] CTAs of a cluster share a tile: each sums over its part of the steps of the summation
 // index, they exchange the sums through shared memory, and each takes some 32 x 32 pieces of the total, added up in the order
 // of the ranks.
 struct NsPlan {
@@ -408,11 +416,11 @@ struct NsPlan {
     int *status;
 };
 
-template <int PARTS, int CG, typename T>
-__global__ void __launch_bounds__(kNsThreads, 1) ns_steps_kernel(const __grid_constant__ NsArgs A, const __grid_constant__ NsPlan P)
+template <int PARTS, int MODE, typename T>
+__global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_kernel(const __grid_constant__ NsArgs A, const __grid_constant__ NsPlan P)
 {
-    using Tile = NsTile<PARTS, CG>;
-    constexpr int S = Tile::kStages, TN = Tile::TN;
+    using Tile = NsTile<PARTS, MODE>;
+    constexpr int CG = Tile::CG, S = Tile::kStages, TN = Tile::TN, kTakers = Tile::kTakers, kPieces = Tile::kPieces;
     extern __shared__ unsigned char smem_raw[];
     unsigned char *smem = (unsigned char *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     // full: this CTA's loads are there; ready: the second CTA's are (at the first); empty: a stage has been read; done: a sum is
@@ -420,7 +428,7 @@ __global__ void __launch_bounds__(kNsThreads, 1) ns_steps_kernel(const __grid_co
     uint64_t *full = (uint64_t *)(smem + S * Tile::kStage), *ready = full + S, *empty = ready + S, *done = empty + S, *taken = done + 2;
     uint64_t *given = taken + 2;
     uint32_t *base_at = (uint32_t *)(given + 3);
-    unsigned char *pieces = smem + S * Tile::kStage + 512;
+    unsigned char *pieces = smem + S * Tile::kStage + 512, *exchange = pieces + kTakers * Tile::kPiece;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)cluster_rank(), pair = CG == 2 ? rank : 0;
     const bool clustered = cluster_size() > 1;
@@ -433,9 +441,9 @@ __global__ void __launch_bounds__(kNsThreads, 1) ns_steps_kernel(const __grid_co
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(done + i, 1);
-            mbar_init(taken + i, 8 * CG);
+            mbar_init(taken + i, kTakers * CG);
         }
-        for (int i = 0; i < 3; ++i) mbar_init(given + i, 8 * P.split[i]);
+        for (int i = 0; i < 3; ++i) mbar_init(given + i, kTakers * P.split[i]);
         mbar_init_fence();
     }
     tensor_fence_before();
@@ -492,6 +500,23 @@ __global__ void __launch_bounds__(kNsThreads, 1) ns_steps_kernel(const __grid_co
         o.k1 = steps * (p.rank + 1) / p.split;
         return o;
     };
+    // Most matrices give a CTA one tile a phase, the same one in every step: worked out once (some 300 instructions one after the
+    // other, which would stand between the phases).
+    __shared__ Phase phases[3];
+    __shared__ Spot firsts[3];
+    if (threadIdx.x < 3) {
+        const Phase p = phase_of(threadIdx.x);
+        phases[threadIdx.x] = p;
+        if (p.tile < p.tiles) firsts[threadIdx.x] = locate(p, p.tile);
+    }
+    __syncthreads();
+    auto phase_at = [&](int ph, int kind) {
+        Phase p = phases[kind];
+        p.from = ph / 3 & 1;
+        p.last = ph + 1 == 3 * P.steps;
+        return p;
+    };
+    auto spot_at = [&](const Phase &p, int tile) { return tile == p.tile ? firsts[p.kind] : locate(p, tile); };
     // whether step k takes an operand from across the diagonal (of the two row blocks of a pair, which take it alike, one may be the
     // diagonal's own, which is the same either way)
     auto left_turned = [&](int kind, int i, int k) { return kind != kGram && (k >> 1) < i + CG - 1; };
@@ -502,14 +527,14 @@ __global__ void __launch_bounds__(kNsThreads, 1) ns_steps_kernel(const __grid_co
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == 0 && lane == 0) {
             int s = 0, turn = 0;
-            for (int ph = 0; fine && ph < 3 * P.steps; ++ph) {
+            for (int ph = 0, kind = 0; fine && ph < 3 * P.steps; ++ph, kind = kind == 2 ? 0 : kind + 1) {
                 if (ph > 0) {
                     if (!grid_wait_bounded(P.arrived, ph * gridDim.x, kWaitLimit)) { fine = false; break; }
-                    fence_async_all();
+                    fence_async_global();
                 }
-                const Phase p = phase_of(ph);
+                const Phase p = phase_at(ph, kind);
                 for (int tile = p.tile; fine && tile < p.tiles; tile += p.step) {
-                    const Spot o = locate(p, tile);
+                    const Spot o = spot_at(p, tile);
                     const NsJob &J = *o.J;
                     const int cbm = ns_cb(J.m), cbn = ns_cb(J.n), rb = ns_rb(J.m);
                     const int cbl = p.kind == kGram ? cbn : cbm, cbr = p.kind == kPolynomial ? cbm : cbn;
@@ -549,10 +574,10 @@ __global__ void __launch_bounds__(kNsThreads, 1) ns_steps_kernel(const __grid_co
             }
         } else if (warp == 1 && lane == 0 && pair == 0) {
             int s = 0, turn = 0, slot = 0, again = 0;
-            for (int ph = 0; fine && ph < 3 * P.steps; ++ph) {
-                const Phase p = phase_of(ph);
+            for (int ph = 0, kind = 0; fine && ph < 3 * P.steps; ++ph, kind = kind == 2 ? 0 : kind + 1) {
+                const Phase p = phase_at(ph, kind);
                 for (int tile = p.tile; fine && tile < p.tiles; tile += p.step) {
-                    const Spot o = locate(p, tile);
+                    const Spot o = spot_at(p, tile);
                     for (int k = o.k0; k < o.k1; ++k) {
                         const bool first = (k - o.k0) % Tile::kGroup == 0;
                         if (first && !mbar_wait_bounded(taken + slot, again ^ 1, kWaitLimit)) { fine = false; break; }
@@ -587,10 +612,10 @@ __global__ void __launch_bounds__(kNsThreads, 1) ns_steps_kernel(const __grid_co
         } else if (CG == 2 && warp == 1 && lane == 0) {
             // the second CTA tells the first what it has loaded
             int s = 0, turn = 0;
-            for (int ph = 0; fine && ph < 3 * P.steps; ++ph) {
-                const Phase p = phase_of(ph);
+            for (int ph = 0, kind = 0; fine && ph < 3 * P.steps; ++ph, kind = kind == 2 ? 0 : kind + 1) {
+                const Phase p = phase_at(ph, kind);
                 for (int tile = p.tile; fine && tile < p.tiles; tile += p.step) {
-                    const Spot o = locate(p, tile);
+                    const Spot o = spot_at(p, tile);
                     for (int k = o.k0; k < o.k1; ++k) {
                         if (!mbar_wait_bounded(full + s, turn, kWaitLimit)) { fine = false; break; }
                         mbar_arrive_at(ready + s, 0);
@@ -603,41 +628,46 @@ __global__ void __launch_bounds__(kNsThreads, 1) ns_steps_kernel(const __grid_co
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         int slot = 0, again = 0;
-        const int w = warp - 4, quarter = warp & 3, half = w >> 2;
+        const int w = warp - 4, quarter = warp & 3;
         unsigned char *piece = pieces + w * Tile::kPiece;
-        for (int ph = 0; fine && ph < 3 * P.steps; ++ph) {
-            const Phase p = phase_of(ph);
+        for (int ph = 0, kind = 0; fine && ph < 3 * P.steps; ++ph, kind = kind == 2 ? 0 : kind + 1) {
+            const Phase p = phase_at(ph, kind);
             if (ph > 0) {
                 // what the phase before has left; and a CTA without a tile must not arrive before its time
                 if (lane == 0) fine = grid_wait_bounded(P.arrived, ph * gridDim.x, kWaitLimit);
                 fine = __all_sync(0xffffffffu, fine);
             }
             for (int tile = p.tile; fine && tile < p.tiles; tile += p.step) {
-                const Spot o = locate(p, tile);
+                const Spot o = spot_at(p, tile);
                 const NsJob &J = *o.J;
                 const int groups = (o.k1 - o.k0 + Tile::kGroup - 1) / Tile::kGroup, rb = ns_rb(J.m);
-                const int il = o.i + pair, c0 = half * (TN / 2), jl = o.j + (c0 >> 7);      // this warp's columns of the tile; its blocks
+                const int il = o.i + pair, c0 = (w >> 2) * Tile::kWide, jl = o.j + (c0 >> 7);      // this warp's columns of the tile; its blocks
                 const bool mine = il < rb && jl < (p.kind != kUpdate ? rb : ns_rb(J.n)) && !(p.kind != kUpdate && jl < il);
                 const int r0 = il * 128 + quarter * 32, c = o.j * 128 + c0;
                 const uint32_t at = acc + ((uint32_t)(quarter * 32) << 16) + c0;
-                float sum[PARTS == 2 ? TN / 64 : 1][32];
+                float sum[PARTS == 2 ? kPieces : 1][32];
                 if constexpr (PARTS == 2) {
 #pragma unroll
-                    for (int u = 0; u < TN / 64; ++u)
+                    for (int u = 0; u < kPieces; ++u)
 #pragma unroll
                         for (int k = 0; k < 32; ++k) sum[u][k] = 0.0f;
                 }
                 NsOld<PARTS> old;
-                if (mine && !(CG == 1 && p.split > 1)) old.request(J, p.kind, p.from, r0, c, lane);
-                // a whole piece: to the others that share the tile (four columns of all rows after one another), or to its end
-                auto pass_on = [&](float (&v)[32], int u) {
-                    if (CG == 1 && p.split > 1) {
-                        float4 *to = (float4 *)smem + ((c0 + u * 32) / 4) * 128 + quarter * 32 + lane;
+                if (mine && !(MODE == kShared && p.split > 1)) old.request(J, p.kind, p.from, r0, c, lane);
+                // To the one of those that share the tile whose piece it is: pieces rank, rank + split, ... of the sixteen, from every
+                // rank in turn.  (Written there, not fetched: a read of another CTA's memory takes 400 cycles, and the stores are
+                // on their way together.)
+                auto give = [&](const float (&v)[32], int u) {
+                    const int id = ((c0 >> 5) + u) * 4 + quarter, to = id & (p.split - 1);
+                    float4 *at = (float4 *)exchange + (p.rank * (16 / p.split) + id / p.split) * 256 + lane;
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) to[k * 128] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+                    for (int k = 0; k < 8; ++k) write_at(at + k * 32, rank - p.rank + to, make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]));
+                };
+                auto pass_on = [&](float (&v)[32], int u) {
+                    if (MODE == kShared && p.split > 1) {
+                        give(v, u);
                     } else {
-                        if (u > 0) old.request(J, p.kind, p.from, r0, c + u * 32, lane);
-                        ns_take_piece<PARTS, T>(A, J, p.kind, p.last, p.from, r0, c + u * 32, v, piece, lane, old);
+                        ns_take_piece<PARTS, T>(A, J, p.kind, p.last, p.from, r0, c + u * 32, v, piece, lane, old, u + 1 < kPieces ? c + (u + 1) * 32 : -1);
                     }
                 };
                 for (int g = 0; g < groups; ++g) {
@@ -646,7 +676,7 @@ __global__ void __launch_bounds__(kNsThreads, 1) ns_steps_kernel(const __grid_co
                     if (mine) {
                         if constexpr (PARTS == 2) {
 #pragma unroll
-                            for (int u = 0; u < TN / 64; ++u) {
+                            for (int u = 0; u < kPieces; ++u) {
                                 float v[32];
                                 tensor_read(v, at + slot * TN + u * 32);
 #pragma unroll
@@ -654,7 +684,7 @@ __global__ void __launch_bounds__(kNsThreads, 1) ns_steps_kernel(const __grid_co
                             }
                         } else {
 #pragma unroll 1
-                            for (int u = 0; u < TN / 64; ++u) {
+                            for (int u = 0; u < kPieces; ++u) {
                                 float v[32];
                                 tensor_read(v, at + slot * TN + u * 32);
                                 pass_on(v, u);
@@ -669,72 +699,59 @@ __global__ void __launch_bounds__(kNsThreads, 1) ns_steps_kernel(const __grid_co
                     }
                     if ((slot ^= 1) == 0) again ^= 1;
                 }
-                if (fine && mine && (PARTS == 2 || groups == 0)) {        // no groups: more CTAs than steps
+                if (PARTS == 2 && MODE == kShared && p.split > 1) {
+#pragma unroll
+                    for (int u = 0; u < kPieces; ++u) give(sum[PARTS == 2 ? u : 0], u);
+                } else if (PARTS == 2 && kPieces == 1) {
+                    if (fine && mine) pass_on(sum[0], 0);
+                } else if (fine && mine && (PARTS == 2 || groups == 0)) {        // no groups: more CTAs than steps
 #pragma unroll 1
-                    for (int u = 0; u < TN / 64; ++u) {
+                    for (int u = 0; u < kPieces; ++u) {
                         float v[32];
 #pragma unroll
                         for (int k = 0; k < 32; ++k) {
                             v[k] = 0.0f;
                             if constexpr (PARTS == 2) {
 #pragma unroll
-                                for (int e = 0; e < TN / 64; ++e) v[k] = u == e ? sum[e][k] : v[k];
+                                for (int e = 0; e < kPieces; ++e) v[k] = u == e ? sum[e][k] : v[k];
                             }
                         }
                         pass_on(v, u);
                     }
                 }
             }
-            if (CG == 1 && p.split > 1) {
+            if (MODE == kShared && p.split > 1) {
                 __syncwarp();
                 if (lane < p.split) mbar_release_at(given + p.kind, rank - p.rank + lane);
                 if (p.tile < p.tiles) {
-                    const Spot o = locate(p, p.tile);
-                    // this CTA's pieces of 32 x 32: rank, rank + split, ...; warp w takes the w-th of them
-                    const int piece_of = w * p.split + p.rank, part = piece_of & 3, c = piece_of >> 2;
+                    const Spot &o = firsts[kind];
+                    // this CTA's pieces of 32 x 32; warp w takes the w-th of them
+                    const int many = 16 / p.split, id = w * p.split + p.rank, part = id & 3, c = id >> 2;
                     NsOld<PARTS> old;
-                    if (piece_of < 16) old.request(*o.J, p.kind, p.from, o.i * 128 + part * 32, o.j * 128 + c * 32, lane);
+                    if (w < many) old.request(*o.J, p.kind, p.from, o.i * 128 + part * 32, o.j * 128 + c * 32, lane);
                     fine = __all_sync(0xffffffffu, mbar_acquire_bounded(given + p.kind, ph / 3 & 1, kWaitLimit)) && fine;
-                    // all threads add up the ranks' sums: 16 columns of four of a row, over 16 / split pieces
-                    float4 *const own = (float4 *)(smem + 128 * 128 * 4);      // behind what the others read
-                    const int many = 16 / p.split * 256;                       // float4 of this CTA's pieces
-                    for (int e0 = 0; e0 < many; e0 += 256) {
-                        const int e = e0 + threadIdx.x - 128, q = (e >> 8) * p.split + p.rank;
-                        const float4 *at = (const float4 *)smem + ((q >> 2) * 8 + ((e >> 5) & 7)) * 128 + (q & 3) * 32 + (e & 31);
-                        float4 x[8];
+                    if (w < many) {
+                        float v[32] = {};
+                        for (int r = 0; r < p.split; ++r) {
+                            const float4 *at = (const float4 *)exchange + (r * many + w) * 256 + lane;
 #pragma unroll
-                        for (int r = 0; r < 8; ++r)
-                            if (r < p.split) x[r] = read_at(at, rank - p.rank + r);
-                        float4 total = x[0];
-#pragma unroll
-                        for (int r = 1; r < 8; ++r)
-                            if (r < p.split) {
-                                total.x += x[r].x;
-                                total.y += x[r].y;
-                                total.z += x[r].z;
-                                total.w += x[r].w;
+                            for (int k = 0; k < 8; ++k) {
+                                const float4 x = at[k * 32];
+                                v[4 * k] += x.x;
+                                v[4 * k + 1] += x.y;
+                                v[4 * k + 2] += x.z;
+                                v[4 * k + 3] += x.w;
                             }
-                        own[e] = total;
-                    }
-                    fine = all_agree(2, 256, fine);
-                    if (piece_of < 16) {
-                        float v[32];
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            const float4 x = own[w * 256 + k * 32 + lane];
-                            v[4 * k] = x.x;
-                            v[4 * k + 1] = x.y;
-                            v[4 * k + 2] = x.z;
-                            v[4 * k + 3] = x.w;
                         }
-                        ns_take_piece<PARTS, T>(A, *o.J, p.kind, p.last, p.from, o.i * 128 + part * 32, o.j * 128 + c * 32, v, piece, lane, old);
+                        ns_take_piece<PARTS, T>(A, *o.J, p.kind, p.last, p.from, o.i * 128 + part * 32, o.j * 128 + c * 32, v, piece, lane, old, -1);
                     }
                 }
             }
             if (!p.last) {
                 // what this CTA has written is there for the others' loads
-                fence_async_all();
-                fine = all_agree(1, 256, fine);            // a warp that gave up takes the others along
+                if (MODE == kShared && p.split > 1) fence_async_all();
+                else fence_async_global();
+                fine = all_agree(1, 32 * kTakers, fine);   // a warp that gave up takes the others along
                 if (threadIdx.x == 128) grid_arrive(P.arrived);
             }
         }
@@ -1140,9 +1157,10 @@ static void ns_take(NsJob &J, int parts, unsigned char *&at)
     at = J.b + a;
 }
 
-template <typename T, int PARTS, int CG>
+template <typename T, int PARTS, int MODE>
 static int ns_run(NsArgs &A, int steps, cudaStream_t st)
 {
+    constexpr int CG = NsTile<PARTS, MODE>::CG;
     NsPlan P = {};
     P.steps = steps;
     P.status = device_status_word();
@@ -1168,14 +1186,14 @@ static int ns_run(NsArgs &A, int steps, cudaStream_t st)
     }
     P.tiles[kPolynomial] = P.tiles[kGram];
 
-    auto kern = ns_steps_kernel<PARTS, CG, T>;
-    constexpr size_t smem = NsTile<PARTS, CG>::kSmem;
+    auto kern = ns_steps_kernel<PARTS, MODE, T>;
+    constexpr size_t smem = NsTile<PARTS, MODE>::kSmem;
     int rc = reserve_dynamic_smem((const void *)kern, smem);
     if (rc) return rc;
     // CTAs that share a tile where there are too few tiles for the SMs, each with two steps of 64 at least
     const int index[3] = {ns_cb(n), ns_cb(m), ns_cb(m)};
     int ranks = CG, resident = 0;
-    for (int most = CG == 1 ? 8 : 1;; most = ranks) {
+    for (int most = MODE == kShared ? 8 : 1;; most = ranks) {
         ranks = CG;
         const int sms = resident ? resident : sm_count();
         for (int k = 0; k < 3; ++k) {
@@ -1183,14 +1201,14 @@ static int ns_run(NsArgs &A, int steps, cudaStream_t st)
             while (P.split[k] < most && P.tiles[k] * P.split[k] * 2 <= sms && index[k] >= P.split[k] * 4) P.split[k] *= 2;
             if (CG == 1) ranks = P.split[k] > ranks ? P.split[k] : ranks;
         }
-        const int held = resident_clusters((const void *)kern, ranks, kNsThreads, smem) * ranks;
+        const int held = resident_clusters((const void *)kern, ranks, NsTile<PARTS, MODE>::kThreads, smem) * ranks;
         if (held <= 0) {
             set_error("Newton-Schulz products: the device holds no cluster of %d CTAs", ranks);
             return SLAYER_B200_EUNSUPPORTED;
         }
         const bool settled = resident == held;
         resident = held;
-        if (settled || CG == 2) break;
+        if (settled || MODE != kShared) break;
     }
     int grid = 0;
     for (int k = 0; k < 3; ++k) {
@@ -1206,7 +1224,7 @@ static int ns_run(NsArgs &A, int steps, cudaStream_t st)
     if (rc) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(kNsThreads);
+    cfg.blockDim = dim3(NsTile<PARTS, MODE>::kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
@@ -1318,7 +1336,10 @@ static int ns_tiled(NsArgs &A, int steps, cudaStream_t st)
     // tiles of two CTAs where there are enough of them
     int64_t tiles = 0;
     for (int j = 0; j < A.jobs; ++j) tiles += (int64_t)((ns_rb(A.job[j].m) + 1) / 2) * ((ns_rb(A.job[j].n) + 1) / 2);
-    return tiles >= sm_count() / 2 ? ns_run<T, PARTS, 2>(A, steps, st) : ns_run<T, PARTS, 1>(A, steps, st);
+    if (tiles >= sm_count() / 2) return ns_run<T, PARTS, kPair>(A, steps, st);
+    int small = 0;
+    for (int j = 0; j < A.jobs; ++j) small += ns_rb(A.job[j].m) * (ns_rb(A.job[j].m) + 1) / 2;
+    return small * 4 <= sm_count() ? ns_run<T, PARTS, kShared>(A, steps, st) : ns_run<T, PARTS, kAlone>(A, steps, st);
 }
 
 static int ns_dispatch(NsArgs &A, int dtype, int steps, cudaStream_t st)

@@ -161,8 +161,9 @@ __device__ __forceinline__ bool mbar_acquire_bounded(uint64_t *bar, unsigned par
     return false;
 }
 
-// Between plain accesses and asynchronous copies of the same global or shared memory, in either order.
+// Between plain accesses and asynchronous copies of the same memory, in either order: global and shared, or global alone.
 __device__ __forceinline__ void fence_async_all() { asm volatile("fence.proxy.async;" ::: "memory"); }
+__device__ __forceinline__ void fence_async_global() { asm volatile("fence.proxy.async.global;" ::: "memory"); }
 
 // a barrier of `threads` threads of the CTA, which says whether all of them came with `value`
 __device__ __forceinline__ bool all_agree(int barrier, int threads, bool value)
@@ -209,6 +210,15 @@ __device__ __forceinline__ void cluster_wait_all()
 {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void write_at(void *p, unsigned rank, float4 v)
+{
+    asm volatile(
+        "{\n\t.reg .b32 far;\n\t"
+        "mapa.shared::cluster.u32 far, %0, %1;\n\t"
+        "st.shared::cluster.v4.f32 [far], {%2, %3, %4, %5};\n\t}"
+        ::"r"(smem_u32(p)), "r"(rank), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
 
 // 16 bytes at the same place of another CTA's shared memory
