@@ -523,8 +523,10 @@ __global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_ker
     auto right_turned = [&](int kind, int j, int k) { return kind == kPolynomial ? (k >> 1) < j + CG - 1 : kind == kUpdate; };
 
     if (warp < 4) {
-        // 128 threads give registers to the 256 that hold sums: 128 * 56 + 256 * 216 <= 384 * 168
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        // 128 threads give registers to the 256 that hold sums: 128 * 40 + 256 * 224 = 128 * 56 + 256 * 216 <= 384 * 168.  (Sums of 128
+        // columns in two parts need the last eight; elsewhere the loads' addresses do.)
+        if constexpr (MODE == kPair && PARTS == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        else asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == 0 && lane == 0) {
             int s = 0, turn = 0;
             for (int ph = 0, kind = 0; fine && ph < 3 * P.steps; ++ph, kind = kind == 2 ? 0 : kind + 1) {
@@ -626,14 +628,16 @@ __global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_ker
         }
         __syncwarp();
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        if constexpr (MODE == kPair && PARTS == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        else asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         int slot = 0, again = 0;
         const int w = warp - 4, quarter = warp & 3;
         unsigned char *piece = pieces + w * Tile::kPiece;
         for (int ph = 0, kind = 0; fine && ph < 3 * P.steps; ++ph, kind = kind == 2 ? 0 : kind + 1) {
             const Phase p = phase_at(ph, kind);
-            if (ph > 0) {
-                // what the phase before has left; and a CTA without a tile must not arrive before its time
+            // what the phase before has left, for what is requested before the products are done; and a CTA without a tile must not
+            // arrive before its time
+            if (ph > 0 && (MODE != kPair || p.tile >= p.tiles)) {
                 if (lane == 0) fine = grid_wait_bounded(P.arrived, ph * gridDim.x, kWaitLimit);
                 fine = __all_sync(0xffffffffu, fine);
             }
@@ -652,8 +656,9 @@ __global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_ker
 #pragma unroll
                         for (int k = 0; k < 32; ++k) sum[u][k] = 0.0f;
                 }
+                // (a pair's threads hold 128 sums: requested early there, the old values cost more in registers than they save)
                 NsOld<PARTS> old;
-                if (mine && !(MODE == kShared && p.split > 1)) old.request(J, p.kind, p.from, r0, c, lane);
+                if (MODE != kPair && mine && !(MODE == kShared && p.split > 1)) old.request(J, p.kind, p.from, r0, c, lane);
                 // To the one of those that share the tile whose piece it is: pieces rank, rank + split, ... of the sixteen, from every
                 // rank in turn.  (Written there, not fetched: a read of another CTA's memory takes 400 cycles, and the stores are
                 // on their way together.)
@@ -674,6 +679,7 @@ __global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_ker
                     if (!__all_sync(0xffffffffu, mbar_wait_bounded(done + slot, again, kWaitLimit))) { fine = false; break; }
                     tensor_fence_after();
                     if (mine) {
+                        if (MODE == kPair && PARTS == 1) old.request(J, p.kind, p.from, r0, c, lane);
                         if constexpr (PARTS == 2) {
 #pragma unroll
                             for (int u = 0; u < kPieces; ++u) {
@@ -705,6 +711,7 @@ __global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_ker
                 } else if (PARTS == 2 && kPieces == 1) {
                     if (fine && mine) pass_on(sum[0], 0);
                 } else if (fine && mine && (PARTS == 2 || groups == 0)) {        // no groups: more CTAs than steps
+                    if (MODE == kPair) old.request(J, p.kind, p.from, r0, c, lane);
 #pragma unroll 1
                     for (int u = 0; u < kPieces; ++u) {
                         float v[32];
@@ -778,8 +785,8 @@ constexpr int kSmallThreads = 512;
 constexpr int kSmallScratch = 16 * 32 * 17 * 4;          // a 32 x 16 piece of each warp
 
 struct NsSmall {
-    int rows, per, block, x, ab, scratch, total;         // rows and bytes
-    bool fits;
+    int rows, per, block, x, ab, scratch, sums, spread, total;         // rows and bytes
+    bool fits, few;
 };
 
 // where things lie in the shared memory of a CTA with `per` column blocks of a matrix of m rows
@@ -797,6 +804,11 @@ static __host__ __device__ __forceinline__ NsSmall ns_small(int m, int per, int 
     // results on their way to the weight: over B where all columns fit tensor memory at once, so that B is not needed any more
     s.scratch = s.rows > 64 ? s.x : s.x + s.ab;
     s.total = s.rows > 64 ? s.x + (s.ab > kSmallScratch ? s.ab : kSmallScratch) : s.scratch + kSmallScratch;
+    // of up to 32 rows, all CTAs' sums (of two steps), and a product on its way to threads that cannot read its tensor memory
+    s.few = s.rows <= 32 && per <= 8 && s.total + 2 * 8 * sums + per * 64 * s.rows * 4 <= 226 * 1024 - 1024;
+    s.sums = s.total;
+    s.spread = s.sums + 2 * 8 * sums;
+    if (s.few) s.total = s.spread + per * 64 * s.rows * 4;
     s.fits = s.total <= 226 * 1024 - 1024 && (s.rows <= 64 || per <= 8);
     return s;
 }
@@ -1003,12 +1015,41 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
                     for (int k = 0; k < 16; ++k) v[k] *= kScaleA / (kScaleX * kScaleX);
                     ns_put16<PARTS>(ab + (c >> 6) * L.block + r * 128, side, (c >> 3) & 7, r, v);
                 } else if (row_there) {
-                    // four columns of all rows after one another
+                    // four columns of all rows after one another; few rows, to everybody
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) ((float4 *)ab)[(c / 4 + k) * R + r] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+                    for (int k = 0; k < 4; ++k) {
+                        const float4 sum = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+                        const int e = (c / 4 + k) * R + r;
+                        if (L.few)
+                            for (int o = 0; o < C; ++o) write_at((float4 *)(smem + L.sums) + ((s & 1) * 8 + rank) * (R * R / 4) + e, o, sum);
+                        else ((float4 *)ab)[e] = sum;
+                    }
                 }
             }
-        if (C > 1) {
+        if (C > 1 && L.few) {
+            // (a CTA that is a step ahead writes to the other half)
+            __syncwarp();
+            cluster_wait_all();
+            const float4 *sums = (const float4 *)(smem + L.sums) + (s & 1) * 8 * (R * R / 4);
+            if (tid < R * R / 4) {
+                float4 total = sums[tid];
+                for (int o = 1; o < C; ++o) {
+                    const float4 y = sums[o * (R * R / 4) + tid];
+                    total.x += y.x;
+                    total.y += y.y;
+                    total.z += y.z;
+                    total.w += y.w;
+                }
+                const float f = kScaleA / (kScaleX * kScaleX);
+                const int row = tid % R, c = tid / R * 4;
+                uint2 hi, lo;
+                ns_split<PARTS>(total.x * f, total.y * f, hi.x, lo.x);
+                ns_split<PARTS>(total.z * f, total.w * f, hi.y, lo.y);
+                unsigned char *to = ab + row * 128 + ((((c >> 3) ^ row) & 7) * 16) + (c & 4) * 2;
+                *(uint2 *)to = hi;
+                if (PARTS == 2) *(uint2 *)(to + side) = lo;
+            }
+        } else if (C > 1) {
             __syncwarp();
             cluster_wait_all();
             const int all = R * R / 4, e0 = all * rank / C, e1 = all * (rank + 1) / C;
@@ -1086,7 +1127,66 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
             }
             made();
             if (last) __syncthreads();                   // B may be written over
-            if (mine)
+            if (L.few) {
+                // Four of the sixteen warps can read these rows: they pass them on, and all threads do the rest, eight columns of a row
+                // each (10 x 4096: 12 -> TIME us a step).
+                float4 *spread = (float4 *)(smem + L.spread);
+                if (mine)
+                    for (int c = first; c < (n1 - n0) * 64; c += 64) {
+                        float v[16];
+                        __syncwarp();
+                        tensor_read(v, at + c);
+                        if (row_there)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) spread[(c / 4 + k) * R + r] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+                    }
+                __syncthreads();
+                const int many = (n1 - n0) * 8;
+                for (int i = tid; i < many * R; i += kSmallThreads) {
+                    // neighbours are rows of a column, or, where they go to a weight with rows of its own, its columns
+                    const bool across = last && !tall;
+                    const int row = across ? i / many : i % R, ch = across ? i % many : i / R;
+                    const float4 a = spread[(2 * ch) * R + row], b = spread[(2 * ch + 1) * R + row];
+                    float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                    unsigned char *chunk = x + (n0 + (ch >> 3)) * L.block + row * 128 + ((ch ^ row) & 7) * 16;
+                    const uint4 hi = *(const uint4 *)chunk;
+                    uint4 lo = make_uint4(0, 0, 0, 0);
+                    if (PARTS == 2) lo = *(const uint4 *)(chunk + side);
+                    const uint32_t hs[4] = {hi.x, hi.y, hi.z, hi.w}, ls[4] = {lo.x, lo.y, lo.z, lo.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float2 o = __half22float2(*reinterpret_cast<const __half2 *>(&hs[e]));
+                        if (PARTS == 2) {
+                            const float2 l = __half22float2(*reinterpret_cast<const __half2 *>(&ls[e]));
+                            o.x += l.x;
+                            o.y += l.y;
+                        }
+                        v[2 * e] = fmaf(A.ca, o.x, (1.0f / kScaleA) * v[2 * e]);
+                        v[2 * e + 1] = fmaf(A.ca, o.y, (1.0f / kScaleA) * v[2 * e + 1]);
+                    }
+                    if (!last) {
+                        uint4 nh, nl;
+                        ns_split<PARTS>(v[0], v[1], nh.x, nl.x);
+                        ns_split<PARTS>(v[2], v[3], nh.y, nl.y);
+                        ns_split<PARTS>(v[4], v[5], nh.z, nl.z);
+                        ns_split<PARTS>(v[6], v[7], nh.w, nl.w);
+                        *(uint4 *)chunk = nh;
+                        if (PARTS == 2) *(uint4 *)(chunk + side) = nl;
+                    } else {
+                        T *dst = (T *)J.dst;
+                        const int c0 = (b0 + n0) * 64 + ch * 8;
+                        const int64_t to = tall ? (int64_t)c0 * J.cols + row : (int64_t)row * J.cols + c0, step = tall ? J.cols : 1;
+                        float w[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) w[k] = J.mom && row < J.m && c0 + k < J.n ? ns_in(dst[to + k * step]) : 0.0f;
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const float o = v[k] * (1.0f / kScaleX);
+                            if (row < J.m && c0 + k < J.n) dst[to + k * step] = ns_out<T>(J.mom ? fmaf(J.keep, w[k], -J.step * o) : o);
+                        }
+                    }
+                }
+            } else if (mine)
                 for (int c = first; c < (n1 - n0) * 64; c += 64) {
                     float v[16];
                     __syncwarp();
