@@ -273,8 +273,9 @@ struct NsTile {
     static constexpr size_t kSmem = kFixed + (size_t)kStages * kStage;
     // Steps of 64 whose sum stays in tensor memory.  The tensor core cuts what it adds to a sum instead of rounding it: over the
     // 375 additions of a sum of 2000 products in two parts that is a bias of 1e-5, ten times the rounding of fp32 sums.  So
-    // with two parts the sums of 128 products are added up in registers, rounded, while the next ones are made.
-    static constexpr int kGroup = PARTS == 2 ? 2 : 1 << 20;
+    // with two parts the sums of 64 products are added up in registers, rounded, while the next ones are made: 2000 x 333 is 2.0e-6
+    // off after five steps (fp32 products: 2.2e-6), with sums of 128 3.5e-6; 4096 x 4096 takes 3.86 ms for it instead of 3.6.
+    static constexpr int kGroup = PARTS == 2 ? 1 : 1 << 20;
 };
 
 // 32 rows x 32 columns of a block in global memory and a warp's piece of shared memory: row by row 64 bytes, of which a lane
