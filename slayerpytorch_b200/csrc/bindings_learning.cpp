@@ -1,10 +1,14 @@
 // Python module `slayerCuda`, second part: the losses of rows of logits (actionLogProb, policyLoss, preferenceLoss) as autograd
-// functions - a step of a small network is bound by the host, and these are half as long there as their Python form - and the orthogonalised updates (orthogonalize, muonStep).  They take float32, bfloat16 and float16 logits, matrices
-// and weights; everything that belongs to a row, and the momenta, are float32.
+// functions - a step of a small network is bound by the host, and these are half as long there as their Python form - and the
+// orthogonalised updates (orthogonalize, muonStep).  They take float32, bfloat16 and float16 logits, matrices and weights; everything
+// that belongs to a row, and the momenta, are float32.
 #include "bindings_common.h"
 
 #include <cuda_runtime_api.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <math.h>
+
+#include <algorithm>
 
 using namespace sb200py;
 
@@ -134,7 +138,11 @@ torch::Tensor logit_grad(const torch::Tensor &logits, const torch::Tensor &actio
                                         mask.defined() ? reinterpret_cast<const uint8_t *>(mask.data_ptr<bool>()) : nullptr, stats, coef, coef_len,
                                         upstream.data_ptr<float>(), by_row, into != nullptr, rows, V, x.stride(0), (float)scale, current_stream()),
                  op);
-    return grad.view(logits.sizes());
+    grad = grad.view(logits.sizes());
+    if (!at::GradMode::is_enabled()) return grad;
+    // create_graph: the gradient can be had, its derivative cannot (and must not read as zero)
+    grad = grad.detach().set_requires_grad(true);
+    return (*std::make_shared<torch::autograd::DelayedError>(std::string(op) + ": has first derivatives only", 1))({grad})[0];
 }
 
 // Forward reads the logits once and keeps two floats per row; backward reads them again and writes their gradient.
@@ -333,7 +341,7 @@ torch::Tensor orthogonalizeCuda(torch::Tensor x, int64_t steps, double a, double
     auto out = torch::empty_like(x);
     const int64_t rows = x.size(-2), cols = x.size(-1), batch = x.numel() ? x.numel() / (rows * cols) : 0;
     auto workspace = torch::empty({slayer_b200_orthogonalize_workspace(batch, rows, cols, dtype)}, x.options().dtype(torch::kUInt8));
-    check_rc(slayer_b200_orthogonalize(out.data_ptr(), x.data_ptr(), dtype, batch, rows, cols, (int)std::min<int64_t>(steps, 1 << 20),
+    check_rc(slayer_b200_orthogonalize(out.data_ptr(), x.data_ptr(), dtype, batch, rows, cols, (int)std::clamp<int64_t>(steps, 0, 1 << 20),
                                        (float)a, (float)b, (float)c, (float)eps, workspace.data_ptr(), current_stream()),
              "orthogonalize");
     return out;
@@ -367,7 +375,7 @@ void muonStepCuda(std::vector<torch::Tensor> weights, const std::vector<torch::T
     auto workspace = torch::empty({slayer_b200_muon_step_workspace(list.data(), (int64_t)list.size(), dtype)},
                                   weights[0].options().dtype(torch::kUInt8));
     check_rc(slayer_b200_muon_step(list.data(), (int64_t)list.size(), dtype, (float)lr, (float)momentum, nesterov, (float)weightDecay,
-                                   (int)adjust, (int)std::min<int64_t>(steps, 1 << 20), (float)a, (float)b, (float)c, (float)eps,
+                                   (int)adjust, (int)std::clamp<int64_t>(steps, 0, 1 << 20), (float)a, (float)b, (float)c, (float)eps,
                                    workspace.data_ptr(), current_stream()),
              "muonStep");
     for (auto &w : weights) w.unsafeGetTensorImpl()->bump_version();      // autograd sees that they changed

@@ -11,7 +11,7 @@
 //   PARTS = 2 (float32, float16 weights): v = hi + lo, two fp16 values, 22 bits and a sign;  v w ~ hi hi + hi lo + lo hi, the
 //     left out lo lo being 2^-24 of it.  Three products instead of one, and results as good as fp32 arithmetic's.
 //   PARTS = 1 (bfloat16 weights, whose update is rounded to 8 bits in the end): v = hi.
-// Sums are fp32 in tensor memory.
+// Sums are fp32: of 64 products in tensor memory where there are two parts, longer ones in registers (see kGroup).
 //
 // X, A and B = b A + c A A live in the workspace as blocks of 128 x 64 elements, padded with zeros, each block laid out as the
 // tensor core reads it from shared memory (tensor.cuh), hi before lo: every load is a contiguous copy of 8 to 32 KB, whatever
@@ -86,6 +86,18 @@ __device__ __forceinline__ int ns_find(const NsArgs &A, int at)
     while (j + 1 < A.jobs && A.job[j + 1].first[WHICH] <= at) ++j;
     return j;
 }
+
+// What turns u into the scaled X0: one factor, or two where the norm is so small that its inverse is no float.
+struct NsScale {
+    float lift, inv;
+    __device__ __forceinline__ NsScale(double squares, float eps)
+    {
+        const double norm = sqrt(squares) + (double)eps;
+        lift = norm < 1e-25 ? 0x1p80f : 1.0f;
+        inv = (float)((double)kScaleX / (norm * (double)lift));
+    }
+    __device__ __forceinline__ float operator()(float u) const { return u * lift * inv; }
+};
 
 __device__ __forceinline__ bool ns_wide(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
@@ -205,7 +217,7 @@ __global__ void __launch_bounds__(256) ns_normalise_kernel(const __grid_constant
     const NsJob &J = A.job[ns_find<0>(A, blockIdx.x)];
     const int me = blockIdx.x - J.first[0];
     const double sq = ns_block_sum((int)threadIdx.x < J.norm_parts ? J.parts[threadIdx.x] : 0.0, part);
-    const float inv = (float)((double)kScaleX / (sqrt(sq) + (double)A.eps));
+    const NsScale scale(sq, A.eps);
     const T *g = (const T *)J.src;
     const bool tall = J.rows > J.cols, wide = !tall && J.cols % 8 == 0 && ns_wide(g) && ns_wide(J.mom);
     const int rows = ns_rb(J.m) * 128, cbs = ns_cb(J.n), chunks = cbs * 8;
@@ -227,7 +239,7 @@ __global__ void __launch_bounds__(256) ns_normalise_kernel(const __grid_constant
                 }
             }
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = r < J.m ? v[k] * inv : 0.0f;
+            for (int k = 0; k < 8; ++k) v[k] = r < J.m ? scale(v[k]) : 0.0f;
         } else
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
@@ -236,7 +248,7 @@ __global__ void __launch_bounds__(256) ns_normalise_kernel(const __grid_constant
                 const int64_t at = tall ? (int64_t)(c + k) * J.cols + r : (int64_t)r * J.cols + c + k;
                 float u = ns_in(g[at]);
                 if (J.mom) u = A.nesterov ? fmaf(A.mu, J.mom[at], u) : J.mom[at];
-                v[k] = u * inv;
+                v[k] = scale(u);
             }
         }
         uint4 hi, lo;
@@ -933,16 +945,16 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
         sq = 0.0;
         for (int r = 0; r < C; ++r) sq += read_double_at(&square, r);
     }
-    const float inv = (float)((double)kScaleX / (sqrt(sq) + (double)A.eps));
+    const NsScale scale(sq, A.eps);
     for (int i = tid; i < R * chunks; i += kSmallThreads) {
         const int r = tall ? i % R : i / chunks, ch = tall ? i / R : i % chunks;
         float v[8] = {};
         if (r < J.m) ns_load_u<T>(A, J, r, b0 * 64 + ch * 8, false, v);
         uint4 hi, lo;
-        ns_split<PARTS>(v[0] * inv, v[1] * inv, hi.x, lo.x);
-        ns_split<PARTS>(v[2] * inv, v[3] * inv, hi.y, lo.y);
-        ns_split<PARTS>(v[4] * inv, v[5] * inv, hi.z, lo.z);
-        ns_split<PARTS>(v[6] * inv, v[7] * inv, hi.w, lo.w);
+        ns_split<PARTS>(scale(v[0]), scale(v[1]), hi.x, lo.x);
+        ns_split<PARTS>(scale(v[2]), scale(v[3]), hi.y, lo.y);
+        ns_split<PARTS>(scale(v[4]), scale(v[5]), hi.z, lo.z);
+        ns_split<PARTS>(scale(v[6]), scale(v[7]), hi.w, lo.w);
         unsigned char *at = x + (ch >> 3) * L.block + r * 128 + ((ch ^ r) & 7) * 16;
         *(uint4 *)at = hi;
         if (PARTS == 2) *(uint4 *)(at + side) = lo;
@@ -1130,7 +1142,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
             if (last) __syncthreads();                   // B may be written over
             if (L.few) {
                 // Four of the sixteen warps can read these rows: they pass them on, and all threads do the rest, eight columns of a row
-                // each (10 x 4096: 12 -> TIME us a step).
+                // each (10 x 4096: 12.6 -> 9.6 us a step).
                 float4 *spread = (float4 *)(smem + L.spread);
                 if (mine)
                     for (int c = first; c < (n1 - n0) * 64; c += 64) {

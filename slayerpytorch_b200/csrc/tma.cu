@@ -53,9 +53,18 @@ int *device_status_word()
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
     std::lock_guard<std::mutex> lock(g_status_mu);
     if (!g_status[dev]) {
+        // the first call may be one that is being captured: not a part of the capture
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) { (void)cudaGetLastError(); return nullptr; }
         int *p = nullptr;
-        if (cudaMalloc(&p, 256) != cudaSuccess) { (void)cudaGetLastError(); return nullptr; }
-        if (cudaMemset(p, 0, 256) != cudaSuccess) { (void)cudaGetLastError(); cudaFree(p); return nullptr; }
+        cudaStream_t st = nullptr;
+        bool fine = cudaMalloc(&p, 256) == cudaSuccess && cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking) == cudaSuccess &&
+                    cudaMemsetAsync(p, 0, 256, st) == cudaSuccess && cudaStreamSynchronize(st) == cudaSuccess;
+        if (!fine) (void)cudaGetLastError();
+        if (st) cudaStreamDestroy(st);
+        if (!fine && p) cudaFree(p);
+        (void)cudaThreadExchangeStreamCaptureMode(&mode);
+        if (!fine) return nullptr;
         g_status[dev] = p;
     }
     return g_status[dev];

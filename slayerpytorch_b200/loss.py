@@ -15,7 +15,7 @@ in the backward pass, exactly as the reference's ``spikeDesired`` built from ``.
 
 Where there is no desired answer but a judgement of the one given, ``policyLoss`` and ``preferenceLoss`` take rows of logits and
 the entry chosen in each (``actionLogProb`` gives the values of the policy that chose); ``spikeLoss.policy`` and
-``spikeLoss.preference`` take the logits from the output neurons' spike counts.
+``spikeLoss.preference`` take the logits from the output neurons' spike counts.  They have first derivatives only.
 """
 import numpy as np
 import torch

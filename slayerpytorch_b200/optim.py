@@ -43,7 +43,7 @@ def muonStep(weights, grads, momenta, lr, momentum=0.95, nesterov=True, weightDe
         weight = weight * (1 - lr * weightDecay) - lr * factor * update
 
     A weight of shape ``[d0, d1, ...]`` is a matrix of ``d0`` rows.  Weights and their gradients are float32, bfloat16 or float16,
-    momenta float32.  ``factor`` is ``sqrt(max(1, rows / cols))`` (``adjust='shape'``), ``0.2 * sqrt(max(rows, cols))`` (``'rms'``: updates
+    momenta float32; none of them overlap, but for gradients.  ``factor`` is ``sqrt(max(1, rows / cols))`` (``adjust='shape'``), ``0.2 * sqrt(max(rows, cols))`` (``'rms'``: updates
     as large as Adam's) or 1 (``None``)."""
     weights, grads, momenta = list(weights), list(grads), list(momenta)
     if not len(weights) == len(grads) == len(momenta):
@@ -63,6 +63,8 @@ def muonStep(weights, grads, momenta, lr, momentum=0.95, nesterov=True, weightDe
                 raise ValueError("muonStep: the same weight or momentum twice")
             seen.add(t.data_ptr())
         groups.setdefault((w.device, w.dtype), []).append((w, g, m))
+    if any(g.numel() and g.data_ptr() in seen for g in grads):
+        raise ValueError("muonStep: a gradient in the memory of a weight or momentum")
     for items in groups.values():
         # a weight whose elements are in another order is updated in a copy
         there = [w if w.is_contiguous() else w.contiguous() for w, _, _ in items]

@@ -269,6 +269,20 @@ def test_policy_rows_that_are_all_masked_or_missing():
     assert lp.shape == (0,)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_a_second_derivative_is_refused(dtype):
+    x = torch.randn(6, 4, 9, device="cuda").to(dtype).requires_grad_()
+    a = torch.randint(0, 9, (6, 4), device="cuda")
+    zero = torch.zeros(6, 4, device="cuda")
+    for make in (lambda: loss.actionLogProb(x, a).sum(), lambda: loss.policyLoss(x, a, zero - 2, zero + 1),
+                 lambda: loss.preferenceLoss(x, a, zero[:, 0])):
+        plain, = torch.autograd.grad(make(), x)
+        g, = torch.autograd.grad(make(), x, create_graph=True)
+        assert torch.equal(g, plain)
+        with pytest.raises(RuntimeError, match="first derivatives only"):
+            g.float().square().sum().backward()
+
+
 def test_policy_without_gradients_writes_none():
     x, action, old, adv, ref, mask = policy_case(3, 4, 2000, torch.bfloat16, 2)
     leaf = x.cuda().requires_grad_()

@@ -13,6 +13,8 @@ def test_lists_shapes_and_options_are_checked():
                 dict(weights=[w, w], grads=[g, g], momenta=[m, m.clone()]), dict(weights=[w, w + 1], grads=[g, g], momenta=[m, m])):
         with pytest.raises(ValueError):
             optim.muonStep(**{**dict(weights=[w], grads=[g], momenta=[m], lr=0.1), **bad})
+    with pytest.raises(ValueError, match="in the memory of"):
+        optim.muonStep([w], [m], [m], lr=0.1)
     with pytest.raises(ValueError, match="sparse"):
         optim.muonStep([w], [g.to_sparse()], [m], lr=0.1)
     with pytest.raises(ValueError, match="two dimensions"):

@@ -8,6 +8,9 @@ directions that have arrived (|p'| <= 4 there, which random signs and five steps
 products of 22 bits with fp32 sums, e = 2^-22, t = 8; bfloat16: products of fp16 values, e = 2^-12, t = 4.  The result's own
 rounding is half a step of its type."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -122,6 +125,49 @@ def test_orthogonalize_degenerate_matrices():
         s = A * s + B * s ** 3 + C * s ** 5
     assert abs(strong - s) < 1e-4
     assert float(torch.linalg.vector_norm(got)) < s + 485 * 8 * 2.0 ** -22
+
+
+@pytest.mark.parametrize("shape", [(20, 30), (30, 20), (200, 260)])
+def test_orthogonalize_of_the_smallest_numbers(shape):
+    """A norm whose inverse is no float: with eps = 0 the result is that of the same matrix scaled by a power of two, bit for bit."""
+    x = torch.randint(-3, 4, shape, generator=torch.Generator().manual_seed(2)).float().cuda()
+    tiny = torch.ldexp(torch.ldexp(x, torch.tensor(-100.0, device="cuda")), torch.tensor(-49.0, device="cuda"))
+    assert float(tiny.double().abs().max()) == 3 * 2.0 ** -149
+    assert torch.equal(optim.orthogonalize(tiny, eps=0.0), optim.orthogonalize(x, eps=0.0))
+
+
+def test_the_first_call_of_a_process_in_a_graph():
+    code = '''
+import torch
+from slayerpytorch_b200 import optim
+x = [torch.randn(s, device="cuda") for s in ((300, 500), (20, 30))]
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = [optim.orthogonalize(v) for v in x]
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, optim.orthogonalize(b)) for a, b in zip(y, x))
+print("as eager")
+'''
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
+                          cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert done.returncode == 0 and "as eager" in done.stdout, done.stderr[-2000:]
+
+
+def test_two_streams_at_once():
+    xs = [torch.randn(700, 900, device="cuda"), torch.randn(60, 400, device="cuda"), torch.randn(1100, 1300, device="cuda")]
+    want = [optim.orthogonalize(x) for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    got = [[] for _ in xs]
+    for _ in range(5):
+        for x, st, g in zip(xs, streams, got):
+            with torch.cuda.stream(st):
+                g.append(optim.orthogonalize(x))
+    torch.cuda.synchronize()
+    for w, g in zip(want, got):
+        assert all(torch.equal(w, y) for y in g)
 
 
 def test_orthogonalize_is_repeatable_and_stream_ordered():
