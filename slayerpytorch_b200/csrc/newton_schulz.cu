@@ -120,6 +120,31 @@ __device__ __forceinline__ void ns_load8(float (&v)[8], const T *p)
     }
 }
 
+// o, or keep w + o where a weight is updated, as 16 bytes
+template <typename T>
+__device__ __forceinline__ void ns_store16(T *at, const float (&o)[16 / sizeof(T)], const uint4 &w, float keep, bool update)
+{
+    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+    uint32_t out[4];
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) out[i] = __float_as_uint(update ? fmaf(keep, __uint_as_float(ws[i]), o[i]) : o[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint16_t h[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const uint16_t old = (uint16_t)(ws[i] >> 16 * e);
+                const T x = ns_out<T>(update ? fmaf(keep, ns_in(*reinterpret_cast<const T *>(&old)), o[2 * i + e]) : o[2 * i + e]);
+                h[e] = *reinterpret_cast<const uint16_t *>(&x);
+            }
+            out[i] = h[0] | (uint32_t)h[1] << 16;
+        }
+    }
+    *(uint4 *)at = make_uint4(out[0], out[1], out[2], out[3]);
+}
+
 // momentum, and the squares' partial sums (double: a sum over up to 2^31 squares, of values of any size)
 template <typename T>
 __global__ void __launch_bounds__(256) ns_momentum_kernel(const __grid_constant__ NsArgs A, unsigned *arrived)
@@ -362,30 +387,50 @@ __device__ __forceinline__ void ns_take_piece(const NsArgs &A, const NsJob &J, i
     }
     __syncwarp();
     if (last) {
-        // to the weight, 32 elements next to each other at a time: of a tall matrix, what the lanes hold of a column
+        // to the weight, of which the piece is 32 x 32 as well, turned if it is tall: 16 bytes a lane where its rows allow it, else
+        // 32 elements next to each other at a time
+        constexpr int E = 16 / sizeof(T), U = 4;
         T *dst = (T *)J.dst;
-        const bool tall = J.rows > J.cols;
-        float *turned = (float *)piece;
-        if (!tall) {
-#pragma unroll
-            for (int k = 0; k < 32; ++k) turned[lane * 33 + k] = v[k];
-            __syncwarp();
-        }
+        const bool tall = J.rows > J.cols, update = J.mom != nullptr;
+        const int row0 = tall ? c : r0, col0 = tall ? r0 : c, rows = min(32, J.rows - row0), cols = min(32, J.cols - col0);
         const int64_t step = J.cols;
-        const int many = min(32, tall ? J.n - c : J.m - r0);          // rows of the weight
-        const bool mine = tall ? r0 + lane < J.m : c + lane < J.n;
-        T *at = dst + (tall ? (int64_t)c * step + r0 + lane : (int64_t)r0 * step + c + lane);
+        const float keep = J.keep, by = update ? -J.step * (1.0f / kScaleX) : 1.0f / kScaleX;
+        float *turned = (float *)piece;
 #pragma unroll
-        for (int k0 = 0; k0 < 32; k0 += 8) {
-            float w[8];
+        for (int k = 0; k < 32; ++k) turned[tall ? k * 33 + lane : lane * 33 + k] = v[k];
+        __syncwarp();
+        if (J.cols % E == 0 && ns_wide(dst)) {
+            const int row = lane / (32 / E), col = lane % (32 / E) * E;
+            const float *from = turned + row * 33 + col;
+            T *at = dst + (row0 + row) * step + col0 + col;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) w[k] = J.mom && mine && k0 + k < many ? ns_in(at[k * step]) : 0.0f;
+            for (int i0 = 0; i0 < 32 / E; i0 += U) {
+                uint4 w[U];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float o = (tall ? v[k0 + k] : turned[(k0 + k) * 33 + lane]) * (1.0f / kScaleX);
-                if (mine && k0 + k < many) at[k * step] = ns_out<T>(J.mom ? fmaf(J.keep, w[k], -J.step * o) : o);
+                for (int i = 0; i < U; ++i)
+                    if (update && row + (i0 + i) * E < rows && col < cols) w[i] = *(const uint4 *)(at + (i0 + i) * E * step);
+#pragma unroll
+                for (int i = 0; i < U; ++i) {
+                    float o[E];
+#pragma unroll
+                    for (int e = 0; e < E; ++e) o[e] = from[(i0 + i) * E * 33 + e] * by;
+                    if (row + (i0 + i) * E < rows && col < cols) ns_store16<T>(at + (i0 + i) * E * step, o, w[i], keep, update);
+                }
             }
-            at += 8 * step;
+        } else {
+            T *at = dst + row0 * step + col0 + lane;
+#pragma unroll 1
+            for (int k0 = 0; k0 < rows; k0 += 8) {
+                float w[8], o[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) w[k] = update && lane < cols && k0 + k < rows ? ns_in(at[k * step]) : 0.0f;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) o[k] = turned[(k0 + k) * 33 + lane] * by;
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (lane < cols && k0 + k < rows) at[k * step] = ns_out<T>(update ? fmaf(keep, w[k], o[k]) : o[k]);
+                at += 8 * step;
+            }
         }
         __syncwarp();
     } else {
@@ -434,6 +479,8 @@ __global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_ker
 {
     using Tile = NsTile<PARTS, MODE>;
     constexpr int CG = Tile::CG, S = Tile::kStages, TN = Tile::TN, kTakers = Tile::kTakers, kPieces = Tile::kPieces;
+    // pieces of the old values that a warp requests before its sums are complete (two parts: as many as the registers hold)
+    constexpr int kAhead = PARTS == 2 && MODE != kAlone ? 1 : kPieces;
     extern __shared__ unsigned char smem_raw[];
     unsigned char *smem = (unsigned char *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     // full: this CTA's loads are there; ready: the second CTA's are (at the first); empty: a stage has been read; done: a sum is
@@ -486,17 +533,17 @@ __global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_ker
     };
     // tile -> its job, its first row block and its first column block, and this CTA's part of the summation index
     struct Spot {
-        const NsJob *J;
-        int i, j, k0, k1;
+        int job, i, j, k0, k1;
     };
     auto locate = [&](const Phase &p, int tile) {
         Spot o;
         const bool symmetric = p.kind != kUpdate;
         int n = 0;
         while (n + 1 < A.jobs && A.job[n + 1].first[symmetric ? 1 : 2] <= tile) ++n;
-        o.J = &A.job[n];
-        int at = tile - o.J->first[symmetric ? 1 : 2];
-        const int rt = (ns_rb(o.J->m) + CG - 1) / CG;
+        o.job = n;
+        const NsJob &J = A.job[n];
+        int at = tile - J.first[symmetric ? 1 : 2];
+        const int rt = (ns_rb(J.m) + CG - 1) / CG;
         if (symmetric) {
             // a row of tiles begins at the diagonal
             for (o.i = 0; at >= rt - o.i; ++o.i) at -= rt - o.i;
@@ -508,7 +555,7 @@ __global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_ker
         }
         o.i *= CG;
         o.j *= CG;
-        const int steps = p.kind == kGram ? ns_cb(o.J->n) : ns_cb(o.J->m);
+        const int steps = p.kind == kGram ? ns_cb(J.n) : ns_cb(J.m);
         o.k0 = steps * p.rank / p.split;
         o.k1 = steps * (p.rank + 1) / p.split;
         return o;
@@ -550,7 +597,7 @@ __global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_ker
                 const Phase p = phase_at(ph, kind);
                 for (int tile = p.tile; fine && tile < p.tiles; tile += p.step) {
                     const Spot o = spot_at(p, tile);
-                    const NsJob &J = *o.J;
+                    const NsJob &J = A.job[o.job];
                     const int cbm = ns_cb(J.m), cbn = ns_cb(J.n), rb = ns_rb(J.m);
                     const int cbl = p.kind == kGram ? cbn : cbm, cbr = p.kind == kPolynomial ? cbm : cbn;
                     const unsigned char *left = p.kind == kGram ? J.x[p.from] : p.kind == kPolynomial ? J.a : J.b;
@@ -650,13 +697,13 @@ __global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_ker
             const Phase p = phase_at(ph, kind);
             // what the phase before has left, for what is requested before the products are done; and a CTA without a tile must not
             // arrive before its time
-            if (ph > 0 && (MODE != kPair || p.tile >= p.tiles)) {
+            if (ph > 0) {
                 if (lane == 0) fine = grid_wait_bounded(P.arrived, ph * gridDim.x, kWaitLimit);
                 fine = __all_sync(0xffffffffu, fine);
             }
             for (int tile = p.tile; fine && tile < p.tiles; tile += p.step) {
                 const Spot o = spot_at(p, tile);
-                const NsJob &J = *o.J;
+                const NsJob &J = A.job[o.job];
                 const int groups = (o.k1 - o.k0 + Tile::kGroup - 1) / Tile::kGroup, rb = ns_rb(J.m);
                 const int il = o.i + pair, c0 = (w >> 2) * Tile::kWide, jl = o.j + (c0 >> 7);      // this warp's columns of the tile; its blocks
                 const bool mine = il < rb && jl < (p.kind != kUpdate ? rb : ns_rb(J.n)) && !(p.kind != kUpdate && jl < il);
@@ -669,9 +716,11 @@ __global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_ker
 #pragma unroll
                         for (int k = 0; k < 32; ++k) sum[u][k] = 0.0f;
                 }
-                // (a pair's threads hold 128 sums: requested early there, the old values cost more in registers than they save)
-                NsOld<PARTS> old;
-                if (MODE != kPair && mine && !(MODE == kShared && p.split > 1)) old.request(J, p.kind, p.from, r0, c, lane);
+                NsOld<PARTS> old[kAhead];
+                if (mine && !(MODE == kShared && p.split > 1)) {
+#pragma unroll
+                    for (int u = 0; u < kAhead; ++u) old[u].request(J, p.kind, p.from, r0, c + u * 32, lane);
+                }
                 // To the one of those that share the tile whose piece it is: pieces rank, rank + split, ... of the sixteen, from every
                 // rank in turn.  (Written there, not fetched: a read of another CTA's memory takes 400 cycles, and the stores are
                 // on their way together.)
@@ -685,14 +734,13 @@ __global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_ker
                     if (MODE == kShared && p.split > 1) {
                         give(v, u);
                     } else {
-                        ns_take_piece<PARTS, T>(A, J, p.kind, p.last, p.from, r0, c + u * 32, v, piece, lane, old, u + 1 < kPieces ? c + (u + 1) * 32 : -1);
+                        ns_take_piece<PARTS, T>(A, J, p.kind, p.last, p.from, r0, c + u * 32, v, piece, lane, old[u % kAhead], u + kAhead < kPieces ? c + (u + kAhead) * 32 : -1);
                     }
                 };
                 for (int g = 0; g < groups; ++g) {
                     if (!__all_sync(0xffffffffu, mbar_wait_bounded(done + slot, again, kWaitLimit))) { fine = false; break; }
                     tensor_fence_after();
                     if (mine) {
-                        if (MODE == kPair && PARTS == 1) old.request(J, p.kind, p.from, r0, c, lane);
                         if constexpr (PARTS == 2) {
 #pragma unroll
                             for (int u = 0; u < kPieces; ++u) {
@@ -702,7 +750,7 @@ __global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_ker
                                 for (int k = 0; k < 32; ++k) sum[u][k] += v[k];
                             }
                         } else {
-#pragma unroll 1
+#pragma unroll
                             for (int u = 0; u < kPieces; ++u) {
                                 float v[32];
                                 tensor_read(v, at + slot * TN + u * 32);
@@ -721,22 +769,15 @@ __global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_ker
                 if (PARTS == 2 && MODE == kShared && p.split > 1) {
 #pragma unroll
                     for (int u = 0; u < kPieces; ++u) give(sum[PARTS == 2 ? u : 0], u);
-                } else if (PARTS == 2 && kPieces == 1) {
-                    if (fine && mine) pass_on(sum[0], 0);
                 } else if (fine && mine && (PARTS == 2 || groups == 0)) {        // no groups: more CTAs than steps
-                    if (MODE == kPair) old.request(J, p.kind, p.from, r0, c, lane);
-#pragma unroll 1
+#pragma unroll
                     for (int u = 0; u < kPieces; ++u) {
-                        float v[32];
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) {
-                            v[k] = 0.0f;
-                            if constexpr (PARTS == 2) {
-#pragma unroll
-                                for (int e = 0; e < kPieces; ++e) v[k] = u == e ? sum[e][k] : v[k];
-                            }
+                        if constexpr (PARTS == 2) {
+                            pass_on(sum[u], u);
+                        } else {
+                            float v[32] = {};
+                            pass_on(v, u);
                         }
-                        pass_on(v, u);
                     }
                 }
             }
@@ -748,7 +789,7 @@ __global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_ker
                     // this CTA's pieces of 32 x 32; warp w takes the w-th of them
                     const int many = 16 / p.split, id = w * p.split + p.rank, part = id & 3, c = id >> 2;
                     NsOld<PARTS> old;
-                    if (w < many) old.request(*o.J, p.kind, p.from, o.i * 128 + part * 32, o.j * 128 + c * 32, lane);
+                    if (w < many) old.request(A.job[o.job], p.kind, p.from, o.i * 128 + part * 32, o.j * 128 + c * 32, lane);
                     fine = __all_sync(0xffffffffu, mbar_acquire_bounded(given + p.kind, ph / 3 & 1, kWaitLimit)) && fine;
                     if (w < many) {
                         float v[32] = {};
@@ -763,7 +804,7 @@ __global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_ker
                                 v[4 * k + 3] += x.w;
                             }
                         }
-                        ns_take_piece<PARTS, T>(A, *o.J, p.kind, p.last, p.from, o.i * 128 + part * 32, o.j * 128 + c * 32, v, piece, lane, old, -1);
+                        ns_take_piece<PARTS, T>(A, A.job[o.job], p.kind, p.last, p.from, o.i * 128 + part * 32, o.j * 128 + c * 32, v, piece, lane, old, -1);
                     }
                 }
             }
