@@ -11,7 +11,7 @@
 //   PARTS = 2 (float32, float16 weights): v = hi + lo, two fp16 values, 22 bits and a sign;  v w ~ hi hi + hi lo + lo hi, the
 //     left out lo lo being 2^-24 of it.  Three products instead of one, and results as good as fp32 arithmetic's.
 //   PARTS = 1 (bfloat16 weights, whose update is rounded to 8 bits in the end): v = hi.
-// Sums are fp32: of 64 products in tensor memory where there are two parts, longer ones in registers (see kGroup).
+// Sums are fp32: of 64 products in tensor memory where there are two parts, longer ones in registers (see NsTile::group).
 //
 // X, A and B = b A + c A A live in the workspace as blocks of 128 x 64 elements, padded with zeros, each block laid out as the
 // tensor core reads it from shared memory (tensor.cuh), hi before lo: every load is a contiguous copy of 8 to 32 KB, whatever
@@ -308,11 +308,18 @@ struct NsTile {
     static constexpr int kFixed = 1024 + 512 + kTakers * kPiece + kExchange;
     static constexpr int kStages = (227 * 1024 - kFixed) / kStage > 6 ? 6 : (227 * 1024 - kFixed) / kStage;
     static constexpr size_t kSmem = kFixed + (size_t)kStages * kStage;
-    // Steps of 64 whose sum stays in tensor memory.  The tensor core cuts what it adds to a sum instead of rounding it: over the
-    // 375 additions of a sum of 2000 products in two parts that is a bias of 1e-5, ten times the rounding of fp32 sums.  So
-    // with two parts the sums of 64 products are added up in registers, rounded, while the next ones are made: 2000 x 333 is 2.0e-6
-    // off after five steps (fp32 products: 2.2e-6), with sums of 128 3.5e-6; 4096 x 4096 takes 3.86 ms for it instead of 3.6.
-    static constexpr int kGroup = PARTS == 2 ? 1 : 1 << 20;
+    // Of `steps` steps of 64, how many have their sum in tensor memory at a time.  The tensor core cuts what it adds to a sum instead of
+    // rounding it: over the 375 additions of a sum of 2000 products in two parts that is a bias of 1e-5, ten times the rounding
+    // of fp32 sums.  So with two parts the sums of 64 products are added up in registers, rounded, while the next ones are made:
+    // 2000 x 333 is 2.4e-6 off after five steps (fp32 products: 2.5e-6), with sums of 128 4e-6.  In a pair's tiles, groups of more
+    // steps let the products run further ahead while a tile's results are taken, and long sums are further off in fp32 too:
+    // 4096 x 4096 3.70 / 3.47 / 3.36 / 3.35 ms and 1.0 / 1.2 / 1.6 / 1.9e-6 off with groups of 1 / 2 / 3 / 4 (fp32 products 4.8e-6), 700 x 700
+    // 1.5 / 2.0e-6 with 2 / 3 (2.7e-6), 260 x 140 0.9 / 1.8 / 2.1e-6 with 1 / 2 / 3 (1.6e-6).
+    static __device__ __forceinline__ int group(int steps)
+    {
+        if (PARTS == 1) return 1 << 20;
+        return MODE != kPair || steps < 8 ? 1 : steps < 16 ? 2 : 3;
+    }
 };
 
 // 32 rows x 32 columns of a block in global memory and a warp's piece of shared memory: row by row 64 bytes, of which a lane
@@ -640,8 +647,9 @@ __global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_ker
                 const Phase p = phase_at(ph, kind);
                 for (int tile = p.tile; fine && tile < p.tiles; tile += p.step) {
                     const Spot o = spot_at(p, tile);
-                    for (int k = o.k0; k < o.k1; ++k) {
-                        const bool first = (k - o.k0) % Tile::kGroup == 0;
+                    const int group = Tile::group(o.k1 - o.k0);
+                    for (int k = o.k0, in = 0; k < o.k1; ++k) {
+                        const bool first = in == 0;
                         if (first && !mbar_wait_bounded(taken + slot, again ^ 1, kWaitLimit)) { fine = false; break; }
                         if (!mbar_wait_bounded(full + s, turn, kWaitLimit)) { fine = false; break; }
                         if (CG == 2 && !mbar_wait_bounded(ready + s, turn, kWaitLimit)) { fine = false; break; }
@@ -664,7 +672,8 @@ __global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_ker
                         for (int q = 0; q < 4; ++q) product<CG>(d, l + q * dl, r + q * dr, shape, PARTS == 2 || !first || q > 0);
                         product_commit<CG>(empty + s);
                         if (++s == S) { s = 0; turn ^= 1; }
-                        if ((k + 1 - o.k0) % Tile::kGroup == 0 || k + 1 == o.k1) {
+                        if (++in == group || k + 1 == o.k1) {
+                            in = 0;
                             product_commit<CG>(done + slot);
                             if ((slot ^= 1) == 0) again ^= 1;
                         }
@@ -704,7 +713,7 @@ __global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_ker
             for (int tile = p.tile; fine && tile < p.tiles; tile += p.step) {
                 const Spot o = spot_at(p, tile);
                 const NsJob &J = A.job[o.job];
-                const int groups = (o.k1 - o.k0 + Tile::kGroup - 1) / Tile::kGroup, rb = ns_rb(J.m);
+                const int group = Tile::group(o.k1 - o.k0), groups = (o.k1 - o.k0 + group - 1) / group, rb = ns_rb(J.m);
                 const int il = o.i + pair, c0 = (w >> 2) * Tile::kWide, jl = o.j + (c0 >> 7);      // this warp's columns of the tile; its blocks
                 const bool mine = il < rb && jl < (p.kind != kUpdate ? rb : ns_rb(J.n)) && !(p.kind != kUpdate && jl < il);
                 const int r0 = il * 128 + quarter * 32, c = o.j * 128 + c0;
@@ -1037,7 +1046,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
         for (int q = 0; q < 4; ++q)
             if (q < count) product<1>(d, left + q * dl, right + q * dr, shape, PARTS == 2 || add || q > 0);
     };
-    // sums of at most a few blocks each, added up in registers (see kGroup)
+    // sums of at most a few blocks each, added up in registers (see NsTile::group)
     const int sums = PARTS == 2 ? max(1, min(512 / R, (nb + 1) / 2)) : 1;
 
     for (int s = 0; s < steps; ++s) {
