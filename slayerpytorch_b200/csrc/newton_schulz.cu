@@ -567,14 +567,16 @@ __global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_ker
         o.k1 = steps * (p.rank + 1) / p.split;
         return o;
     };
-    // Most matrices give a CTA one tile a phase, the same one in every step: worked out once (some 300 instructions one after the
-    // other, which would stand between the phases).
+    // The same tiles in every step: the first few are worked out once (some 300 instructions one after the other, which would stand
+    // between the phases, and between the tiles of a phase).
+    constexpr int kSpots = 4;
     __shared__ Phase phases[3];
-    __shared__ Spot firsts[3];
-    if (threadIdx.x < 3) {
-        const Phase p = phase_of(threadIdx.x);
-        phases[threadIdx.x] = p;
-        if (p.tile < p.tiles) firsts[threadIdx.x] = locate(p, p.tile);
+    __shared__ Spot spots[3][kSpots];
+    if (threadIdx.x < 3 * kSpots) {
+        const int kind = threadIdx.x / kSpots, it = threadIdx.x % kSpots;
+        const Phase p = phase_of(kind);
+        if (it == 0) phases[kind] = p;
+        if (p.tile + it * p.step < p.tiles) spots[kind][it] = locate(p, p.tile + it * p.step);
     }
     __syncthreads();
     auto phase_at = [&](int ph, int kind) {
@@ -583,7 +585,7 @@ __global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_ker
         p.last = ph + 1 == 3 * P.steps;
         return p;
     };
-    auto spot_at = [&](const Phase &p, int tile) { return tile == p.tile ? firsts[p.kind] : locate(p, tile); };
+    auto spot_at = [&](const Phase &p, int tile, int it) { return it < kSpots ? spots[p.kind][it] : locate(p, tile); };
     // whether step k takes an operand from across the diagonal (of the two row blocks of a pair, which take it alike, one may be the
     // diagonal's own, which is the same either way)
     auto left_turned = [&](int kind, int i, int k) { return kind != kGram && (k >> 1) < i + CG - 1; };
@@ -602,8 +604,8 @@ __global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_ker
                     fence_async_global();
                 }
                 const Phase p = phase_at(ph, kind);
-                for (int tile = p.tile; fine && tile < p.tiles; tile += p.step) {
-                    const Spot o = spot_at(p, tile);
+                for (int tile = p.tile, it = 0; fine && tile < p.tiles; tile += p.step, ++it) {
+                    const Spot o = spot_at(p, tile, it);
                     const NsJob &J = A.job[o.job];
                     const int cbm = ns_cb(J.m), cbn = ns_cb(J.n), rb = ns_rb(J.m);
                     const int cbl = p.kind == kGram ? cbn : cbm, cbr = p.kind == kPolynomial ? cbm : cbn;
@@ -645,8 +647,8 @@ __global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_ker
             int s = 0, turn = 0, slot = 0, again = 0;
             for (int ph = 0, kind = 0; fine && ph < 3 * P.steps; ++ph, kind = kind == 2 ? 0 : kind + 1) {
                 const Phase p = phase_at(ph, kind);
-                for (int tile = p.tile; fine && tile < p.tiles; tile += p.step) {
-                    const Spot o = spot_at(p, tile);
+                for (int tile = p.tile, it = 0; fine && tile < p.tiles; tile += p.step, ++it) {
+                    const Spot o = spot_at(p, tile, it);
                     const int group = Tile::group(o.k1 - o.k0);
                     for (int k = o.k0, in = 0; k < o.k1; ++k) {
                         const bool first = in == 0;
@@ -685,8 +687,8 @@ __global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_ker
             int s = 0, turn = 0;
             for (int ph = 0, kind = 0; fine && ph < 3 * P.steps; ++ph, kind = kind == 2 ? 0 : kind + 1) {
                 const Phase p = phase_at(ph, kind);
-                for (int tile = p.tile; fine && tile < p.tiles; tile += p.step) {
-                    const Spot o = spot_at(p, tile);
+                for (int tile = p.tile, it = 0; fine && tile < p.tiles; tile += p.step, ++it) {
+                    const Spot o = spot_at(p, tile, it);
                     for (int k = o.k0; k < o.k1; ++k) {
                         if (!mbar_wait_bounded(full + s, turn, kWaitLimit)) { fine = false; break; }
                         mbar_arrive_at(ready + s, 0);
@@ -710,8 +712,8 @@ __global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_ker
                 if (lane == 0) fine = grid_wait_bounded(P.arrived, ph * gridDim.x, kWaitLimit);
                 fine = __all_sync(0xffffffffu, fine);
             }
-            for (int tile = p.tile; fine && tile < p.tiles; tile += p.step) {
-                const Spot o = spot_at(p, tile);
+            for (int tile = p.tile, it = 0; fine && tile < p.tiles; tile += p.step, ++it) {
+                const Spot o = spot_at(p, tile, it);
                 const NsJob &J = A.job[o.job];
                 const int group = Tile::group(o.k1 - o.k0), groups = (o.k1 - o.k0 + group - 1) / group, rb = ns_rb(J.m);
                 const int il = o.i + pair, c0 = (w >> 2) * Tile::kWide, jl = o.j + (c0 >> 7);      // this warp's columns of the tile; its blocks
@@ -794,7 +796,7 @@ __global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_ker
                 __syncwarp();
                 if (lane < p.split) mbar_release_at(given + p.kind, rank - p.rank + lane);
                 if (p.tile < p.tiles) {
-                    const Spot &o = firsts[kind];
+                    const Spot &o = spots[kind][0];
                     // this CTA's pieces of 32 x 32; warp w takes the w-th of them
                     const int many = 16 / p.split, id = w * p.split + p.rank, part = id & 3, c = id >> 2;
                     NsOld<PARTS> old;
