@@ -419,7 +419,8 @@ int slayer_b200_srm_get_spikes_noalloc_status(int64_t rows, int64_t T, int64_t *
  * hardware barrier (bulk tensor copies) poll a bounded number of times; if a wait ever runs
  * out they record a non-zero code here and return instead of hanging.  *status_out is 0 when
  * nothing went wrong.  This call synchronises with the device (it copies the word back), so
- * it belongs after a batch of work, not between launches.  It has no counterpart in the
+ * it belongs after a batch of work, not between launches.  Codes: 0x5101 a lost bulk copy, 0x5102
+ * the filters' buffers, 0x5103 the Newton-Schulz products.  It has no counterpart in the
  * reference, whose kernels neither wait on anything nor report errors.
  */
 int slayer_b200_device_status(int *status_out);
