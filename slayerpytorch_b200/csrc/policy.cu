@@ -6,11 +6,11 @@
 //                     d per / d lp = -(r A where that is the smaller one) + kl (1 - exp(d))
 //   preference        m_s = sum of a sequence's lp - ref_s,  h = beta (m_first - m_second),
 //                     per pair (1 - e) log(1 + exp(-h)) + e log(1 + exp(h))
-// What bounds the kernels is one read of the logits and one write of their gradient (HBM).  A row is read once: its running
+// What bounds the kernels is one read of the logits and one write of their gradient (HBM).  A row is read once from there: its running
 // maximum and its sum of exponentials relative to that maximum are carried along (each thread's own, joined at the row's
-// end), and the row itself waits in shared memory until its coefficient is known; the gradient is then formed from there.
-// A thread keeps and takes back the 16-byte pieces that it loaded itself, so the copy needs no barrier.  A long row has a CTA of
-// its own, a few of them on an SM: while one waits for its row's coefficient the others load.  Sums of
+// end), and the gradient is formed from a second read, out of the L2 cache, which holds the rows that are being worked on.  (Kept in shared
+// memory instead, a row of 64 KB leaves room for three CTAs on an SM, not four: 4096 x 32768 bfloat16 115 us, read again 108.)
+// A long row has a CTA of its own, a few of them on an SM: while one waits for its row's coefficient the others load.  Sums of
 // exponentials are fp32 (each relative to the row's maximum, at most V terms of at most 1, added in a tree over the
 // threads); what is said of one row - lp, the ratio, the loss - is computed in double, because a ratio that lies next to a
 // border of the clip range decides whether the row has a gradient at all.  A double exponential takes as long as a quarter of a
@@ -355,13 +355,11 @@ __global__ void __launch_bounds__(256) rows_short_kernel(RowArgs A)
 
 // -------------------------------------------------------------------------------------------- long rows
 // A CTA per row, or a cluster of them; each has its own stretch of the row, cut at 16-byte boundaries.
-template <typename T, RowMode MODE, bool KEEP>
+template <typename T, RowMode MODE>
 __global__ void __launch_bounds__(512, 2) rows_long_kernel(RowArgs A)
 {
     using P = Piece<T>;
     constexpr int N = P::N;
-    extern __shared__ __align__(16) unsigned char kept_bytes[];
-    uint4 *kept = (uint4 *)kept_bytes;
     __shared__ float2 part[16];          // the warps' maxima and sums
     __shared__ float2 whole[2];          // this CTA's, by the row's parity: the others of a cluster may read the one before
     __shared__ float4 result;
@@ -387,7 +385,7 @@ __global__ void __launch_bounds__(512, 2) rows_long_kernel(RowArgs A)
         // a piece of the gradient: as one if it lies like the logits, else element by element
         const auto store = [&](int p, const float (&f)[N]) {
             if (wide) {
-                gp[p] = P::close(f);
+                __stcs(gp + p, P::close(f));
             } else {
 #pragma unroll
                 for (int i = 0; i < N; ++i) g[head + p * N + i] = from_f<T>(f[i]);
@@ -413,22 +411,14 @@ __global__ void __launch_bounds__(512, 2) rows_long_kernel(RowArgs A)
                 uint4 v[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[i] = xp[p + i * threads];
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (KEEP) kept[p - p0 + i * threads] = v[i];
                 soft.template add<T>(v, A.k);
             }
             for (; p + threads < p1; p += 2 * threads) {
                 const uint4 v[2] = {xp[p], xp[p + threads]};
-                if (KEEP) {
-                    kept[p - p0] = v[0];
-                    kept[p - p0 + threads] = v[1];
-                }
                 soft.template add<T>(v, A.k);
             }
             if (p < p1) {
                 const uint4 v[1] = {xp[p]};
-                if (KEEP) kept[p - p0] = v[0];
                 soft.template add<T>(v, A.k);
             }
             if (has_head) {
@@ -479,10 +469,11 @@ __global__ void __launch_bounds__(512, 2) rows_long_kernel(RowArgs A)
             const float cx = result.x, cs = result.y, m = result.z, shift = Soft::shift(m, A.k);
             const int a = __float_as_int(result.w);
             const auto value = [&](float v, float chosen) { return fmaf(-cs, Soft::power(v, m, shift, A.k), chosen); };
-            for (int p = p0 + tid; p < p1; p += threads) {
+            const bool large = Soft::huge(m);
+            const auto make = [&](int p, const uint4 &v) {
                 float e[N];
-                P::open(e, KEEP ? kept[p - p0] : xp[p]);
-                if (Soft::huge(m)) {
+                P::open(e, v);
+                if (large) {
 #pragma unroll
                     for (int i = 0; i < N; ++i) e[i] = value(e[i], 0.0f);
                 } else {
@@ -490,7 +481,16 @@ __global__ void __launch_bounds__(512, 2) rows_long_kernel(RowArgs A)
                     for (int i = 0; i < N; ++i) e[i] = -cs * two_to(fmaf(e[i], A.k, -shift));
                 }
                 store(p, e);
+            };
+            int p = p0 + tid;
+            for (; p + 3 * threads < p1; p += 4 * threads) {
+                uint4 v[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = xp[p + i * threads];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) make(p + i * threads, v[i]);
             }
+            for (; p < p1; p += threads) make(p, xp[p]);
             // the chosen entry, behind its piece's own store
             const int pa = (a - head) / N;
             if (a >= head && pa >= p0 && pa < p1 && (pa - p0) % threads == tid) g[a] = from_f<T>(value(to_f(x[a]), cx));
@@ -514,30 +514,24 @@ int launch_rows(const RowArgs &A, cudaStream_t stream)
         else rows_short_kernel<T, MODE, 32><<<grid, 256, 0, stream>>>(A);
         return check_launch("rows kernel launch");
     }
-    const size_t bytes = ((size_t)A.V * sizeof(T) + 15) / 16 * 16, most = 100 * 1024;
-    // us with 128 / 256 / 512 threads (value and gradient): 4096 x 32768 bfloat16 160 / 123 / 127, 1505 x 50021 float32 182 / 149 / 142
-    const int threads = bytes <= 4096 ? 128 : bytes <= 80 * 1024 ? 256 : 512;
-    // CTAs per row: while there are SMs without one.  (A row that is too long for the shared memory kept for it is read again, out
-    // of the L2 cache: 1505 x 50021 float32 141 us, cut in two to be kept 158.)
+    const size_t bytes = (size_t)A.V * sizeof(T);
+    // us with 128 / 256 / 512 threads (value and gradient): 20000 x 2048 bfloat16 107 / 164 / 298, 6000 x 8192 float32 87 / 97 / 144,
+    // 3000 x 16384 float32 105 / 89, 4096 x 32768 bfloat16 144 / 122 / 144, 1505 x 50021 float32 191 / 167 / 146
+    const int threads = bytes <= 32 * 1024 ? 128 : bytes <= 128 * 1024 ? 256 : 512;
+    // CTAs per row: while there are SMs without one
     int C = 1;
     while (C < 8 && A.rows * C * 2 <= sms && (size_t)A.V / C > 8192) C *= 2;
     if (A.rows * C > 0x7fffffff) {
         set_error("%lld rows of %d entries", (long long)A.rows, A.V);
         return SLAYER_B200_EUNSUPPORTED;
     }
-    const int64_t stretch = (ceil_div(bytes / 16, C) + 1) * 16;
-    const bool keep = MODE == kPolicy && A.grad && stretch <= (int64_t)most;
-    const size_t smem = keep ? (size_t)stretch : 0;
-    auto kern = keep ? rows_long_kernel<T, MODE, MODE == kPolicy> : rows_long_kernel<T, MODE, false>;
-    int rc = reserve_dynamic_smem((const void *)kern, smem);
-    if (rc) return rc;
+    auto kern = rows_long_kernel<T, MODE>;
     cudaLaunchConfig_t cfg = {};
     // a row each: with rows dealt out to resident CTAs, masked rows make some end early (4096 x 32768 bfloat16, a third of the rows
     // masked, 128 us, as it is 116).  A gradient that may be there already should be told so to few CTAs.
     const int64_t cap = sms * 8 / C;
     cfg.gridDim = dim3((unsigned)((MODE == kGrad && A.only_if_not_one && A.rows > cap ? cap : A.rows) * C));
     cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
