@@ -528,7 +528,7 @@ int launch_rows(const RowArgs &A, cudaStream_t stream)
     auto kern = rows_long_kernel<T, MODE>;
     cudaLaunchConfig_t cfg = {};
     // a row each: with rows dealt out to resident CTAs, masked rows make some end early (4096 x 32768 bfloat16, a third of the rows
-    // masked, 128 us, as it is 116).  A gradient that may be there already should be told so to few CTAs.
+    // masked, 128 us, a row each 116 in the same build).  A gradient that may be there already should be told so to few CTAs.
     const int64_t cap = sms * 8 / C;
     cfg.gridDim = dim3((unsigned)((MODE == kGrad && A.only_if_not_one && A.rows > cap ? cap : A.rows) * C));
     cfg.blockDim = dim3(threads);
