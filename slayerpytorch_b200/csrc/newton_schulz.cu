@@ -290,9 +290,9 @@ __global__ void __launch_bounds__(256) ns_normalise_kernel(const __grid_constant
 // ------------------------------------------------------------------------------------------------ products
 enum NsPhase { kGram, kPolynomial, kUpdate };
 
-
-// MODE kAlone: a CTA makes tiles of 128 x 128.  kShared: so, and where there are few tiles several CTAs share one.  kPair: two CTAs make tiles of 256 x 256 together, each with half of either operand, so
-// that a CTA loads as much per step for four times the products of a pair.
+// MODE kAlone: a CTA makes tiles of 128 x 128.  kShared: so, and where there are few tiles several CTAs share one.  kPair: two CTAs
+// make tiles of 256 x 256 together, each with half of either operand, so that a CTA loads as much per step for four times the
+// products of a pair.
 enum NsMode { kAlone, kShared, kPair };
 
 template <int PARTS, int MODE>
@@ -1355,7 +1355,10 @@ static int ns_run(NsArgs &A, int steps, cudaStream_t st)
     constexpr size_t smem = NsTile<PARTS, MODE>::kSmem;
     int rc = reserve_dynamic_smem((const void *)kern, smem);
     if (rc) return rc;
-    // CTAs that share a tile where there are too few tiles for the SMs, each with two steps of 64 at least
+    // CTAs that share a tile where there are too few tiles for the SMs, each with two steps of 64 at least, of one part (a third of the
+    // products) four.  Five steps with two / four / eight, us: float32 512 x 512 130 / 149 / 173, 2000 x 333 153 / 162 / 173; bfloat16 300 x 300
+    // 109 / 99 / 99, 512 x 512 109 / 114 / 108, 768 x 768 122 / 128 / 129, 2000 x 333 126 / 114 / 118.
+    const int least = PARTS == 2 ? 4 : 8;
     const int index[3] = {ns_cb(n), ns_cb(m), ns_cb(m)};
     int ranks = CG, resident = 0;
     for (int most = MODE == kShared ? 8 : 1;; most = ranks) {
@@ -1363,7 +1366,7 @@ static int ns_run(NsArgs &A, int steps, cudaStream_t st)
         const int sms = resident ? resident : sm_count();
         for (int k = 0; k < 3; ++k) {
             P.split[k] = 1;
-            while (P.split[k] < most && P.tiles[k] * P.split[k] * 2 <= sms && index[k] >= P.split[k] * 4) P.split[k] *= 2;
+            while (P.split[k] < most && P.tiles[k] * P.split[k] * 2 <= sms && index[k] >= P.split[k] * least) P.split[k] *= 2;
             if (CG == 1) ranks = P.split[k] > ranks ? P.split[k] : ranks;
         }
         const int held = resident_clusters((const void *)kern, ranks, NsTile<PARTS, MODE>::kThreads, smem) * ranks;
@@ -1498,7 +1501,9 @@ static int ns_tiled(NsArgs &A, int steps, cudaStream_t st)
     const int C = ns_small_cluster(A, PARTS);
     if (C) return ns_run_small<T, PARTS>(A, C, steps, st);
 
-    // tiles of two CTAs where there are enough of them
+    // Tiles of two CTAs where there are enough of them; where there are few tiles, CTAs that share them.  Five steps, us, alone / shared /
+    // in pairs: float32 512 x 512 170 / 130 / 266, 1024 x 1024 257 / 208 / 373, 1536 x 1536 362 / 368 / 483, 2048 x 2048 586 / 591 / 618,
+    // 2304 x 2304 1079 / 1075 / 870; bfloat16 1024 x 2048 188 / 173 / 231, 2048 x 2048 325 / 326 / 315, 2304 x 2304 545 / 549 / 430
     int64_t tiles = 0;
     for (int j = 0; j < A.jobs; ++j) tiles += (int64_t)((ns_rb(A.job[j].m) + 1) / 2) * ((ns_rb(A.job[j].n) + 1) / 2);
     if (tiles >= sm_count() / 2) return ns_run<T, PARTS, kPair>(A, steps, st);
