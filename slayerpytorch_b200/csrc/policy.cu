@@ -138,21 +138,40 @@ struct Piece {
     }
 };
 
-// Maximum m and sum of exponentials s of part of a row: s = sum of 2^(x k - c), c = m k rounded.  One multiply-add an entry; that c
-// is not m k exactly changes s and the gradient's exponentials alike, and log_sum takes it out again.  Only where m k
-// would overflow are the exponentials taken of (x - m) k.
+// The exponentials of a part of a row with maximum m: 2^((x - base) k - c).  Near zero base is 0 and c = m k rounded: one multiply-add
+// an entry.  That c is not m k exactly changes sums and the gradient's exponentials alike, and log_sum takes it out again.
+// But the rounding of c grows with it (half a step is 2^-11 at 2^14 and 128 at 2^32, where 2^that is no float any more): where
+// |m k| > 2^14, in rows that are filled with something or lie far from zero, base is m and c is 0, one instruction more an entry.
+struct Frame {
+    float base = 0.0f, c = 0.0f;
+    __device__ __forceinline__ Frame(float m, float k)
+    {
+        c = __fmul_rn(m, k);
+        if (!(fabsf(c) <= 16384.0f)) {
+            base = m > -INFINITY ? m : 0.0f;           // (a part that holds only -inf has exponentials of 0, not of -inf + inf)
+            c = 0.0f;
+        }
+    }
+    __device__ __forceinline__ bool near() const { return base == 0.0f; }
+    __device__ __forceinline__ float power(float x, float k) const { return two_to(fmaf(x - base, k, -c)); }
+};
+
+// Maximum and sum of exponentials of part of a row.
 struct Soft {
     float m = -INFINITY, s = 0.0f;
-    __device__ __forceinline__ static bool huge(float m) { return fabsf(m) > 1e37f; }
-    // (a part that holds only -inf has exponentials of 0, not of -inf + inf)
-    __device__ __forceinline__ static float shift(float m, float k) { return huge(m) ? 0.0f : __fmul_rn(m, k); }
-    __device__ __forceinline__ static float power(float x, float m, float c, float k) { return two_to(huge(m) && m > -INFINITY ? (x - m) * k : fmaf(x, k, -c)); }
-    // a sum relative to m as one relative to n >= m
-    __device__ __forceinline__ void raise(float n, float k)
+    // the sum as one relative to n >= m, whose frame that of m becomes
+    __device__ __forceinline__ void raise(float n, float k, Frame &f)
     {
         if (n == m) return;
-        s *= m == -INFINITY ? 0.0f : two_to(huge(n) || huge(m) ? (m - n) * k : shift(m, k) - shift(n, k));
+        const Frame to(n, k);
+        s *= m == -INFINITY ? 0.0f : two_to(fmaf(f.base - to.base, k, f.c - to.c));
         m = n;
+        f = to;
+    }
+    __device__ __forceinline__ void raise(float n, float k)
+    {
+        Frame f(m, k);
+        raise(n, k, f);
     }
     template <int N>
     __device__ __forceinline__ void add(const float (&v)[N], float k)
@@ -161,11 +180,21 @@ struct Soft {
 #pragma unroll
         for (int i = 0; i < N; ++i) n = fmaxf(n, v[i]);
         raise(n, k);
-        const float c = shift(m, k);
+        const Frame f(m, k);
         float t = 0.0f;
 #pragma unroll
-        for (int i = 0; i < N; ++i) t += power(v[i], m, c, k);
+        for (int i = 0; i < N; ++i) t += f.power(v[i], k);
         s += t;
+    }
+    // a short row's elements, `step` apart; the frame of m is carried along (200000 x 500 float32 233 us; made anew an element 419)
+    template <typename T>
+    __device__ __forceinline__ void add_row(const T *x, int n, int step, float k, Frame &f)
+    {
+        for (int j = 0; j < n; j += step) {
+            const float v = to_f(x[j]);
+            raise(fmaxf(m, v), k, f);
+            s += f.power(v, k);
+        }
     }
     // pieces of a row: their maximum first, of 16-bit entries two at a time
     template <typename T, int NB>
@@ -188,15 +217,15 @@ struct Soft {
             n = fmaxf(n, fmaxf(both[0], both[1]));
         }
         raise(n, k);
-        const float c = shift(m, k);
+        const Frame f(m, k);
         float t[4] = {};
-        if (!huge(m)) {
+        if (f.near()) {
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 float e[P::N];
                 P::open(e, v[b]);
 #pragma unroll
-                for (int i = 0; i < P::N; ++i) t[i & 3] += two_to(fmaf(e[i], k, -c));
+                for (int i = 0; i < P::N; ++i) t[i & 3] += two_to(fmaf(e[i], k, -f.c));
             }
         } else {
 #pragma unroll
@@ -204,7 +233,7 @@ struct Soft {
                 float e[P::N];
                 P::open(e, v[b]);
 #pragma unroll
-                for (int i = 0; i < P::N; ++i) t[0] += power(e[i], m, c, k);
+                for (int i = 0; i < P::N; ++i) t[0] += f.power(e[i], k);
             }
         }
         s += (t[0] + t[1]) + (t[2] + t[3]);
@@ -213,17 +242,24 @@ struct Soft {
     template <int G>
     __device__ __forceinline__ void meet(float k)
     {
+        Frame f(m, k);
+        meet<G>(k, f);
+    }
+    template <int G>
+    __device__ __forceinline__ void meet(float k, Frame &f)
+    {
         float n = m;
 #pragma unroll
         for (int o = G / 2; o > 0; o >>= 1) n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, o));
-        raise(n, k);
+        raise(n, k, f);
 #pragma unroll
         for (int o = G / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     }
-    // log of c's rounding: sum of exp((x - m) scale) = s (1 + that)
+    // log of c's rounding: sum of exp((x - m) scale) = s exp(that)
     __device__ __forceinline__ static double rounding(float m, float k)
     {
-        return huge(m) ? 0.0 : ((double)shift(m, k) - (double)m * (double)k) * 0.6931471805599453;
+        const Frame f(m, k);
+        return f.near() && m > -INFINITY ? ((double)f.c - (double)m * (double)k) * 0.6931471805599453 : 0.0;
     }
     __device__ __forceinline__ static double log_sum(float m, float s, float k) { return log((double)s) + rounding(m, k); }
 };
@@ -273,7 +309,7 @@ __device__ __forceinline__ RowFacts row_facts(const RowArgs &A, int64_t row, con
 
 // What one row comes to, from its maximum m and sum s.  Called by `lanes` together (lane: which of its row's); `write`: the first of
 // these lanes stores the row's results.  Returns (c, c (1 / s)) to the first lane: the gradient is
-// c * (j == a) - c (1 / s) * 2^(x[j] k - m k).
+// c * (j == a) - c (1 / s) * 2^((x[j] - base) k - c').
 template <RowMode MODE>
 __device__ __forceinline__ float2 row_result(const RowArgs &A, int64_t row, const RowFacts &f, float m, float s, int lane, unsigned lanes, bool write)
 {
@@ -289,7 +325,7 @@ __device__ __forceinline__ float2 row_result(const RowArgs &A, int64_t row, cons
         } else {
             // the first lane's is the ratio's exponential, the second's the KL term's
             const double e = exp(lane == 0 ? gap - (double)f.old_lp : (double)f.ref_lp - gap);
-            const double off = Soft::rounding(m, A.k), sum = (double)s * (1.0 + off + 0.5 * off * off);      // off < 1e-5, or s is 0
+            const double off = Soft::rounding(m, A.k), sum = (double)s * (1.0 + off + 0.5 * off * off);      // |off| < 2^-11: exp(off) to 2e-11
             const double kl = A.ref_lp ? A.kl * (__shfl_down_sync(lanes, e, 1) * sum - 1.0) : 0.0;
             c = (float)(f.share * (clipped(A, e / sum, f.gain).y - kl));
             if (write) {
@@ -329,18 +365,16 @@ __global__ void __launch_bounds__(256) rows_short_kernel(RowArgs A)
         f.a = -1;
         if (live) f = row_facts<MODE>(A, row, x, A.action[row]);
         Soft soft;
+        Frame frame(soft.m, A.k);
         if (MODE != kGrad) {
-            if (live)
-                for (int j = lane; j < A.V; j += G) {
-                    const float v[1] = {to_f(x[j])};
-                    soft.add(v, A.k);
-                }
+            if (live) soft.add_row(x + lane, A.V - lane, G, A.k, frame);
             __syncwarp();
-            soft.meet<G>(A.k);
+            soft.meet<G>(A.k, frame);
         } else if (live) {
             const float2 st = A.stats[row];
             soft.m = st.x;
             soft.s = st.y;
+            frame = Frame(st.x, A.k);
         }
         __syncwarp();
         float2 c = row_result<MODE>(A, live ? row : 0, f, soft.m, soft.s, lane, 0xffffffffu, live);
@@ -349,7 +383,7 @@ __global__ void __launch_bounds__(256) rows_short_kernel(RowArgs A)
         c.y = __shfl_sync(0xffffffffu, c.y, 0, G);
         if (g)
             for (int j = lane; j < A.V; j += G)
-                g[j] = from_f<T>(live ? fmaf(-c.y, Soft::power(to_f(x[j]), soft.m, Soft::shift(soft.m, A.k), A.k), j == f.a ? c.x : 0.0f) : 0.0f);
+                g[j] = from_f<T>(live ? fmaf(-c.y, frame.power(to_f(x[j]), A.k), j == f.a ? c.x : 0.0f) : 0.0f);
     }
 }
 
@@ -466,19 +500,20 @@ __global__ void __launch_bounds__(512, 2) rows_long_kernel(RowArgs A)
         }
         if (g) {
             __syncthreads();
-            const float cx = result.x, cs = result.y, m = result.z, shift = Soft::shift(m, A.k);
+            const float cx = result.x, cs = result.y;
+            const Frame frame(result.z, A.k);
             const int a = __float_as_int(result.w);
-            const auto value = [&](float v, float chosen) { return fmaf(-cs, Soft::power(v, m, shift, A.k), chosen); };
-            const bool large = Soft::huge(m);
+            const auto value = [&](float v, float chosen) { return fmaf(-cs, frame.power(v, A.k), chosen); };
+            const bool near = frame.near();
             const auto make = [&](int p, const uint4 &v) {
                 float e[N];
                 P::open(e, v);
-                if (large) {
+                if (!near) {
 #pragma unroll
                     for (int i = 0; i < N; ++i) e[i] = value(e[i], 0.0f);
                 } else {
 #pragma unroll
-                    for (int i = 0; i < N; ++i) e[i] = -cs * two_to(fmaf(e[i], A.k, -shift));
+                    for (int i = 0; i < N; ++i) e[i] = -cs * two_to(fmaf(e[i], A.k, -frame.c));
                 }
                 store(p, e);
             };

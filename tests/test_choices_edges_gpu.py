@@ -1,0 +1,106 @@
+"""GPU: the losses of choices at their edges - logits filled with large values, margins without bound, empty inputs, many rows.
+
+Tolerances.  A row's sum of exponentials 2^((x - m) k) is held in fp32.  The argument d has up to three roundings of 2^-24 |d| (the
+difference, the product, k itself), which weigh on the sum as 3 ln 2 2^-24 E|d|, with E|d| <= log2(V) + 1 < 17: 2.2e-6; the exponential's
+own error is 2^-22; a running sum is raised to a new maximum at most 32 times (a lane of a short row; long rows 10 times) at
+2^-22 + 2^-24 each, 9.6e-6, and added to as often, 2e-6.  Together 1.4e-5 < SUM = 1.5e-5.  A softmax entry of more than
+2^-126 has its own exponential's 3 ln 2 2^-24 126 = 1.6e-5 on top of that: with the roundings of the coefficient and the product
+below REL = 4e-5 of |c| (delta + p).  The result's rounding is half a step of its type (`close`)."""
+import math
+
+import pytest
+import torch
+
+from slayerpytorch_b200 import loss
+from tests.test_choices_gpu import CLIP, SUM, TYPES, close, policy_want, want_grad, want_logp
+
+pytestmark = pytest.mark.gpu
+
+FILLS = [-1e4, -1e9, -1e10, -1e12, -1e20, -1e30, -1e36, -3.3895e38]
+
+
+def of_ratio(x, action, size, scale):
+    """What a gradient is off by where a coefficient made of `size` has its ratio from a log-probability that is off by SUM."""
+    p = torch.softmax(x.double() * scale, -1)
+    return scale * (size * SUM)[..., None] * (torch.zeros_like(p).scatter_(-1, action[..., None], 1.0) + p)
+
+
+def filled(V, dtype, seed):
+    """Rows of ordinary logits in which something is filled: (logits, an entry that is not)"""
+    gen = torch.Generator().manual_seed(seed)
+    fills = [f for f in FILLS if f >= torch.finfo(dtype).min] + [torch.finfo(dtype).min]
+    rows, action = [], []
+    for f in fills:
+        for where in (slice(0, 1), slice(V - 1, V), slice(0, V // 2), slice(V // 2, V), slice(1, V, 2), slice(0, V - 1)):
+            x = torch.randn(V, generator=gen) * 3
+            x[where] = f
+            left = (x > -1e3).nonzero()[:, 0]
+            rows.append(x)
+            action.append(left[torch.randint(0, len(left), (1,), generator=gen)])
+    x = torch.stack(rows).to(dtype)
+    return x, torch.cat(action), gen
+
+
+@pytest.mark.parametrize("scale", [1.0, 0.7, 0.2])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [10, 300, 5003, 40003])
+def test_filled_entries(V, dtype, scale):
+    """Illegal actions, a padded vocabulary, all but one entry: any finite fill leaves the row what it is without these entries."""
+    x, action, gen = filled(V, dtype, V)
+    up = torch.randn(len(x), generator=gen)
+    for rows in (slice(0, len(x)), slice(0, 12)):            # a CTA for each row; a cluster for each
+        leaf = x[rows].cuda().requires_grad_()
+        lp = loss.actionLogProb(leaf, action[rows].cuda(), scale=scale)
+        (g,) = torch.autograd.grad(lp, [leaf], up[rows].cuda())
+        close(lp.detach(), want_logp(x[rows], action[rows], scale), SUM)
+        close(g, *want_grad(x[rows], action[rows], up[rows].double(), scale))
+    lp = want_logp(x, action, scale)
+    old = (lp - torch.randint(0, 2, (len(x),), generator=gen) * 0.1 + 0.05).float()
+    adv = torch.randn(len(x), generator=gen)
+    leaf = x.cuda().requires_grad_()
+    got = loss.policyLoss(leaf, action.cuda(), old.cuda(), adv.cuda(), clip=CLIP, scale=scale)
+    (g,) = torch.autograd.grad(got, [leaf])
+    value, slack, coef, size = policy_want(x[:, None], action[:, None], old[:, None], adv[:, None], None, None, 0.0, "sum", scale)
+    assert abs(float(got.detach()) - float(value)) <= float(slack) + 2 ** -24 * abs(float(value))
+    grad, spare = want_grad(x, action, coef[:, 0], scale)
+    close(g, grad, spare + of_ratio(x, action, size[:, 0], scale))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [10, 300, 5003, 40003])
+def test_rows_of_equal_entries_of_any_size(V, dtype):
+    values = [s * 10.0 ** e for e in (0, 3, 4, 5, 6, 8, 9, 10, 12, 20, 30, 36, 37, 38) for s in (1, -1)]
+    x = torch.tensor(values)[:, None].expand(-1, V).to(dtype)
+    action = torch.arange(len(values)) % V
+    for scale in (1.0, 0.3, 7.0):
+        leaf = x.cuda().requires_grad_()
+        lp = loss.actionLogProb(leaf, action.cuda(), scale=scale)
+        (g,) = torch.autograd.grad(lp.sum(), [leaf])
+        close(lp.detach(), torch.full((len(values),), -math.log(V), dtype=torch.float64), SUM)
+        close(g, *want_grad(x, action, torch.ones(len(values), dtype=torch.float64), scale))
+
+
+@pytest.mark.parametrize("V", [10, 300, 5003, 40003])
+@pytest.mark.parametrize("top", [1e3, 1e4, 1.2e4, 1e5, 1e6, 1e7, 1e8, 1e12])
+def test_policy_value_and_gradient_have_one_ratio(top, V):
+    """Rows that lie far from zero: the gradient's ratio is the loss's, as near to 64 bits as anywhere."""
+    gen = torch.Generator().manual_seed(int(top))
+    step = max(1.0, top * 2.0 ** -23)                         # the entries are a few steps of float32 apart
+    scale = 0.9 / step
+    x = top + 3 * step * torch.randn(24, 1, V, generator=gen, dtype=torch.float64)
+    x = torch.cat([x, -x]).float()
+    action = torch.randint(0, V, (48, 1), generator=gen)
+    lp = want_logp(x, action, scale)
+    ratio = torch.tensor([0.3, 0.7, 0.95, 1.0, 1.1, 1.22, 2.5], dtype=torch.float64)[torch.randint(0, 7, (48, 1), generator=gen)]
+    old = (lp - ratio.log()).float()
+    ref = (lp + 0.5 * torch.randn(48, 1, generator=gen)).float()
+    adv = torch.randn(48, 1, generator=gen)
+    leaf = x.cuda().requires_grad_()
+    got = loss.policyLoss(leaf, action.cuda(), old.cuda(), adv.cuda(), refLogProb=ref.cuda(), clip=CLIP, klCoef=0.3, scale=scale)
+    (g,) = torch.autograd.grad(got, [leaf])
+    scale = float(torch.tensor(scale, dtype=torch.float32))   # what the kernels take it as
+    value, slack, coef, size = policy_want(x, action, old, adv, ref, None, 0.3, "sum", scale)
+    # |gap| <= 30 here: the scale's rounding is in `scale` itself
+    assert abs(float(got.detach()) - float(value)) <= float(slack) + 2 ** -24 * abs(float(value))
+    grad, spare = want_grad(x, action, coef, scale)
+    close(g, grad, spare + of_ratio(x, action, size, scale))
