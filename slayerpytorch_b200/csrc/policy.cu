@@ -680,11 +680,12 @@ __global__ void __launch_bounds__(256) pair_kernel(float *loss, float *coef, con
             const double h = fine ? beta * (margin[i] - margin[j]) : (double)NAN;
             const double tail = log1p(exp(-fabs(h)));
             const double down = h < 0.0 ? -h : h > 0.0 ? 0.0 : h, up = h > 0.0 ? h : h < 0.0 ? 0.0 : h;    // max(-h, 0), max(h, 0)
-            total += share * ((1.0 - smoothing) * (down + tail) + smoothing * (up + tail));
+            // (h has no bound where a choice is impossible: a term of weight 0 is 0 there too, and the slopes are the limits)
+            total += share * ((smoothing < 1.0 ? (1.0 - smoothing) * (down + tail) : 0.0) + (smoothing > 0.0 ? smoothing * (up + tail) : 0.0));
             const double e = exp(-fabs(h)), sig = (h >= 0.0 ? 1.0 : e) / (1.0 + e);
             first[threadIdx.x] = i;
             second[threadIdx.x] = j;
-            slope[threadIdx.x] = share * beta * (sig - (1.0 - smoothing)) + 0.0 * h;
+            slope[threadIdx.x] = share * beta * (sig - (1.0 - smoothing));
         }
         __syncthreads();
         const int n = (int)(P - p0 < 256 ? P - p0 : 256);

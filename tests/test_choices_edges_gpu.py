@@ -104,3 +104,35 @@ def test_policy_value_and_gradient_have_one_ratio(top, V):
     assert abs(float(got.detach()) - float(value)) <= float(slack) + 2 ** -24 * abs(float(value))
     grad, spare = want_grad(x, action, coef, scale)
     close(g, grad, spare + of_ratio(x, action, size, scale))
+
+
+def test_preference_of_impossible_choices():
+    """A choice of probability zero in one sequence of a pair: h is without bound, the slopes are its limits, and a term of weight 0 is 0."""
+    inf = float("inf")
+    for V in (6, 2000):
+        gen = torch.Generator().manual_seed(V)
+        x = torch.randn(4, 3, V, generator=gen)
+        action = torch.randint(1, V, (4, 3), generator=gen)
+        ref = torch.randn(4, generator=gen)
+        lp = want_logp(x, action).sum(1) - ref.double()
+        for at, smoothing in ((0, 0.0), (2, 0.0), (0, 0.25), (2, 0.25), (0, 1.0), (2, 1.0)):        # the preferred one's, the rejected one's
+            y = x.clone()
+            y[at, 1, action[at, 1]] = -inf
+            leaf = y.cuda().requires_grad_()
+            got = loss.preferenceLoss(leaf, action.cuda(), ref.cuda(), beta=0.4, labelSmoothing=smoothing)
+            (g,) = torch.autograd.grad(got, [leaf])
+            h = 0.4 * float(lp[1] - lp[3])
+            other = (1 - smoothing) * math.log1p(math.exp(-h)) + smoothing * math.log1p(math.exp(h))
+            weight = 1 - smoothing if at == 0 else smoothing        # of the side that has no bound
+            if weight:
+                assert float(got.detach()) == inf
+            else:
+                assert abs(float(got.detach()) - other) <= 0.8 * 3 * (SUM + 2 ** -24 * 20) + 2 ** -23 * other
+            slope = 0.4 * ((0.0 if at == 0 else 1.0) - (1 - smoothing))
+            rest = 0.4 * (1 / (1 + math.exp(-h)) - (1 - smoothing))
+            coef = torch.tensor([slope, rest, -slope, -rest], dtype=torch.float64)[:, None].expand(4, 3)
+            grad, spare = want_grad(y, action, coef)
+            p = torch.softmax(y.double(), -1)
+            delta = torch.zeros_like(p).scatter_(-1, action[..., None], 1.0)
+            # a slope is off by beta^2 / 4 of what the margins are off by
+            close(g, grad, spare + 0.04 * 2 * 3 * (SUM + 2 ** -24 * 20) * (delta + p))
