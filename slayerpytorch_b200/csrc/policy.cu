@@ -317,7 +317,7 @@ __device__ __forceinline__ float2 row_result(const RowArgs &A, int64_t row, cons
     if constexpr (MODE == kGrad) {
         c = (A.coef ? A.coef[(unsigned)row / (unsigned)A.coef_len] : 1.0f) * (A.upstream_rows ? A.upstream[row] : A.upstream[0]) * A.scale;
     } else {
-        const double gap = (double)(f.xa - m) * (double)A.scale;
+        const double gap = ((double)f.xa - (double)m) * (double)A.scale;
         write = write && lane == 0;
         if (write && A.stats) A.stats[row] = make_float2(m, s);
         if constexpr (MODE == kLogProb) {

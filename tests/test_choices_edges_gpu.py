@@ -136,3 +136,19 @@ def test_preference_of_impossible_choices():
             delta = torch.zeros_like(p).scatter_(-1, action[..., None], 1.0)
             # a slope is off by beta^2 / 4 of what the margins are off by
             close(g, grad, spare + 0.04 * 2 * 3 * (SUM + 2 ** -24 * 20) * (delta + p))
+
+
+@pytest.mark.parametrize("V", [10, 300, 5003, 40003])
+def test_choices_far_below_the_maximum(V):
+    """The distance of the chosen entry from the maximum is not rounded on the way (it may not even be a float32)."""
+    gen = torch.Generator().manual_seed(V)
+    x = torch.randn(64, V, generator=gen)
+    action = torch.randint(1, V, (64,), generator=gen)
+    x[:, 0] = 3000.0 + 40.0 * torch.rand(64, generator=gen)
+    x[0, 0], x[0, action[0]] = 3e38, -3e38
+    x[1, 0], x[1, action[1]] = 1e30, -2e38
+    # the maximum is all there is to the sum: off by its own exponential's 2^-22 and the sum's rounding; then one rounding of the result
+    for scale in (0.1, 0.4):
+        lp = loss.actionLogProb(x.cuda(), action.cuda(), scale=scale)
+        exact = float(torch.tensor(scale, dtype=torch.float32))
+        close(lp, want_logp(x, action, exact), 2.0 ** -21)
