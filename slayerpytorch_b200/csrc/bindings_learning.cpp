@@ -105,21 +105,20 @@ torch::Tensor rows_of(const torch::Tensor &logits)
     return rows;
 }
 
-// What the backward passes need of a row, in one buffer: stats (two floats a row), logp, coef, and a workspace.
+// What the backward passes need, in one buffer: stats (two floats a row) and coef, and behind them what the forward pass works with.
 struct RowBuffer {
     torch::Tensor all;
-    float *stats, *logp, *coef;
+    float *stats, *coef;
     void *workspace;
     RowBuffer(const torch::Tensor &like, int64_t rows, int64_t coefs, int64_t workspace_bytes)
-        : RowBuffer(torch::empty({4 + 2 * rows + rows + coefs + (workspace_bytes + 3) / 4}, like.options().dtype(torch::kFloat32)), rows, coefs)
+        : RowBuffer(torch::empty({2 + 2 * rows + coefs + (workspace_bytes + 3) / 4}, like.options().dtype(torch::kFloat32)), rows, coefs)
     {
     }
     RowBuffer(torch::Tensor buffer, int64_t rows, int64_t coefs) : all(std::move(buffer))
     {
-        const int64_t even = (3 * rows + coefs + 1) / 2 * 2;       // the workspace is aligned to 8 bytes
+        const int64_t even = (2 * rows + coefs + 1) / 2 * 2;       // the workspace is aligned to 8 bytes
         stats = all.data_ptr<float>();
-        logp = stats + 2 * rows;
-        coef = logp + rows;
+        coef = stats + 2 * rows;
         workspace = stats + even;
     }
 };
@@ -198,11 +197,12 @@ struct PolicyLoss : public torch::autograd::Function<PolicyLoss> {
         check_rows(advantage, "advantage", torch::kFloat32, rows / advLen, x);
         c10::cuda::CUDAGuard guard(x.device());
         auto loss = torch::empty({}, x.options().dtype(torch::kFloat32));
+        auto logp = torch::empty(action.sizes(), loss.options());       // the caller's own: nothing here reads it again
         RowBuffer buffer(x, rows, rows, slayer_b200_policy_loss_workspace(rows, seqLen));
         const bool early = want && x.scalar_type() != torch::kFloat16;
         torch::Tensor grad;
         if (early) grad = torch::empty({rows, V}, x.options());
-        check_rc(slayer_b200_policy_loss(loss.data_ptr<float>(), early ? grad.data_ptr() : nullptr, buffer.logp, buffer.stats, buffer.coef,
+        check_rc(slayer_b200_policy_loss(loss.data_ptr<float>(), early ? grad.data_ptr() : nullptr, logp.data_ptr<float>(), buffer.stats, buffer.coef,
                                          buffer.workspace, x.data_ptr(), dtype_code(x, "logits"), act.data_ptr<int64_t>(), old.data_ptr<float>(),
                                          advantage.data_ptr<float>(), advLen, or_null<float>(ref), m, rows, seqLen, V, x.stride(0), (float)scale,
                                          (float)low, (float)high, (float)kl, (int)reduction, current_stream()),
@@ -215,7 +215,6 @@ struct PolicyLoss : public torch::autograd::Function<PolicyLoss> {
                 ctx->saved_data["capture"] = capture_id(x);
             }
         }
-        auto logp = buffer.all.narrow(0, 2 * rows, rows).view(action.sizes());
         ctx->mark_non_differentiable({logp});
         return {loss, logp};
     }
@@ -255,11 +254,13 @@ struct PreferenceLoss : public torch::autograd::Function<PreferenceLoss> {
         const uint8_t *m = mask_of(keep, rows, x);
         c10::cuda::CUDAGuard guard(x.device());
         auto loss = torch::empty({}, x.options().dtype(torch::kFloat32));
-        RowBuffer buffer(x, rows, S, slayer_b200_preference_loss_workspace(S));
-        check_rc(slayer_b200_log_prob(buffer.logp, buffer.stats, x.data_ptr(), dtype_code(x, "logits"), act.data_ptr<int64_t>(), m, rows, x.size(1),
+        const int64_t bytes = slayer_b200_preference_loss_workspace(S);
+        RowBuffer buffer(x, rows, S, bytes + 4 * rows);
+        float *logp = (float *)((char *)buffer.workspace + bytes);
+        check_rc(slayer_b200_log_prob(logp, buffer.stats, x.data_ptr(), dtype_code(x, "logits"), act.data_ptr<int64_t>(), m, rows, x.size(1),
                                       x.stride(0), (float)scale, current_stream()),
                  "preferenceLoss");
-        check_rc(slayer_b200_preference_loss(loss.data_ptr<float>(), buffer.coef, buffer.workspace, buffer.logp, ref.data_ptr<float>(),
+        check_rc(slayer_b200_preference_loss(loss.data_ptr<float>(), buffer.coef, buffer.workspace, logp, ref.data_ptr<float>(),
                                              pairs.data_ptr<int64_t>(), S, L, pairs.size(0), (float)beta, (float)smoothing, (int)reduction,
                                              current_stream()),
                  "preferenceLoss");

@@ -152,3 +152,21 @@ def test_choices_far_below_the_maximum(V):
         lp = loss.actionLogProb(x.cuda(), action.cuda(), scale=scale)
         exact = float(torch.tensor(scale, dtype=torch.float32))
         close(lp, want_logp(x, action, exact), 2.0 ** -21)
+
+
+@pytest.mark.parametrize("V", [9, 1500])
+def test_the_returned_log_probabilities_are_the_callers_own(V):
+    gen = torch.Generator().manual_seed(V)
+    x, action = torch.randn(3, 4, V, generator=gen), torch.randint(0, V, (3, 4), generator=gen)
+    z = torch.zeros(3, 4, device="cuda")
+    leaf = x.cuda().requires_grad_()
+    want = torch.autograd.grad(loss.policyLoss(leaf, action.cuda(), z - 2, z + 1), [leaf])[0]
+    value, lp = loss.policyLoss(leaf, action.cuda(), z - 2, z + 1, returnLogProb=True)
+    kept = lp.clone()
+    lp.add_(5.0).exp_()                                       # written over before the backward passes
+    for up in (1.0, 1.0, 2.0):
+        (g,) = torch.autograd.grad(value * up, [leaf], retain_graph=True)
+        assert torch.equal(g, want * up)
+    close(kept, want_logp(x, action), SUM)
+    # and it holds no more than its rows
+    assert lp.untyped_storage().nbytes() <= 4 * 12 + 512
