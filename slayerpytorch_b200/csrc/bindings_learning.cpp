@@ -193,8 +193,8 @@ struct PolicyLoss : public torch::autograd::Function<PolicyLoss> {
         check_rows(old, "oldLogProb", torch::kFloat32, rows, x);
         if (ref.has_value()) check_rows(*ref, "refLogProb", torch::kFloat32, rows, x);
         const uint8_t *m = mask_of(keep, rows, x);
-        const int64_t advLen = advantage.numel() == rows ? 1 : seqLen;
-        check_rows(advantage, "advantage", torch::kFloat32, rows / advLen, x);
+        const int64_t advLen = rows == 0 || advantage.numel() == rows ? 1 : seqLen;
+        check_rows(advantage, "advantage", torch::kFloat32, rows == 0 ? advantage.numel() : rows / advLen, x);   // its shape has been checked
         c10::cuda::CUDAGuard guard(x.device());
         auto loss = torch::empty({}, x.options().dtype(torch::kFloat32));
         auto logp = torch::empty(action.sizes(), loss.options());       // the caller's own: nothing here reads it again

@@ -170,3 +170,12 @@ def test_the_returned_log_probabilities_are_the_callers_own(V):
     close(kept, want_logp(x, action), SUM)
     # and it holds no more than its rows
     assert lp.untyped_storage().nbytes() <= 4 * 12 + 512
+
+
+@pytest.mark.parametrize("reduction", ["sum", "mean", "sequence"])
+def test_sequences_without_choices_and_one_advantage_each(reduction):
+    leaf = torch.zeros(4, 0, 7, device="cuda", requires_grad=True)
+    none = torch.zeros(4, 0, device="cuda")
+    got = loss.policyLoss(leaf, none.long(), none, torch.ones(4, device="cuda"), reduction=reduction)
+    (g,) = torch.autograd.grad(got, [leaf])
+    assert float(got.detach()) == 0.0 and g.shape == leaf.shape
