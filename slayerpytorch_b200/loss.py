@@ -161,7 +161,7 @@ class spikeLoss(torch.nn.Module):
         region = self.errorDescriptor['tgtSpikeRegion']
         Ts = self.simulation['Ts']
         start, stop = int(np.rint(region['start'] / Ts)), int(np.rint(region['stop'] / Ts))
-        return torch.sum(spikeOut[..., start:stop], -1).reshape(spikeOut.shape[0], -1) * Ts
+        return torch.sum(spikeOut[..., start:stop], -1).reshape(spikeOut.shape[0], spikeOut.shape[1:-1].numel()) * Ts
 
     def actionLogProb(self, spikeOut, action):
         """Log-probability of each sample's choice among the output neurons: a softmax of ``countScale`` times their spike counts
@@ -189,7 +189,7 @@ class spikeLoss(torch.nn.Module):
         if action.dim() != 2 or action.numel() != counts.shape[0]:
             raise ValueError("preference: action must be [sequences, choices] with one entry per sample, got %s for %d samples"
                              % (tuple(action.shape), counts.shape[0]))
-        return preferenceLoss(counts.reshape(action.shape + (-1,)), action, refLogProb, pairs=pairs, mask=mask, beta=e.get('beta', 0.1),
+        return preferenceLoss(counts.reshape(action.shape + counts.shape[1:]), action, refLogProb, pairs=pairs, mask=mask, beta=e.get('beta', 0.1),
                               labelSmoothing=e.get('labelSmoothing', 0.0), scale=e.get('countScale', 1.0))
 
 

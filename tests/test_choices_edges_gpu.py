@@ -12,7 +12,7 @@ import pytest
 import torch
 
 from slayerpytorch_b200 import loss
-from tests.test_choices_gpu import CLIP, SUM, TYPES, close, policy_want, want_grad, want_logp
+from tests.test_choices_gpu import CLIP, SUM, TYPES, close, descriptor, policy_want, want_grad, want_logp
 
 pytestmark = pytest.mark.gpu
 
@@ -179,3 +179,19 @@ def test_sequences_without_choices_and_one_advantage_each(reduction):
     got = loss.policyLoss(leaf, none.long(), none, torch.ones(4, device="cuda"), reduction=reduction)
     (g,) = torch.autograd.grad(got, [leaf])
     assert float(got.detach()) == 0.0 and g.shape == leaf.shape
+
+
+def test_spike_losses_of_no_samples():
+    d = descriptor("Policy")
+    spikes = torch.zeros(0, 7, 1, 1, 50, device="cuda", requires_grad=True)
+    none = torch.zeros(0, device="cuda")
+    net = loss.spikeLoss(d).cuda()
+    assert net.actionLogProb(spikes, none.long()).shape == (0,)
+    got = net.policy(spikes, none.long(), none, none)
+    (g,) = torch.autograd.grad(got, [spikes])
+    assert float(got.detach()) == 0.0 and g.shape == spikes.shape
+    net = loss.spikeLoss(descriptor("Preference")).cuda()
+    for shape, value in (((0, 3), 0.0), ((2, 0), math.log(2.0))):
+        got = net.preference(spikes, none.long().reshape(shape), torch.zeros(shape[0], device="cuda"))
+        (g,) = torch.autograd.grad(got, [spikes])
+        assert abs(float(got.detach()) - value) < 1e-6 and g.shape == spikes.shape
