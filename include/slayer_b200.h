@@ -290,8 +290,8 @@ int slayer_b200_log_prob(float *logp, float *stats, const void *logits, int dtyp
  * Gradient of rows' log-probabilities with respect to the logits:
  *   grad[r, j] = upstream * coef[r / coef_len] * scale * ((j == action[r]) - softmax(z)[j]),
  * 0 in masked rows (which are not read).  grad: [rows, V] of type `dtype`, contiguous.  stats: as
- * slayer_b200_log_prob or slayer_b200_policy_loss left them.  coef: rows / coef_len floats, or
- * NULL for 1.  upstream: a float on the device, or one per row if upstream_rows is not 0.  With
+ * slayer_b200_log_prob or slayer_b200_policy_loss left them.  coef: rows / coef_len floats (rows a
+ * multiple of coef_len), or NULL for 1.  upstream: a float on the device, or one per row if upstream_rows is not 0.  With
  * only_if_not_one (and one upstream) nothing is done if that upstream is 1.  It has no counterpart
  * in the reference.
  */
@@ -301,7 +301,7 @@ int slayer_b200_logit_grad(void *grad, const void *logits, int dtype, const int6
 
 /*
  * Clipped policy loss with a KL term, value and gradient in one pass.  Per row, with logp as above:
- *   ratio = exp(logp - old_logp[r]),  A = advantage[r / adv_len],  d = ref_logp[r] - logp
+ *   ratio = exp(logp - old_logp[r]),  A = advantage[r / adv_len],  d = ref_logp[r] - logp   (rows a multiple of adv_len)
  *   per   = -min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A) + kl (exp(d) - d - 1)
  * loss = sum of per over the rows (SLAYER_B200_SUM), its mean over the rows that are not masked
  * (SLAYER_B200_MEAN), or the mean over the rows / seq_len sequences of the mean over each one's rows

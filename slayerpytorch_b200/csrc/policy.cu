@@ -757,7 +757,7 @@ extern "C" int slayer_b200_logit_grad(void *grad, const void *logits, int dtype,
     if (rows == 0) return SLAYER_B200_OK;
     SB200_REQUIRE(grad && logits && action && stats && upstream, "logit_grad: null pointer");
     SB200_REQUIRE(grad != logits, "logit_grad: grad must not alias logits");
-    SB200_REQUIRE(coef_len >= 1, "logit_grad: coef_len must be at least 1");
+    SB200_REQUIRE(coef_len >= 1 && (!coef || rows % coef_len == 0), "logit_grad: rows must be whole groups of coef_len");
     RowArgs A = row_args(logits, action, mask, rows, V, stride, scale);
     A.stats = (float2 *)stats;
     A.coef = (float *)coef;
@@ -787,7 +787,7 @@ extern "C" int slayer_b200_policy_loss(float *loss, void *grad, float *logp, flo
     SB200_REQUIRE(loss, "policy_loss: null pointer");
     SB200_REQUIRE(clip_low >= 0.0f && clip_high >= 0.0f, "policy_loss: the clip range must not be negative");
     SB200_REQUIRE(reduction >= 0 && reduction <= 2, "policy_loss: unknown reduction %d", reduction);
-    SB200_REQUIRE(adv_len >= 1, "policy_loss: adv_len must be at least 1");
+    SB200_REQUIRE(adv_len >= 1 && rows % adv_len == 0, "policy_loss: rows must be whole groups of adv_len");
     SB200_REQUIRE(rows == 0 || (seq_len >= 1 && rows % seq_len == 0), "policy_loss: rows must be whole sequences");
     if (rows == 0) {
         if (cudaMemsetAsync(loss, 0, sizeof(float), (cudaStream_t)stream) != cudaSuccess) return check_launch("policy_loss");
