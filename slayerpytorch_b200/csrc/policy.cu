@@ -707,6 +707,8 @@ static int check_rows(const char *what, int dtype, int64_t rows, int64_t V, int6
     SB200_REQUIRE(dtype == SLAYER_B200_F32 || dtype == SLAYER_B200_BF16 || dtype == SLAYER_B200_F16, "%s: unknown type %d", what, dtype);
     SB200_REQUIRE(rows >= 0 && V >= 1 && stride >= 0, "%s: bad size", what);
     SB200_REQUIRE(scale > 0.0 && scale < INFINITY, "%s: scale must be positive and finite", what);
+    // scale log2(e), by which the exponents are multiplied, has to be an ordinary float32
+    SB200_REQUIRE(scale >= 1.2e-38 && scale <= 2.3e38, "%s: scale must lie between 1.2e-38 and 2.3e38", what);
     if (V > (1 << 30) || rows > 0x7fffffff) {
         set_error("%s: %lld rows of %lld entries", what, (long long)rows, (long long)V);
         return SLAYER_B200_EUNSUPPORTED;

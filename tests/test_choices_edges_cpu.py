@@ -29,3 +29,11 @@ def test_groups_of_rows_are_whole():
         assert b"whole groups" in capi.load().slayer_b200_last_error()
         assert policy_loss(adv_len=length) == -1, length
         assert b"whole groups" in capi.load().slayer_b200_last_error()
+
+
+def test_scales_that_no_power_of_two_can_hold():
+    """scale * log2(e) is a float32 that is neither infinite nor flushed to zero."""
+    for scale in (2.4e38, 3.4e38, 1e-39, 1e-45):
+        for call in (log_prob, logit_grad, policy_loss):
+            assert call(scale=scale) == -1, scale
+            assert b"scale" in capi.load().slayer_b200_last_error()
