@@ -395,15 +395,14 @@ __global__ void __launch_bounds__(512, 2) rows_long_kernel(RowArgs A)
     using P = Piece<T>;
     constexpr int N = P::N;
     __shared__ float2 part[16];          // the warps' maxima and sums
-    __shared__ float2 whole[2];          // this CTA's, by the row's parity: the others of a cluster may read the one before
+    __shared__ float2 whole;             // this CTA's (a cluster has one row)
     __shared__ float4 result;
     if (MODE == kGrad && A.only_if_not_one && A.upstream[0] == 1.0f) return;
     if (MODE == kPolicy && blockIdx.x == 0 && threadIdx.x == 0) *A.arrived = 0;
     cg::cluster_group cluster = cg::this_cluster();
     const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, warp = tid >> 5;
-    // a row each; or, where that costs less than more CTAs (launch_rows), several
-    int parity = 0;
+    // a row each; or, where that costs less than more CTAs (launch_rows), several to a CTA alone
     for (int64_t row = blockIdx.x / C; row < A.rows; row += gridDim.x / C) {
         const T *x = (const T *)A.logits + row * A.stride;
         T *g = A.grad ? (T *)A.grad + row * (int64_t)A.V : nullptr;
@@ -476,18 +475,17 @@ __global__ void __launch_bounds__(512, 2) rows_long_kernel(RowArgs A)
                 soft.meet<16>(A.k);
             }
             if (C > 1) {
-                if (tid == 0) whole[parity] = make_float2(soft.m, soft.s);
+                if (tid == 0) whole = make_float2(soft.m, soft.s);
                 cluster.sync();
                 if (warp == 0) {
                     soft = Soft();
                     if (lane < C) {
-                        const float2 o = *cluster.map_shared_rank(&whole[parity], lane);
+                        const float2 o = *cluster.map_shared_rank(&whole, lane);
                         soft.m = o.x;
                         soft.s = o.y;
                     }
                     soft.meet<8>(A.k);
                 }
-                parity ^= 1;
             }
         } else if (warp == 0) {
             const float2 st = A.stats[row];

@@ -195,3 +195,65 @@ def test_spike_losses_of_no_samples():
         got = net.preference(spikes, none.long().reshape(shape), torch.zeros(shape[0], device="cuda"))
         (g,) = torch.autograd.grad(got, [spikes])
         assert abs(float(got.detach()) - value) < 1e-6 and g.shape == spikes.shape
+
+
+def check_policy(x, action, old, ref, adv, mask, up, scale=0.9):
+    """A multiple of the policy loss, its log-probabilities and its gradient (all on the device)"""
+    leaf = x.detach().requires_grad_()
+    got, lp = loss.policyLoss(leaf, action, old, adv, refLogProb=ref, mask=mask, clip=CLIP, klCoef=0.3, scale=scale, returnLogProb=True)
+    (g,) = torch.autograd.grad(got * up, [leaf])
+    value, slack, coef, size = policy_want(x, action, old, adv, ref, mask, 0.3, "sum", scale)
+    assert abs(float(got.detach()) - float(value)) <= float(slack) + 2 ** -24 * abs(float(value))
+    close(lp, torch.where(mask, want_logp(x, action, scale), 0.0).cpu(), SUM)
+    assert bool((g[~mask] == 0).all())
+    for r in range(0, len(x), 400):
+        part = slice(r, r + 400)
+        grad, spare = want_grad(x[part], action[part], up * coef[part], scale)
+        close(g[part], grad.cpu(), (spare + abs(up) * of_ratio(x[part], action[part], size[part], scale)).cpu())
+
+
+def many_rows(rows, V, dtype, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    x = (torch.randn(rows, 1, V, generator=gen, device="cuda") * 3).to(dtype)
+    action = torch.randint(0, V, (rows, 1), generator=gen, device="cuda")
+    lp = torch.cat([want_logp(x[r:r + 400], action[r:r + 400], 0.9) for r in range(0, rows, 400)])
+    ratio = torch.tensor([0.3, 0.7, 0.95, 1.0, 1.1, 1.22, 2.5], dtype=torch.float64, device="cuda")[torch.randint(0, 7, (rows, 1), generator=gen, device="cuda")]
+    old = (lp - ratio.log()).float()
+    ref = (lp + 0.5 * torch.randn(rows, 1, generator=gen, device="cuda")).float()
+    adv = torch.randn(rows, 1, generator=gen, device="cuda")
+    mask = torch.rand(rows, 1, generator=gen, device="cuda") < 0.6
+    mask[1183:1187] = torch.tensor([[True], [False], [False], [True]], device="cuda")
+    return x, action, old, ref, adv, mask
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [1030, 4097])
+@pytest.mark.parametrize("up", [1.0, 0.5])
+def test_policy_more_long_rows_than_a_rescaled_gradient_has_ctas(up, V, dtype):
+    """The gradient of a loss that was multiplied by something is formed by at most eight CTAs per SM, which walk over the rows."""
+    rows = 8 * torch.cuda.get_device_properties(0).multi_processor_count * 2 + 77
+    check_policy(*many_rows(rows, V, dtype, V), up)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V,per_cta", [(7, 32), (32, 32), (33, 8), (80, 8)])
+@pytest.mark.parametrize("up", [1.0, 0.5])
+def test_policy_more_short_rows_than_ctas_hold(up, V, per_cta, dtype):
+    rows = 8 * torch.cuda.get_device_properties(0).multi_processor_count * per_cta + 1001
+    check_policy(*many_rows(rows, V, dtype, V), up)
+
+
+def test_more_than_2_to_31_logits():
+    rows, V = 70001, 32768
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    x = torch.randn(rows, V, generator=gen, device="cuda", dtype=torch.bfloat16)
+    action = torch.randint(0, V, (rows,), generator=gen, device="cuda")
+    leaf = x.requires_grad_()
+    lp = loss.actionLogProb(leaf, action)
+    up = torch.randn(rows, generator=gen, device="cuda")
+    (g,) = torch.autograd.grad(lp, [leaf], up)
+    for part in (slice(0, 3), slice(65530, 65545), slice(rows - 3, rows)):
+        y = x.detach()[part]
+        close(lp.detach()[part], want_logp(y, action[part]).cpu(), SUM)
+        grad, spare = want_grad(y, action[part], up[part].double())
+        close(g[part], grad.cpu(), spare.cpu())
