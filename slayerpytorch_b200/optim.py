@@ -77,7 +77,8 @@ def muonStep(weights, grads, momenta, lr, momentum=0.95, nesterov=True, weightDe
 
 class Muon(torch.optim.Optimizer):
     """``muonStep`` as a PyTorch optimiser, for the weights of dense and convolution layers.  Parameters of fewer than two
-    dimensions (delays, thresholds) belong to another optimiser.  The state of a parameter is its float32 ``'momentum'``."""
+    dimensions (delays, thresholds) belong to another optimiser.  The state of a parameter is its float32 ``'momentum'``, made by its
+    first step: a step may be captured in a CUDA graph once every parameter has taken one (or a state was loaded)."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weightDecay=0.0, steps=5, coefficients=COEFFICIENTS, eps=1e-7,
                  adjust='shape'):
@@ -114,11 +115,13 @@ class Muon(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        missing = [p for group in self.param_groups for p in group['params'] if p.grad is not None and 'momentum' not in self.state.get(p, ())]
+        if any(p.is_cuda for p in missing) and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("Muon: momenta that are made in a capture would be zero in every replay; take a step before the capture")
+        for p in missing:
+            self.state[p]['momentum'] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
         for group in self.param_groups:
             weights = [p for p in group['params'] if p.grad is not None]
-            for p in weights:
-                if 'momentum' not in self.state[p]:
-                    self.state[p]['momentum'] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
             muonStep(weights, [p.grad for p in weights], [self.state[p]['momentum'] for p in weights],
                      **{k: group[k] for k in ('lr', 'momentum', 'nesterov', 'weightDecay', 'steps', 'coefficients', 'eps', 'adjust')})
         return loss
