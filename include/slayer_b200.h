@@ -340,10 +340,10 @@ int64_t slayer_b200_preference_loss_workspace(int64_t sequences);
  *   X = u / (|u|_F + eps),   `steps` times  X <- a X + (b A + c A A) X,  A = X X^T
  * (of a matrix with more rows than columns, the transpose's).  out may be in.  Float32 and float16
  * matrices are worked on with products of 22 bits, bfloat16 ones with 11.  Coefficients whose steps
- * take singular values from [0, 1] past 3.5 are refused.  At most 32768 on the shorter side and
- * 2^31 elements per matrix, else SLAYER_B200_EUNSUPPORTED.  workspace:
- * slayer_b200_orthogonalize_workspace(...) bytes of device memory, aligned to 256.  It has
- * no counterpart in the reference.
+ * take singular values from [0, 1] past 3.5 are refused.  At most 32768 on the shorter side, 2^22 on
+ * the longer and 2^31 elements per matrix, else SLAYER_B200_EUNSUPPORTED.  workspace:
+ * slayer_b200_orthogonalize_workspace(...) bytes of device memory, aligned to 256 (that code where a
+ * matrix is too large).  It has no counterpart in the reference.
  */
 int slayer_b200_orthogonalize(void *out, const void *in, int dtype, int64_t batch, int64_t rows, int64_t cols, int steps, float a, float b,
                               float c, float eps, void *workspace, void *stream);
@@ -367,8 +367,8 @@ typedef struct {
  * returns), in a fixed number of launches:
  *   momentum <- mu momentum + grad,   u = grad + mu momentum if nesterov else momentum,
  *   weight   <- weight (1 - lr weight_decay) - lr factor X,   X = u made orthogonal as above.
- * The weights must not overlap.  workspace: slayer_b200_muon_step_workspace(...) bytes of device
- * memory, aligned to 256.  It has no counterpart in the reference, whose optimizer is Nadam
+ * The weights must not overlap.  Sizes and workspace (slayer_b200_muon_step_workspace(...) bytes) as
+ * above; nothing is launched where a matrix is refused.  It has no counterpart in the reference, whose optimizer is Nadam
  * (src/optimizer.py:6-113).
  */
 int slayer_b200_muon_step(const slayer_b200_muon_matrix *list, int64_t count, int dtype, float lr, float mu, int nesterov,

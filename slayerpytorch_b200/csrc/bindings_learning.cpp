@@ -333,15 +333,22 @@ void check_matrix(const torch::Tensor &x, const char *name)
     TORCH_CHECK(x.dim() >= 2, name, " must have at least two dimensions, it has ", x.dim());
 }
 
+// bytes that are not a negative code
+int64_t size_of(int64_t bytes, const char *op)
+{
+    if (bytes < 0) check_rc((int)bytes, op);
+    return bytes;
+}
+
 // A matrix, or a stack of them, made near orthogonal.
 torch::Tensor orthogonalizeCuda(torch::Tensor x, int64_t steps, double a, double b, double c, double eps)
 {
     check_matrix(x, "matrix");
     const int dtype = dtype_code(x, "matrix");
     c10::cuda::CUDAGuard guard(x.device());
-    auto out = torch::empty_like(x);
     const int64_t rows = x.size(-2), cols = x.size(-1), batch = x.numel() ? x.numel() / (rows * cols) : 0;
-    auto workspace = torch::empty({slayer_b200_orthogonalize_workspace(batch, rows, cols, dtype)}, x.options().dtype(torch::kUInt8));
+    auto workspace = torch::empty({size_of(slayer_b200_orthogonalize_workspace(batch, rows, cols, dtype), "orthogonalize")}, x.options().dtype(torch::kUInt8));
+    auto out = torch::empty_like(x);
     check_rc(slayer_b200_orthogonalize(out.data_ptr(), x.data_ptr(), dtype, batch, rows, cols, (int)std::clamp<int64_t>(steps, 0, 1 << 20),
                                        (float)a, (float)b, (float)c, (float)eps, workspace.data_ptr(), current_stream()),
              "orthogonalize");
@@ -373,7 +380,7 @@ void muonStepCuda(std::vector<torch::Tensor> weights, const std::vector<torch::T
         list.push_back({w.data_ptr(), g.data_ptr(), m.data_ptr<float>(), rows, w.numel() ? w.numel() / rows : 0});
     }
     c10::cuda::CUDAGuard guard(weights[0].device());
-    auto workspace = torch::empty({slayer_b200_muon_step_workspace(list.data(), (int64_t)list.size(), dtype)},
+    auto workspace = torch::empty({size_of(slayer_b200_muon_step_workspace(list.data(), (int64_t)list.size(), dtype), "muonStep")},
                                   weights[0].options().dtype(torch::kUInt8));
     check_rc(slayer_b200_muon_step(list.data(), (int64_t)list.size(), dtype, (float)lr, (float)momentum, nesterov, (float)weightDecay,
                                    (int)adjust, (int)std::clamp<int64_t>(steps, 0, 1 << 20), (float)a, (float)b, (float)c, (float)eps,

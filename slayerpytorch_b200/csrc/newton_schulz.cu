@@ -1529,6 +1529,8 @@ using namespace sb200;
 extern "C" int64_t slayer_b200_orthogonalize_workspace(int64_t batch, int64_t rows, int64_t cols, int dtype)
 {
     if (batch <= 0 || rows <= 0 || cols <= 0) return 0;
+    clear_error();
+    if (const int rc = ns_shape("orthogonalize", rows, cols)) return rc;
     return (int64_t)ns_job_bytes(rows < cols ? rows : cols, rows < cols ? cols : rows, dtype) * (batch < kMaxJobs ? batch : kMaxJobs);
 }
 
@@ -1571,11 +1573,13 @@ extern "C" int slayer_b200_orthogonalize(void *out, const void *in, int dtype, i
 
 extern "C" int64_t slayer_b200_muon_step_workspace(const slayer_b200_muon_matrix *list, int64_t count, int dtype)
 {
+    clear_error();
     size_t most = 0, now = 0;
     int in = 0;
     for (int64_t i = 0; list && i < count; ++i) {
         const int64_t rows = list[i].rows, cols = list[i].cols;
         if (rows <= 0 || cols <= 0) continue;
+        if (const int rc = ns_shape("muon_step", rows, cols)) return rc;
         if (in++ == kMaxJobs) {
             in = 1;
             now = 0;
