@@ -355,37 +355,49 @@ torch::Tensor orthogonalizeCuda(torch::Tensor x, int64_t steps, double a, double
     return out;
 }
 
-// One optimiser step, in place, of weights of one type on one device: [d0, d1, ...] is a matrix of d0 rows.
+// One optimiser step, in place: [d0, d1, ...] is a matrix of d0 rows.  Weights of one type on one device are worked on together; whatever
+// can be refused is, before the first of them changes.
 void muonStepCuda(std::vector<torch::Tensor> weights, const std::vector<torch::Tensor> &grads, std::vector<torch::Tensor> momenta, double lr,
                   double momentum, bool nesterov, double weightDecay, int64_t adjust, int64_t steps, double a, double b, double c, double eps)
 {
     TORCH_CHECK(weights.size() == grads.size() && weights.size() == momenta.size(), "as many gradients and momenta as weights");
-    if (weights.empty()) return;
-    const int dtype = dtype_code(weights[0], "weight");
-    std::vector<slayer_b200_muon_matrix> list;
-    list.reserve(weights.size());
+    struct Group {
+        torch::Tensor first, workspace;
+        int dtype;
+        std::vector<slayer_b200_muon_matrix> list;
+    };
+    std::vector<Group> groups;
     for (size_t i = 0; i < weights.size(); ++i) {
         const torch::Tensor &w = weights[i], &g = grads[i], &m = momenta[i];
         check_matrix(w, "weight");
         check_matrix(g, "grad");
         check_matrix(m, "momentum");
-        TORCH_CHECK(w.scalar_type() == weights[0].scalar_type(), "the weights of one call must have one dtype");
+        const int dtype = dtype_code(w, "weight");
         TORCH_CHECK(g.scalar_type() == w.scalar_type(), "grad must have the dtype of its weight");
         TORCH_CHECK(m.scalar_type() == torch::kFloat32, "momentum must be a float32 tensor");
         TORCH_CHECK(g.sizes() == w.sizes() && m.sizes() == w.sizes(), "grad and momentum must have the shape of their weight");
-        check_device(w, weights[0], "weight", "the first weight");
         check_device(g, w, "grad", "weight");
         check_device(m, w, "momentum", "weight");
+        TORCH_CHECK(c10::InferenceMode::is_enabled() || !(w.is_inference() || m.is_inference()),
+                    "weights and momenta made in inference mode are updated in it only");
         const int64_t rows = w.size(0);
-        list.push_back({w.data_ptr(), g.data_ptr(), m.data_ptr<float>(), rows, w.numel() ? w.numel() / rows : 0});
+        size_t at = 0;
+        while (at < groups.size() && !(groups[at].dtype == dtype && groups[at].first.device() == w.device())) ++at;
+        if (at == groups.size()) groups.push_back({w, torch::Tensor(), dtype, {}});
+        groups[at].list.push_back({w.data_ptr(), g.data_ptr(), m.data_ptr<float>(), rows, w.numel() ? w.numel() / rows : 0});
     }
-    c10::cuda::CUDAGuard guard(weights[0].device());
-    auto workspace = torch::empty({size_of(slayer_b200_muon_step_workspace(list.data(), (int64_t)list.size(), dtype), "muonStep")},
-                                  weights[0].options().dtype(torch::kUInt8));
-    check_rc(slayer_b200_muon_step(list.data(), (int64_t)list.size(), dtype, (float)lr, (float)momentum, nesterov, (float)weightDecay,
-                                   (int)adjust, (int)std::clamp<int64_t>(steps, 0, 1 << 20), (float)a, (float)b, (float)c, (float)eps,
-                                   workspace.data_ptr(), current_stream()),
-             "muonStep");
+    for (Group &k : groups) {
+        c10::cuda::CUDAGuard guard(k.first.device());
+        k.workspace = torch::empty({size_of(slayer_b200_muon_step_workspace(k.list.data(), (int64_t)k.list.size(), k.dtype), "muonStep")},
+                                   k.first.options().dtype(torch::kUInt8));
+    }
+    for (Group &k : groups) {
+        c10::cuda::CUDAGuard guard(k.first.device());
+        check_rc(slayer_b200_muon_step(k.list.data(), (int64_t)k.list.size(), k.dtype, (float)lr, (float)momentum, nesterov, (float)weightDecay,
+                                       (int)adjust, (int)std::clamp<int64_t>(steps, 0, 1 << 20), (float)a, (float)b, (float)c, (float)eps,
+                                       k.workspace.data_ptr(), current_stream()),
+                 "muonStep");
+    }
     for (auto &w : weights) w.unsafeGetTensorImpl()->bump_version();      // autograd sees that they changed
     for (auto &m : momenta) m.unsafeGetTensorImpl()->bump_version();
 }

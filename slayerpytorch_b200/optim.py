@@ -44,14 +44,17 @@ def muonStep(weights, grads, momenta, lr, momentum=0.95, nesterov=True, weightDe
         weight = weight * (1 - lr * weightDecay) - lr * factor * update
 
     A weight of shape ``[d0, d1, ...]`` is a matrix of ``d0`` rows.  Weights and their gradients are float32, bfloat16 or float16,
-    momenta float32; none of them overlap, but for gradients.  ``factor`` is ``sqrt(max(1, rows / cols))`` (``adjust='shape'``), ``0.2 * sqrt(max(rows, cols))`` (``'rms'``: updates
-    as large as Adam's) or 1 (``None``)."""
+    momenta float32; none of them overlap, but for gradients.  ``factor`` is ``sqrt(max(1, rows / cols))`` (``adjust='shape'``),
+    ``0.2 * sqrt(max(rows, cols))`` (``'rms'``: updates as large as Adam's) or 1 (``None``).  A call that is refused changes nothing.
+
+    The products wait on barriers for a limited time.  If one ever runs out, weights may be partly updated, and
+    ``capi.device_status()`` says 0x5103."""
     weights, grads, momenta = list(weights), list(grads), list(momenta)
     if not len(weights) == len(grads) == len(momenta):
         raise ValueError("muonStep: %d weights, %d gradients, %d momenta" % (len(weights), len(grads), len(momenta)))
     if adjust not in _ADJUST:
         raise ValueError("muonStep: adjust must be one of %s, got %r" % (list(_ADJUST), adjust))
-    groups, seen = {}, set()
+    seen = set()
     for w, g, m in zip(weights, grads, momenta):
         if w.dim() < 2:
             raise ValueError("muonStep: a weight has at least two dimensions, got %s" % (tuple(w.shape),))
@@ -59,21 +62,21 @@ def muonStep(weights, grads, momenta, lr, momentum=0.95, nesterov=True, weightDe
             raise ValueError("muonStep: sparse gradients are not taken")
         if not m.is_contiguous():
             raise ValueError("muonStep: momenta must be contiguous")
+        if not w.is_contiguous() and any(n > 1 and s == 0 for n, s in zip(w.shape, w.stride())):
+            raise ValueError("muonStep: a weight whose elements share memory")
         for t in (w, m):
             if t.numel() and t.data_ptr() in seen:
                 raise ValueError("muonStep: the same weight or momentum twice")
             seen.add(t.data_ptr())
-        groups.setdefault((w.device, w.dtype), []).append((w, g, m))
     if any(g.numel() and g.data_ptr() in seen for g in grads):
         raise ValueError("muonStep: a gradient in the memory of a weight or momentum")
-    for items in groups.values():
-        # a weight whose elements are in another order is updated in a copy
-        there = [w if w.is_contiguous() else w.contiguous() for w, _, _ in items]
-        slayerCuda.muonStep(there, [g.contiguous() for _, g, _ in items], [m for _, _, m in items], float(lr), float(momentum),
-                            bool(nesterov), float(weightDecay), _ADJUST[adjust], int(steps), *_coefficients(coefficients), float(eps))
-        for (w, _, _), t in zip(items, there):
-            if t is not w:
-                w.copy_(t)
+    # a weight whose elements are in another order is updated in a copy
+    there = [w if w.is_contiguous() else w.contiguous() for w in weights]
+    slayerCuda.muonStep(there, [g.contiguous() for g in grads], momenta, float(lr), float(momentum), bool(nesterov), float(weightDecay),
+                        _ADJUST[adjust], int(steps), *_coefficients(coefficients), float(eps))
+    for w, t in zip(weights, there):
+        if t is not w:
+            w.copy_(t)
 
 
 class Muon(torch.optim.Optimizer):

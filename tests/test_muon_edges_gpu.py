@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from slayerpytorch_b200 import optim
+from tests.test_muon_gpu import step_case
 
 pytestmark = pytest.mark.gpu
 
@@ -37,3 +38,22 @@ def test_a_first_step_of_the_optimiser_is_not_captured():
     torch.cuda.synchronize()
     for p, q in zip(params, other):
         assert torch.equal(p, q) and torch.equal(opt.state[p]["momentum"], eager.state[q]["momentum"])
+
+
+def test_a_refused_step_changes_nothing():
+    """Lists of several types are worked on one type after the other: what the second is refused for is found before the first."""
+    ws, gs, ms = step_case([(24, 30), (16, 20)], torch.float32, 11)
+    w, g, m = ([t.cuda() for t in ts] for ts in (ws, gs, ms))
+    long = torch.zeros(1, (1 << 22) + 1, device="cuda")       # longer than a matrix may be
+    far = torch.zeros(1, 1, device="cuda", dtype=torch.bfloat16)
+    for second in ((w[1].double(), g[1].double(), m[1]), (w[1].bfloat16(), g[1], m[1]), (w[1].bfloat16(), g[1].bfloat16(), m[1].bfloat16()),
+                   (w[1].bfloat16(), g[1].bfloat16(), m[1][:8]), (w[1].bfloat16(), g[1].bfloat16()[:8], m[1]), (w[1].cpu(), g[1].cpu(), m[1].cpu()),
+                   (w[1].bfloat16(), g[1].bfloat16().cpu(), m[1]), (far.expand(16, 20), g[1].bfloat16(), m[1]),
+                   (long.bfloat16(), long.bfloat16(), long.clone())):
+        with pytest.raises((RuntimeError, ValueError)):
+            optim.muonStep([w[0], second[0]], [g[0], second[1]], [m[0], second[2]], lr=0.1)
+        assert torch.equal(w[0].cpu(), ws[0]) and torch.equal(m[0].cpu(), ms[0])
+    for more in (dict(steps=0), dict(eps=-1.0), dict(coefficients=(9.0, 0.0, 0.0))):
+        with pytest.raises(RuntimeError):
+            optim.muonStep(w, g, m, lr=0.1, **more)
+        assert all(torch.equal(a.cpu(), b) for a, b in zip(w + m, ws + ms))
