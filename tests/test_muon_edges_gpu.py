@@ -1,10 +1,11 @@
 """GPU: the orthogonalised updates at their edges - refused calls, a first step in a capture, every way of sharing out the tiles."""
+import math
 
 import pytest
 import torch
 
 from slayerpytorch_b200 import optim
-from tests.test_muon_gpu import step_case
+from tests.test_muon_gpu import TYPES, gradient, near, slack, step_case, want_orthogonal, want_step
 
 pytestmark = pytest.mark.gpu
 
@@ -57,3 +58,96 @@ def test_a_refused_step_changes_nothing():
         with pytest.raises(RuntimeError):
             optim.muonStep(w, g, m, lr=0.1, **more)
         assert all(torch.equal(a.cpu(), b) for a, b in zip(w + m, ws + ms))
+
+
+def blocks(v):
+    return (v + 127) // 128
+
+
+def sharing(shapes, dtype):
+    """How a launch of matrices that do not stay on the chip shares out its tiles, and how many tiles there are for each CTA (pair)."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    sides = [(min(s), max(s)) for s in shapes]
+    pairs = sum(((blocks(m) + 1) // 2) * ((blocks(n) + 1) // 2) for m, n in sides)
+    if pairs >= sms // 2:
+        return "pairs", pairs / (sms // 2)
+    if sum(blocks(m) * (blocks(m) + 1) // 2 for m, _ in sides) * 4 <= sms:
+        return "shared", 1
+    return "alone", sum(blocks(m) * blocks(n) for m, n in sides) / sms
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(1100, 1300), (1300, 1100), (4, 512, 512), (4, 513, 600), (2, 768, 777), (1664, 1280), (30, 200, 140)])
+def test_orthogonalize_tiles_of_a_cta_alone(shape, dtype):
+    assert sharing([shape[-2:]] * math.prod(shape[:-2]), dtype)[0] == "alone"
+    x = gradient(shape, sum(shape), dtype)
+    near(optim.orthogonalize(x.cuda()), want_orthogonal(x.cuda()).cpu(), dtype, min(shape[-2:]) * math.prod(shape[:-2]))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shapes", [[(1100, 1300)], [(512, 600), (640, 512), (30, 20), (10, 512), (700, 800)]])
+def test_muon_step_tiles_of_a_cta_alone(shapes, dtype):
+    assert sharing(shapes, dtype)[0] == "alone"
+    check_step(shapes, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shapes", [[(2600, 7700)], [(300, 520)] * 17 + [(1290, 5000)] * 3 + [(5000, 1290), (4, 9)]])
+def test_more_tiles_than_are_worked_out_ahead(shapes, dtype):
+    """A CTA's first four tiles are located once, later ones as they come."""
+    mode, each = sharing(shapes, dtype)
+    assert mode == "pairs" and each > 4
+    check_step(shapes, dtype)
+
+
+def check_step(shapes, dtype):
+    ws, gs, ms = ([t.cuda() for t in ts] for ts in step_case(shapes, dtype, 60))
+    dw, dm = [t.clone() for t in ws], [t.clone() for t in ms]
+    optim.muonStep(dw, gs, dm, lr=0.03, weightDecay=0.1)
+    for w, g, m, gw, gm in zip(ws, gs, ms, dw, dm):
+        want, mom, step = want_step(w, g, m, 0.03, decay=0.1)
+        assert bool(((gm.double() - mom).abs() <= 2.0 ** -23 * (m.double().abs() + mom.abs())).all())
+        off = torch.linalg.vector_norm(gw.double() - want)
+        rank = min(w.shape)
+        half = torch.finfo(dtype).eps / 2 + 2.0 ** -22
+        assert float(off) <= step * slack(dtype, rank) * math.sqrt(rank) * 1.2 + half * float(torch.linalg.vector_norm(want)) + 1e-30
+
+
+def off(got, want):
+    return float(torch.linalg.vector_norm(got.double() - want) / torch.linalg.vector_norm(want))
+
+
+def fp32_products(x):
+    """The definition in fp32 throughout."""
+    a, b, c = optim.COEFFICIENTS
+    if x.shape[0] > x.shape[1]:
+        return fp32_products(x.mT).mT
+    x = x / (torch.linalg.vector_norm(x) + 1e-7)
+    for _ in range(5):
+        g = x @ x.mT
+        x = a * x + (b * g + c * (g @ g)) @ x
+    return x
+
+
+@pytest.mark.parametrize("strong", [True, False])
+@pytest.mark.parametrize("shape", [(16, 50), (64, 288), (100, 300), (128, 128), (128, 1024), (128, 2500), (10, 4096), (200, 256), (333, 2000), (2000, 333),
+                                   (512, 2312), (700, 700), (1100, 1300), (2048, 2048)])
+def test_errors_against_those_of_fp32_products(shape, strong):
+    """Products of two 16-bit parts (22 bits) whose sums beyond 64 to 192 products are added up in fp32 are no further off than fp32
+    products.  Matrices that stay on the chip (up to 128 rows) have sums of up to 128 products in tensor memory, where each of 24 additions
+    is cut instead of rounded: half a step each, all to one side, against fp32's 128 roundings to either side of about sqrt(128 / 12) =
+    3.3 half steps.  12 half steps against 3.3: up to 4 times as far off."""
+    x = (gradient(shape, 5) if strong else torch.randn(shape, generator=torch.Generator().manual_seed(5))).cuda()
+    want = want_orthogonal(x)
+    assert not torch.backends.cuda.matmul.allow_tf32
+    assert off(optim.orthogonalize(x), want) <= (4 if min(shape) <= 128 else 1) * off(fp32_products(x), want)
+
+
+@pytest.mark.parametrize("shape", [(16, 50), (100, 300), (128, 1024), (10, 4096), (333, 2000), (700, 700), (1023, 2049), (2048, 2048)])
+def test_errors_of_bfloat16_matrices(shape):
+    """Four roundings a step (x, a, b, and x again) to 11 bits, each 2^-12 / sqrt(3) of the matrix in the mean; what one step leaves is
+    multiplied by |p'| <= 1.71 in each later one (p' of the singular values that have arrived, 0.68 to 1.13): sqrt(4 (1 + 1.71^2 + ... +
+    1.71^8)) 2^-12 / sqrt(3) = 2.96e-3, beside the result's own rounding.  (Products of bfloat16's 8 bits would be eight times as far off.)"""
+    x = gradient(shape, 6, torch.bfloat16).cuda()
+    want = want_orthogonal(x)
+    assert off(optim.orthogonalize(x), want) <= math.hypot(2.96e-3, off(want.bfloat16(), want))
