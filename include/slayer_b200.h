@@ -279,9 +279,10 @@ int slayer_b200_num_spikes_loss(float *grad, double *row_sq, const float *s, con
  * logits: [rows, V] of type `dtype` (SLAYER_B200_F32 ...), `stride` elements from row to row, the
  * entries of a row next to each other; any alignment of a multiple of the element.  mask: one byte
  * per row or NULL; a row whose byte is 0 is not read, its logp is 0.  stats: 2 * rows floats for
- * slayer_b200_logit_grad, or NULL.  An action outside [0, V) gives NaN.  scale, between 1.2e-38 and
- * 2.3e38 in all entries of these losses: spike counts are logits with a gain.  It has no counterpart
- * in the reference, whose classifier takes the largest spike count (src/spikeClassifier.py:9-20).
+ * slayer_b200_logit_grad, aligned to 8 bytes, or NULL.  An action outside [0, V) gives NaN.  scale,
+ * between 1.2e-38 and 2.3e38 in all entries of these losses: spike counts are logits with a gain.
+ * It has no counterpart in the reference, whose classifier takes the largest spike count
+ * (src/spikeClassifier.py:9-20).
  */
 int slayer_b200_log_prob(float *logp, float *stats, const void *logits, int dtype, const int64_t *action, const uint8_t *mask,
                          int64_t rows, int64_t V, int64_t stride, float scale, void *stream);

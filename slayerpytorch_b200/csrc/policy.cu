@@ -714,6 +714,15 @@ static int check_rows(const char *what, int dtype, int64_t rows, int64_t V, int6
     return SLAYER_B200_OK;
 }
 
+// logits and gradient at a multiple of their element, stats (read and written in pairs) at one of 8
+static int check_places(const char *what, int dtype, const void *logits, const void *grad, const float *stats)
+{
+    const uintptr_t element = dtype == SLAYER_B200_F32 ? 3 : 1;
+    SB200_REQUIRE((((uintptr_t)logits | (uintptr_t)grad) & element) == 0, "%s: logits and grad must be aligned to their elements", what);
+    SB200_REQUIRE(((uintptr_t)stats & 7) == 0, "%s: stats must be aligned to 8 bytes", what);
+    return SLAYER_B200_OK;
+}
+
 static RowArgs row_args(const void *logits, const int64_t *action, const uint8_t *mask, int64_t rows, int64_t V, int64_t stride, float scale)
 {
     RowArgs A = {};
@@ -740,6 +749,8 @@ extern "C" int slayer_b200_log_prob(float *logp, float *stats, const void *logit
     if (rc) return rc;
     if (rows == 0) return SLAYER_B200_OK;
     SB200_REQUIRE(logp && logits && action, "log_prob: null pointer");
+    rc = check_places("log_prob", dtype, logits, nullptr, stats);
+    if (rc) return rc;
     RowArgs A = row_args(logits, action, mask, rows, V, stride, scale);
     A.logp = logp;
     A.stats = (float2 *)stats;
@@ -757,6 +768,8 @@ extern "C" int slayer_b200_logit_grad(void *grad, const void *logits, int dtype,
     if (rows == 0) return SLAYER_B200_OK;
     SB200_REQUIRE(grad && logits && action && stats && upstream, "logit_grad: null pointer");
     SB200_REQUIRE(grad != logits, "logit_grad: grad must not alias logits");
+    rc = check_places("logit_grad", dtype, logits, grad, stats);
+    if (rc) return rc;
     SB200_REQUIRE(coef_len >= 1 && (!coef || rows % coef_len == 0), "logit_grad: rows must be whole groups of coef_len");
     RowArgs A = row_args(logits, action, mask, rows, V, stride, scale);
     A.stats = (float2 *)stats;
@@ -795,6 +808,8 @@ extern "C" int slayer_b200_policy_loss(float *loss, void *grad, float *logp, flo
     }
     SB200_REQUIRE(coef && stats && workspace && logits && action && old_logp && advantage, "policy_loss: null pointer");
     SB200_REQUIRE(grad != logits, "policy_loss: grad must not alias logits");
+    rc = check_places("policy_loss", dtype, logits, grad, stats);
+    if (rc) return rc;
     SB200_REQUIRE(((uintptr_t)workspace & 7) == 0, "policy_loss: the workspace must be aligned to 8 bytes");
     const cudaStream_t st = (cudaStream_t)stream;
     RowArgs A = row_args(logits, action, mask, rows, V, stride, scale);

@@ -37,3 +37,16 @@ def test_scales_that_no_power_of_two_can_hold():
         for call in (log_prob, logit_grad, policy_loss):
             assert call(scale=scale) == -1, scale
             assert b"scale" in capi.load().slayer_b200_last_error()
+
+
+def test_places_that_the_kernels_cannot_access():
+    """Stats are read and written in pairs of floats, logits and gradients by their elements."""
+    at = ctypes.c_void_p
+    for call in (log_prob, logit_grad, policy_loss):
+        for bad in (dict(stats=at(20)), dict(logits=at(34)), dict(logits=at(33), dtype=1), dict(logits=at(33), dtype=2)):
+            assert call(**bad) == -1, bad
+            assert b"aligned" in capi.load().slayer_b200_last_error()
+    for call in (logit_grad, policy_loss):
+        for bad in (dict(grad=at(18)), dict(grad=at(17), dtype=1)):
+            assert call(**bad) == -1, bad
+            assert b"aligned" in capi.load().slayer_b200_last_error()
