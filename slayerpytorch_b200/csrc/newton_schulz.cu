@@ -1448,6 +1448,9 @@ static int ns_shape(const char *what, int64_t rows, int64_t cols)
     return SLAYER_B200_OK;
 }
 
+// whether something of this type may lie there
+static bool ns_placed(const void *p, int dtype) { return ((uintptr_t)p & (dtype == SLAYER_B200_F32 ? 3 : 1)) == 0; }
+
 // CTAs for each of the small matrices of a launch: up to four column blocks each, more where there are many matrices; 0: a matrix
 // does not fit.  Five steps with up to one / two / four / eight blocks, float32, us: 64 x 288 55 / 57 / 59 / 62, 64 x 576 62 / 62 / 65 / 78,
 // 100 x 300 94 / 88 / 88 / 85, 20 x 128 x 256 90 / 83 / 69 / 69.
@@ -1548,6 +1551,7 @@ extern "C" int slayer_b200_orthogonalize(void *out, const void *in, int dtype, i
     if (batch == 0 || rows == 0 || cols == 0) return SLAYER_B200_OK;
     SB200_REQUIRE(out && in && workspace, "orthogonalize: null pointer");
     SB200_REQUIRE(((uintptr_t)workspace & 255) == 0, "orthogonalize: the workspace must be aligned to 256 bytes");
+    SB200_REQUIRE(ns_placed(out, dtype) && ns_placed(in, dtype), "orthogonalize: out and in must be aligned to their elements");
     const size_t bytes = (size_t)rows * cols * (dtype == SLAYER_B200_F32 ? 4 : 2);
     for (int64_t first = 0; first < batch; first += kMaxJobs) {
         NsArgs A = {};
@@ -1608,6 +1612,8 @@ extern "C" int slayer_b200_muon_step(const slayer_b200_muon_matrix *list, int64_
         rc = ns_shape("muon_step", M.rows, M.cols);
         if (rc) return rc;
         SB200_REQUIRE(M.rows == 0 || M.cols == 0 || (M.weight && M.grad && M.momentum && workspace), "muon_step: null pointer");
+        SB200_REQUIRE(ns_placed(M.weight, dtype) && ns_placed(M.grad, dtype) && ns_placed(M.momentum, SLAYER_B200_F32),
+                      "muon_step: weight, grad and momentum must be aligned to their elements");
     }
     int64_t i = 0;
     while (i < count) {

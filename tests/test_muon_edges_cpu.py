@@ -18,3 +18,16 @@ def test_matrices_that_are_too_large_have_no_workspace():
     lst[1].rows, lst[1].cols = 1, 1 << 22
     assert lib.slayer_b200_orthogonalize_workspace(1, 1, 1 << 22, 0) > 0
     assert lib.slayer_b200_muon_step_workspace(ctypes.cast(lst, ctypes.c_void_p), 2, 0) > 0
+
+
+def test_places_that_the_kernels_cannot_access():
+    lib, at = capi.load(), ctypes.c_void_p
+    for dtype, off in ((0, 2), (0, 1), (1, 1), (2, 1)):
+        for out, src in ((256 + off, 256), (256, 256 + off)):
+            assert lib.slayer_b200_orthogonalize(at(out), at(src), dtype, 1, 4, 5, 5, 3.4445, -4.775, 2.0315, 1e-7, at(256), at(0)) == -1
+            assert b"aligned" in lib.slayer_b200_last_error()
+    for dtype, bad in ((0, dict(weight=258)), (0, dict(grad=258)), (1, dict(weight=257)), (2, dict(grad=257)), (1, dict(momentum=258))):
+        m = capi.MuonMatrix(**{**dict(weight=256, grad=256, momentum=256, rows=4, cols=5), **bad})
+        assert lib.slayer_b200_muon_step(ctypes.cast(ctypes.pointer(m), at), 1, dtype, 0.1, 0.9, 1, 0.0, 1, 5, 3.4445, -4.775, 2.0315, 1e-7, at(256),
+                                         at(0)) == -1
+        assert b"aligned" in lib.slayer_b200_last_error()
