@@ -366,12 +366,12 @@ typedef struct {
 
 /*
  * One step of the Muon optimiser on `count` weights (list: host memory, read before the call
- * returns), in a fixed number of launches:
+ * returns), in one to three launches for up to 48 of them (fewer where 4 GB hold no more):
  *   momentum <- mu momentum + grad,   u = grad + mu momentum if nesterov else momentum,
  *   weight   <- weight (1 - lr weight_decay) - lr factor X,   X = u made orthogonal as above.
  * The weights must not overlap.  Sizes and workspace (slayer_b200_muon_step_workspace(...) bytes) as
- * above; nothing is launched where a matrix is refused.  It has no counterpart in the reference, whose optimizer is Nadam
- * (src/optimizer.py:6-113).
+ * above; nothing is launched where a matrix is refused.  It has no counterpart in the reference,
+ * whose optimizer is Nadam (src/optimizer.py:6-113).
  */
 int slayer_b200_muon_step(const slayer_b200_muon_matrix *list, int64_t count, int dtype, float lr, float mu, int nesterov,
                           float weight_decay, int adjust, int steps, float a, float b, float c, float eps, void *workspace, void *stream);

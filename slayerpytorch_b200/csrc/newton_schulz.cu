@@ -27,7 +27,8 @@
 
 namespace sb200 {
 
-constexpr int kMaxJobs = 48;         // matrices per launch
+constexpr int kMaxJobs = 48;         // matrices per launch,
+constexpr int64_t kMostBytes = 4ll << 30;      // fewer where their workspace would pass this (one of 2300 x 2300 fills the SMs alone)
 constexpr int kNormParts = 256;      // partial sums of squares per matrix
 constexpr int kStatusNsTimeout = 0x5103;
 constexpr int kWaitLimit = 1 << 22;
@@ -1312,6 +1313,9 @@ static size_t ns_job_bytes(int64_t m, int64_t n, int dtype)
     return kNormParts * 8 + 256 + (size_t)(2 * rb * cbn + 4 * rb * rb) * (size_t)(parts * kBlock);
 }
 
+// how many matrices of this many bytes a launch takes
+static int ns_at_once(int64_t bytes) { return bytes * kMaxJobs <= kMostBytes ? kMaxJobs : bytes <= kMostBytes ? (int)(kMostBytes / bytes) : 1; }
+
 static void ns_take(NsJob &J, int parts, unsigned char *&at)
 {
     const int64_t rb = ns_rb(J.m), x = rb * ns_cb(J.n) * parts * kBlock, a = 2 * rb * rb * parts * kBlock;
@@ -1536,7 +1540,8 @@ extern "C" int64_t slayer_b200_orthogonalize_workspace(int64_t batch, int64_t ro
     if (batch <= 0 || rows <= 0 || cols <= 0) return 0;
     clear_error();
     if (const int rc = ns_shape("orthogonalize", rows, cols)) return rc;
-    return (int64_t)ns_job_bytes(rows < cols ? rows : cols, rows < cols ? cols : rows, dtype) * (batch < kMaxJobs ? batch : kMaxJobs);
+    const int64_t each = (int64_t)ns_job_bytes(rows < cols ? rows : cols, rows < cols ? cols : rows, dtype), most = ns_at_once(each);
+    return each * (batch < most ? batch : most);
 }
 
 extern "C" int slayer_b200_orthogonalize(void *out, const void *in, int dtype, int64_t batch, int64_t rows, int64_t cols, int steps,
@@ -1553,9 +1558,10 @@ extern "C" int slayer_b200_orthogonalize(void *out, const void *in, int dtype, i
     SB200_REQUIRE(((uintptr_t)workspace & 255) == 0, "orthogonalize: the workspace must be aligned to 256 bytes");
     SB200_REQUIRE(ns_placed(out, dtype) && ns_placed(in, dtype), "orthogonalize: out and in must be aligned to their elements");
     const size_t bytes = (size_t)rows * cols * (dtype == SLAYER_B200_F32 ? 4 : 2);
-    for (int64_t first = 0; first < batch; first += kMaxJobs) {
+    const int most = ns_at_once((int64_t)ns_job_bytes(rows < cols ? rows : cols, rows < cols ? cols : rows, dtype));
+    for (int64_t first = 0; first < batch; first += most) {
         NsArgs A = {};
-        A.jobs = (int)(batch - first < kMaxJobs ? batch - first : kMaxJobs);
+        A.jobs = (int)(batch - first < most ? batch - first : most);
         A.ca = a;
         A.cb = b;
         A.cc = c;
@@ -1580,20 +1586,19 @@ extern "C" int slayer_b200_orthogonalize(void *out, const void *in, int dtype, i
 extern "C" int64_t slayer_b200_muon_step_workspace(const slayer_b200_muon_matrix *list, int64_t count, int dtype)
 {
     clear_error();
-    size_t most = 0, now = 0;
+    int64_t most = 0, now = 0;
     int in = 0;
     for (int64_t i = 0; list && i < count; ++i) {
         const int64_t rows = list[i].rows, cols = list[i].cols;
         if (rows <= 0 || cols <= 0) continue;
         if (const int rc = ns_shape("muon_step", rows, cols)) return rc;
-        if (in++ == kMaxJobs) {
-            in = 1;
-            now = 0;
-        }
-        now += ns_job_bytes(rows < cols ? rows : cols, rows < cols ? cols : rows, dtype);
+        const int64_t bytes = (int64_t)ns_job_bytes(rows < cols ? rows : cols, rows < cols ? cols : rows, dtype);
+        if (in == kMaxJobs || (in > 0 && now + bytes > kMostBytes)) in = 0, now = 0;       // as slayer_b200_muon_step does
+        ++in;
+        now += bytes;
         most = now > most ? now : most;
     }
-    return (int64_t)most;
+    return most;
 }
 
 extern "C" int slayer_b200_muon_step(const slayer_b200_muon_matrix *list, int64_t count, int dtype, float lr, float momentum, int nesterov,
@@ -1628,14 +1633,16 @@ extern "C" int slayer_b200_muon_step(const slayer_b200_muon_matrix *list, int64_
         for (; i < count && A.jobs < kMaxJobs; ++i) {
             const slayer_b200_muon_matrix &M = list[i];
             if (M.rows == 0 || M.cols == 0) continue;
+            const int64_t m = M.rows < M.cols ? M.rows : M.cols, n = M.rows < M.cols ? M.cols : M.rows;
+            if (A.jobs > 0 && (at - (unsigned char *)workspace) + (int64_t)ns_job_bytes(m, n, dtype) > kMostBytes) break;
             NsJob &J = A.job[A.jobs++];
             J.src = M.grad;
             J.mom = M.momentum;
             J.dst = M.weight;
             J.rows = (int)M.rows;
             J.cols = (int)M.cols;
-            J.m = J.rows < J.cols ? J.rows : J.cols;
-            J.n = J.rows < J.cols ? J.cols : J.rows;
+            J.m = (int)m;
+            J.n = (int)n;
             const double r = (double)J.rows / J.cols;
             const double factor = adjust == SLAYER_B200_MUON_SHAPE ? (r > 1.0 ? sqrt(r) : 1.0)
                                 : adjust == SLAYER_B200_MUON_RMS   ? 0.2 * sqrt((double)J.n) : 1.0;

@@ -38,7 +38,7 @@ def orthogonalize(matrix, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
 @torch.no_grad()
 def muonStep(weights, grads, momenta, lr, momentum=0.95, nesterov=True, weightDecay=0.0, steps=5, coefficients=COEFFICIENTS, eps=1e-7,
              adjust='shape'):
-    """One optimiser step on lists of weights, in place, in a fixed number of launches for all of them::
+    """One optimiser step on lists of weights, in place, in one to three launches for up to 48 of them (fewer of the largest)::
 
         mom    = momentum * mom + grad
         update = orthogonalize(grad + momentum * mom if nesterov else mom)

@@ -31,3 +31,16 @@ def test_places_that_the_kernels_cannot_access():
         assert lib.slayer_b200_muon_step(ctypes.cast(ctypes.pointer(m), at), 1, dtype, 0.1, 0.9, 1, 0.0, 1, 5, 3.4445, -4.775, 2.0315, 1e-7, at(256),
                                          at(0)) == -1
         assert b"aligned" in lib.slayer_b200_last_error()
+
+
+def test_workspaces_of_many_large_matrices_are_bounded():
+    """A stack or a list of large matrices is worked on a few at a time: 4 GB, or what one of them needs."""
+    lib = capi.load()
+    for side, count in ((4096, 48), (8192, 100), (16384, 25)):
+        for dtype in (0, 1, 2):
+            one = lib.slayer_b200_orthogonalize_workspace(1, side, side, dtype)
+            assert 0 < lib.slayer_b200_orthogonalize_workspace(count, side, side, dtype) <= max(one, 4 << 30)
+            lst = (capi.MuonMatrix * (2 * count))()
+            for i, m in enumerate(lst):
+                m.rows, m.cols = (side, side) if i % 2 else (300, 500)
+            assert one <= lib.slayer_b200_muon_step_workspace(ctypes.cast(lst, ctypes.c_void_p), 2 * count, dtype) <= max(one, 4 << 30)

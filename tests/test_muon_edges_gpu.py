@@ -151,3 +151,22 @@ def test_errors_of_bfloat16_matrices(shape):
     x = gradient(shape, 6, torch.bfloat16).cuda()
     want = want_orthogonal(x)
     assert off(optim.orthogonalize(x), want) <= math.hypot(2.96e-3, off(want.bfloat16(), want))
+
+
+def test_stacks_and_lists_that_a_launch_does_not_hold():
+    """More matrices than 4 GB of workspace take at once; each comes out as it does alone."""
+    x = torch.randn(40, 4096, 4096, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda", dtype=torch.bfloat16)
+    got = optim.orthogonalize(x)
+    for i in (0, 29, 30, 31, 32, 39):
+        assert torch.equal(got[i], optim.orthogonalize(x[i]))
+    small = torch.randn(30, 300, 500, generator=torch.Generator(device="cuda").manual_seed(2), device="cuda", dtype=torch.bfloat16)
+    grads = [t for pair in zip(x, small) for t in pair] + list(x[30:])
+    weights, momenta = [torch.zeros_like(g) for g in grads], [torch.zeros(g.shape, device="cuda") for g in grads]
+    optim.muonStep(weights, grads, momenta, lr=1.0, nesterov=False, adjust=None)
+    for w, g, m in zip(weights, grads, momenta):
+        assert torch.equal(m, g.float())
+    for i in (0, 28, 58, 59, 60, 69):
+        if grads[i].shape[0] == 4096:
+            assert torch.equal(weights[i], -optim.orthogonalize(grads[i]))
+        else:
+            near(-weights[i], want_orthogonal(grads[i]).cpu(), torch.bfloat16, 300)
