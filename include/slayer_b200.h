@@ -339,9 +339,9 @@ int64_t slayer_b200_preference_loss_workspace(int64_t sequences);
  * A stack of matrices made near orthogonal by Newton-Schulz products: each [rows, cols] matrix u of
  * in (type `dtype`, contiguous, `batch` of them) becomes X after
  *   X = u / (|u|_F + eps),   `steps` times  X <- a X + (b A + c A A) X,  A = X X^T
- * (of a matrix with more rows than columns, the transpose's).  out may be in.  Float32 and float16
- * matrices are worked on with products of 22 bits, bfloat16 ones with 11 (entries of X are held to
- * 2^-37 at best, which is fewer where |u| is below a thousandth of eps).  Coefficients whose steps
+ * (of a matrix with more rows than columns, the transpose's).  out may be in.  All types are worked on
+ * with products of 22 bits (entries of X are held to 2^-37 at best, which is fewer where |u| is below
+ * a thousandth of eps).  Coefficients whose steps
  * take singular values from [0, 1] past 3.5 are refused.  At most 32768 on the shorter side, 2^22 on
  * the longer and 2^31 elements per matrix, else SLAYER_B200_EUNSUPPORTED.  workspace:
  * slayer_b200_orthogonalize_workspace(...) bytes of device memory, aligned to 256 (that code where a

@@ -8,11 +8,11 @@
 // The work is matrix products, m m n + m m m + 2 m m n multiply-adds a step for m <= n with the symmetric halves left out, so
 // they run on the tensor cores, on 16-bit parts of the 32-bit values.  Everything has a known size - |X|_F <= 1 at the start, no
 // singular value ever above 3.5 - so fp16 with a fixed power-of-two scale holds it, and holds 11 bits where bf16 holds 8.
-//   PARTS = 2 (float32, float16 weights): v = hi + lo, two fp16 values, 22 bits and a sign;  v w ~ hi hi + hi lo + lo hi, the
-//     left out lo lo being 2^-24 of it.  Three products instead of one.
-//   PARTS = 1 (bfloat16 weights, whose update is rounded to 8 bits in the end): v = hi.
-// Sums are fp32: with two parts those of 64 to 192 products in tensor memory, of up to 128 in matrices that stay on the chip, longer ones in
-// registers (see NsTile::group).  Five steps end 0.2 to 0.7 times as far off as with fp32 products, on the chip 0.8 to 2.9 times.
+//     v = hi + lo, two fp16 values, 22 bits and a sign;  v w ~ hi hi + hi lo + lo hi, the left out lo lo being 2^-24 of it.
+// Three products instead of one, for bfloat16 matrices too: with hi alone, 11 bits, their results ended 1.2 to 2.2 times as far off as
+// their own rounding to 8 bits (6 x 1023 x 2049 in 387 us instead of 715).
+// Sums are fp32: those of 64 to 192 products in tensor memory, of up to 128 in matrices that stay on the chip, longer ones in registers
+// (see NsTile::group).  Five steps end 0.2 to 0.7 times as far off as with fp32 products, on the chip 0.8 to 2.9 times.
 // Entries of X are held to 2^-37 at best (an fp16's smallest step over the scale): enough where the norm is not far below eps.
 //
 // X, A and B = b A + c A A live in the workspace as blocks of 128 x 64 elements, padded with zeros, each block laid out as the
@@ -21,6 +21,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 #include "tensor.cuh"
@@ -32,6 +34,7 @@ constexpr int64_t kMostBytes = 4ll << 30;      // fewer where their workspace wo
 constexpr int kNormParts = 256;      // partial sums of squares per matrix
 constexpr int kStatusNsTimeout = 0x5103;
 constexpr int kWaitLimit = 1 << 22;
+constexpr int kParts = 2;            // fp16 values that a value is kept as
 constexpr int kBlock = 128 * 64 * 2; // bytes of a block
 constexpr float kScaleX = 8192.0f, kScaleA = 4096.0f;      // of X; of A and B
 
@@ -218,27 +221,23 @@ __global__ void __launch_bounds__(256) ns_momentum_kernel(const __grid_constant_
 }
 
 // two values next to each other as their fp16 parts
-template <int PARTS>
 __device__ __forceinline__ void ns_split(float v0, float v1, uint32_t &hi, uint32_t &lo)
 {
     const __half2 h = __floats2half2_rn(v0, v1);
     hi = *reinterpret_cast<const uint32_t *>(&h);
-    if (PARTS == 2) {
-        const float2 f = __half22float2(h);
-        const __half2 l = __floats2half2_rn(v0 - f.x, v1 - f.y);
-        lo = *reinterpret_cast<const uint32_t *>(&l);
-    }
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(v0 - f.x, v1 - f.y);
+    lo = *reinterpret_cast<const uint32_t *>(&l);
 }
 
 // where the 16-byte chunk (8 columns from c on) of element (r, c) begins, in blocks of cbs column blocks per row block
-template <int PARTS>
 __device__ __forceinline__ unsigned char *ns_chunk(unsigned char *x, int cbs, int r, int c)
 {
-    return x + ((int64_t)(r >> 7) * cbs + (c >> 6)) * (PARTS * kBlock) + (r & 127) * 128 + (((c >> 3) & 7) ^ (r & 7)) * 16;
+    return x + ((int64_t)(r >> 7) * cbs + (c >> 6)) * (kParts * kBlock) + (r & 127) * 128 + (((c >> 3) & 7) ^ (r & 7)) * 16;
 }
 
 // X0, as blocks: a thread makes a chunk of eight columns
-template <typename T, int PARTS>
+template <typename T>
 __global__ void __launch_bounds__(256) ns_normalise_kernel(const __grid_constant__ NsArgs A)
 {
     __shared__ double part[32];
@@ -280,13 +279,13 @@ __global__ void __launch_bounds__(256) ns_normalise_kernel(const __grid_constant
             }
         }
         uint4 hi, lo;
-        ns_split<PARTS>(v[0], v[1], hi.x, lo.x);
-        ns_split<PARTS>(v[2], v[3], hi.y, lo.y);
-        ns_split<PARTS>(v[4], v[5], hi.z, lo.z);
-        ns_split<PARTS>(v[6], v[7], hi.w, lo.w);
-        unsigned char *at = ns_chunk<PARTS>(J.x[0], cbs, r, c);
+        ns_split(v[0], v[1], hi.x, lo.x);
+        ns_split(v[2], v[3], hi.y, lo.y);
+        ns_split(v[4], v[5], hi.z, lo.z);
+        ns_split(v[6], v[7], hi.w, lo.w);
+        unsigned char *at = ns_chunk(J.x[0], cbs, r, c);
         *(uint4 *)at = hi;
-        if (PARTS == 2) *(uint4 *)(at + kBlock) = lo;
+        *(uint4 *)(at + kBlock) = lo;
     }
 }
 
@@ -298,30 +297,30 @@ enum NsPhase { kGram, kPolynomial, kUpdate };
 // products of a pair.
 enum NsMode { kAlone, kShared, kPair };
 
-template <int PARTS, int MODE>
+template <int MODE>
 struct NsTile {
     static constexpr int CG = MODE == kPair ? 2 : 1;
     static constexpr int TN = 128 * CG;                      // columns of the result, of which each CTA has 128 rows
-    static constexpr int kA = PARTS * kBlock, kB = PARTS * kBlock, kStage = kA + kB;
+    static constexpr int kA = kParts * kBlock, kB = kParts * kBlock, kStage = kA + kB;
     // a warp that loads, one that issues products, two to fill up; and those that take the results
     static constexpr int kTakers = 8, kThreads = 128 + 32 * kTakers;
     static constexpr int kWide = TN / (kTakers / 4), kPieces = kWide / 32;       // columns of a warp's 32 rows, pieces
     static constexpr int kPiece = 32 * 33 * 4;               // a 32 x 32 piece of each of these warps
     static constexpr int kExchange = MODE == kShared ? 128 * 128 * 4 : 0;          // the sums of those that share a tile
     static constexpr int kFixed = 1024 + 512 + kTakers * kPiece + kExchange;
-    static constexpr int kStages = (227 * 1024 - kFixed) / kStage > 6 ? 6 : (227 * 1024 - kFixed) / kStage;
+    static constexpr int kStages = (227 * 1024 - kFixed) / kStage;
     static constexpr size_t kSmem = kFixed + (size_t)kStages * kStage;
     // Of `steps` steps of 64, how many have their sum in tensor memory at a time.  The tensor core cuts what it adds to a sum instead of
-    // rounding it: over the 375 additions of a sum of 2000 products in two parts that is a bias of 1e-5, ten times the rounding
-    // of fp32 sums.  So with two parts the sums of 64 products are added up in registers, rounded, while the next ones are made:
+    // rounding it: over the 375 additions of a sum of 2000 products of two parts each that is a bias of 1e-5, ten times the rounding
+    // of fp32 sums.  So the sums of 64 products are added up in registers, rounded, while the next ones are made:
     // 2000 x 333 is 2.4e-6 off after five steps (fp32 products: 2.5e-6), with sums of 128 4e-6.  In a pair's tiles, groups of more
     // steps let the products run further ahead while a tile's results are taken, and long sums are further off in fp32 too:
     // 4096 x 4096 3.70 / 3.47 / 3.36 / 3.35 ms and 1.0 / 1.2 / 1.6 / 1.9e-6 off with groups of 1 / 2 / 3 / 4 (fp32 products 4.8e-6), 700 x 700
-    // 1.5 / 2.0e-6 with 2 / 3 (2.7e-6), 260 x 140 0.9 / 1.8 / 2.1e-6 with 1 / 2 / 3 (1.6e-6).
-    static __device__ __forceinline__ int group(int steps)
+    // 1.5 / 2.0e-6 with 2 / 3 (2.7e-6), 260 x 140 0.9 / 1.8 / 2.1e-6 with 1 / 2 / 3 (1.6e-6).  Results that are rounded to 8 bits (brief)
+    // can do with sums of 1024 products, a bias of 1e-5: 6 x 1023 x 2049 768 -> 715 us, 4096 x 4096 3.54 -> 3.42 ms.
+    static __device__ __forceinline__ int group(int steps, bool brief)
     {
-        if (PARTS == 1) return 1 << 20;
-        return MODE != kPair || steps < 8 ? 1 : steps < 16 ? 2 : 3;
+        return brief ? 16 : MODE != kPair || steps < 8 ? 1 : steps < 16 ? 2 : 3;
     }
 };
 
@@ -337,24 +336,23 @@ __device__ __forceinline__ uint4 *ns_piece_line(unsigned char *block, int r0, in
 }
 
 // What the result is made of besides the product: of b, a; of x', x.
-template <int PARTS>
 struct NsOld {
-    uint4 v[PARTS][4];
+    uint4 v[kParts][4];
     // requested early, put into the piece when it is wanted
     __device__ __forceinline__ void request(const NsJob &J, int kind, int from, int r0, int c, int lane)
     {
         if (kind == kGram) return;
         const int cbs = kind == kUpdate ? ns_cb(J.n) : ns_cb(J.m);
-        unsigned char *block = (kind == kPolynomial ? J.a : J.x[from]) + ((int64_t)(r0 >> 7) * cbs + (c >> 6)) * (PARTS * kBlock);
+        unsigned char *block = (kind == kPolynomial ? J.a : J.x[from]) + ((int64_t)(r0 >> 7) * cbs + (c >> 6)) * (kParts * kBlock);
 #pragma unroll
-        for (int p = 0; p < PARTS; ++p)
+        for (int p = 0; p < kParts; ++p)
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[p][i] = __ldcg(ns_piece_line(block, r0, c, lane) + (p * kBlock + i * 1024) / 16);
     }
     __device__ __forceinline__ void put(unsigned char *piece, int lane) const
     {
 #pragma unroll
-        for (int p = 0; p < PARTS; ++p)
+        for (int p = 0; p < kParts; ++p)
 #pragma unroll
             for (int i = 0; i < 4; ++i) *(uint4 *)(piece + ns_piece_at(lane >> 2, lane & 3) + p * 2048 + i * 512) = v[p][i];
     }
@@ -362,9 +360,9 @@ struct NsOld {
 
 // What a warp does with 32 rows (from r0, lane = row) x 32 columns (from c) of a result.  next: the columns of the piece that
 // follows, whose old values are requested meanwhile, or -1.
-template <int PARTS, typename T>
+template <typename T>
 __device__ __forceinline__ void ns_take_piece(const NsArgs &A, const NsJob &J, int kind, bool last, int from, int r0, int c, float (&v)[32],
-                                              unsigned char *piece, int lane, NsOld<PARTS> &old, int next)
+                                              unsigned char *piece, int lane, NsOld &old, int next)
 {
     if (kind == kGram) {
 #pragma unroll
@@ -380,16 +378,14 @@ __device__ __forceinline__ void ns_take_piece(const NsArgs &A, const NsJob &J, i
         for (int k = 0; k < 4; ++k) {
             const uint4 hi = *(const uint4 *)(piece + ns_piece_at(lane, k));
             uint4 lo = make_uint4(0, 0, 0, 0);
-            if (PARTS == 2) lo = *(const uint4 *)(piece + 2048 + ns_piece_at(lane, k));
+            lo = *(const uint4 *)(piece + 2048 + ns_piece_at(lane, k));
             const uint32_t hs[4] = {hi.x, hi.y, hi.z, hi.w}, ls[4] = {lo.x, lo.y, lo.z, lo.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 float2 o = __half22float2(*reinterpret_cast<const __half2 *>(&hs[e]));
-                if (PARTS == 2) {
-                    const float2 l = __half22float2(*reinterpret_cast<const __half2 *>(&ls[e]));
-                    o.x += l.x;
-                    o.y += l.y;
-                }
+                const float2 l = __half22float2(*reinterpret_cast<const __half2 *>(&ls[e]));
+                o.x += l.x;
+                o.y += l.y;
                 v[8 * k + 2 * e] = fmaf(f, o.x, by * v[8 * k + 2 * e]);
                 v[8 * k + 2 * e + 1] = fmaf(f, o.y, by * v[8 * k + 2 * e + 1]);
             }
@@ -445,20 +441,20 @@ __device__ __forceinline__ void ns_take_piece(const NsArgs &A, const NsJob &J, i
         __syncwarp();
     } else {
         const int cbs = kind == kUpdate ? ns_cb(J.n) : ns_cb(J.m);
-        unsigned char *to = (kind == kGram ? J.a : kind == kPolynomial ? J.b : J.x[from ^ 1]) + ((int64_t)(r0 >> 7) * cbs + (c >> 6)) * (PARTS * kBlock);
+        unsigned char *to = (kind == kGram ? J.a : kind == kPolynomial ? J.b : J.x[from ^ 1]) + ((int64_t)(r0 >> 7) * cbs + (c >> 6)) * (kParts * kBlock);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             uint4 hi, lo;
-            ns_split<PARTS>(v[8 * k], v[8 * k + 1], hi.x, lo.x);
-            ns_split<PARTS>(v[8 * k + 2], v[8 * k + 3], hi.y, lo.y);
-            ns_split<PARTS>(v[8 * k + 4], v[8 * k + 5], hi.z, lo.z);
-            ns_split<PARTS>(v[8 * k + 6], v[8 * k + 7], hi.w, lo.w);
+            ns_split(v[8 * k], v[8 * k + 1], hi.x, lo.x);
+            ns_split(v[8 * k + 2], v[8 * k + 3], hi.y, lo.y);
+            ns_split(v[8 * k + 4], v[8 * k + 5], hi.z, lo.z);
+            ns_split(v[8 * k + 6], v[8 * k + 7], hi.w, lo.w);
             *(uint4 *)(piece + ns_piece_at(lane, k)) = hi;
-            if (PARTS == 2) *(uint4 *)(piece + 2048 + ns_piece_at(lane, k)) = lo;
+            *(uint4 *)(piece + 2048 + ns_piece_at(lane, k)) = lo;
         }
         __syncwarp();
 #pragma unroll
-        for (int p = 0; p < PARTS; ++p)
+        for (int p = 0; p < kParts; ++p)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 ns_piece_line(to, r0, c, lane)[(p * kBlock + i * 1024) / 16] = *(const uint4 *)(piece + ns_piece_at(lane >> 2, lane & 3) + p * 2048 + i * 512);
@@ -484,13 +480,13 @@ struct NsPlan {
     int *status;
 };
 
-template <int PARTS, int MODE, typename T>
-__global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_kernel(const __grid_constant__ NsArgs A, const __grid_constant__ NsPlan P)
+template <int MODE, typename T>
+__global__ void __launch_bounds__(NsTile<MODE>::kThreads, 1) ns_steps_kernel(const __grid_constant__ NsArgs A, const __grid_constant__ NsPlan P)
 {
-    using Tile = NsTile<PARTS, MODE>;
+    using Tile = NsTile<MODE>;
     constexpr int CG = Tile::CG, S = Tile::kStages, TN = Tile::TN, kTakers = Tile::kTakers, kPieces = Tile::kPieces;
-    // pieces of the old values that a warp requests before its sums are complete (two parts: as many as the registers hold)
-    constexpr int kAhead = PARTS == 2 && MODE != kAlone ? 1 : kPieces;
+    // pieces of the old values that a warp requests before its sums are complete (as many as the registers hold)
+    constexpr int kAhead = MODE != kAlone ? 1 : kPieces;
     extern __shared__ unsigned char smem_raw[];
     unsigned char *smem = (unsigned char *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     // full: this CTA's loads are there; ready: the second CTA's are (at the first); empty: a stage has been read; done: a sum is
@@ -595,9 +591,9 @@ __global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_ker
     auto right_turned = [&](int kind, int j, int k) { return kind == kPolynomial ? (k >> 1) < j + CG - 1 : kind == kUpdate; };
 
     if (warp < 4) {
-        // 128 threads give registers to the 256 that hold sums: 128 * 40 + 256 * 224 = 128 * 56 + 256 * 216 <= 384 * 168.  (Sums of 128
-        // columns in two parts need the last eight; elsewhere the loads' addresses do.)
-        if constexpr (MODE == kPair && PARTS == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        // 128 threads give registers to the 256 that hold sums: 128 * 40 + 256 * 224 = 128 * 56 + 256 * 216 <= 384 * 168.  (A pair's sums
+        // of 128 columns need the last eight; elsewhere the loads' addresses do.)
+        if constexpr (MODE == kPair) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         else asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == 0 && lane == 0) {
             int s = 0, turn = 0;
@@ -616,13 +612,13 @@ __global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_ker
                     const unsigned char *right = p.kind == kPolynomial ? J.a : J.x[p.from];
                     const int il = o.i + pair, jr = o.j + pair;        // this CTA's row block and column block; behind the last one, nothing
                     const bool has_left = il < rb, has_right = jr < (p.kind != kUpdate ? rb : ns_rb(J.n));
-                    const unsigned bytes = PARTS * kBlock * (has_left + has_right);
+                    const unsigned bytes = kParts * kBlock * (has_left + has_right);
                     // 64 rows of two blocks of 64 columns: [part][column block]
                     auto columns = [&](unsigned char *to, const unsigned char *x, int cbs, int k, int block) {
-                        const unsigned char *row = x + ((int64_t)(k >> 1) * cbs + 2 * block) * (PARTS * kBlock) + (k & 1) * (kBlock / 2);
+                        const unsigned char *row = x + ((int64_t)(k >> 1) * cbs + 2 * block) * (kParts * kBlock) + (k & 1) * (kBlock / 2);
                         for (int b = 0; b < 2; ++b)
-                            for (int q = 0; q < PARTS; ++q)
-                                bulk_load(to + q * kBlock + b * (kBlock / 2), row + (b * PARTS + q) * kBlock, kBlock / 2, full + s);
+                            for (int q = 0; q < kParts; ++q)
+                                bulk_load(to + q * kBlock + b * (kBlock / 2), row + (b * kParts + q) * kBlock, kBlock / 2, full + s);
                     };
                     for (int k = o.k0; k < o.k1; ++k) {
                         if (!mbar_wait_bounded(empty + s, turn ^ 1, kWaitLimit)) { fine = false; break; }
@@ -630,12 +626,12 @@ __global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_ker
                         mbar_expect_tx(full + s, bytes);
                         if (has_left) {
                             if (left_turned(p.kind, o.i, k)) columns(to, left, cbl, k, il);
-                            else bulk_load(to, left + ((int64_t)il * cbl + k) * (PARTS * kBlock), PARTS * kBlock, full + s);
+                            else bulk_load(to, left + ((int64_t)il * cbl + k) * (kParts * kBlock), kParts * kBlock, full + s);
                         }
                         to += Tile::kA;
                         if (has_right) {
                             if (right_turned(p.kind, o.j, k)) columns(to, right, cbr, k, jr);
-                            else bulk_load(to, right + ((int64_t)jr * cbr + k) * (PARTS * kBlock), PARTS * kBlock, full + s);
+                            else bulk_load(to, right + ((int64_t)jr * cbr + k) * (kParts * kBlock), kParts * kBlock, full + s);
                         }
                         if (++s == S) { s = 0; turn ^= 1; }
                     }
@@ -652,7 +648,7 @@ __global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_ker
                 const Phase p = phase_at(ph, kind);
                 for (int tile = p.tile, it = 0; fine && tile < p.tiles; tile += p.step, ++it) {
                     const Spot o = spot_at(p, tile, it);
-                    const int group = Tile::group(o.k1 - o.k0);
+                    const int group = Tile::group(o.k1 - o.k0, std::is_same<T, __nv_bfloat16>::value);
                     for (int k = o.k0, in = 0; k < o.k1; ++k) {
                         const bool first = in == 0;
                         if (first && !mbar_wait_bounded(taken + slot, again ^ 1, kWaitLimit)) { fine = false; break; }
@@ -666,15 +662,13 @@ __global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_ker
                         const uint64_t l = lt ? desc_columns(a0, kBlock / 2) : desc_rows(a0), r = rt ? desc_columns(b0, kBlock / 2) : desc_rows(b0);
                         const unsigned dl = lt ? 128 : 2, dr = rt ? 128 : 2, other = kBlock / 16;
                         // the small products first: what they lose to the sum's size is less while it is small
-                        if (PARTS == 2) {
 #pragma unroll
-                            for (int q = 0; q < 4; ++q) {
-                                product<CG>(d, l + q * dl, r + q * dr + other, shape, !first || q > 0);
-                                product<CG>(d, l + q * dl + other, r + q * dr, shape, true);
-                            }
+                        for (int q = 0; q < 4; ++q) {
+                            product<CG>(d, l + q * dl, r + q * dr + other, shape, !first || q > 0);
+                            product<CG>(d, l + q * dl + other, r + q * dr, shape, true);
                         }
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) product<CG>(d, l + q * dl, r + q * dr, shape, PARTS == 2 || !first || q > 0);
+                        for (int q = 0; q < 4; ++q) product<CG>(d, l + q * dl, r + q * dr, shape, true);
                         product_commit<CG>(empty + s);
                         if (++s == S) { s = 0; turn ^= 1; }
                         if (++in == group || k + 1 == o.k1) {
@@ -702,7 +696,7 @@ __global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_ker
         }
         __syncwarp();
     } else {
-        if constexpr (MODE == kPair && PARTS == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        if constexpr (MODE == kPair) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         else asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         int slot = 0, again = 0;
         const int w = warp - 4, quarter = warp & 3;
@@ -718,19 +712,17 @@ __global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_ker
             for (int tile = p.tile, it = 0; fine && tile < p.tiles; tile += p.step, ++it) {
                 const Spot o = spot_at(p, tile, it);
                 const NsJob &J = A.job[o.job];
-                const int group = Tile::group(o.k1 - o.k0), groups = (o.k1 - o.k0 + group - 1) / group, rb = ns_rb(J.m);
+                const int group = Tile::group(o.k1 - o.k0, std::is_same<T, __nv_bfloat16>::value), groups = (o.k1 - o.k0 + group - 1) / group, rb = ns_rb(J.m);
                 const int il = o.i + pair, c0 = (w >> 2) * Tile::kWide, jl = o.j + (c0 >> 7);      // this warp's columns of the tile; its blocks
                 const bool mine = il < rb && jl < (p.kind != kUpdate ? rb : ns_rb(J.n)) && !(p.kind != kUpdate && jl < il);
                 const int r0 = il * 128 + quarter * 32, c = o.j * 128 + c0;
                 const uint32_t at = acc + ((uint32_t)(quarter * 32) << 16) + c0;
-                float sum[PARTS == 2 ? kPieces : 1][32];
-                if constexpr (PARTS == 2) {
+                float sum[kPieces][32];
 #pragma unroll
-                    for (int u = 0; u < kPieces; ++u)
+                for (int u = 0; u < kPieces; ++u)
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) sum[u][k] = 0.0f;
-                }
-                NsOld<PARTS> old[kAhead];
+                    for (int k = 0; k < 32; ++k) sum[u][k] = 0.0f;
+                NsOld old[kAhead];
                 if (mine && !(MODE == kShared && p.split > 1)) {
 #pragma unroll
                     for (int u = 0; u < kAhead; ++u) old[u].request(J, p.kind, p.from, r0, c + u * 32, lane);
@@ -748,28 +740,19 @@ __global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_ker
                     if (MODE == kShared && p.split > 1) {
                         give(v, u);
                     } else {
-                        ns_take_piece<PARTS, T>(A, J, p.kind, p.last, p.from, r0, c + u * 32, v, piece, lane, old[u % kAhead], u + kAhead < kPieces ? c + (u + kAhead) * 32 : -1);
+                        ns_take_piece<T>(A, J, p.kind, p.last, p.from, r0, c + u * 32, v, piece, lane, old[u % kAhead], u + kAhead < kPieces ? c + (u + kAhead) * 32 : -1);
                     }
                 };
                 for (int g = 0; g < groups; ++g) {
                     if (!__all_sync(0xffffffffu, mbar_wait_bounded(done + slot, again, kWaitLimit))) { fine = false; break; }
                     tensor_fence_after();
                     if (mine) {
-                        if constexpr (PARTS == 2) {
 #pragma unroll
-                            for (int u = 0; u < kPieces; ++u) {
-                                float v[32];
-                                tensor_read(v, at + slot * TN + u * 32);
+                        for (int u = 0; u < kPieces; ++u) {
+                            float v[32];
+                            tensor_read(v, at + slot * TN + u * 32);
 #pragma unroll
-                                for (int k = 0; k < 32; ++k) sum[u][k] += v[k];
-                            }
-                        } else {
-#pragma unroll
-                            for (int u = 0; u < kPieces; ++u) {
-                                float v[32];
-                                tensor_read(v, at + slot * TN + u * 32);
-                                pass_on(v, u);
-                            }
+                            for (int k = 0; k < 32; ++k) sum[u][k] += v[k];
                         }
                     }
                     tensor_fence_before();
@@ -780,18 +763,13 @@ __global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_ker
                     }
                     if ((slot ^= 1) == 0) again ^= 1;
                 }
-                if (PARTS == 2 && MODE == kShared && p.split > 1) {
+                if (MODE == kShared && p.split > 1) {
 #pragma unroll
-                    for (int u = 0; u < kPieces; ++u) give(sum[PARTS == 2 ? u : 0], u);
-                } else if (fine && mine && (PARTS == 2 || groups == 0)) {        // no groups: more CTAs than steps
+                    for (int u = 0; u < kPieces; ++u) give(sum[u], u);
+                } else if (fine && mine) {
 #pragma unroll
                     for (int u = 0; u < kPieces; ++u) {
-                        if constexpr (PARTS == 2) {
-                            pass_on(sum[u], u);
-                        } else {
-                            float v[32] = {};
-                            pass_on(v, u);
-                        }
+                        pass_on(sum[u], u);
                     }
                 }
             }
@@ -802,7 +780,7 @@ __global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_ker
                     const Spot &o = spots[kind][0];
                     // this CTA's pieces of 32 x 32; warp w takes the w-th of them
                     const int many = 16 / p.split, id = w * p.split + p.rank, part = id & 3, c = id >> 2;
-                    NsOld<PARTS> old;
+                    NsOld old;
                     if (w < many) old.request(A.job[o.job], p.kind, p.from, o.i * 128 + part * 32, o.j * 128 + c * 32, lane);
                     fine = __all_sync(0xffffffffu, mbar_acquire_bounded(given + p.kind, ph / 3 & 1, kWaitLimit)) && fine;
                     if (w < many) {
@@ -818,7 +796,7 @@ __global__ void __launch_bounds__(NsTile<PARTS, MODE>::kThreads, 1) ns_steps_ker
                                 v[4 * k + 3] += x.w;
                             }
                         }
-                        ns_take_piece<PARTS, T>(A, A.job[o.job], p.kind, p.last, p.from, o.i * 128 + part * 32, o.j * 128 + c * 32, v, piece, lane, old, -1);
+                        ns_take_piece<T>(A, A.job[o.job], p.kind, p.last, p.from, o.i * 128 + part * 32, o.j * 128 + c * 32, v, piece, lane, old, -1);
                     }
                 }
             }
@@ -858,12 +836,12 @@ struct NsSmall {
 };
 
 // where things lie in the shared memory of a CTA with `per` column blocks of a matrix of m rows
-static __host__ __device__ __forceinline__ NsSmall ns_small(int m, int per, int parts)
+static __host__ __device__ __forceinline__ NsSmall ns_small(int m, int per)
 {
     NsSmall s;
     s.rows = (m + 15) / 16 * 16;
     s.per = per;
-    s.block = parts * s.rows * 128;
+    s.block = kParts * s.rows * 128;
     s.x = per * s.block;
     // A, later B: as blocks; before that, fp32 sums for the exchange.  The last operand's 128 rows reach 16 KB behind its start.
     const int abs = (s.rows + 63) / 64 * s.block, sums = s.rows * s.rows * 4, reach = abs - s.rows * 128 + kBlock;
@@ -917,24 +895,22 @@ __device__ __forceinline__ void ns_load_u(const NsArgs &A, const NsJob &J, int r
 }
 
 // sixteen columns of a row, as two chunks of a block
-template <int PARTS>
 __device__ __forceinline__ void ns_put16(unsigned char *row, int part_bytes, int chunk, int r, const float (&v)[16])
 {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
         uint4 hi, lo;
-        ns_split<PARTS>(v[8 * k], v[8 * k + 1], hi.x, lo.x);
-        ns_split<PARTS>(v[8 * k + 2], v[8 * k + 3], hi.y, lo.y);
-        ns_split<PARTS>(v[8 * k + 4], v[8 * k + 5], hi.z, lo.z);
-        ns_split<PARTS>(v[8 * k + 6], v[8 * k + 7], hi.w, lo.w);
+        ns_split(v[8 * k], v[8 * k + 1], hi.x, lo.x);
+        ns_split(v[8 * k + 2], v[8 * k + 3], hi.y, lo.y);
+        ns_split(v[8 * k + 4], v[8 * k + 5], hi.z, lo.z);
+        ns_split(v[8 * k + 6], v[8 * k + 7], hi.w, lo.w);
         unsigned char *at = row + (((chunk + k) ^ r) & 7) * 16;
         *(uint4 *)at = hi;
-        if (PARTS == 2) *(uint4 *)(at + part_bytes) = lo;
+        *(uint4 *)(at + part_bytes) = lo;
     }
 }
 
 // v <- f old + by v for the same
-template <int PARTS>
 __device__ __forceinline__ void ns_add16(const unsigned char *row, int part_bytes, int chunk, int r, float f, float by, float (&v)[16])
 {
 #pragma unroll
@@ -942,23 +918,21 @@ __device__ __forceinline__ void ns_add16(const unsigned char *row, int part_byte
         const unsigned char *at = row + (((chunk + k) ^ r) & 7) * 16;
         const uint4 hi = *(const uint4 *)at;
         uint4 lo = make_uint4(0, 0, 0, 0);
-        if (PARTS == 2) lo = *(const uint4 *)(at + part_bytes);
+        lo = *(const uint4 *)(at + part_bytes);
         const uint32_t hs[4] = {hi.x, hi.y, hi.z, hi.w}, ls[4] = {lo.x, lo.y, lo.z, lo.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             float2 o = __half22float2(*reinterpret_cast<const __half2 *>(&hs[e]));
-            if (PARTS == 2) {
-                const float2 l = __half22float2(*reinterpret_cast<const __half2 *>(&ls[e]));
-                o.x += l.x;
-                o.y += l.y;
-            }
+            const float2 l = __half22float2(*reinterpret_cast<const __half2 *>(&ls[e]));
+            o.x += l.x;
+            o.y += l.y;
             v[8 * k + 2 * e] = fmaf(f, o.x, by * v[8 * k + 2 * e]);
             v[8 * k + 2 * e + 1] = fmaf(f, o.y, by * v[8 * k + 2 * e + 1]);
         }
     }
 }
 
-template <typename T, int PARTS>
+template <typename T>
 __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid_constant__ NsArgs A, int steps, int *status)
 {
     extern __shared__ unsigned char smem_raw[];
@@ -970,7 +944,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
     const int C = (int)cluster_size(), rank = (int)cluster_rank();
     const NsJob &J = A.job[blockIdx.x / C];
     const int blocks = (J.n + 63) / 64;
-    const NsSmall L = ns_small(J.m, (blocks + C - 1) / C, PARTS);
+    const NsSmall L = ns_small(J.m, (blocks + C - 1) / C);
     const int b0 = min(rank * L.per, blocks), nb = min(L.per, blocks - b0), R = L.rows, side = R * 128;
     unsigned char *x = smem, *ab = smem + L.x;
     if (warp == 0) tensor_alloc<1>(&base_at, 512);
@@ -1006,13 +980,13 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
         float v[8] = {};
         if (r < J.m) ns_load_u<T>(A, J, r, b0 * 64 + ch * 8, false, v);
         uint4 hi, lo;
-        ns_split<PARTS>(scale(v[0]), scale(v[1]), hi.x, lo.x);
-        ns_split<PARTS>(scale(v[2]), scale(v[3]), hi.y, lo.y);
-        ns_split<PARTS>(scale(v[4]), scale(v[5]), hi.z, lo.z);
-        ns_split<PARTS>(scale(v[6]), scale(v[7]), hi.w, lo.w);
+        ns_split(scale(v[0]), scale(v[1]), hi.x, lo.x);
+        ns_split(scale(v[2]), scale(v[3]), hi.y, lo.y);
+        ns_split(scale(v[4]), scale(v[5]), hi.z, lo.z);
+        ns_split(scale(v[6]), scale(v[7]), hi.w, lo.w);
         unsigned char *at = x + (ch >> 3) * L.block + r * 128 + ((ch ^ r) & 7) * 16;
         *(uint4 *)at = hi;
-        if (PARTS == 2) *(uint4 *)(at + side) = lo;
+        *(uint4 *)(at + side) = lo;
     }
 
     // this warp's rows of a result, and its first sixteen columns of each 64
@@ -1039,20 +1013,18 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
     // sum's size is less while it is small
     const unsigned other = side / 16;
     const auto multiply = [&](uint32_t d, uint64_t left, unsigned dl, uint64_t right, unsigned dr, uint32_t shape, int count, bool add) {
-        if (PARTS == 2) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                if (q < count) {
-                    product<1>(d, left + q * dl, right + q * dr + other, shape, add || q > 0);
-                    product<1>(d, left + q * dl + other, right + q * dr, shape, true);
-                }
-        }
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-            if (q < count) product<1>(d, left + q * dl, right + q * dr, shape, PARTS == 2 || add || q > 0);
+            if (q < count) {
+                product<1>(d, left + q * dl, right + q * dr + other, shape, add || q > 0);
+                product<1>(d, left + q * dl + other, right + q * dr, shape, true);
+            }
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            if (q < count) product<1>(d, left + q * dl, right + q * dr, shape, true);
     };
     // sums of at most a few blocks each, added up in registers (see NsTile::group)
-    const int sums = PARTS == 2 ? max(1, min(512 / R, (nb + 1) / 2)) : 1;
+    const int sums = max(1, min(512 / R, (nb + 1) / 2));
 
     for (int s = 0; s < steps; ++s) {
         const bool last = s + 1 == steps;
@@ -1081,7 +1053,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
                 if (row_there && C == 1) {
 #pragma unroll
                     for (int k = 0; k < 16; ++k) v[k] *= kScaleA / (kScaleX * kScaleX);
-                    ns_put16<PARTS>(ab + (c >> 6) * L.block + r * 128, side, (c >> 3) & 7, r, v);
+                    ns_put16(ab + (c >> 6) * L.block + r * 128, side, (c >> 3) & 7, r, v);
                 } else if (row_there) {
                     // four columns of all rows after one another; few rows, to everybody
 #pragma unroll
@@ -1111,11 +1083,11 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
                 const float f = kScaleA / (kScaleX * kScaleX);
                 const int row = tid % R, c = tid / R * 4;
                 uint2 hi, lo;
-                ns_split<PARTS>(total.x * f, total.y * f, hi.x, lo.x);
-                ns_split<PARTS>(total.z * f, total.w * f, hi.y, lo.y);
+                ns_split(total.x * f, total.y * f, hi.x, lo.x);
+                ns_split(total.z * f, total.w * f, hi.y, lo.y);
                 unsigned char *to = ab + row * 128 + ((((c >> 3) ^ row) & 7) * 16) + (c & 4) * 2;
                 *(uint2 *)to = hi;
-                if (PARTS == 2) *(uint2 *)(to + side) = lo;
+                *(uint2 *)(to + side) = lo;
             }
         } else if (C > 1) {
             __syncwarp();
@@ -1149,12 +1121,12 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
                 if (e < e1) {
                     const float f = kScaleA / (kScaleX * kScaleX);
                     uint32_t h0, h1, l0, l1;
-                    ns_split<PARTS>(total[k].x * f, total[k].y * f, h0, l0);
-                    ns_split<PARTS>(total[k].z * f, total[k].w * f, h1, l1);
+                    ns_split(total[k].x * f, total[k].y * f, h0, l0);
+                    ns_split(total[k].z * f, total[k].w * f, h1, l1);
                     unsigned char *to = ab + (c >> 6) * L.block + row * 128 + ((((c >> 3) ^ row) & 7) * 16) + (c & 4) * 2;
                     for (int o = 0; o < C; ++o) {
                         write_at(to, o, h0, h1);
-                        if (PARTS == 2) write_at(to + side, o, l0, l1);
+                        write_at(to + side, o, l0, l1);
                     }
                 }
             }
@@ -1178,8 +1150,8 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
                 tensor_read(v, at + c);
                 if (row_there) {
                     unsigned char *row = ab + (c >> 6) * L.block + r * 128;
-                    ns_add16<PARTS>(row, side, (c >> 3) & 7, r, A.cb, A.cc / kScaleA, v);
-                    ns_put16<PARTS>(row, side, (c >> 3) & 7, r, v);
+                    ns_add16(row, side, (c >> 3) & 7, r, A.cb, A.cc / kScaleA, v);
+                    ns_put16(row, side, (c >> 3) & 7, r, v);
                 }
             }
         // up to 512 columns of x at a time
@@ -1219,27 +1191,25 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
                     unsigned char *chunk = x + (n0 + (ch >> 3)) * L.block + row * 128 + ((ch ^ row) & 7) * 16;
                     const uint4 hi = *(const uint4 *)chunk;
                     uint4 lo = make_uint4(0, 0, 0, 0);
-                    if (PARTS == 2) lo = *(const uint4 *)(chunk + side);
+                    lo = *(const uint4 *)(chunk + side);
                     const uint32_t hs[4] = {hi.x, hi.y, hi.z, hi.w}, ls[4] = {lo.x, lo.y, lo.z, lo.w};
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         float2 o = __half22float2(*reinterpret_cast<const __half2 *>(&hs[e]));
-                        if (PARTS == 2) {
-                            const float2 l = __half22float2(*reinterpret_cast<const __half2 *>(&ls[e]));
-                            o.x += l.x;
-                            o.y += l.y;
-                        }
+                        const float2 l = __half22float2(*reinterpret_cast<const __half2 *>(&ls[e]));
+                        o.x += l.x;
+                        o.y += l.y;
                         v[2 * e] = fmaf(A.ca, o.x, (1.0f / kScaleA) * v[2 * e]);
                         v[2 * e + 1] = fmaf(A.ca, o.y, (1.0f / kScaleA) * v[2 * e + 1]);
                     }
                     if (!last) {
                         uint4 nh, nl;
-                        ns_split<PARTS>(v[0], v[1], nh.x, nl.x);
-                        ns_split<PARTS>(v[2], v[3], nh.y, nl.y);
-                        ns_split<PARTS>(v[4], v[5], nh.z, nl.z);
-                        ns_split<PARTS>(v[6], v[7], nh.w, nl.w);
+                        ns_split(v[0], v[1], nh.x, nl.x);
+                        ns_split(v[2], v[3], nh.y, nl.y);
+                        ns_split(v[4], v[5], nh.z, nl.z);
+                        ns_split(v[6], v[7], nh.w, nl.w);
                         *(uint4 *)chunk = nh;
-                        if (PARTS == 2) *(uint4 *)(chunk + side) = nl;
+                        *(uint4 *)(chunk + side) = nl;
                     } else {
                         T *dst = (T *)J.dst;
                         const int c0 = (b0 + n0) * 64 + ch * 8;
@@ -1261,9 +1231,9 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
                     tensor_read(v, at + c);
                     const int column = n0 * 64 + c;
                     unsigned char *row = x + (column >> 6) * L.block + r * 128;
-                    if (row_there) ns_add16<PARTS>(row, side, (c >> 3) & 7, r, A.ca, 1.0f / kScaleA, v);
+                    if (row_there) ns_add16(row, side, (c >> 3) & 7, r, A.ca, 1.0f / kScaleA, v);
                     if (!last) {
-                        if (row_there) ns_put16<PARTS>(row, side, (c >> 3) & 7, r, v);
+                        if (row_there) ns_put16(row, side, (c >> 3) & 7, r, v);
                         continue;
                     }
                     // to the weight: of a tall matrix what the lanes hold of a column, else sixteen elements of two rows at a time
@@ -1307,18 +1277,18 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
     }
 }
 
-static size_t ns_job_bytes(int64_t m, int64_t n, int dtype)
+static size_t ns_job_bytes(int64_t m, int64_t n)
 {
-    const int64_t parts = dtype == SLAYER_B200_BF16 ? 1 : 2, rb = ns_rb((int)m), cbn = ns_cb((int)n);
-    return kNormParts * 8 + 256 + (size_t)(2 * rb * cbn + 4 * rb * rb) * (size_t)(parts * kBlock);
+    const int64_t rb = ns_rb((int)m), cbn = ns_cb((int)n);
+    return kNormParts * 8 + 256 + (size_t)(2 * rb * cbn + 4 * rb * rb) * (size_t)(kParts * kBlock);
 }
 
 // how many matrices of this many bytes a launch takes
 static int ns_at_once(int64_t bytes) { return bytes * kMaxJobs <= kMostBytes ? kMaxJobs : bytes <= kMostBytes ? (int)(kMostBytes / bytes) : 1; }
 
-static void ns_take(NsJob &J, int parts, unsigned char *&at)
+static void ns_take(NsJob &J, unsigned char *&at)
 {
-    const int64_t rb = ns_rb(J.m), x = rb * ns_cb(J.n) * parts * kBlock, a = 2 * rb * rb * parts * kBlock;
+    const int64_t rb = ns_rb(J.m), x = rb * ns_cb(J.n) * kParts * kBlock, a = 2 * rb * rb * kParts * kBlock;
     J.parts = (double *)at;
     at += kNormParts * 8 + 256;                  // and a count
     J.x[0] = at;
@@ -1328,10 +1298,10 @@ static void ns_take(NsJob &J, int parts, unsigned char *&at)
     at = J.b + a;
 }
 
-template <typename T, int PARTS, int MODE>
+template <typename T, int MODE>
 static int ns_run(NsArgs &A, int steps, cudaStream_t st)
 {
-    constexpr int CG = NsTile<PARTS, MODE>::CG;
+    constexpr int CG = NsTile<MODE>::CG;
     NsPlan P = {};
     P.steps = steps;
     P.status = device_status_word();
@@ -1357,14 +1327,13 @@ static int ns_run(NsArgs &A, int steps, cudaStream_t st)
     }
     P.tiles[kPolynomial] = P.tiles[kGram];
 
-    auto kern = ns_steps_kernel<PARTS, MODE, T>;
-    constexpr size_t smem = NsTile<PARTS, MODE>::kSmem;
+    auto kern = ns_steps_kernel<MODE, T>;
+    constexpr size_t smem = NsTile<MODE>::kSmem;
     int rc = reserve_dynamic_smem((const void *)kern, smem);
     if (rc) return rc;
-    // CTAs that share a tile where there are too few tiles for the SMs, each with two steps of 64 at least, of one part (a third of the
-    // products) four.  Five steps with two / four / eight, us: float32 512 x 512 130 / 149 / 173, 2000 x 333 153 / 162 / 173; bfloat16 300 x 300
-    // 109 / 99 / 99, 512 x 512 109 / 114 / 108, 768 x 768 122 / 128 / 129, 2000 x 333 126 / 114 / 118.
-    const int least = PARTS == 2 ? 4 : 8;
+    // CTAs that share a tile where there are too few tiles for the SMs, each with two steps of 64 at least.  Five steps with two / four /
+    // eight, us: float32 512 x 512 130 / 149 / 173, 2000 x 333 153 / 162 / 173.
+    const int least = 4;
     const int index[3] = {ns_cb(n), ns_cb(m), ns_cb(m)};
     int ranks = CG, resident = 0;
     for (int most = MODE == kShared ? 8 : 1;; most = ranks) {
@@ -1375,7 +1344,7 @@ static int ns_run(NsArgs &A, int steps, cudaStream_t st)
             while (P.split[k] < most && P.tiles[k] * P.split[k] * 2 <= sms && index[k] >= P.split[k] * least) P.split[k] *= 2;
             if (CG == 1) ranks = P.split[k] > ranks ? P.split[k] : ranks;
         }
-        const int held = resident_clusters((const void *)kern, ranks, NsTile<PARTS, MODE>::kThreads, smem) * ranks;
+        const int held = resident_clusters((const void *)kern, ranks, NsTile<MODE>::kThreads, smem) * ranks;
         if (held <= 0) {
             set_error("Newton-Schulz products: the device holds no cluster of %d CTAs", ranks);
             return SLAYER_B200_EUNSUPPORTED;
@@ -1393,12 +1362,12 @@ static int ns_run(NsArgs &A, int steps, cudaStream_t st)
     grid = (int)ceil_div(grid, ranks) * ranks;
 
     ns_momentum_kernel<T><<<blocks, 256, 0, st>>>(A, P.arrived);
-    ns_normalise_kernel<T, PARTS><<<blocks, 256, 0, st>>>(A);
+    ns_normalise_kernel<T><<<blocks, 256, 0, st>>>(A);
     rc = check_launch("Newton-Schulz normalisation launch");
     if (rc) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(NsTile<PARTS, MODE>::kThreads);
+    cfg.blockDim = dim3(NsTile<MODE>::kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
@@ -1458,14 +1427,14 @@ static bool ns_placed(const void *p, int dtype) { return ((uintptr_t)p & (dtype 
 // CTAs for each of the small matrices of a launch: up to four column blocks each, more where there are many matrices; 0: a matrix
 // does not fit.  Five steps with up to one / two / four / eight blocks, float32, us: 64 x 288 55 / 57 / 59 / 62, 64 x 576 62 / 62 / 65 / 78,
 // 100 x 300 94 / 88 / 88 / 85, 20 x 128 x 256 90 / 83 / 69 / 69.
-static int ns_small_cluster(const NsArgs &A, int parts)
+static int ns_small_cluster(const NsArgs &A)
 {
     int C = 1;
     for (; C <= 8; C *= 2) {
         bool fits = true, roomy = true;
         for (int j = 0; j < A.jobs && fits; ++j) {
             const int per = ((A.job[j].n + 63) / 64 + C - 1) / C;
-            fits = A.job[j].m <= 128 && ns_small(A.job[j].m, per, parts).fits;
+            fits = A.job[j].m <= 128 && ns_small(A.job[j].m, per).fits;
             roomy = roomy && per <= 4;
         }
         if (fits && (roomy || C == 8 || A.jobs * C * 2 > sm_count())) return C;
@@ -1473,7 +1442,7 @@ static int ns_small_cluster(const NsArgs &A, int parts)
     return 0;
 }
 
-template <typename T, int PARTS>
+template <typename T>
 static int ns_run_small(const NsArgs &A, int C, int steps, cudaStream_t st)
 {
     int *status = device_status_word();
@@ -1484,10 +1453,10 @@ static int ns_run_small(const NsArgs &A, int C, int steps, cudaStream_t st)
     // one CTA per SM, since each takes all of its tensor memory
     size_t smem = 120 * 1024;
     for (int j = 0; j < A.jobs; ++j) {
-        const size_t want = 1024 + ns_small(A.job[j].m, ((A.job[j].n + 63) / 64 + C - 1) / C, PARTS).total;
+        const size_t want = 1024 + ns_small(A.job[j].m, ((A.job[j].n + 63) / 64 + C - 1) / C).total;
         smem = want > smem ? want : smem;
     }
-    auto kern = ns_small_kernel<T, PARTS>;
+    auto kern = ns_small_kernel<T>;
     int rc = reserve_dynamic_smem((const void *)kern, smem);
     if (rc) return rc;
     cudaLaunchConfig_t cfg = {};
@@ -1505,29 +1474,29 @@ static int ns_run_small(const NsArgs &A, int C, int steps, cudaStream_t st)
     return check_launch("Newton-Schulz launch for small matrices");
 }
 
-template <typename T, int PARTS>
+template <typename T>
 static int ns_tiled(NsArgs &A, int steps, cudaStream_t st)
 {
-    const int C = ns_small_cluster(A, PARTS);
-    if (C) return ns_run_small<T, PARTS>(A, C, steps, st);
+    const int C = ns_small_cluster(A);
+    if (C) return ns_run_small<T>(A, C, steps, st);
 
     // Tiles of two CTAs where there are enough of them; where there are few tiles, CTAs that share them.  Five steps, us, alone / shared /
     // in pairs: float32 512 x 512 170 / 130 / 266, 1024 x 1024 257 / 208 / 373, 1536 x 1536 362 / 368 / 483, 2048 x 2048 586 / 591 / 618,
-    // 2304 x 2304 1079 / 1075 / 870; bfloat16 1024 x 2048 188 / 173 / 231, 2048 x 2048 325 / 326 / 315, 2304 x 2304 545 / 549 / 430
+    // 2304 x 2304 1079 / 1075 / 870
     int64_t tiles = 0;
     for (int j = 0; j < A.jobs; ++j) tiles += (int64_t)((ns_rb(A.job[j].m) + 1) / 2) * ((ns_rb(A.job[j].n) + 1) / 2);
-    if (tiles >= sm_count() / 2) return ns_run<T, PARTS, kPair>(A, steps, st);
+    if (tiles >= sm_count() / 2) return ns_run<T, kPair>(A, steps, st);
     int small = 0;
     for (int j = 0; j < A.jobs; ++j) small += ns_rb(A.job[j].m) * (ns_rb(A.job[j].m) + 1) / 2;
-    return small * 4 <= sm_count() ? ns_run<T, PARTS, kShared>(A, steps, st) : ns_run<T, PARTS, kAlone>(A, steps, st);
+    return small * 4 <= sm_count() ? ns_run<T, kShared>(A, steps, st) : ns_run<T, kAlone>(A, steps, st);
 }
 
 static int ns_dispatch(NsArgs &A, int dtype, int steps, cudaStream_t st)
 {
     switch (dtype) {
-    case SLAYER_B200_F32: return ns_tiled<float, 2>(A, steps, st);
-    case SLAYER_B200_BF16: return ns_tiled<__nv_bfloat16, 1>(A, steps, st);
-    default: return ns_tiled<__half, 2>(A, steps, st);
+    case SLAYER_B200_F32: return ns_tiled<float>(A, steps, st);
+    case SLAYER_B200_BF16: return ns_tiled<__nv_bfloat16>(A, steps, st);
+    default: return ns_tiled<__half>(A, steps, st);
     }
 }
 
@@ -1540,7 +1509,7 @@ extern "C" int64_t slayer_b200_orthogonalize_workspace(int64_t batch, int64_t ro
     if (batch <= 0 || rows <= 0 || cols <= 0) return 0;
     clear_error();
     if (const int rc = ns_shape("orthogonalize", rows, cols)) return rc;
-    const int64_t each = (int64_t)ns_job_bytes(rows < cols ? rows : cols, rows < cols ? cols : rows, dtype), most = ns_at_once(each);
+    const int64_t each = (int64_t)ns_job_bytes(rows < cols ? rows : cols, rows < cols ? cols : rows), most = ns_at_once(each);
     return each * (batch < most ? batch : most);
 }
 
@@ -1558,7 +1527,7 @@ extern "C" int slayer_b200_orthogonalize(void *out, const void *in, int dtype, i
     SB200_REQUIRE(((uintptr_t)workspace & 255) == 0, "orthogonalize: the workspace must be aligned to 256 bytes");
     SB200_REQUIRE(ns_placed(out, dtype) && ns_placed(in, dtype), "orthogonalize: out and in must be aligned to their elements");
     const size_t bytes = (size_t)rows * cols * (dtype == SLAYER_B200_F32 ? 4 : 2);
-    const int most = ns_at_once((int64_t)ns_job_bytes(rows < cols ? rows : cols, rows < cols ? cols : rows, dtype));
+    const int most = ns_at_once((int64_t)ns_job_bytes(rows < cols ? rows : cols, rows < cols ? cols : rows));
     for (int64_t first = 0; first < batch; first += most) {
         NsArgs A = {};
         A.jobs = (int)(batch - first < most ? batch - first : most);
@@ -1575,7 +1544,7 @@ extern "C" int slayer_b200_orthogonalize(void *out, const void *in, int dtype, i
             J.cols = (int)cols;
             J.m = (int)(rows < cols ? rows : cols);
             J.n = (int)(rows < cols ? cols : rows);
-            ns_take(J, dtype == SLAYER_B200_BF16 ? 1 : 2, at);
+            ns_take(J, at);
         }
         rc = ns_dispatch(A, dtype, steps, (cudaStream_t)stream);
         if (rc) return rc;
@@ -1592,7 +1561,7 @@ extern "C" int64_t slayer_b200_muon_step_workspace(const slayer_b200_muon_matrix
         const int64_t rows = list[i].rows, cols = list[i].cols;
         if (rows <= 0 || cols <= 0) continue;
         if (const int rc = ns_shape("muon_step", rows, cols)) return rc;
-        const int64_t bytes = (int64_t)ns_job_bytes(rows < cols ? rows : cols, rows < cols ? cols : rows, dtype);
+        const int64_t bytes = (int64_t)ns_job_bytes(rows < cols ? rows : cols, rows < cols ? cols : rows);
         if (in == kMaxJobs || (in > 0 && now + bytes > kMostBytes)) in = 0, now = 0;       // as slayer_b200_muon_step does
         ++in;
         now += bytes;
@@ -1634,7 +1603,7 @@ extern "C" int slayer_b200_muon_step(const slayer_b200_muon_matrix *list, int64_
             const slayer_b200_muon_matrix &M = list[i];
             if (M.rows == 0 || M.cols == 0) continue;
             const int64_t m = M.rows < M.cols ? M.rows : M.cols, n = M.rows < M.cols ? M.cols : M.rows;
-            if (A.jobs > 0 && (at - (unsigned char *)workspace) + (int64_t)ns_job_bytes(m, n, dtype) > kMostBytes) break;
+            if (A.jobs > 0 && (at - (unsigned char *)workspace) + (int64_t)ns_job_bytes(m, n) > kMostBytes) break;
             NsJob &J = A.job[A.jobs++];
             J.src = M.grad;
             J.mom = M.momentum;
@@ -1648,7 +1617,7 @@ extern "C" int slayer_b200_muon_step(const slayer_b200_muon_matrix *list, int64_
                                 : adjust == SLAYER_B200_MUON_RMS   ? 0.2 * sqrt((double)J.n) : 1.0;
             J.keep = (float)(1.0 - (double)lr * (double)weight_decay);
             J.step = (float)((double)lr * factor);
-            ns_take(J, dtype == SLAYER_B200_BF16 ? 1 : 2, at);
+            ns_take(J, at);
         }
         if (A.jobs == 0) break;
         rc = ns_dispatch(A, dtype, steps, (cudaStream_t)stream);

@@ -25,8 +25,8 @@ def orthogonalize(matrix, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
     ``a X + (b A + c A A) X`` with ``A = X X^T`` (of a matrix with more rows than columns, its transpose's).
 
     With the default coefficients all singular values end between 0.68 and 1.13, those below 1/500 of the norm excepted.
-    float32 and float16 matrices are worked on with products of 22 bits, bfloat16 ones with 11 (fewer where the norm is below a
-    thousandth of ``eps`` and the result near zero: entries after the division are held to 2**-37).  No gradient flows through it.
+    Matrices of all types are worked on with products of 22 bits (fewer where the norm is below a thousandth of ``eps`` and the result
+    near zero: entries after the division are held to 2**-37).  No gradient flows through it.
     A matrix has at most 32768 rows or columns on its shorter side, 2**22 on the longer, and 2**31 elements."""
     if matrix.dim() < 2:
         raise ValueError("orthogonalize: a matrix has at least two dimensions, got %s" % (tuple(matrix.shape),))
