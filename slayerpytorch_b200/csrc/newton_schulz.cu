@@ -11,8 +11,8 @@
 //     v = hi + lo, two fp16 values, 22 bits and a sign;  v w ~ hi hi + hi lo + lo hi, the left out lo lo being 2^-24 of it.
 // Three products instead of one, for bfloat16 matrices too: with hi alone, 11 bits, their results ended 1.2 to 2.2 times as far off as
 // their own rounding to 8 bits (6 x 1023 x 2049 in 387 us instead of 715).
-// Sums are fp32: those of 64 to 192 products in tensor memory, of up to 128 in matrices that stay on the chip, longer ones in registers
-// (see NsTile::group).  Five steps end 0.2 to 0.7 times as far off as with fp32 products, on the chip 0.8 to 2.9 times.
+// Sums are fp32: those of 64 to 192 products in tensor memory, longer ones in registers (see NsTile::group).  Five steps end 0.2 to 0.7
+// times as far off as with fp32 products; matrices that stay on the chip, whose fp32 sums are short, 0.6 to 1.9 times.
 // Entries of X are held to 2^-37 at best (an fp16's smallest step over the scale): enough where the norm is not far below eps.
 //
 // X, A and B = b A + c A A live in the workspace as blocks of 128 x 64 elements, padded with zeros, each block laid out as the
@@ -1023,7 +1023,8 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
         for (int q = 0; q < 4; ++q)
             if (q < count) product<1>(d, left + q * dl, right + q * dr, shape, true);
     };
-    // sums of at most a few blocks each, added up in registers (see NsTile::group)
+    // sums of a few blocks each, added up in registers (see NsTile::group); those of A A and B X have 64 products each too, where tensor
+    // memory has room (with sums of 128: 128 x 1024 119.5 us instead of 121.2, and 3.9e-6 off instead of 2.4e-6)
     const int sums = max(1, min(512 / R, (nb + 1) / 2));
 
     for (int s = 0; s < steps; ++s) {
@@ -1138,7 +1139,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
         if (tid == 0) {
             for (int k = 0; k < R; k += 64) {
                 const uint64_t rows = desc_rows(abs + (k >> 6) * L.block);
-                multiply(acc, rows, 2, rows, 2, product_shape(128, R, false, false), (R - k) / 16, k > 0);
+                multiply(acc + (k >> 6) * R, rows, 2, rows, 2, product_shape(128, R, false, false), (R - k) / 16, false);
             }
             product_commit<1>(&bar);
         }
@@ -1148,6 +1149,12 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
                 float v[16];
                 __syncwarp();
                 tensor_read(v, at + c);
+                if (R > 64) {
+                    float t[16];
+                    tensor_read(t, at + R + c);
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) v[k] += t[k];
+                }
                 if (row_there) {
                     unsigned char *row = ab + (c >> 6) * L.block + r * 128;
                     ns_add16(row, side, (c >> 3) & 7, r, A.cb, A.cc / kScaleA, v);
@@ -1157,12 +1164,13 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
         // up to 512 columns of x at a time
         for (int n0 = 0; n0 < nb; n0 += 8) {
             const int n1 = min(n0 + 8, nb);
+            const bool two = R > 64 && n1 - n0 <= 4;       // as many sums as tensor memory has room for
             ready();
             if (tid == 0) {
                 for (int b = n0; b < n1; b += 4)
                     for (int k = 0; k < R; k += 64)
-                        multiply(acc + (b - n0) * 64, desc_rows(abs + (k >> 6) * L.block), 2, desc_columns(xs + b * L.block + k * 128, L.block), 128,
-                                 product_shape(128, min(4, n1 - b) * 64, false, true), (R - k) / 16, k > 0);
+                        multiply(acc + (b - n0) * 64 + (two ? (k >> 6) * 256 : 0), desc_rows(abs + (k >> 6) * L.block), 2, desc_columns(xs + b * L.block + k * 128, L.block), 128,
+                                 product_shape(128, min(4, n1 - b) * 64, false, true), (R - k) / 16, !two && k > 0);
                 product_commit<1>(&bar);
             }
             made();
@@ -1229,6 +1237,12 @@ __global__ void __launch_bounds__(kSmallThreads, 1) ns_small_kernel(const __grid
                     float v[16];
                     __syncwarp();
                     tensor_read(v, at + c);
+                    if (two) {
+                        float t[16];
+                        tensor_read(t, at + 256 + c);
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) v[k] += t[k];
+                    }
                     const int column = n0 * 64 + c;
                     unsigned char *row = x + (column >> 6) * L.block + r * 128;
                     if (row_there) ns_add16(row, side, (c >> 3) & 7, r, A.ca, 1.0f / kScaleA, v);
