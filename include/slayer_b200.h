@@ -377,6 +377,77 @@ int slayer_b200_muon_step(const slayer_b200_muon_matrix *list, int64_t count, in
                           float weight_decay, int adjust, int steps, float a, float b, float c, float eps, void *workspace, void *stream);
 int64_t slayer_b200_muon_step_workspace(const slayer_b200_muon_matrix *list, int64_t count, int dtype);
 
+/* Flags of the gated leaky integrator. */
+#define SLAYER_B200_LEAK_LOGIT   1   /* f = sigmoid(gate); without it f = gate              */
+#define SLAYER_B200_LEAK_COUPLED 2   /* the input is (1 - f) x; without it x                */
+
+/*
+ * A gated leaky integrator along each row of x [rows, T] (type `dtype`, as y):
+ *   y_t = f_t y_{t-1} + x_t   or   f_t y_{t-1} + (1 - f_t) x_t
+ * from initial[row] (NULL: 0) on.  gate_period 0: gate is [rows, T] of x's type; else it is float32, and
+ * row r has the entry (r / gate_inner) % gate_period at every step (rows: whole groups of gate_inner *
+ * gate_period).  lengths (NULL: all T): steps that count, one entry for every sample_rows rows, taken
+ * into [0, T]; the steps behind them are not used, y is 0 there and the state stays.  state (NULL: not
+ * wanted): the state after the last step.  starts (NULL: no backward pass): rows x
+ * slayer_b200_leak_chunks(T, dtype) float32, states that the backward pass starts from.  States are
+ * float32 outside of a call and double within.  y may not be x or gate.  workspace:
+ * slayer_b200_leak_workspace(...) bytes of device memory, aligned to 16, for either pass.  It has
+ * no counterpart in the reference, whose psp has one fixed kernel (src/slayer.py:875-899).
+ */
+int slayer_b200_leak_forward(void *y, float *state, float *starts, const void *x, const void *gate, const float *initial, int dtype, int flags,
+                             int64_t rows, int64_t T, const int64_t *lengths, int64_t sample_rows, int64_t gate_inner, int64_t gate_period,
+                             void *workspace, void *stream);
+int64_t slayer_b200_leak_chunks(int64_t T, int dtype);
+int64_t slayer_b200_leak_workspace(int64_t rows, int64_t T, int dtype, int64_t gate_inner, int64_t gate_period);
+
+/*
+ * The gradients of the above for g [rows, T] (of y) and gstate [rows] (of the last state; NULL: 0): dx as x,
+ * dgate as gate (of a gate per row: summed over its rows in a fixed order), dinitial [rows].  Each of the
+ * three may be NULL.  starts: from the forward pass on the same x, gate, initial and lengths.  It has
+ * no counterpart in the reference.
+ */
+int slayer_b200_leak_backward(void *dx, void *dgate, float *dinitial, const void *g, const float *gstate, const float *starts, const void *x,
+                              const void *gate, int dtype, int flags, int64_t rows, int64_t T, const int64_t *lengths, int64_t sample_rows,
+                              int64_t gate_inner, int64_t gate_period, void *workspace, void *stream);
+
+/*
+ * One time step of it on rows of a stream: state [rows], float32, is updated in place and y [rows] is the new state
+ * in x's type.  gate: [rows] (gate_period 0), or an entry for each group of rows as above; float32 or x's type
+ * (gate_dtype).  y may be x.  It has no counterpart in the reference.
+ */
+int slayer_b200_leak_step(void *y, float *state, const void *x, const void *gate, int dtype, int gate_dtype, int flags, int64_t rows,
+                          int64_t gate_inner, int64_t gate_period, void *stream);
+
+/*
+ * A tensor x [rows, T] (type `dtype`) kept in 8 bits: of each 32 consecutive steps of a row, q = x / 2^e rounded to the
+ * nearest whole number (ties to even), with the smallest e in [-126, 121] such that |x| <= 127 2^e for all of
+ * them that are finite.  q: [rows, 32 ceil(T / 32)], zeros behind the last step, aligned to 16 bytes; what is not
+ * finite is -128.  scale: [rows, ceil(T / 32)], e + 127.  It has no counterpart in the reference.
+ */
+int slayer_b200_compress8(int8_t *q, uint8_t *scale, const void *x, int dtype, int64_t rows, int64_t T, void *stream);
+
+/* What that stands for: out [rows, T] = q 2^e, NaN where q is -128.  It has no counterpart in the reference. */
+int slayer_b200_restore8(void *out, const int8_t *q, const uint8_t *scale, int dtype, int64_t rows, int64_t T, void *stream);
+
+/*
+ * slayer_b200_spike_grad on a membrane potential kept so: out [rows, T] =
+ *   g * (scale / tau * exp(-|q 2^e - theta| / tau));   out may be g.
+ * Surrogate gradient as src/slayer.py:858-865.
+ */
+int slayer_b200_spike_grad8(float *out, const float *g, const int8_t *q, const uint8_t *scale_bytes, int64_t rows, int64_t T, float theta,
+                            float tau, float scale, void *stream);
+
+/*
+ * Weight gradient of a dense layer whose input x [N, I, T] is kept so, for the gradient g [N, O, T] of its output:
+ *   out[o, i] = sum over n and t of g[n, o, t] x[n, i, t],
+ * in float32 precision, the same bits in every call.  workspace: slayer_b200_weight_grad8_workspace(...) bytes of device
+ * memory, aligned to 16.  It has no counterpart in the reference, whose weights are PyTorch's
+ * (src/slayer.py:393-437).
+ */
+int slayer_b200_weight_grad8(float *out, const float *g, const int8_t *q, const uint8_t *scale, int64_t N, int64_t O, int64_t I, int64_t T,
+                             void *workspace, void *stream);
+int64_t slayer_b200_weight_grad8_workspace(int64_t N, int64_t O, int64_t I, int64_t T);
+
 /*
  * slayer_b200_srm_get_spikes without any memory allocation, for callers that cannot allocate
  * device memory: an application that has already given all device memory to its own pool, or

@@ -42,11 +42,13 @@ CUDA_SOURCES = {
     "loss.cu": ["-ftz=true"],
     "policy.cu": ["-ftz=true"],      # exponentials below 1.2e-38 are nothing beside a row's sum of at least 1
     "newton_schulz.cu": [],
+    "leak.cu": [],
+    "checkpoint.cu": [],
     "tma.cu": [],
 }
 HEADERS = ["common.cuh", "tile.cuh", "tma.cuh", "tensor.cuh", "fir_sparse.cuh", os.path.join(INCLUDE, "slayer_b200.h")]
 
-MODULES = {"slayerCuda": ["bindings_slayer.cpp", "bindings_learning.cpp"], "slayerLoihiCuda": ["bindings_loihi.cpp"]}
+MODULES = {"slayerCuda": ["bindings_slayer.cpp", "bindings_learning.cpp", "bindings_sequence.cpp"], "slayerLoihiCuda": ["bindings_loihi.cpp"]}
 
 
 def _newer(target, deps):

@@ -49,6 +49,16 @@ SYMBOLS = {
     "slayer_b200_orthogonalize_workspace": (_i64, [_i64, _i64, _i64, _int]),
     "slayer_b200_muon_step": (_int, [_p, _i64, _int, _f, _f, _int, _f, _int, _int, _f, _f, _f, _f, _p, _p]),
     "slayer_b200_muon_step_workspace": (_i64, [_p, _i64, _int]),
+    "slayer_b200_leak_forward": (_int, [_p, _p, _p, _p, _p, _p, _int, _int, _i64, _i64, _p, _i64, _i64, _i64, _p, _p]),
+    "slayer_b200_leak_chunks": (_i64, [_i64, _int]),
+    "slayer_b200_leak_workspace": (_i64, [_i64, _i64, _int, _i64, _i64]),
+    "slayer_b200_leak_backward": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _int, _int, _i64, _i64, _p, _i64, _i64, _i64, _p, _p]),
+    "slayer_b200_leak_step": (_int, [_p, _p, _p, _p, _int, _int, _int, _i64, _i64, _i64, _p]),
+    "slayer_b200_compress8": (_int, [_p, _p, _p, _int, _i64, _i64, _p]),
+    "slayer_b200_restore8": (_int, [_p, _p, _p, _int, _i64, _i64, _p]),
+    "slayer_b200_spike_grad8": (_int, [_p, _p, _p, _p, _i64, _i64, _f, _f, _f, _p]),
+    "slayer_b200_weight_grad8": (_int, [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _p, _p]),
+    "slayer_b200_weight_grad8_workspace": (_i64, [_i64, _i64, _i64, _i64]),
     "slayer_b200_loihi_get_spikes": (_int, [_p, _p, _p, _p, _i64, _i64, _u32, _u32, _u32, _u32, _u32, _p]),
     "slayer_b200_loihi_spikes_only": (_int, [_p, _p, _i64, _i64, _u32, _u32, _u32, _u32, _u32, _i64, _p]),
     "slayer_b200_loihi_get_spikes_delayed": (_int, [_p, _p, _p, _p, _i64, _i64, _u32, _u32, _u32, _u32, _u32, _i64, _p]),

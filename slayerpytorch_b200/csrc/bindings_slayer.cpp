@@ -432,6 +432,7 @@ static torch::Tensor binEventsPackedCuda(std::vector<int64_t> shape, torch::Tens
 }
 
 void bind_learning(pybind11::module_ &m);        // bindings_learning.cpp
+void bind_sequence(pybind11::module_ &m);        // bindings_sequence.cpp
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
 {
@@ -457,5 +458,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
     m.def("binEvents", &binEventsCuda, "Address events -> spike tensor (CUDA)");
     m.def("binEventsPacked", &binEventsPackedCuda, "Address events -> bit-packed spike tensor (CUDA)");
     bind_learning(m);
+    bind_sequence(m);
     m.attr("backend") = "slayer_b200";
 }

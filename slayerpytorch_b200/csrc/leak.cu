@@ -1,0 +1,585 @@
+// Gated leaky integrator, along the time steps of each row:
+//   y_t = f_t y_{t-1} + u_t,   f = sigmoid(gate) or the gate itself,   u = x, or (1 - f) x ("coupled").
+// A step is the map h -> A h + B with A = f_t, B = u_t; maps compose to maps, so a row is a scan over them: a lane composes its 16 bytes
+// of steps, the lanes of a row's group scan their maps with shuffles, and each walks its steps from the state that the lanes before
+// it leave.  The backward pass is the same from the other end: c_t = f_t (g_t + c_{t+1}) is what step t hands to step t - 1, and
+//   lambda_t = g_t + c_{t+1},   dx = lambda (or (1 - f) lambda),   df = lambda (y_{t-1} - (coupled) x).
+// It forms y again from x and the gate, out of the states that the forward pass keeps at the start of each chunk (4 bytes for 512), so that
+// it reads x, gate and g and writes dx and dgate: no y is kept, and none that is rounded to 16 bits is used.
+//
+// States and maps are double: a slow leak's f is next to one, where its rounding to 32 bits, taken at each of the thousands of steps that such
+// a state remembers, adds up to 1e-5 of it; 1 - f is known to 32 bits from the gate, and double's f keeps them.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace sb200 {
+
+template <typename E> __device__ __forceinline__ float to_float(E v);
+template <> __device__ __forceinline__ float to_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <> __device__ __forceinline__ float to_float<__half>(__half v) { return __half2float(v); }
+template <typename E> __device__ __forceinline__ E from_float(float v);
+template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+
+// Steps of a row that a lane holds: 16 bytes of them.  They start at multiples of 16 bytes of the tensor, not of the row, so a row's first
+// lane may begin with steps of the row before, and all lanes' steps are loaded at once whatever T is.
+template <typename E> constexpr int kSteps = 16 / (int)sizeof(E);
+
+struct LeakShape {
+    int64_t rows, T;
+    int64_t gate_inner, gate_period;     // gate per row: entry (row / inner) % period; period 0: a gate per step
+    int64_t sample_rows;                 // rows with one length
+    const int64_t *lengths;              // null: all T
+    int64_t chunks;                      // of a row
+    int64_t segments, segment_chunks;    // a row's chunks are worked on by `segments` groups of lanes
+    bool logit, coupled;
+};
+
+// steps that lie outside of the row, or behind its length, keep the state: f = 1, u = 0
+struct Row {
+    int64_t base, length;      // first element; steps that count
+    int skew;                  // elements between the 16-byte boundary and the first element
+};
+
+template <typename E>
+__device__ __forceinline__ Row row_of(const LeakShape &s, int64_t row)
+{
+    Row r;
+    r.base = row * s.T;
+    r.skew = (int)(r.base % kSteps<E>);
+    r.length = s.T;
+    if (s.lengths) {
+        const int64_t n = s.lengths[row / s.sample_rows];
+        r.length = n < 0 ? 0 : (n < s.T ? n : s.T);
+    }
+    return r;
+}
+
+// elements [t, t + kSteps) of a row, those in [0, end) of them
+template <typename E, bool VEC>
+__device__ __forceinline__ void load_steps(float (&v)[kSteps<E>], const E *p, int64_t base, int64_t t, int64_t end, float rest)
+{
+    constexpr int N = kSteps<E>;
+    if (VEC && t >= 0 && t + N <= end) {
+        const uint4 raw = __ldg(reinterpret_cast<const uint4 *>(p + base + t));
+        const E *e = reinterpret_cast<const E *>(&raw);
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = to_float<E>(e[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = t + j >= 0 && t + j < end ? to_float<E>(p[base + t + j]) : rest;
+    }
+}
+
+template <typename E, bool VEC>
+__device__ __forceinline__ void store_steps(E *p, int64_t base, int64_t t, int64_t T, const float (&v)[kSteps<E>])
+{
+    constexpr int N = kSteps<E>;
+    if (VEC && t >= 0 && t + N <= T) {
+        uint4 raw;
+        E *e = reinterpret_cast<E *>(&raw);
+#pragma unroll
+        for (int j = 0; j < N; ++j) e[j] = from_float<E>(v[j]);
+        *reinterpret_cast<uint4 *>(p + base + t) = raw;
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (t + j >= 0 && t + j < T) p[base + t + j] = from_float<E>(v[j]);
+    }
+}
+
+// f and 1 - f, each to its own 32 bits
+__device__ __forceinline__ void decay_of(float gate, bool logit, double &f, float &rest)
+{
+    if (logit) {
+        const float e = expf(-fabsf(gate)), large = __fdividef(1.0f, 1.0f + e), small = e * large;
+        f = gate < 0.0f ? (double)small : 1.0 - (double)small;
+        rest = gate < 0.0f ? large : small;
+    } else {
+        f = (double)gate;
+        rest = (float)(1.0 - (double)gate);
+    }
+}
+
+// What a lane knows of its steps.
+template <typename E>
+struct Steps {
+    double f[kSteps<E>];
+    float rest[kSteps<E>], x[kSteps<E>];
+
+    template <bool VEC>
+    __device__ __forceinline__ void load(const LeakShape &s, const Row &row, const E *x_, const E *gate, double row_f, float row_rest, int64_t t)
+    {
+        load_steps<E, VEC>(x, x_, row.base, t, row.length, 0.0f);
+        if (s.gate_period == 0) {
+            float g[kSteps<E>];
+            load_steps<E, VEC>(g, gate, row.base, t, row.length, 0.0f);
+#pragma unroll
+            for (int j = 0; j < kSteps<E>; ++j) decay_of(g[j], s.logit, f[j], rest[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < kSteps<E>; ++j) f[j] = row_f, rest[j] = row_rest;
+        }
+#pragma unroll
+        for (int j = 0; j < kSteps<E>; ++j)
+            if (t + j < 0 || t + j >= row.length) f[j] = 1.0, rest[j] = 0.0f;
+    }
+    __device__ __forceinline__ double input(const LeakShape &s, int j) const { return (double)(s.coupled ? rest[j] * x[j] : x[j]); }
+};
+
+struct Map {
+    double a, b;
+    __device__ __forceinline__ double operator()(double h) const { return fma(a, h, b); }
+};
+
+// first, then second
+__device__ __forceinline__ Map compose(const Map &first, const Map &second) { return {first.a * second.a, second(first.b)}; }
+
+template <int G>
+__device__ __forceinline__ Map shift_up(const Map &m, int d) { return {__shfl_up_sync(~0u, m.a, d, G), __shfl_up_sync(~0u, m.b, d, G)}; }
+template <int G>
+__device__ __forceinline__ Map shift_down(const Map &m, int d) { return {__shfl_down_sync(~0u, m.a, d, G), __shfl_down_sync(~0u, m.b, d, G)}; }
+
+// the map of this lane and all before it (FORWARD), or all behind it
+template <int G, bool FORWARD>
+__device__ __forceinline__ Map scan(Map m, int lane)
+{
+#pragma unroll
+    for (int d = 1; d < G; d *= 2) {
+        const Map o = FORWARD ? shift_up<G>(m, d) : shift_down<G>(m, d);
+        if (FORWARD ? lane >= d : lane + d < G) m = compose(o, m);
+    }
+    return m;
+}
+
+// the map of the lanes before (behind) this one, from scan()
+template <int G, bool FORWARD>
+__device__ __forceinline__ Map others(const Map &m, int lane)
+{
+    const Map o = FORWARD ? shift_up<G>(m, 1) : shift_down<G>(m, 1);
+    return lane == (FORWARD ? 0 : G - 1) ? Map{1.0, 0.0} : o;
+}
+
+// Composition of the maps of segments [from, to) of a row, in the order of time (FORWARD) or against it; all lanes of a warp get it.
+template <bool FORWARD>
+__device__ __forceinline__ Map segments_map(const Map *maps, int64_t from, int64_t to, int lane)
+{
+    const int64_t n = to - from, each = (n + 31) / 32;
+    Map m = {1.0, 0.0};
+    for (int64_t i = 0; i < each; ++i) {
+        const int64_t k = lane * each + i;
+        if (k < n) m = compose(m, maps[FORWARD ? from + k : to - 1 - k]);
+    }
+    m = scan<32, true>(m, lane);
+    return {__shfl_sync(~0u, m.a, 31), __shfl_sync(~0u, m.b, 31)};
+}
+
+template <typename E>
+__device__ __forceinline__ Map forward_map(const LeakShape &s, const Steps<E> &st)
+{
+    Map m = {1.0, 0.0};
+#pragma unroll
+    for (int j = 0; j < kSteps<E>; ++j) m = compose(m, Map{st.f[j], st.input(s, j)});
+    return m;
+}
+
+template <typename E>
+__device__ __forceinline__ Map backward_map(const double (&f)[kSteps<E>], const float (&g)[kSteps<E>])
+{
+    Map m = {1.0, 0.0};
+#pragma unroll
+    for (int j = kSteps<E> - 1; j >= 0; --j) m = Map{m.a * f[j], f[j] * (m.b + (double)g[j])};
+    return m;
+}
+
+// Which row, segment and lane of its group a thread is; false: none.
+template <int G>
+__device__ __forceinline__ bool place(const LeakShape &s, int64_t &row, int64_t &segment, int &lane)
+{
+    const int64_t group = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / G;
+    lane = threadIdx.x % G;
+    row = group / s.segments;
+    segment = group % s.segments;
+    return row < s.rows;
+}
+
+template <typename E>
+__device__ __forceinline__ void row_gate(const LeakShape &s, const void *gate, int64_t row, double &f, float &rest)
+{
+    f = 1.0, rest = 0.0f;
+    if (s.gate_period) decay_of(((const float *)gate)[row / s.gate_inner % s.gate_period], s.logit, f, rest);
+}
+
+// Maps of segments: rows too few to fill the GPU are split, and each segment starts from the composition of those before it.
+template <typename E, bool VEC>
+__global__ void __launch_bounds__(256)
+leak_maps_kernel(Map *maps, const E *x, const void *gate, const E *g, const LeakShape s, bool forward)
+{
+    int64_t row, segment;
+    int lane;
+    if (!place<32>(s, row, segment, lane)) return;
+    const Row r = row_of<E>(s, row);
+    double row_f;
+    float row_rest;
+    row_gate<E>(s, gate, row, row_f, row_rest);
+    Map all = {1.0, 0.0};
+    const int64_t first = segment * s.segment_chunks, last = min(first + s.segment_chunks, s.chunks);
+    for (int64_t i = first; i < last; ++i) {
+        const int64_t c = forward ? i : last - 1 - (i - first);
+        const int64_t t = (c * 32 + lane) * kSteps<E> - r.skew;
+        Steps<E> st;
+        st.template load<VEC>(s, r, forward ? x : g, (const E *)gate, row_f, row_rest, t);
+        Map m;
+        if (forward) {
+            m = scan<32, true>(forward_map<E>(s, st), lane);
+            m = {__shfl_sync(~0u, m.a, 31), __shfl_sync(~0u, m.b, 31)};
+        } else {
+            m = scan<32, false>(backward_map<E>(st.f, st.x), lane);
+            m = {__shfl_sync(~0u, m.a, 0), __shfl_sync(~0u, m.b, 0)};
+        }
+        all = compose(all, m);
+    }
+    if (lane == 0) maps[row * s.segments + segment] = all;
+}
+
+template <typename E, int G, bool VEC>
+__global__ void __launch_bounds__(256)
+leak_forward_kernel(E *y, float *state, float *starts, const E *x, const void *gate, const float *initial, const Map *maps, const LeakShape s)
+{
+    int64_t row, segment;
+    int lane;
+    const bool there = place<G>(s, row, segment, lane);
+    if (G == 32 && !there) return;
+    if (!there) row = s.rows - 1, segment = 0;      // the shuffles want every lane
+    const Row r = row_of<E>(s, row);
+    double row_f;
+    float row_rest;
+    row_gate<E>(s, gate, row, row_f, row_rest);
+    double h = initial ? (double)initial[row] : 0.0;
+    if (G == 32 && segment > 0) h = segments_map<true>(maps + row * s.segments, 0, segment, lane)(h);
+    const int64_t first = segment * s.segment_chunks, last = min(first + s.segment_chunks, s.chunks);
+    for (int64_t c = first; c < last; ++c) {
+        if (starts && there && lane == 0) starts[row * s.chunks + c] = (float)h;
+        const int64_t t = (c * G + lane) * kSteps<E> - r.skew;
+        Steps<E> st;
+        st.template load<VEC>(s, r, x, (const E *)gate, row_f, row_rest, t);
+        double at = others<G, true>(scan<G, true>(forward_map<E>(s, st), lane), lane)(h);
+        float out[kSteps<E>];
+#pragma unroll
+        for (int j = 0; j < kSteps<E>; ++j) {
+            at = fma(st.f[j], at, st.input(s, j));
+            out[j] = t + j < r.length ? (float)at : 0.0f;
+        }
+        if (there) store_steps<E, VEC>(y, r.base, t, s.T, out);
+        h = __shfl_sync(~0u, at, G - 1, G);
+    }
+    if (state && there && lane == 0 && segment == s.segments - 1) state[row] = (float)h;
+}
+
+// sums: per row and segment, of df: the gradient of a gate per row
+template <typename E, int G, bool VEC>
+__global__ void __launch_bounds__(256)
+leak_backward_kernel(E *dx, E *dgate, double *sums, float *dinitial, const E *g, const float *gstate, const float *starts, const E *x, const void *gate,
+                     const Map *maps, const LeakShape s)
+{
+    constexpr int N = kSteps<E>;
+    int64_t row, segment;
+    int lane;
+    const bool there = place<G>(s, row, segment, lane);
+    if (G == 32 && !there) return;
+    if (!there) row = s.rows - 1, segment = 0;
+    const Row r = row_of<E>(s, row);
+    double row_f;
+    float row_rest;
+    row_gate<E>(s, gate, row, row_f, row_rest);
+    double carry = gstate ? (double)gstate[row] : 0.0, sum = 0.0;
+    if (G == 32 && segment + 1 < s.segments) carry = segments_map<false>(maps + row * s.segments, segment + 1, s.segments, lane)(carry);
+    const int64_t first = segment * s.segment_chunks, last = min(first + s.segment_chunks, s.chunks);
+    for (int64_t c = last - 1; c >= first; --c) {
+        const int64_t t = (c * G + lane) * N - r.skew;
+        Steps<E> st;
+        float gv[N], before[N];
+        st.template load<VEC>(s, r, x, (const E *)gate, row_f, row_rest, t);
+        load_steps<E, VEC>(gv, g, r.base, t, r.length, 0.0f);
+        double at = others<G, true>(scan<G, true>(forward_map<E>(s, st), lane), lane)((double)starts[row * s.chunks + c]);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            before[j] = (float)at;
+            at = fma(st.f[j], at, st.input(s, j));
+        }
+        at = others<G, false>(scan<G, false>(backward_map<E>(st.f, gv), lane), lane)(carry);
+        float ox[N], og[N];
+#pragma unroll
+        for (int j = N - 1; j >= 0; --j) {
+            const double lambda = at + (double)gv[j];
+            at = st.f[j] * lambda;
+            const bool counts = t + j >= 0 && t + j < r.length;
+            const float l = (float)lambda, df = l * (s.coupled ? before[j] - st.x[j] : before[j]);
+            ox[j] = counts ? (s.coupled ? st.rest[j] * l : l) : 0.0f;
+            og[j] = counts ? (s.logit ? df * ((float)st.f[j] * st.rest[j]) : df) : 0.0f;
+            sum += (double)og[j];
+        }
+        if (there && dx) store_steps<E, VEC>(dx, r.base, t, s.T, ox);
+        if (there && dgate) store_steps<E, VEC>(dgate, r.base, t, s.T, og);
+        carry = __shfl_sync(~0u, at, 0, G);
+    }
+    if (sums) {
+#pragma unroll
+        for (int d = G / 2; d > 0; d /= 2) sum += __shfl_down_sync(~0u, sum, d, G);
+        if (there && lane == 0) sums[row * s.segments + segment] = sum;
+    }
+    if (dinitial && there && lane == 0 && segment == 0) dinitial[row] = (float)carry;
+}
+
+// The gradient of a gate per row is the sum over the rows that have it, in a fixed order: rows (k period + i) inner + j of gate i.  parts > 1:
+// each of them sums every parts-th entry, and a second launch (inner = parts, period = gates, outer = 1) those.
+__global__ void __launch_bounds__(256)
+leak_gate_sum_kernel(double *part, float *out, const double *sums, int64_t outer, int64_t period, int64_t inner, int64_t parts)
+{
+    __shared__ double warp_sum[8];
+    const int64_t i = blockIdx.x / parts, p = blockIdx.x % parts, count = outer * inner;
+    double sum = 0.0;
+    for (int64_t n = p * 256 + threadIdx.x; n < count; n += parts * 256) sum += sums[(n / inner * period + i) * inner + n % inner];
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) sum += __shfl_down_sync(~0u, sum, d);
+    if (threadIdx.x % 32 == 0) warp_sum[threadIdx.x / 32] = sum;
+    __syncthreads();
+    if (threadIdx.x) return;
+    sum = 0.0;
+    for (int w = 0; w < 8; ++w) sum += warp_sum[w];
+    if (part) part[blockIdx.x] = sum;
+    else out[i] = (float)sum;
+}
+
+// one time step: state and output of each row
+template <typename E, typename EG>
+__global__ void __launch_bounds__(256)
+leak_step_kernel(E *y, float *state, const E *x, const EG *gate, int64_t rows, int64_t inner, int64_t period, bool logit, bool coupled)
+{
+    const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (row >= rows) return;
+    double f;
+    float rest;
+    decay_of(to_float<EG>(gate[period ? row / inner % period : row]), logit, f, rest);
+    const float v = to_float<E>(x[row]);
+    const float h = (float)fma(f, (double)state[row], (double)(coupled ? rest * v : v));
+    state[row] = h;
+    y[row] = from_float<E>(h);
+}
+
+// ------------------------------------------------------------------------------------------------ host side
+constexpr int64_t kGateCount = 8192;      // entries that one CTA adds up
+
+static int lanes_of(int64_t T, int steps)
+{
+    int g = 1;
+    while (g < 32 && (int64_t)g * steps < T + (T % steps ? steps - 1 : 0)) g *= 2;
+    return g;
+}
+
+static int64_t chunks_of(int64_t T, int steps) { return ceil_div(T + (T % steps ? steps - 1 : 0), (int64_t)lanes_of(T, steps) * steps); }
+
+static int steps_of(int dtype) { return dtype == SLAYER_B200_F32 ? 4 : 8; }
+
+// groups per row: rows with many chunks, too few to give every SM 32 warps, are split.
+static int64_t segments_of(int64_t rows, int64_t T, int steps)
+{
+    const int64_t chunks = chunks_of(T, steps), warps = (int64_t)sm_count() * 32;
+    if (lanes_of(T, steps) < 32 || chunks < 4 || rows * 2 > warps) return 1;
+    int64_t n = warps / rows;
+    if (n > chunks / 2) n = chunks / 2;
+    if (n > 1024) n = 1024;
+    return ceil_div(chunks, ceil_div(chunks, n));
+}
+
+static bool known(int dtype) { return dtype == SLAYER_B200_F32 || dtype == SLAYER_B200_BF16 || dtype == SLAYER_B200_F16; }
+
+struct LeakPlan {
+    LeakShape s;
+    int lanes;
+    int64_t maps_bytes, sums_bytes, gate_parts;
+};
+
+static int plan_leak(LeakPlan &p, const char *op, int dtype, int flags, int64_t rows, int64_t T, const int64_t *lengths, int64_t sample_rows,
+                     int64_t gate_inner, int64_t gate_period)
+{
+    SB200_REQUIRE(known(dtype), "%s: unknown element type %d", op, dtype);
+    SB200_REQUIRE((flags & ~3) == 0, "%s: unknown flags %d", op, flags);
+    SB200_REQUIRE(rows >= 0 && T >= 0, "%s: negative size", op);
+    SB200_REQUIRE(rows <= (int64_t)1 << 40 && T <= (int64_t)1 << 40 && rows * (T >> 20) <= (int64_t)1 << 40, "%s: sizes overflow", op);
+    SB200_REQUIRE(gate_period >= 0 && (gate_period == 0 || gate_inner >= 1), "%s: bad gate layout", op);
+    SB200_REQUIRE(gate_period == 0 || (gate_period <= rows && gate_inner <= rows && rows % (gate_inner * gate_period) == 0) || rows == 0,
+                  "%s: rows must be whole groups of gates", op);
+    SB200_REQUIRE(!lengths || sample_rows >= 1, "%s: lengths need the number of rows that have one", op);
+    const int steps = steps_of(dtype);
+    p.s = {rows, T, gate_inner, gate_period, sample_rows, lengths, chunks_of(T, steps), 1, 0, (flags & SLAYER_B200_LEAK_LOGIT) != 0,
+           (flags & SLAYER_B200_LEAK_COUPLED) != 0};
+    p.s.segments = rows ? segments_of(rows, T, steps) : 1;
+    p.s.segment_chunks = ceil_div(p.s.chunks, p.s.segments);
+    p.lanes = lanes_of(T, steps);
+    p.maps_bytes = p.s.segments > 1 ? rows * p.s.segments * (int64_t)sizeof(Map) : 0;
+    p.sums_bytes = p.gate_parts = 0;
+    if (gate_period && rows) {
+        const int64_t count = rows / gate_period * p.s.segments;
+        p.gate_parts = ceil_div(count, kGateCount);
+        if (p.gate_parts > 1024) p.gate_parts = 1024;
+        p.sums_bytes = (rows * p.s.segments + (p.gate_parts > 1 ? gate_period * p.gate_parts : 0)) * (int64_t)sizeof(double);
+    }
+    SB200_REQUIRE(ceil_div(rows * p.s.segments * p.lanes, 256) <= 0x7fffffff, "%s: too many rows", op);
+    SB200_REQUIRE(p.gate_parts * gate_period <= 0x7fffffff, "%s: too many gates", op);
+    return SLAYER_B200_OK;
+}
+
+template <typename E, int G, bool VEC>
+static void run_forward(const LeakPlan &p, void *y, float *state, float *starts, const void *x, const void *gate, const float *initial, void *workspace,
+                        cudaStream_t st)
+{
+    Map *maps = (Map *)workspace;
+    const unsigned blocks = (unsigned)ceil_div(p.s.rows * p.s.segments * G, 256);
+    if constexpr (G == 32)
+        if (p.s.segments > 1) leak_maps_kernel<E, VEC><<<blocks, 256, 0, st>>>(maps, (const E *)x, gate, nullptr, p.s, true);
+    leak_forward_kernel<E, G, VEC><<<blocks, 256, 0, st>>>((E *)y, state, starts, (const E *)x, gate, initial, maps, p.s);
+}
+
+template <typename E, int G, bool VEC>
+static void run_backward(const LeakPlan &p, void *dx, void *dgate, float *dinitial, const void *g, const float *gstate, const float *starts, const void *x,
+                         const void *gate, void *workspace, cudaStream_t st)
+{
+    Map *maps = (Map *)workspace;
+    double *sums = (double *)((char *)workspace + p.maps_bytes);
+    const bool per_row = p.s.gate_period > 0;
+    const unsigned blocks = (unsigned)ceil_div(p.s.rows * p.s.segments * G, 256);
+    if constexpr (G == 32)
+        if (p.s.segments > 1) leak_maps_kernel<E, VEC><<<blocks, 256, 0, st>>>(maps, nullptr, gate, (const E *)g, p.s, false);
+    leak_backward_kernel<E, G, VEC><<<blocks, 256, 0, st>>>((E *)dx, per_row ? nullptr : (E *)dgate, per_row && dgate ? sums : nullptr, dinitial, (const E *)g,
+                                                          gstate, starts, (const E *)x, gate, maps, p.s);
+    if (per_row && dgate) {
+        const int64_t inner = p.s.gate_inner * p.s.segments, outer = p.s.rows / (p.s.gate_inner * p.s.gate_period);
+        double *part = sums + p.s.rows * p.s.segments;
+        const unsigned gates = (unsigned)p.s.gate_period;
+        if (p.gate_parts > 1) {
+            leak_gate_sum_kernel<<<gates * (unsigned)p.gate_parts, 256, 0, st>>>(part, nullptr, sums, outer, p.s.gate_period, inner, p.gate_parts);
+            leak_gate_sum_kernel<<<gates, 256, 0, st>>>(nullptr, (float *)dgate, part, 1, p.s.gate_period, p.gate_parts, 1);
+        } else {
+            leak_gate_sum_kernel<<<gates, 256, 0, st>>>(nullptr, (float *)dgate, sums, outer, p.s.gate_period, inner, 1);
+        }
+    }
+}
+
+#define SB200_LEAK_LANES(E, VEC, CALL)                       \
+    switch (p.lanes) {                                       \
+    case 1: CALL(E, 1, VEC); break;                          \
+    case 2: CALL(E, 2, VEC); break;                          \
+    case 4: CALL(E, 4, VEC); break;                          \
+    case 8: CALL(E, 8, VEC); break;                          \
+    case 16: CALL(E, 16, VEC); break;                        \
+    default: CALL(E, 32, VEC); break;                        \
+    }
+#define SB200_LEAK_ALIGN(E, CALL)                            \
+    if (vec) { SB200_LEAK_LANES(E, true, CALL) } else { SB200_LEAK_LANES(E, false, CALL) }
+#define SB200_LEAK_TYPES(CALL)                                                     \
+    if (dtype == SLAYER_B200_F32) { SB200_LEAK_ALIGN(float, CALL) }               \
+    else if (dtype == SLAYER_B200_BF16) { SB200_LEAK_ALIGN(__nv_bfloat16, CALL) } \
+    else { SB200_LEAK_ALIGN(__half, CALL) }
+
+static bool element_aligned(const void *p, int dtype) { return ((uintptr_t)p & (dtype == SLAYER_B200_F32 ? 3 : 1)) == 0; }
+static bool aligned_to(const void *p, unsigned n) { return ((uintptr_t)p & (n - 1)) == 0; }
+
+}  // namespace sb200
+
+extern "C" int64_t slayer_b200_leak_chunks(int64_t T, int dtype)
+{
+    using namespace sb200;
+    clear_error();
+    SB200_REQUIRE(known(dtype), "leak_chunks: unknown element type %d", dtype);
+    SB200_REQUIRE(T >= 0 && T <= (int64_t)1 << 40, "leak_chunks: bad length");
+    return chunks_of(T, steps_of(dtype));
+}
+
+extern "C" int64_t slayer_b200_leak_workspace(int64_t rows, int64_t T, int dtype, int64_t gate_inner, int64_t gate_period)
+{
+    using namespace sb200;
+    clear_error();
+    LeakPlan p;
+    const int rc = plan_leak(p, "leak_workspace", dtype, 0, rows, T, nullptr, 1, gate_inner, gate_period);
+    return rc ? rc : p.maps_bytes + p.sums_bytes;
+}
+
+extern "C" int slayer_b200_leak_forward(void *y, float *state, float *starts, const void *x, const void *gate, const float *initial, int dtype, int flags,
+                                        int64_t rows, int64_t T, const int64_t *lengths, int64_t sample_rows, int64_t gate_inner, int64_t gate_period,
+                                        void *workspace, void *stream)
+{
+    using namespace sb200;
+    clear_error();
+    LeakPlan p;
+    const int rc = plan_leak(p, "leak_forward", dtype, flags, rows, T, lengths, sample_rows, gate_inner, gate_period);
+    if (rc) return rc;
+    if (rows == 0) return SLAYER_B200_OK;
+    SB200_REQUIRE((y && x) || T == 0, "leak_forward: null pointer");
+    SB200_REQUIRE(gate || (T == 0 && gate_period == 0), "leak_forward: null pointer");
+    SB200_REQUIRE(p.maps_bytes == 0 || (workspace && aligned16(workspace)), "leak_forward: the workspace must be aligned to 16 bytes");
+    SB200_REQUIRE(element_aligned(y, dtype) && element_aligned(x, dtype) && element_aligned(gate, gate_period ? SLAYER_B200_F32 : dtype) &&
+                      aligned_to(state, 4) && aligned_to(starts, 4) && aligned_to(initial, 4) && aligned_to(lengths, 8),
+                  "leak_forward: a pointer off its element's alignment");
+    const bool vec = aligned16(y) && aligned16(x) && (gate_period || aligned16(gate));
+    const cudaStream_t st = (cudaStream_t)stream;
+#define SB200_LEAK_CALL(E, G, VEC) run_forward<E, G, VEC>(p, y, state, starts, x, gate, initial, workspace, st)
+    SB200_LEAK_TYPES(SB200_LEAK_CALL)
+#undef SB200_LEAK_CALL
+    return check_launch("leak_forward kernel launch");
+}
+
+extern "C" int slayer_b200_leak_backward(void *dx, void *dgate, float *dinitial, const void *g, const float *gstate, const float *starts, const void *x,
+                                         const void *gate, int dtype, int flags, int64_t rows, int64_t T, const int64_t *lengths, int64_t sample_rows,
+                                         int64_t gate_inner, int64_t gate_period, void *workspace, void *stream)
+{
+    using namespace sb200;
+    clear_error();
+    LeakPlan p;
+    const int rc = plan_leak(p, "leak_backward", dtype, flags, rows, T, lengths, sample_rows, gate_inner, gate_period);
+    if (rc) return rc;
+    if (rows == 0) return SLAYER_B200_OK;
+    SB200_REQUIRE((g && x && starts) || T == 0, "leak_backward: null pointer");
+    SB200_REQUIRE(gate || (T == 0 && gate_period == 0), "leak_backward: null pointer");
+    SB200_REQUIRE(p.maps_bytes + p.sums_bytes == 0 || (workspace && aligned16(workspace)), "leak_backward: the workspace must be aligned to 16 bytes");
+    SB200_REQUIRE(element_aligned(dx, dtype) && element_aligned(dgate, gate_period ? SLAYER_B200_F32 : dtype) && element_aligned(g, dtype) &&
+                      element_aligned(x, dtype) && element_aligned(gate, gate_period ? SLAYER_B200_F32 : dtype) && aligned_to(dinitial, 4) &&
+                      aligned_to(gstate, 4) && aligned_to(starts, 4) && aligned_to(lengths, 8),
+                  "leak_backward: a pointer off its element's alignment");
+    const bool vec = aligned16(dx) && aligned16(g) && aligned16(x) && (gate_period || (aligned16(gate) && aligned16(dgate)));
+    const cudaStream_t st = (cudaStream_t)stream;
+#define SB200_LEAK_CALL(E, G, VEC) run_backward<E, G, VEC>(p, dx, dgate, dinitial, g, gstate, starts, x, gate, workspace, st)
+    SB200_LEAK_TYPES(SB200_LEAK_CALL)
+#undef SB200_LEAK_CALL
+    return check_launch("leak_backward kernel launch");
+}
+
+extern "C" int slayer_b200_leak_step(void *y, float *state, const void *x, const void *gate, int dtype, int gate_dtype, int flags, int64_t rows,
+                                     int64_t gate_inner, int64_t gate_period, void *stream)
+{
+    using namespace sb200;
+    clear_error();
+    LeakPlan p;
+    const int rc = plan_leak(p, "leak_step", dtype, flags, rows, 1, nullptr, 1, gate_inner, gate_period);
+    if (rc) return rc;
+    SB200_REQUIRE(gate_dtype == dtype || gate_dtype == SLAYER_B200_F32, "leak_step: the gate has x's type or float32");
+    if (rows == 0) return SLAYER_B200_OK;
+    SB200_REQUIRE(y && state && x && gate, "leak_step: null pointer");
+    SB200_REQUIRE(element_aligned(y, dtype) && element_aligned(x, dtype) && element_aligned(gate, gate_dtype) && aligned_to(state, 4),
+                  "leak_step: a pointer off its element's alignment");
+    const unsigned blocks = (unsigned)ceil_div(rows, 256);
+    const cudaStream_t st = (cudaStream_t)stream;
+#define SB200_LEAK_STEP(E, EG)                                                                                                                       \
+    leak_step_kernel<E, EG><<<blocks, 256, 0, st>>>((E *)y, state, (const E *)x, (const EG *)gate, rows, gate_inner, gate_period, p.s.logit, p.s.coupled)
+    if (dtype == SLAYER_B200_F32) SB200_LEAK_STEP(float, float);
+    else if (dtype == SLAYER_B200_BF16 && gate_dtype == SLAYER_B200_F32) SB200_LEAK_STEP(__nv_bfloat16, float);
+    else if (dtype == SLAYER_B200_BF16) SB200_LEAK_STEP(__nv_bfloat16, __nv_bfloat16);
+    else if (gate_dtype == SLAYER_B200_F32) SB200_LEAK_STEP(__half, float);
+    else SB200_LEAK_STEP(__half, __half);
+#undef SB200_LEAK_STEP
+    return check_launch("leak_step kernel launch");
+}

@@ -25,6 +25,7 @@ import torch
 import torch.nn.functional as F
 
 from . import load_ops
+from .recurrence import gatedLeak, gatedLeakStep
 from .response import alpha_kernel, loihi_psp_kernel, loihi_ref_kernel
 
 slayerCuda, slayerLoihiCuda = load_ops()
@@ -64,6 +65,53 @@ class _SpikeFunction(torch.autograd.Function):
     def backward(ctx, grad):
         (u,) = ctx.saved_tensors
         return slayerCuda.spikeGrad(grad.contiguous(), u, ctx.theta, ctx.tau, ctx.scale), None, None, None
+
+
+class _SpikeFunction8(torch.autograd.Function):
+    """_SpikeFunction with the membrane potential kept in 8 bits: the same spikes, and the surrogate gradient of what is kept."""
+
+    @staticmethod
+    def forward(ctx, u, refKernel, neuron, Ts):
+        u = u.contiguous()
+        spikes = slayerCuda.getSpikes(u, refKernel, neuron['theta'], Ts)
+        if ctx.needs_input_grad[0]:
+            ctx.save_for_backward(*slayerCuda.compress8(u))
+        ctx.theta = float(neuron['theta'])
+        ctx.tau = float(neuron['tauRho'] * neuron['theta'])
+        ctx.scale = float(neuron['scaleRho'])
+        return spikes
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        q, scale = ctx.saved_tensors
+        return slayerCuda.spikeGrad8(grad.contiguous(), q, scale, ctx.theta, ctx.tau, ctx.scale), None, None, None
+
+
+class _DenseFunction8(torch.autograd.Function):
+    """A dense layer whose input is kept in 8 bits: the forward pass and the input's gradient are PyTorch's, the weight gradient is formed from
+    what is kept."""
+
+    @staticmethod
+    def forward(ctx, x, weight):
+        if ctx.needs_input_grad[1]:
+            ctx.save_for_backward(weight, *slayerCuda.compress8(x))
+        else:
+            ctx.save_for_backward(weight)
+        ctx.shape = x.shape
+        return F.conv3d(x, weight)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        weight, *kept = ctx.saved_tensors
+        grad = grad.contiguous()
+        gradInput = gradWeight = None
+        if ctx.needs_input_grad[0]:
+            gradInput = torch.nn.grad.conv3d_input(ctx.shape, weight, grad)
+        if ctx.needs_input_grad[1]:
+            gradWeight = slayerCuda.weightGrad8(grad, *kept, ctx.shape)
+        return gradInput, gradWeight
 
 
 class PackedSpikes:
@@ -265,7 +313,7 @@ class _DenseLayer(torch.nn.Conv3d):
     exception texts - because it is the interface the reference's networks are written against;
     weighting is not part of the hot path."""
 
-    def __init__(self, inFeatures, outFeatures, weightScale=1):
+    def __init__(self, inFeatures, outFeatures, weightScale=1, checkpoint=False):
         if isinstance(inFeatures, int):
             kernel, channels = (1, 1, 1), inFeatures
         elif len(inFeatures) == 2:
@@ -279,8 +327,13 @@ class _DenseLayer(torch.nn.Conv3d):
         super().__init__(channels, outFeatures, kernel, bias=False)
         if weightScale != 1:
             self.weight = torch.nn.Parameter(weightScale * self.weight)
+        self.checkpoint = checkpoint
 
     def forward(self, x):
+        if self.checkpoint:
+            if x.dim() != 5 or x.shape[2:4] != self.weight.shape[2:4]:
+                raise ValueError('dense: a layer that keeps its input in 8 bits takes inputs of its own size, got {}'.format(tuple(x.shape)))
+            return _DenseFunction8.apply(x, self.weight)
         return F.conv3d(x, self.weight, self.bias, self.stride, self.padding, self.dilation, self.groups)
 
 
@@ -305,6 +358,30 @@ class _DelayLayer(torch.nn.Module):
         if x.numel() != self.delay.numel() * Ns * N:
             return _DelayFunction.apply(x, self.delay.repeat((1, H, W)), self.Ts)
         return _DelayFunction.apply(x, self.delay, self.Ts)
+
+
+class _LeakLayer(torch.nn.Module):
+    """Gated leaky integrator with a learnable decay per neuron or per channel, made like _DelayLayer.  ``gate`` holds logits:
+    decays ``sigmoid(gate)``, drawn as 1 - 1/tau with time constants tau from 2 to 100 steps, evenly on a logarithmic scale."""
+
+    def __init__(self, inputSize, coupled=False):
+        super().__init__()
+        if isinstance(inputSize, int):
+            shape = (inputSize, 1, 1, 1)
+        elif len(inputSize) == 3:
+            shape = tuple(inputSize) + (1,)
+        else:
+            raise Exception('inputSize can only be 1 or 2 dimension. It was: {}'.format(inputSize))
+        tau = 2 * 50 ** torch.rand(shape)
+        self.gate = torch.nn.Parameter(torch.log(tau - 1), requires_grad=True)
+        self.coupled = coupled
+
+    def forward(self, x, initial=None, lengths=None, returnState=False):
+        return gatedLeak(x, self.gate, initial=initial, lengths=lengths, coupled=self.coupled, returnState=returnState)
+
+    def step(self, x, state):
+        """One time step of a stream: ``x [N, C, H, W]``, ``state`` updated in place."""
+        return gatedLeakStep(x, self.gate.detach()[..., 0], state, coupled=self.coupled)
 
 
 class spikeLayer(torch.nn.Module):
@@ -342,8 +419,18 @@ class spikeLayer(torch.nn.Module):
         out, bits = _SpikePspFunction.apply(membranePotential, self.srmKernel, self.refKernel, self.neuron, Ts)
         return out, PackedSpikes(bits, membranePotential.shape[-1], 1.0 / Ts)
 
-    def spike(self, membranePotential):
-        return _SpikeFunction.apply(membranePotential, self.refKernel, self.neuron, self.simulation['Ts'])
+    def gatedPsp(self, x, gate, initial=None, lengths=None, kind='logit', coupled=False, returnState=False):
+        """A psp filter whose decay is an input: ``recurrence.gatedLeak``.  Not part of the reference's interface."""
+        return gatedLeak(x, gate, initial=initial, lengths=lengths, kind=kind, coupled=coupled, returnState=returnState)
+
+    def leak(self, inputSize, coupled=False):
+        """A layer that is a ``gatedPsp`` with a learnable decay: ``inputSize`` as in ``delay``.  Not part of the reference's interface."""
+        return _LeakLayer(inputSize, coupled)
+
+    def spike(self, membranePotential, checkpoint=False):
+        """``checkpoint``: the membrane potential is kept in 8 bits for the backward pass (not part of the reference's interface)."""
+        function = _SpikeFunction8 if checkpoint else _SpikeFunction
+        return function.apply(membranePotential, self.refKernel, self.neuron, self.simulation['Ts'])
 
     def delayShift(self, input, delay, Ts=1):
         return _DelayShiftFunction.apply(input, delay, Ts)
@@ -366,8 +453,9 @@ class spikeLayer(torch.nn.Module):
     def delay(self, inputSize):
         return _DelayLayer(inputSize, self.simulation['Ts'])
 
-    def dense(self, inFeatures, outFeatures, weightScale=10):
-        return _DenseLayer(inFeatures, outFeatures, weightScale)
+    def dense(self, inFeatures, outFeatures, weightScale=10, checkpoint=False):
+        """``checkpoint``: the layer's input is kept in 8 bits for the weight gradient (not part of the reference's interface)."""
+        return _DenseLayer(inFeatures, outFeatures, weightScale, checkpoint)
 
 
 class loihiLayer(spikeLayer):
@@ -400,5 +488,5 @@ class loihiLayer(spikeLayer):
     def spikeLoihiFull(self, weightedSpikes):
         return _LoihiSpikeFunction.loihi(weightedSpikes, self.neuron, self.simulation['Ts'])
 
-    def dense(self, inFeatures, outFeatures, weightScale=100):
-        return _DenseLayer(inFeatures, outFeatures, weightScale)
+    def dense(self, inFeatures, outFeatures, weightScale=100, checkpoint=False):
+        return _DenseLayer(inFeatures, outFeatures, weightScale, checkpoint)
