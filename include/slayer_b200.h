@@ -422,7 +422,7 @@ int slayer_b200_leak_step(void *y, float *state, const void *x, const void *gate
  * A tensor x [rows, T] (type `dtype`) kept in 8 bits: of each 32 consecutive steps of a row, q = x / 2^e rounded to the
  * nearest whole number (ties to even), with the smallest e in [-126, 121] such that |x| <= 127 2^e for all of
  * them that are finite.  q: [rows, 32 ceil(T / 32)], zeros behind the last step, aligned to 16 bytes; what is not
- * finite is -128.  scale: [rows, ceil(T / 32)], e + 127.  It has no counterpart in the reference.
+ * finite is -128.  scale: [ceil(T / 32), rows], e + 127.  It has no counterpart in the reference.
  */
 int slayer_b200_compress8(int8_t *q, uint8_t *scale, const void *x, int dtype, int64_t rows, int64_t T, void *stream);
 
@@ -440,7 +440,8 @@ int slayer_b200_spike_grad8(float *out, const float *g, const int8_t *q, const u
 /*
  * Weight gradient of a dense layer whose input x [N, I, T] is kept so, for the gradient g [N, O, T] of its output:
  *   out[o, i] = sum over n and t of g[n, o, t] x[n, i, t],
- * in float32 precision, the same bits in every call.  workspace: slayer_b200_weight_grad8_workspace(...) bytes of device
+ * in float32 precision, the same bits in every call.  Its products wait on barriers for a limited time; if one ever
+ * runs out, the result is not complete and slayer_b200_device_status() says 0x5104.  workspace: slayer_b200_weight_grad8_workspace(...) bytes of device
  * memory, aligned to 16.  It has no counterpart in the reference, whose weights are PyTorch's
  * (src/slayer.py:393-437).
  */

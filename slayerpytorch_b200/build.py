@@ -44,6 +44,7 @@ CUDA_SOURCES = {
     "newton_schulz.cu": [],
     "leak.cu": [],
     "checkpoint.cu": [],
+    "weight_grad.cu": [],
     "tma.cu": [],
 }
 HEADERS = ["common.cuh", "tile.cuh", "tma.cuh", "tensor.cuh", "fir_sparse.cuh", os.path.join(INCLUDE, "slayer_b200.h")]

@@ -15,8 +15,8 @@ slayerCuda, _ = load_ops()
 
 
 class Checkpoint:
-    """A tensor ``[..., T]`` in 8 bits, made by ``compress``: ``q`` (int8, rows of whole groups of 32 steps) and ``scale`` (uint8, one
-    for each group: the values are ``q * 2**(scale - 127)``)."""
+    """A tensor ``[..., T]`` in 8 bits, made by ``compress``: ``q`` (int8, ``[rows, 32 * groups]``) and ``scale`` (uint8,
+    ``[groups, rows]``, one for each 32 steps of a row: the values are ``q * 2**(scale - 127)``)."""
 
     def __init__(self, q, scale, shape, dtype):
         self.q, self.scale, self.shape, self.dtype = q, scale, torch.Size(shape), dtype

@@ -223,8 +223,8 @@ void check_kept(const torch::Tensor &q, const torch::Tensor &scale, at::IntArray
     const int64_t rows = product(sizes, 0, (int64_t)sizes.size() - 1), groups = (sizes.back() + 31) / 32;
     TORCH_CHECK(q.is_cuda() && scale.is_cuda(), op, ": a checkpoint must be on a CUDA device");
     check_device(q, scale, "q", "scale");
-    TORCH_CHECK_VALUE(q.sizes() == at::IntArrayRef({rows, groups * 32}) && scale.sizes() == at::IntArrayRef({rows, groups}), op, ": a checkpoint of ",
-                      sizes, " has values ", at::IntArrayRef({rows, groups * 32}), " and scales ", at::IntArrayRef({rows, groups}), ", got ", q.sizes(), " and ",
+    TORCH_CHECK_VALUE(q.sizes() == at::IntArrayRef({rows, groups * 32}) && scale.sizes() == at::IntArrayRef({groups, rows}), op, ": a checkpoint of ",
+                      sizes, " has values ", at::IntArrayRef({rows, groups * 32}), " and scales ", at::IntArrayRef({groups, rows}), ", got ", q.sizes(), " and ",
                       scale.sizes());
     TORCH_CHECK(q.scalar_type() == torch::kInt8 && scale.scalar_type() == torch::kUInt8 && q.is_contiguous() && scale.is_contiguous(), op,
                 ": a checkpoint has contiguous int8 values and uint8 scales");
@@ -238,7 +238,7 @@ std::vector<torch::Tensor> compress8Cuda(const torch::Tensor &x)
     c10::cuda::CUDAGuard guard(x.device());
     const auto in = x.detach().contiguous();
     const int64_t rows = product(x.sizes(), 0, x.dim() - 1), T = x.size(-1), groups = (T + 31) / 32;
-    auto q = torch::empty({rows, groups * 32}, x.options().dtype(torch::kInt8)), scale = torch::empty({rows, groups}, x.options().dtype(torch::kUInt8));
+    auto q = torch::empty({rows, groups * 32}, x.options().dtype(torch::kInt8)), scale = torch::empty({groups, rows}, x.options().dtype(torch::kUInt8));
     check_rc(slayer_b200_compress8(q.data_ptr<int8_t>(), scale.data_ptr<uint8_t>(), in.data_ptr(), dtype, rows, T, current_stream()), "compress");
     return {q, scale};
 }

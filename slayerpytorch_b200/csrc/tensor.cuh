@@ -27,6 +27,12 @@ __device__ __forceinline__ uint32_t product_shape(int m, int n, bool a_columns, 
     return 1u << 4 | (a_columns ? 1u << 15 : 0u) | (b_columns ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24;
 }
 
+// bf16 x bf16 -> fp32, M x N; both given by desc_rows
+__host__ __device__ constexpr uint32_t product_shape_bf16(int m, int n)
+{
+    return 1u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24;
+}
+
 // The operations come for one CTA (CG = 1), or for a cluster of two (CG = 2) whose tensor cores make one product of twice the rows:
 // each CTA has half of the first operand's rows and half of the second's, at the same places of its shared memory, and gets
 // its own rows of the result.  The first CTA issues it.

@@ -1,0 +1,432 @@
+// Weight gradient of a dense layer from an input kept in 8 bits (checkpoint.cu):
+//   dW[o, i] = sum over samples n and steps t of g[n, o, t] x[n, i, t],  x = q 2^e,
+// as products of bfloat16 tiles on the tensor cores.  q 2^e is a bfloat16 as it is; g, a float32, is the sum of three: its upper 8 bits, the
+// next 8 and the last 8, cut off and not rounded, so that the three parts are g exactly.  Three products, summed in float32, have the
+// precision of float32 products.  Both operands have time as their summation index and next to each other in memory, as the tensor cores
+// like it, but neither is in a form that they read: 16 warps load tiles, two or three steps ahead of their use, take them apart in registers
+// and write them to shared memory as 128-byte rows; one thread issues the products.
+//
+// The tensor core cuts sums off where it adds: sums of kSteps blocks of 64 steps are made there, and added up in registers, rounded.
+//
+// x is the operand with the tile's rows (i), g the one with its columns (o): large layers take tiles of 256 x 256 by pairs of CTAs, each of which loads and
+// takes apart one half of either; layers of up to 128 outputs tiles of 128 x 16 to 128 x 128 by one CTA.  The tiles' blocks of 64 steps are dealt out
+// to all SMs in equal shares (tile after tile: a share has the end of one tile, some whole ones and the start of another), and the shares'
+// sums are added up by a second launch, in order.
+#include <algorithm>
+
+#include "tensor.cuh"
+
+namespace sb200 {
+
+constexpr int kWgWaitLimit = 1 << 22;
+constexpr int kStatusWeightTimeout = 0x5104;
+constexpr int kWgWorkers = 512, kWgThreads = kWgWorkers + 128;
+constexpr int kSteps = 2;        // blocks of 64 steps in a sum of the tensor core
+
+template <int CG, int NT>
+struct WgTile {
+    static constexpr int NB = NT / CG;                      // columns (of g) that a CTA loads
+    static constexpr int kA = 128 * 128, kB = NB * 128;     // bytes of a block of 64 steps: x, and one part of g
+    static constexpr int kStage = kA + 3 * kB;
+    static constexpr int kStages = 3 * kStage > 160 * 1024 ? 3 : (200 * 1024 / kStage < 6 ? 200 * 1024 / kStage : 6);
+    static constexpr int kCols = NT >= 64 ? NT / 4 : 16;    // of a warp's sums
+    static constexpr int kItems = NB >= 32 ? NB / 32 : 1;   // float4 of g a thread has of a block
+    static constexpr uint32_t kMem = NT < 16 ? 32 : 2 * NT;
+    static constexpr size_t kShared = kStages * kStage + 1024;
+};
+
+struct WgArgs {
+    const float *g;
+    const int8_t *q;
+    const uint8_t *scale;
+    float *part;
+    int *status;
+    int64_t N, O, I, T, G;
+    int64_t units, blocks;       // 16 steps of a sample; 4 of those
+    int U;                       // units of a sample
+    int64_t tiles_o, work;       // tiles next to each other share their rows; tiles x blocks
+    int shares;
+};
+
+// First of the 16-step units that a thread loads, and the next ones, four further on.
+struct WgUnit {
+    int64_t unit;
+    int64_t n;
+    int t16;
+    __device__ __forceinline__ void start(int64_t u, int U)
+    {
+        unit = u;
+        n = u / U;
+        t16 = (int)(u - n * U);
+    }
+    __device__ __forceinline__ void next(int U)
+    {
+        unit += 4;
+        t16 += 4;
+        while (t16 >= U) {
+            t16 -= U;
+            ++n;
+        }
+    }
+};
+
+// the upper 16 bits of two floats
+__device__ __forceinline__ uint32_t upper(float a, float b) { return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632); }
+__device__ __forceinline__ float cut(float a) { return __uint_as_float(__float_as_uint(a) & 0xffff0000u); }
+
+// 16 whole numbers times a power of two, as bfloat16
+__device__ __forceinline__ void wg_expand(uint4 raw, unsigned byte, uint4 &lo, uint4 &hi)
+{
+    const uint32_t w[4] = {raw.x ^ 0x80808080u, raw.y ^ 0x80808080u, raw.z ^ 0x80808080u, raw.w ^ 0x80808080u};     // q + 128
+    const float s = __uint_as_float(byte << 23);
+    uint32_t out[8];
+    uint32_t none = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        float f[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = (__uint_as_float(__byte_perm(w[k], 0x4b000000u, 0x7540 | j)) - 8388736.0f) * s;     // 2^23 + q + 128
+        out[2 * k] = upper(f[0], f[1]);
+        out[2 * k + 1] = upper(f[2], f[3]);
+        none |= (w[k] - 0x01010101u) & ~w[k] & 0x80808080u;       // a byte of 0: -128, which stands for what is not finite
+    }
+    if (none) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (((w[k] >> (8 * j)) & 0xff) == 0) {
+                    uint32_t &two = out[2 * k + j / 2];
+                    two = j & 1 ? (two & 0xffffu) | 0x7fc00000u : (two & 0xffff0000u) | 0x7fc0u;
+                }
+    }
+    lo = make_uint4(out[0], out[1], out[2], out[3]);
+    hi = make_uint4(out[4], out[5], out[6], out[7]);
+}
+
+template <int CG, int NT, bool VEC>
+__global__ void __launch_bounds__(kWgThreads, 1) weight_grad_kernel(const __grid_constant__ WgArgs A)
+{
+    using Tile = WgTile<CG, NT>;
+    constexpr int S = Tile::kStages;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char *smem = (unsigned char *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    __shared__ uint64_t full[S], empty[S], made[2], taken[2], last;
+    __shared__ uint32_t base_at;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rank = CG == 2 ? (int)cluster_rank() : 0;
+    if (warp == 16) tensor_alloc<CG>(&base_at, Tile::kMem);
+    if (tid == 0) {
+        for (int s = 0; s < S; ++s) {
+            mbar_init(full + s, 16 * CG);
+            mbar_init(empty + s, 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(made + b, 1);
+            mbar_init(taken + b, 16 * CG);
+        }
+        mbar_init(&last, 1);
+        mbar_init_fence();
+    }
+    tensor_fence_before();
+    __syncthreads();
+    if (CG == 2) cluster_wait_all();
+    tensor_fence_after();
+    const uint32_t acc = base_at;
+    const int share = blockIdx.x / CG;
+    const int64_t from = A.work * share / A.shares, to = A.work * (share + 1) / A.shares;
+    bool fine = true;
+
+    // registers: 512 * 112 + 128 * 32 = 640 * 96
+    if (warp < 16) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
+        // x: a row and one of the four units; g: rows of 8 (in an order that keeps the stores of a half warp on different banks), one unit
+        const int arow = warp * 8 + (lane >> 2), au = lane & 3, quarter = lane & 3, bu = warp & 3;
+        const int brow = (warp >> 2) * (Tile::NB >= 32 ? Tile::NB / 4 : 8) + 2 * ((lane >> 2) & 3) + (lane >> 4);
+        const bool has_b = Tile::NB >= 32 || (warp >> 2) * 8 < Tile::NB;
+        const int64_t rows = A.N * A.I;
+        unsigned char *const ato = smem + arow * 128;
+        unsigned char *const bto = smem + Tile::kA + brow * 128 + (((2 * bu + (quarter >> 1)) ^ (brow & 7)) * 16) + (quarter & 1) * 8;
+        const bool sums_here = (warp >> 2) * Tile::kCols < NT;
+        const uint32_t at = acc + ((uint32_t)((warp & 3) * 32) << 16) + (warp >> 2) * Tile::kCols;
+        int s = 0, turn = 0, slot = 0, again = 0;
+        for (int64_t w = from; fine && w < to;) {
+            const int64_t tile = w / A.blocks, k0 = w - tile * A.blocks, k1 = k0 + (to - w < A.blocks - k0 ? to - w : A.blocks - k0);
+            const int64_t ti = tile / A.tiles_o, i0 = (ti * CG + rank) * 128, o0 = (tile - ti * A.tiles_o) * NT + rank * Tile::NB;
+            const bool arow_there = i0 + arow < A.I;
+            WgUnit ua, ub;
+            ua.start(k0 * 4 + au, A.U);
+            ub.start(k0 * 4 + bu, A.U);
+            uint4 raw;
+            unsigned byte;
+            float4 gv[Tile::kItems];
+            const auto load = [&] {
+                raw = make_uint4(0, 0, 0, 0);
+                byte = 127;
+                if (arow_there && ua.unit < A.units) {
+                    const int64_t row = ua.n * A.I + i0 + arow;
+                    raw = __ldg((const uint4 *)(A.q + row * (A.G * 32) + ua.t16 * 16));
+                    byte = __ldg(A.scale + (int64_t)(ua.t16 >> 1) * rows + row);
+                }
+                const int64_t t = (int64_t)ub.t16 * 16 + quarter * 4;
+                const float *p = A.g + (ub.n * A.O + o0 + brow) * A.T + t;
+#pragma unroll
+                for (int j = 0; j < Tile::kItems; ++j, p += 8 * A.T) {
+                    gv[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (has_b && ub.unit < A.units && o0 + brow + 8 * j < A.O) {
+                        if (VEC) {
+                            if (t < A.T) gv[j] = __ldg((const float4 *)p);
+                        } else {
+                            if (t < A.T) gv[j].x = __ldg(p);
+                            if (t + 1 < A.T) gv[j].y = __ldg(p + 1);
+                            if (t + 2 < A.T) gv[j].z = __ldg(p + 2);
+                            if (t + 3 < A.T) gv[j].w = __ldg(p + 3);
+                        }
+                    }
+                }
+            };
+            float sum[Tile::kCols];
+#pragma unroll
+            for (int k = 0; k < Tile::kCols; ++k) sum[k] = 0.0f;
+            const auto take = [&] {
+                if (!__all_sync(0xffffffffu, mbar_wait_bounded(made + slot, again, kWgWaitLimit))) {
+                    fine = false;
+                    return;
+                }
+                tensor_fence_after();
+                if (sums_here) {
+                    constexpr int kPiece = 16;
+#pragma unroll
+                    for (int c = 0; c < Tile::kCols; c += kPiece) {
+                        float v[kPiece];
+                        tensor_read(v, at + slot * NT + c);
+#pragma unroll
+                        for (int k = 0; k < kPiece; ++k) sum[c + k] += v[k];
+                    }
+                }
+                tensor_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if (CG == 2) mbar_arrive_at(taken + slot, 0);
+                    else mbar_arrive(taken + slot);
+                }
+                if ((slot ^= 1) == 0) again ^= 1;
+            };
+            load();
+            int64_t groups = 0;        // sums that have been taken
+            for (int64_t k = k0; k < k1; ++k) {
+                if (!__all_sync(0xffffffffu, mbar_wait_bounded(empty + s, turn ^ 1, kWgWaitLimit))) { fine = false; break; }
+                uint4 lo, hi;
+                wg_expand(raw, byte, lo, hi);
+                unsigned char *a = ato + s * Tile::kStage, *b = bto + s * Tile::kStage;
+                *(uint4 *)(a + (((2 * au) ^ arow) & 7) * 16) = lo;
+                *(uint4 *)(a + (((2 * au + 1) ^ arow) & 7) * 16) = hi;
+#pragma unroll
+                for (int j = 0; j < Tile::kItems; ++j) {
+                    if (!has_b) continue;
+                    const float4 v = gv[j];
+                    const float4 r = make_float4(v.x - cut(v.x), v.y - cut(v.y), v.z - cut(v.z), v.w - cut(v.w));
+                    *(uint2 *)(b + j * 1024) = make_uint2(upper(v.x, v.y), upper(v.z, v.w));
+                    *(uint2 *)(b + Tile::kB + j * 1024) = make_uint2(upper(r.x, r.y), upper(r.z, r.w));
+                    *(uint2 *)(b + 2 * Tile::kB + j * 1024) =
+                        make_uint2(upper(r.x - cut(r.x), r.y - cut(r.y)), upper(r.z - cut(r.z), r.w - cut(r.w)));
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) {
+                    if (CG == 2) mbar_arrive_at(full + s, 0);
+                    else mbar_arrive(full + s);
+                }
+                if (++s == S) { s = 0; turn ^= 1; }
+                if (k + 1 < k1) {
+                    ua.next(A.U);
+                    ub.next(A.U);
+                    load();
+                }
+                // the sum before the one whose last block this is: its products are done by now, or nearly so
+                const int64_t done = k - k0 + 1;
+                if (done % kSteps == 0 && done / kSteps >= 2) {
+                    take();
+                    ++groups;
+                    if (!fine) break;
+                }
+            }
+            for (const int64_t all = (k1 - k0 + kSteps - 1) / kSteps; fine && groups < all; ++groups) take();
+            if (fine && sums_here) {
+                // the part of this share and tile: [column][row]
+                float *out = A.part + (share + tile) * (int64_t)(128 * CG * NT) + (int64_t)((warp >> 2) * Tile::kCols) * (128 * CG) + rank * 128 + (warp & 3) * 32 + lane;
+#pragma unroll
+                for (int k = 0; k < Tile::kCols; ++k) out[k * (128 * CG)] = sum[k];
+            }
+            w += k1 - k0;
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
+    }
+    if (warp == 16 && lane == 0 && rank == 0) {
+        constexpr uint32_t kShape = product_shape_bf16(128 * CG, NT);
+        int s = 0, turn = 0, slot = 0, again = 0;
+        for (int64_t w = from; fine && w < to;) {
+            const int64_t k0 = w % A.blocks, n = to - w < A.blocks - k0 ? to - w : A.blocks - k0;
+            for (int64_t k = 0; k < n; ++k) {
+                const bool first = k % kSteps == 0;
+                if (first && !mbar_wait_bounded(taken + slot, again ^ 1, kWgWaitLimit)) { fine = false; break; }
+                if (!mbar_wait_bounded(full + s, turn, kWgWaitLimit)) { fine = false; break; }
+                tensor_fence_after();
+                const unsigned a0 = smem_u32(smem + s * Tile::kStage), b0 = a0 + Tile::kA;
+                const uint64_t a = desc_rows(a0);
+                // the small parts first: what they lose to the sum's size is less while it is small
+#pragma unroll
+                for (int part = 2; part >= 0; --part) {
+                    const uint64_t b = desc_rows(b0 + part * Tile::kB);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) product<CG>(acc + slot * NT, a + 2 * j, b + 2 * j, kShape, !(first && part == 2 && j == 0));
+                }
+                product_commit<CG>(empty + s);
+                if (++s == S) { s = 0; turn ^= 1; }
+                if ((k + 1) % kSteps == 0 || k + 1 == n) {
+                    product_commit<CG>(made + slot);
+                    if ((slot ^= 1) == 0) again ^= 1;
+                }
+            }
+            w += n;
+        }
+        product_commit<CG>(&last);
+    }
+    // all products have read their operands, and told so, before a CTA leaves
+    if (warp == 16 && lane == 0 && !mbar_wait_bounded(&last, 0, kWgWaitLimit)) fine = false;
+    __syncwarp();
+    if (!fine) atomicExch(A.status, kStatusWeightTimeout);
+    tensor_fence_before();
+    __syncthreads();
+    if (CG == 2) cluster_wait_all();
+    if (warp == 16) {
+        tensor_fence_after();
+        tensor_free<CG>(acc, Tile::kMem);
+    }
+}
+
+// The shares' parts of each output, in order.
+template <int CG, int NT>
+__global__ void __launch_bounds__(256) weight_sum_kernel(float *out, const WgArgs A)
+{
+    constexpr int R = 128 * CG;
+    const int64_t tile = blockIdx.x, ti = tile / A.tiles_o, to = tile - ti * A.tiles_o;
+    const int row = blockIdx.z * 128 + threadIdx.x % 128, col = blockIdx.y * 2 + threadIdx.x / 128;
+    const int64_t i = ti * R + row;
+    // share p begins at work * p / shares: the one that has a block is the last to begin before or at it
+    const int64_t first = ((tile * A.blocks + 1) * A.shares - 1) / A.work, last = ((tile + 1) * A.blocks * A.shares - 1) / A.work;
+    const int64_t o = to * NT + col;
+    if (i >= A.I || o >= A.O) return;
+    const float *p = A.part + (first + tile) * (int64_t)(R * NT) + (int64_t)col * R + row;
+    double sum = 0.0;
+#pragma unroll 4
+    for (int64_t s = first; s <= last; ++s, p += R * NT) sum += (double)__ldg(p);
+    out[o * A.I + i] = (float)sum;
+}
+
+// ------------------------------------------------------------------------------------------------ host side
+struct WgPlan {
+    int cg, nt;
+    int64_t tiles, tiles_o, blocks, shares;
+    int64_t bytes;
+};
+
+static WgPlan wg_plan(int64_t N, int64_t O, int64_t I, int64_t T)
+{
+    WgPlan p;
+    // a pair's tile of 256 outputs where there are more than 128; else the smallest tile that has them all
+    p.cg = O > 128 ? 2 : 1;
+    p.nt = O > 128 ? 256 : O > 64 ? 128 : O > 32 ? 64 : O > 16 ? 32 : 16;
+    p.tiles_o = ceil_div(O, p.nt);
+    p.tiles = p.tiles_o * ceil_div(I, 128 * p.cg);
+    p.blocks = ceil_div(N * ceil_div(T, 16), 4);
+    // a share has four blocks at least: less is not worth its part of the sum
+    const int64_t most = sm_count() / p.cg, work = p.tiles * p.blocks;
+    p.shares = std::max<int64_t>(1, std::min(most, ceil_div(work, 4)));
+    p.bytes = (p.tiles + p.shares) * (int64_t)(128 * p.cg * p.nt) * 4;
+    return p;
+}
+
+static int wg_check(const char *op, int64_t N, int64_t O, int64_t I, int64_t T)
+{
+    SB200_REQUIRE(N >= 0 && O >= 0 && I >= 0 && T >= 0, "%s: negative size", op);
+    const int64_t most = (int64_t)1 << 31;
+    SB200_REQUIRE(N < most && O <= (int64_t)1 << 22 && I < most && T < most, "%s: sizes are too large", op);
+    SB200_REQUIRE(N * ceil_div(T, 16) < most && (O >> 7) * (I >> 7) < (int64_t)1 << 22, "%s: sizes are too large", op);
+    return SLAYER_B200_OK;
+}
+
+template <int CG, int NT, bool VEC>
+static int wg_launch(const WgArgs &A, float *out, int64_t tiles, cudaStream_t st)
+{
+    using Tile = WgTile<CG, NT>;
+    auto kern = weight_grad_kernel<CG, NT, VEC>;
+    const int rc = reserve_dynamic_smem((const void *)kern, Tile::kShared);
+    if (rc) return rc;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(A.shares * CG));
+    cfg.blockDim = dim3(kWgThreads);
+    cfg.dynamicSmemBytes = Tile::kShared;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = CG;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, kern, A);
+    const int bad = check_launch("weight_grad8 kernel launch");
+    if (bad) return bad;
+    weight_sum_kernel<CG, NT><<<dim3((unsigned)tiles, NT / 2, CG), 256, 0, st>>>(out, A);
+    return check_launch("weight_grad8 sum launch");
+}
+
+template <int CG, int NT>
+static int wg_align(const WgArgs &A, float *out, int64_t tiles, cudaStream_t st)
+{
+    return A.T % 4 == 0 && aligned16(A.g) ? wg_launch<CG, NT, true>(A, out, tiles, st) : wg_launch<CG, NT, false>(A, out, tiles, st);
+}
+
+}  // namespace sb200
+
+extern "C" int64_t slayer_b200_weight_grad8_workspace(int64_t N, int64_t O, int64_t I, int64_t T)
+{
+    using namespace sb200;
+    clear_error();
+    const int rc = wg_check("weight_grad8_workspace", N, O, I, T);
+    if (rc) return rc;
+    return N == 0 || O == 0 || I == 0 || T == 0 ? 0 : wg_plan(N, O, I, T).bytes;
+}
+
+extern "C" int slayer_b200_weight_grad8(float *out, const float *g, const int8_t *q, const uint8_t *scale, int64_t N, int64_t O, int64_t I, int64_t T,
+                                        void *workspace, void *stream)
+{
+    using namespace sb200;
+    clear_error();
+    const int rc = wg_check("weight_grad8", N, O, I, T);
+    if (rc) return rc;
+    if (O == 0 || I == 0) return SLAYER_B200_OK;
+    SB200_REQUIRE(out, "weight_grad8: null pointer");
+    const cudaStream_t st = (cudaStream_t)stream;
+    if (N == 0 || T == 0) {
+        const cudaError_t e = cudaMemsetAsync(out, 0, (size_t)(O * I) * 4, st);
+        if (e != cudaSuccess) { set_error("weight_grad8: %s", cudaGetErrorString(e)); return SLAYER_B200_ECUDA; }
+        return SLAYER_B200_OK;
+    }
+    SB200_REQUIRE(g && q && scale, "weight_grad8: null pointer");
+    SB200_REQUIRE(((uintptr_t)out & 3) == 0 && ((uintptr_t)g & 3) == 0 && aligned16(q), "weight_grad8: a pointer off its alignment");
+    SB200_REQUIRE(workspace && aligned16(workspace), "weight_grad8: the workspace must be aligned to 16 bytes");
+    int *status = device_status_word();
+    if (!status) { set_error("weight_grad8: no status word on this device"); return SLAYER_B200_ECUDA; }
+    const WgPlan p = wg_plan(N, O, I, T);
+    const int U = (int)ceil_div(T, 16);
+    const WgArgs A = {g, q, scale, (float *)workspace, status, N, O, I, T, ceil_div(T, 32), N * U, p.blocks, U, p.tiles_o, p.tiles * p.blocks, (int)p.shares};
+    switch (p.nt) {
+    case 256: return wg_align<2, 256>(A, out, p.tiles, st);
+    case 128: return wg_align<1, 128>(A, out, p.tiles, st);
+    case 64: return wg_align<1, 64>(A, out, p.tiles, st);
+    case 32: return wg_align<1, 32>(A, out, p.tiles, st);
+    default: return wg_align<1, 16>(A, out, p.tiles, st);
+    }
+}
