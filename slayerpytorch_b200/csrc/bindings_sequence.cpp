@@ -285,8 +285,9 @@ torch::Tensor weightGrad8Cuda(const torch::Tensor &grad, const torch::Tensor &q,
     sizes.front() = O;
     sizes.back() = 1;
     auto out = torch::empty(sizes, grad.options());
+    const auto g = (uintptr_t)grad.data_ptr() % 16 ? grad.clone() : grad;
     auto workspace = torch::empty({size_of(slayer_b200_weight_grad8_workspace(N, O, I, T), "weightGrad")}, grad.options().dtype(torch::kUInt8));
-    check_rc(slayer_b200_weight_grad8(out.data_ptr<float>(), grad.data_ptr<float>(), q.data_ptr<int8_t>(), scale.data_ptr<uint8_t>(), N, O, I, T,
+    check_rc(slayer_b200_weight_grad8(out.data_ptr<float>(), g.data_ptr<float>(), q.data_ptr<int8_t>(), scale.data_ptr<uint8_t>(), N, O, I, T,
                                       workspace.data_ptr(), current_stream()),
              "weightGrad");
     return out;

@@ -3,8 +3,8 @@
 // as products of bfloat16 tiles on the tensor cores.  q 2^e is a bfloat16 as it is; g, a float32, is the sum of three: its upper 8 bits, the
 // next 8 and the last 8, cut off and not rounded, so that the three parts are g exactly.  Three products, summed in float32, have the
 // precision of float32 products.  Both operands have time as their summation index and next to each other in memory, as the tensor cores
-// like it, but neither is in a form that they read: 16 warps load tiles, two or three steps ahead of their use, take them apart in registers
-// and write them to shared memory as 128-byte rows; one thread issues the products.
+// like it, but neither is in a form that they read: 16 warps fetch tiles (16-byte copies to shared memory that nobody waits for, two blocks
+// ahead), take them apart in registers and write them to shared memory again as 128-byte rows; one thread issues the products.
 //
 // The tensor core cuts sums off where it adds: sums of kSteps blocks of 64 steps are made there, and added up in registers, rounded.
 //
@@ -23,16 +23,19 @@ constexpr int kStatusWeightTimeout = 0x5104;
 constexpr int kWgWorkers = 512, kWgThreads = kWgWorkers + 128;
 constexpr int kSteps = 2;        // blocks of 64 steps in a sum of the tensor core
 
-template <int CG, int NT>
+template <int CG, int NT, bool VEC>
 struct WgTile {
     static constexpr int NB = NT / CG;                      // columns (of g) that a CTA loads
     static constexpr int kA = 128 * 128, kB = NB * 128;     // bytes of a block of 64 steps: x, and one part of g
     static constexpr int kStage = kA + 3 * kB;
-    static constexpr int kStages = 3 * kStage > 160 * 1024 ? 3 : (200 * 1024 / kStage < 6 ? 200 * 1024 / kStage : 6);
     static constexpr int kCols = NT >= 64 ? NT / 4 : 16;    // of a warp's sums
     static constexpr int kItems = NB >= 32 ? NB / 32 : 1;   // float4 of g a thread has of a block
-    static constexpr uint32_t kMem = NT < 16 ? 32 : 2 * NT;
-    static constexpr size_t kShared = kStages * kStage + 1024;
+    static constexpr uint32_t kMem = 2 * NT;
+    // as fetched: a thread's 16 bytes of x, its float4s of g, and those after them
+    static constexpr int kRaw = (1 + kItems) * kWgWorkers * 16 + (VEC ? 0 : kItems * kWgWorkers / 4 * 16);
+    static constexpr int kStages = (225 * 1024 - 2 * kRaw) / kStage < 4 ? (225 * 1024 - 2 * kRaw) / kStage : 4;
+    static constexpr size_t kShared = kStages * kStage + 2 * kRaw + 1024;
+    static_assert(kStages >= 2 && kShared <= 226 * 1024, "shared memory");
 };
 
 struct WgArgs {
@@ -41,23 +44,20 @@ struct WgArgs {
     const uint8_t *scale;
     float *part;
     int *status;
-    int64_t N, O, I, T, G;
-    int64_t units, blocks;       // 16 steps of a sample; 4 of those
-    int U;                       // units of a sample
+    int64_t N, O, I, T, G, g_size;
+    int units, blocks, U;        // 16 steps of a sample; 4 of those; units of a sample
     int64_t tiles_o, work;       // tiles next to each other share their rows; tiles x blocks
     int shares;
 };
 
-// First of the 16-step units that a thread loads, and the next ones, four further on.
+// A 16-step unit that a thread has, and the ones four further on.
 struct WgUnit {
-    int64_t unit;
-    int64_t n;
-    int t16;
-    __device__ __forceinline__ void start(int64_t u, int U)
+    int unit, n, t16;
+    __device__ __forceinline__ void start(int u, int U)
     {
         unit = u;
         n = u / U;
-        t16 = (int)(u - n * U);
+        t16 = u - n * U;
     }
     __device__ __forceinline__ void next(int U)
     {
@@ -74,31 +74,65 @@ struct WgUnit {
 __device__ __forceinline__ uint32_t upper(float a, float b) { return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632); }
 __device__ __forceinline__ float cut(float a) { return __uint_as_float(__float_as_uint(a) & 0xffff0000u); }
 
+// 16 bytes on their way to shared memory, zeros behind the first `bytes`
+__device__ __forceinline__ void wg_copy(void *to, const void *from, int bytes)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void wg_copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void wg_copies_wait() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
+__device__ __forceinline__ void wg_copies_wait_all() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+
+// the four of a's and b's eight that begin `skew` behind a's first, zeros behind the first `left`
+__device__ __forceinline__ float4 wg_shift(float4 a, float4 b, int skew, int left)
+{
+    const bool two = skew & 2, one = skew & 1;
+    const float v0 = two ? a.z : a.x, v1 = two ? a.w : a.y, v2 = two ? b.x : a.z, v3 = two ? b.y : a.w, v4 = two ? b.z : b.x;
+    return make_float4(left > 0 ? (one ? v1 : v0) : 0.0f, left > 1 ? (one ? v2 : v1) : 0.0f, left > 2 ? (one ? v3 : v2) : 0.0f,
+                       left > 3 ? (one ? v4 : v3) : 0.0f);
+}
+
+// two floats at once: a b + c
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
+{
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+        "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\t"
+        "mov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+
+// what is left of two floats without their upper 16 bits
+__device__ __forceinline__ float2 rest2(float2 v) { return fma2(make_float2(cut(v.x), cut(v.y)), make_float2(-1.0f, -1.0f), v); }
+
 // 16 whole numbers times a power of two, as bfloat16
 __device__ __forceinline__ void wg_expand(uint4 raw, unsigned byte, uint4 &lo, uint4 &hi)
 {
+    constexpr float kBias = 8388608.0f + 128.0f;
     const uint32_t w[4] = {raw.x ^ 0x80808080u, raw.y ^ 0x80808080u, raw.z ^ 0x80808080u, raw.w ^ 0x80808080u};     // q + 128
-    const float s = __uint_as_float(byte << 23);
-    uint32_t out[8];
     uint32_t none = 0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        float f[4];
+    for (int k = 0; k < 4; ++k) none |= (w[k] - 0x01010101u) & ~w[k] & 0x80808080u;      // a byte of 0: q is -128, what was not finite
+    // 2^23 + q + 128 as the float that ends in that byte, times the scale, minus (2^23 + 128) times it: exact, unless that is too large
+    const float s = __uint_as_float(byte << 23);
+    uint32_t out[8];
+    if (!none && byte < 220) {
+        const float2 s2 = make_float2(s, s), c2 = make_float2(-kBias * s, -kBias * s);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) f[j] = (__uint_as_float(__byte_perm(w[k], 0x4b000000u, 0x7540 | j)) - 8388736.0f) * s;     // 2^23 + q + 128
-        out[2 * k] = upper(f[0], f[1]);
-        out[2 * k + 1] = upper(f[2], f[3]);
-        none |= (w[k] - 0x01010101u) & ~w[k] & 0x80808080u;       // a byte of 0: -128, which stands for what is not finite
-    }
-    if (none) {
+        for (int k = 0; k < 8; ++k) {
+            const float2 v = make_float2(__uint_as_float(__byte_perm(w[k / 2], 0x4b000000u, 0x7540 | (k & 1) * 2)),
+                                         __uint_as_float(__byte_perm(w[k / 2], 0x4b000000u, 0x7541 | (k & 1) * 2)));
+            const float2 f = fma2(v, s2, c2);
+            out[k] = upper(f.x, f.y);
+        }
+    } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (((w[k] >> (8 * j)) & 0xff) == 0) {
-                    uint32_t &two = out[2 * k + j / 2];
-                    two = j & 1 ? (two & 0xffffu) | 0x7fc00000u : (two & 0xffff0000u) | 0x7fc0u;
-                }
+        for (int k = 0; k < 8; ++k) {
+            const int q0 = (int)((w[k / 2] >> ((k & 1) * 16)) & 0xff) - 128, q1 = (int)((w[k / 2] >> ((k & 1) * 16 + 8)) & 0xff) - 128;
+            out[k] = upper(q0 == -128 ? __uint_as_float(0x7fc00000u) : (float)q0 * s, q1 == -128 ? __uint_as_float(0x7fc00000u) : (float)q1 * s);
+        }
     }
     lo = make_uint4(out[0], out[1], out[2], out[3]);
     hi = make_uint4(out[4], out[5], out[6], out[7]);
@@ -107,8 +141,8 @@ __device__ __forceinline__ void wg_expand(uint4 raw, unsigned byte, uint4 &lo, u
 template <int CG, int NT, bool VEC>
 __global__ void __launch_bounds__(kWgThreads, 1) weight_grad_kernel(const __grid_constant__ WgArgs A)
 {
-    using Tile = WgTile<CG, NT>;
-    constexpr int S = Tile::kStages;
+    using Tile = WgTile<CG, NT, VEC>;
+    constexpr int S = Tile::kStages, kItems = Tile::kItems;
     extern __shared__ unsigned char smem_raw[];
     unsigned char *smem = (unsigned char *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     __shared__ uint64_t full[S], empty[S], made[2], taken[2], last;
@@ -144,47 +178,79 @@ __global__ void __launch_bounds__(kWgThreads, 1) weight_grad_kernel(const __grid
         const int arow = warp * 8 + (lane >> 2), au = lane & 3, quarter = lane & 3, bu = warp & 3;
         const int brow = (warp >> 2) * (Tile::NB >= 32 ? Tile::NB / 4 : 8) + 2 * ((lane >> 2) & 3) + (lane >> 4);
         const bool has_b = Tile::NB >= 32 || (warp >> 2) * 8 < Tile::NB;
-        const int64_t rows = A.N * A.I;
-        unsigned char *const ato = smem + arow * 128;
-        unsigned char *const bto = smem + Tile::kA + brow * 128 + (((2 * bu + (quarter >> 1)) ^ (brow & 7)) * 16) + (quarter & 1) * 8;
         const bool sums_here = (warp >> 2) * Tile::kCols < NT;
         const uint32_t at = acc + ((uint32_t)((warp & 3) * 32) << 16) + (warp >> 2) * Tile::kCols;
-        int s = 0, turn = 0, slot = 0, again = 0;
-        for (int64_t w = from; fine && w < to;) {
-            const int64_t tile = w / A.blocks, k0 = w - tile * A.blocks, k1 = k0 + (to - w < A.blocks - k0 ? to - w : A.blocks - k0);
-            const int64_t ti = tile / A.tiles_o, i0 = (ti * CG + rank) * 128, o0 = (tile - ti * A.tiles_o) * NT + rank * Tile::NB;
-            const bool arow_there = i0 + arow < A.I;
-            WgUnit ua, ub;
-            ua.start(k0 * 4 + au, A.U);
-            ub.start(k0 * 4 + bu, A.U);
-            uint4 raw;
-            unsigned byte;
-            float4 gv[Tile::kItems];
-            const auto load = [&] {
-                raw = make_uint4(0, 0, 0, 0);
-                byte = 127;
-                if (arow_there && ua.unit < A.units) {
-                    const int64_t row = ua.n * A.I + i0 + arow;
-                    raw = __ldg((const uint4 *)(A.q + row * (A.G * 32) + ua.t16 * 16));
-                    byte = __ldg(A.scale + (int64_t)(ua.t16 >> 1) * rows + row);
+        // what a thread has fetched lies where nobody else (VEC), or nobody else of another warp, reads it
+        unsigned char *const raw = smem + S * Tile::kStage + tid * 16;
+        // what comes after them, where the next thread does not have it: for one of the four threads of a row's unit
+        const unsigned beyond = (1 + kItems) * 8192 - tid * 16 + (tid >> 2) * 16;
+
+        // The block after next, on its way.  Rows behind the last are the last once more: their results are nobody's.  Steps behind the last are zeros.
+        int64_t ahead = from;
+        int k_ahead = A.blocks;
+        const int8_t *aq = A.q;
+        const uint8_t *as = A.scale;
+        const float *bg = A.g;
+        int b_last = 0;                 // of this thread's kItems rows, 8 apart
+        WgUnit ua, ub;
+        unsigned scale_0 = 127, scale_1 = 127;
+        const int64_t a_stride = A.I * A.G * 32, b_stride = A.O * A.T, rows = A.N * A.I;
+        const int far = (int)A.T * 8;
+        const auto fetch = [&](int slot) {
+            scale_0 = scale_1;
+            if (ahead < to) {
+                if (k_ahead == A.blocks) {
+                    const int64_t tile = ahead / A.blocks, ti = tile / A.tiles_o;
+                    k_ahead = (int)(ahead - tile * A.blocks);
+                    const int64_t i = min((ti * CG + rank) * 128 + arow, A.I - 1), o = (tile - ti * A.tiles_o) * NT + rank * Tile::NB + brow;
+                    aq = A.q + i * (A.G * 32);
+                    as = A.scale + i;
+                    bg = A.g + min(o, A.O - 1) * A.T + quarter * 4;
+                    b_last = o >= A.O ? 0 : (int)min((A.O - 1 - o) / 8, (int64_t)kItems - 1);
+                    ua.start(k_ahead * 4 + au, A.U);
+                    ub.start(k_ahead * 4 + bu, A.U);
                 }
-                const int64_t t = (int64_t)ub.t16 * 16 + quarter * 4;
-                const float *p = A.g + (ub.n * A.O + o0 + brow) * A.T + t;
+                unsigned char *const into = raw + slot * Tile::kRaw;
+                const bool a = ua.unit < A.units;
+                wg_copy(into, a ? aq + ua.n * a_stride + ua.t16 * 16 : A.q, a ? 16 : 0);
+                scale_1 = a ? __ldg(as + (ua.t16 >> 1) * rows + ua.n * A.I) : 127u;
+                if (has_b) {
+                    const int t = ub.t16 * 16 + quarter * 4;
+                    const bool b = ub.unit < A.units && t < A.T;
+                    const int apart = b ? far : 0;
+                    const float *p = b ? bg + ub.n * b_stride + ub.t16 * 16 : A.g;
+                    if (VEC) {
 #pragma unroll
-                for (int j = 0; j < Tile::kItems; ++j, p += 8 * A.T) {
-                    gv[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    if (has_b && ub.unit < A.units && o0 + brow + 8 * j < A.O) {
-                        if (VEC) {
-                            if (t < A.T) gv[j] = __ldg((const float4 *)p);
-                        } else {
-                            if (t < A.T) gv[j].x = __ldg(p);
-                            if (t + 1 < A.T) gv[j].y = __ldg(p + 1);
-                            if (t + 2 < A.T) gv[j].z = __ldg(p + 2);
-                            if (t + 3 < A.T) gv[j].w = __ldg(p + 3);
+                        for (int j = 0; j < kItems; ++j) wg_copy(into + (1 + j) * 8192, p + (int64_t)min(j, b_last) * apart, b ? 16 : 0);
+                    } else {
+                        // The 16 bytes that the four steps begin in, and, where the thread beside has no more steps of the row or a quarter is the
+                        // unit's last, the 16 after them.  The tensor may end inside.
+                        p -= (p - A.g) & 3;
+                        const bool more = b && (quarter == 3 || t + 4 >= A.T);
+                        const bool end = ub.n == A.N - 1;
+#pragma unroll
+                        for (int j = 0; j < kItems; ++j) {
+                            const float *v = p + (int64_t)min(j, b_last) * apart;
+                            const int64_t there = end ? A.g_size - (v - A.g) : 8;
+                            wg_copy(into + (1 + j) * 8192, v, b ? (there < 4 ? (int)there * 4 : 16) : 0);
+                            if (more) wg_copy(into + beyond + j * 2048, there > 4 ? v + 4 : v, there > 4 ? (there < 8 ? (int)there * 4 - 16 : 16) : 0);
                         }
                     }
                 }
-            };
+                ++ahead;
+                ++k_ahead;
+                ua.next(A.U);
+                ub.next(A.U);
+            }
+            wg_copies_commit();
+        };
+        int s = 0, turn = 0, slot = 0, again = 0, from_slot = 0;
+        fetch(0);
+        fetch(1);
+        WgUnit uc;        // of g in the block that is worked on: what lies behind T is not g's
+        for (int64_t w = from; fine && w < to;) {
+            const int64_t tile = w / A.blocks;
+            const int k0 = (int)(w - tile * A.blocks), k1 = (int)min((int64_t)A.blocks, k0 + (to - w));
             float sum[Tile::kCols];
 #pragma unroll
             for (int k = 0; k < Tile::kCols; ++k) sum[k] = 0.0f;
@@ -212,24 +278,40 @@ __global__ void __launch_bounds__(kWgThreads, 1) weight_grad_kernel(const __grid
                 }
                 if ((slot ^= 1) == 0) again ^= 1;
             };
-            load();
-            int64_t groups = 0;        // sums that have been taken
-            for (int64_t k = k0; k < k1; ++k) {
+            if (!VEC) uc.start(k0 * 4 + bu, A.U);
+            const unsigned o = (unsigned)min((tile % A.tiles_o) * NT + rank * Tile::NB + brow, A.O - 1);
+            int groups = 0;        // sums that have been taken
+            for (int k = k0; k < k1; ++k) {
+                wg_copies_wait();
+                if (!VEC) __syncwarp();
                 if (!__all_sync(0xffffffffu, mbar_wait_bounded(empty + s, turn ^ 1, kWgWaitLimit))) { fine = false; break; }
-                uint4 lo, hi;
-                wg_expand(raw, byte, lo, hi);
-                unsigned char *a = ato + s * Tile::kStage, *b = bto + s * Tile::kStage;
-                *(uint4 *)(a + (((2 * au) ^ arow) & 7) * 16) = lo;
-                *(uint4 *)(a + (((2 * au + 1) ^ arow) & 7) * 16) = hi;
+                const unsigned char *const in = raw + from_slot * Tile::kRaw;
+                unsigned char *const a = smem + s * Tile::kStage + arow * 128;
+                unsigned char *const b = smem + s * Tile::kStage + Tile::kA + brow * 128 + (((2 * bu + (quarter >> 1)) ^ (brow & 7)) * 16) + (quarter & 1) * 8;
+                {
+                    uint4 lo, hi;
+                    wg_expand(*(const uint4 *)in, scale_0, lo, hi);
+                    *(uint4 *)(a + (((2 * au) ^ arow) & 7) * 16) = lo;
+                    *(uint4 *)(a + (((2 * au + 1) ^ arow) & 7) * 16) = hi;
+                }
+                if (has_b) {
+                    int skew = 0, left = 4;
+                    bool more = false;
+                    if (!VEC) {
+                        const int t = uc.t16 * 16 + quarter * 4;
+                        skew = (int)(((unsigned)uc.n * (unsigned)A.O + o) * (unsigned)A.T & 3u);        // (8 rows on it is the same)
+                        left = uc.unit < A.units ? (int)min(A.T - t, (int64_t)4) : 0;
+                        more = quarter == 3 || t + 4 >= A.T;
+                    }
 #pragma unroll
-                for (int j = 0; j < Tile::kItems; ++j) {
-                    if (!has_b) continue;
-                    const float4 v = gv[j];
-                    const float4 r = make_float4(v.x - cut(v.x), v.y - cut(v.y), v.z - cut(v.z), v.w - cut(v.w));
-                    *(uint2 *)(b + j * 1024) = make_uint2(upper(v.x, v.y), upper(v.z, v.w));
-                    *(uint2 *)(b + Tile::kB + j * 1024) = make_uint2(upper(r.x, r.y), upper(r.z, r.w));
-                    *(uint2 *)(b + 2 * Tile::kB + j * 1024) =
-                        make_uint2(upper(r.x - cut(r.x), r.y - cut(r.y)), upper(r.z - cut(r.z), r.w - cut(r.w)));
+                    for (int j = 0; j < kItems; ++j) {
+                        float4 v = *(const float4 *)(in + (1 + j) * 8192);
+                        if (!VEC) v = wg_shift(v, *(const float4 *)(in + (more ? beyond + j * 2048 : (1 + j) * 8192 + 16)), skew, left);
+                        const float2 u = rest2(make_float2(v.x, v.y)), w = rest2(make_float2(v.z, v.w)), x = rest2(u), y = rest2(w);
+                        *(uint2 *)(b + j * 1024) = make_uint2(upper(v.x, v.y), upper(v.z, v.w));
+                        *(uint2 *)(b + Tile::kB + j * 1024) = make_uint2(upper(u.x, u.y), upper(w.x, w.y));
+                        *(uint2 *)(b + 2 * Tile::kB + j * 1024) = make_uint2(upper(x.x, x.y), upper(y.x, y.y));
+                    }
                 }
                 fence_proxy_async();
                 __syncwarp();
@@ -238,20 +320,18 @@ __global__ void __launch_bounds__(kWgThreads, 1) weight_grad_kernel(const __grid
                     else mbar_arrive(full + s);
                 }
                 if (++s == S) { s = 0; turn ^= 1; }
-                if (k + 1 < k1) {
-                    ua.next(A.U);
-                    ub.next(A.U);
-                    load();
-                }
-                // the sum before the one whose last block this is: its products are done by now, or nearly so
-                const int64_t done = k - k0 + 1;
+                fetch(from_slot);
+                from_slot ^= 1;
+                if (!VEC) uc.next(A.U);
+                // the sum before the one whose last block this is: its products are done, or nearly so
+                const int done = k - k0 + 1;
                 if (done % kSteps == 0 && done / kSteps >= 2) {
                     take();
                     ++groups;
                     if (!fine) break;
                 }
             }
-            for (const int64_t all = (k1 - k0 + kSteps - 1) / kSteps; fine && groups < all; ++groups) take();
+            for (const int all = (k1 - k0 + kSteps - 1) / kSteps; fine && groups < all; ++groups) take();
             if (fine && sums_here) {
                 // the part of this share and tile: [column][row]
                 float *out = A.part + (share + tile) * (int64_t)(128 * CG * NT) + (int64_t)((warp >> 2) * Tile::kCols) * (128 * CG) + rank * 128 + (warp & 3) * 32 + lane;
@@ -260,6 +340,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) weight_grad_kernel(const __grid
             }
             w += k1 - k0;
         }
+        wg_copies_wait_all();
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
     }
@@ -267,8 +348,8 @@ __global__ void __launch_bounds__(kWgThreads, 1) weight_grad_kernel(const __grid
         constexpr uint32_t kShape = product_shape_bf16(128 * CG, NT);
         int s = 0, turn = 0, slot = 0, again = 0;
         for (int64_t w = from; fine && w < to;) {
-            const int64_t k0 = w % A.blocks, n = to - w < A.blocks - k0 ? to - w : A.blocks - k0;
-            for (int64_t k = 0; k < n; ++k) {
+            const int n = (int)min(A.blocks - w % A.blocks, to - w);
+            for (int k = 0; k < n; ++k) {
                 const bool first = k % kSteps == 0;
                 if (first && !mbar_wait_bounded(taken + slot, again ^ 1, kWgWaitLimit)) { fine = false; break; }
                 if (!mbar_wait_bounded(full + s, turn, kWgWaitLimit)) { fine = false; break; }
@@ -352,15 +433,15 @@ static int wg_check(const char *op, int64_t N, int64_t O, int64_t I, int64_t T)
 {
     SB200_REQUIRE(N >= 0 && O >= 0 && I >= 0 && T >= 0, "%s: negative size", op);
     const int64_t most = (int64_t)1 << 31;
-    SB200_REQUIRE(N < most && O <= (int64_t)1 << 22 && I < most && T < most, "%s: sizes are too large", op);
-    SB200_REQUIRE(N * ceil_div(T, 16) < most && (O >> 7) * (I >> 7) < (int64_t)1 << 22, "%s: sizes are too large", op);
+    SB200_REQUIRE(N < most && O <= (int64_t)1 << 22 && I < most && T <= (int64_t)1 << 27, "%s: sizes are too large", op);
+    SB200_REQUIRE(N * ceil_div(T, 16) < most - 64 && (O >> 7) * (I >> 7) < (int64_t)1 << 22, "%s: sizes are too large", op);
     return SLAYER_B200_OK;
 }
 
 template <int CG, int NT, bool VEC>
 static int wg_launch(const WgArgs &A, float *out, int64_t tiles, cudaStream_t st)
 {
-    using Tile = WgTile<CG, NT>;
+    using Tile = WgTile<CG, NT, VEC>;
     auto kern = weight_grad_kernel<CG, NT, VEC>;
     const int rc = reserve_dynamic_smem((const void *)kern, Tile::kShared);
     if (rc) return rc;
@@ -385,7 +466,7 @@ static int wg_launch(const WgArgs &A, float *out, int64_t tiles, cudaStream_t st
 template <int CG, int NT>
 static int wg_align(const WgArgs &A, float *out, int64_t tiles, cudaStream_t st)
 {
-    return A.T % 4 == 0 && aligned16(A.g) ? wg_launch<CG, NT, true>(A, out, tiles, st) : wg_launch<CG, NT, false>(A, out, tiles, st);
+    return A.T % 4 == 0 ? wg_launch<CG, NT, true>(A, out, tiles, st) : wg_launch<CG, NT, false>(A, out, tiles, st);
 }
 
 }  // namespace sb200
@@ -415,13 +496,13 @@ extern "C" int slayer_b200_weight_grad8(float *out, const float *g, const int8_t
         return SLAYER_B200_OK;
     }
     SB200_REQUIRE(g && q && scale, "weight_grad8: null pointer");
-    SB200_REQUIRE(((uintptr_t)out & 3) == 0 && ((uintptr_t)g & 3) == 0 && aligned16(q), "weight_grad8: a pointer off its alignment");
+    SB200_REQUIRE(((uintptr_t)out & 3) == 0 && aligned16(g) && aligned16(q), "weight_grad8: a pointer off its alignment");
     SB200_REQUIRE(workspace && aligned16(workspace), "weight_grad8: the workspace must be aligned to 16 bytes");
     int *status = device_status_word();
     if (!status) { set_error("weight_grad8: no status word on this device"); return SLAYER_B200_ECUDA; }
     const WgPlan p = wg_plan(N, O, I, T);
     const int U = (int)ceil_div(T, 16);
-    const WgArgs A = {g, q, scale, (float *)workspace, status, N, O, I, T, ceil_div(T, 32), N * U, p.blocks, U, p.tiles_o, p.tiles * p.blocks, (int)p.shares};
+    const WgArgs A = {g, q, scale, (float *)workspace, status, N, O, I, T, ceil_div(T, 32), N * O * T, (int)(N * U), (int)p.blocks, U, p.tiles_o, p.tiles * p.blocks, (int)p.shares};
     switch (p.nt) {
     case 256: return wg_align<2, 256>(A, out, p.tiles, st);
     case 128: return wg_align<1, 128>(A, out, p.tiles, st);
