@@ -21,7 +21,7 @@ namespace sb200 {
 constexpr int kWgWaitLimit = 1 << 22;
 constexpr int kStatusWeightTimeout = 0x5104;
 constexpr int kWgWorkers = 512, kWgThreads = kWgWorkers + 128;
-constexpr int kSteps = 2;        // blocks of 64 steps in a sum of the tensor core
+constexpr int kSteps = 4;        // blocks of 64 steps in a sum of the tensor core
 
 template <int CG, int NT, bool VEC>
 struct WgTile {
@@ -59,14 +59,17 @@ struct WgUnit {
         n = u / U;
         t16 = u - n * U;
     }
-    __device__ __forceinline__ void next(int U)
+    // true: of another sample
+    __device__ __forceinline__ bool next(int U)
     {
         unit += 4;
         t16 += 4;
-        while (t16 >= U) {
+        if (t16 < U) return false;
+        do {
             t16 -= U;
             ++n;
-        }
+        } while (t16 >= U);
+        return true;
     }
 };
 
@@ -104,6 +107,17 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
     return d;
 }
 
+__device__ __forceinline__ float2 add2(float2 a, float2 b)
+{
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\t"
+        "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "add.rn.f32x2 d, a, b;\n\t"
+        "mov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
 // what is left of two floats without their upper 16 bits
 __device__ __forceinline__ float2 rest2(float2 v) { return fma2(make_float2(cut(v.x), cut(v.y)), make_float2(-1.0f, -1.0f), v); }
 
@@ -114,11 +128,11 @@ __device__ __forceinline__ void wg_expand(uint4 raw, unsigned byte, uint4 &lo, u
     const uint32_t w[4] = {raw.x ^ 0x80808080u, raw.y ^ 0x80808080u, raw.z ^ 0x80808080u, raw.w ^ 0x80808080u};     // q + 128
     uint32_t none = 0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) none |= (w[k] - 0x01010101u) & ~w[k] & 0x80808080u;      // a byte of 0: q is -128, what was not finite
+    for (int k = 0; k < 4; ++k) none |= (w[k] - 0x01010101u) & ~w[k];      // a byte of 0: q is -128, what was not finite
     // 2^23 + q + 128 as the float that ends in that byte, times the scale, minus (2^23 + 128) times it: exact, unless that is too large
     const float s = __uint_as_float(byte << 23);
     uint32_t out[8];
-    if (!none && byte < 220) {
+    if (!(none & 0x80808080u) && byte < 220) {
         const float2 s2 = make_float2(s, s), c2 = make_float2(-kBias * s, -kBias * s);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
@@ -187,60 +201,70 @@ __global__ void __launch_bounds__(kWgThreads, 1) weight_grad_kernel(const __grid
 
         // The block after next, on its way.  Rows behind the last are the last once more: their results are nobody's.  Steps behind the last are zeros.
         int64_t ahead = from;
-        int k_ahead = A.blocks;
-        const int8_t *aq = A.q;
+        int tile_left = 0;              // blocks
+        const int8_t *aq = A.q;         // this thread's unit
         const uint8_t *as = A.scale;
         const float *bg = A.g;
-        int b_last = 0;                 // of this thread's kItems rows, 8 apart
+        int b_far[kItems];              // its rows of g from the first one on
         WgUnit ua, ub;
         unsigned scale_0 = 127, scale_1 = 127;
-        const int64_t a_stride = A.I * A.G * 32, b_stride = A.O * A.T, rows = A.N * A.I;
-        const int far = (int)A.T * 8;
+        int64_t i = 0, o = 0;
+        const auto find_a = [&] {
+            aq = A.q + ((int64_t)ua.n * A.I + i) * (A.G * 32) + ua.t16 * 16;
+            as = A.scale + ((ua.t16 >> 1) * A.N + ua.n) * A.I + i;
+        };
+        const auto find_b = [&] { bg = A.g + ((int64_t)ub.n * A.O + o) * A.T + ub.t16 * 16 + quarter * 4; };
+        const int64_t a_groups = 2 * A.N * A.I;
         const auto fetch = [&](int slot) {
             scale_0 = scale_1;
             if (ahead < to) {
-                if (k_ahead == A.blocks) {
+                if (tile_left == 0) {
                     const int64_t tile = ahead / A.blocks, ti = tile / A.tiles_o;
-                    k_ahead = (int)(ahead - tile * A.blocks);
-                    const int64_t i = min((ti * CG + rank) * 128 + arow, A.I - 1), o = (tile - ti * A.tiles_o) * NT + rank * Tile::NB + brow;
-                    aq = A.q + i * (A.G * 32);
-                    as = A.scale + i;
-                    bg = A.g + min(o, A.O - 1) * A.T + quarter * 4;
-                    b_last = o >= A.O ? 0 : (int)min((A.O - 1 - o) / 8, (int64_t)kItems - 1);
-                    ua.start(k_ahead * 4 + au, A.U);
-                    ub.start(k_ahead * 4 + bu, A.U);
+                    const int k = (int)(ahead - tile * A.blocks);
+                    tile_left = A.blocks - k;
+                    i = min((ti * CG + rank) * 128 + arow, A.I - 1);
+                    o = min((tile - ti * A.tiles_o) * NT + rank * Tile::NB + brow, A.O - 1);
+                    const int last = (int)min((A.O - 1 - o) / 8, (int64_t)kItems - 1);
+#pragma unroll
+                    for (int j = 0; j < kItems; ++j) b_far[j] = min(j, last) * 8 * (int)A.T;
+                    ua.start(k * 4 + au, A.U);
+                    ub.start(k * 4 + bu, A.U);
+                    find_a();
+                    find_b();
                 }
                 unsigned char *const into = raw + slot * Tile::kRaw;
                 const bool a = ua.unit < A.units;
-                wg_copy(into, a ? aq + ua.n * a_stride + ua.t16 * 16 : A.q, a ? 16 : 0);
-                scale_1 = a ? __ldg(as + (ua.t16 >> 1) * rows + ua.n * A.I) : 127u;
+                wg_copy(into, a ? aq : A.q, a ? 16 : 0);
+                if (a) scale_1 = __ldg(as);
                 if (has_b) {
                     const int t = ub.t16 * 16 + quarter * 4;
-                    const bool b = ub.unit < A.units && t < A.T;
-                    const int apart = b ? far : 0;
-                    const float *p = b ? bg + ub.n * b_stride + ub.t16 * 16 : A.g;
+                    const bool b = ub.unit < A.units && t < (int)A.T;
                     if (VEC) {
 #pragma unroll
-                        for (int j = 0; j < kItems; ++j) wg_copy(into + (1 + j) * 8192, p + (int64_t)min(j, b_last) * apart, b ? 16 : 0);
+                        for (int j = 0; j < kItems; ++j) wg_copy(into + (1 + j) * 8192, b ? bg + b_far[j] : A.g, b ? 16 : 0);
                     } else {
                         // The 16 bytes that the four steps begin in, and, where the thread beside has no more steps of the row or a quarter is the
                         // unit's last, the 16 after them.  The tensor may end inside.
-                        p -= (p - A.g) & 3;
-                        const bool more = b && (quarter == 3 || t + 4 >= A.T);
-                        const bool end = ub.n == A.N - 1;
+                        const float *const p = b ? bg - ((bg - A.g) & 3) : A.g;
+                        const bool more = b && (quarter == 3 || t + 4 >= (int)A.T);
+                        const bool end = ub.n == (int)A.N - 1;
 #pragma unroll
                         for (int j = 0; j < kItems; ++j) {
-                            const float *v = p + (int64_t)min(j, b_last) * apart;
-                            const int64_t there = end ? A.g_size - (v - A.g) : 8;
-                            wg_copy(into + (1 + j) * 8192, v, b ? (there < 4 ? (int)there * 4 : 16) : 0);
-                            if (more) wg_copy(into + beyond + j * 2048, there > 4 ? v + 4 : v, there > 4 ? (there < 8 ? (int)there * 4 - 16 : 16) : 0);
+                            const float *v = p + (b ? b_far[j] : 0);
+                            const int there = end ? (int)min(A.g_size - (v - A.g), (int64_t)8) : 8;
+                            wg_copy(into + (1 + j) * 8192, v, b ? min(there * 4, 16) : 0);
+                            if (more) wg_copy(into + beyond + j * 2048, there > 4 ? v + 4 : v, max(there * 4 - 16, 0));
                         }
                     }
                 }
                 ++ahead;
-                ++k_ahead;
-                ua.next(A.U);
-                ub.next(A.U);
+                --tile_left;
+                // the next unit: mostly the same sample's, two groups of steps on
+                aq += 64;
+                as += a_groups;
+                bg += 64;
+                if (ua.next(A.U)) find_a();
+                if (ub.next(A.U)) find_b();
             }
             wg_copies_commit();
         };
@@ -267,7 +291,11 @@ __global__ void __launch_bounds__(kWgThreads, 1) weight_grad_kernel(const __grid
                         float v[kPiece];
                         tensor_read(v, at + slot * NT + c);
 #pragma unroll
-                        for (int k = 0; k < kPiece; ++k) sum[c + k] += v[k];
+                        for (int k = 0; k < kPiece; k += 2) {
+                            const float2 two = add2(make_float2(sum[c + k], sum[c + k + 1]), make_float2(v[k], v[k + 1]));
+                            sum[c + k] = two.x;
+                            sum[c + k + 1] = two.y;
+                        }
                     }
                 }
                 tensor_fence_before();
@@ -433,7 +461,7 @@ static int wg_check(const char *op, int64_t N, int64_t O, int64_t I, int64_t T)
 {
     SB200_REQUIRE(N >= 0 && O >= 0 && I >= 0 && T >= 0, "%s: negative size", op);
     const int64_t most = (int64_t)1 << 31;
-    SB200_REQUIRE(N < most && O <= (int64_t)1 << 22 && I < most && T <= (int64_t)1 << 27, "%s: sizes are too large", op);
+    SB200_REQUIRE(N < most && O <= (int64_t)1 << 22 && I < most && T <= (int64_t)1 << 26, "%s: sizes are too large", op);
     SB200_REQUIRE(N * ceil_div(T, 16) < most - 64 && (O >> 7) * (I >> 7) < (int64_t)1 << 22, "%s: sizes are too large", op);
     return SLAYER_B200_OK;
 }
