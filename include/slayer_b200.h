@@ -426,12 +426,15 @@ int slayer_b200_leak_step(void *y, float *state, const void *x, const void *gate
  */
 int slayer_b200_compress8(int8_t *q, uint8_t *scale, const void *x, int dtype, int64_t rows, int64_t T, void *stream);
 
-/* What that stands for: out [rows, T] = q 2^e, NaN where q is -128.  It has no counterpart in the reference. */
+/*
+ * What that stands for: out [rows, T] = q 2^e, NaN where q is -128; aligned to 16 bytes.  It has no counterpart
+ * in the reference.
+ */
 int slayer_b200_restore8(void *out, const int8_t *q, const uint8_t *scale, int dtype, int64_t rows, int64_t T, void *stream);
 
 /*
  * slayer_b200_spike_grad on a membrane potential kept so: out [rows, T] =
- *   g * (scale / tau * exp(-|q 2^e - theta| / tau));   out may be g.
+ *   g * (scale / tau * exp(-|q 2^e - theta| / tau));   out may be g; both aligned to 16 bytes.
  * Surrogate gradient as src/slayer.py:858-865.
  */
 int slayer_b200_spike_grad8(float *out, const float *g, const int8_t *q, const uint8_t *scale_bytes, int64_t rows, int64_t T, float theta,

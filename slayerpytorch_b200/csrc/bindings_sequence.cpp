@@ -230,6 +230,9 @@ void check_kept(const torch::Tensor &q, const torch::Tensor &scale, at::IntArray
                 ": a checkpoint has contiguous int8 values and uint8 scales");
 }
 
+// itself, or a copy where it does not begin at 16 bytes
+torch::Tensor aligned(const torch::Tensor &x) { return (uintptr_t)x.data_ptr() % 16 ? x.clone() : x; }
+
 std::vector<torch::Tensor> compress8Cuda(const torch::Tensor &x)
 {
     TORCH_CHECK_VALUE(x.dim() >= 1, "compress: x must have a time dimension");
@@ -264,7 +267,8 @@ torch::Tensor spikeGrad8Cuda(const torch::Tensor &grad, const torch::Tensor &q, 
     check_device(grad, q, "grad", "the checkpoint");
     c10::cuda::CUDAGuard guard(grad.device());
     auto out = torch::empty_like(grad);
-    check_rc(slayer_b200_spike_grad8(out.data_ptr<float>(), grad.data_ptr<float>(), q.data_ptr<int8_t>(), scaleBytes.data_ptr<uint8_t>(),
+    const auto g = aligned(grad);
+    check_rc(slayer_b200_spike_grad8(out.data_ptr<float>(), g.data_ptr<float>(), q.data_ptr<int8_t>(), scaleBytes.data_ptr<uint8_t>(),
                                      product(grad.sizes(), 0, grad.dim() - 1), grad.size(-1), theta, tau, scale, current_stream()),
              "spikeGrad");
     return out;
@@ -285,7 +289,7 @@ torch::Tensor weightGrad8Cuda(const torch::Tensor &grad, const torch::Tensor &q,
     sizes.front() = O;
     sizes.back() = 1;
     auto out = torch::empty(sizes, grad.options());
-    const auto g = (uintptr_t)grad.data_ptr() % 16 ? grad.clone() : grad;
+    const auto g = aligned(grad);
     auto workspace = torch::empty({size_of(slayer_b200_weight_grad8_workspace(N, O, I, T), "weightGrad")}, grad.options().dtype(torch::kUInt8));
     check_rc(slayer_b200_weight_grad8(out.data_ptr<float>(), g.data_ptr<float>(), q.data_ptr<int8_t>(), scale.data_ptr<uint8_t>(), N, O, I, T,
                                       workspace.data_ptr(), current_stream()),

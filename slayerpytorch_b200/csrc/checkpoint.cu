@@ -40,48 +40,256 @@ __device__ __forceinline__ int quantise(float v, unsigned byte)
     return max(min(__float2int_rn(v * inverse), 127), -127);
 }
 
-__device__ __forceinline__ float restored(int q, unsigned byte)
+// The kernels here move bytes.  A thread has 16 bytes of the tensor at a time, and loads several of them before it uses the first.
+//
+// Rows are cut into pieces of equal size (groups of 32 steps, or 16 bytes); those of all rows are counted through, and a CTA has kBlock of them, so that
+// a piece's row is the CTA's first one or one of the next: found with 32-bit numbers.
+struct Pieces {
+    int64_t rows, T, G;
+    int64_t each, all;           // pieces of a row, of all rows
+    unsigned magic;              // 2^32 / each, rounded up: exact quotients of numbers below 4096 for each < 1024
+};
+
+template <int kBlock>
+struct Place {
+    static_assert(kBlock <= 1024, "a CTA's pieces");
+    int64_t first, row0;
+    unsigned rest0;
+    __device__ __forceinline__ Place(const Pieces &s)
+    {
+        first = (int64_t)blockIdx.x * kBlock;
+        row0 = first / s.each;
+        rest0 = (unsigned)(first - row0 * s.each);
+    }
+    // rows from the CTA's first one, and which piece of its row the CTA's local-th one is
+    __device__ __forceinline__ void operator()(const Pieces &s, unsigned local, unsigned &down, unsigned &piece) const
+    {
+        const unsigned r = rest0 + local, each = (unsigned)s.each;
+        if (each >= 1024) down = r >= each;
+        else down = each == 1 ? r : __umulhi(r, s.magic);
+        piece = r - down * each;
+    }
+};
+
+// 16 bytes a thread: kLanes of them have a group.  LINED: all rows' steps lie on 16 bytes; else they are loaded one by one (a line's other steps are in L1 by
+// then: 52 us instead of 142 with a lane for each step of a group, 64 x 2312 x 301).
+constexpr int kCompressUnroll = 4;
+template <typename E> constexpr int kCompressBlock = 256 / (32 * (int)sizeof(E) / 16) * kCompressUnroll;
+
+template <typename E, bool LINED>
+__global__ void __launch_bounds__(256)
+compress_kernel(int8_t *q, uint8_t *scale, const E *x, const Pieces s)
 {
-    return q == -128 ? __uint_as_float(0x7fc00000u) : (float)q * __uint_as_float(byte << 23);
+    constexpr int W = 16 / (int)sizeof(E), kLanes = 32 / W;
+    const Place<kCompressBlock<E>> place(s);
+    const unsigned t = (threadIdx.x % kLanes) * W, pad = (unsigned)(s.G * kGroup - s.T);
+    const E *const x0 = x + place.row0 * s.T;
+    unsigned down[kCompressUnroll], group[kCompressUnroll];
+    float v[kCompressUnroll][W];
+#pragma unroll
+    for (int u = 0; u < kCompressUnroll; ++u) {
+        const unsigned local = u * (256 / kLanes) + threadIdx.x / kLanes;
+        place(s, local, down[u], group[u]);
+        const E *p = x0 + (place.rest0 + local) * kGroup - down[u] * pad + t;
+        const unsigned at = group[u] * kGroup + t;
+        const bool there = place.first + local < s.all;
+        if (LINED) {
+            uint4 raw = make_uint4(0, 0, 0, 0);
+            if (there && at < (unsigned)s.T) raw = __ldg(reinterpret_cast<const uint4 *>(p));
+            const E *e = reinterpret_cast<const E *>(&raw);
+#pragma unroll
+            for (int j = 0; j < W; ++j) v[u][j] = as_float<E>(e[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < W; ++j) v[u][j] = there && at + j < (unsigned)s.T ? as_float<E>(__ldg(p + j)) : 0.0f;
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kCompressUnroll; ++u) {
+        const unsigned local = u * (256 / kLanes) + threadIdx.x / kLanes;
+        unsigned top = 0;
+#pragma unroll
+        for (int j = 0; j < W; ++j) top = max(top, __float_as_uint(v[u][j]) & 0x7fffffffu);
+#pragma unroll
+        for (int d = kLanes / 2; d > 0; d /= 2) top = max(top, __shfl_xor_sync(~0u, top, d));
+        unsigned byte, out[W / 4];
+        if (!__any_sync(~0u, top >= 0x7e800000u)) {
+            // whole multiples by adding 1.5 2^23, in whose last byte they are then: rounded to nearest, ties to even
+            byte = scale_byte(top);
+            const float inverse = __uint_as_float((254u - byte) << 23);
+#pragma unroll
+            for (int j = 0; j < W; j += 4) {
+                unsigned n[4];
+#pragma unroll
+                for (int l = 0; l < 4; ++l) n[l] = __float_as_uint(fmaf(v[u][j + l], inverse, 12582912.0f));
+                out[j / 4] = __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
+            }
+        } else {
+            // something large, or not finite
+            top = 0;
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                const unsigned bits = __float_as_uint(v[u][j]) & 0x7fffffffu;
+                top = max(top, bits < 0x7f800000u ? bits : 0u);
+            }
+#pragma unroll
+            for (int d = kLanes / 2; d > 0; d /= 2) top = max(top, __shfl_xor_sync(~0u, top, d));
+            byte = scale_byte(top);
+#pragma unroll
+            for (int j = 0; j < W; j += 4) {
+                out[j / 4] = 0;
+#pragma unroll
+                for (int l = 0; l < 4; ++l) out[j / 4] |= (unsigned)(quantise(v[u][j + l], byte) & 0xff) << (8 * l);
+            }
+        }
+        if (place.first + local < s.all) {
+            unsigned *to = reinterpret_cast<unsigned *>(q + (place.first + local) * kGroup + t);
+            if (W == 4) to[0] = out[0];
+            else *reinterpret_cast<uint2 *>(to) = make_uint2(out[0], out[W / 4 - 1]);
+            if (t == 0) scale[group[u] * s.rows + place.row0 + down[u]] = (uint8_t)byte;
+        }
+    }
 }
 
-// a warp per group, a lane per step
-template <typename E>
-__global__ void __launch_bounds__(256)
-compress_kernel(int8_t *q, uint8_t *scale, const E *x, int64_t groups_all, int64_t T, int64_t G)
+// 16 bytes of a tensor that is read from 8 bits: W steps of a row from t on, some of them before its first or behind its last where rows do not lie
+// on 16 bytes (not LINED).
+template <int W>
+struct Kept {
+    static constexpr int kWords = W / 4 + 1;
+    uint32_t word[kWords];
+    unsigned byte, next;         // scales of the first step's group and of the one after it
+
+    template <bool LINED>
+    __device__ __forceinline__ void load(const int8_t *q, const uint8_t *scale, const Pieces &s, int64_t row, int t)
+    {
+        const uint32_t *const p = reinterpret_cast<const uint32_t *>(q) + row * (s.G * (kGroup / 4));
+        const int last = (int)(s.G * (kGroup / 4)) - 1, at = t >> 2;
+        if (LINED && W == 8) {
+            const uint2 two = __ldg(reinterpret_cast<const uint2 *>(p + at));
+            word[0] = two.x;
+            word[1] = two.y;
+        } else {
+#pragma unroll
+            for (int k = 0; k < (LINED ? W / 4 : kWords); ++k) word[k] = __ldg(p + (LINED ? at + k : min(max(at + k, 0), last)));
+        }
+        const int group = max(t, 0) >> 5;
+        byte = __ldg(scale + group * s.rows + row);
+        next = byte;
+        if (!LINED && t > 0 && (t & 31) > 32 - W && group + 1 < (int)s.G) next = __ldg(scale + (group + 1) * s.rows + row);
+    }
+    template <bool LINED>
+    __device__ __forceinline__ void restore(float (&v)[W], int t) const
+    {
+        const float s0 = __uint_as_float(byte << 23), s1 = __uint_as_float(next << 23);
+#pragma unroll
+        for (int k = 0; k < W / 4; ++k) {
+            const uint32_t w = (LINED ? word[k] : __funnelshift_r(word[k], word[k + 1], (t & 3) * 8)) ^ 0x80808080u;       // q + 128
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                // 2^23 + q + 128 is the float that ends in that byte
+                const float n = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7540 | j));
+                const float f = (n - 8388736.0f) * (LINED || (t & 31) + 4 * k + j < 32 ? s0 : s1);
+                v[4 * k + j] = n == 8388608.0f ? __uint_as_float(0x7fc00000u) : f;
+            }
+        }
+    }
+};
+
+template <typename E, bool LINED>
+__device__ __forceinline__ void store_steps(E *p, int t, int T, const float (&v)[16 / sizeof(E)])
 {
-    const int lane = threadIdx.x & 31;
-    const int64_t group = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5;
-    if (group >= groups_all) return;
-    const int64_t row = group / G, t = (group - row * G) * kGroup + lane;
-    const float v = t < T ? as_float<E>(x[row * T + t]) : 0.0f;
-    const unsigned bits = __float_as_uint(v) & 0x7fffffffu;
-    const unsigned byte = scale_byte(__reduce_max_sync(~0u, bits < 0x7f800000u ? bits : 0u));
-    q[group * kGroup + lane] = (int8_t)quantise(v, byte);
-    if (lane == 0) scale[(group - row * G) * (groups_all / G) + row] = (uint8_t)byte;
+    constexpr int W = 16 / (int)sizeof(E);
+    if (LINED || (t >= 0 && t + W <= T)) {
+        uint4 raw;
+        E *e = reinterpret_cast<E *>(&raw);
+#pragma unroll
+        for (int j = 0; j < W; ++j) e[j] = as_type<E>(v[j]);
+        *reinterpret_cast<uint4 *>(p) = raw;
+    } else {
+#pragma unroll
+        for (int j = 0; j < W; ++j)
+            if (t + j >= 0 && t + j < T) p[j] = as_type<E>(v[j]);
+    }
 }
 
-template <typename E>
-__global__ void __launch_bounds__(256)
-restore_kernel(E *out, const int8_t *q, const uint8_t *scale, int64_t groups_all, int64_t T, int64_t G)
+constexpr int kReadUnroll = 4, kReadBlock = 256 * kReadUnroll;
+
+// the u-th 16 bytes of a thread: its row, and the step that they begin with
+template <int W, bool LINED>
+__device__ __forceinline__ bool read_place(const Pieces &s, const Place<kReadBlock> &place, int u, int64_t &row, int &t)
 {
-    const int lane = threadIdx.x & 31;
-    const int64_t group = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5;
-    if (group >= groups_all) return;
-    const int64_t row = group / G, t = (group - row * G) * kGroup + lane;
-    if (t < T) out[row * T + t] = as_type<E>(restored(q[group * kGroup + lane], scale[(group - row * G) * (groups_all / G) + row]));
+    const unsigned local = u * 256 + threadIdx.x;
+    unsigned down, piece;
+    place(s, local, down, piece);
+    row = place.row0 + down;
+    t = (int)piece * W - (LINED ? 0 : (int)(((unsigned)row * (unsigned)s.T) & (W - 1)));
+    return place.first + local < s.all && t < (int)s.T;
 }
 
-// the surrogate gradient (as spike_grad.cu has it) on a membrane potential in 8 bits
+template <typename E, bool LINED>
 __global__ void __launch_bounds__(256)
-spike_grad_8_kernel(float *out, const float *g, const int8_t *q, const uint8_t *scale, int64_t groups_all, int64_t T, int64_t G, float theta, float tau,
-                    float c)
+restore_kernel(E *out, const int8_t *q, const uint8_t *scale, const Pieces s)
 {
-    const int lane = threadIdx.x & 31;
-    const int64_t group = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5;
-    if (group >= groups_all) return;
-    const int64_t row = group / G, t = (group - row * G) * kGroup + lane;
-    if (t < T) out[row * T + t] = rho_times(g[row * T + t], restored(q[group * kGroup + lane], scale[(group - row * G) * (groups_all / G) + row]), theta, tau, c);
+    constexpr int W = 16 / (int)sizeof(E);
+    const Place<kReadBlock> place(s);
+    int64_t row[kReadUnroll];
+    int t[kReadUnroll];
+    bool there[kReadUnroll];
+    Kept<W> kept[kReadUnroll];
+#pragma unroll
+    for (int u = 0; u < kReadUnroll; ++u) {
+        there[u] = read_place<W, LINED>(s, place, u, row[u], t[u]);
+        if (there[u]) kept[u].template load<LINED>(q, scale, s, row[u], t[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kReadUnroll; ++u)
+        if (there[u]) {
+            float v[W];
+            kept[u].template restore<LINED>(v, t[u]);
+            store_steps<E, LINED>(out + row[u] * s.T + t[u], t[u], (int)s.T, v);
+        }
+}
+
+// The surrogate gradient (as spike_grad.cu has it) on a membrane potential in 8 bits: g c exp(-|u - theta| / tau), c = scale / tau, the exponential as
+// 2^(-|u - theta| k) with k = log2(e) / tau in two floats, so that the product is rounded once, as a division would be.
+template <bool LINED>
+__global__ void __launch_bounds__(256)
+spike_grad_8_kernel(float *out, const float *g, const int8_t *q, const uint8_t *scale, const Pieces s, float theta, float k, float k_rest, float c)
+{
+    const Place<kReadBlock> place(s);
+    int64_t row[kReadUnroll];
+    int t[kReadUnroll];
+    bool there[kReadUnroll];
+    Kept<4> kept[kReadUnroll];
+    float4 gv[kReadUnroll];
+#pragma unroll
+    for (int u = 0; u < kReadUnroll; ++u) {
+        there[u] = read_place<4, LINED>(s, place, u, row[u], t[u]);
+        if (!there[u]) continue;
+        kept[u].template load<LINED>(q, scale, s, row[u], t[u]);
+        const float *p = g + row[u] * s.T + t[u];
+        if (LINED || (t[u] >= 0 && t[u] + 4 <= (int)s.T)) {
+            gv[u] = *reinterpret_cast<const float4 *>(p);
+        } else {
+            gv[u].x = t[u] >= 0 ? p[0] : 0.0f;
+            gv[u].y = t[u] + 1 >= 0 && t[u] + 1 < (int)s.T ? p[1] : 0.0f;
+            gv[u].z = t[u] + 2 >= 0 && t[u] + 2 < (int)s.T ? p[2] : 0.0f;
+            gv[u].w = t[u] + 3 < (int)s.T ? p[3] : 0.0f;
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kReadUnroll; ++u)
+        if (there[u]) {
+            float v[4];
+            const float up[4] = {gv[u].x, gv[u].y, gv[u].z, gv[u].w};
+            kept[u].template restore<LINED>(v, t[u]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float d = fabsf(v[j] - theta);
+                v[j] = up[j] * (c * exp2f(-fmaf(d, k, d * k_rest)));
+            }
+            store_steps<float, LINED>(out + row[u] * s.T + t[u], t[u], (int)s.T, v);
+        }
 }
 
 // ------------------------------------------------------------------------------------------------ host side
@@ -91,8 +299,34 @@ static bool off_element(const void *p, int dtype) { return ((uintptr_t)p & (dtyp
 static int check_rows(const char *op, int64_t rows, int64_t T)
 {
     SB200_REQUIRE(rows >= 0 && T >= 0, "%s: negative size", op);
-    SB200_REQUIRE(rows <= (int64_t)1 << 40 && T <= (int64_t)1 << 40 && ceil_div(rows * ceil_div(T, kGroup), 8) <= 0x7fffffff, "%s: too many steps", op);
+    SB200_REQUIRE(rows <= (int64_t)1 << 40 && T <= (int64_t)1 << 30 && ceil_div(rows, 32) <= ((int64_t)1 << 31) / ceil_div(T + 1, kGroup), "%s: too many steps",
+                  op);
     return SLAYER_B200_OK;
+}
+
+static Pieces pieces_of(int64_t rows, int64_t T, int64_t each)
+{
+    return {rows, T, ceil_div(T, kGroup), each, rows * each, each < 1024 ? (unsigned)((((uint64_t)1 << 32) + each - 1) / each) : 0u};
+}
+
+template <typename E>
+static void run_compress(int8_t *q, uint8_t *scale, const void *x, int64_t rows, int64_t T, cudaStream_t st)
+{
+    const Pieces s = pieces_of(rows, T, ceil_div(T, kGroup));
+    const unsigned blocks = (unsigned)ceil_div(s.all, kCompressBlock<E>);
+    if (T % (16 / (int)sizeof(E)) == 0 && aligned16(x)) compress_kernel<E, true><<<blocks, 256, 0, st>>>(q, scale, (const E *)x, s);
+    else compress_kernel<E, false><<<blocks, 256, 0, st>>>(q, scale, (const E *)x, s);
+}
+
+template <typename E>
+static void run_restore(void *out, const int8_t *q, const uint8_t *scale, int64_t rows, int64_t T, cudaStream_t st)
+{
+    constexpr int W = 16 / (int)sizeof(E);
+    const bool lined = T % W == 0;
+    const Pieces s = pieces_of(rows, T, ceil_div(T + (lined ? 0 : W - 1), W));
+    const unsigned blocks = (unsigned)ceil_div(s.all, kReadBlock);
+    if (lined) restore_kernel<E, true><<<blocks, 256, 0, st>>>((E *)out, q, scale, s);
+    else restore_kernel<E, false><<<blocks, 256, 0, st>>>((E *)out, q, scale, s);
 }
 
 }  // namespace sb200
@@ -107,12 +341,10 @@ extern "C" int slayer_b200_compress8(int8_t *q, uint8_t *scale, const void *x, i
     if (rows == 0 || T == 0) return SLAYER_B200_OK;
     SB200_REQUIRE(q && scale && x, "compress8: null pointer");
     SB200_REQUIRE(!off_element(x, dtype) && aligned16(q), "compress8: a pointer off its alignment");
-    const int64_t G = ceil_div(T, kGroup), all = rows * G;
-    const unsigned blocks = (unsigned)ceil_div(all, 8);
     const cudaStream_t st = (cudaStream_t)stream;
-    if (dtype == SLAYER_B200_F32) compress_kernel<float><<<blocks, 256, 0, st>>>(q, scale, (const float *)x, all, T, G);
-    else if (dtype == SLAYER_B200_BF16) compress_kernel<__nv_bfloat16><<<blocks, 256, 0, st>>>(q, scale, (const __nv_bfloat16 *)x, all, T, G);
-    else compress_kernel<__half><<<blocks, 256, 0, st>>>(q, scale, (const __half *)x, all, T, G);
+    if (dtype == SLAYER_B200_F32) run_compress<float>(q, scale, x, rows, T, st);
+    else if (dtype == SLAYER_B200_BF16) run_compress<__nv_bfloat16>(q, scale, x, rows, T, st);
+    else run_compress<__half>(q, scale, x, rows, T, st);
     return check_launch("compress8 kernel launch");
 }
 
@@ -125,13 +357,11 @@ extern "C" int slayer_b200_restore8(void *out, const int8_t *q, const uint8_t *s
     if (rc) return rc;
     if (rows == 0 || T == 0) return SLAYER_B200_OK;
     SB200_REQUIRE(out && q && scale, "restore8: null pointer");
-    SB200_REQUIRE(!off_element(out, dtype) && aligned16(q), "restore8: a pointer off its alignment");
-    const int64_t G = ceil_div(T, kGroup), all = rows * G;
-    const unsigned blocks = (unsigned)ceil_div(all, 8);
+    SB200_REQUIRE(aligned16(out) && aligned16(q), "restore8: a pointer off its alignment");
     const cudaStream_t st = (cudaStream_t)stream;
-    if (dtype == SLAYER_B200_F32) restore_kernel<float><<<blocks, 256, 0, st>>>((float *)out, q, scale, all, T, G);
-    else if (dtype == SLAYER_B200_BF16) restore_kernel<__nv_bfloat16><<<blocks, 256, 0, st>>>((__nv_bfloat16 *)out, q, scale, all, T, G);
-    else restore_kernel<__half><<<blocks, 256, 0, st>>>((__half *)out, q, scale, all, T, G);
+    if (dtype == SLAYER_B200_F32) run_restore<float>(out, q, scale, rows, T, st);
+    else if (dtype == SLAYER_B200_BF16) run_restore<__nv_bfloat16>(out, q, scale, rows, T, st);
+    else run_restore<__half>(out, q, scale, rows, T, st);
     return check_launch("restore8 kernel launch");
 }
 
@@ -144,8 +374,14 @@ extern "C" int slayer_b200_spike_grad8(float *out, const float *g, const int8_t 
     if (rc) return rc;
     if (rows == 0 || T == 0) return SLAYER_B200_OK;
     SB200_REQUIRE(out && g && q && scale_bytes, "spike_grad8: null pointer");
-    SB200_REQUIRE(!off_element(out, SLAYER_B200_F32) && !off_element(g, SLAYER_B200_F32) && aligned16(q), "spike_grad8: a pointer off its alignment");
-    const int64_t G = ceil_div(T, kGroup), all = rows * G;
-    spike_grad_8_kernel<<<(unsigned)ceil_div(all, 8), 256, 0, (cudaStream_t)stream>>>(out, g, q, scale_bytes, all, T, G, theta, tau, scale / tau);
+    SB200_REQUIRE(aligned16(out) && aligned16(g) && aligned16(q), "spike_grad8: a pointer off its alignment");
+    const cudaStream_t st = (cudaStream_t)stream;
+    const double exact = 1.4426950408889634 / (double)tau;
+    const float k = (float)exact, k_rest = (float)(exact - (double)k);
+    const bool lined = T % 4 == 0;
+    const Pieces s = pieces_of(rows, T, ceil_div(T + (lined ? 0 : 3), 4));
+    const unsigned blocks = (unsigned)ceil_div(s.all, kReadBlock);
+    if (lined) spike_grad_8_kernel<true><<<blocks, 256, 0, st>>>(out, g, q, scale_bytes, s, theta, k, k_rest, scale / tau);
+    else spike_grad_8_kernel<false><<<blocks, 256, 0, st>>>(out, g, q, scale_bytes, s, theta, k, k_rest, scale / tau);
     return check_launch("spike_grad8 kernel launch");
 }
