@@ -36,6 +36,9 @@ int64_t product(at::IntArrayRef sizes, int64_t from, int64_t to)
     return std::accumulate(sizes.begin() + from, sizes.begin() + to, (int64_t)1, std::multiplies<int64_t>());
 }
 
+// itself, or a copy where it does not begin at 16 bytes
+torch::Tensor aligned(const torch::Tensor &x) { return (uintptr_t)x.data_ptr() % 16 ? x.clone() : x; }
+
 // A gate that is broadcast to x, as the kernels take it: a value per step (period 0), or one for each group of rows at all steps.
 struct Gate {
     torch::Tensor values;
@@ -55,7 +58,7 @@ Gate gate_of(const torch::Tensor &gate, const torch::Tensor &x, const char *op)
     const auto steps = [&](const torch::Tensor &g) {
         TORCH_CHECK_TYPE(g.scalar_type() == x.scalar_type(), op, ": a gate for every step must have the type of x (", x.scalar_type(), "), got ",
                          g.scalar_type());
-        return Gate{g.contiguous()};
+        return Gate{aligned(g.contiguous())};
     };
     if (full) return steps(gate);
     if (x.numel() == 0) return {gate.expand(x.sizes()).to(x.scalar_type()).contiguous()};       // nothing to do, and no rows to divide
@@ -106,7 +109,7 @@ struct GatedLeak : public torch::autograd::Function<GatedLeak> {
         const auto floats = x.options().dtype(torch::kFloat32);
         torch::Tensor state, starts;
         if (wantState) state = torch::empty(x.sizes().slice(0, x.dim() - 1), floats);
-        if (want) starts = torch::empty({s.rows, slayer_b200_leak_chunks(s.T, s.dtype)}, floats);
+        if (want) starts = torch::empty({s.rows, slayer_b200_leak_chunks(s.T)}, floats);
         const auto workspace = s.workspace(x);
         check_rc(slayer_b200_leak_forward(y.data_ptr(), wantState ? state.data_ptr<float>() : nullptr, want ? starts.data_ptr<float>() : nullptr, x.data_ptr(),
                                           gate.data_ptr(), initial.has_value() ? initial->data_ptr<float>() : nullptr, s.dtype, s.flags, s.rows, s.T,
@@ -132,7 +135,7 @@ struct GatedLeak : public torch::autograd::Function<GatedLeak> {
         const bool some = up[0].defined() || (up.size() > 1 && up[1].defined());
         if (!some) return out;
         c10::cuda::CUDAGuard guard(x.device());
-        const auto g = up[0].defined() ? up[0].contiguous() : torch::zeros_like(x);
+        const auto g = up[0].defined() ? aligned(up[0].contiguous()) : torch::zeros_like(x);
         torch::Tensor gstate;
         if (up.size() > 1 && up[1].defined()) gstate = up[1].contiguous();
         if (ctx->needs_input_grad(0)) out[0] = torch::empty_like(x);
@@ -186,7 +189,7 @@ std::vector<torch::Tensor> gatedLeakCuda(const torch::Tensor &x, const torch::Te
     }
     const auto values = g.period ? g.values.to(torch::kFloat32) : g.values;
     const bool want = at::GradMode::is_enabled() && (x.requires_grad() || gate.requires_grad() || (initial.has_value() && initial->requires_grad()));
-    return GatedLeak::apply(x.contiguous(), values, first, steps, g.inner, g.period, flags, wantState, want);
+    return GatedLeak::apply(aligned(x.contiguous()), values, first, steps, g.inner, g.period, flags, wantState, want);
 }
 
 torch::Tensor gatedLeakStepCuda(const torch::Tensor &x, const torch::Tensor &gate, torch::Tensor state, int64_t flags)
@@ -229,9 +232,6 @@ void check_kept(const torch::Tensor &q, const torch::Tensor &scale, at::IntArray
     TORCH_CHECK(q.scalar_type() == torch::kInt8 && scale.scalar_type() == torch::kUInt8 && q.is_contiguous() && scale.is_contiguous(), op,
                 ": a checkpoint has contiguous int8 values and uint8 scales");
 }
-
-// itself, or a copy where it does not begin at 16 bytes
-torch::Tensor aligned(const torch::Tensor &x) { return (uintptr_t)x.data_ptr() % 16 ? x.clone() : x; }
 
 std::vector<torch::Tensor> compress8Cuda(const torch::Tensor &x)
 {

@@ -4,7 +4,7 @@
 // of steps, the lanes of a row's group scan their maps with shuffles, and each walks its steps from the state that the lanes before
 // it leave.  The backward pass is the same from the other end: c_t = f_t (g_t + c_{t+1}) is what step t hands to step t - 1, and
 //   lambda_t = g_t + c_{t+1},   dx = lambda (or (1 - f) lambda),   df = lambda (y_{t-1} - (coupled) x).
-// It forms y again from x and the gate, out of the states that the forward pass keeps at the start of each chunk (4 bytes for 512), so that
+// It forms y again from x and the gate, out of the states that the forward pass keeps at the start of each chunk (4 bytes for 1200 and more), so that
 // it reads x, gate and g and writes dx and dgate: no y is kept, and none that is rounded to 16 bits is used.
 //
 // States and maps are double: a slow leak's f is next to one, where its rounding to 32 bits, taken at each of the thousands of steps that such
@@ -16,6 +16,8 @@
 
 namespace sb200 {
 
+constexpr int kLeakThreads = 128;
+
 template <typename E> __device__ __forceinline__ float to_float(E v);
 template <> __device__ __forceinline__ float to_float<float>(float v) { return v; }
 template <> __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -25,70 +27,91 @@ template <> __device__ __forceinline__ float from_float<float>(float v) { return
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 
-// Steps of a row that a lane holds: 16 bytes of them.  They start at multiples of 16 bytes of the tensor, not of the row, so a row's first
-// lane may begin with steps of the row before, and all lanes' steps are loaded at once whatever T is.
-template <typename E> constexpr int kSteps = 16 / (int)sizeof(E);
+// A lane has K vectors of four steps, next to each other; they begin at multiples of four elements of the tensor, not of the row, so that a row's
+// first lane may begin with steps of the row before, and vectors are loaded whole whatever T is.  G lanes have a row, or a chunk of it.
+constexpr int kVector = 4;
 
 struct LeakShape {
-    int64_t rows, T;
+    int64_t rows;
+    int T;
     int64_t gate_inner, gate_period;     // gate per row: entry (row / inner) % period; period 0: a gate per step
     int64_t sample_rows;                 // rows with one length
     const int64_t *lengths;              // null: all T
-    int64_t chunks;                      // of a row
-    int64_t segments, segment_chunks;    // a row's chunks are worked on by `segments` groups of lanes
+    int chunks;                          // of a row
+    int segments, segment_chunks;        // a row's chunks are worked on by `segments` groups of lanes
     bool logit, coupled;
 };
 
-// steps that lie outside of the row, or behind its length, keep the state: f = 1, u = 0
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b)
+{
+    return ((a | b) >> 32) == 0 ? (int64_t)((unsigned)a / (unsigned)b) : a / b;
+}
+
 struct Row {
-    int64_t base, length;      // first element; steps that count
-    int skew;                  // elements between the 16-byte boundary and the first element
+    int64_t base;              // first element
+    int skew, length;          // elements between the vector it begins in and itself; steps that count
 };
 
-template <typename E>
 __device__ __forceinline__ Row row_of(const LeakShape &s, int64_t row)
 {
     Row r;
     r.base = row * s.T;
-    r.skew = (int)(r.base % kSteps<E>);
+    r.skew = (int)(r.base & (kVector - 1));
     r.length = s.T;
     if (s.lengths) {
-        const int64_t n = s.lengths[row / s.sample_rows];
-        r.length = n < 0 ? 0 : (n < s.T ? n : s.T);
+        const int64_t n = s.lengths[quotient(row, s.sample_rows)];
+        r.length = n < 0 ? 0 : (n < s.T ? (int)n : s.T);
     }
     return r;
 }
 
-// elements [t, t + kSteps) of a row, those in [0, end) of them
-template <typename E, bool VEC>
-__device__ __forceinline__ void load_steps(float (&v)[kSteps<E>], const E *p, int64_t base, int64_t t, int64_t end, float rest)
+template <typename E> struct Packed { using type = uint2; };
+template <> struct Packed<float> { using type = uint4; };
+
+// steps [t, t + 4 K) of a row, `fill` where they are outside [0, end)
+template <typename E, int K>
+__device__ __forceinline__ void load_steps(float (&v)[4 * K], const E *row, int t, int end, float fill)
 {
-    constexpr int N = kSteps<E>;
-    if (VEC && t >= 0 && t + N <= end) {
-        const uint4 raw = __ldg(reinterpret_cast<const uint4 *>(p + base + t));
-        const E *e = reinterpret_cast<const E *>(&raw);
+    using P = typename Packed<E>::type;
 #pragma unroll
-        for (int j = 0; j < N; ++j) v[j] = to_float<E>(e[j]);
-    } else {
+    for (int k = 0; k < K; ++k) {
+        const int at = t + 4 * k;
+        if (at >= 0 && at + 4 <= end) {
+            const P raw = __ldg(reinterpret_cast<const P *>(row + at));
+            const E *e = reinterpret_cast<const E *>(&raw);
 #pragma unroll
-        for (int j = 0; j < N; ++j) v[j] = t + j >= 0 && t + j < end ? to_float<E>(p[base + t + j]) : rest;
+            for (int j = 0; j < 4; ++j) v[4 * k + j] = to_float<E>(e[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[4 * k + j] = fill;
+            if (at < end && at + 4 > 0) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (at + j >= 0 && at + j < end) v[4 * k + j] = to_float<E>(row[at + j]);
+            }
+        }
     }
 }
 
-template <typename E, bool VEC>
-__device__ __forceinline__ void store_steps(E *p, int64_t base, int64_t t, int64_t T, const float (&v)[kSteps<E>])
+// results of steps in [0, length), zeros in [length, T)
+template <typename E, int K>
+__device__ __forceinline__ void store_steps(E *row, int t, int length, int T, const float (&v)[4 * K])
 {
-    constexpr int N = kSteps<E>;
-    if (VEC && t >= 0 && t + N <= T) {
-        uint4 raw;
-        E *e = reinterpret_cast<E *>(&raw);
+    using P = typename Packed<E>::type;
 #pragma unroll
-        for (int j = 0; j < N; ++j) e[j] = from_float<E>(v[j]);
-        *reinterpret_cast<uint4 *>(p + base + t) = raw;
-    } else {
+    for (int k = 0; k < K; ++k) {
+        const int at = t + 4 * k;
+        if (at >= 0 && at + 4 <= length) {
+            P raw;
+            E *e = reinterpret_cast<E *>(&raw);
 #pragma unroll
-        for (int j = 0; j < N; ++j)
-            if (t + j >= 0 && t + j < T) p[base + t + j] = from_float<E>(v[j]);
+            for (int j = 0; j < 4; ++j) e[j] = from_float<E>(v[4 * k + j]);
+            *reinterpret_cast<P *>(row + at) = raw;
+        } else if (at < T) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (at + j >= 0 && at + j < T) row[at + j] = from_float<E>(at + j < length ? v[4 * k + j] : 0.0f);
+        }
     }
 }
 
@@ -105,30 +128,38 @@ __device__ __forceinline__ void decay_of(float gate, bool logit, double &f, floa
     }
 }
 
-// What a lane knows of its steps.
-template <typename E>
+// What a lane knows of its steps.  Those outside of the row, or behind its length, keep the state: f = 1, u = 0.
+template <typename E, int K>
 struct Steps {
-    double f[kSteps<E>];
-    float rest[kSteps<E>], x[kSteps<E>];
+    double f[4 * K];
+    float rest[4 * K], x[4 * K];
 
-    template <bool VEC>
-    __device__ __forceinline__ void load(const LeakShape &s, const Row &row, const E *x_, const E *gate, double row_f, float row_rest, int64_t t)
+    __device__ __forceinline__ void load(const LeakShape &s, const Row &row, const E *x_, const E *gate, double row_f, float row_rest, int t)
     {
-        load_steps<E, VEC>(x, x_, row.base, t, row.length, 0.0f);
+        load_steps<E, K>(x, x_ + row.base, t, row.length, 0.0f);
         if (s.gate_period == 0) {
-            float g[kSteps<E>];
-            load_steps<E, VEC>(g, gate, row.base, t, row.length, 0.0f);
+            float g[4 * K];
+            load_steps<E, K>(g, gate + row.base, t, row.length, s.logit ? INFINITY : 1.0f);
 #pragma unroll
-            for (int j = 0; j < kSteps<E>; ++j) decay_of(g[j], s.logit, f[j], rest[j]);
+            for (int j = 0; j < 4 * K; ++j) decay_of(g[j], s.logit, f[j], rest[j]);
         } else {
 #pragma unroll
-            for (int j = 0; j < kSteps<E>; ++j) f[j] = row_f, rest[j] = row_rest;
-        }
+            for (int j = 0; j < 4 * K; ++j) f[j] = row_f, rest[j] = row_rest;
+            if (t < 0 || t + 4 * K > row.length) {
 #pragma unroll
-        for (int j = 0; j < kSteps<E>; ++j)
-            if (t + j < 0 || t + j >= row.length) f[j] = 1.0, rest[j] = 0.0f;
+                for (int j = 0; j < 4 * K; ++j)
+                    if (t + j < 0 || t + j >= row.length) f[j] = 1.0, rest[j] = 0.0f;
+            }
+        }
     }
-    __device__ __forceinline__ double input(const LeakShape &s, int j) const { return (double)(s.coupled ? rest[j] * x[j] : x[j]); }
+    // x is what is added from here on
+    __device__ __forceinline__ void couple(bool coupled)
+    {
+        if (coupled) {
+#pragma unroll
+            for (int j = 0; j < 4 * K; ++j) x[j] *= rest[j];
+        }
+    }
 };
 
 struct Map {
@@ -160,85 +191,92 @@ __device__ __forceinline__ Map scan(Map m, int lane)
 template <int G, bool FORWARD>
 __device__ __forceinline__ Map others(const Map &m, int lane)
 {
+    if (G == 1) return {1.0, 0.0};
     const Map o = FORWARD ? shift_up<G>(m, 1) : shift_down<G>(m, 1);
     return lane == (FORWARD ? 0 : G - 1) ? Map{1.0, 0.0} : o;
 }
 
 // Composition of the maps of segments [from, to) of a row, in the order of time (FORWARD) or against it; all lanes of a warp get it.
 template <bool FORWARD>
-__device__ __forceinline__ Map segments_map(const Map *maps, int64_t from, int64_t to, int lane)
+__device__ __forceinline__ Map segments_map(const Map *maps, int from, int to, int lane)
 {
-    const int64_t n = to - from, each = (n + 31) / 32;
+    const int n = to - from, each = (n + 31) / 32;
     Map m = {1.0, 0.0};
-    for (int64_t i = 0; i < each; ++i) {
-        const int64_t k = lane * each + i;
+    for (int i = 0; i < each; ++i) {
+        const int k = lane * each + i;
         if (k < n) m = compose(m, maps[FORWARD ? from + k : to - 1 - k]);
     }
     m = scan<32, true>(m, lane);
     return {__shfl_sync(~0u, m.a, 31), __shfl_sync(~0u, m.b, 31)};
 }
 
-template <typename E>
-__device__ __forceinline__ Map forward_map(const LeakShape &s, const Steps<E> &st)
+template <typename E, int K>
+__device__ __forceinline__ Map forward_map(const Steps<E, K> &st)
 {
-    Map m = {1.0, 0.0};
+    Map m = {st.f[0], (double)st.x[0]};
 #pragma unroll
-    for (int j = 0; j < kSteps<E>; ++j) m = compose(m, Map{st.f[j], st.input(s, j)});
+    for (int j = 1; j < 4 * K; ++j) m = compose(m, Map{st.f[j], (double)st.x[j]});
     return m;
 }
 
-template <typename E>
-__device__ __forceinline__ Map backward_map(const double (&f)[kSteps<E>], const float (&g)[kSteps<E>])
+template <int N>
+__device__ __forceinline__ Map backward_map(const double (&f)[N], const float (&g)[N])
 {
-    Map m = {1.0, 0.0};
+    Map m = {f[N - 1], f[N - 1] * (double)g[N - 1]};
 #pragma unroll
-    for (int j = kSteps<E> - 1; j >= 0; --j) m = Map{m.a * f[j], f[j] * (m.b + (double)g[j])};
+    for (int j = N - 2; j >= 0; --j) m = Map{m.a * f[j], f[j] * (m.b + (double)g[j])};
     return m;
 }
 
 // Which row, segment and lane of its group a thread is; false: none.
 template <int G>
-__device__ __forceinline__ bool place(const LeakShape &s, int64_t &row, int64_t &segment, int &lane)
+__device__ __forceinline__ bool place(const LeakShape &s, int64_t &row, int &segment, int &lane)
 {
-    const int64_t group = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / G;
+    const int64_t group = ((int64_t)blockIdx.x * kLeakThreads + threadIdx.x) / G;
     lane = threadIdx.x % G;
-    row = group / s.segments;
-    segment = group % s.segments;
+    row = group;
+    segment = 0;
+    if (s.segments > 1) {
+        row = quotient(group, s.segments);
+        segment = (int)(group - row * s.segments);
+    }
     return row < s.rows;
 }
 
-template <typename E>
 __device__ __forceinline__ void row_gate(const LeakShape &s, const void *gate, int64_t row, double &f, float &rest)
 {
     f = 1.0, rest = 0.0f;
-    if (s.gate_period) decay_of(((const float *)gate)[row / s.gate_inner % s.gate_period], s.logit, f, rest);
+    if (s.gate_period) {
+        const int64_t n = quotient(row, s.gate_inner);
+        decay_of(((const float *)gate)[n - quotient(n, s.gate_period) * s.gate_period], s.logit, f, rest);
+    }
 }
 
 // Maps of segments: rows too few to fill the GPU are split, and each segment starts from the composition of those before it.
-template <typename E, bool VEC>
-__global__ void __launch_bounds__(256)
+template <typename E, int K>
+__global__ void __launch_bounds__(kLeakThreads)
 leak_maps_kernel(Map *maps, const E *x, const void *gate, const E *g, const LeakShape s, bool forward)
 {
-    int64_t row, segment;
-    int lane;
+    int64_t row;
+    int segment, lane;
     if (!place<32>(s, row, segment, lane)) return;
-    const Row r = row_of<E>(s, row);
+    const Row r = row_of(s, row);
     double row_f;
     float row_rest;
-    row_gate<E>(s, gate, row, row_f, row_rest);
+    row_gate(s, gate, row, row_f, row_rest);
     Map all = {1.0, 0.0};
-    const int64_t first = segment * s.segment_chunks, last = min(first + s.segment_chunks, s.chunks);
-    for (int64_t i = first; i < last; ++i) {
-        const int64_t c = forward ? i : last - 1 - (i - first);
-        const int64_t t = (c * 32 + lane) * kSteps<E> - r.skew;
-        Steps<E> st;
-        st.template load<VEC>(s, r, forward ? x : g, (const E *)gate, row_f, row_rest, t);
+    const int first = segment * s.segment_chunks, last = min(first + s.segment_chunks, s.chunks);
+    for (int i = first; i < last; ++i) {
+        const int c = forward ? i : last - 1 - (i - first);
+        Steps<E, K> st;
+        st.load(s, r, forward ? x : g, (const E *)gate, row_f, row_rest, (c * 32 + lane) * (4 * K) - r.skew);
         Map m;
         if (forward) {
-            m = scan<32, true>(forward_map<E>(s, st), lane);
+            st.couple(s.coupled);
+            m = scan<32, true>(forward_map<E, K>(st), lane);
             m = {__shfl_sync(~0u, m.a, 31), __shfl_sync(~0u, m.b, 31)};
         } else {
-            m = scan<32, false>(backward_map<E>(st.f, st.x), lane);
+            m = scan<32, false>(backward_map<4 * K>(st.f, st.x), lane);
             m = {__shfl_sync(~0u, m.a, 0), __shfl_sync(~0u, m.b, 0)};
         }
         all = compose(all, m);
@@ -246,85 +284,92 @@ leak_maps_kernel(Map *maps, const E *x, const void *gate, const E *g, const Leak
     if (lane == 0) maps[row * s.segments + segment] = all;
 }
 
-template <typename E, int G, bool VEC>
-__global__ void __launch_bounds__(256)
+template <typename E, int G, int K>
+__global__ void __launch_bounds__(kLeakThreads)
 leak_forward_kernel(E *y, float *state, float *starts, const E *x, const void *gate, const float *initial, const Map *maps, const LeakShape s)
 {
-    int64_t row, segment;
-    int lane;
+    int64_t row;
+    int segment, lane;
     const bool there = place<G>(s, row, segment, lane);
     if (G == 32 && !there) return;
     if (!there) row = s.rows - 1, segment = 0;      // the shuffles want every lane
-    const Row r = row_of<E>(s, row);
+    const Row r = row_of(s, row);
     double row_f;
     float row_rest;
-    row_gate<E>(s, gate, row, row_f, row_rest);
+    row_gate(s, gate, row, row_f, row_rest);
     double h = initial ? (double)initial[row] : 0.0;
     if (G == 32 && segment > 0) h = segments_map<true>(maps + row * s.segments, 0, segment, lane)(h);
-    const int64_t first = segment * s.segment_chunks, last = min(first + s.segment_chunks, s.chunks);
-    for (int64_t c = first; c < last; ++c) {
+    const int first = segment * s.segment_chunks, last = min(first + s.segment_chunks, s.chunks);
+    for (int c = first; c < last; ++c) {
         if (starts && there && lane == 0) starts[row * s.chunks + c] = (float)h;
-        const int64_t t = (c * G + lane) * kSteps<E> - r.skew;
-        Steps<E> st;
-        st.template load<VEC>(s, r, x, (const E *)gate, row_f, row_rest, t);
-        double at = others<G, true>(scan<G, true>(forward_map<E>(s, st), lane), lane)(h);
-        float out[kSteps<E>];
+        const int t = (c * G + lane) * (4 * K) - r.skew;
+        Steps<E, K> st;
+        st.load(s, r, x, (const E *)gate, row_f, row_rest, t);
+        st.couple(s.coupled);
+        double at = others<G, true>(scan<G, true>(forward_map<E, K>(st), lane), lane)(h);
+        float out[4 * K];
 #pragma unroll
-        for (int j = 0; j < kSteps<E>; ++j) {
-            at = fma(st.f[j], at, st.input(s, j));
-            out[j] = t + j < r.length ? (float)at : 0.0f;
+        for (int j = 0; j < 4 * K; ++j) {
+            at = fma(st.f[j], at, (double)st.x[j]);
+            out[j] = (float)at;
         }
-        if (there) store_steps<E, VEC>(y, r.base, t, s.T, out);
+        if (there) store_steps<E, K>(y + r.base, t, r.length, s.T, out);
         h = __shfl_sync(~0u, at, G - 1, G);
     }
     if (state && there && lane == 0 && segment == s.segments - 1) state[row] = (float)h;
 }
 
 // sums: per row and segment, of df: the gradient of a gate per row
-template <typename E, int G, bool VEC>
-__global__ void __launch_bounds__(256)
+template <typename E, int G, int K>
+__global__ void __launch_bounds__(kLeakThreads)
 leak_backward_kernel(E *dx, E *dgate, double *sums, float *dinitial, const E *g, const float *gstate, const float *starts, const E *x, const void *gate,
                      const Map *maps, const LeakShape s)
 {
-    constexpr int N = kSteps<E>;
-    int64_t row, segment;
-    int lane;
+    constexpr int N = 4 * K;
+    int64_t row;
+    int segment, lane;
     const bool there = place<G>(s, row, segment, lane);
     if (G == 32 && !there) return;
     if (!there) row = s.rows - 1, segment = 0;
-    const Row r = row_of<E>(s, row);
+    const Row r = row_of(s, row);
     double row_f;
     float row_rest;
-    row_gate<E>(s, gate, row, row_f, row_rest);
+    row_gate(s, gate, row, row_f, row_rest);
     double carry = gstate ? (double)gstate[row] : 0.0, sum = 0.0;
     if (G == 32 && segment + 1 < s.segments) carry = segments_map<false>(maps + row * s.segments, segment + 1, s.segments, lane)(carry);
-    const int64_t first = segment * s.segment_chunks, last = min(first + s.segment_chunks, s.chunks);
-    for (int64_t c = last - 1; c >= first; --c) {
-        const int64_t t = (c * G + lane) * N - r.skew;
-        Steps<E> st;
-        float gv[N], before[N];
-        st.template load<VEC>(s, r, x, (const E *)gate, row_f, row_rest, t);
-        load_steps<E, VEC>(gv, g, r.base, t, r.length, 0.0f);
-        double at = others<G, true>(scan<G, true>(forward_map<E>(s, st), lane), lane)((double)starts[row * s.chunks + c]);
+    const int first = segment * s.segment_chunks, last = min(first + s.segment_chunks, s.chunks);
+    for (int c = last - 1; c >= first; --c) {
+        const int t = (c * G + lane) * N - r.skew;
+        float gv[N], slope[N];       // slope: what lambda is multiplied by in dgate
+        Steps<E, K> st;
+        st.load(s, r, x, (const E *)gate, row_f, row_rest, t);
+        load_steps<E, K>(gv, g + r.base, t, r.length, 0.0f);
+        const double start = (double)starts[row * s.chunks + c];
+#pragma unroll
+        for (int j = 0; j < N; ++j) slope[j] = s.coupled ? st.x[j] : 0.0f;
+        st.couple(s.coupled);
+        double at = others<G, true>(scan<G, true>(forward_map<E, K>(st), lane), lane)(start);
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            before[j] = (float)at;
-            at = fma(st.f[j], at, st.input(s, j));
+            slope[j] = (float)at - slope[j];
+            if (s.logit) slope[j] *= (float)st.f[j] * st.rest[j];
+            at = fma(st.f[j], at, (double)st.x[j]);
         }
-        at = others<G, false>(scan<G, false>(backward_map<E>(st.f, gv), lane), lane)(carry);
-        float ox[N], og[N];
+        at = others<G, false>(scan<G, false>(backward_map<N>(st.f, gv), lane), lane)(carry);
 #pragma unroll
         for (int j = N - 1; j >= 0; --j) {
             const double lambda = at + (double)gv[j];
             at = st.f[j] * lambda;
-            const bool counts = t + j >= 0 && t + j < r.length;
-            const float l = (float)lambda, df = l * (s.coupled ? before[j] - st.x[j] : before[j]);
-            ox[j] = counts ? (s.coupled ? st.rest[j] * l : l) : 0.0f;
-            og[j] = counts ? (s.logit ? df * ((float)st.f[j] * st.rest[j]) : df) : 0.0f;
-            sum += (double)og[j];
+            gv[j] = s.coupled ? (float)lambda * st.rest[j] : (float)lambda;
+            slope[j] *= (float)lambda;
         }
-        if (there && dx) store_steps<E, VEC>(dx, r.base, t, s.T, ox);
-        if (there && dgate) store_steps<E, VEC>(dgate, r.base, t, s.T, og);
+        if (there && dx) store_steps<E, K>(dx + r.base, t, r.length, s.T, gv);
+        if (there && dgate) store_steps<E, K>(dgate + r.base, t, r.length, s.T, slope);
+        if (sums) {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (t + j >= 0 && t + j < r.length) sum += (double)slope[j];
+        }
         carry = __shfl_sync(~0u, at, 0, G);
     }
     if (sums) {
@@ -374,24 +419,38 @@ leak_step_kernel(E *y, float *state, const E *x, const EG *gate, int64_t rows, i
 // ------------------------------------------------------------------------------------------------ host side
 constexpr int64_t kGateCount = 8192;      // entries that one CTA adds up
 
-static int lanes_of(int64_t T, int steps)
+// Lanes of a row and vectors of a lane.  Rows of up to 512 steps have as few lanes as hold them, with three or four vectors each (two maps of 16 bytes are
+// passed on in each doubling of the lanes, whatever a lane holds); longer ones are worked on in chunks of 32 lanes with four.
+struct LeakLanes {
+    int lanes, vectors;
+};
+
+static LeakLanes lanes_of(int64_t T)
 {
-    int g = 1;
-    while (g < 32 && (int64_t)g * steps < T + (T % steps ? steps - 1 : 0)) g *= 2;
-    return g;
+    const int64_t n = ceil_div(T + (T % kVector ? kVector - 1 : 0), kVector);
+    if (n <= 1) return {1, 1};
+    if (n <= 2) return {1, 2};
+    if (n <= 4) return {1, 4};
+    for (int g = 2; g <= 32; g *= 2) {
+        if (n <= 3 * g) return {g, 3};
+        if (n <= 4 * g) return {g, 4};
+    }
+    return {32, 4};
 }
 
-static int64_t chunks_of(int64_t T, int steps) { return ceil_div(T + (T % steps ? steps - 1 : 0), (int64_t)lanes_of(T, steps) * steps); }
-
-static int steps_of(int dtype) { return dtype == SLAYER_B200_F32 ? 4 : 8; }
-
-// groups per row: rows with many chunks, too few to give every SM 32 warps, are split.
-static int64_t segments_of(int64_t rows, int64_t T, int steps)
+static int64_t chunks_of(int64_t T)
 {
-    const int64_t chunks = chunks_of(T, steps), warps = (int64_t)sm_count() * 32;
-    if (lanes_of(T, steps) < 32 || chunks < 4 || rows * 2 > warps) return 1;
+    const LeakLanes l = lanes_of(T);
+    return ceil_div(T + (T % kVector ? kVector - 1 : 0), (int64_t)l.lanes * l.vectors * kVector);
+}
+
+// groups per row: rows with many chunks, too few to give every SM 16 warps, are split.
+static int64_t segments_of(int64_t rows, int64_t T)
+{
+    const int64_t chunks = chunks_of(T), warps = (int64_t)sm_count() * 16;
+    if (chunks < 2 || rows * 2 > warps) return 1;
     int64_t n = warps / rows;
-    if (n > chunks / 2) n = chunks / 2;
+    if (n > chunks) n = chunks;
     if (n > 1024) n = 1024;
     return ceil_div(chunks, ceil_div(chunks, n));
 }
@@ -400,7 +459,7 @@ static bool known(int dtype) { return dtype == SLAYER_B200_F32 || dtype == SLAYE
 
 struct LeakPlan {
     LeakShape s;
-    int lanes;
+    LeakLanes l;
     int64_t maps_bytes, sums_bytes, gate_parts;
 };
 
@@ -410,53 +469,51 @@ static int plan_leak(LeakPlan &p, const char *op, int dtype, int flags, int64_t 
     SB200_REQUIRE(known(dtype), "%s: unknown element type %d", op, dtype);
     SB200_REQUIRE((flags & ~3) == 0, "%s: unknown flags %d", op, flags);
     SB200_REQUIRE(rows >= 0 && T >= 0, "%s: negative size", op);
-    SB200_REQUIRE(rows <= (int64_t)1 << 40 && T <= (int64_t)1 << 40 && rows * (T >> 20) <= (int64_t)1 << 40, "%s: sizes overflow", op);
+    SB200_REQUIRE(rows <= (int64_t)1 << 40 && T <= (int64_t)1 << 30 && rows * (T >> 20) <= (int64_t)1 << 40, "%s: sizes overflow", op);
     SB200_REQUIRE(gate_period >= 0 && (gate_period == 0 || gate_inner >= 1), "%s: bad gate layout", op);
     SB200_REQUIRE(gate_period == 0 || (gate_period <= rows && gate_inner <= rows && rows % (gate_inner * gate_period) == 0) || rows == 0,
                   "%s: rows must be whole groups of gates", op);
     SB200_REQUIRE(!lengths || sample_rows >= 1, "%s: lengths need the number of rows that have one", op);
-    const int steps = steps_of(dtype);
-    p.s = {rows, T, gate_inner, gate_period, sample_rows, lengths, chunks_of(T, steps), 1, 0, (flags & SLAYER_B200_LEAK_LOGIT) != 0,
-           (flags & SLAYER_B200_LEAK_COUPLED) != 0};
-    p.s.segments = rows ? segments_of(rows, T, steps) : 1;
-    p.s.segment_chunks = ceil_div(p.s.chunks, p.s.segments);
-    p.lanes = lanes_of(T, steps);
-    p.maps_bytes = p.s.segments > 1 ? rows * p.s.segments * (int64_t)sizeof(Map) : 0;
+    p.l = lanes_of(T);
+    const int64_t chunks = chunks_of(T), segments = rows ? segments_of(rows, T) : 1;
+    p.s = {rows, (int)T, gate_inner, gate_period, sample_rows, lengths, (int)chunks, (int)segments, (int)ceil_div(chunks, segments),
+           (flags & SLAYER_B200_LEAK_LOGIT) != 0, (flags & SLAYER_B200_LEAK_COUPLED) != 0};
+    p.maps_bytes = segments > 1 ? rows * segments * (int64_t)sizeof(Map) : 0;
     p.sums_bytes = p.gate_parts = 0;
     if (gate_period && rows) {
-        const int64_t count = rows / gate_period * p.s.segments;
+        const int64_t count = rows / gate_period * segments;
         p.gate_parts = ceil_div(count, kGateCount);
         if (p.gate_parts > 1024) p.gate_parts = 1024;
-        p.sums_bytes = (rows * p.s.segments + (p.gate_parts > 1 ? gate_period * p.gate_parts : 0)) * (int64_t)sizeof(double);
+        p.sums_bytes = (rows * segments + (p.gate_parts > 1 ? gate_period * p.gate_parts : 0)) * (int64_t)sizeof(double);
     }
-    SB200_REQUIRE(ceil_div(rows * p.s.segments * p.lanes, 256) <= 0x7fffffff, "%s: too many rows", op);
+    SB200_REQUIRE(ceil_div(rows * segments * p.l.lanes, kLeakThreads) <= 0x7fffffff, "%s: too many rows", op);
     SB200_REQUIRE(p.gate_parts * gate_period <= 0x7fffffff, "%s: too many gates", op);
     return SLAYER_B200_OK;
 }
 
-template <typename E, int G, bool VEC>
+template <typename E, int G, int K>
 static void run_forward(const LeakPlan &p, void *y, float *state, float *starts, const void *x, const void *gate, const float *initial, void *workspace,
                         cudaStream_t st)
 {
     Map *maps = (Map *)workspace;
-    const unsigned blocks = (unsigned)ceil_div(p.s.rows * p.s.segments * G, 256);
+    const unsigned blocks = (unsigned)ceil_div(p.s.rows * p.s.segments * G, kLeakThreads);
     if constexpr (G == 32)
-        if (p.s.segments > 1) leak_maps_kernel<E, VEC><<<blocks, 256, 0, st>>>(maps, (const E *)x, gate, nullptr, p.s, true);
-    leak_forward_kernel<E, G, VEC><<<blocks, 256, 0, st>>>((E *)y, state, starts, (const E *)x, gate, initial, maps, p.s);
+        if (p.s.segments > 1) leak_maps_kernel<E, K><<<blocks, kLeakThreads, 0, st>>>(maps, (const E *)x, gate, nullptr, p.s, true);
+    leak_forward_kernel<E, G, K><<<blocks, kLeakThreads, 0, st>>>((E *)y, state, starts, (const E *)x, gate, initial, maps, p.s);
 }
 
-template <typename E, int G, bool VEC>
+template <typename E, int G, int K>
 static void run_backward(const LeakPlan &p, void *dx, void *dgate, float *dinitial, const void *g, const float *gstate, const float *starts, const void *x,
                          const void *gate, void *workspace, cudaStream_t st)
 {
     Map *maps = (Map *)workspace;
     double *sums = (double *)((char *)workspace + p.maps_bytes);
     const bool per_row = p.s.gate_period > 0;
-    const unsigned blocks = (unsigned)ceil_div(p.s.rows * p.s.segments * G, 256);
+    const unsigned blocks = (unsigned)ceil_div(p.s.rows * p.s.segments * G, kLeakThreads);
     if constexpr (G == 32)
-        if (p.s.segments > 1) leak_maps_kernel<E, VEC><<<blocks, 256, 0, st>>>(maps, nullptr, gate, (const E *)g, p.s, false);
-    leak_backward_kernel<E, G, VEC><<<blocks, 256, 0, st>>>((E *)dx, per_row ? nullptr : (E *)dgate, per_row && dgate ? sums : nullptr, dinitial, (const E *)g,
-                                                          gstate, starts, (const E *)x, gate, maps, p.s);
+        if (p.s.segments > 1) leak_maps_kernel<E, K><<<blocks, kLeakThreads, 0, st>>>(maps, nullptr, gate, (const E *)g, p.s, false);
+    leak_backward_kernel<E, G, K><<<blocks, kLeakThreads, 0, st>>>((E *)dx, per_row ? nullptr : (E *)dgate, per_row && dgate ? sums : nullptr, dinitial,
+                                                                (const E *)g, gstate, starts, (const E *)x, gate, maps, p.s);
     if (per_row && dgate) {
         const int64_t inner = p.s.gate_inner * p.s.segments, outer = p.s.rows / (p.s.gate_inner * p.s.gate_period);
         double *part = sums + p.s.rows * p.s.segments;
@@ -470,34 +527,32 @@ static void run_backward(const LeakPlan &p, void *dx, void *dgate, float *diniti
     }
 }
 
-#define SB200_LEAK_LANES(E, VEC, CALL)                       \
-    switch (p.lanes) {                                       \
-    case 1: CALL(E, 1, VEC); break;                          \
-    case 2: CALL(E, 2, VEC); break;                          \
-    case 4: CALL(E, 4, VEC); break;                          \
-    case 8: CALL(E, 8, VEC); break;                          \
-    case 16: CALL(E, 16, VEC); break;                        \
-    default: CALL(E, 32, VEC); break;                        \
+// the kernel of a plan's lanes and vectors
+#define SB200_LEAK_LANES(E, CALL)                                                              \
+    switch (p.l.lanes) {                                                                       \
+    case 1: if (p.l.vectors == 1) CALL(E, 1, 1); else if (p.l.vectors == 2) CALL(E, 1, 2); else CALL(E, 1, 4); break; \
+    case 2: if (p.l.vectors == 3) CALL(E, 2, 3); else CALL(E, 2, 4); break;                    \
+    case 4: if (p.l.vectors == 3) CALL(E, 4, 3); else CALL(E, 4, 4); break;                    \
+    case 8: if (p.l.vectors == 3) CALL(E, 8, 3); else CALL(E, 8, 4); break;                    \
+    case 16: if (p.l.vectors == 3) CALL(E, 16, 3); else CALL(E, 16, 4); break;                 \
+    default: if (p.l.vectors == 3) CALL(E, 32, 3); else CALL(E, 32, 4); break;                 \
     }
-#define SB200_LEAK_ALIGN(E, CALL)                            \
-    if (vec) { SB200_LEAK_LANES(E, true, CALL) } else { SB200_LEAK_LANES(E, false, CALL) }
-#define SB200_LEAK_TYPES(CALL)                                                     \
-    if (dtype == SLAYER_B200_F32) { SB200_LEAK_ALIGN(float, CALL) }               \
-    else if (dtype == SLAYER_B200_BF16) { SB200_LEAK_ALIGN(__nv_bfloat16, CALL) } \
-    else { SB200_LEAK_ALIGN(__half, CALL) }
+#define SB200_LEAK_TYPES(CALL)                                                \
+    if (dtype == SLAYER_B200_F32) { SB200_LEAK_LANES(float, CALL) }           \
+    else if (dtype == SLAYER_B200_BF16) { SB200_LEAK_LANES(__nv_bfloat16, CALL) } \
+    else { SB200_LEAK_LANES(__half, CALL) }
 
 static bool element_aligned(const void *p, int dtype) { return ((uintptr_t)p & (dtype == SLAYER_B200_F32 ? 3 : 1)) == 0; }
 static bool aligned_to(const void *p, unsigned n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
 }  // namespace sb200
 
-extern "C" int64_t slayer_b200_leak_chunks(int64_t T, int dtype)
+extern "C" int64_t slayer_b200_leak_chunks(int64_t T)
 {
     using namespace sb200;
     clear_error();
-    SB200_REQUIRE(known(dtype), "leak_chunks: unknown element type %d", dtype);
-    SB200_REQUIRE(T >= 0 && T <= (int64_t)1 << 40, "leak_chunks: bad length");
-    return chunks_of(T, steps_of(dtype));
+    SB200_REQUIRE(T >= 0 && T <= (int64_t)1 << 30, "leak_chunks: bad length");
+    return chunks_of(T);
 }
 
 extern "C" int64_t slayer_b200_leak_workspace(int64_t rows, int64_t T, int dtype, int64_t gate_inner, int64_t gate_period)
@@ -522,12 +577,11 @@ extern "C" int slayer_b200_leak_forward(void *y, float *state, float *starts, co
     SB200_REQUIRE((y && x) || T == 0, "leak_forward: null pointer");
     SB200_REQUIRE(gate || (T == 0 && gate_period == 0), "leak_forward: null pointer");
     SB200_REQUIRE(p.maps_bytes == 0 || (workspace && aligned16(workspace)), "leak_forward: the workspace must be aligned to 16 bytes");
-    SB200_REQUIRE(element_aligned(y, dtype) && element_aligned(x, dtype) && element_aligned(gate, gate_period ? SLAYER_B200_F32 : dtype) &&
-                      aligned_to(state, 4) && aligned_to(starts, 4) && aligned_to(initial, 4) && aligned_to(lengths, 8),
-                  "leak_forward: a pointer off its element's alignment");
-    const bool vec = aligned16(y) && aligned16(x) && (gate_period || aligned16(gate));
+    SB200_REQUIRE(aligned16(y) && aligned16(x) && aligned_to(gate, gate_period ? 4 : 16) && aligned_to(state, 4) && aligned_to(starts, 4) &&
+                      aligned_to(initial, 4) && aligned_to(lengths, 8),
+                  "leak_forward: a pointer off its alignment");
     const cudaStream_t st = (cudaStream_t)stream;
-#define SB200_LEAK_CALL(E, G, VEC) run_forward<E, G, VEC>(p, y, state, starts, x, gate, initial, workspace, st)
+#define SB200_LEAK_CALL(E, G, K) run_forward<E, G, K>(p, y, state, starts, x, gate, initial, workspace, st)
     SB200_LEAK_TYPES(SB200_LEAK_CALL)
 #undef SB200_LEAK_CALL
     return check_launch("leak_forward kernel launch");
@@ -546,13 +600,11 @@ extern "C" int slayer_b200_leak_backward(void *dx, void *dgate, float *dinitial,
     SB200_REQUIRE((g && x && starts) || T == 0, "leak_backward: null pointer");
     SB200_REQUIRE(gate || (T == 0 && gate_period == 0), "leak_backward: null pointer");
     SB200_REQUIRE(p.maps_bytes + p.sums_bytes == 0 || (workspace && aligned16(workspace)), "leak_backward: the workspace must be aligned to 16 bytes");
-    SB200_REQUIRE(element_aligned(dx, dtype) && element_aligned(dgate, gate_period ? SLAYER_B200_F32 : dtype) && element_aligned(g, dtype) &&
-                      element_aligned(x, dtype) && element_aligned(gate, gate_period ? SLAYER_B200_F32 : dtype) && aligned_to(dinitial, 4) &&
-                      aligned_to(gstate, 4) && aligned_to(starts, 4) && aligned_to(lengths, 8),
-                  "leak_backward: a pointer off its element's alignment");
-    const bool vec = aligned16(dx) && aligned16(g) && aligned16(x) && (gate_period || (aligned16(gate) && aligned16(dgate)));
+    SB200_REQUIRE(aligned16(dx) && aligned_to(dgate, gate_period ? 4 : 16) && aligned16(g) && aligned16(x) && aligned_to(gate, gate_period ? 4 : 16) &&
+                      aligned_to(dinitial, 4) && aligned_to(gstate, 4) && aligned_to(starts, 4) && aligned_to(lengths, 8),
+                  "leak_backward: a pointer off its alignment");
     const cudaStream_t st = (cudaStream_t)stream;
-#define SB200_LEAK_CALL(E, G, VEC) run_backward<E, G, VEC>(p, dx, dgate, dinitial, g, gstate, starts, x, gate, workspace, st)
+#define SB200_LEAK_CALL(E, G, K) run_backward<E, G, K>(p, dx, dgate, dinitial, g, gstate, starts, x, gate, workspace, st)
     SB200_LEAK_TYPES(SB200_LEAK_CALL)
 #undef SB200_LEAK_CALL
     return check_launch("leak_backward kernel launch");

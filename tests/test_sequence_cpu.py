@@ -64,10 +64,10 @@ def test_c_entries_of_the_leak():
                 dict(period=3, inner=1)):
         assert call(**bad) == -1, bad
     assert call(rows=0, y=null) == 0
-    # a row of T steps has chunks of 128 (16-bit types: 256), and up to a whole 16 bytes before its first step
-    for T, dtype, n in ((0, 0, 0), (1, 0, 1), (128, 0, 1), (129, 0, 2), (126, 0, 2), (300, 0, 3), (300, 1, 2), (1450, 2, 6), (100000, 0, 782)):
-        assert lib.slayer_b200_leak_chunks(T, dtype) == n, (T, dtype)
-    assert lib.slayer_b200_leak_chunks(-1, 0) == -1 and lib.slayer_b200_leak_chunks(5, 4) == -1
+    # a row of up to 512 steps, with up to three before its first one, is a chunk, longer ones have chunks of 512
+    for T, n in ((0, 0), (1, 1), (128, 1), (129, 1), (509, 1), (511, 2), (512, 1), (513, 2), (1450, 3), (2000, 4), (100000, 196)):
+        assert lib.slayer_b200_leak_chunks(T) == n, T
+    assert lib.slayer_b200_leak_chunks(-1) == -1 and lib.slayer_b200_leak_chunks(1 << 31) == -1
     assert lib.slayer_b200_leak_workspace(-1, 5, 0, 0, 0) == -1
     assert lib.slayer_b200_leak_workspace(1 << 20, 300, 0, 0, 0) == 0
 
