@@ -7,8 +7,9 @@
 // It forms y again from x and the gate, out of the states that the forward pass keeps at the start of each chunk (4 bytes for 1200 and more), so that
 // it reads x, gate and g and writes dx and dgate: no y is kept, and none that is rounded to 16 bits is used.
 //
-// States and maps are double: a slow leak's f is next to one, where its rounding to 32 bits, taken at each of the thousands of steps that such
-// a state remembers, adds up to 1e-5 of it; 1 - f is known to 32 bits from the gate, and double's f keeps them.
+// Maps are floats: A, and 1 - A by itself (R), and B.  A slow leak's f is next to one, where its rounding to 32 bits, taken at each of the thousands of
+// steps that such a state remembers, adds up to 1e-4 of it; R has 24 bits of what is forgotten instead.  States are double from chunk to chunk, and
+// float within the up to 16 steps that a lane walks.  (All of it in double, with half as many instructions again: 39 + 74 us instead of 29 + 51, 64 x 512 x 300.)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -17,6 +18,10 @@
 namespace sb200 {
 
 constexpr int kLeakThreads = 128;
+
+// CTAs of an SM that registers are rationed for: the most that leave none of a lane's steps in memory
+template <int K> constexpr int kForwardBlocks = K < 4 ? 8 : 7;
+template <int K> constexpr int kBackwardBlocks = K < 4 ? 5 : 4;
 
 template <typename E> __device__ __forceinline__ float to_float(E v);
 template <> __device__ __forceinline__ float to_float<float>(float v) { return v; }
@@ -32,34 +37,28 @@ template <> __device__ __forceinline__ __half from_float<__half>(float v) { retu
 constexpr int kVector = 4;
 
 struct LeakShape {
-    int64_t rows;
-    int T;
-    int64_t gate_inner, gate_period;     // gate per row: entry (row / inner) % period; period 0: a gate per step
-    int64_t sample_rows;                 // rows with one length
+    int rows, T;
+    int gate_inner, gate_period;         // gate per row: entry (row / inner) % period; period 0: a gate per step
+    int sample_rows;                     // rows with one length
     const int64_t *lengths;              // null: all T
     int chunks;                          // of a row
     int segments, segment_chunks;        // a row's chunks are worked on by `segments` groups of lanes
     bool logit, coupled;
 };
 
-__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b)
-{
-    return ((a | b) >> 32) == 0 ? (int64_t)((unsigned)a / (unsigned)b) : a / b;
-}
-
 struct Row {
     int64_t base;              // first element
     int skew, length;          // elements between the vector it begins in and itself; steps that count
 };
 
-__device__ __forceinline__ Row row_of(const LeakShape &s, int64_t row)
+__device__ __forceinline__ Row row_of(const LeakShape &s, int row)
 {
     Row r;
-    r.base = row * s.T;
+    r.base = (int64_t)row * s.T;
     r.skew = (int)(r.base & (kVector - 1));
     r.length = s.T;
     if (s.lengths) {
-        const int64_t n = s.lengths[quotient(row, s.sample_rows)];
+        const int64_t n = __ldg(s.lengths + (unsigned)row / (unsigned)s.sample_rows);
         r.length = n < 0 ? 0 : (n < s.T ? (int)n : s.T);
     }
     return r;
@@ -68,87 +67,117 @@ __device__ __forceinline__ Row row_of(const LeakShape &s, int64_t row)
 template <typename E> struct Packed { using type = uint2; };
 template <> struct Packed<float> { using type = uint4; };
 
-// steps [t, t + 4 K) of a row, `fill` where they are outside [0, end)
+// Which of a lane's vectors lie in [0, end) of a row as a whole, and whether one of them lies there in part.
+template <int K>
+struct Inside {
+    int t, end;
+    bool whole[K], part;
+    __device__ __forceinline__ Inside(int t_, int end_) : t(t_), end(end_)
+    {
+        part = false;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int at = t + 4 * k;
+            whole[k] = at >= 0 && at <= end - 4;
+            part = part || (!whole[k] && at < end && at > -4);
+        }
+    }
+};
+
+// steps [t, t + 4 K) of a row, `fill` where they are outside
 template <typename E, int K>
-__device__ __forceinline__ void load_steps(float (&v)[4 * K], const E *row, int t, int end, float fill)
+__device__ __forceinline__ void load_steps(float (&v)[4 * K], const E *row, const Inside<K> &in, float fill)
 {
     using P = typename Packed<E>::type;
+    P raw[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        const int at = t + 4 * k;
-        if (at >= 0 && at + 4 <= end) {
-            const P raw = __ldg(reinterpret_cast<const P *>(row + at));
-            const E *e = reinterpret_cast<const E *>(&raw);
+        E none[4] = {from_float<E>(fill), from_float<E>(fill), from_float<E>(fill), from_float<E>(fill)};
+        raw[k] = *reinterpret_cast<P *>(none);
+        if (in.whole[k]) raw[k] = __ldg(reinterpret_cast<const P *>(row + in.t + 4 * k));
+    }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[4 * k + j] = to_float<E>(e[j]);
-        } else {
+    for (int k = 0; k < K; ++k) {
+        const E *e = reinterpret_cast<const E *>(&raw[k]);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[4 * k + j] = fill;
-            if (at < end && at + 4 > 0) {
+        for (int j = 0; j < 4; ++j) v[4 * k + j] = to_float<E>(e[j]);
+    }
+    if (in.part) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (at + j >= 0 && at + j < end) v[4 * k + j] = to_float<E>(row[at + j]);
+        for (int k = 0; k < K; ++k)
+            if (!in.whole[k]) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int at = in.t + 4 * k + j;
+                    if (at >= 0 && at < in.end) v[4 * k + j] = to_float<E>(row[at]);
+                }
             }
-        }
     }
 }
 
-// results of steps in [0, length), zeros in [length, T)
+// results of steps in [0, end), zeros in [end, T)
 template <typename E, int K>
-__device__ __forceinline__ void store_steps(E *row, int t, int length, int T, const float (&v)[4 * K])
+__device__ __forceinline__ void store_steps(E *row, const Inside<K> &in, int T, const float (&v)[4 * K])
 {
     using P = typename Packed<E>::type;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        const int at = t + 4 * k;
-        if (at >= 0 && at + 4 <= length) {
-            P raw;
-            E *e = reinterpret_cast<E *>(&raw);
+        P raw;
+        E *e = reinterpret_cast<E *>(&raw);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) e[j] = from_float<E>(v[4 * k + j]);
-            *reinterpret_cast<P *>(row + at) = raw;
-        } else if (at < T) {
+        for (int j = 0; j < 4; ++j) e[j] = from_float<E>(v[4 * k + j]);
+        if (in.whole[k]) *reinterpret_cast<P *>(row + in.t + 4 * k) = raw;
+    }
+    if (in.part || in.end < T) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (at + j >= 0 && at + j < T) row[at + j] = from_float<E>(at + j < length ? v[4 * k + j] : 0.0f);
-        }
+        for (int k = 0; k < K; ++k)
+            if (!in.whole[k]) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int at = in.t + 4 * k + j;
+                    if (at >= 0 && at < T) row[at] = from_float<E>(at < in.end ? v[4 * k + j] : 0.0f);
+                }
+            }
     }
 }
 
-// f and 1 - f, each to its own 32 bits
-__device__ __forceinline__ void decay_of(float gate, bool logit, double &f, float &rest)
+// f and 1 - f, each to its own 24 bits
+struct Decay {
+    float f, rest;
+};
+
+__device__ __forceinline__ Decay decay_of(float gate, bool logit)
 {
-    if (logit) {
-        const float e = expf(-fabsf(gate)), large = __fdividef(1.0f, 1.0f + e), small = e * large;
-        f = gate < 0.0f ? (double)small : 1.0 - (double)small;
-        rest = gate < 0.0f ? large : small;
-    } else {
-        f = (double)gate;
-        rest = (float)(1.0 - (double)gate);
-    }
+    if (!logit) return {gate, 1.0f - gate};
+    // e^-|gate| as a power of two, log2(e) in two floats
+    float e;
+    const float a = fabsf(gate);
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-fmaf(a, 1.44269502f, a * 1.92596303e-8f)));
+    const float large = __fdividef(1.0f, 1.0f + e), small = e * large;
+    return gate < 0.0f ? Decay{small, large} : Decay{1.0f - small, small};
 }
 
 // What a lane knows of its steps.  Those outside of the row, or behind its length, keep the state: f = 1, u = 0.
 template <typename E, int K>
 struct Steps {
-    double f[4 * K];
-    float rest[4 * K], x[4 * K];
+    Decay d[4 * K];
+    float x[4 * K];
 
-    __device__ __forceinline__ void load(const LeakShape &s, const Row &row, const E *x_, const E *gate, double row_f, float row_rest, int t)
+    __device__ __forceinline__ void load(const LeakShape &s, const Row &row, const E *x_, const E *gate, const Decay &row_d, const Inside<K> &in)
     {
-        load_steps<E, K>(x, x_ + row.base, t, row.length, 0.0f);
+        load_steps<E, K>(x, x_ + row.base, in, 0.0f);
         if (s.gate_period == 0) {
             float g[4 * K];
-            load_steps<E, K>(g, gate + row.base, t, row.length, s.logit ? INFINITY : 1.0f);
+            load_steps<E, K>(g, gate + row.base, in, s.logit ? INFINITY : 1.0f);
 #pragma unroll
-            for (int j = 0; j < 4 * K; ++j) decay_of(g[j], s.logit, f[j], rest[j]);
+            for (int j = 0; j < 4 * K; ++j) d[j] = decay_of(g[j], s.logit);
         } else {
 #pragma unroll
-            for (int j = 0; j < 4 * K; ++j) f[j] = row_f, rest[j] = row_rest;
-            if (t < 0 || t + 4 * K > row.length) {
+            for (int j = 0; j < 4 * K; ++j) d[j] = in.whole[j / 4] ? row_d : Decay{1.0f, 0.0f};
+            if (in.part) {
 #pragma unroll
                 for (int j = 0; j < 4 * K; ++j)
-                    if (t + j < 0 || t + j >= row.length) f[j] = 1.0, rest[j] = 0.0f;
+                    if (in.t + j >= 0 && in.t + j < in.end) d[j] = row_d;
             }
         }
     }
@@ -157,23 +186,45 @@ struct Steps {
     {
         if (coupled) {
 #pragma unroll
-            for (int j = 0; j < 4 * K; ++j) x[j] *= rest[j];
+            for (int j = 0; j < 4 * K; ++j) x[j] *= d[j].rest;
         }
     }
 };
 
+// h -> a h + b, r = 1 - a
 struct Map {
-    double a, b;
-    __device__ __forceinline__ double operator()(double h) const { return fma(a, h, b); }
+    float a, r, b;
+    // by what is forgotten of h, or by what is kept: whichever is less
+    __device__ __forceinline__ double operator()(double h) const
+    {
+        const bool little = r < 0.5f;
+        return (little ? h : 0.0) + fma((double)(little ? -r : a), h, (double)b);
+    }
 };
 
 // first, then second
-__device__ __forceinline__ Map compose(const Map &first, const Map &second) { return {first.a * second.a, second(first.b)}; }
+__device__ __forceinline__ Map compose(const Map &first, const Map &second)
+{
+    const bool little = second.r < 0.5f;
+    const float r = fmaf(first.a, second.r, first.r);
+    // a product of many factors next to one is off by as many roundings; 1 - r is not
+    return {r < 0.5f ? 1.0f - r : first.a * second.a, r, (little ? first.b : 0.0f) + fmaf(little ? -second.r : second.a, first.b, second.b)};
+}
+
+// a map, then one step
+__device__ __forceinline__ Map step_after(const Map &m, const Decay &d, float u) { return {m.a * d.f, fmaf(m.a, d.rest, m.r), fmaf(d.f, m.b, u)}; }
 
 template <int G>
-__device__ __forceinline__ Map shift_up(const Map &m, int d) { return {__shfl_up_sync(~0u, m.a, d, G), __shfl_up_sync(~0u, m.b, d, G)}; }
+__device__ __forceinline__ Map shift_up(const Map &m, int d)
+{
+    return {__shfl_up_sync(~0u, m.a, d, G), __shfl_up_sync(~0u, m.r, d, G), __shfl_up_sync(~0u, m.b, d, G)};
+}
 template <int G>
-__device__ __forceinline__ Map shift_down(const Map &m, int d) { return {__shfl_down_sync(~0u, m.a, d, G), __shfl_down_sync(~0u, m.b, d, G)}; }
+__device__ __forceinline__ Map shift_down(const Map &m, int d)
+{
+    return {__shfl_down_sync(~0u, m.a, d, G), __shfl_down_sync(~0u, m.r, d, G), __shfl_down_sync(~0u, m.b, d, G)};
+}
+__device__ __forceinline__ Map shift_from(const Map &m, int lane) { return {__shfl_sync(~0u, m.a, lane), __shfl_sync(~0u, m.r, lane), __shfl_sync(~0u, m.b, lane)}; }
 
 // the map of this lane and all before it (FORWARD), or all behind it
 template <int G, bool FORWARD>
@@ -191,191 +242,179 @@ __device__ __forceinline__ Map scan(Map m, int lane)
 template <int G, bool FORWARD>
 __device__ __forceinline__ Map others(const Map &m, int lane)
 {
-    if (G == 1) return {1.0, 0.0};
+    if (G == 1) return {1.0f, 0.0f, 0.0f};
     const Map o = FORWARD ? shift_up<G>(m, 1) : shift_down<G>(m, 1);
-    return lane == (FORWARD ? 0 : G - 1) ? Map{1.0, 0.0} : o;
+    return lane == (FORWARD ? 0 : G - 1) ? Map{1.0f, 0.0f, 0.0f} : o;
 }
 
-// Composition of the maps of segments [from, to) of a row, in the order of time (FORWARD) or against it; all lanes of a warp get it.
+// A state after (FORWARD), or a gradient before, the segments [from, to) of a row; all lanes of a warp get it.  The states of groups of 32 segments
+// are double, as those of chunks are.
 template <bool FORWARD>
-__device__ __forceinline__ Map segments_map(const Map *maps, int from, int to, int lane)
+__device__ __forceinline__ double through_segments(const Map *maps, int from, int to, int lane, double h)
 {
-    const int n = to - from, each = (n + 31) / 32;
-    Map m = {1.0, 0.0};
-    for (int i = 0; i < each; ++i) {
-        const int k = lane * each + i;
-        if (k < n) m = compose(m, maps[FORWARD ? from + k : to - 1 - k]);
+    for (int at = 0; at < to - from; at += 32) {
+        const int k = at + lane;
+        Map m = {1.0f, 0.0f, 0.0f};
+        if (k < to - from) m = maps[FORWARD ? from + k : to - 1 - k];
+        h = shift_from(scan<32, true>(m, lane), 31)(h);
     }
-    m = scan<32, true>(m, lane);
-    return {__shfl_sync(~0u, m.a, 31), __shfl_sync(~0u, m.b, 31)};
+    return h;
 }
 
 template <typename E, int K>
 __device__ __forceinline__ Map forward_map(const Steps<E, K> &st)
 {
-    Map m = {st.f[0], (double)st.x[0]};
+    Map m = {st.d[0].f, st.d[0].rest, st.x[0]};
 #pragma unroll
-    for (int j = 1; j < 4 * K; ++j) m = compose(m, Map{st.f[j], (double)st.x[j]});
+    for (int j = 1; j < 4 * K; ++j) m = step_after(m, st.d[j], st.x[j]);
     return m;
 }
 
+// c -> f (g + c) for all steps, from the last; what is kept of c is what is kept of a state (`kept`)
 template <int N>
-__device__ __forceinline__ Map backward_map(const double (&f)[N], const float (&g)[N])
+__device__ __forceinline__ Map backward_map(const Decay (&d)[N], const float (&g)[N], const Map &kept)
 {
-    Map m = {f[N - 1], f[N - 1] * (double)g[N - 1]};
+    float b = d[N - 1].f * g[N - 1];
 #pragma unroll
-    for (int j = N - 2; j >= 0; --j) m = Map{m.a * f[j], f[j] * (m.b + (double)g[j])};
-    return m;
+    for (int j = N - 2; j >= 0; --j) b = d[j].f * (b + g[j]);
+    return {kept.a, kept.r, b};
 }
 
 // Which row, segment and lane of its group a thread is; false: none.
 template <int G>
-__device__ __forceinline__ bool place(const LeakShape &s, int64_t &row, int &segment, int &lane)
+__device__ __forceinline__ bool place(const LeakShape &s, int &row, int &segment, int &lane)
 {
     const int64_t group = ((int64_t)blockIdx.x * kLeakThreads + threadIdx.x) / G;
     lane = threadIdx.x % G;
-    row = group;
     segment = 0;
-    if (s.segments > 1) {
-        row = quotient(group, s.segments);
-        segment = (int)(group - row * s.segments);
+    if (s.segments > 1) {       // (rows x segments is small then)
+        row = (int)((unsigned)group / (unsigned)s.segments);
+        segment = (int)group - row * s.segments;
+        return row < s.rows;
     }
-    return row < s.rows;
+    row = (int)group;
+    return group < s.rows;
 }
 
-__device__ __forceinline__ void row_gate(const LeakShape &s, const void *gate, int64_t row, double &f, float &rest)
+__device__ __forceinline__ Decay row_gate(const LeakShape &s, const void *gate, int row)
 {
-    f = 1.0, rest = 0.0f;
-    if (s.gate_period) {
-        const int64_t n = quotient(row, s.gate_inner);
-        decay_of(((const float *)gate)[n - quotient(n, s.gate_period) * s.gate_period], s.logit, f, rest);
-    }
+    if (s.gate_period == 0) return {1.0f, 0.0f};
+    return decay_of(__ldg((const float *)gate + (unsigned)row / (unsigned)s.gate_inner % (unsigned)s.gate_period), s.logit);
 }
 
-// Maps of segments: rows too few to fill the GPU are split, and each segment starts from the composition of those before it.
-template <typename E, int K>
+// Maps of segments: rows too few to fill the GPU are split, and each segment starts from what those before it leave.
+template <typename E, int K, bool FORWARD>
 __global__ void __launch_bounds__(kLeakThreads)
-leak_maps_kernel(Map *maps, const E *x, const void *gate, const E *g, const LeakShape s, bool forward)
+leak_maps_kernel(Map *maps, const E *x, const void *gate, const LeakShape s)
 {
-    int64_t row;
-    int segment, lane;
+    int row, segment, lane;
     if (!place<32>(s, row, segment, lane)) return;
     const Row r = row_of(s, row);
-    double row_f;
-    float row_rest;
-    row_gate(s, gate, row, row_f, row_rest);
-    Map all = {1.0, 0.0};
+    const Decay row_d = row_gate(s, gate, row);
+    Map all = {1.0f, 0.0f, 0.0f};
     const int first = segment * s.segment_chunks, last = min(first + s.segment_chunks, s.chunks);
     for (int i = first; i < last; ++i) {
-        const int c = forward ? i : last - 1 - (i - first);
+        const int c = FORWARD ? i : last - 1 - (i - first);
         Steps<E, K> st;
-        st.load(s, r, forward ? x : g, (const E *)gate, row_f, row_rest, (c * 32 + lane) * (4 * K) - r.skew);
-        Map m;
-        if (forward) {
+        st.load(s, r, x, (const E *)gate, row_d, Inside<K>((c * 32 + lane) * (4 * K) - r.skew, r.length));
+        if (FORWARD) {
             st.couple(s.coupled);
-            m = scan<32, true>(forward_map<E, K>(st), lane);
-            m = {__shfl_sync(~0u, m.a, 31), __shfl_sync(~0u, m.b, 31)};
+            all = compose(all, shift_from(scan<32, true>(forward_map<E, K>(st), lane), 31));
         } else {
-            m = scan<32, false>(backward_map<4 * K>(st.f, st.x), lane);
-            m = {__shfl_sync(~0u, m.a, 0), __shfl_sync(~0u, m.b, 0)};
+            all = compose(all, shift_from(scan<32, false>(backward_map<4 * K>(st.d, st.x, forward_map<E, K>(st)), lane), 0));
         }
-        all = compose(all, m);
     }
     if (lane == 0) maps[row * s.segments + segment] = all;
 }
 
 template <typename E, int G, int K>
-__global__ void __launch_bounds__(kLeakThreads)
+__global__ void __launch_bounds__(kLeakThreads, kForwardBlocks<K>)
 leak_forward_kernel(E *y, float *state, float *starts, const E *x, const void *gate, const float *initial, const Map *maps, const LeakShape s)
 {
-    int64_t row;
-    int segment, lane;
+    int row, segment, lane;
     const bool there = place<G>(s, row, segment, lane);
     if (G == 32 && !there) return;
     if (!there) row = s.rows - 1, segment = 0;      // the shuffles want every lane
     const Row r = row_of(s, row);
-    double row_f;
-    float row_rest;
-    row_gate(s, gate, row, row_f, row_rest);
+    const Decay row_d = row_gate(s, gate, row);
     double h = initial ? (double)initial[row] : 0.0;
-    if (G == 32 && segment > 0) h = segments_map<true>(maps + row * s.segments, 0, segment, lane)(h);
+    if (G == 32 && segment > 0) h = through_segments<true>(maps + row * s.segments, 0, segment, lane, h);
     const int first = segment * s.segment_chunks, last = min(first + s.segment_chunks, s.chunks);
     for (int c = first; c < last; ++c) {
-        if (starts && there && lane == 0) starts[row * s.chunks + c] = (float)h;
-        const int t = (c * G + lane) * (4 * K) - r.skew;
+        if (starts && there && lane == 0) starts[(int64_t)row * s.chunks + c] = (float)h;
+        const Inside<K> in((c * G + lane) * (4 * K) - r.skew, r.length);
         Steps<E, K> st;
-        st.load(s, r, x, (const E *)gate, row_f, row_rest, t);
+        st.load(s, r, x, (const E *)gate, row_d, in);
         st.couple(s.coupled);
-        double at = others<G, true>(scan<G, true>(forward_map<E, K>(st), lane), lane)(h);
-        float out[4 * K];
+        const Map m = scan<G, true>(forward_map<E, K>(st), lane);
+        float at = (float)others<G, true>(m, lane)(h);
+        h = __shfl_sync(~0u, m(h), G - 1, G);
 #pragma unroll
         for (int j = 0; j < 4 * K; ++j) {
-            at = fma(st.f[j], at, (double)st.x[j]);
-            out[j] = (float)at;
+            at = fmaf(st.d[j].f, at, st.x[j]);
+            st.x[j] = at;
         }
-        if (there) store_steps<E, K>(y + r.base, t, r.length, s.T, out);
-        h = __shfl_sync(~0u, at, G - 1, G);
+        if (there) store_steps<E, K>(y + r.base, in, s.T, st.x);
     }
     if (state && there && lane == 0 && segment == s.segments - 1) state[row] = (float)h;
 }
 
 // sums: per row and segment, of df: the gradient of a gate per row
 template <typename E, int G, int K>
-__global__ void __launch_bounds__(kLeakThreads)
+__global__ void __launch_bounds__(kLeakThreads, kBackwardBlocks<K>)
 leak_backward_kernel(E *dx, E *dgate, double *sums, float *dinitial, const E *g, const float *gstate, const float *starts, const E *x, const void *gate,
                      const Map *maps, const LeakShape s)
 {
     constexpr int N = 4 * K;
-    int64_t row;
-    int segment, lane;
+    int row, segment, lane;
     const bool there = place<G>(s, row, segment, lane);
     if (G == 32 && !there) return;
     if (!there) row = s.rows - 1, segment = 0;
     const Row r = row_of(s, row);
-    double row_f;
-    float row_rest;
-    row_gate(s, gate, row, row_f, row_rest);
+    const Decay row_d = row_gate(s, gate, row);
     double carry = gstate ? (double)gstate[row] : 0.0, sum = 0.0;
-    if (G == 32 && segment + 1 < s.segments) carry = segments_map<false>(maps + row * s.segments, segment + 1, s.segments, lane)(carry);
+    if (G == 32 && segment + 1 < s.segments) carry = through_segments<false>(maps + row * s.segments, segment + 1, s.segments, lane, carry);
     const int first = segment * s.segment_chunks, last = min(first + s.segment_chunks, s.chunks);
     for (int c = last - 1; c >= first; --c) {
-        const int t = (c * G + lane) * N - r.skew;
+        const Inside<K> in((c * G + lane) * N - r.skew, r.length);
         float gv[N], slope[N];       // slope: what lambda is multiplied by in dgate
         Steps<E, K> st;
-        st.load(s, r, x, (const E *)gate, row_f, row_rest, t);
-        load_steps<E, K>(gv, g + r.base, t, r.length, 0.0f);
-        const double start = (double)starts[row * s.chunks + c];
+        load_steps<E, K>(gv, g + r.base, in, 0.0f);
+        st.load(s, r, x, (const E *)gate, row_d, in);
+        const double start = (double)starts[(int64_t)row * s.chunks + c];
 #pragma unroll
         for (int j = 0; j < N; ++j) slope[j] = s.coupled ? st.x[j] : 0.0f;
         st.couple(s.coupled);
-        double at = others<G, true>(scan<G, true>(forward_map<E, K>(st), lane), lane)(start);
+        const Map steps = forward_map<E, K>(st);
+        float at = (float)others<G, true>(scan<G, true>(steps, lane), lane)(start);
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            slope[j] = (float)at - slope[j];
-            if (s.logit) slope[j] *= (float)st.f[j] * st.rest[j];
-            at = fma(st.f[j], at, (double)st.x[j]);
+            slope[j] = at - slope[j];
+            if (s.logit) slope[j] *= st.d[j].f * st.d[j].rest;
+            at = fmaf(st.d[j].f, at, st.x[j]);
         }
-        at = others<G, false>(scan<G, false>(backward_map<N>(st.f, gv), lane), lane)(carry);
+        const Map m = scan<G, false>(backward_map<N>(st.d, gv, steps), lane);
+        at = (float)others<G, false>(m, lane)(carry);
+        carry = __shfl_sync(~0u, m(carry), 0, G);
 #pragma unroll
         for (int j = N - 1; j >= 0; --j) {
-            const double lambda = at + (double)gv[j];
-            at = st.f[j] * lambda;
-            gv[j] = s.coupled ? (float)lambda * st.rest[j] : (float)lambda;
-            slope[j] *= (float)lambda;
+            const float lambda = gv[j] + at;
+            at = st.d[j].f * lambda;
+            gv[j] = s.coupled ? lambda * st.d[j].rest : lambda;
+            slope[j] *= lambda;
         }
-        if (there && dx) store_steps<E, K>(dx + r.base, t, r.length, s.T, gv);
-        if (there && dgate) store_steps<E, K>(dgate + r.base, t, r.length, s.T, slope);
+        if (there && dx) store_steps<E, K>(dx + r.base, in, s.T, gv);
+        if (there && dgate) store_steps<E, K>(dgate + r.base, in, s.T, slope);
         if (sums) {
 #pragma unroll
             for (int j = 0; j < N; ++j)
-                if (t + j >= 0 && t + j < r.length) sum += (double)slope[j];
+                if (in.t + j >= 0 && in.t + j < in.end) sum += (double)slope[j];
         }
-        carry = __shfl_sync(~0u, at, 0, G);
     }
     if (sums) {
 #pragma unroll
         for (int d = G / 2; d > 0; d /= 2) sum += __shfl_down_sync(~0u, sum, d, G);
-        if (there && lane == 0) sums[row * s.segments + segment] = sum;
+        if (there && lane == 0) sums[(int64_t)row * s.segments + segment] = sum;
     }
     if (dinitial && there && lane == 0 && segment == 0) dinitial[row] = (float)carry;
 }
@@ -407,11 +446,9 @@ leak_step_kernel(E *y, float *state, const E *x, const EG *gate, int64_t rows, i
 {
     const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (row >= rows) return;
-    double f;
-    float rest;
-    decay_of(to_float<EG>(gate[period ? row / inner % period : row]), logit, f, rest);
-    const float v = to_float<E>(x[row]);
-    const float h = (float)fma(f, (double)state[row], (double)(coupled ? rest * v : v));
+    const Decay d = decay_of(to_float<EG>(gate[period ? row / inner % period : row]), logit);
+    const float v = to_float<E>(x[row]), at = state[row];
+    const float h = (float)((double)(coupled ? d.rest * v : v) + (d.f < 0.5f ? (double)d.f * (double)at : fma(-(double)d.rest, (double)at, (double)at)));
     state[row] = h;
     y[row] = from_float<E>(h);
 }
@@ -469,16 +506,16 @@ static int plan_leak(LeakPlan &p, const char *op, int dtype, int flags, int64_t 
     SB200_REQUIRE(known(dtype), "%s: unknown element type %d", op, dtype);
     SB200_REQUIRE((flags & ~3) == 0, "%s: unknown flags %d", op, flags);
     SB200_REQUIRE(rows >= 0 && T >= 0, "%s: negative size", op);
-    SB200_REQUIRE(rows <= (int64_t)1 << 40 && T <= (int64_t)1 << 30 && rows * (T >> 20) <= (int64_t)1 << 40, "%s: sizes overflow", op);
+    SB200_REQUIRE(rows <= ((int64_t)1 << 31) - 64 && T <= (int64_t)1 << 30, "%s: at most 2^31 - 64 rows of 2^30 steps", op);
     SB200_REQUIRE(gate_period >= 0 && (gate_period == 0 || gate_inner >= 1), "%s: bad gate layout", op);
     SB200_REQUIRE(gate_period == 0 || (gate_period <= rows && gate_inner <= rows && rows % (gate_inner * gate_period) == 0) || rows == 0,
                   "%s: rows must be whole groups of gates", op);
     SB200_REQUIRE(!lengths || sample_rows >= 1, "%s: lengths need the number of rows that have one", op);
     p.l = lanes_of(T);
     const int64_t chunks = chunks_of(T), segments = rows ? segments_of(rows, T) : 1;
-    p.s = {rows, (int)T, gate_inner, gate_period, sample_rows, lengths, (int)chunks, (int)segments, (int)ceil_div(chunks, segments),
-           (flags & SLAYER_B200_LEAK_LOGIT) != 0, (flags & SLAYER_B200_LEAK_COUPLED) != 0};
-    p.maps_bytes = segments > 1 ? rows * segments * (int64_t)sizeof(Map) : 0;
+    p.s = {(int)rows, (int)T, (int)gate_inner, (int)gate_period, (int)(sample_rows < rows ? sample_rows : rows), lengths, (int)chunks, (int)segments,
+           (int)ceil_div(chunks, segments), (flags & SLAYER_B200_LEAK_LOGIT) != 0, (flags & SLAYER_B200_LEAK_COUPLED) != 0};
+    p.maps_bytes = segments > 1 ? ceil_div(rows * segments * (int64_t)sizeof(Map), 16) * 16 : 0;
     p.sums_bytes = p.gate_parts = 0;
     if (gate_period && rows) {
         const int64_t count = rows / gate_period * segments;
@@ -496,9 +533,9 @@ static void run_forward(const LeakPlan &p, void *y, float *state, float *starts,
                         cudaStream_t st)
 {
     Map *maps = (Map *)workspace;
-    const unsigned blocks = (unsigned)ceil_div(p.s.rows * p.s.segments * G, kLeakThreads);
+    const unsigned blocks = (unsigned)ceil_div((int64_t)p.s.rows * p.s.segments * G, kLeakThreads);
     if constexpr (G == 32)
-        if (p.s.segments > 1) leak_maps_kernel<E, K><<<blocks, kLeakThreads, 0, st>>>(maps, (const E *)x, gate, nullptr, p.s, true);
+        if (p.s.segments > 1) leak_maps_kernel<E, K, true><<<blocks, kLeakThreads, 0, st>>>(maps, (const E *)x, gate, p.s);
     leak_forward_kernel<E, G, K><<<blocks, kLeakThreads, 0, st>>>((E *)y, state, starts, (const E *)x, gate, initial, maps, p.s);
 }
 
@@ -509,14 +546,14 @@ static void run_backward(const LeakPlan &p, void *dx, void *dgate, float *diniti
     Map *maps = (Map *)workspace;
     double *sums = (double *)((char *)workspace + p.maps_bytes);
     const bool per_row = p.s.gate_period > 0;
-    const unsigned blocks = (unsigned)ceil_div(p.s.rows * p.s.segments * G, kLeakThreads);
+    const unsigned blocks = (unsigned)ceil_div((int64_t)p.s.rows * p.s.segments * G, kLeakThreads);
     if constexpr (G == 32)
-        if (p.s.segments > 1) leak_maps_kernel<E, K><<<blocks, kLeakThreads, 0, st>>>(maps, nullptr, gate, (const E *)g, p.s, false);
+        if (p.s.segments > 1) leak_maps_kernel<E, K, false><<<blocks, kLeakThreads, 0, st>>>(maps, (const E *)g, gate, p.s);
     leak_backward_kernel<E, G, K><<<blocks, kLeakThreads, 0, st>>>((E *)dx, per_row ? nullptr : (E *)dgate, per_row && dgate ? sums : nullptr, dinitial,
                                                                 (const E *)g, gstate, starts, (const E *)x, gate, maps, p.s);
     if (per_row && dgate) {
-        const int64_t inner = p.s.gate_inner * p.s.segments, outer = p.s.rows / (p.s.gate_inner * p.s.gate_period);
-        double *part = sums + p.s.rows * p.s.segments;
+        const int64_t inner = (int64_t)p.s.gate_inner * p.s.segments, outer = p.s.rows / ((int64_t)p.s.gate_inner * p.s.gate_period);
+        double *part = sums + (int64_t)p.s.rows * p.s.segments;
         const unsigned gates = (unsigned)p.s.gate_period;
         if (p.gate_parts > 1) {
             leak_gate_sum_kernel<<<gates * (unsigned)p.gate_parts, 256, 0, st>>>(part, nullptr, sums, outer, p.s.gate_period, inner, p.gate_parts);

@@ -1,11 +1,15 @@
-"""GPU: the gated leaky integrator against the recurrence in double, a step after another.
+"""GPU: the gated leaky integrator against the recurrence in double.
 
-Tolerances.  f = sigmoid(gate) comes from e = exp(-|gate|) (2 steps of 2^-23 off at most), 1 / (1 + e) (2 steps) and their product (half a
-step): the smaller of f and 1 - f is off by less than D = 10 * 2^-24 of itself, and the larger by D of itself at most.  What
-this does to a state is followed along the recurrence (`want`): each step adds D min(f, 1 - f) |y_before|, and for a coupled input
-(D + 2^-24) (1 - f) |x|, to f times the error so far; the maps and states themselves are double.  The backward pass starts from states of
-32 bits and forms differences and products there, at 2^-24 of each.  A result is rounded to its type: half a step of it, and
-2^-24 on the way through float32."""
+Tolerances, in steps of S = 2^-24.
+f = sigmoid(gate): e = 2^z, z = -|gate| log2(e), is off by half a step of z, |gate| S at most, and 4 S of the power itself; 1 + e, its
+reciprocal and their product add 4 S: the smaller of f and 1 - f is off by D = (8 + |gate|) S of itself.
+A lane's map of up to 16 steps: f is rounded once more and each step rounds once, so that what is added (B) is off by 32 S of its terms'
+magnitudes, the product A of f's by 32 S of itself, R = 1 - A by 48 S.  Composing two maps, R is off by r (R1 + R2) / (R1 + R2 - R1 R2) + 2, at
+most 1.4 times as much while it is used (below 1/2), A by what R is or, beyond, by the sum of both, which is less than the same multiple of
+what the steps forget; B by what is lost of the first map's.  So all of it is as if each step forgot, and added, 160 S of itself too much or
+too little: followed along the recurrence (`want`) with magnitudes that no sign cancels.  The walk of up to 16 steps from a lane's state
+rounds f and the result, 3 S of the largest state each time.  States between calls and for the backward pass are 32 bits, differences and
+products there are rounded once.  A result is rounded to its type: half a step of it, and S on the way through float32."""
 import pytest
 import torch
 
@@ -16,7 +20,7 @@ pytestmark = pytest.mark.gpu
 
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
 STEP = 2.0 ** -24
-D = 10 * STEP
+MAPS = 160 * STEP
 
 
 def scan(f, u, first):
@@ -37,42 +41,52 @@ def shifted(h, first):
     return torch.cat([first[:, None], h[:, :-1]], 1)
 
 
+def window(v):
+    """sums over a step and the 16 before it"""
+    total = torch.nn.functional.pad(v, (17, 0)).cumsum(1)
+    return total[:, 17:] - total[:, :-17] + 1e-12 * total[:, -1:]
+
+
 def want(x, gate, initial, lengths, kind, coupled, g=None, gstate=None):
     """(value, bound) of y, the last state and, with g, the gradients of x, gate (per step) and initial; rows [R, T], in double"""
     x, gate = x.double(), gate.double().expand(x.shape)
     R, T = x.shape
     f = torch.sigmoid(gate) if kind == 'logit' else gate
     rest = torch.sigmoid(-gate) if kind == 'logit' else 1.0 - gate
-    off = D * torch.minimum(f, rest) if kind == 'logit' else torch.zeros_like(f)
-    offr = (D if kind == 'logit' else STEP) * rest.abs()
+    D = (8 + gate.abs()) * STEP if kind == 'logit' else torch.full_like(f, STEP)
+    off, offr = (D + MAPS) * torch.minimum(f, rest), D * torch.minimum(f, rest) + STEP * rest
     on = torch.arange(T, device=x.device)[None] < (torch.full((R,), T, device=x.device) if lengths is None else lengths)[:, None]
     x = torch.where(on, x, 0.0)
     u = rest * x if coupled else x
-    offu = offr * x.abs() + STEP * u.abs() if coupled else torch.zeros_like(x)
+    offu = MAPS * u.abs() + (offr * x.abs() + STEP * u.abs() if coupled else 0.0)
     zero = torch.zeros(R, dtype=torch.float64, device=x.device)
     h0 = zero if initial is None else initial.double()
     keep = torch.where(on, f, 1.0)                       # behind a length the state stays what it is
     h = scan(keep, torch.where(on, u, 0.0), h0)
+    size = scan(keep, torch.where(on, u.abs(), 0.0), h0.abs())
     before = shifted(h, h0)
-    e = scan(keep.abs(), torch.where(on, (off + 1e-14) * before.abs() + offu, 0.0), zero)
-    out = [(h * on, e * on), (h[:, -1], e[:, -1])]
+    e = scan(keep, torch.where(on, off * shifted(size, h0.abs()) + offu, 0.0), zero)
+    walk = 3 * STEP * (window(size) + h0.abs()[:, None])
+    out = [(h * on, (e + walk) * on), (h[:, -1], e[:, -1])]
     if g is None:
         return out
     g = torch.where(on, g.double(), 0.0)
     gs = zero if gstate is None else gstate.double()
     # c_t = f_t (g_t + c_{t+1}): what step t hands back
     c = scan(keep.flip(1), (keep * g).flip(1), gs).flip(1)
-    lam = g + torch.cat([c[:, 1:], gs[:, None]], 1)
-    ec = scan(keep.abs().flip(1), torch.where(on, (off + 1e-14) * lam.abs() + STEP * (f * lam).abs(), 0.0).flip(1), zero).flip(1)
-    el = torch.cat([ec[:, 1:], zero[:, None]], 1) + STEP * lam.abs()
+    csize = scan(keep.flip(1), (keep * g.abs()).flip(1), gs.abs()).flip(1)
+    after = lambda v, last: torch.cat([v[:, 1:], last[:, None]], 1)  # noqa: E731
+    lam, lsize = g + after(c, gs), g.abs() + after(csize, gs.abs())
+    ec = scan(keep.flip(1), torch.where(on, off * lsize + MAPS * f * g.abs(), 0.0).flip(1), zero).flip(1)
+    el = after(ec, zero) + 3 * STEP * (window(lsize.flip(1)).flip(1) + gs.abs()[:, None])
     # a state of 32 bits at a chunk's start, carried on
-    eb = shifted(e, zero) + 2 * STEP * torch.maximum(before.abs().amax(1, keepdim=True), before.abs())
+    eb = shifted(e + walk, zero) + 2 * STEP * torch.maximum(before.abs().amax(1, keepdim=True), size)
     r = rest if coupled else torch.ones_like(rest)
     dx, edx = lam * r, el * r.abs() + lam.abs() * ((offr if coupled else 0.0) + STEP * r.abs())
     d = before - x if coupled else before
     ed = eb + STEP * d.abs()
     m = f * rest if kind == 'logit' else torch.ones_like(f)
-    dg, edg = lam * d * m, (el * d.abs() + lam.abs() * ed) * m.abs() + (2 * D + 4 * STEP) * (lam * d * m).abs()
+    dg, edg = lam * d * m, (el * d.abs() + lam.abs() * ed) * m.abs() + (2 * D + 6 * STEP) * (lam * d * m).abs()
     return out + [(dx * on, edx * on), (dg * on, edg * on), (c[:, 0], ec[:, 0])]
 
 
@@ -218,8 +232,8 @@ def test_a_slow_leak_over_many_steps():
     y = gatedLeak(x, gate)
     f = torch.sigmoid(gate[0, 0].double())
     value = (1 - f ** torch.arange(1, T + 1, device="cuda", dtype=torch.float64)) / (1 - f)
-    # an error of D in 1 - f changes the sum of its powers by D of itself at most
-    close(y, value.expand(2, T), (D * value).expand(2, T))
+    # what is forgotten too much changes the sum by as much of itself at most; the walk: 17 times 3 steps
+    close(y, value.expand(2, T), ((8 + 9.9 + 2 * 160 + 51) * STEP * value).expand(2, T))
 
 
 def test_streams_of_parts_and_of_single_steps():
