@@ -115,9 +115,9 @@ __device__ __forceinline__ void load_steps(float (&v)[4 * K], const E *row, cons
     }
 }
 
-// results of steps in [0, end), zeros in [end, T)
+// results of the steps inside
 template <typename E, int K>
-__device__ __forceinline__ void store_steps(E *row, const Inside<K> &in, int T, const float (&v)[4 * K])
+__device__ __forceinline__ void store_inside(E *row, const Inside<K> &in, const float (&v)[4 * K])
 {
     using P = typename Packed<E>::type;
 #pragma unroll
@@ -128,16 +128,29 @@ __device__ __forceinline__ void store_steps(E *row, const Inside<K> &in, int T, 
         for (int j = 0; j < 4; ++j) e[j] = from_float<E>(v[4 * k + j]);
         if (in.whole[k]) *reinterpret_cast<P *>(row + in.t + 4 * k) = raw;
     }
-    if (in.part || in.end < T) {
+    if (in.part) {
 #pragma unroll
         for (int k = 0; k < K; ++k)
             if (!in.whole[k]) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int at = in.t + 4 * k + j;
-                    if (at >= 0 && at < T) row[at] = from_float<E>(at < in.end ? v[4 * k + j] : 0.0f);
+                    if (at >= 0 && at < in.end) row[at] = from_float<E>(v[4 * k + j]);
                 }
             }
+    }
+}
+
+// and zeros from `in.end` to T
+template <typename E, int K>
+__device__ __forceinline__ void store_steps(E *row, const Inside<K> &in, int T, float (&v)[4 * K])
+{
+    if (in.end == T) {
+        store_inside<E, K>(row, in, v);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4 * K; ++j) v[j] = in.t + j < in.end ? v[j] : 0.0f;
+        store_inside<E, K>(row, Inside<K>(in.t, T), v);
     }
 }
 
@@ -296,10 +309,14 @@ __device__ __forceinline__ bool place(const LeakShape &s, int &row, int &segment
     return group < s.rows;
 }
 
+// (one for a whole row: as exact as 32 bits can be)
 __device__ __forceinline__ Decay row_gate(const LeakShape &s, const void *gate, int row)
 {
     if (s.gate_period == 0) return {1.0f, 0.0f};
-    return decay_of(__ldg((const float *)gate + (unsigned)row / (unsigned)s.gate_inner % (unsigned)s.gate_period), s.logit);
+    const float g = __ldg((const float *)gate + (unsigned)row / (unsigned)s.gate_inner % (unsigned)s.gate_period);
+    if (!s.logit) return {g, 1.0f - g};
+    const float e = expf(-fabsf(g)), small = __fdiv_rn(e, 1.0f + e);
+    return g < 0.0f ? Decay{small, 1.0f - small} : Decay{1.0f - small, small};
 }
 
 // Maps of segments: rows too few to fill the GPU are split, and each segment starts from what those before it leave.
@@ -406,9 +423,10 @@ leak_backward_kernel(E *dx, E *dgate, double *sums, float *dinitial, const E *g,
         if (there && dx) store_steps<E, K>(dx + r.base, in, s.T, gv);
         if (there && dgate) store_steps<E, K>(dgate + r.base, in, s.T, slope);
         if (sums) {
+            float part = 0.0f;
 #pragma unroll
-            for (int j = 0; j < N; ++j)
-                if (in.t + j >= 0 && in.t + j < in.end) sum += (double)slope[j];
+            for (int j = 0; j < N; ++j) part += (unsigned)(in.t + j) < (unsigned)in.end ? slope[j] : 0.0f;
+            sum += (double)part;
         }
     }
     if (sums) {

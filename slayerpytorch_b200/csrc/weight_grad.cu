@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) weight_grad_kernel(const __grid
         const uint8_t *as = A.scale;
         const float *bg = A.g;
         int b_far[kItems];              // its rows of g from the first one on
-        WgUnit ua, ub;
+        WgUnit ua = {}, ub = {};
         unsigned scale_0 = 127, scale_1 = 127;
         int64_t i = 0, o = 0;
         const auto find_a = [&] {
