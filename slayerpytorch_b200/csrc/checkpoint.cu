@@ -26,12 +26,9 @@ template <> __device__ __forceinline__ __nv_bfloat16 as_type<__nv_bfloat16>(floa
 template <> __device__ __forceinline__ __half as_type<__half>(float v) { return __float2half_rn(v); }
 
 // Byte of the scale for a largest magnitude given by its bits.  With amax = m 2^k, 1 <= m < 2: amax <= 127 2^(k-6) where m <= 127/64, else
-// 127 2^(k-5).  From 2^-126 on, and up to 2^121, so that 127 2^e is finite (multiples beyond 127 are cut there: by less than a step).
-__device__ __forceinline__ unsigned scale_byte(unsigned amax)
-{
-    const int e = (int)(amax >> 23) - 6 + ((amax & 0x7fffff) > 0x7e0000);
-    return (unsigned)min(max(e, 1), 248);
-}
+// 127 2^(k-5): one more where the mantissa is above 0x7e0000.  From 2^-126 on, and up to 2^121, so that 127 2^e is finite (multiples
+// beyond 127 are cut there: by less than a step).
+__device__ __forceinline__ unsigned scale_byte(unsigned amax) { return (unsigned)min(max((int)((amax + 0x1ffffu) >> 23) - 6, 1), 248); }
 
 __device__ __forceinline__ int quantise(float v, unsigned byte)
 {
@@ -47,26 +44,30 @@ __device__ __forceinline__ int quantise(float v, unsigned byte)
 struct Pieces {
     int64_t rows, T, G;
     int64_t each, all;           // pieces of a row, of all rows
-    unsigned magic;              // 2^32 / each, rounded up: exact quotients of numbers below 4096 for each < 1024
+    // 2^64 / each and 2^32 / each, rounded up (0 for 1): the upper half of a product is an exact quotient for numbers below 2^64 / each, or below
+    // 4096 (each < 1024).  A division of 64 bits is 100 instructions, half of what 16 bytes take otherwise.
+    uint64_t magic_far;
+    unsigned magic;
 };
 
 template <int kBlock>
 struct Place {
     static_assert(kBlock <= 1024, "a CTA's pieces");
-    int64_t first, row0;
-    unsigned rest0;
+    int64_t first, row0;         // of the CTA: piece, row
+    unsigned rest0, here;        // which piece of its row the first one is; pieces
     __device__ __forceinline__ Place(const Pieces &s)
     {
         first = (int64_t)blockIdx.x * kBlock;
-        row0 = first / s.each;
+        row0 = s.magic_far ? (int64_t)__umul64hi((uint64_t)first, s.magic_far) : first;
         rest0 = (unsigned)(first - row0 * s.each);
+        here = (unsigned)min(s.all - first, (int64_t)kBlock);
     }
     // rows from the CTA's first one, and which piece of its row the CTA's local-th one is
     __device__ __forceinline__ void operator()(const Pieces &s, unsigned local, unsigned &down, unsigned &piece) const
     {
         const unsigned r = rest0 + local, each = (unsigned)s.each;
         if (each >= 1024) down = r >= each;
-        else down = each == 1 ? r : __umulhi(r, s.magic);
+        else down = s.magic ? __umulhi(r, s.magic) : r;
         piece = r - down * each;
     }
 };
@@ -82,31 +83,33 @@ compress_kernel(int8_t *q, uint8_t *scale, const E *x, const Pieces s)
 {
     constexpr int W = 16 / (int)sizeof(E), kLanes = 32 / W;
     const Place<kCompressBlock<E>> place(s);
-    const unsigned t = (threadIdx.x % kLanes) * W, pad = (unsigned)(s.G * kGroup - s.T);
-    const E *const x0 = x + place.row0 * s.T;
+    const unsigned t = (threadIdx.x % kLanes) * W, T = (unsigned)s.T, pad = (unsigned)(s.G * kGroup - s.T), lane0 = threadIdx.x / kLanes;
+    const E *const x0 = x + (place.row0 * s.T + place.rest0 * (int64_t)kGroup);        // (of the CTA's first group)
+    int8_t *const q0 = q + place.first * kGroup;
+    uint8_t *const scale0 = scale + place.row0;
     unsigned down[kCompressUnroll], group[kCompressUnroll];
     float v[kCompressUnroll][W];
 #pragma unroll
     for (int u = 0; u < kCompressUnroll; ++u) {
-        const unsigned local = u * (256 / kLanes) + threadIdx.x / kLanes;
+        const unsigned local = u * (256 / kLanes) + lane0;
         place(s, local, down[u], group[u]);
-        const E *p = x0 + (place.rest0 + local) * kGroup - down[u] * pad + t;
+        const E *p = x0 + (int)(local * kGroup + t - down[u] * pad);
         const unsigned at = group[u] * kGroup + t;
-        const bool there = place.first + local < s.all;
         if (LINED) {
             uint4 raw = make_uint4(0, 0, 0, 0);
-            if (there && at < (unsigned)s.T) raw = __ldg(reinterpret_cast<const uint4 *>(p));
+            if (local < place.here && at < T) raw = __ldg(reinterpret_cast<const uint4 *>(p));
             const E *e = reinterpret_cast<const E *>(&raw);
 #pragma unroll
             for (int j = 0; j < W; ++j) v[u][j] = as_float<E>(e[j]);
         } else {
+            const unsigned end = local < place.here ? T : 0;
 #pragma unroll
-            for (int j = 0; j < W; ++j) v[u][j] = there && at + j < (unsigned)s.T ? as_float<E>(__ldg(p + j)) : 0.0f;
+            for (int j = 0; j < W; ++j) v[u][j] = at + j < end ? as_float<E>(__ldg(p + j)) : 0.0f;
         }
     }
 #pragma unroll
     for (int u = 0; u < kCompressUnroll; ++u) {
-        const unsigned local = u * (256 / kLanes) + threadIdx.x / kLanes;
+        const unsigned local = u * (256 / kLanes) + lane0;
         unsigned top = 0;
 #pragma unroll
         for (int j = 0; j < W; ++j) top = max(top, __float_as_uint(v[u][j]) & 0x7fffffffu);
@@ -115,7 +118,7 @@ compress_kernel(int8_t *q, uint8_t *scale, const E *x, const Pieces s)
         unsigned byte, out[W / 4];
         if (!__any_sync(~0u, top >= 0x7e800000u)) {
             // whole multiples by adding 1.5 2^23, in whose last byte they are then: rounded to nearest, ties to even
-            byte = scale_byte(top);
+            byte = (unsigned)max((int)((top + 0x1ffffu) >> 23) - 6, 1);
             const float inverse = __uint_as_float((254u - byte) << 23);
 #pragma unroll
             for (int j = 0; j < W; j += 4) {
@@ -142,11 +145,11 @@ compress_kernel(int8_t *q, uint8_t *scale, const E *x, const Pieces s)
                 for (int l = 0; l < 4; ++l) out[j / 4] |= (unsigned)(quantise(v[u][j + l], byte) & 0xff) << (8 * l);
             }
         }
-        if (place.first + local < s.all) {
-            unsigned *to = reinterpret_cast<unsigned *>(q + (place.first + local) * kGroup + t);
+        if (local < place.here) {
+            unsigned *to = reinterpret_cast<unsigned *>(q0 + (local * kGroup + t));
             if (W == 4) to[0] = out[0];
             else *reinterpret_cast<uint2 *>(to) = make_uint2(out[0], out[W / 4 - 1]);
-            if (t == 0) scale[group[u] * s.rows + place.row0 + down[u]] = (uint8_t)byte;
+            if (t == 0) scale0[(int64_t)group[u] * s.rows + down[u]] = (uint8_t)byte;
         }
     }
 }
@@ -159,37 +162,53 @@ struct Kept {
     uint32_t word[kWords];
     unsigned byte, next;         // scales of the first step's group and of the one after it
 
+    // q and scale of the CTA's first row; down: rows from there
     template <bool LINED>
-    __device__ __forceinline__ void load(const int8_t *q, const uint8_t *scale, const Pieces &s, int64_t row, int t)
+    __device__ __forceinline__ void load(const uint32_t *q, const uint8_t *scale, const Pieces &s, unsigned down, int t)
     {
-        const uint32_t *const p = reinterpret_cast<const uint32_t *>(q) + row * (s.G * (kGroup / 4));
-        const int last = (int)(s.G * (kGroup / 4)) - 1, at = t >> 2;
+        const int words = (int)s.G * (kGroup / 4), at = t >> 2;
+        const uint32_t *const p = q + down * (unsigned)words;
         if (LINED && W == 8) {
             const uint2 two = __ldg(reinterpret_cast<const uint2 *>(p + at));
             word[0] = two.x;
             word[1] = two.y;
         } else {
 #pragma unroll
-            for (int k = 0; k < (LINED ? W / 4 : kWords); ++k) word[k] = __ldg(p + (LINED ? at + k : min(max(at + k, 0), last)));
+            for (int k = 0; k < (LINED ? W / 4 : kWords); ++k) word[k] = __ldg(p + (LINED ? at + k : min(max(at + k, 0), words - 1)));
         }
-        const int group = max(t, 0) >> 5;
-        byte = __ldg(scale + group * s.rows + row);
-        next = byte;
-        if (!LINED && t > 0 && (t & 31) > 32 - W && group + 1 < (int)s.G) next = __ldg(scale + (group + 1) * s.rows + row);
+        const int group = (LINED ? t : max(t, 0)) >> 5;
+        const uint8_t *const g = scale + ((int64_t)group * s.rows + down);
+        byte = __ldg(g);
+        if (!LINED) next = t > 0 && (t & 31) > 32 - W && group + 1 < (int)s.G ? __ldg(g + s.rows) : byte;
     }
     template <bool LINED>
     __device__ __forceinline__ void restore(float (&v)[W], int t) const
     {
-        const float s0 = __uint_as_float(byte << 23), s1 = __uint_as_float(next << 23);
+        constexpr float kBias = 8388608.0f + 128.0f;
+        const float s0 = __uint_as_float(byte << 23);
+        uint32_t w[W / 4], none = 0;
 #pragma unroll
         for (int k = 0; k < W / 4; ++k) {
-            const uint32_t w = (LINED ? word[k] : __funnelshift_r(word[k], word[k + 1], (t & 3) * 8)) ^ 0x80808080u;       // q + 128
+            w[k] = (LINED ? word[k] : __funnelshift_r(word[k], word[k + 1], (t & 3) * 8)) ^ 0x80808080u;       // q + 128
+            none |= (w[k] - 0x01010101u) & ~w[k];                                                             // a byte of 0: q is -128
+        }
+        if (!(none & 0x80808080u) && max(byte, LINED ? 0u : next) < 220u) {
+            // 2^23 + q + 128 is the float that ends in that byte; times the scale, minus (2^23 + 128) times it: exact
+            const float c0 = -kBias * s0;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                // 2^23 + q + 128 is the float that ends in that byte
-                const float n = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7540 | j));
-                const float f = (n - 8388736.0f) * (LINED || (t & 31) + 4 * k + j < 32 ? s0 : s1);
-                v[4 * k + j] = n == 8388608.0f ? __uint_as_float(0x7fc00000u) : f;
+            for (int j = 0; j < W; ++j) v[j] = fmaf(__uint_as_float(__byte_perm(w[j / 4], 0x4b000000u, 0x7540 | (j % 4))), s0, c0);
+            if (!LINED && next != byte) {
+                const float s1 = __uint_as_float(next << 23), c1 = -kBias * s1;
+#pragma unroll
+                for (int j = 1; j < W; ++j)
+                    if ((t & 31) + j >= 32) v[j] = fmaf(__uint_as_float(__byte_perm(w[j / 4], 0x4b000000u, 0x7540 | (j % 4))), s1, c1);
+            }
+        } else {
+            // something that was not finite, or products that would not be
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                const int q = (int)((w[j / 4] >> (8 * (j % 4))) & 0xff) - 128;
+                v[j] = q == -128 ? __uint_as_float(0x7fc00000u) : (float)q * __uint_as_float((LINED || (t & 31) + j < 32 ? byte : next) << 23);
             }
         }
     }
@@ -214,16 +233,15 @@ __device__ __forceinline__ void store_steps(E *p, int t, int T, const float (&v)
 
 constexpr int kReadUnroll = 4, kReadBlock = 256 * kReadUnroll;
 
-// the u-th 16 bytes of a thread: its row, and the step that they begin with
+// the u-th 16 bytes of a thread: rows from the CTA's first one, and the step that they begin with
 template <int W, bool LINED>
-__device__ __forceinline__ bool read_place(const Pieces &s, const Place<kReadBlock> &place, int u, int64_t &row, int &t)
+__device__ __forceinline__ bool read_place(const Pieces &s, const Place<kReadBlock> &place, int u, unsigned &down, int &t)
 {
     const unsigned local = u * 256 + threadIdx.x;
-    unsigned down, piece;
+    unsigned piece;
     place(s, local, down, piece);
-    row = place.row0 + down;
-    t = (int)piece * W - (LINED ? 0 : (int)(((unsigned)row * (unsigned)s.T) & (W - 1)));
-    return place.first + local < s.all && t < (int)s.T;
+    t = (int)piece * W - (LINED ? 0 : (int)((((unsigned)place.row0 + down) * (unsigned)s.T) & (W - 1)));
+    return local < place.here && t < (int)s.T;
 }
 
 template <typename E, bool LINED>
@@ -232,49 +250,59 @@ restore_kernel(E *out, const int8_t *q, const uint8_t *scale, const Pieces s)
 {
     constexpr int W = 16 / (int)sizeof(E);
     const Place<kReadBlock> place(s);
-    int64_t row[kReadUnroll];
+    E *const out0 = out + place.row0 * s.T;
+    const uint32_t *const q0 = reinterpret_cast<const uint32_t *>(q) + place.row0 * (s.G * (kGroup / 4));
+    const uint8_t *const scale0 = scale + place.row0;
+    unsigned down[kReadUnroll];
     int t[kReadUnroll];
     bool there[kReadUnroll];
     Kept<W> kept[kReadUnroll];
 #pragma unroll
     for (int u = 0; u < kReadUnroll; ++u) {
-        there[u] = read_place<W, LINED>(s, place, u, row[u], t[u]);
-        if (there[u]) kept[u].template load<LINED>(q, scale, s, row[u], t[u]);
+        there[u] = read_place<W, LINED>(s, place, u, down[u], t[u]);
+        if (there[u]) kept[u].template load<LINED>(q0, scale0, s, down[u], t[u]);
     }
 #pragma unroll
     for (int u = 0; u < kReadUnroll; ++u)
         if (there[u]) {
             float v[W];
             kept[u].template restore<LINED>(v, t[u]);
-            store_steps<E, LINED>(out + row[u] * s.T + t[u], t[u], (int)s.T, v);
+            store_steps<E, LINED>(out0 + ((int)(down[u] * (unsigned)s.T) + t[u]), t[u], (int)s.T, v);
         }
 }
 
 // The surrogate gradient (as spike_grad.cu has it) on a membrane potential in 8 bits: g c exp(-|u - theta| / tau), c = scale / tau, the exponential as
-// 2^(-|u - theta| k) with k = log2(e) / tau in two floats, so that the product is rounded once, as a division would be.
+// 2^(-|u - theta| k) with k = log2(e) / tau in two floats, so that the product is rounded once, as a division would be.  Exponentials
+// below 1.2e-38 are zero.
 template <bool LINED>
 __global__ void __launch_bounds__(256)
 spike_grad_8_kernel(float *out, const float *g, const int8_t *q, const uint8_t *scale, const Pieces s, float theta, float k, float k_rest, float c)
 {
     const Place<kReadBlock> place(s);
-    int64_t row[kReadUnroll];
-    int t[kReadUnroll];
+    const float *const g0 = g + place.row0 * s.T;
+    float *const out0 = out + place.row0 * s.T;
+    const uint32_t *const q0 = reinterpret_cast<const uint32_t *>(q) + place.row0 * (s.G * (kGroup / 4));
+    const uint8_t *const scale0 = scale + place.row0;
+    const int T = (int)s.T;
+    int at[kReadUnroll], t[kReadUnroll];
     bool there[kReadUnroll];
     Kept<4> kept[kReadUnroll];
     float4 gv[kReadUnroll];
 #pragma unroll
     for (int u = 0; u < kReadUnroll; ++u) {
-        there[u] = read_place<4, LINED>(s, place, u, row[u], t[u]);
+        unsigned down;
+        there[u] = read_place<4, LINED>(s, place, u, down, t[u]);
+        at[u] = (int)(down * (unsigned)T) + t[u];
         if (!there[u]) continue;
-        kept[u].template load<LINED>(q, scale, s, row[u], t[u]);
-        const float *p = g + row[u] * s.T + t[u];
-        if (LINED || (t[u] >= 0 && t[u] + 4 <= (int)s.T)) {
+        kept[u].template load<LINED>(q0, scale0, s, down, t[u]);
+        const float *p = g0 + at[u];
+        if (LINED || (t[u] >= 0 && t[u] + 4 <= T)) {
             gv[u] = *reinterpret_cast<const float4 *>(p);
         } else {
             gv[u].x = t[u] >= 0 ? p[0] : 0.0f;
-            gv[u].y = t[u] + 1 >= 0 && t[u] + 1 < (int)s.T ? p[1] : 0.0f;
-            gv[u].z = t[u] + 2 >= 0 && t[u] + 2 < (int)s.T ? p[2] : 0.0f;
-            gv[u].w = t[u] + 3 < (int)s.T ? p[3] : 0.0f;
+            gv[u].y = t[u] + 1 >= 0 && t[u] + 1 < T ? p[1] : 0.0f;
+            gv[u].z = t[u] + 2 >= 0 && t[u] + 2 < T ? p[2] : 0.0f;
+            gv[u].w = t[u] + 3 < T ? p[3] : 0.0f;
         }
     }
 #pragma unroll
@@ -286,9 +314,11 @@ spike_grad_8_kernel(float *out, const float *g, const int8_t *q, const uint8_t *
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const float d = fabsf(v[j] - theta);
-                v[j] = up[j] * (c * exp2f(-fmaf(d, k, d * k_rest)));
+                float e;
+                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-fmaf(d, k, d * k_rest)));
+                v[j] = up[j] * (c * e);
             }
-            store_steps<float, LINED>(out + row[u] * s.T + t[u], t[u], (int)s.T, v);
+            store_steps<float, LINED>(out0 + at[u], t[u], T, v);
         }
 }
 
@@ -306,7 +336,8 @@ static int check_rows(const char *op, int64_t rows, int64_t T)
 
 static Pieces pieces_of(int64_t rows, int64_t T, int64_t each)
 {
-    return {rows, T, ceil_div(T, kGroup), each, rows * each, each < 1024 ? (unsigned)((((uint64_t)1 << 32) + each - 1) / each) : 0u};
+    const uint64_t far = each == 1 ? 0 : ~(uint64_t)0 / (uint64_t)each + 1;
+    return {rows, T, ceil_div(T, kGroup), each, rows * each, far, each == 1 || each >= 1024 ? 0u : (unsigned)((((uint64_t)1 << 32) + each - 1) / each)};
 }
 
 template <typename E>
