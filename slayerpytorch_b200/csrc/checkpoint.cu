@@ -72,43 +72,50 @@ struct Place {
     }
 };
 
-// 16 bytes a thread: kLanes of them have a group.  LINED: all rows' steps lie on 16 bytes; else they are loaded one by one (a line's other steps are in L1 by
-// then: 52 us instead of 142 with a lane for each step of a group, 64 x 2312 x 301).
-constexpr int kCompressUnroll = 4;
-template <typename E> constexpr int kCompressBlock = 256 / (32 * (int)sizeof(E) / 16) * kCompressUnroll;
+// 16 bytes a thread: kLanes of them have a group.  L: steps of a load, 16 bytes of them where rows' steps lie on 16 bytes; rows of other lengths are
+// loaded in as large pieces as divide them (a line's other pieces are in L1 by then: one by one 52 us instead of 142 with a lane
+// for each step of a group, 64 x 2312 x 301).
+template <typename E> constexpr int kCompressUnroll = sizeof(E) == 4 ? 4 : 2;
+template <typename E> constexpr int kCompressBlock = 256 / (32 * (int)sizeof(E) / 16) * kCompressUnroll<E>;
 
-template <typename E, bool LINED>
+template <int BYTES> struct Load;
+template <> struct Load<16> { using type = uint4; };
+template <> struct Load<8> { using type = uint2; };
+template <> struct Load<4> { using type = uint32_t; };
+template <> struct Load<2> { using type = uint16_t; };
+
+template <typename E, int L>
 __global__ void __launch_bounds__(256, 6)
 compress_kernel(int8_t *q, uint8_t *scale, const E *x, const Pieces s)
 {
-    constexpr int W = 16 / (int)sizeof(E), kLanes = 32 / W;
+    constexpr int W = 16 / (int)sizeof(E), kLanes = 32 / W, kUnroll = kCompressUnroll<E>;
+    using Part = typename Load<L * (int)sizeof(E)>::type;
     const Place<kCompressBlock<E>> place(s);
     const unsigned t = (threadIdx.x % kLanes) * W, T = (unsigned)s.T, pad = (unsigned)(s.G * kGroup - s.T), lane0 = threadIdx.x / kLanes;
     const E *const x0 = x + (place.row0 * s.T + place.rest0 * (int64_t)kGroup);        // (of the CTA's first group)
     int8_t *const q0 = q + place.first * kGroup;
     uint8_t *const scale0 = scale + place.row0;
-    unsigned down[kCompressUnroll], group[kCompressUnroll];
-    float v[kCompressUnroll][W];
+    unsigned down[kUnroll], group[kUnroll];
+    float v[kUnroll][W];
 #pragma unroll
-    for (int u = 0; u < kCompressUnroll; ++u) {
+    for (int u = 0; u < kUnroll; ++u) {
         const unsigned local = u * (256 / kLanes) + lane0;
         place(s, local, down[u], group[u]);
         const E *p = x0 + (int)(local * kGroup + t - down[u] * pad);
         const unsigned at = group[u] * kGroup + t;
-        if (LINED) {
-            uint4 raw = make_uint4(0, 0, 0, 0);
-            if (local < place.here && at < T) raw = __ldg(reinterpret_cast<const uint4 *>(p));
-            const E *e = reinterpret_cast<const E *>(&raw);
+        const unsigned end = local < place.here ? T : 0;
+        Part raw[W / L];
 #pragma unroll
-            for (int j = 0; j < W; ++j) v[u][j] = as_float<E>(e[j]);
-        } else {
-            const unsigned end = local < place.here ? T : 0;
-#pragma unroll
-            for (int j = 0; j < W; ++j) v[u][j] = at + j < end ? as_float<E>(__ldg(p + j)) : 0.0f;
+        for (int j = 0; j < W / L; ++j) {
+            raw[j] = Part();
+            if (at + j * L < end) raw[j] = __ldg(reinterpret_cast<const Part *>(p) + j);
         }
+        const E *e = reinterpret_cast<const E *>(raw);
+#pragma unroll
+        for (int j = 0; j < W; ++j) v[u][j] = as_float<E>(e[j]);
     }
 #pragma unroll
-    for (int u = 0; u < kCompressUnroll; ++u) {
+    for (int u = 0; u < kUnroll; ++u) {
         const unsigned local = u * (256 / kLanes) + lane0;
         float largest = 0.0f;        // of magnitudes, some sign, NaN if one is
 #pragma unroll
@@ -342,13 +349,13 @@ static Pieces pieces_of(int64_t rows, int64_t T, int64_t each)
     return {rows, T, ceil_div(T, kGroup), each, rows * each, far, each == 1 || each >= 1024 ? 0u : (unsigned)((((uint64_t)1 << 32) + each - 1) / each)};
 }
 
-template <typename E>
+template <typename E, int L>
 static void run_compress(int8_t *q, uint8_t *scale, const void *x, int64_t rows, int64_t T, cudaStream_t st)
 {
+    if constexpr (L > 1)
+        if (T % L != 0 || ((uintptr_t)x & (L * sizeof(E) - 1)) != 0) return run_compress<E, L / 2>(q, scale, x, rows, T, st);
     const Pieces s = pieces_of(rows, T, ceil_div(T, kGroup));
-    const unsigned blocks = (unsigned)ceil_div(s.all, kCompressBlock<E>);
-    if (T % (16 / (int)sizeof(E)) == 0 && aligned16(x)) compress_kernel<E, true><<<blocks, 256, 0, st>>>(q, scale, (const E *)x, s);
-    else compress_kernel<E, false><<<blocks, 256, 0, st>>>(q, scale, (const E *)x, s);
+    compress_kernel<E, L><<<(unsigned)ceil_div(s.all, kCompressBlock<E>), 256, 0, st>>>(q, scale, (const E *)x, s);
 }
 
 template <typename E>
@@ -375,9 +382,9 @@ extern "C" int slayer_b200_compress8(int8_t *q, uint8_t *scale, const void *x, i
     SB200_REQUIRE(q && scale && x, "compress8: null pointer");
     SB200_REQUIRE(!off_element(x, dtype) && aligned16(q), "compress8: a pointer off its alignment");
     const cudaStream_t st = (cudaStream_t)stream;
-    if (dtype == SLAYER_B200_F32) run_compress<float>(q, scale, x, rows, T, st);
-    else if (dtype == SLAYER_B200_BF16) run_compress<__nv_bfloat16>(q, scale, x, rows, T, st);
-    else run_compress<__half>(q, scale, x, rows, T, st);
+    if (dtype == SLAYER_B200_F32) run_compress<float, 4>(q, scale, x, rows, T, st);
+    else if (dtype == SLAYER_B200_BF16) run_compress<__nv_bfloat16, 8>(q, scale, x, rows, T, st);
+    else run_compress<__half, 8>(q, scale, x, rows, T, st);
     return check_launch("compress8 kernel launch");
 }
 
