@@ -338,8 +338,8 @@ static bool off_element(const void *p, int dtype) { return ((uintptr_t)p & (dtyp
 static int check_rows(const char *op, int64_t rows, int64_t T)
 {
     SB200_REQUIRE(rows >= 0 && T >= 0, "%s: negative size", op);
-    SB200_REQUIRE(rows <= (int64_t)1 << 40 && T <= (int64_t)1 << 30 && ceil_div(rows, 32) <= ((int64_t)1 << 31) / ceil_div(T + 1, kGroup), "%s: too many steps",
-                  op);
+    // (pieces x pieces of a row below 2^64: Place)
+    SB200_REQUIRE(rows <= (int64_t)1 << 37 && T <= (int64_t)1 << 29 && rows <= ((int64_t)1 << 37) / (ceil_div(T + 1, kGroup) * kGroup), "%s: too many steps", op);
     return SLAYER_B200_OK;
 }
 

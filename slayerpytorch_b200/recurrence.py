@@ -24,8 +24,8 @@ def gatedLeak(x, gate, initial=None, lengths=None, kind='logit', coupled=False, 
 
         y_t = f_t * y_{t-1} + x_t                   (coupled: f_t * y_{t-1} + (1 - f_t) * x_t)
 
-    with ``f = sigmoid(gate)`` (``kind='logit'``) or ``f = gate`` (``'decay'``: meant for values from -1 to 1; products of larger ones
-    may overflow where single steps do not).  ``x [..., T]``: float32, bfloat16 or float16, any strides (a copy is made where it is not
+    with ``f = sigmoid(gate)`` (``kind='logit'``) or ``f = gate`` (``'decay'``: from 0 to 1; values outside are taken as they are, with less
+    exact results where -1 is near, and products that may overflow where single steps do not).  ``x [..., T]``: float32, bfloat16 or float16, any strides (a copy is made where it is not
     contiguous); ``y`` is like it.  ``gate`` broadcasts to ``x``: one of the shape of ``x`` (or with a time dimension of ``T``) has
     the type of ``x``; one per neuron, ``[C, H, W, 1]`` say, may have any of the three, and is not copied where its dimensions lie
     next to each other.  ``initial [...]``: the state before the first step (default 0).
@@ -34,8 +34,8 @@ def gatedLeak(x, gate, initial=None, lengths=None, kind='logit', coupled=False, 
     used, whatever they hold, ``y`` and all gradients are 0 there, and the state stays what it was.  With ``returnState`` the
     state after the last step comes too, float32, of the shape of ``initial``.
 
-    Differentiable once in ``x``, ``gate`` and ``initial``.  States are held in double within a call; nothing but ``x``, ``gate`` and one
-    state for 128 (float32) or 256 steps is kept for the backward pass.  A state that is not finite makes those after it so, as NaN
+    Differentiable once in ``x``, ``gate`` and ``initial``.  Results are off by a few steps of float32, however slow the leak.  Nothing but
+    ``x``, ``gate`` and one state for 512 steps is kept for the backward pass.  A state that is not finite makes those after it so, as NaN
     possibly where single steps would give an infinity."""
     out = slayerCuda.gatedLeak(x, gate, initial, lengths, _flags("gatedLeak", kind, coupled), returnState)
     return (out[0], out[1]) if returnState else out[0]

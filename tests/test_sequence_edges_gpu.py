@@ -1,0 +1,142 @@
+"""GPU: the gated leak and tensors in 8 bits at their edges - offsets past 32 bits, streams and graphs side by side, the order of rows, exact powers."""
+import pytest
+import torch
+
+from slayerpytorch_b200 import capi, checkpoint
+from slayerpytorch_b200.recurrence import gatedLeak, gatedLeakStep
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("T", [8, 300, 2000])
+def test_leaks_of_more_than_2_to_31_elements(T):
+    """A row's result does not depend on where it lies: the last rows equal those of a call of their own."""
+    rows = (1 << 31) // T + 4096
+    x = torch.empty(rows, T, dtype=torch.bfloat16, device="cuda").normal_()
+    gate = torch.full((1,), 2.0, device="cuda").expand(rows).reshape(rows, 1).contiguous()
+    last = x[-4096:].clone()
+    y = gatedLeak(x, gate, coupled=True)
+    assert torch.equal(y[-4096:], gatedLeak(last, gate[-4096:], coupled=True))
+    del y
+    leaf, own = x.requires_grad_(), last.requires_grad_()
+    (a,) = torch.autograd.grad(gatedLeak(leaf, gate), [leaf], x.detach())
+    (b,) = torch.autograd.grad(gatedLeak(own, gate[-4096:]), [own], last.detach())
+    assert torch.equal(a[-4096:], b)
+
+
+def test_tensors_in_8_bits_of_more_than_2_to_31_elements():
+    for T in (300, 301):
+        rows = (1 << 31) // T + 4096
+        x = torch.empty(rows, T, dtype=torch.bfloat16, device="cuda").normal_()
+        kept = checkpoint.compress(x)
+        own = checkpoint.compress(x[-4096:].clone())
+        assert torch.equal(kept.q[-4096:], own.q) and torch.equal(kept.scale[:, -4096:], own.scale)
+        assert torch.equal(kept.restore()[-4096:], own.restore())
+        u = torch.empty(rows, T, device="cuda").normal_()
+        got = checkpoint.spikeGrad(u, kept, 1.0, 1.0, 1.0)
+        assert torch.equal(got[-4096:], checkpoint.spikeGrad(u[-4096:].clone(), own, 1.0, 1.0, 1.0))
+        del x, kept, u, got
+
+
+@pytest.mark.parametrize("N,O,I,T", [(70000, 2, 1000, 32), (40000, 1800, 3, 31)])
+def test_weight_gradients_of_more_than_2_to_31_elements(N, O, I, T):
+    """Only the last samples' gradients are not zero: the result is theirs, up to the order of sums."""
+    x = torch.randint(-100, 101, (N, I, T), device="cuda", dtype=torch.int8).to(torch.bfloat16)
+    g = torch.zeros(N, O, T, device="cuda")
+    g[-3:].normal_()
+    kept = checkpoint.compress(x)
+    got = checkpoint.weightGrad(g, kept)
+    a = g[-3:].transpose(0, 1).reshape(O, -1).double()
+    b = checkpoint.compress(x[-3:].clone()).restore(torch.float32).transpose(0, 1).reshape(I, -1).double()
+    # three times T products of float32 precision
+    assert bool(((got[..., 0].double() - a @ b.T).abs() <= (8 + (3 * T) ** 0.5) * 2.0 ** -24 * (a.abs() @ b.abs().T)).all())
+
+
+def test_streams_side_by_side():
+    """Calls of all operators on four streams at once give what they give one after the other."""
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    data = [(torch.randn(3, 40, 1, 1, 5000, device="cuda", generator=gen), torch.randn(3, 40, 1, 1, 5000, device="cuda", generator=gen),
+             torch.randn(3, 300, 1, 1, 5000, device="cuda", generator=gen)) for _ in range(4)]
+
+    def work(x, gate, g):
+        y, s = gatedLeak(x, gate, returnState=True)
+        kept = checkpoint.compress(y)
+        return [y, s, kept.restore(), checkpoint.spikeGrad(x, kept, 1.0, 2.0, 1.0), checkpoint.weightGrad(g, kept)]
+    alone = [work(*d) for d in data]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in data]
+    out = []
+    for s, d in zip(streams, data):
+        with torch.cuda.stream(s):
+            out.append([work(*d) for _ in range(3)])
+    torch.cuda.synchronize()
+    for a, runs in zip(alone, out):
+        for b in runs:
+            assert all(torch.equal(v, w) for v, w in zip(a, b))
+    assert capi.device_status() == 0
+
+
+def test_two_graphs():
+    """Two captured graphs, replayed in turn and on two streams, each with workspaces of its own."""
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    made = []
+    for k in range(2):
+        x, gate = (torch.randn(1, 3, 20000, device="cuda", generator=gen) for _ in range(2))
+        g = torch.randn(1, 70, 20000, device="cuda", generator=gen)
+        eager = [gatedLeak(x, gate), checkpoint.weightGrad(g, checkpoint.compress(x))]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = [gatedLeak(x, gate), checkpoint.weightGrad(g, checkpoint.compress(x))]
+        made.append((graph, eager, out, x, gate, g))
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        made[0][0].replay()
+        with torch.cuda.stream(side):
+            made[1][0].replay()
+    torch.cuda.synchronize()
+    for graph, eager, out, *_ in made:
+        assert all(torch.equal(a, b) for a, b in zip(eager, out))
+
+
+def test_rows_do_not_depend_on_one_another():
+    """The same rows in another order, and rows of T steps as the start of longer ones."""
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    for T in (7, 100, 301, 1500):
+        x, gate = (torch.randn(64, T, device="cuda", generator=gen) for _ in range(2))
+        order = torch.randperm(64, device="cuda", generator=gen)
+        y, z = gatedLeak(x, gate), gatedLeak(x[order], gate[order])
+        assert torch.allclose(y[order], z, rtol=0, atol=float(y.abs().max()) * 2.0 ** -20)
+        if T % 4 == 0:          # lanes begin at the same steps
+            assert torch.equal(y[order], z)
+        kept, other = checkpoint.compress(x), checkpoint.compress(x[order])
+        assert torch.equal(kept.q[order], other.q) and torch.equal(kept.scale[:, order], other.scale)
+
+
+@pytest.mark.parametrize("kind", ['logit', 'decay'])
+def test_a_stop_forgets_everything(kind):
+    """A step that keeps nothing stops whatever was before it, however large, for the rest of the row, wherever it lies."""
+    stop = float("-inf") if kind == 'logit' else 0.0
+    for T in (40, 300, 513, 3000):
+        for at in {0, 1, 15, 16, 17, 31, 39, T // 2, T - 1}:
+            x, gate = torch.ones(2, T, device="cuda"), torch.full((2, T), 5.0 if kind == 'logit' else 0.99, device="cuda")
+            x[1, :at], gate[:, at] = 1e30, stop
+            # (a call for each: in one, rows of odd lengths lie differently, and lanes begin at other steps)
+            y, z = (gatedLeak(x[i:i + 1].clone(), gate[i:i + 1].clone(), kind=kind, initial=torch.tensor([h], device="cuda"))
+                    for i, h in ((0, 0.0), (1, 1e35)))
+            assert torch.equal(y[0, at:], z[0, at:]) and float(z[0, at]) == 1.0
+
+
+def test_single_steps_of_a_long_stream():
+    """Ten thousand steps with a slow leak: states are rounded to 32 bits each time, half a step at random."""
+    gate = torch.tensor([8.0, 5.0, -2.0, 12.0], device="cuda")
+    f = torch.sigmoid(gate.double())
+    state, want = torch.zeros(4, device="cuda"), torch.zeros(4, dtype=torch.float64, device="cuda")
+    x = torch.ones(4, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gatedLeakStep(x, gate, state)
+    for _ in range(10000):
+        graph.replay()
+        want = f * want + 1
+    # one minus f is known to (8 + |gate|) 2^-24; roundings of up to 10000 states, 2^-24 each, at random: less than 500 of them
+    assert bool(((state.double() - want).abs() <= (8 + gate.abs() + 500) * 2.0 ** -24 * want).all())
