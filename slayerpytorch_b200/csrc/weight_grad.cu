@@ -21,7 +21,7 @@ namespace sb200 {
 constexpr int kWgWaitLimit = 1 << 22;
 constexpr int kStatusWeightTimeout = 0x5104;
 constexpr int kWgWorkers = 512, kWgThreads = kWgWorkers + 128;
-constexpr int kSteps = 4;        // blocks of 64 steps in a sum of the tensor core
+constexpr int kSteps = 2;        // blocks of 64 steps in a sum of the tensor core (4: 1.5 % faster, results twice as far off)
 
 template <int CG, int NT, bool VEC>
 struct WgTile {
@@ -415,23 +415,47 @@ __global__ void __launch_bounds__(kWgThreads, 1) weight_grad_kernel(const __grid
     }
 }
 
-// The shares' parts of each output, in order.
-template <int CG, int NT>
+// The shares' parts of each output, in order: SPLIT warps have 128 rows of a column, four of them a thread, and every SPLIT-th part.
+template <int CG, int NT, int SPLIT>
 __global__ void __launch_bounds__(256) weight_sum_kernel(float *out, const WgArgs A)
 {
     constexpr int R = 128 * CG;
+    __shared__ int range[2];
+    __shared__ double sums[SPLIT > 1 ? 8 : 1][4][32];
     const int64_t tile = blockIdx.x, ti = tile / A.tiles_o, to = tile - ti * A.tiles_o;
-    const int row = blockIdx.z * 128 + threadIdx.x % 128, col = blockIdx.y * 2 + threadIdx.x / 128;
-    const int64_t i = ti * R + row;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.y * 128 + lane * 4;
+    const int col = blockIdx.z * (8 / SPLIT) + warp / SPLIT, turn = warp % SPLIT;
     // share p begins at work * p / shares: the one that has a block is the last to begin before or at it
-    const int64_t first = ((tile * A.blocks + 1) * A.shares - 1) / A.work, last = ((tile + 1) * A.blocks * A.shares - 1) / A.work;
-    const int64_t o = to * NT + col;
-    if (i >= A.I || o >= A.O) return;
-    const float *p = A.part + (first + tile) * (int64_t)(R * NT) + (int64_t)col * R + row;
-    double sum = 0.0;
-#pragma unroll 4
-    for (int64_t s = first; s <= last; ++s, p += R * NT) sum += (double)__ldg(p);
-    out[o * A.I + i] = (float)sum;
+    if (threadIdx.x < 2) range[threadIdx.x] = (int)((((tile + threadIdx.x) * A.blocks + 1 - threadIdx.x) * A.shares - 1) / A.work);
+    __syncthreads();
+    const int first = range[0], last = range[1];
+    const int64_t i = ti * R + row, o = to * NT + col;
+    const bool there = i < A.I && o < A.O;
+    double sum[4] = {};
+    const float *p = A.part + (first + turn + tile) * (int64_t)(R * NT) + (int64_t)col * R + row;
+#pragma unroll 8
+    for (int s = first + turn; s <= last && there; s += SPLIT, p += SPLIT * (int64_t)(R * NT)) {
+        const float4 v = __ldg(reinterpret_cast<const float4 *>(p));
+        sum[0] += (double)v.x, sum[1] += (double)v.y, sum[2] += (double)v.z, sum[3] += (double)v.w;
+    }
+    if (SPLIT > 1) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sums[warp][k][lane] = sum[k];
+        __syncthreads();
+#pragma unroll
+        for (int w = 1; w < SPLIT; ++w)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) sum[k] += sums[(warp - turn + w) & 7][k][lane];
+    }
+    if (!there || turn > 0) return;
+    float *to_row = out + o * A.I + i;
+    if (A.I % 4 == 0 && ((uintptr_t)out & 15) == 0) {
+        *reinterpret_cast<float4 *>(to_row) = make_float4((float)sum[0], (float)sum[1], (float)sum[2], (float)sum[3]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (i + k < A.I) to_row[k] = (float)sum[k];
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ host side
@@ -487,7 +511,9 @@ static int wg_launch(const WgArgs &A, float *out, int64_t tiles, cudaStream_t st
     cudaLaunchKernelEx(&cfg, kern, A);
     const int bad = check_launch("weight_grad8 kernel launch");
     if (bad) return bad;
-    weight_sum_kernel<CG, NT><<<dim3((unsigned)tiles, NT / 2, CG), 256, 0, st>>>(out, A);
+    // (a tile with many parts: 37 of them one after the other 7.5 us, in fours 4.7)
+    if (A.shares / tiles >= 16) weight_sum_kernel<CG, NT, 4><<<dim3((unsigned)tiles, CG, NT / 2), 256, 0, st>>>(out, A);
+    else weight_sum_kernel<CG, NT, 1><<<dim3((unsigned)tiles, CG, NT / 8), 256, 0, st>>>(out, A);
     return check_launch("weight_grad8 sum launch");
 }
 
