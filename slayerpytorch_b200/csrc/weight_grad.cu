@@ -46,6 +46,7 @@ struct WgArgs {
     int *status;
     int64_t N, O, I, T, G, g_size;
     int units, blocks, U;        // 16 steps of a sample; 4 of those; units of a sample
+    int inner_samples;           // samples with at least eight elements of g behind them
     int64_t tiles_o, work;       // tiles next to each other share their rows; tiles x blocks
     int shares;
 };
@@ -91,8 +92,14 @@ __device__ __forceinline__ float4 wg_shift(float4 a, float4 b, int skew, int lef
 {
     const bool two = skew & 2, one = skew & 1;
     const float v0 = two ? a.z : a.x, v1 = two ? a.w : a.y, v2 = two ? b.x : a.z, v3 = two ? b.y : a.w, v4 = two ? b.z : b.x;
-    return make_float4(left > 0 ? (one ? v1 : v0) : 0.0f, left > 1 ? (one ? v2 : v1) : 0.0f, left > 2 ? (one ? v3 : v2) : 0.0f,
-                       left > 3 ? (one ? v4 : v3) : 0.0f);
+    float4 v = make_float4(one ? v1 : v0, one ? v2 : v1, one ? v3 : v2, one ? v4 : v3);
+    if (left < 4) {
+        v.x = left > 0 ? v.x : 0.0f;
+        v.y = left > 1 ? v.y : 0.0f;
+        v.z = left > 2 ? v.z : 0.0f;
+        v.w = 0.0f;
+    }
+    return v;
 }
 
 // two floats at once: a b + c
@@ -245,15 +252,23 @@ __global__ void __launch_bounds__(kWgThreads, 1) weight_grad_kernel(const __grid
                     } else {
                         // The 16 bytes that the four steps begin in, and, where the thread beside has no more steps of the row or a quarter is the
                         // unit's last, the 16 after them.  The tensor may end inside.
-                        const float *const p = b ? bg - ((bg - A.g) & 3) : A.g;
+                        const float *const p = b ? bg - ((int)(bg - A.g) & 3) : A.g;
                         const bool more = b && (quarter == 3 || t + 4 >= (int)A.T);
-                        const bool end = ub.n == (int)A.N - 1;
+                        if (ub.n < A.inner_samples) {
 #pragma unroll
-                        for (int j = 0; j < kItems; ++j) {
-                            const float *v = p + (b ? b_far[j] : 0);
-                            const int there = end ? (int)min(A.g_size - (v - A.g), (int64_t)8) : 8;
-                            wg_copy(into + (1 + j) * 8192, v, b ? min(there * 4, 16) : 0);
-                            if (more) wg_copy(into + beyond + j * 2048, there > 4 ? v + 4 : v, max(there * 4 - 16, 0));
+                            for (int j = 0; j < kItems; ++j) {
+                                const float *v = p + (b ? b_far[j] : 0);
+                                wg_copy(into + (1 + j) * 8192, v, b ? 16 : 0);
+                                if (more) wg_copy(into + beyond + j * 2048, v + 4, 16);
+                            }
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < kItems; ++j) {
+                                const float *v = p + (b ? b_far[j] : 0);
+                                const int there = (int)min(A.g_size - (v - A.g), (int64_t)8);
+                                wg_copy(into + (1 + j) * 8192, v, b ? min(there * 4, 16) : 0);
+                                if (more) wg_copy(into + beyond + j * 2048, there > 4 ? v + 4 : v, max(there * 4 - 16, 0));
+                            }
                         }
                     }
                 }
@@ -556,7 +571,7 @@ extern "C" int slayer_b200_weight_grad8(float *out, const float *g, const int8_t
     if (!status) { set_error("weight_grad8: no status word on this device"); return SLAYER_B200_ECUDA; }
     const WgPlan p = wg_plan(N, O, I, T);
     const int U = (int)ceil_div(T, 16);
-    const WgArgs A = {g, q, scale, (float *)workspace, status, N, O, I, T, ceil_div(T, 32), N * O * T, (int)(N * U), (int)p.blocks, U, p.tiles_o, p.tiles * p.blocks, (int)p.shares};
+    const WgArgs A = {g, q, scale, (float *)workspace, status, N, O, I, T, ceil_div(T, 32), N * O * T, (int)(N * U), (int)p.blocks, U, (int)std::max<int64_t>(0, N - ceil_div(8, O * T)), p.tiles_o, p.tiles * p.blocks, (int)p.shares};
     switch (p.nt) {
     case 256: return wg_align<2, 256>(A, out, p.tiles, st);
     case 128: return wg_align<1, 128>(A, out, p.tiles, st);

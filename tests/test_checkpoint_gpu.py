@@ -124,6 +124,13 @@ def test_weight_gradient(N, O, sizes, T):
     check_weight(N, O, sizes, T, N + O)
 
 
+@pytest.mark.parametrize("O,T", [(1, 1), (1, 2), (1, 3), (2, 1), (3, 1), (2, 3), (7, 1), (1, 7), (3, 5)])
+@pytest.mark.parametrize("N", [1, 2, 3, 9, 20])
+def test_weight_gradient_of_few_elements(N, O, T):
+    """Samples of fewer elements than two loads of 16 bytes: the tensor ends within the reach of several."""
+    check_weight(N, O, (5,), T, N + O + T)
+
+
 def test_weight_gradient_at_its_ends():
     """Values of very different sizes, what is not finite, no samples, no steps."""
     x = torch.randn(3, 40, 70, device="cuda") * 2.0 ** torch.randint(-100, 30, (3, 40, 1), device="cuda")
