@@ -7,6 +7,7 @@ The package holds
 * ``lib/``     the built binaries (``libslayer_b200.so``, ``slayerCuda``, ``slayerLoihiCuda``);
 * ``layer``    a host-side mirror of the reference's ``spikeLayer`` hot-path methods
                (psp, spike, delay, delayShift, spikeLoihi) with fused backward passes;
+* ``recurrence``, ``checkpoint``  gated leaky integrators, and tensors kept in 8 bits until the backward pass;
 * ``capi``     a ctypes view of the C ABI for callers that hold raw device pointers.
 
 ``import slayerpytorch_b200`` makes ``import slayerCuda`` / ``import slayerLoihiCuda`` resolve
