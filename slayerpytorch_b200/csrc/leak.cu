@@ -1,15 +1,15 @@
 // Gated leaky integrator, along the time steps of each row:
 //   y_t = f_t y_{t-1} + u_t,   f = sigmoid(gate) or the gate itself,   u = x, or (1 - f) x ("coupled").
-// A step is the map h -> A h + B with A = f_t, B = u_t; maps compose to maps, so a row is a scan over them: a lane composes its 16 bytes
-// of steps, the lanes of a row's group scan their maps with shuffles, and each walks its steps from the state that the lanes before
+// A step is the map h -> A h + B with A = f_t, B = u_t; maps compose to maps, so a row is a scan over them: a lane composes its steps,
+// the lanes of a row's group scan their maps with shuffles, and each walks its steps from the state that the lanes before
 // it leave.  The backward pass is the same from the other end: c_t = f_t (g_t + c_{t+1}) is what step t hands to step t - 1, and
 //   lambda_t = g_t + c_{t+1},   dx = lambda (or (1 - f) lambda),   df = lambda (y_{t-1} - (coupled) x).
-// It forms y again from x and the gate, out of the states that the forward pass keeps at the start of each chunk (4 bytes for 1200 and more), so that
+// It forms y again from x and the gate, out of the states that the forward pass keeps at the start of each chunk (4 bytes for 512 steps), so that
 // it reads x, gate and g and writes dx and dgate: no y is kept, and none that is rounded to 16 bits is used.
 //
 // Maps are floats: A, and 1 - A by itself (R), and B.  A slow leak's f is next to one, where its rounding to 32 bits, taken at each of the thousands of
 // steps that such a state remembers, adds up to 1e-4 of it; R has 24 bits of what is forgotten instead.  States are double from chunk to chunk, and
-// float within the up to 16 steps that a lane walks.  (All of it in double, with half as many instructions again: 39 + 74 us instead of 29 + 51, 64 x 512 x 300.)
+// float within the up to 16 steps that a lane walks.  (All of it in double, with half as many instructions again: 39 + 74 us instead of 28 + 49, 64 x 512 x 300.)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
