@@ -389,7 +389,7 @@ int64_t slayer_b200_muon_step_workspace(const slayer_b200_muon_matrix *list, int
  * gate_period).  lengths (NULL: all T): steps that count, one entry for every sample_rows rows, taken
  * into [0, T]; the steps behind them are not used, y is 0 there and the state stays.  state (NULL: not
  * wanted): the state after the last step.  starts (NULL: no backward pass): rows x
- * slayer_b200_leak_chunks(T) float32, states that the backward pass starts from.  States are
+ * slayer_b200_leak_states(T) float32, states that the backward pass starts from (one for 12 or 16 steps of longer rows).  States are
  * float32 outside of a call and double within.  y may not be x or gate; they (a gate of x's type) are aligned
  * to 16 bytes.  workspace:
  * slayer_b200_leak_workspace(...) bytes of device memory, aligned to 16, for either pass.  It has
@@ -398,7 +398,7 @@ int64_t slayer_b200_muon_step_workspace(const slayer_b200_muon_matrix *list, int
 int slayer_b200_leak_forward(void *y, float *state, float *starts, const void *x, const void *gate, const float *initial, int dtype, int flags,
                              int64_t rows, int64_t T, const int64_t *lengths, int64_t sample_rows, int64_t gate_inner, int64_t gate_period,
                              void *workspace, void *stream);
-int64_t slayer_b200_leak_chunks(int64_t T);
+int64_t slayer_b200_leak_states(int64_t T);
 int64_t slayer_b200_leak_workspace(int64_t rows, int64_t T, int dtype, int64_t gate_inner, int64_t gate_period);
 
 /*

@@ -50,7 +50,7 @@ SYMBOLS = {
     "slayer_b200_muon_step": (_int, [_p, _i64, _int, _f, _f, _int, _f, _int, _int, _f, _f, _f, _f, _p, _p]),
     "slayer_b200_muon_step_workspace": (_i64, [_p, _i64, _int]),
     "slayer_b200_leak_forward": (_int, [_p, _p, _p, _p, _p, _p, _int, _int, _i64, _i64, _p, _i64, _i64, _i64, _p, _p]),
-    "slayer_b200_leak_chunks": (_i64, [_i64]),
+    "slayer_b200_leak_states": (_i64, [_i64]),
     "slayer_b200_leak_workspace": (_i64, [_i64, _i64, _int, _i64, _i64]),
     "slayer_b200_leak_backward": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _int, _int, _i64, _i64, _p, _i64, _i64, _i64, _p, _p]),
     "slayer_b200_leak_step": (_int, [_p, _p, _p, _p, _int, _int, _int, _i64, _i64, _i64, _p]),

@@ -98,7 +98,7 @@ struct Shape {
     }
 };
 
-// Forward keeps x, the gate and the state at the start of each chunk of steps; backward forms the other states from them again.
+// Forward keeps x, the gate and a state for each dozen steps; backward forms the other states from them again.
 struct GatedLeak : public torch::autograd::Function<GatedLeak> {
     static variable_list forward(AutogradContext *ctx, const torch::Tensor &x, const torch::Tensor &gate, const c10::optional<torch::Tensor> &initial,
                                  const c10::optional<torch::Tensor> &lengths, int64_t inner, int64_t period, int64_t flags, bool wantState, bool want)
@@ -109,7 +109,7 @@ struct GatedLeak : public torch::autograd::Function<GatedLeak> {
         const auto floats = x.options().dtype(torch::kFloat32);
         torch::Tensor state, starts;
         if (wantState) state = torch::empty(x.sizes().slice(0, x.dim() - 1), floats);
-        if (want) starts = torch::empty({s.rows, slayer_b200_leak_chunks(s.T)}, floats);
+        if (want) starts = torch::empty({s.rows, slayer_b200_leak_states(s.T)}, floats);
         const auto workspace = s.workspace(x);
         check_rc(slayer_b200_leak_forward(y.data_ptr(), wantState ? state.data_ptr<float>() : nullptr, want ? starts.data_ptr<float>() : nullptr, x.data_ptr(),
                                           gate.data_ptr(), initial.has_value() ? initial->data_ptr<float>() : nullptr, s.dtype, s.flags, s.rows, s.T,

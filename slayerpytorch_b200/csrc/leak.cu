@@ -4,12 +4,15 @@
 // the lanes of a row's group scan their maps with shuffles, and each walks its steps from the state that the lanes before
 // it leave.  The backward pass is the same from the other end: c_t = f_t (g_t + c_{t+1}) is what step t hands to step t - 1, and
 //   lambda_t = g_t + c_{t+1},   dx = lambda (or (1 - f) lambda),   df = lambda (y_{t-1} - (coupled) x).
-// It forms y again from x and the gate, out of the states that the forward pass keeps at the start of each chunk (4 bytes for 512 steps), so that
-// it reads x, gate and g and writes dx and dgate: no y is kept, and none that is rounded to 16 bits is used.
+// It forms y again from x and the gate, out of the states that the forward pass keeps where each lane begins (4 bytes for 12 or 16 steps), so that
+// it reads x, gate and g and writes dx and dgate, and scans once: no y is kept, and none that is rounded to 16 bits is used.  (With states at
+// the start of each chunk alone, and a scan for the others, the backward pass took 49 us instead of 46, 64 x 512 x 300, and 127 instead
+// of 111, 262144 x 100.)
 //
 // Maps are floats: A, and 1 - A by itself (R), and B.  A slow leak's f is next to one, where its rounding to 32 bits, taken at each of the thousands of
 // steps that such a state remembers, adds up to 1e-4 of it; R has 24 bits of what is forgotten instead.  States are double from chunk to chunk, and
-// float within the up to 16 steps that a lane walks.  (All of it in double, with half as many instructions again: 39 + 74 us instead of 28 + 49, 64 x 512 x 300.)
+// float within the up to 16 steps that a lane walks.  (All of it in double, with half as many instructions again: 39 + 74 us instead of
+// 28 + 49 of the time, 64 x 512 x 300.)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -19,9 +22,9 @@ namespace sb200 {
 
 constexpr int kLeakThreads = 128;
 
-// CTAs of an SM that registers are rationed for: the most that leave none of a lane's steps in memory
-template <int K> constexpr int kForwardBlocks = K < 4 ? 8 : 7;
-template <int K> constexpr int kBackwardBlocks = K < 4 ? 5 : 4;
+// CTAs of an SM that registers are rationed for: the most that leave (nearly) none of a lane's steps in memory
+template <int K> constexpr int kForwardBlocks = K < 4 ? 9 : 7;
+template <int K> constexpr int kBackwardBlocks = K < 4 ? 6 : 5;
 
 template <typename E> __device__ __forceinline__ float to_float(E v);
 template <> __device__ __forceinline__ float to_float<float>(float v) { return v; }
@@ -283,14 +286,14 @@ __device__ __forceinline__ Map forward_map(const Steps<E, K> &st)
     return m;
 }
 
-// c -> f (g + c) for all steps, from the last; what is kept of c is what is kept of a state (`kept`)
+// c -> f (g + c) for all steps, from the last
 template <int N>
-__device__ __forceinline__ Map backward_map(const Decay (&d)[N], const float (&g)[N], const Map &kept)
+__device__ __forceinline__ Map backward_map(const Decay (&d)[N], const float (&g)[N])
 {
-    float b = d[N - 1].f * g[N - 1];
+    Map m = {d[N - 1].f, d[N - 1].rest, d[N - 1].f * g[N - 1]};
 #pragma unroll
-    for (int j = N - 2; j >= 0; --j) b = d[j].f * (b + g[j]);
-    return {kept.a, kept.r, b};
+    for (int j = N - 2; j >= 0; --j) m = {m.a * d[j].f, fmaf(m.a, d[j].rest, m.r), d[j].f * (m.b + g[j])};
+    return m;
 }
 
 // Which row, segment and lane of its group a thread is; false: none.
@@ -338,7 +341,7 @@ leak_maps_kernel(Map *maps, const E *x, const void *gate, const LeakShape s)
             st.couple(s.coupled);
             all = compose(all, shift_from(scan<32, true>(forward_map<E, K>(st), lane), 31));
         } else {
-            all = compose(all, shift_from(scan<32, false>(backward_map<4 * K>(st.d, st.x, forward_map<E, K>(st)), lane), 0));
+            all = compose(all, shift_from(scan<32, false>(backward_map<4 * K>(st.d, st.x), lane), 0));
         }
     }
     if (lane == 0) maps[row * s.segments + segment] = all;
@@ -358,13 +361,13 @@ leak_forward_kernel(E *y, float *state, float *starts, const E *x, const void *g
     if (G == 32 && segment > 0) h = through_segments<true>(maps + row * s.segments, 0, segment, lane, h);
     const int first = segment * s.segment_chunks, last = min(first + s.segment_chunks, s.chunks);
     for (int c = first; c < last; ++c) {
-        if (starts && there && lane == 0) starts[(int64_t)row * s.chunks + c] = (float)h;
         const Inside<K> in((c * G + lane) * (4 * K) - r.skew, r.length);
         Steps<E, K> st;
         st.load(s, r, x, (const E *)gate, row_d, in);
         st.couple(s.coupled);
         const Map m = scan<G, true>(forward_map<E, K>(st), lane);
         float at = (float)others<G, true>(m, lane)(h);
+        if (starts && there) starts[((int64_t)row * s.chunks + c) * G + lane] = at;
         h = __shfl_sync(~0u, m(h), G - 1, G);
 #pragma unroll
         for (int j = 0; j < 4 * K; ++j) {
@@ -398,19 +401,17 @@ leak_backward_kernel(E *dx, E *dgate, double *sums, float *dinitial, const E *g,
         Steps<E, K> st;
         load_steps<E, K>(gv, g + r.base, in, 0.0f);
         st.load(s, r, x, (const E *)gate, row_d, in);
-        const double start = (double)starts[(int64_t)row * s.chunks + c];
+        float at = starts[((int64_t)row * s.chunks + c) * G + lane];
 #pragma unroll
         for (int j = 0; j < N; ++j) slope[j] = s.coupled ? st.x[j] : 0.0f;
         st.couple(s.coupled);
-        const Map steps = forward_map<E, K>(st);
-        float at = (float)others<G, true>(scan<G, true>(steps, lane), lane)(start);
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             slope[j] = at - slope[j];
             if (s.logit) slope[j] *= st.d[j].f * st.d[j].rest;
             at = fmaf(st.d[j].f, at, st.x[j]);
         }
-        const Map m = scan<G, false>(backward_map<N>(st.d, gv, steps), lane);
+        const Map m = scan<G, false>(backward_map<N>(st.d, gv), lane);
         at = (float)others<G, false>(m, lane)(carry);
         carry = __shfl_sync(~0u, m(carry), 0, G);
 #pragma unroll
@@ -602,12 +603,12 @@ static bool aligned_to(const void *p, unsigned n) { return ((uintptr_t)p & (n - 
 
 }  // namespace sb200
 
-extern "C" int64_t slayer_b200_leak_chunks(int64_t T)
+extern "C" int64_t slayer_b200_leak_states(int64_t T)
 {
     using namespace sb200;
     clear_error();
-    SB200_REQUIRE(T >= 0 && T <= (int64_t)1 << 30, "leak_chunks: bad length");
-    return chunks_of(T);
+    SB200_REQUIRE(T >= 0 && T <= (int64_t)1 << 30, "leak_states: bad length");
+    return chunks_of(T) * lanes_of(T).lanes;
 }
 
 extern "C" int64_t slayer_b200_leak_workspace(int64_t rows, int64_t T, int dtype, int64_t gate_inner, int64_t gate_period)

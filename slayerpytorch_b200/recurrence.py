@@ -35,7 +35,7 @@ def gatedLeak(x, gate, initial=None, lengths=None, kind='logit', coupled=False, 
     state after the last step comes too, float32, of the shape of ``initial``.
 
     Differentiable once in ``x``, ``gate`` and ``initial``.  Results are off by a few steps of float32, however slow the leak.  Nothing but
-    ``x``, ``gate`` and one state for 512 steps is kept for the backward pass.  A state that is not finite makes those after it so, as NaN
+    ``x``, ``gate`` and one float32 state for 12 or 16 steps is kept for the backward pass.  A state that is not finite makes those after it so, as NaN
     possibly where single steps would give an infinity."""
     out = slayerCuda.gatedLeak(x, gate, initial, lengths, _flags("gatedLeak", kind, coupled), returnState)
     return (out[0], out[1]) if returnState else out[0]

@@ -64,10 +64,11 @@ def test_c_entries_of_the_leak():
                 dict(period=3, inner=1)):
         assert call(**bad) == -1, bad
     assert call(rows=0, y=null) == 0
-    # a row of up to 512 steps, with up to three before its first one, is a chunk, longer ones have chunks of 512
-    for T, n in ((0, 0), (1, 1), (128, 1), (129, 1), (509, 1), (511, 2), (512, 1), (513, 2), (1450, 3), (2000, 4), (100000, 196)):
-        assert lib.slayer_b200_leak_chunks(T) == n, T
-    assert lib.slayer_b200_leak_chunks(-1) == -1 and lib.slayer_b200_leak_chunks(1 << 31) == -1
+    # a state for each lane: of 4, 8 or 16 steps (up to 16 of them), else of 12 or 16, with up to three before the first one
+    for T, n in ((0, 0), (1, 1), (4, 1), (5, 1), (16, 1), (17, 2), (128, 8), (129, 16), (300, 32), (509, 32), (511, 64), (512, 32), (513, 64), (1450, 96),
+                 (2000, 128), (100000, 196 * 32)):
+        assert lib.slayer_b200_leak_states(T) == n, T
+    assert lib.slayer_b200_leak_states(-1) == -1 and lib.slayer_b200_leak_states(1 << 31) == -1
     assert lib.slayer_b200_leak_workspace(-1, 5, 0, 0, 0) == -1
     assert lib.slayer_b200_leak_workspace(1 << 20, 300, 0, 0, 0) == 0
 
