@@ -60,7 +60,7 @@ Gate gate_of(const torch::Tensor &gate, const torch::Tensor &x, const char *op)
                          g.scalar_type());
         return Gate{aligned(g.contiguous())};
     };
-    if (full) return steps(gate);
+    if (full && (gate.size(-1) != 1 || gate.scalar_type() == x.scalar_type())) return steps(gate);      // (of one step: either)
     if (x.numel() == 0) return {gate.expand(x.sizes()).to(x.scalar_type()).contiguous()};       // nothing to do, and no rows to divide
     if (gate.dim() > 0 && gate.size(-1) != 1) return steps(gate.expand(x.sizes()));
     // the same at every step: the dimensions that it has must lie next to each other

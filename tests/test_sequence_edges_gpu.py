@@ -140,3 +140,24 @@ def test_single_steps_of_a_long_stream():
         want = f * want + 1
     # one minus f is known to (8 + |gate|) 2^-24; roundings of up to 10000 states, 2^-24 each, at random: less than 500 of them
     assert bool(((state.double() - want).abs() <= (8 + gate.abs() + 500) * 2.0 ** -24 * want).all())
+
+
+def test_a_gate_of_another_type_on_one_step():
+    """A sequence of one step, of one sample: a float32 gate per neuron has as many elements as x then, and is taken as for longer ones."""
+    gate, h = torch.linspace(-3, 3, 5, device="cuda"), torch.linspace(1, 2, 5, device="cuda").reshape(1, 5)
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        x = torch.linspace(-1, 1, 10, device="cuda").reshape(2, 5, 1).to(dtype)
+        leaf = gate.clone().requires_grad_()
+        y = gatedLeak(x, leaf[None, :, None], initial=h.expand(2, 5))
+        (whole,) = torch.autograd.grad(y, leaf, torch.ones_like(y))
+        for i in range(2):
+            one = gatedLeak(x[i:i + 1], leaf[None, :, None], initial=h)
+            # a float32 gate of one step is taken as one for each step, whose decay is formed otherwise: two decays, each off by (8 + |gate|)
+            # 2^-24 of itself, of a state of up to 2, and two roundings of results of up to 3 each
+            assert torch.allclose(one, y[i:i + 1], rtol=0, atol=(2 * (8 + 3) * 2 + 4 * 3) * 2.0 ** -24 if dtype == torch.float32 else 0)
+            (part,) = torch.autograd.grad(one, leaf, torch.ones_like(one))
+            # one sample's share, h f (1 - f): x has no part in it; f and 1 - f as above, on both sides, and eight roundings
+            assert part.dtype == torch.float32 and torch.allclose(2 * part, whole, rtol=(4 * (8 + 3) + 8) * 2.0 ** -24, atol=0)
+            state = h.clone()
+            step = gatedLeakStep(x[i:i + 1, :, 0], gate[None], state)
+            assert torch.allclose(step.float(), one[..., 0].float(), rtol=2 * torch.finfo(dtype).eps, atol=1e-6)
