@@ -414,7 +414,7 @@ int slayer_b200_leak_backward(void *dx, void *dgate, float *dinitial, const void
 /*
  * One time step of it on rows of a stream: state [rows], float32, is updated in place and y [rows] is the new state
  * in x's type.  gate: [rows] (gate_period 0), or an entry for each group of rows as above; float32 or x's type
- * (gate_dtype).  y may be x.  It has no counterpart in the reference.
+ * (gate_dtype).  y may be x; state shares no memory with the others.  It has no counterpart in the reference.
  */
 int slayer_b200_leak_step(void *y, float *state, const void *x, const void *gate, int dtype, int gate_dtype, int flags, int64_t rows,
                           int64_t gate_inner, int64_t gate_period, void *stream);

@@ -212,6 +212,12 @@ torch::Tensor gatedLeakStepCuda(const torch::Tensor &x, const torch::Tensor &gat
     if (values.scalar_type() != x.scalar_type()) values = values.to(torch::kFloat32);
     c10::cuda::CUDAGuard guard(x.device());
     const auto in = x.contiguous();
+    // a thread would read what another has written
+    const auto apart = [&](const torch::Tensor &v) {
+        const auto a = (uintptr_t)v.data_ptr(), b = (uintptr_t)state.data_ptr();
+        return a + v.nbytes() <= b || b + state.nbytes() <= a;
+    };
+    TORCH_CHECK_VALUE(apart(in) && apart(gate.is_contiguous() ? gate : values), op, ": state must not share memory with x or gate");
     auto y = torch::empty(x.sizes(), x.options());
     check_rc(slayer_b200_leak_step(y.data_ptr(), state.data_ptr<float>(), in.data_ptr(), values.data_ptr(), dtype, dtype_code(values, "gate"), (int)flags,
                                    x.numel(), g.inner, g.period, current_stream()),

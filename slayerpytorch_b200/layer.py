@@ -107,10 +107,10 @@ class _DenseFunction8(torch.autograd.Function):
         weight, *kept = ctx.saved_tensors
         grad = grad.contiguous()
         gradInput = gradWeight = None
-        if ctx.needs_input_grad[0]:
-            gradInput = torch.nn.grad.conv3d_input(ctx.shape, weight, grad)
+        if ctx.needs_input_grad[0]:     # (the forward pass is in 16 bits under autocast, whatever the weight is)
+            gradInput = torch.nn.grad.conv3d_input(ctx.shape, weight.to(grad.dtype), grad)
         if ctx.needs_input_grad[1]:
-            gradWeight = slayerCuda.weightGrad8(grad, *kept, ctx.shape)
+            gradWeight = slayerCuda.weightGrad8(grad.float(), *kept, ctx.shape).to(weight.dtype)
         return gradInput, gradWeight
 
 
@@ -312,6 +312,8 @@ class _DenseLayer(torch.nn.Conv3d):
     reference's dense layer (src/slayer.py:393-437) - same argument forms, same branches, same
     exception texts - because it is the interface the reference's networks are written against;
     weighting is not part of the hot path."""
+
+    checkpoint = False      # of layers that were saved whole before they had it
 
     def __init__(self, inFeatures, outFeatures, weightScale=1, checkpoint=False):
         if isinstance(inFeatures, int):

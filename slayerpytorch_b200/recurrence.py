@@ -43,6 +43,6 @@ def gatedLeak(x, gate, initial=None, lengths=None, kind='logit', coupled=False, 
 
 def gatedLeakStep(x, gate, state, kind='logit', coupled=False):
     """One time step of ``gatedLeak`` on a stream, in one launch: ``x [...]``, ``gate`` broadcasting to it (any of the three types), ``state``
-    of the shape of ``x``, float32 and contiguous, updated in place.  Returns the new state in the type of ``x``.  No gradient
-    flows through it."""
+    of the shape of ``x``, float32 and contiguous, updated in place; it may not share memory with the other two.  Returns the new
+    state in the type of ``x``.  No gradient flows through it."""
     return slayerCuda.gatedLeakStep(x, gate, state, _flags("gatedLeakStep", kind, coupled))

@@ -35,6 +35,9 @@ def test_layers():
     assert net.dense(5, 4, checkpoint=True).checkpoint and not net.dense(5, 4).checkpoint
     with pytest.raises(ValueError, match="inputs of its own size"):
         net.dense((4, 4, 2), 3, checkpoint=True)(torch.zeros(1, 2, 5, 4, 6))
+    old = net.dense(5, 4)
+    del old.__dict__["checkpoint"]      # saved whole before layers had it
+    assert old(torch.zeros(1, 5, 1, 1, 6)).shape == (1, 4, 1, 1, 6)
 
 
 def test_c_entries_of_the_leak():

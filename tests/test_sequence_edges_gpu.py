@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from slayerpytorch_b200 import capi, checkpoint
+from slayerpytorch_b200 import capi, checkpoint, layer
 from slayerpytorch_b200.recurrence import gatedLeak, gatedLeakStep
 
 pytestmark = pytest.mark.gpu
@@ -161,3 +161,49 @@ def test_a_gate_of_another_type_on_one_step():
             state = h.clone()
             step = gatedLeakStep(x[i:i + 1, :, 0], gate[None], state)
             assert torch.allclose(step.float(), one[..., 0].float(), rtol=2 * torch.finfo(dtype).eps, atol=1e-6)
+
+
+def test_a_state_apart_from_what_is_read():
+    """One buffer may hold state, x and gate, but not in the same places."""
+    buffer = torch.rand(40, device="cuda")
+    x, gate, state = buffer[:10], buffer[10:20], buffer[20:30]
+    want = torch.sigmoid(gate.double()) * state.double() + x.double()
+    assert torch.allclose(gatedLeakStep(x, gate, state).double(), want, rtol=16 * 2.0 ** -24, atol=0)
+    for bad in ((buffer[15:25], gate), (x, buffer[29:39]), (x, state[:1]), (state, gate)):
+        before = buffer.clone()
+        with pytest.raises(ValueError, match="share memory"):
+            gatedLeakStep(*bad, state)
+        assert torch.equal(buffer, before)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("auto", [False, True])
+def test_dense_layers_in_16_bits(dtype, auto):
+    """A layer of 16-bit weights, or one under autocast, keeps its input in 8 bits too; its gradients are those of what is kept, in 32 bits."""
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    net = layer.spikeLayer({"type": "SRMALPHA", "theta": 10, "tauSr": 10.0, "tauRef": 1.0, "scaleRef": 2, "tauRho": 1, "scaleRho": 1},
+                           {"Ts": 1.0, "tSample": 50})
+    dense, plain = net.dense(30, 12, checkpoint=True).cuda(), net.dense(30, 12).cuda()
+    plain.load_state_dict(dense.state_dict())
+    kind = torch.float32 if auto else dtype
+    dense, plain = dense.to(kind), plain.to(kind)
+    x = torch.randint(-127, 128, (3, 30, 1, 1, 50), device="cuda", generator=gen).to(kind)      # kept as it is
+    x[..., 0] = 127
+    x[..., 32] = 127
+    leaf = x.clone().requires_grad_()
+    with torch.autocast("cuda", dtype=dtype, enabled=auto):
+        y, z = dense(leaf), plain(x)
+    assert y.dtype == z.dtype == dtype and torch.equal(y, z)
+    g = torch.randn(y.shape, device="cuda", generator=gen).to(dtype)
+    y.backward(g)
+    assert leaf.grad.dtype == dense.weight.grad.dtype == kind
+    # weights: 150 products each, in 32 bits
+    a, b = g.transpose(0, 1).reshape(12, -1).double(), x.transpose(0, 1).reshape(30, -1).double()
+    half = torch.finfo(kind).eps / 2
+    want = (a @ b.T).reshape(dense.weight.shape)
+    assert bool(((dense.weight.grad.double() - want).abs() <= half * 1.01 * want.abs() + (8 + 150 ** 0.5) * 2.0 ** -24 * (a.abs() @ b.abs().T).reshape(want.shape)).all())
+    # inputs: 12 products each, rounded to 16 bits (float16: also to whole multiples of 2^-24)
+    w, up = dense.weight.to(dtype).double().reshape(12, 30), g.double().reshape(3, 12, 50)
+    back, size = torch.einsum("oi,not->nit", w, up), torch.einsum("oi,not->nit", w.abs(), up.abs())
+    half = torch.finfo(dtype).eps / 2
+    assert bool(((leaf.grad.double().reshape(back.shape) - back).abs() <= half * 1.01 * back.abs() + 13 * 2.0 ** -24 * size + 2.0 ** -25).all())
