@@ -11,7 +11,8 @@
 // x is the operand with the tile's rows (i), g the one with its columns (o): large layers take tiles of 256 x 256 by pairs of CTAs, each of which loads and
 // takes apart one half of either; layers of up to 128 outputs tiles of 128 x 16 to 128 x 128 by one CTA.  The tiles' blocks of 64 steps are dealt out
 // to all SMs in equal shares (tile after tile: a share has the end of one tile, some whole ones and the start of another), and the shares'
-// sums are added up by a second launch, in order.
+// sums are added up by a second launch, in order.  Its CTAs start as the first launch's leave, and wait there for the last of them (2 us less than one
+// launch after the other, at every size).
 #include <algorithm>
 
 #include "tensor.cuh"
@@ -417,6 +418,8 @@ __global__ void __launch_bounds__(kWgThreads, 1) weight_grad_kernel(const __grid
         }
         product_commit<CG>(&last);
     }
+    // the CTAs that add the parts up may take the place of this one
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     // all products have read their operands, and told so, before a CTA leaves
     if (warp == 16 && lane == 0 && !mbar_wait_bounded(&last, 0, kWgWaitLimit)) fine = false;
     __syncwarp();
@@ -444,13 +447,14 @@ __global__ void __launch_bounds__(256) weight_sum_kernel(float *out, const WgArg
     if (threadIdx.x < 2) range[threadIdx.x] = (int)((((tile + threadIdx.x) * A.blocks + 1 - threadIdx.x) * A.shares - 1) / A.work);
     __syncthreads();
     const int first = range[0], last = range[1];
+    asm volatile("griddepcontrol.wait;" ::: "memory");       // all parts are there
     const int64_t i = ti * R + row, o = to * NT + col;
     const bool there = i < A.I && o < A.O;
     double sum[4] = {};
     const float *p = A.part + (first + turn + tile) * (int64_t)(R * NT) + (int64_t)col * R + row;
 #pragma unroll 8
     for (int s = first + turn; s <= last && there; s += SPLIT, p += SPLIT * (int64_t)(R * NT)) {
-        const float4 v = __ldg(reinterpret_cast<const float4 *>(p));
+        const float4 v = *reinterpret_cast<const float4 *>(p);        // (__ldg might be moved before the wait)
         sum[0] += (double)v.x, sum[1] += (double)v.y, sum[2] += (double)v.z, sum[3] += (double)v.w;
     }
     if (SPLIT > 1) {
@@ -527,8 +531,16 @@ static int wg_launch(const WgArgs &A, float *out, int64_t tiles, cudaStream_t st
     const int bad = check_launch("weight_grad8 kernel launch");
     if (bad) return bad;
     // (a tile with many parts: 37 of them one after the other 7.5 us, in fours 4.7)
-    if (A.shares / tiles >= 16) weight_sum_kernel<CG, NT, 4><<<dim3((unsigned)tiles, CG, NT / 2), 256, 0, st>>>(out, A);
-    else weight_sum_kernel<CG, NT, 1><<<dim3((unsigned)tiles, CG, NT / 8), 256, 0, st>>>(out, A);
+    const bool many = A.shares / tiles >= 16;
+    cudaLaunchConfig_t then = {};
+    then.gridDim = dim3((unsigned)tiles, CG, many ? NT / 2 : NT / 8);
+    then.blockDim = dim3(256);
+    then.stream = st;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    then.attrs = attr;
+    then.numAttrs = 1;
+    cudaLaunchKernelEx(&then, many ? weight_sum_kernel<CG, NT, 4> : weight_sum_kernel<CG, NT, 1>, out, A);
     return check_launch("weight_grad8 sum launch");
 }
 
@@ -571,7 +583,9 @@ extern "C" int slayer_b200_weight_grad8(float *out, const float *g, const int8_t
     if (!status) { set_error("weight_grad8: no status word on this device"); return SLAYER_B200_ECUDA; }
     const WgPlan p = wg_plan(N, O, I, T);
     const int U = (int)ceil_div(T, 16);
-    const WgArgs A = {g, q, scale, (float *)workspace, status, N, O, I, T, ceil_div(T, 32), N * O * T, (int)(N * U), (int)p.blocks, U, (int)std::max<int64_t>(0, N - ceil_div(8, O * T)), p.tiles_o, p.tiles * p.blocks, (int)p.shares};
+    const int inner = (int)std::max<int64_t>(0, N - ceil_div(8, O * T));
+    const WgArgs A = {g, q, scale, (float *)workspace, status, N, O, I, T, ceil_div(T, 32), N * O * T, (int)(N * U), (int)p.blocks, U, inner,
+                      p.tiles_o, p.tiles * p.blocks, (int)p.shares};
     switch (p.nt) {
     case 256: return wg_align<2, 256>(A, out, p.tiles, st);
     case 128: return wg_align<1, 128>(A, out, p.tiles, st);
