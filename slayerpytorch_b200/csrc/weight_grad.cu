@@ -171,27 +171,18 @@ __global__ void __launch_bounds__(kWgThreads, 1) weight_grad_kernel(const __grid
     __shared__ uint32_t base_at;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = CG == 2 ? (int)cluster_rank() : 0;
-    if (warp == 16) tensor_alloc<CG>(&base_at, Tile::kMem);
-    if (tid == 0) {
-        for (int s = 0; s < S; ++s) {
-            mbar_init(full + s, 16 * CG);
-            mbar_init(empty + s, 1);
-        }
-        for (int b = 0; b < 2; ++b) {
-            mbar_init(made + b, 1);
-            mbar_init(taken + b, 16 * CG);
-        }
-        mbar_init(&last, 1);
-        mbar_init_fence();
-    }
-    tensor_fence_before();
-    __syncthreads();
-    if (CG == 2) cluster_wait_all();
-    tensor_fence_after();
-    const uint32_t acc = base_at;
     const int share = blockIdx.x / CG;
     const int64_t from = A.work * share / A.shares, to = A.work * (share + 1) / A.shares;
+    uint32_t acc = 0;
     bool fine = true;
+    // barriers and tensor memory are there: what the workers wait for with their first blocks on the way
+    const auto ready = [&] {
+        tensor_fence_before();
+        asm volatile("barrier.cta.sync 1, %0;" ::"n"(kWgThreads) : "memory");
+        if (CG == 2) cluster_wait_all();
+        tensor_fence_after();
+        acc = base_at;
+    };
 
     // registers: 512 * 112 + 128 * 32 = 640 * 96
     if (warp < 16) {
@@ -201,7 +192,6 @@ __global__ void __launch_bounds__(kWgThreads, 1) weight_grad_kernel(const __grid
         const int brow = (warp >> 2) * (Tile::NB >= 32 ? Tile::NB / 4 : 8) + 2 * ((lane >> 2) & 3) + (lane >> 4);
         const bool has_b = Tile::NB >= 32 || (warp >> 2) * 8 < Tile::NB;
         const bool sums_here = (warp >> 2) * Tile::kCols < NT;
-        const uint32_t at = acc + ((uint32_t)((warp & 3) * 32) << 16) + (warp >> 2) * Tile::kCols;
         // what a thread has fetched lies where nobody else (VEC), or nobody else of another warp, reads it
         unsigned char *const raw = smem + S * Tile::kStage + tid * 16;
         // what comes after them, where the next thread does not have it: for one of the four threads of a row's unit
@@ -223,8 +213,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) weight_grad_kernel(const __grid
         };
         const auto find_b = [&] { bg = A.g + ((int64_t)ub.n * A.O + o) * A.T + ub.t16 * 16 + quarter * 4; };
         const int64_t a_groups = 2 * A.N * A.I;
-        const auto fetch = [&](int slot) {
-            scale_0 = scale_1;
+        const auto fetch = [&](int slot, unsigned &scale) {
             if (ahead < to) {
                 if (tile_left == 0) {
                     const int64_t tile = ahead / A.blocks, ti = tile / A.tiles_o;
@@ -243,7 +232,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) weight_grad_kernel(const __grid
                 unsigned char *const into = raw + slot * Tile::kRaw;
                 const bool a = ua.unit < A.units;
                 wg_copy(into, a ? aq : A.q, a ? 16 : 0);
-                if (a) scale_1 = __ldg(as);
+                if (a) scale = __ldg(as);
                 if (has_b) {
                     const int t = ub.t16 * 16 + quarter * 4;
                     const bool b = ub.unit < A.units && t < (int)A.T;
@@ -285,8 +274,10 @@ __global__ void __launch_bounds__(kWgThreads, 1) weight_grad_kernel(const __grid
             wg_copies_commit();
         };
         int s = 0, turn = 0, slot = 0, again = 0, from_slot = 0;
-        fetch(0);
-        fetch(1);
+        fetch(0, scale_0);
+        fetch(1, scale_1);
+        ready();
+        const uint32_t at = acc + ((uint32_t)((warp & 3) * 32) << 16) + (warp >> 2) * Tile::kCols;
         WgUnit uc;        // of g in the block that is worked on: what lies behind T is not g's
         for (int64_t w = from; fine && w < to;) {
             const int64_t tile = w / A.blocks;
@@ -364,7 +355,8 @@ __global__ void __launch_bounds__(kWgThreads, 1) weight_grad_kernel(const __grid
                     else mbar_arrive(full + s);
                 }
                 if (++s == S) { s = 0; turn ^= 1; }
-                fetch(from_slot);
+                scale_0 = scale_1;
+                fetch(from_slot, scale_1);
                 from_slot ^= 1;
                 if (!VEC) uc.next(A.U);
                 // the sum before the one whose last block this is: its products are done, or nearly so
@@ -387,6 +379,21 @@ __global__ void __launch_bounds__(kWgThreads, 1) weight_grad_kernel(const __grid
         wg_copies_wait_all();
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
+        if (warp == 16) tensor_alloc<CG>(&base_at, Tile::kMem);
+        if (tid == kWgWorkers) {
+            for (int s = 0; s < S; ++s) {
+                mbar_init(full + s, 16 * CG);
+                mbar_init(empty + s, 1);
+            }
+            for (int b = 0; b < 2; ++b) {
+                mbar_init(made + b, 1);
+                mbar_init(taken + b, 16 * CG);
+            }
+            mbar_init(&last, 1);
+            mbar_init_fence();
+        }
+        __syncwarp();
+        ready();
     }
     if (warp == 16 && lane == 0 && rank == 0) {
         constexpr uint32_t kShape = product_shape_bf16(128 * CG, NT);
