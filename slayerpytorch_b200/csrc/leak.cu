@@ -12,7 +12,7 @@
 // Maps are floats: A, and 1 - A by itself (R), and B.  A slow leak's f is next to one, where its rounding to 32 bits, taken at each of the thousands of
 // steps that such a state remembers, adds up to 1e-4 of it; R has 24 bits of what is forgotten instead.  States are double from chunk to chunk, and
 // float within the up to 16 steps that a lane walks.  (All of it in double, with half as many instructions again: 39 + 74 us instead of
-// 28 + 49 of the time, 64 x 512 x 300.)
+// 28 + 49 of the time, 64 x 512 x 300.)  Single steps, and rows of few, are in double throughout.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -438,6 +438,120 @@ leak_backward_kernel(E *dx, E *dgate, double *sums, float *dinitial, const E *g,
     if (dinitial && there && lane == 0 && segment == 0) dinitial[row] = (float)carry;
 }
 
+// One step of a state in double: by what is forgotten of it, or by what is kept, whichever is less.
+__device__ __forceinline__ double step_state(const Decay &d, double h, double u) { return u + (d.f < 0.5f ? (double)d.f * h : fma(-(double)d.rest, h, h)); }
+
+// Rows of up to 13 steps that do not end on vectors, which a lane has alone.  Their vectors would all be picked apart, an element at a time (8000000 x 5
+// float32: 162 us forward and 309 backward; so it is 113 and 207).  A CTA's rows are one piece of memory that begins at 16 bytes: it is copied to
+// shared memory as it is, a thread walks a row there, its state in double, and results go back the same way.
+constexpr int kShortSteps = 13;
+
+template <typename E>
+__device__ __forceinline__ void short_fetch(E *tile, const E *from, int count)
+{
+    constexpr int W = 16 / (int)sizeof(E);
+    const int whole = count / W;
+    for (int i = threadIdx.x; i < whole; i += kLeakThreads)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(tile + i * W)), "l"(from + i * W) : "memory");
+    for (int i = whole * W + threadIdx.x; i < count; i += kLeakThreads) tile[i] = from[i];
+}
+
+__device__ __forceinline__ void short_fetched()
+{
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+}
+
+template <typename E>
+__device__ __forceinline__ void short_store(E *to, const E *tile, int count)
+{
+    constexpr int W = 16 / (int)sizeof(E);
+    const int whole = count / W;
+    for (int i = threadIdx.x; i < whole; i += kLeakThreads) reinterpret_cast<uint4 *>(to)[i] = reinterpret_cast<const uint4 *>(tile)[i];
+    for (int i = whole * W + threadIdx.x; i < count; i += kLeakThreads) to[i] = tile[i];
+}
+
+template <typename E>
+__global__ void __launch_bounds__(kLeakThreads)
+leak_short_forward_kernel(E *y, float *state, float *starts, const E *x, const void *gate, const float *initial, const LeakShape s)
+{
+    extern __shared__ __align__(16) unsigned char short_memory[];
+    E *const xs = reinterpret_cast<E *>(short_memory), *const gs = xs + kLeakThreads * s.T;
+    const int64_t first = (int64_t)blockIdx.x * kLeakThreads;
+    const int here = (int)min((int64_t)kLeakThreads, s.rows - first), count = here * s.T;
+    short_fetch(xs, x + first * s.T, count);
+    if (s.gate_period == 0) short_fetch(gs, (const E *)gate + first * s.T, count);
+    short_fetched();
+    if (threadIdx.x < here) {
+        const int row = (int)first + threadIdx.x, length = row_of(s, row).length;
+        const Decay row_d = row_gate(s, gate, row);
+        E *const xr = xs + threadIdx.x * s.T;
+        const E *const gr = gs + threadIdx.x * s.T;
+        double h = initial ? (double)initial[row] : 0.0;
+        if (starts) starts[row] = (float)h;
+        for (int t = 0; t < s.T; ++t) {
+            if (t < length) {
+                const Decay d = s.gate_period ? row_d : decay_of(to_float<E>(gr[t]), s.logit);
+                const float v = to_float<E>(xr[t]);
+                h = step_state(d, h, (double)(s.coupled ? d.rest * v : v));
+            }
+            xr[t] = from_float<E>(t < length ? (float)h : 0.0f);
+        }
+        if (state) state[row] = (float)h;
+    }
+    __syncthreads();
+    short_store(y + first * s.T, xs, count);
+}
+
+template <typename E>
+__global__ void __launch_bounds__(kLeakThreads)
+leak_short_backward_kernel(E *dx, E *dgate, double *sums, float *dinitial, const E *g, const float *gstate, const float *starts, const E *x, const void *gate,
+                           const LeakShape s)
+{
+    extern __shared__ __align__(16) unsigned char short_memory[];
+    E *const xs = reinterpret_cast<E *>(short_memory), *const gs = xs + kLeakThreads * s.T, *const up = gs + kLeakThreads * s.T;
+    float *const slopes = reinterpret_cast<float *>(up + kLeakThreads * s.T);        // what lambda is multiplied by in dgate
+    const int64_t first = (int64_t)blockIdx.x * kLeakThreads;
+    const int here = (int)min((int64_t)kLeakThreads, s.rows - first), count = here * s.T;
+    short_fetch(xs, x + first * s.T, count);
+    short_fetch(up, g + first * s.T, count);
+    if (s.gate_period == 0) short_fetch(gs, (const E *)gate + first * s.T, count);
+    short_fetched();
+    if (threadIdx.x < here) {
+        const int row = (int)first + threadIdx.x, length = row_of(s, row).length;
+        const Decay row_d = row_gate(s, gate, row);
+        E *const xr = xs + threadIdx.x * s.T, *const gr = gs + threadIdx.x * s.T;
+        const E *const ur = up + threadIdx.x * s.T;
+        float *const slope = slopes + threadIdx.x * s.T;
+        double at = starts[row], sum = 0.0;
+        for (int t = 0; t < length; ++t) {
+            const Decay d = s.gate_period ? row_d : decay_of(to_float<E>(gr[t]), s.logit);
+            const float v = to_float<E>(xr[t]), k = (float)at - (s.coupled ? v : 0.0f);
+            slope[t] = s.logit ? k * (d.f * d.rest) : k;
+            at = step_state(d, at, (double)(s.coupled ? d.rest * v : v));
+        }
+        double carry = gstate ? (double)gstate[row] : 0.0;
+        for (int t = s.T - 1; t >= 0; --t) {
+            float to_x = 0.0f, to_gate = 0.0f;
+            if (t < length) {
+                const Decay d = s.gate_period ? row_d : decay_of(to_float<E>(gr[t]), s.logit);
+                const double lambda = (double)to_float<E>(ur[t]) + carry;
+                carry = step_state(d, lambda, 0.0);
+                to_x = s.coupled ? (float)lambda * d.rest : (float)lambda;
+                to_gate = (float)lambda * slope[t];
+                sum += (double)to_gate;
+            }
+            xr[t] = from_float<E>(to_x);
+            if (dgate) gr[t] = from_float<E>(to_gate);
+        }
+        if (sums) sums[row] = sum;
+        if (dinitial) dinitial[row] = (float)carry;
+    }
+    __syncthreads();
+    if (dx) short_store(dx + first * s.T, xs, count);
+    if (dgate) short_store(dgate + first * s.T, gs, count);
+}
+
 // The gradient of a gate per row is the sum over the rows that have it, in a fixed order: rows (k period + i) inner + j of gate i.  parts > 1:
 // each of them sums every parts-th entry, and a second launch (inner = parts, period = gates, outer = 1) those.
 __global__ void __launch_bounds__(256)
@@ -466,8 +580,8 @@ leak_step_kernel(E *y, float *state, const E *x, const EG *gate, int64_t rows, i
     const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (row >= rows) return;
     const Decay d = decay_of(to_float<EG>(gate[period ? row / inner % period : row]), logit);
-    const float v = to_float<E>(x[row]), at = state[row];
-    const float h = (float)((double)(coupled ? d.rest * v : v) + (d.f < 0.5f ? (double)d.f * (double)at : fma(-(double)d.rest, (double)at, (double)at)));
+    const float v = to_float<E>(x[row]);
+    const float h = (float)step_state(d, (double)state[row], (double)(coupled ? d.rest * v : v));
     state[row] = h;
     y[row] = from_float<E>(h);
 }
@@ -555,6 +669,12 @@ static void run_forward(const LeakPlan &p, void *y, float *state, float *starts,
     const unsigned blocks = (unsigned)ceil_div((int64_t)p.s.rows * p.s.segments * G, kLeakThreads);
     if constexpr (G == 32)
         if (p.s.segments > 1) leak_maps_kernel<E, K, true><<<blocks, kLeakThreads, 0, st>>>(maps, (const E *)x, gate, p.s);
+    if constexpr (G == 1)
+        if (p.s.T % kVector != 0 && p.s.T <= kShortSteps) {
+            leak_short_forward_kernel<E><<<blocks, kLeakThreads, 2 * kLeakThreads * p.s.T * sizeof(E), st>>>((E *)y, state, starts, (const E *)x, gate, initial,
+                                                                                                            p.s);
+            return;
+        }
     leak_forward_kernel<E, G, K><<<blocks, kLeakThreads, 0, st>>>((E *)y, state, starts, (const E *)x, gate, initial, maps, p.s);
 }
 
@@ -568,8 +688,18 @@ static void run_backward(const LeakPlan &p, void *dx, void *dgate, float *diniti
     const unsigned blocks = (unsigned)ceil_div((int64_t)p.s.rows * p.s.segments * G, kLeakThreads);
     if constexpr (G == 32)
         if (p.s.segments > 1) leak_maps_kernel<E, K, false><<<blocks, kLeakThreads, 0, st>>>(maps, (const E *)g, gate, p.s);
-    leak_backward_kernel<E, G, K><<<blocks, kLeakThreads, 0, st>>>((E *)dx, per_row ? nullptr : (E *)dgate, per_row && dgate ? sums : nullptr, dinitial,
-                                                                (const E *)g, gstate, starts, (const E *)x, gate, maps, p.s);
+    E *const to_gate = per_row ? nullptr : (E *)dgate;
+    double *const to_sums = per_row && dgate ? sums : nullptr;
+    bool done = false;
+    if constexpr (G == 1)
+        if (p.s.T % kVector != 0 && p.s.T <= kShortSteps) {
+            leak_short_backward_kernel<E><<<blocks, kLeakThreads, kLeakThreads * p.s.T * (3 * sizeof(E) + sizeof(float)), st>>>(
+                (E *)dx, to_gate, to_sums, dinitial, (const E *)g, gstate, starts, (const E *)x, gate, p.s);
+            done = true;
+        }
+    if (!done)
+        leak_backward_kernel<E, G, K><<<blocks, kLeakThreads, 0, st>>>((E *)dx, to_gate, to_sums, dinitial, (const E *)g, gstate, starts, (const E *)x, gate, maps,
+                                                                       p.s);
     if (per_row && dgate) {
         const int64_t inner = (int64_t)p.s.gate_inner * p.s.segments, outer = p.s.rows / ((int64_t)p.s.gate_inner * p.s.gate_period);
         double *part = sums + (int64_t)p.s.rows * p.s.segments;

@@ -143,6 +143,19 @@ def test_lengths_of_rows(T, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T", [1, 2, 3, 4, 5, 6, 7, 9, 10, 11, 12, 13, 14, 15, 17])
+def test_many_short_rows(T, dtype):
+    """Rows that end inside of vectors, more than a CTA has and not a multiple of it; with lengths, and gates per step and per row."""
+    gen = torch.Generator(device="cuda").manual_seed(40 + T)
+    for N, C in ((1, 127), (1, 128), (7, 43)):
+        for coupled, kind in ((False, 'decay'), (True, 'logit')):
+            for shape in ((N, C, T), (C, 1)):
+                x, gate, h, g, gs, _ = made(N, C, T, dtype, kind, T + N, shape)
+                lengths = torch.randint(-1, T + 2, (N,), device="cuda", generator=gen) if coupled else None
+                check(x, gate, h, lengths, kind, coupled, g, gs)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("N,C,T", [(1, 1, 700), (1, 1, 5003), (1, 3, 20001), (2, 16, 4099), (1, 300, 2048), (1, 1500, 1030), (7, 700, 600)])
 def test_long_rows_and_few(N, C, T, dtype):
     """Rows that are split among groups of lanes, and those that are just not."""
