@@ -23,7 +23,7 @@ namespace sb200 {
 constexpr int kLeakThreads = 128;
 
 // CTAs of an SM that registers are rationed for: the most that leave (nearly) none of a lane's steps in memory
-template <int K> constexpr int kForwardBlocks = K < 4 ? 9 : 7;
+template <int K, bool LINED> constexpr int kForwardBlocks = K < 4 ? 9 : LINED ? 7 : 6;
 template <int K> constexpr int kBackwardBlocks = K < 4 ? 6 : 5;
 
 template <typename E> __device__ __forceinline__ float to_float(E v);
@@ -52,6 +52,7 @@ struct LeakShape {
 struct Row {
     int64_t base;              // first element
     int skew, length;          // elements between the vector it begins in and itself; steps that count
+    int reach;                 // elements from its first to the tensor's last, as far as that matters
 };
 
 __device__ __forceinline__ Row row_of(const LeakShape &s, int row)
@@ -59,6 +60,7 @@ __device__ __forceinline__ Row row_of(const LeakShape &s, int row)
     Row r;
     r.base = (int64_t)row * s.T;
     r.skew = (int)(r.base & (kVector - 1));
+    r.reach = (int)min((int64_t)(s.rows - row) * s.T, (int64_t)s.T + kVector);
     r.length = s.T;
     if (s.lengths) {
         const int64_t n = __ldg(s.lengths + (unsigned)row / (unsigned)s.sample_rows);
@@ -70,26 +72,27 @@ __device__ __forceinline__ Row row_of(const LeakShape &s, int row)
 template <typename E> struct Packed { using type = uint2; };
 template <> struct Packed<float> { using type = uint4; };
 
-// Which of a lane's vectors lie in [0, end) of a row as a whole, and whether one of them lies there in part.
-template <int K>
+// Which of a lane's vectors lie in [0, end) of a row as a whole, and whether one of them lies there in part: its first one, which may begin before the row,
+// or the one that `end` is in.  Vectors that begin before `stop` are read whole, though other rows' steps are in them: reach elements from the row's
+// first on are the tensor's.  LINED: rows end with their vectors, and all steps count.
+// (Without that it was 86 us forward and 158 backward instead of 82 and 154, float32, 78125 x 512.)
+template <int K, bool LINED>
 struct Inside {
-    int t, end;
+    int t, end, stop;
     bool whole[K], part;
-    __device__ __forceinline__ Inside(int t_, int end_) : t(t_), end(end_)
+    __device__ __forceinline__ Inside(int t_, int end_, int reach) : t(t_), end(end_), stop(min(end_, reach - 3))
     {
-        part = false;
+        const int left = end - t;
+        part = !LINED && (t < 0 || (left > 0 && left < 4 * K && (left & 3) != 0));
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const int at = t + 4 * k;
-            whole[k] = at >= 0 && at <= end - 4;
-            part = part || (!whole[k] && at < end && at > -4);
-        }
+        for (int k = 0; k < K; ++k) whole[k] = LINED ? left > 4 * k : (k > 0 || t >= 0) && left >= 4 * k + 4;
     }
 };
 
-// steps [t, t + 4 K) of a row, `fill` where they are outside
-template <typename E, int K>
-__device__ __forceinline__ void load_steps(float (&v)[4 * K], const E *row, const Inside<K> &in, float fill)
+// Steps [t, t + 4 K) of a row, `fill` where they are outside.  A vector that is there in part is read whole, other rows' steps with it: only
+// the tensor's last one may not be.  (One by one it was 133 us forward and 254 backward instead of 131 and 219, float32, 1212121 x 33.)
+template <typename E, int K, bool LINED>
+__device__ __forceinline__ void load_steps(float (&v)[4 * K], const E *row, const Inside<K, LINED> &in, float fill)
 {
     using P = typename Packed<E>::type;
     P raw[K];
@@ -97,7 +100,7 @@ __device__ __forceinline__ void load_steps(float (&v)[4 * K], const E *row, cons
     for (int k = 0; k < K; ++k) {
         E none[4] = {from_float<E>(fill), from_float<E>(fill), from_float<E>(fill), from_float<E>(fill)};
         raw[k] = *reinterpret_cast<P *>(none);
-        if (in.whole[k]) raw[k] = __ldg(reinterpret_cast<const P *>(row + in.t + 4 * k));
+        if (LINED ? in.whole[k] : in.t + 4 * k < in.stop) raw[k] = __ldg(reinterpret_cast<const P *>(row + in.t + 4 * k));
     }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -107,20 +110,20 @@ __device__ __forceinline__ void load_steps(float (&v)[4 * K], const E *row, cons
     }
     if (in.part) {
 #pragma unroll
-        for (int k = 0; k < K; ++k)
-            if (!in.whole[k]) {
+        for (int j = 0; j < 4 * K; ++j) v[j] = (unsigned)(in.t + j) < (unsigned)in.end ? v[j] : fill;
+        if (in.stop < in.end) {     // the tensor's last row
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int at = in.t + 4 * k + j;
-                    if (at >= 0 && at < in.end) v[4 * k + j] = to_float<E>(row[at]);
-                }
+            for (int j = 0; j < 4 * K; ++j) {
+                const int at = in.t + j;
+                if (at >= 0 && at < in.end && in.t + (j & ~3) >= in.stop) v[j] = to_float<E>(row[at]);
             }
+        }
     }
 }
 
 // results of the steps inside
-template <typename E, int K>
-__device__ __forceinline__ void store_inside(E *row, const Inside<K> &in, const float (&v)[4 * K])
+template <typename E, int K, bool LINED>
+__device__ __forceinline__ void store_inside(E *row, const Inside<K, LINED> &in, const float (&v)[4 * K])
 {
     using P = typename Packed<E>::type;
 #pragma unroll
@@ -132,28 +135,39 @@ __device__ __forceinline__ void store_inside(E *row, const Inside<K> &in, const 
         if (in.whole[k]) *reinterpret_cast<P *>(row + in.t + 4 * k) = raw;
     }
     if (in.part) {
+        // the vector that begins before the row, and the one that it ends in
+        const int last = (in.end - in.t) >> 2;
+        if (in.t < 0) {
 #pragma unroll
-        for (int k = 0; k < K; ++k)
-            if (!in.whole[k]) {
+            for (int j = 1; j < 4; ++j)
+                if (in.t + j >= 0 && in.t + j < in.end) row[in.t + j] = from_float<E>(v[j]);
+        }
+        if (last < K && (last > 0 || in.t >= 0)) {
+            float e[3];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int at = in.t + 4 * k + j;
-                    if (at >= 0 && at < in.end) row[at] = from_float<E>(v[4 * k + j]);
-                }
+            for (int j = 0; j < 3; ++j) {
+                e[j] = v[j];
+#pragma unroll
+                for (int k = 1; k < K; ++k) e[j] = last == k ? v[4 * k + j] : e[j];
             }
+            const int at = in.t + 4 * last;
+#pragma unroll
+            for (int j = 0; j < 3; ++j)
+                if (at + j < in.end) row[at + j] = from_float<E>(e[j]);
+        }
     }
 }
 
 // and zeros from `in.end` to T
-template <typename E, int K>
-__device__ __forceinline__ void store_steps(E *row, const Inside<K> &in, int T, float (&v)[4 * K])
+template <typename E, int K, bool LINED>
+__device__ __forceinline__ void store_steps(E *row, const Inside<K, LINED> &in, int T, float (&v)[4 * K])
 {
-    if (in.end == T) {
-        store_inside<E, K>(row, in, v);
+    if (LINED || in.end == T) {
+        store_inside<E, K, LINED>(row, in, v);
     } else {
 #pragma unroll
         for (int j = 0; j < 4 * K; ++j) v[j] = in.t + j < in.end ? v[j] : 0.0f;
-        store_inside<E, K>(row, Inside<K>(in.t, T), v);
+        store_inside<E, K, LINED>(row, Inside<K, LINED>(in.t, T, T), v);
     }
 }
 
@@ -179,12 +193,13 @@ struct Steps {
     Decay d[4 * K];
     float x[4 * K];
 
-    __device__ __forceinline__ void load(const LeakShape &s, const Row &row, const E *x_, const E *gate, const Decay &row_d, const Inside<K> &in)
+    template <bool LINED>
+    __device__ __forceinline__ void load(const LeakShape &s, const Row &row, const E *x_, const E *gate, const Decay &row_d, const Inside<K, LINED> &in)
     {
-        load_steps<E, K>(x, x_ + row.base, in, 0.0f);
+        load_steps<E, K, LINED>(x, x_ + row.base, in, 0.0f);
         if (s.gate_period == 0) {
             float g[4 * K];
-            load_steps<E, K>(g, gate + row.base, in, s.logit ? INFINITY : 1.0f);
+            load_steps<E, K, LINED>(g, gate + row.base, in, s.logit ? INFINITY : 1.0f);
 #pragma unroll
             for (int j = 0; j < 4 * K; ++j) d[j] = decay_of(g[j], s.logit);
         } else {
@@ -323,7 +338,7 @@ __device__ __forceinline__ Decay row_gate(const LeakShape &s, const void *gate, 
 }
 
 // Maps of segments: rows too few to fill the GPU are split, and each segment starts from what those before it leave.
-template <typename E, int K, bool FORWARD>
+template <typename E, int K, bool LINED, bool FORWARD>
 __global__ void __launch_bounds__(kLeakThreads)
 leak_maps_kernel(Map *maps, const E *x, const void *gate, const LeakShape s)
 {
@@ -336,7 +351,7 @@ leak_maps_kernel(Map *maps, const E *x, const void *gate, const LeakShape s)
     for (int i = first; i < last; ++i) {
         const int c = FORWARD ? i : last - 1 - (i - first);
         Steps<E, K> st;
-        st.load(s, r, x, (const E *)gate, row_d, Inside<K>((c * 32 + lane) * (4 * K) - r.skew, r.length));
+        st.load(s, r, x, (const E *)gate, row_d, Inside<K, LINED>((c * 32 + lane) * (4 * K) - r.skew, r.length, r.reach));
         if (FORWARD) {
             st.couple(s.coupled);
             all = compose(all, shift_from(scan<32, true>(forward_map<E, K>(st), lane), 31));
@@ -347,8 +362,8 @@ leak_maps_kernel(Map *maps, const E *x, const void *gate, const LeakShape s)
     if (lane == 0) maps[row * s.segments + segment] = all;
 }
 
-template <typename E, int G, int K>
-__global__ void __launch_bounds__(kLeakThreads, kForwardBlocks<K>)
+template <typename E, int G, int K, bool LINED>
+__global__ void __launch_bounds__(kLeakThreads, kForwardBlocks<K, LINED>)
 leak_forward_kernel(E *y, float *state, float *starts, const E *x, const void *gate, const float *initial, const Map *maps, const LeakShape s)
 {
     int row, segment, lane;
@@ -361,7 +376,7 @@ leak_forward_kernel(E *y, float *state, float *starts, const E *x, const void *g
     if (G == 32 && segment > 0) h = through_segments<true>(maps + row * s.segments, 0, segment, lane, h);
     const int first = segment * s.segment_chunks, last = min(first + s.segment_chunks, s.chunks);
     for (int c = first; c < last; ++c) {
-        const Inside<K> in((c * G + lane) * (4 * K) - r.skew, r.length);
+        const Inside<K, LINED> in((c * G + lane) * (4 * K) - r.skew, r.length, r.reach);
         Steps<E, K> st;
         st.load(s, r, x, (const E *)gate, row_d, in);
         st.couple(s.coupled);
@@ -374,13 +389,13 @@ leak_forward_kernel(E *y, float *state, float *starts, const E *x, const void *g
             at = fmaf(st.d[j].f, at, st.x[j]);
             st.x[j] = at;
         }
-        if (there) store_steps<E, K>(y + r.base, in, s.T, st.x);
+        if (there) store_steps<E, K, LINED>(y + r.base, in, s.T, st.x);
     }
     if (state && there && lane == 0 && segment == s.segments - 1) state[row] = (float)h;
 }
 
 // sums: per row and segment, of df: the gradient of a gate per row
-template <typename E, int G, int K>
+template <typename E, int G, int K, bool LINED>
 __global__ void __launch_bounds__(kLeakThreads, kBackwardBlocks<K>)
 leak_backward_kernel(E *dx, E *dgate, double *sums, float *dinitial, const E *g, const float *gstate, const float *starts, const E *x, const void *gate,
                      const Map *maps, const LeakShape s)
@@ -396,10 +411,10 @@ leak_backward_kernel(E *dx, E *dgate, double *sums, float *dinitial, const E *g,
     if (G == 32 && segment + 1 < s.segments) carry = through_segments<false>(maps + row * s.segments, segment + 1, s.segments, lane, carry);
     const int first = segment * s.segment_chunks, last = min(first + s.segment_chunks, s.chunks);
     for (int c = last - 1; c >= first; --c) {
-        const Inside<K> in((c * G + lane) * N - r.skew, r.length);
+        const Inside<K, LINED> in((c * G + lane) * N - r.skew, r.length, r.reach);
         float gv[N], slope[N];       // slope: what lambda is multiplied by in dgate
         Steps<E, K> st;
-        load_steps<E, K>(gv, g + r.base, in, 0.0f);
+        load_steps<E, K, LINED>(gv, g + r.base, in, 0.0f);
         st.load(s, r, x, (const E *)gate, row_d, in);
         float at = starts[((int64_t)row * s.chunks + c) * G + lane];
 #pragma unroll
@@ -421,8 +436,8 @@ leak_backward_kernel(E *dx, E *dgate, double *sums, float *dinitial, const E *g,
             gv[j] = s.coupled ? lambda * st.d[j].rest : lambda;
             slope[j] *= lambda;
         }
-        if (there && dx) store_steps<E, K>(dx + r.base, in, s.T, gv);
-        if (there && dgate) store_steps<E, K>(dgate + r.base, in, s.T, slope);
+        if (there && dx) store_steps<E, K, LINED>(dx + r.base, in, s.T, gv);
+        if (there && dgate) store_steps<E, K, LINED>(dgate + r.base, in, s.T, slope);
         if (sums) {
             float part = 0.0f;
 #pragma unroll
@@ -630,6 +645,7 @@ static bool known(int dtype) { return dtype == SLAYER_B200_F32 || dtype == SLAYE
 struct LeakPlan {
     LeakShape s;
     LeakLanes l;
+    bool lined;                          // rows end with their vectors, and all of their steps count
     int64_t maps_bytes, sums_bytes, gate_parts;
 };
 
@@ -645,6 +661,7 @@ static int plan_leak(LeakPlan &p, const char *op, int dtype, int flags, int64_t 
                   "%s: rows must be whole groups of gates", op);
     SB200_REQUIRE(!lengths || sample_rows >= 1, "%s: lengths need the number of rows that have one", op);
     p.l = lanes_of(T);
+    p.lined = T % kVector == 0 && !lengths;
     const int64_t chunks = chunks_of(T), segments = rows ? segments_of(rows, T) : 1;
     p.s = {(int)rows, (int)T, (int)gate_inner, (int)gate_period, (int)(sample_rows < rows ? sample_rows : rows), lengths, (int)chunks, (int)segments,
            (int)ceil_div(chunks, segments), (flags & SLAYER_B200_LEAK_LOGIT) != 0, (flags & SLAYER_B200_LEAK_COUPLED) != 0};
@@ -661,24 +678,24 @@ static int plan_leak(LeakPlan &p, const char *op, int dtype, int flags, int64_t 
     return SLAYER_B200_OK;
 }
 
-template <typename E, int G, int K>
+template <typename E, int G, int K, bool LINED>
 static void run_forward(const LeakPlan &p, void *y, float *state, float *starts, const void *x, const void *gate, const float *initial, void *workspace,
                         cudaStream_t st)
 {
     Map *maps = (Map *)workspace;
     const unsigned blocks = (unsigned)ceil_div((int64_t)p.s.rows * p.s.segments * G, kLeakThreads);
     if constexpr (G == 32)
-        if (p.s.segments > 1) leak_maps_kernel<E, K, true><<<blocks, kLeakThreads, 0, st>>>(maps, (const E *)x, gate, p.s);
-    if constexpr (G == 1)
+        if (p.s.segments > 1) leak_maps_kernel<E, K, LINED, true><<<blocks, kLeakThreads, 0, st>>>(maps, (const E *)x, gate, p.s);
+    if constexpr (G == 1 && !LINED)
         if (p.s.T % kVector != 0 && p.s.T <= kShortSteps) {
             leak_short_forward_kernel<E><<<blocks, kLeakThreads, 2 * kLeakThreads * p.s.T * sizeof(E), st>>>((E *)y, state, starts, (const E *)x, gate, initial,
                                                                                                             p.s);
             return;
         }
-    leak_forward_kernel<E, G, K><<<blocks, kLeakThreads, 0, st>>>((E *)y, state, starts, (const E *)x, gate, initial, maps, p.s);
+    leak_forward_kernel<E, G, K, LINED><<<blocks, kLeakThreads, 0, st>>>((E *)y, state, starts, (const E *)x, gate, initial, maps, p.s);
 }
 
-template <typename E, int G, int K>
+template <typename E, int G, int K, bool LINED>
 static void run_backward(const LeakPlan &p, void *dx, void *dgate, float *dinitial, const void *g, const float *gstate, const float *starts, const void *x,
                          const void *gate, void *workspace, cudaStream_t st)
 {
@@ -687,18 +704,18 @@ static void run_backward(const LeakPlan &p, void *dx, void *dgate, float *diniti
     const bool per_row = p.s.gate_period > 0;
     const unsigned blocks = (unsigned)ceil_div((int64_t)p.s.rows * p.s.segments * G, kLeakThreads);
     if constexpr (G == 32)
-        if (p.s.segments > 1) leak_maps_kernel<E, K, false><<<blocks, kLeakThreads, 0, st>>>(maps, (const E *)g, gate, p.s);
+        if (p.s.segments > 1) leak_maps_kernel<E, K, LINED, false><<<blocks, kLeakThreads, 0, st>>>(maps, (const E *)g, gate, p.s);
     E *const to_gate = per_row ? nullptr : (E *)dgate;
     double *const to_sums = per_row && dgate ? sums : nullptr;
     bool done = false;
-    if constexpr (G == 1)
+    if constexpr (G == 1 && !LINED)
         if (p.s.T % kVector != 0 && p.s.T <= kShortSteps) {
             leak_short_backward_kernel<E><<<blocks, kLeakThreads, kLeakThreads * p.s.T * (3 * sizeof(E) + sizeof(float)), st>>>(
                 (E *)dx, to_gate, to_sums, dinitial, (const E *)g, gstate, starts, (const E *)x, gate, p.s);
             done = true;
         }
     if (!done)
-        leak_backward_kernel<E, G, K><<<blocks, kLeakThreads, 0, st>>>((E *)dx, to_gate, to_sums, dinitial, (const E *)g, gstate, starts, (const E *)x, gate, maps,
+        leak_backward_kernel<E, G, K, LINED><<<blocks, kLeakThreads, 0, st>>>((E *)dx, to_gate, to_sums, dinitial, (const E *)g, gstate, starts, (const E *)x, gate, maps,
                                                                        p.s);
     if (per_row && dgate) {
         const int64_t inner = (int64_t)p.s.gate_inner * p.s.segments, outer = p.s.rows / ((int64_t)p.s.gate_inner * p.s.gate_period);
@@ -767,7 +784,11 @@ extern "C" int slayer_b200_leak_forward(void *y, float *state, float *starts, co
                       aligned_to(initial, 4) && aligned_to(lengths, 8),
                   "leak_forward: a pointer off its alignment");
     const cudaStream_t st = (cudaStream_t)stream;
-#define SB200_LEAK_CALL(E, G, K) run_forward<E, G, K>(p, y, state, starts, x, gate, initial, workspace, st)
+#define SB200_LEAK_CALL(E, G, K)                                                                               \
+    do {                                                                                                       \
+        if (p.lined) run_forward<E, G, K, true>(p, y, state, starts, x, gate, initial, workspace, st);         \
+        else run_forward<E, G, K, false>(p, y, state, starts, x, gate, initial, workspace, st);                \
+    } while (0)
     SB200_LEAK_TYPES(SB200_LEAK_CALL)
 #undef SB200_LEAK_CALL
     return check_launch("leak_forward kernel launch");
@@ -790,7 +811,11 @@ extern "C" int slayer_b200_leak_backward(void *dx, void *dgate, float *dinitial,
                       aligned_to(dinitial, 4) && aligned_to(gstate, 4) && aligned_to(starts, 4) && aligned_to(lengths, 8),
                   "leak_backward: a pointer off its alignment");
     const cudaStream_t st = (cudaStream_t)stream;
-#define SB200_LEAK_CALL(E, G, K) run_backward<E, G, K>(p, dx, dgate, dinitial, g, gstate, starts, x, gate, workspace, st)
+#define SB200_LEAK_CALL(E, G, K)                                                                                \
+    do {                                                                                                        \
+        if (p.lined) run_backward<E, G, K, true>(p, dx, dgate, dinitial, g, gstate, starts, x, gate, workspace, st); \
+        else run_backward<E, G, K, false>(p, dx, dgate, dinitial, g, gstate, starts, x, gate, workspace, st);   \
+    } while (0)
     SB200_LEAK_TYPES(SB200_LEAK_CALL)
 #undef SB200_LEAK_CALL
     return check_launch("leak_backward kernel launch");

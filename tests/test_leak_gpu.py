@@ -237,6 +237,30 @@ def test_gates_at_their_ends():
     assert torch.equal(y.cpu(), (-0.5) ** torch.arange(10.0)[None])
 
 
+@pytest.mark.parametrize("T", [1, 3, 13, 14, 15, 16, 17, 33, 101, 510, 511, 513, 1027, 8195])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("short", [False, True])
+def test_rows_keep_to_themselves(T, dtype, short):
+    """Rows share vectors where T is no multiple of four: what every second row and the memory around the tensors hold changes nothing elsewhere."""
+    def run(other):
+        rng = torch.Generator("cuda").manual_seed(T)
+        leaves, R = [], 9
+        for _ in range(3):
+            # the tensor's first element lies on 16 bytes, its last one is followed at once by others' memory
+            memory = torch.full((R * T + 64,), other, dtype=dtype, device="cuda")
+            v = memory[16:16 + R * T].view(R, T)
+            v.copy_(torch.randn(R, T, generator=rng, device="cuda"))
+            v[1::2] = other
+            leaves.append(v)
+        lengths = torch.tensor([T, T, T - 1, T, 0, T, T // 2, T, T], device="cuda") if short else None
+        x, gate = leaves[0].requires_grad_(), leaves[1].requires_grad_()
+        y, last = gatedLeak(x, gate, lengths=lengths, returnState=True)
+        return [v[::2] for v in (y, last, *torch.autograd.grad(y, [x, gate], leaves[2]))]
+    clean, dirty = run(0.5), run(float("nan"))
+    for a, b in zip(clean, dirty):
+        assert bool(a.isfinite().all()) and torch.equal(a, b)
+
+
 def test_a_slow_leak_over_many_steps():
     """A time constant of 20000 steps over 100000: what rounding f to 32 bits would take from it is 1e-3."""
     T = 100000
