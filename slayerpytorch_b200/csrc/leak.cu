@@ -456,8 +456,8 @@ leak_backward_kernel(E *dx, E *dgate, double *sums, float *dinitial, const E *g,
 // One step of a state in double: by what is forgotten of it, or by what is kept, whichever is less.
 __device__ __forceinline__ double step_state(const Decay &d, double h, double u) { return u + (d.f < 0.5f ? (double)d.f * h : fma(-(double)d.rest, h, h)); }
 
-// Rows of up to 13 steps that do not end on vectors, which a lane has alone.  Their vectors would all be picked apart, an element at a time (8000000 x 5
-// float32: 162 us forward and 309 backward; so it is 113 and 207).  A CTA's rows are one piece of memory that begins at 16 bytes: it is copied to
+// Rows of up to 13 steps that do not end on vectors, which a lane has alone.  Hardly a vector would be one row's alone, and results would go an element at
+// a time (float32: 8000000 x 5 149 us forward and 262 backward, 3000000 x 13 117 and 215; so it is 113 and 207, 80 and 172).  A CTA's rows are one piece of memory that begins at 16 bytes: it is copied to
 // shared memory as it is, a thread walks a row there, its state in double, and results go back the same way.
 constexpr int kShortSteps = 13;
 
