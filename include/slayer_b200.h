@@ -428,8 +428,8 @@ int slayer_b200_leak_step(void *y, float *state, const void *x, const void *gate
 int slayer_b200_compress8(int8_t *q, uint8_t *scale, const void *x, int dtype, int64_t rows, int64_t T, void *stream);
 
 /*
- * What that stands for: out [rows, T] = q 2^e, NaN where q is -128; aligned to 16 bytes.  It has no counterpart
- * in the reference.
+ * What that stands for: out [rows, T] = q 2^e, NaN where q is -128; aligned to 16 bytes.  In float16 65536, which values of
+ * that type above 65024 are kept as, is its largest number, 65504.  It has no counterpart in the reference.
  */
 int slayer_b200_restore8(void *out, const int8_t *q, const uint8_t *scale, int dtype, int64_t rows, int64_t T, void *stream);
 

@@ -22,7 +22,8 @@ class Checkpoint:
         self.q, self.scale, self.shape, self.dtype = q, scale, torch.Size(shape), dtype
 
     def restore(self, dtype=None):
-        """What the 8 bits stand for, in the type that was compressed, or another (rounded to it)."""
+        """What the 8 bits stand for, in the type that was compressed, or another (rounded to it).  In float16 65536 is 65504, the type's largest
+        number: what is finite there comes back finite."""
         dtype = self.dtype if dtype is None else dtype
         return slayerCuda.restore8(self.q, self.scale, self.shape, torch.empty((), dtype=dtype))
 

@@ -23,7 +23,8 @@ template <> __device__ __forceinline__ float as_float<__half>(__half v) { return
 template <typename E> __device__ __forceinline__ E as_type(float v);
 template <> __device__ __forceinline__ float as_type<float>(float v) { return v; }
 template <> __device__ __forceinline__ __nv_bfloat16 as_type<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-template <> __device__ __forceinline__ __half as_type<__half>(float v) { return __float2half_rn(v); }
+// A float16 above 65024 is kept as 64 * 2^10, half a step beyond the largest one, which it comes back as.
+template <> __device__ __forceinline__ __half as_type<__half>(float v) { return __float2half_rn(fabsf(v) == 65536.0f ? copysignf(65504.0f, v) : v); }
 
 // Byte of the scale for a largest magnitude given by its bits.  With amax = m 2^k, 1 <= m < 2: amax <= 127 2^(k-6) where m <= 127/64, else
 // 127 2^(k-5): one more where the mantissa is above 0x7e0000.  From 2^-126 on, and up to 2^121, so that 127 2^e is finite (multiples
