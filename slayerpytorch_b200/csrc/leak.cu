@@ -337,6 +337,19 @@ __device__ __forceinline__ Decay row_gate(const LeakShape &s, const void *gate, 
     return g < 0.0f ? Decay{small, 1.0f - small} : Decay{1.0f - small, small};
 }
 
+// Maps one after the other, in double, as states are from chunk to chunk: a segment may have thousands of them, whose sums in float were 130 steps of
+// 2^-24 off after 512.
+struct Chain {
+    double a = 1.0, r = 0.0, b = 0.0;
+    __device__ __forceinline__ void add(const Map &m)
+    {
+        const bool little = m.r < 0.5f;
+        r = fma(a, (double)m.r, r);
+        a = r < 0.5 ? 1.0 - r : a * (double)m.a;
+        b = (little ? b : 0.0) + fma((double)(little ? -m.r : m.a), b, (double)m.b);
+    }
+};
+
 // Maps of segments: rows too few to fill the GPU are split, and each segment starts from what those before it leave.
 template <typename E, int K, bool LINED, bool FORWARD>
 __global__ void __launch_bounds__(kLeakThreads)
@@ -346,7 +359,7 @@ leak_maps_kernel(Map *maps, const E *x, const void *gate, const LeakShape s)
     if (!place<32>(s, row, segment, lane)) return;
     const Row r = row_of(s, row);
     const Decay row_d = row_gate(s, gate, row);
-    Map all = {1.0f, 0.0f, 0.0f};
+    Chain all;
     const int first = segment * s.segment_chunks, last = min(first + s.segment_chunks, s.chunks);
     for (int i = first; i < last; ++i) {
         const int c = FORWARD ? i : last - 1 - (i - first);
@@ -354,12 +367,12 @@ leak_maps_kernel(Map *maps, const E *x, const void *gate, const LeakShape s)
         st.load(s, r, x, (const E *)gate, row_d, Inside<K, LINED>((c * 32 + lane) * (4 * K) - r.skew, r.length, r.reach));
         if (FORWARD) {
             st.couple(s.coupled);
-            all = compose(all, shift_from(scan<32, true>(forward_map<E, K>(st), lane), 31));
+            all.add(shift_from(scan<32, true>(forward_map<E, K>(st), lane), 31));
         } else {
-            all = compose(all, shift_from(scan<32, false>(backward_map<4 * K>(st.d, st.x), lane), 0));
+            all.add(shift_from(scan<32, false>(backward_map<4 * K>(st.d, st.x), lane), 0));
         }
     }
-    if (lane == 0) maps[row * s.segments + segment] = all;
+    if (lane == 0) maps[row * s.segments + segment] = {(float)all.a, (float)all.r, (float)all.b};
 }
 
 template <typename E, int G, int K, bool LINED>
