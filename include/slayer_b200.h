@@ -388,7 +388,7 @@ int64_t slayer_b200_muon_step_workspace(const slayer_b200_muon_matrix *list, int
  * row r has the entry (r / gate_inner) % gate_period at every step (rows: whole groups of gate_inner *
  * gate_period).  lengths (NULL: all T): steps that count, one entry for every sample_rows rows, taken
  * into [0, T]; the steps behind them are not used, y is 0 there and the state stays.  state (NULL: not
- * wanted): the state after the last step.  starts (NULL: no backward pass): rows x
+ * wanted): the state after the last step; it may be initial, for a stream's next part.  starts (NULL: no backward pass): rows x
  * slayer_b200_leak_states(T) float32, states that the backward pass starts from (one for 12 or 16 steps of longer rows).  States are
  * float32 outside of a call and double within.  y may not be x or gate; they (a gate of x's type) are aligned
  * to 16 bytes.  workspace:
@@ -403,8 +403,8 @@ int64_t slayer_b200_leak_workspace(int64_t rows, int64_t T, int dtype, int64_t g
 
 /*
  * The gradients of the above for g [rows, T] (of y) and gstate [rows] (of the last state; NULL: 0): dx as x,
- * dgate as gate (of a gate per row: summed over its rows in a fixed order), dinitial [rows]; aligned as above.  Each of the
- * three may be NULL.  starts: from the forward pass on the same x, gate, initial and lengths.  It has
+ * dgate as gate (of a gate per row: summed over its rows in a fixed order), dinitial [rows], which may be gstate; aligned as above.
+ * Each of the three may be NULL.  starts: from the forward pass on the same x, gate, initial and lengths.  It has
  * no counterpart in the reference.
  */
 int slayer_b200_leak_backward(void *dx, void *dgate, float *dinitial, const void *g, const float *gstate, const float *starts, const void *x,

@@ -350,10 +350,11 @@ struct Chain {
     }
 };
 
-// Maps of segments: rows too few to fill the GPU are split, and each segment starts from what those before it leave.
+// Maps of segments: rows too few to fill the GPU are split, and each segment starts from what those before it leave.  ends: what a row's first segment
+// (FORWARD), or its last, starts from, in a copy, which the next launch reads: the result that its other end writes may take its place.
 template <typename E, int K, bool LINED, bool FORWARD>
 __global__ void __launch_bounds__(kLeakThreads)
-leak_maps_kernel(Map *maps, const E *x, const void *gate, const LeakShape s)
+leak_maps_kernel(Map *maps, float *ends, const E *x, const void *gate, const float *end, const LeakShape s)
 {
     int row, segment, lane;
     if (!place<32>(s, row, segment, lane)) return;
@@ -373,6 +374,7 @@ leak_maps_kernel(Map *maps, const E *x, const void *gate, const LeakShape s)
         }
     }
     if (lane == 0) maps[row * s.segments + segment] = {(float)all.a, (float)all.r, (float)all.b};
+    if (end && lane == 0 && segment == 0) ends[row] = end[row];
 }
 
 template <typename E, int G, int K, bool LINED>
@@ -659,7 +661,7 @@ struct LeakPlan {
     LeakShape s;
     LeakLanes l;
     bool lined;                          // rows end with their vectors, and all of their steps count
-    int64_t maps_bytes, sums_bytes, gate_parts;
+    int64_t ends_at, maps_bytes, sums_bytes, gate_parts;         // (maps_bytes: with ends)
 };
 
 static int plan_leak(LeakPlan &p, const char *op, int dtype, int flags, int64_t rows, int64_t T, const int64_t *lengths, int64_t sample_rows,
@@ -678,7 +680,8 @@ static int plan_leak(LeakPlan &p, const char *op, int dtype, int flags, int64_t 
     const int64_t chunks = chunks_of(T), segments = rows ? segments_of(rows, T) : 1;
     p.s = {(int)rows, (int)T, (int)gate_inner, (int)gate_period, (int)(sample_rows < rows ? sample_rows : rows), lengths, (int)chunks, (int)segments,
            (int)ceil_div(chunks, segments), (flags & SLAYER_B200_LEAK_LOGIT) != 0, (flags & SLAYER_B200_LEAK_COUPLED) != 0};
-    p.maps_bytes = segments > 1 ? ceil_div(rows * segments * (int64_t)sizeof(Map), 16) * 16 : 0;
+    p.ends_at = ceil_div(rows * segments * (int64_t)sizeof(Map), 16) * 16;
+    p.maps_bytes = segments > 1 ? p.ends_at + ceil_div(rows * (int64_t)sizeof(float), 16) * 16 : 0;
     p.sums_bytes = p.gate_parts = 0;
     if (gate_period && rows) {
         const int64_t count = rows / gate_period * segments;
@@ -698,7 +701,11 @@ static void run_forward(const LeakPlan &p, void *y, float *state, float *starts,
     Map *maps = (Map *)workspace;
     const unsigned blocks = (unsigned)ceil_div((int64_t)p.s.rows * p.s.segments * G, kLeakThreads);
     if constexpr (G == 32)
-        if (p.s.segments > 1) leak_maps_kernel<E, K, LINED, true><<<blocks, kLeakThreads, 0, st>>>(maps, (const E *)x, gate, p.s);
+        if (p.s.segments > 1) {
+            float *const ends = (float *)((char *)workspace + p.ends_at);
+            leak_maps_kernel<E, K, LINED, true><<<blocks, kLeakThreads, 0, st>>>(maps, ends, (const E *)x, gate, initial, p.s);
+            if (initial) initial = ends;
+        }
     if constexpr (G == 1 && !LINED)
         if (p.s.T % kVector != 0 && p.s.T <= kShortSteps) {
             leak_short_forward_kernel<E><<<blocks, kLeakThreads, 2 * kLeakThreads * p.s.T * sizeof(E), st>>>((E *)y, state, starts, (const E *)x, gate, initial,
@@ -717,7 +724,11 @@ static void run_backward(const LeakPlan &p, void *dx, void *dgate, float *diniti
     const bool per_row = p.s.gate_period > 0;
     const unsigned blocks = (unsigned)ceil_div((int64_t)p.s.rows * p.s.segments * G, kLeakThreads);
     if constexpr (G == 32)
-        if (p.s.segments > 1) leak_maps_kernel<E, K, LINED, false><<<blocks, kLeakThreads, 0, st>>>(maps, (const E *)g, gate, p.s);
+        if (p.s.segments > 1) {
+            float *const ends = (float *)((char *)workspace + p.ends_at);
+            leak_maps_kernel<E, K, LINED, false><<<blocks, kLeakThreads, 0, st>>>(maps, ends, (const E *)g, gate, gstate, p.s);
+            if (gstate) gstate = ends;
+        }
     E *const to_gate = per_row ? nullptr : (E *)dgate;
     double *const to_sums = per_row && dgate ? sums : nullptr;
     bool done = false;

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from slayerpytorch_b200 import capi
 from slayerpytorch_b200.recurrence import gatedLeak
 from test_leak_gpu import STEP
 
@@ -45,3 +46,41 @@ def test_no_loss_from_chunk_to_chunk():
     assert float(off) <= 60 * STEP, float(off) / STEP
     # a product of the two for each step, added up in double
     assert abs(float(dgate) / (v * v * T * (T * T - 1) / 6) - 1) <= 130 * STEP
+
+
+def pointer(v):
+    return None if v is None else v.data_ptr()
+
+
+def passes(x, gate, g, initial, state, gstate, dinitial, lengths=None):
+    """Both passes through the C entries, rows with a gate per step: (y, state, dx, dgate, dinitial)"""
+    lib, (R, T) = capi.load(), x.shape
+    stream = torch.cuda.current_stream().cuda_stream
+    y, dx, dgate = torch.empty_like(x), torch.empty_like(x), torch.empty_like(x)
+    starts = torch.empty(R, lib.slayer_b200_leak_states(T), device="cuda")
+    size = lib.slayer_b200_leak_workspace(R, T, 0, 0, 0)
+    assert size >= 0
+    room = torch.empty(max(size, 16), dtype=torch.uint8, device="cuda")
+    args = (0, 1, R, T, pointer(lengths), 1, 0, 0, room.data_ptr(), stream)
+    rc = lib.slayer_b200_leak_forward(pointer(y), pointer(state), pointer(starts), pointer(x), pointer(gate), pointer(initial), *args)
+    assert rc == 0, lib.slayer_b200_last_error()
+    kept = state.clone()
+    rc = lib.slayer_b200_leak_backward(pointer(dx), pointer(dgate), pointer(dinitial), pointer(g), pointer(gstate), pointer(starts), pointer(x), pointer(gate), *args)
+    assert rc == 0, lib.slayer_b200_last_error()
+    return y, kept, dx, dgate, dinitial.clone()
+
+
+@pytest.mark.parametrize("R,T", [(3, 20000), (1, 1000001), (40, 5003), (7, 700), (5000, 600), (300, 100), (1000, 5), (64, 40)])
+def test_states_in_place(R, T):
+    """A state that is the initial one's memory, and the gradient of the latter in the former's, whether rows are split or not."""
+    gen = torch.Generator(device="cuda").manual_seed(R)
+    x, gate, g = (torch.randn(R, T, device="cuda", generator=gen) for _ in range(3))
+    h, up = (100 * torch.randn(R, device="cuda", generator=gen) for _ in range(2))
+    gate += 6.0         # what is there at the start matters for hundreds of steps
+    for lengths in (None, torch.randint(0, T + 1, (R,), device="cuda", generator=gen)):
+        apart = passes(x, gate, g, h, torch.empty_like(h), up, torch.empty_like(h), lengths)
+        y, state = gatedLeak(x, gate, initial=h, lengths=lengths, returnState=True)
+        assert torch.equal(apart[0], y) and torch.equal(apart[1], state)
+        for _ in range(5):
+            own, back = h.clone(), up.clone()
+            assert all(torch.equal(a, b) for a, b in zip(apart, passes(x, gate, g, own, own, back, back, lengths)))
