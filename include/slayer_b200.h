@@ -390,8 +390,8 @@ int64_t slayer_b200_muon_step_workspace(const slayer_b200_muon_matrix *list, int
  * into [0, T]; the steps behind them are not used, y is 0 there and the state stays.  state (NULL: not
  * wanted): the state after the last step; it may be initial, for a stream's next part.  starts (NULL: no backward pass): rows x
  * slayer_b200_leak_states(T) float32, states that the backward pass starts from (one for 12 or 16 steps of longer rows).  States are
- * float32 outside of a call and double within.  y may not be x or gate; they (a gate of x's type) are aligned
- * to 16 bytes.  workspace:
+ * float32 outside of a call and double within.  Nothing else that is written (y, state, starts, workspace) may share memory with the rest.
+ * x, y and a gate of x's type are aligned to 16 bytes.  workspace:
  * slayer_b200_leak_workspace(...) bytes of device memory, aligned to 16, for either pass.  It has
  * no counterpart in the reference, whose psp has one fixed kernel (src/slayer.py:875-899).
  */
@@ -404,7 +404,7 @@ int64_t slayer_b200_leak_workspace(int64_t rows, int64_t T, int dtype, int64_t g
 /*
  * The gradients of the above for g [rows, T] (of y) and gstate [rows] (of the last state; NULL: 0): dx as x,
  * dgate as gate (of a gate per row: summed over its rows in a fixed order), dinitial [rows], which may be gstate; aligned as above.
- * Each of the three may be NULL.  starts: from the forward pass on the same x, gate, initial and lengths.  It has
+ * Each of the three may be NULL.  Nothing else that is written may share memory with the rest.  starts: from the forward pass on the same x, gate, initial and lengths.  It has
  * no counterpart in the reference.
  */
 int slayer_b200_leak_backward(void *dx, void *dgate, float *dinitial, const void *g, const float *gstate, const float *starts, const void *x,
@@ -414,7 +414,7 @@ int slayer_b200_leak_backward(void *dx, void *dgate, float *dinitial, const void
 /*
  * One time step of it on rows of a stream: state [rows], float32, is updated in place and y [rows] is the new state
  * in x's type.  gate: [rows] (gate_period 0), or an entry for each group of rows as above; float32 or x's type
- * (gate_dtype).  y may be x; state shares no memory with the others.  It has no counterpart in the reference.
+ * (gate_dtype).  y may be x, or a gate for each row of its type; state shares no memory with the others.  It has no counterpart in the reference.
  */
 int slayer_b200_leak_step(void *y, float *state, const void *x, const void *gate, int dtype, int gate_dtype, int flags, int64_t rows,
                           int64_t gate_inner, int64_t gate_period, void *stream);

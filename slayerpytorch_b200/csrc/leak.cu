@@ -772,6 +772,30 @@ static void run_backward(const LeakPlan &p, void *dx, void *dgate, float *diniti
 static bool element_aligned(const void *p, int dtype) { return ((uintptr_t)p & (dtype == SLAYER_B200_F32 ? 3 : 1)) == 0; }
 static bool aligned_to(const void *p, unsigned n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
+struct Memory {
+    const void *p;
+    int64_t bytes;
+};
+
+static bool apart(const Memory &a, const Memory &b)
+{
+    return !a.p || !b.p || (uintptr_t)a.p + (uintptr_t)a.bytes <= (uintptr_t)b.p || (uintptr_t)b.p + (uintptr_t)b.bytes <= (uintptr_t)a.p;
+}
+
+// What is written shares nothing with the rest: groups of lanes read what others would have written.  list: the first `written` of it are; `end` of those may
+// be `start` of the others.
+template <int N>
+static bool all_apart(const Memory (&list)[N], int written, int end, int start)
+{
+    for (int i = 0; i < written; ++i)
+        for (int j = i + 1; j < N; ++j)
+            if (!apart(list[i], list[j]) && !(i == end && j == start && list[i].p == list[j].p)) return false;
+    return true;
+}
+
+static int64_t gate_bytes(const LeakPlan &p, int64_t element) { return p.s.gate_period ? p.s.gate_period * (int64_t)sizeof(float) : (int64_t)p.s.rows * p.s.T * element; }
+static int64_t lengths_bytes(const LeakPlan &p) { return p.s.lengths ? ceil_div(p.s.rows, p.s.sample_rows) * (int64_t)sizeof(int64_t) : 0; }
+
 }  // namespace sb200
 
 extern "C" int64_t slayer_b200_leak_states(int64_t T)
@@ -807,6 +831,10 @@ extern "C" int slayer_b200_leak_forward(void *y, float *state, float *starts, co
     SB200_REQUIRE(aligned16(y) && aligned16(x) && aligned_to(gate, gate_period ? 4 : 16) && aligned_to(state, 4) && aligned_to(starts, 4) &&
                       aligned_to(initial, 4) && aligned_to(lengths, 8),
                   "leak_forward: a pointer off its alignment");
+    const int64_t element = dtype == SLAYER_B200_F32 ? 4 : 2, all = rows * T * element, per_row = rows * (int64_t)sizeof(float);
+    const Memory list[] = {{y, all}, {state, per_row}, {starts, per_row * p.s.chunks * p.l.lanes}, {workspace, p.maps_bytes},
+                           {x, all}, {gate, gate_bytes(p, element)}, {initial, per_row}, {lengths, lengths_bytes(p)}};
+    SB200_REQUIRE(all_apart(list, 4, 1, 6), "leak_forward: y, state, starts and the workspace share memory with one another or with what is read");
     const cudaStream_t st = (cudaStream_t)stream;
 #define SB200_LEAK_CALL(E, G, K)                                                                               \
     do {                                                                                                       \
@@ -834,6 +862,11 @@ extern "C" int slayer_b200_leak_backward(void *dx, void *dgate, float *dinitial,
     SB200_REQUIRE(aligned16(dx) && aligned_to(dgate, gate_period ? 4 : 16) && aligned16(g) && aligned16(x) && aligned_to(gate, gate_period ? 4 : 16) &&
                       aligned_to(dinitial, 4) && aligned_to(gstate, 4) && aligned_to(starts, 4) && aligned_to(lengths, 8),
                   "leak_backward: a pointer off its alignment");
+    const int64_t element = dtype == SLAYER_B200_F32 ? 4 : 2, all = rows * T * element, per_row = rows * (int64_t)sizeof(float);
+    const Memory list[] = {{dx, all}, {dgate, gate_bytes(p, element)}, {dinitial, per_row}, {workspace, p.maps_bytes + p.sums_bytes},
+                           {g, all}, {gstate, per_row}, {starts, per_row * p.s.chunks * p.l.lanes}, {x, all}, {gate, gate_bytes(p, element)},
+                           {lengths, lengths_bytes(p)}};
+    SB200_REQUIRE(all_apart(list, 4, 2, 5), "leak_backward: dx, dgate, dinitial and the workspace share memory with one another or with what is read");
     const cudaStream_t st = (cudaStream_t)stream;
 #define SB200_LEAK_CALL(E, G, K)                                                                                \
     do {                                                                                                        \
@@ -858,6 +891,12 @@ extern "C" int slayer_b200_leak_step(void *y, float *state, const void *x, const
     SB200_REQUIRE(y && state && x && gate, "leak_step: null pointer");
     SB200_REQUIRE(element_aligned(y, dtype) && element_aligned(x, dtype) && element_aligned(gate, gate_dtype) && aligned_to(state, 4),
                   "leak_step: a pointer off its element's alignment");
+    const int64_t element = dtype == SLAYER_B200_F32 ? 4 : 2, gates = (gate_period ? gate_period : rows) * (gate_dtype == SLAYER_B200_F32 ? 4 : 2);
+    const Memory out = {y, rows * element}, kept = {state, rows * 4}, in = {x, rows * element}, by = {gate, gates};
+    SB200_REQUIRE(apart(kept, out) && apart(kept, in) && apart(kept, by), "leak_step: state shares memory with y, x or gate");
+    // (a thread reads its own elements of the two before it writes its own of y)
+    SB200_REQUIRE((apart(out, in) || y == x) && (apart(out, by) || (y == gate && gate_period == 0 && gate_dtype == dtype)),
+                  "leak_step: y shares memory with other elements of x or gate");
     const unsigned blocks = (unsigned)ceil_div(rows, 256);
     const cudaStream_t st = (cudaStream_t)stream;
 #define SB200_LEAK_STEP(E, EG)                                                                                                                       \
