@@ -335,7 +335,8 @@ class _DenseLayer(torch.nn.Conv3d):
         if self.checkpoint:
             if x.dim() != 5 or x.shape[2:4] != self.weight.shape[2:4]:
                 raise ValueError('dense: a layer that keeps its input in 8 bits takes inputs of its own size, got {}'.format(tuple(x.shape)))
-            return _DenseFunction8.apply(x, self.weight)
+            if torch.is_grad_enabled():     # (a Function is told that weights need gradients without that too)
+                return _DenseFunction8.apply(x, self.weight)
         return F.conv3d(x, self.weight, self.bias, self.stride, self.padding, self.dilation, self.groups)
 
 
@@ -431,7 +432,7 @@ class spikeLayer(torch.nn.Module):
 
     def spike(self, membranePotential, checkpoint=False):
         """``checkpoint``: the membrane potential is kept in 8 bits for the backward pass (not part of the reference's interface)."""
-        function = _SpikeFunction8 if checkpoint else _SpikeFunction
+        function = _SpikeFunction8 if checkpoint and torch.is_grad_enabled() else _SpikeFunction
         return function.apply(membranePotential, self.refKernel, self.neuron, self.simulation['Ts'])
 
     def delayShift(self, input, delay, Ts=1):

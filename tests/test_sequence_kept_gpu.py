@@ -2,9 +2,11 @@
 import pytest
 import torch
 
-from slayerpytorch_b200 import checkpoint
+from slayerpytorch_b200 import checkpoint, layer
 
 pytestmark = pytest.mark.gpu
+
+NEURON = {"type": "SRMALPHA", "theta": 10, "tauSr": 10.0, "tauRef": 1.0, "scaleRef": 2, "tauRho": 1, "scaleRho": 1}
 
 
 @pytest.mark.parametrize("T", [32, 33, 64, 100])
@@ -24,3 +26,25 @@ def test_the_largest_float16_values_come_back_finite(T):
     # a float32 tensor in float16: rounded to it, infinities where it is beyond
     far = checkpoint.compress(torch.full((1, T), 3e5, device="cuda"))
     assert bool(far.restore(torch.float16).isposinf().all()) and bool(far.restore().isfinite().all())
+
+
+def test_layers_keep_nothing_without_gradients(monkeypatch):
+    """In evaluation a layer that keeps 8 bits does what the plain one does."""
+    net = layer.spikeLayer(NEURON, {"Ts": 1.0, "tSample": 90}).cuda()
+    dense, plain = net.dense(20, 11, checkpoint=True).cuda(), net.dense(20, 11).cuda()
+    plain.load_state_dict(dense.state_dict())
+    x = torch.rand(3, 20, 1, 1, 90, device="cuda")
+    u = 8.0 * torch.randn(3, 11, 1, 1, 90, device="cuda")
+    spikes = net.spike(u.clone())
+
+    def refuse(x):
+        raise AssertionError("compressed without need")
+    monkeypatch.setattr(layer.slayerCuda, "compress8", refuse)
+    leaf = u.clone().requires_grad_()
+    for off in (torch.no_grad, torch.inference_mode):
+        with off():
+            assert torch.equal(dense(x), plain(x))
+    with torch.no_grad():
+        assert torch.equal(net.spike(leaf, checkpoint=True), spikes)
+    with pytest.raises(AssertionError, match="without need"):
+        dense(x)
