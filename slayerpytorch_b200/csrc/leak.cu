@@ -187,28 +187,37 @@ __device__ __forceinline__ Decay decay_of(float gate, bool logit)
     return gate < 0.0f ? Decay{small, large} : Decay{1.0f - small, small};
 }
 
+// The decay of a whole row.  f = 1 - rest is rounded to 24 bits: taken so at each step, the same part of a rounding would add up over the 16 that a lane
+// walks (results 3 to 4 steps of 2^-24 off on average, where it is half of one).  So some steps take the next float above f, and four of
+// them forget what they should to an eighth of a rounding each.  A lane of two vectors at most has one f for each, which saves registers
+// (8 steps: 62 us backward instead of 69, 3200000 x 8).  With a gate per step the roundings differ from step to step.
+struct RowDecay {
+    float f[4], rest;
+    template <int K> __device__ __forceinline__ Decay at(int j) const { return {f[K < 3 ? j / 4 : j % 4], rest}; }
+};
+
 // What a lane knows of its steps.  Those outside of the row, or behind its length, keep the state: f = 1, u = 0.
 template <typename E, int K>
 struct Steps {
     Decay d[4 * K];
     float x[4 * K];
 
-    template <bool LINED>
-    __device__ __forceinline__ void load(const LeakShape &s, const Row &row, const E *x_, const E *gate, const Decay &row_d, const Inside<K, LINED> &in)
+    template <bool ROW, bool LINED>
+    __device__ __forceinline__ void load(const LeakShape &s, const Row &row, const E *x_, const E *gate, const RowDecay &row_d, const Inside<K, LINED> &in)
     {
         load_steps<E, K, LINED>(x, x_ + row.base, in, 0.0f);
-        if (s.gate_period == 0) {
+        if (!ROW) {
             float g[4 * K];
             load_steps<E, K, LINED>(g, gate + row.base, in, s.logit ? INFINITY : 1.0f);
 #pragma unroll
             for (int j = 0; j < 4 * K; ++j) d[j] = decay_of(g[j], s.logit);
         } else {
 #pragma unroll
-            for (int j = 0; j < 4 * K; ++j) d[j] = in.whole[j / 4] ? row_d : Decay{1.0f, 0.0f};
+            for (int j = 0; j < 4 * K; ++j) d[j] = in.whole[j / 4] ? row_d.template at<K>(j) : Decay{1.0f, 0.0f};
             if (in.part) {
 #pragma unroll
                 for (int j = 0; j < 4 * K; ++j)
-                    if (in.t + j >= 0 && in.t + j < in.end) d[j] = row_d;
+                    if (in.t + j >= 0 && in.t + j < in.end) d[j] = row_d.template at<K>(j);
             }
         }
     }
@@ -337,6 +346,22 @@ __device__ __forceinline__ Decay row_gate(const LeakShape &s, const void *gate, 
     return g < 0.0f ? Decay{small, 1.0f - small} : Decay{1.0f - small, small};
 }
 
+// ROW: kernels of their own for a gate per row (with both kinds in one, its four decays cost a gate per step registers and 4 to 6 %).
+template <bool ROW>
+__device__ __forceinline__ RowDecay row_gates(const LeakShape &s, const void *gate, int row)
+{
+    if (!ROW) return {{1.0f, 1.0f, 1.0f, 1.0f}, 0.0f};
+    Decay d = row_gate(s, gate, row);
+    int up = 0;
+    if (s.logit && d.f >= 0.5f) {
+        // the float below 1 - rest, and quarters of the way to the next one, 2^-24, that are left (both differences are exact)
+        d.f = __fsub_rd(1.0f, d.rest);
+        up = __float2int_rn(((1.0f - d.f) - d.rest) * 67108864.0f);
+    }
+    const float above = __int_as_float(__float_as_int(d.f) + 1);
+    return {{up >= 3 ? above : d.f, up >= 1 ? above : d.f, up >= 4 ? above : d.f, up >= 2 ? above : d.f}, d.rest};
+}
+
 // Maps one after the other, in double, as states are from chunk to chunk: a segment may have thousands of them, whose sums in float were 130 steps of
 // 2^-24 off after 512.
 struct Chain {
@@ -352,20 +377,20 @@ struct Chain {
 
 // Maps of segments: rows too few to fill the GPU are split, and each segment starts from what those before it leave.  ends: what a row's first segment
 // (FORWARD), or its last, starts from, in a copy, which the next launch reads: the result that its other end writes may take its place.
-template <typename E, int K, bool LINED, bool FORWARD>
+template <typename E, int K, bool LINED, bool FORWARD, bool ROW>
 __global__ void __launch_bounds__(kLeakThreads)
 leak_maps_kernel(Map *maps, float *ends, const E *x, const void *gate, const float *end, const LeakShape s)
 {
     int row, segment, lane;
     if (!place<32>(s, row, segment, lane)) return;
     const Row r = row_of(s, row);
-    const Decay row_d = row_gate(s, gate, row);
+    const RowDecay row_d = row_gates<ROW>(s, gate, row);
     Chain all;
     const int first = segment * s.segment_chunks, last = min(first + s.segment_chunks, s.chunks);
     for (int i = first; i < last; ++i) {
         const int c = FORWARD ? i : last - 1 - (i - first);
         Steps<E, K> st;
-        st.load(s, r, x, (const E *)gate, row_d, Inside<K, LINED>((c * 32 + lane) * (4 * K) - r.skew, r.length, r.reach));
+        st.template load<ROW>(s, r, x, (const E *)gate, row_d, Inside<K, LINED>((c * 32 + lane) * (4 * K) - r.skew, r.length, r.reach));
         if (FORWARD) {
             st.couple(s.coupled);
             all.add(shift_from(scan<32, true>(forward_map<E, K>(st), lane), 31));
@@ -377,7 +402,7 @@ leak_maps_kernel(Map *maps, float *ends, const E *x, const void *gate, const flo
     if (end && lane == 0 && segment == 0) ends[row] = end[row];
 }
 
-template <typename E, int G, int K, bool LINED>
+template <typename E, int G, int K, bool LINED, bool ROW>
 __global__ void __launch_bounds__(kLeakThreads, kForwardBlocks<K, LINED>)
 leak_forward_kernel(E *y, float *state, float *starts, const E *x, const void *gate, const float *initial, const Map *maps, const LeakShape s)
 {
@@ -386,14 +411,14 @@ leak_forward_kernel(E *y, float *state, float *starts, const E *x, const void *g
     if (G == 32 && !there) return;
     if (!there) row = s.rows - 1, segment = 0;      // the shuffles want every lane
     const Row r = row_of(s, row);
-    const Decay row_d = row_gate(s, gate, row);
+    const RowDecay row_d = row_gates<ROW>(s, gate, row);
     double h = initial ? (double)initial[row] : 0.0;
     if (G == 32 && segment > 0) h = through_segments<true>(maps + row * s.segments, 0, segment, lane, h);
     const int first = segment * s.segment_chunks, last = min(first + s.segment_chunks, s.chunks);
     for (int c = first; c < last; ++c) {
         const Inside<K, LINED> in((c * G + lane) * (4 * K) - r.skew, r.length, r.reach);
         Steps<E, K> st;
-        st.load(s, r, x, (const E *)gate, row_d, in);
+        st.template load<ROW>(s, r, x, (const E *)gate, row_d, in);
         st.couple(s.coupled);
         const Map m = scan<G, true>(forward_map<E, K>(st), lane);
         float at = (float)others<G, true>(m, lane)(h);
@@ -410,7 +435,7 @@ leak_forward_kernel(E *y, float *state, float *starts, const E *x, const void *g
 }
 
 // sums: per row and segment, of df: the gradient of a gate per row
-template <typename E, int G, int K, bool LINED>
+template <typename E, int G, int K, bool LINED, bool ROW>
 __global__ void __launch_bounds__(kLeakThreads, kBackwardBlocks<K>)
 leak_backward_kernel(E *dx, E *dgate, double *sums, float *dinitial, const E *g, const float *gstate, const float *starts, const E *x, const void *gate,
                      const Map *maps, const LeakShape s)
@@ -421,7 +446,7 @@ leak_backward_kernel(E *dx, E *dgate, double *sums, float *dinitial, const E *g,
     if (G == 32 && !there) return;
     if (!there) row = s.rows - 1, segment = 0;
     const Row r = row_of(s, row);
-    const Decay row_d = row_gate(s, gate, row);
+    const RowDecay row_d = row_gates<ROW>(s, gate, row);
     double carry = gstate ? (double)gstate[row] : 0.0, sum = 0.0;
     if (G == 32 && segment + 1 < s.segments) carry = through_segments<false>(maps + row * s.segments, segment + 1, s.segments, lane, carry);
     const int first = segment * s.segment_chunks, last = min(first + s.segment_chunks, s.chunks);
@@ -430,7 +455,7 @@ leak_backward_kernel(E *dx, E *dgate, double *sums, float *dinitial, const E *g,
         float gv[N], slope[N];       // slope: what lambda is multiplied by in dgate
         Steps<E, K> st;
         load_steps<E, K, LINED>(gv, g + r.base, in, 0.0f);
-        st.load(s, r, x, (const E *)gate, row_d, in);
+        st.template load<ROW>(s, r, x, (const E *)gate, row_d, in);
         float at = starts[((int64_t)row * s.chunks + c) * G + lane];
 #pragma unroll
         for (int j = 0; j < N; ++j) slope[j] = s.coupled ? st.x[j] : 0.0f;
@@ -694,7 +719,7 @@ static int plan_leak(LeakPlan &p, const char *op, int dtype, int flags, int64_t 
     return SLAYER_B200_OK;
 }
 
-template <typename E, int G, int K, bool LINED>
+template <typename E, int G, int K, bool LINED, bool ROW>
 static void run_forward(const LeakPlan &p, void *y, float *state, float *starts, const void *x, const void *gate, const float *initial, void *workspace,
                         cudaStream_t st)
 {
@@ -703,7 +728,7 @@ static void run_forward(const LeakPlan &p, void *y, float *state, float *starts,
     if constexpr (G == 32)
         if (p.s.segments > 1) {
             float *const ends = (float *)((char *)workspace + p.ends_at);
-            leak_maps_kernel<E, K, LINED, true><<<blocks, kLeakThreads, 0, st>>>(maps, ends, (const E *)x, gate, initial, p.s);
+            leak_maps_kernel<E, K, LINED, true, ROW><<<blocks, kLeakThreads, 0, st>>>(maps, ends, (const E *)x, gate, initial, p.s);
             if (initial) initial = ends;
         }
     if constexpr (G == 1 && !LINED)
@@ -712,10 +737,10 @@ static void run_forward(const LeakPlan &p, void *y, float *state, float *starts,
                                                                                                             p.s);
             return;
         }
-    leak_forward_kernel<E, G, K, LINED><<<blocks, kLeakThreads, 0, st>>>((E *)y, state, starts, (const E *)x, gate, initial, maps, p.s);
+    leak_forward_kernel<E, G, K, LINED, ROW><<<blocks, kLeakThreads, 0, st>>>((E *)y, state, starts, (const E *)x, gate, initial, maps, p.s);
 }
 
-template <typename E, int G, int K, bool LINED>
+template <typename E, int G, int K, bool LINED, bool ROW>
 static void run_backward(const LeakPlan &p, void *dx, void *dgate, float *dinitial, const void *g, const float *gstate, const float *starts, const void *x,
                          const void *gate, void *workspace, cudaStream_t st)
 {
@@ -726,7 +751,7 @@ static void run_backward(const LeakPlan &p, void *dx, void *dgate, float *diniti
     if constexpr (G == 32)
         if (p.s.segments > 1) {
             float *const ends = (float *)((char *)workspace + p.ends_at);
-            leak_maps_kernel<E, K, LINED, false><<<blocks, kLeakThreads, 0, st>>>(maps, ends, (const E *)g, gate, gstate, p.s);
+            leak_maps_kernel<E, K, LINED, false, ROW><<<blocks, kLeakThreads, 0, st>>>(maps, ends, (const E *)g, gate, gstate, p.s);
             if (gstate) gstate = ends;
         }
     E *const to_gate = per_row ? nullptr : (E *)dgate;
@@ -739,8 +764,8 @@ static void run_backward(const LeakPlan &p, void *dx, void *dgate, float *diniti
             done = true;
         }
     if (!done)
-        leak_backward_kernel<E, G, K, LINED><<<blocks, kLeakThreads, 0, st>>>((E *)dx, to_gate, to_sums, dinitial, (const E *)g, gstate, starts, (const E *)x, gate, maps,
-                                                                       p.s);
+        leak_backward_kernel<E, G, K, LINED, ROW><<<blocks, kLeakThreads, 0, st>>>((E *)dx, to_gate, to_sums, dinitial, (const E *)g, gstate, starts,
+                                                                                   (const E *)x, gate, maps, p.s);
     if (per_row && dgate) {
         const int64_t inner = (int64_t)p.s.gate_inner * p.s.segments, outer = p.s.rows / ((int64_t)p.s.gate_inner * p.s.gate_period);
         double *part = sums + (int64_t)p.s.rows * p.s.segments;
@@ -836,10 +861,11 @@ extern "C" int slayer_b200_leak_forward(void *y, float *state, float *starts, co
                            {x, all}, {gate, gate_bytes(p, element)}, {initial, per_row}, {lengths, lengths_bytes(p)}};
     SB200_REQUIRE(all_apart(list, 4, 1, 6), "leak_forward: y, state, starts and the workspace share memory with one another or with what is read");
     const cudaStream_t st = (cudaStream_t)stream;
-#define SB200_LEAK_CALL(E, G, K)                                                                               \
-    do {                                                                                                       \
-        if (p.lined) run_forward<E, G, K, true>(p, y, state, starts, x, gate, initial, workspace, st);         \
-        else run_forward<E, G, K, false>(p, y, state, starts, x, gate, initial, workspace, st);                \
+#define SB200_LEAK_CALL(E, G, K)                                                                          \
+    do {                                                                                                  \
+        const auto run = p.s.gate_period ? p.lined ? run_forward<E, G, K, true, true> : run_forward<E, G, K, false, true>    \
+                                         : p.lined ? run_forward<E, G, K, true, false> : run_forward<E, G, K, false, false>; \
+        run(p, y, state, starts, x, gate, initial, workspace, st);                                        \
     } while (0)
     SB200_LEAK_TYPES(SB200_LEAK_CALL)
 #undef SB200_LEAK_CALL
@@ -868,10 +894,11 @@ extern "C" int slayer_b200_leak_backward(void *dx, void *dgate, float *dinitial,
                            {lengths, lengths_bytes(p)}};
     SB200_REQUIRE(all_apart(list, 4, 2, 5), "leak_backward: dx, dgate, dinitial and the workspace share memory with one another or with what is read");
     const cudaStream_t st = (cudaStream_t)stream;
-#define SB200_LEAK_CALL(E, G, K)                                                                                \
-    do {                                                                                                        \
-        if (p.lined) run_backward<E, G, K, true>(p, dx, dgate, dinitial, g, gstate, starts, x, gate, workspace, st); \
-        else run_backward<E, G, K, false>(p, dx, dgate, dinitial, g, gstate, starts, x, gate, workspace, st);   \
+#define SB200_LEAK_CALL(E, G, K)                                                                          \
+    do {                                                                                                  \
+        const auto run = p.s.gate_period ? p.lined ? run_backward<E, G, K, true, true> : run_backward<E, G, K, false, true>    \
+                                         : p.lined ? run_backward<E, G, K, true, false> : run_backward<E, G, K, false, false>; \
+        run(p, dx, dgate, dinitial, g, gstate, starts, x, gate, workspace, st);                           \
     } while (0)
     SB200_LEAK_TYPES(SB200_LEAK_CALL)
 #undef SB200_LEAK_CALL

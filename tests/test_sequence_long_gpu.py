@@ -84,3 +84,32 @@ def test_states_in_place(R, T):
         for _ in range(5):
             own, back = h.clone(), up.clone()
             assert all(torch.equal(a, b) for a, b in zip(apart, passes(x, gate, g, own, own, back, back, lengths)))
+
+
+@pytest.mark.parametrize("T", [300, 480, 2000])
+def test_a_decay_of_a_whole_row_is_not_rounded_again_at_each_step(T):
+    """Rows whose f lies 0.4 to 0.5 of a rounding step, 2^-24, below a float32 number: where steps took f so rounded, a lane's 16 of them would forget
+    too little each time, and results were 3 to 4 STEP too large on average.  Decays themselves are off by 6 STEP of 1 - f at most, of any sign: on
+    average over 64 of them hardly by one.  What steps round goes either way."""
+    grid = torch.linspace(3.0, 6.0, 100000)
+    small = torch.sigmoid(-grid.double()).float().double()
+    up = ((1.0 - small).float().double() - (1.0 - small)) / STEP
+    gate = grid[(up > 0.4) & (up < 0.5)]
+    gate = gate[torch.linspace(0, len(gate) - 1, 64).long()]
+    gen = torch.Generator(device="cuda").manual_seed(T)
+    x, g = (0.5 + torch.rand(8, 64, T, device="cuda", generator=gen) for _ in range(2))
+    leaves = [x.requires_grad_(), gate[:, None].cuda().requires_grad_()]
+    y = gatedLeak(*leaves)
+    dx, dgate = torch.autograd.grad(y, leaves, g)
+    f = torch.sigmoid(leaves[1].detach().double())[None]
+
+    def scan(v):
+        out, h = torch.empty_like(v), torch.zeros_like(v[..., 0])
+        for t in range(T):
+            h = f[..., 0] * h + v[..., t]
+            out[..., t] = h
+        return out
+    h, lam = scan(x.detach().double()), scan(g.double().flip(-1)).flip(-1)
+    slope = (lam * f * (1 - f) * torch.cat([torch.zeros_like(h[..., :1]), h[..., :-1]], -1)).sum((0, 2))[:, None]
+    off = [float((a.double() / b - 1).mean()) / STEP for a, b in ((y.detach(), h), (dx, lam), (dgate, slope))]
+    assert abs(off[0]) <= 2 and abs(off[1]) <= 2 and abs(off[2]) <= 4, off
