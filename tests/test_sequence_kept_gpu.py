@@ -48,3 +48,55 @@ def test_layers_keep_nothing_without_gradients(monkeypatch):
         assert torch.equal(net.spike(leaf, checkpoint=True), spikes)
     with pytest.raises(AssertionError, match="without need"):
         dense(x)
+
+
+def test_memory_between_the_passes():
+    """A dense layer and its neurons hold 33/128 of what they hold without checkpoints, beside the spikes."""
+    net = layer.spikeLayer(NEURON, {"Ts": 1.0, "tSample": 320}).cuda()
+    N, I, O, T = 16, 700, 500, 320
+    x = (torch.rand(N, I, 1, 1, T, device="cuda") < 0.1).float()
+    held = {}
+    asked = lambda: torch.cuda.memory_stats()["requested_bytes.all.current"]  # noqa: E731  (blocks are up to 1 MB larger than what is asked for)
+    for keep in (False, True):
+        dense = net.dense(I, O, checkpoint=keep).cuda()
+        for _ in range(2):          # the first one may make libraries' workspaces
+            torch.cuda.synchronize()
+            before = asked()
+            s = net.spike(dense(net.psp(x)), checkpoint=keep)
+            held[keep] = asked() - before - s.numel() * 4
+            s.sum().backward()
+            del s
+            dense.weight.grad = None
+    both = N * (I + O) * T * 4
+    assert both <= held[False] <= both + 65536
+    assert both * 33 // 128 <= held[True] <= both * 33 // 128 + 65536
+
+
+def test_a_replayed_network_of_them():
+    """All of a captured training step's results, the gradient of the leak's gates among them, are the eager step's."""
+    torch.manual_seed(4)
+    net = layer.spikeLayer(NEURON, {"Ts": 1.0, "tSample": 500}).cuda()
+    fc1, leak, fc2 = net.dense(40, 60, checkpoint=True).cuda(), net.leak(60).cuda(), net.dense(60, 10, checkpoint=True).cuda()
+    x = (torch.rand(4, 40, 1, 1, 500, device="cuda") < 0.1).float()
+    weights = [fc1.weight, leak.gate, fc2.weight]
+
+    def step():
+        s = net.spike(leak(fc1(net.psp(x))), checkpoint=True)
+        out = net.spike(fc2(net.psp(s)), checkpoint=True)
+        return [out, *torch.autograd.grad(out.sum(), weights)]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        for _ in range(3):
+            step()
+    torch.cuda.current_stream().wait_stream(stream)
+    eager = [v.detach().clone() for v in step()]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(2):
+        for v in out:
+            v.detach().zero_()
+        graph.replay()
+        for a, b in zip(out, eager):
+            assert torch.equal(a, b)

@@ -4,7 +4,7 @@ import torch
 
 from slayerpytorch_b200 import capi
 from slayerpytorch_b200.recurrence import gatedLeak
-from test_leak_gpu import STEP
+from test_leak_gpu import STEP, TYPES, check, made
 
 pytestmark = pytest.mark.gpu
 
@@ -22,6 +22,23 @@ def segments(rows, T):
     each = -(-chunks // min(warps() // rows, chunks, 1024))
     n = -(-chunks // each)
     return n, each, chunks - (n - 1) * each
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("groups,T,ragged", [(2, 3001, False), (2, 2048, False), (7, 8000, True), (7, 8003, True), (73, 65537, True), (600, 1000500, True)])
+def test_segments_of_several_chunks(groups, T, ragged, dtype):
+    """Rows of which `groups` warps fit; ragged: the last segment has fewer chunks than the others."""
+    C = warps() // groups // 2
+    N = 2 if C else 1
+    C = max(C, 1)
+    n, each, last = segments(N * C, T)
+    assert n > 1 and each > 1 and (last < each) == ragged, (n, each, last)
+    for shape, kind, coupled in (((N, C, T), 'logit', True), ((C, 1), 'logit', False), ((C, 1), 'decay', True)):
+        x, gate, h, g, gs, gen = made(N, C, T, dtype, kind, T + N, shape)
+        check(x, gate, h, None, kind, coupled, g, gs)
+        lengths = torch.randint(0, T + 1, (N,), device="cuda", generator=gen)
+        lengths[0] = T - 700        # ends in an earlier chunk than the row
+        check(x, gate, h, lengths, kind, coupled, g, gs)
 
 
 def test_no_loss_from_chunk_to_chunk():
