@@ -607,8 +607,49 @@ leak_short_backward_kernel(E *dx, E *dgate, double *sums, float *dinitial, const
     if (dgate) short_store(dgate + first * s.T, gs, count);
 }
 
-// The gradient of a gate per row is the sum over the rows that have it, in a fixed order: rows (k period + i) inner + j of gate i.  parts > 1:
-// each of them sums every parts-th entry, and a second launch (inner = parts, period = gates, outer = 1) those.
+// The gradient of a gate per row is the sum over the rows that have it, in a fixed order: rows (k period + i) inner + j of gate i.  By the number of them:
+// up to 16, a thread a gate; up to 512, eight warps for 32 gates, whose entries lie next to each other where inner is 1, or a warp a gate where inner is
+// 16 or more; else, and where all gates' CTAs are resident at once, a CTA a gate.  (A CTA for each of 8000000 gates of one row took 12370 us beside a
+// backward pass of 152, threads take 32; 9248 gates of 32 rows 19.2 and 4.4.  1000 gates of 500 rows: CTAs 5.4, warps 9.5.)
+__device__ __forceinline__ int64_t gate_entry(unsigned n, unsigned inner, int64_t period, int64_t i) { return ((int64_t)(n / inner) * period + i) * inner + n % inner; }
+
+// P warps have 32 gates
+template <int P>
+__global__ void __launch_bounds__(256)
+leak_gates_sum_kernel(float *out, const double *sums, unsigned count, int64_t period, unsigned inner)
+{
+    __shared__ double part[P > 1 ? 8 : 1][32];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, p = warp % P;
+    const int64_t i = ((int64_t)blockIdx.x * (8 / P) + warp / P) * 32 + lane;
+    double sum = 0.0;
+    if (i < period) {
+#pragma unroll 8
+        for (unsigned n = p; n < count; n += P) sum += sums[gate_entry(n, inner, period, i)];
+    }
+    if (P > 1) {
+        part[warp][lane] = sum;
+        __syncthreads();
+        if (p > 0) return;
+#pragma unroll
+        for (int w = 1; w < P; ++w) sum += part[warp + w][lane];
+    }
+    if (i < period) out[i] = (float)sum;
+}
+
+__global__ void __launch_bounds__(256)
+leak_gate_warp_sum_kernel(float *out, const double *sums, unsigned count, int64_t period, unsigned inner)
+{
+    const int64_t i = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
+    if (i >= period) return;
+    double sum = 0.0;
+#pragma unroll 4
+    for (unsigned n = threadIdx.x % 32; n < count; n += 32) sum += sums[gate_entry(n, inner, period, i)];
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) sum += __shfl_down_sync(~0u, sum, d);
+    if (threadIdx.x % 32 == 0) out[i] = (float)sum;
+}
+
+// A CTA.  parts > 1: each of them sums every parts-th entry, and a second launch (inner = parts, period = gates, outer = 1) those.
 __global__ void __launch_bounds__(256)
 leak_gate_sum_kernel(double *part, float *out, const double *sums, int64_t outer, int64_t period, int64_t inner, int64_t parts)
 {
@@ -740,6 +781,16 @@ static void run_forward(const LeakPlan &p, void *y, float *state, float *starts,
     leak_forward_kernel<E, G, K, LINED, ROW><<<blocks, kLeakThreads, 0, st>>>((E *)y, state, starts, (const E *)x, gate, initial, maps, p.s);
 }
 
+static void sum_gates(float *out, const double *sums, int64_t outer, int64_t period, int64_t inner, cudaStream_t st)
+{
+    const int64_t count = outer * inner;
+    const bool one_wave = period <= (int64_t)sm_count() * 8;
+    if (count > 512 || (count > 16 && one_wave)) leak_gate_sum_kernel<<<(unsigned)period, 256, 0, st>>>(nullptr, out, sums, outer, period, inner, 1);
+    else if (count <= 16) leak_gates_sum_kernel<1><<<(unsigned)ceil_div(period, 256), 256, 0, st>>>(out, sums, (unsigned)count, period, (unsigned)inner);
+    else if (inner >= 16) leak_gate_warp_sum_kernel<<<(unsigned)ceil_div(period, 8), 256, 0, st>>>(out, sums, (unsigned)count, period, (unsigned)inner);
+    else leak_gates_sum_kernel<8><<<(unsigned)ceil_div(period, 32), 256, 0, st>>>(out, sums, (unsigned)count, period, (unsigned)inner);
+}
+
 template <typename E, int G, int K, bool LINED, bool ROW>
 static void run_backward(const LeakPlan &p, void *dx, void *dgate, float *dinitial, const void *g, const float *gstate, const float *starts, const void *x,
                          const void *gate, void *workspace, cudaStream_t st)
@@ -769,12 +820,11 @@ static void run_backward(const LeakPlan &p, void *dx, void *dgate, float *diniti
     if (per_row && dgate) {
         const int64_t inner = (int64_t)p.s.gate_inner * p.s.segments, outer = p.s.rows / ((int64_t)p.s.gate_inner * p.s.gate_period);
         double *part = sums + (int64_t)p.s.rows * p.s.segments;
-        const unsigned gates = (unsigned)p.s.gate_period;
         if (p.gate_parts > 1) {
-            leak_gate_sum_kernel<<<gates * (unsigned)p.gate_parts, 256, 0, st>>>(part, nullptr, sums, outer, p.s.gate_period, inner, p.gate_parts);
-            leak_gate_sum_kernel<<<gates, 256, 0, st>>>(nullptr, (float *)dgate, part, 1, p.s.gate_period, p.gate_parts, 1);
+            leak_gate_sum_kernel<<<(unsigned)(p.s.gate_period * p.gate_parts), 256, 0, st>>>(part, nullptr, sums, outer, p.s.gate_period, inner, p.gate_parts);
+            sum_gates((float *)dgate, part, 1, p.s.gate_period, p.gate_parts, st);
         } else {
-            leak_gate_sum_kernel<<<gates, 256, 0, st>>>(nullptr, (float *)dgate, sums, outer, p.s.gate_period, inner, 1);
+            sum_gates((float *)dgate, sums, outer, p.s.gate_period, inner, st);
         }
     }
 }
