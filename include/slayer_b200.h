@@ -444,7 +444,7 @@ int slayer_b200_spike_grad8(float *out, const float *g, const int8_t *q, const u
 /*
  * Weight gradient of a dense layer whose input x [N, I, T] is kept so, for the gradient g [N, O, T] of its output:
  *   out[o, i] = sum over n and t of g[n, o, t] x[n, i, t],
- * in float32 precision, the same bits in every call.  Its products wait on barriers for a limited time; if one ever
+ * in float32 precision, the same bits in every call (of g what lies under 2^-133 is cut off; what is not finite gives NaN).  Its products wait on barriers for a limited time; if one ever
  * runs out, the result is not complete and slayer_b200_device_status() says 0x5104.  workspace: slayer_b200_weight_grad8_workspace(...) bytes of device
  * memory; it, g and q are aligned to 16.  It has no counterpart in the reference, whose weights are PyTorch's
  * (src/slayer.py:393-437).

@@ -48,5 +48,6 @@ def spikeGrad(grad, kept, theta, tau, scale):
 def weightGrad(grad, kept):
     """Weight gradient of a dense layer: ``grad [N, O, 1, 1, T]`` (float32) of its output, ``kept`` its input ``[N, C, H, W, T]`` kept by
     ``compress``; returns ``[O, C, H, W, 1]``, the sum over samples and steps of ``grad * input``, to float32 precision and the same
-    in every call.  Any number of dimensions from three on."""
+    in every call.  Any number of dimensions from three on.  Of gradients below 2**-110 what lies under 2**-133 has no part in it; where one is not
+    finite, or an input was not, the sums that it is in are NaN."""
     return slayerCuda.weightGrad8(grad.contiguous(), kept.q, kept.scale, kept.shape)

@@ -1,7 +1,8 @@
 // Weight gradient of a dense layer from an input kept in 8 bits (checkpoint.cu):
 //   dW[o, i] = sum over samples n and steps t of g[n, o, t] x[n, i, t],  x = q 2^e,
 // as products of bfloat16 tiles on the tensor cores.  q 2^e is a bfloat16 as it is; g, a float32, is the sum of three: its upper 8 bits, the
-// next 8 and the last 8, cut off and not rounded, so that the three parts are g exactly.  Three products, summed in float32, have the
+// next 8 and the last 8, cut off and not rounded, so that the three parts are g exactly (but for what is below 2^-133, bfloat16's smallest number: a g
+// under 2^-110 has bits there).  What is not finite leaves parts that are NaN.  Three products, summed in float32, have the
 // precision of float32 products.  Both operands have time as their summation index and next to each other in memory, as the tensor cores
 // like it, but neither is in a form that they read: 16 warps fetch tiles (16-byte copies to shared memory that nobody waits for, two blocks
 // ahead), take them apart in registers and write them to shared memory again as 128-byte rows; one thread issues the products.

@@ -36,7 +36,7 @@ def gatedLeak(x, gate, initial=None, lengths=None, kind='logit', coupled=False, 
 
     Differentiable once in ``x``, ``gate`` and ``initial``.  Results are off by a few steps of float32, however slow the leak.  Nothing but
     ``x``, ``gate`` and one float32 state for 12 or 16 steps is kept for the backward pass.  A state that is not finite makes those after it so, as NaN
-    possibly where single steps would give an infinity."""
+    possibly where the formula gives an infinity (here and in ``gatedLeakStep``)."""
     out = slayerCuda.gatedLeak(x, gate, initial, lengths, _flags("gatedLeak", kind, coupled), returnState)
     return (out[0], out[1]) if returnState else out[0]
 

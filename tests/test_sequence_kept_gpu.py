@@ -100,3 +100,28 @@ def test_a_replayed_network_of_them():
         graph.replay()
         for a, b in zip(out, eager):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("power", [-60, -110, -120, -130, -145])
+def test_weight_gradients_of_tiny_gradients(power):
+    """A gradient's three bfloat16 parts leave out less than 2^-133 of it; K = 256 products of float32 precision beside that (test_checkpoint_gpu.py)."""
+    gen = torch.Generator(device="cuda").manual_seed(-power)
+    x = torch.randint(-127, 128, (4, 30, 1, 1, 64), device="cuda", generator=gen).float()       # kept as it is
+    x[..., 0] = x[..., 32] = 127
+    x *= 2.0 ** 100
+    g = (torch.randn(4, 20, 1, 1, 64, dtype=torch.float64, device="cuda", generator=gen) * 2.0 ** power).float()
+    got = checkpoint.weightGrad(g, checkpoint.compress(x))[..., 0, 0, 0].double()
+    a, b = g.transpose(0, 1).reshape(20, -1).double(), x.transpose(0, 1).reshape(30, -1).double()
+    limit = (8 + 16) * 2.0 ** -24 * (a.abs() @ b.abs().T) + 2.0 ** -133 * b.abs().sum(1)
+    assert bool(((got - a @ b.T).abs() <= limit).all())
+
+
+def test_weight_gradients_that_are_not_finite():
+    """An infinity or NaN of the gradient is in all sums of its output, one of the input (kept as NaN) in those of its neuron, and in no others."""
+    x, g = torch.ones(2, 30, 1, 1, 70, device="cuda"), torch.ones(2, 20, 1, 1, 70, device="cuda")
+    g[0, 3, 0, 0, 69], g[1, 7, 0, 0, 0], x[1, 11, 0, 0, 40] = float("inf"), float("nan"), float("-inf")
+    got = checkpoint.weightGrad(g, checkpoint.compress(x))[..., 0, 0, 0]
+    bad = torch.zeros_like(got, dtype=torch.bool)
+    bad[[3, 7]] = True
+    bad[:, 11] = True
+    assert torch.equal(got.isnan(), bad) and bool((got[~bad] == 140).all())
