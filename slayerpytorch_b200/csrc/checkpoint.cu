@@ -75,8 +75,8 @@ struct Place {
 };
 
 // 16 bytes a thread: kLanes of them have a group.  L: steps of a load, 16 bytes of them where rows' steps lie on 16 bytes; rows of other lengths are
-// loaded in as large pieces as divide them (a line's other pieces are in L1 by then: one by one 52 us instead of 142 with a lane
-// for each step of a group, 64 x 2312 x 301).
+// loaded in as large pieces as divide them (a line's other pieces are in L1 by then: one by one 48 us, 64 x 2312 x 301; with a
+// lane for each step of a group it was 142).
 template <typename E> constexpr int kCompressUnroll = sizeof(E) == 4 ? 4 : 2;
 template <typename E> constexpr int kCompressBlock = 256 / (32 * (int)sizeof(E) / 16) * kCompressUnroll<E>;
 

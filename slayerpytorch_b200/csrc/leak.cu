@@ -6,8 +6,7 @@
 //   lambda_t = g_t + c_{t+1},   dx = lambda (or (1 - f) lambda),   df = lambda (y_{t-1} - (coupled) x).
 // It forms y again from x and the gate, out of the states that the forward pass keeps where each lane begins (4 bytes for 12 or 16 steps), so that
 // it reads x, gate and g and writes dx and dgate, and scans once: no y is kept, and none that is rounded to 16 bits is used.  (With states at
-// the start of each chunk alone, and a scan for the others, the backward pass took 49 us instead of 46, 64 x 512 x 300, and 127 instead
-// of 111, 262144 x 100.)
+// the start of each chunk alone, and a scan for the others, the backward pass took 6 % longer, 64 x 512 x 300, and 14 %, 262144 x 100.)
 //
 // Maps are floats: A, and 1 - A by itself (R), and B.  A slow leak's f is next to one, where its rounding to 32 bits, taken at each of the thousands of
 // steps that such a state remembers, adds up to 1e-4 of it; R has 24 bits of what is forgotten instead.  States are double from chunk to chunk, and
@@ -75,7 +74,7 @@ template <> struct Packed<float> { using type = uint4; };
 // Which of a lane's vectors lie in [0, end) of a row as a whole, and whether one of them lies there in part: its first one, which may begin before the row,
 // or the one that `end` is in.  Vectors that begin before `stop` are read whole, though other rows' steps are in them: reach elements from the row's
 // first on are the tensor's.  LINED: rows end with their vectors, and all steps count.
-// (Without that it was 86 us forward and 158 backward instead of 82 and 154, float32, 78125 x 512.)
+// (Without that it is 87 us forward and 153 backward instead of 76 and 147, float32, 78125 x 512.)
 template <int K, bool LINED>
 struct Inside {
     int t, end, stop;
@@ -90,7 +89,7 @@ struct Inside {
 };
 
 // Steps [t, t + 4 K) of a row, `fill` where they are outside.  A vector that is there in part is read whole, other rows' steps with it: only
-// the tensor's last one may not be.  (One by one it was 133 us forward and 254 backward instead of 131 and 219, float32, 1212121 x 33.)
+// the tensor's last one may not be.  (One by one it took 2 % longer forward and 16 % backward, float32, 1212121 x 33: 130 and 229 us.)
 template <typename E, int K, bool LINED>
 __device__ __forceinline__ void load_steps(float (&v)[4 * K], const E *row, const Inside<K, LINED> &in, float fill)
 {
@@ -497,7 +496,7 @@ leak_backward_kernel(E *dx, E *dgate, double *sums, float *dinitial, const E *g,
 __device__ __forceinline__ double step_state(const Decay &d, double h, double u) { return u + (d.f < 0.5f ? (double)d.f * h : fma(-(double)d.rest, h, h)); }
 
 // Rows of up to 13 steps that do not end on vectors, which a lane has alone.  Hardly a vector would be one row's alone, and results would go an element at
-// a time (float32: 8000000 x 5 149 us forward and 262 backward, 3000000 x 13 117 and 215; so it is 113 and 207, 80 and 172).  A CTA's rows are one piece of memory that begins at 16 bytes: it is copied to
+// a time (float32: 8000000 x 5 146 us forward and 291 backward, 3000000 x 13 115 and 200; so it is 112 and 206, 77 and 168).  A CTA's rows are one piece of memory that begins at 16 bytes: it is copied to
 // shared memory as it is, a thread walks a row there, its state in double, and results go back the same way.
 constexpr int kShortSteps = 13;
 
