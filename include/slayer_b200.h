@@ -392,7 +392,7 @@ int64_t slayer_b200_muon_step_workspace(const slayer_b200_muon_matrix *list, int
  * slayer_b200_leak_states(T) float32, states that the backward pass starts from (one for 12 or 16 steps of longer rows).  States are
  * float32 outside of a call and double within.  Nothing else that is written (y, state, starts, workspace) may share memory with the rest.
  * x, y and a gate of x's type are aligned to 16 bytes.  workspace:
- * slayer_b200_leak_workspace(...) bytes of device memory, aligned to 16, for either pass.  It has
+ * slayer_b200_leak_workspace(...) bytes of device memory, aligned to 16, for either pass (of gate_period 0 for this one).  It has
  * no counterpart in the reference, whose psp has one fixed kernel (src/slayer.py:875-899).
  */
 int slayer_b200_leak_forward(void *y, float *state, float *starts, const void *x, const void *gate, const float *initial, int dtype, int flags,

@@ -92,9 +92,10 @@ struct Shape {
           inner(inner_), period(period_), dtype(dtype_code(x, "x")), flags((int)flags_)
     {
     }
-    torch::Tensor workspace(const torch::Tensor &x) const
+    // (the backward pass adds up the gradients of a gate per row there, too)
+    torch::Tensor workspace(const torch::Tensor &x, bool backward) const
     {
-        return torch::empty({size_of(slayer_b200_leak_workspace(rows, T, dtype, inner, period), "gatedLeak")}, x.options().dtype(torch::kUInt8));
+        return torch::empty({size_of(slayer_b200_leak_workspace(rows, T, dtype, inner, backward ? period : 0), "gatedLeak")}, x.options().dtype(torch::kUInt8));
     }
 };
 
@@ -110,7 +111,7 @@ struct GatedLeak : public torch::autograd::Function<GatedLeak> {
         torch::Tensor state, starts;
         if (wantState) state = torch::empty(x.sizes().slice(0, x.dim() - 1), floats);
         if (want) starts = torch::empty({s.rows, slayer_b200_leak_states(s.T)}, floats);
-        const auto workspace = s.workspace(x);
+        const auto workspace = s.workspace(x, false);
         check_rc(slayer_b200_leak_forward(y.data_ptr(), wantState ? state.data_ptr<float>() : nullptr, want ? starts.data_ptr<float>() : nullptr, x.data_ptr(),
                                           gate.data_ptr(), initial.has_value() ? initial->data_ptr<float>() : nullptr, s.dtype, s.flags, s.rows, s.T,
                                           lengths.has_value() ? lengths->data_ptr<int64_t>() : nullptr, s.sample_rows, inner, period,
@@ -141,7 +142,7 @@ struct GatedLeak : public torch::autograd::Function<GatedLeak> {
         if (ctx->needs_input_grad(0)) out[0] = torch::empty_like(x);
         if (ctx->needs_input_grad(1)) out[1] = torch::empty_like(gate);
         if (ctx->saved_data["initial"].toBool() && ctx->needs_input_grad(2)) out[2] = torch::empty(x.sizes().slice(0, x.dim() - 1), starts.options());
-        const auto workspace = s.workspace(x);
+        const auto workspace = s.workspace(x, true);
         check_rc(slayer_b200_leak_backward(out[0].defined() ? out[0].data_ptr() : nullptr, out[1].defined() ? out[1].data_ptr() : nullptr,
                                            out[2].defined() ? out[2].data_ptr<float>() : nullptr, g.data_ptr(),
                                            gstate.defined() ? gstate.data_ptr<float>() : nullptr, starts.data_ptr<float>(), x.data_ptr(), gate.data_ptr(),

@@ -35,8 +35,8 @@ def test_gates_of_images():
         assert bool(((got.double() - want).abs() <= 2 * 200 * STEP * size).all())
 
 
-def test_many_gates_are_added_up_in_a_part_of_the_pass():
-    """Times are no test; the launch of millions of gates is: every gate gets its own sum, and the same in every call."""
+def test_millions_of_gates():
+    """Every gate gets its own sum, and the same in every call."""
     C, T = 3000001, 3
     gen = torch.Generator(device="cuda").manual_seed(2)
     x, g = (torch.randn(1, C, T, device="cuda", generator=gen) for _ in range(2))
@@ -51,3 +51,16 @@ def test_many_gates_are_added_up_in_a_part_of_the_pass():
     size = ((f * l2.abs() + g[:, 1].abs()) * y0.abs() + l2.abs() * (f * y0.abs() + x[:, 1].abs())) * f * (1 - f)
     # decays are off by (8 + |gate|) steps each, slopes, states and products by a few
     assert bool(((a[:, 0].double() - want).abs() <= (4 * (8 + gate.detach()[:, 0].abs()) + 20) * STEP * size + 1e-37).all())
+
+
+@pytest.mark.parametrize("rows,T", [(2000000, 4), (3, 20000)])
+def test_a_forward_pass_needs_no_memory_for_the_gates_gradients(rows, T):
+    """Beside its result: nothing, or, of rows that are split, 16 bytes for each segment and row at most."""
+    x, gate = torch.randn(1, rows, T, device="cuda"), torch.randn(rows, 1, device="cuda")
+    with torch.no_grad():
+        gatedLeak(x, gate)
+        torch.cuda.reset_peak_memory_stats()
+        asked = lambda which: torch.cuda.memory_stats()["requested_bytes.all." + which]  # noqa: E731
+        before = asked("current")
+        y = gatedLeak(x, gate)
+        assert asked("peak") - before <= y.numel() * 4 + (rows * 40 * 16 + 64 if T > 512 else 0)
